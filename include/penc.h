@@ -57,6 +57,9 @@ extern "C" {
 #define PENC_ERR_SCRATCH_TOO_SMALL 7    /* penc_backward_static: the problem does not fit the static scratch */
 #define PENC_ERR_WORKSPACE_TOO_SMALL 8  /* penc_backward_rowmajor with positions_grad, penc_forward_rowmajor: no room for the level-major array */
 #define PENC_ERR_UNSUPPORTED_TABLE_FORMAT 9 /* the *_half entry points: table_format is neither PENC_TABLE_FP16 nor PENC_TABLE_BF16 */
+#define PENC_ERR_UNSUPPORTED_TYPE 10        /* the layers: a type is none of PENC_FP32, PENC_FP16, PENC_BF16 */
+#define PENC_ERR_UNSUPPORTED_KIND 11        /* the layers: no such activation or norm */
+#define PENC_ERR_BAD_LAYER_SIZE 12          /* the layers: a negative number of rows, channels not in 1..the entry point's most, or strides it does not take */
 
 const char* penc_status_string(int status);
 
@@ -398,6 +401,93 @@ int penc_transpose(const float* src, float* dst, int64_t rows, int cols, void* s
 int penc_simplex_debug(int pos_dim, int64_t nr_positions, int nr_levels, int capacity,
                        const float* positions, const float* scale_factor, const float* random_shift,
                        int gather_path, int* rem0, int* rank, int* slot, float* barycentric, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * The layers behind the encoding.  No counterpart in the reference, whose scripts take them from torch.
+ *
+ * Rows of `channels` values of a type below; a row stride is counted in values, and channels of a row are adjacent
+ * unless an entry point has a stride for them.  Arrays need the alignment of one value, checkpoints 16 bytes.  No rows is a valid call that
+ * writes nothing (sums over the rows become zero).  Sums, statistics and steps are fp32, results are rounded once, to nearest, ties to even, and do not
+ * depend on the order in which workgroups run.
+ *
+ * A checkpoint keeps rows in 8 bits, in blocks of 32 channels.  With a the largest magnitude of a block, e = the least integer of at least
+ * -126 with a / 2^e < 127.5, and q = x / 2^e rounded, ties to even (e at most 121, q at most 127: values from 127.5 * 2^121 on come back as 127 * 2^121):
+ *     values    int8  [rows][penc_kept_pitch(channels)]     q, zeros behind the row's channels
+ *     exponents uint8 [rows][penc_kept_blocks(channels)]    e + 127; 255 for a block with an infinity or a NaN, which comes back as NaN
+ * Every backward entry point gives the gradient of its forward at the values a checkpoint stands for. */
+#define PENC_FP32 0
+#define PENC_FP16 1
+#define PENC_BF16 2
+
+#define PENC_MAX_CHANNELS (1 << 24)   /* of a row in a checkpoint or an activation */
+#define PENC_MAX_NORM_CHANNELS 8192   /* of a row that is normed */
+
+int64_t penc_kept_pitch(int64_t channels);
+int64_t penc_kept_blocks(int64_t channels);
+
+/* Keeps x; one of the strides is 1 (channel_stride != 1: the encoding's result, which has consecutive rows side by side). */
+int penc_keep(int type, int64_t rows, int64_t channels, const void* x, int64_t row_stride, int64_t channel_stride, int8_t* values,
+              uint8_t* exponents, void* stream);
+/* The values that a checkpoint stands for, as dense rows (fp16: at most 65504 in magnitude). */
+int penc_restore(int type, int64_t rows, int64_t channels, const int8_t* values, const uint8_t* exponents, void* x, void* stream);
+
+#define PENC_GELU 0      /* x Phi(x) */
+#define PENC_SILU 1      /* x / (1 + exp(-x)) */
+#define PENC_SOFTPLUS 2  /* log(1 + exp(x)) */
+/* y = act(x); gated: rows of 2 * channels values [a | b] and y = act(a) b.  `values` (may be NULL, with `exponents`) keeps x; gated: a, and behind it
+ * b, each as a checkpoint of its own. */
+int penc_activation(int type, int kind, int gated, int64_t rows, int64_t channels, const void* x, int64_t row_stride, void* y, int8_t* values,
+                    uint8_t* exponents, void* stream);
+/* dx (dense rows) from the input itself or, where x is NULL, from its checkpoint. */
+int penc_activation_backward(int type, int kind, int gated, int64_t rows, int64_t channels, const void* x, int64_t row_stride, const int8_t* values,
+                             const uint8_t* exponents, const void* grad, int64_t grad_row_stride, void* dx, void* stream);
+
+/* weight_grad[o][c] = sum over the rows of grad[row][o] * x^[row][c] and (may be NULL) bias_grad[o] = sum of grad[row][o], both of result_type: what a
+ * linear layer with `outputs` outputs needs of its kept input.  `workspace` holds partial sums (penc_weight_grad_workspace_bytes, 0: none needed). */
+size_t penc_weight_grad_workspace_bytes(int64_t rows, int64_t channels, int64_t outputs);
+int penc_weight_grad(int type, int result_type, int64_t rows, int64_t channels, int64_t outputs, const int8_t* values, const uint8_t* exponents,
+                     const void* grad, int64_t grad_row_stride, void* weight_grad, void* bias_grad, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* What stands between a block and the next one:
+ *     p = post norm(branch),  y = residual_scale * x + gate * p,  n = pre norm(y)
+ * with norm(v) = (v - mean) / sqrt(variance + eps) * weight + bias (PENC_LAYER) or v / sqrt(mean of v^2 + eps) * weight + bias (PENC_RMS). */
+#define PENC_RMS 0
+#define PENC_LAYER 1
+typedef struct penc_norm {
+    int type;                /* of rows and results */
+    int param_type;          /* of weights and biases: `type` or PENC_FP32 */
+    int gate_type;           /* of the gate, likewise */
+    int kind;                /* PENC_RMS or PENC_LAYER */
+    int post_norm, pre_norm; /* 0: p = branch, no n */
+    float residual_scale, eps;
+    int64_t rows, channels;
+    int64_t rows_per_gate;   /* 0: one gate of `channels` values for all rows; else this many consecutive rows (rows is a multiple) share one */
+    const void* x;           /* backward: NULL where x is kept */
+    int64_t x_stride;
+    const void* branch;      /* forward: NULL: y = residual_scale * x; backward: NULL where it is kept or there is none */
+    int64_t branch_stride;
+    int has_branch;
+    const void *gate, *post_weight, *post_bias, *pre_weight, *pre_bias; /* each may be NULL: 1, or 0 for a bias */
+    int8_t* x_values;        /* checkpoints of x and branch, written by the forward where not NULL, read by the backward where x, branch are NULL */
+    uint8_t* x_exponents;
+    int8_t* branch_values;
+    uint8_t* branch_exponents;
+} penc_norm;
+
+/* y (may be NULL) and, with pre_norm, n: dense rows. */
+int penc_residual_norm(const penc_norm* norm, void* y, void* n, void* stream);
+/* From the gradients of y and n (rows; either may be NULL) those of x, branch (dense rows), gate, weights and biases (of gate_type and param_type); any
+ * may be NULL. */
+typedef struct penc_norm_grads {
+    const void* y;
+    int64_t y_stride;
+    const void* n;
+    int64_t n_stride;
+    void *x, *branch, *gate, *post_weight, *post_bias, *pre_weight, *pre_bias;
+} penc_norm_grads;
+size_t penc_residual_norm_workspace_bytes(int64_t rows, int64_t channels, int64_t rows_per_gate);
+int penc_residual_norm_backward(const penc_norm* norm, const penc_norm_grads* grads, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,190 @@
+// Values in 32, 16 and 8 bits, as the kernels of the layers behind the encoding load and store them.
+//
+// A checkpoint keeps a row of C channels in blocks of 32 (the last one shorter).  With a the largest magnitude of a block,
+//
+//     e = the least integer of at least -126 with a / 2^e < 127.5,     q = round to even (x / 2^e), in -127..127,     x^ = q 2^e.
+//
+// (e is at most 121: from 127.5 2^121 on, the last 0.4% of what fp32 has, a value is kept as 127 2^121, where 64 2^122 would be infinite.)
+// The step is a power of two, so that x / 2^e and q 2^e are exact and q does not depend on how it is computed; x^ is off by at most half a
+// step, and is exact in bfloat16.  Off by, in blocks of normally distributed values (rms, in deviations): 0.0083; with a step of a / 127 0.0053, with
+// values in e4m3 and a scale for every 32 of them 0.029.
+// A block with an infinity or a NaN comes back as NaN.
+//
+//     values     int8  [rows][pitch]                     pitch: C rounded up to 16, the rest of a row zero
+//     exponents  uint8 [rows][ceil(C / 32)]              e + 127, 255 for a block that is not finite
+//
+// A lane works on 8 consecutive channels, four lanes on a block: 16 bytes of a 16-bit type in a load, 8 of a checkpoint.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/penc.h"
+
+namespace penc {
+
+using half_t = _Float16;
+using bf16_t = __bf16;
+
+constexpr int kChunk = 8;   // channels of a lane
+constexpr int kKeptBlock = 32;
+constexpr int kKeptPitch = 16;
+
+__host__ __device__ __forceinline__ int64_t kept_pitch(int64_t channels) { return (channels + kKeptPitch - 1) / kKeptPitch * kKeptPitch; }
+__host__ __device__ __forceinline__ int64_t kept_blocks(int64_t channels) { return (channels + kKeptBlock - 1) / kKeptBlock; }
+
+// Eight values, aligned as one is: rows of any length and stride (gfx950 takes such an address in one 16-byte access).
+template <class E>
+using chunk_t = E __attribute__((ext_vector_type(kChunk), aligned(sizeof(E))));
+using float8 = float __attribute__((ext_vector_type(kChunk)));
+
+// `valid`: how many of the eight are in the row; the others are zero.
+template <class E>
+__device__ __forceinline__ void load_chunk(const E* __restrict__ p, int valid, float (&v)[kChunk]) {
+    if (valid >= kChunk) {
+        const float8 x = __builtin_convertvector(*reinterpret_cast<const chunk_t<E>*>(p), float8);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) v[i] = x[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) v[i] = i < valid ? static_cast<float>(p[i]) : 0.0f;
+    }
+}
+
+// (rounded to nearest, ties to even: the only rounding to 16 bits)
+template <class E>
+__device__ __forceinline__ void store_chunk(E* __restrict__ p, int valid, const float (&v)[kChunk]) {
+    float8 x;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) x[i] = v[i];
+    const auto y = __builtin_convertvector(x, E __attribute__((ext_vector_type(kChunk))));
+    if (valid >= kChunk) {
+        *reinterpret_cast<chunk_t<E>*>(p) = y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i)
+            if (i < valid) p[i] = y[i];
+    }
+}
+
+// A parameter: fp32, or of the type of the rows it is applied to.
+template <class E>
+__device__ __forceinline__ void load_param(const void* p, bool fp32, int64_t at, int valid, float (&v)[kChunk]) {
+    if (fp32) load_chunk(static_cast<const float*>(p) + at, valid, v);
+    else load_chunk(static_cast<const E*>(p) + at, valid, v);
+}
+
+template <int kControl>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kControl, 0xF, 0xF, true));
+}
+constexpr int kSwapPairs = 0xB1, kSwapTwos = 0x4E;  // quad_perm: lane ^ 1, lane ^ 2
+constexpr int kMirrorHalfRow = 0x141, kMirrorRow = 0x140;
+
+// What a block's largest magnitude (as an integer: an infinity or a NaN is the largest) makes of its values.
+struct BlockStep {
+    uint32_t exponent;
+    float per_step;
+    bool finite, top;
+
+    __device__ __forceinline__ explicit BlockStep(uint32_t largest) {
+        finite = largest < 0x7F800000u;
+        // a = m 2^k with m in [1, 2): e = k - 6, and one more from m = 127.5 / 64 on, where the sum below carries into the exponent
+        exponent = max((largest + 0x10000u) >> 23, 7u) - 6u;
+        top = exponent > 248u;
+        exponent = min(exponent, 248u);
+        per_step = __uint_as_float((254u - exponent) << 23);
+        if (!finite) exponent = 255u;
+    }
+    // Before the values of a block at the top of the range are quantised (all but never).
+    template <int kValues>
+    __device__ __forceinline__ void saturate(float (&v)[kValues]) const {
+        if (!top) return;
+        constexpr float kMost = 0x1.FCp+127f;  // 127 2^121
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) v[i] = fminf(fmaxf(v[i], -kMost), kMost);
+    }
+    // Four of the block's values: round(x 2^-e) in the low bits of x 2^-e + 1.5 2^23, one rounding, to even.
+    __device__ __forceinline__ uint32_t quantised(const float* v) const {
+        uint32_t t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = __float_as_uint(__builtin_fmaf(v[i], per_step, 12582912.0f));
+        const uint32_t lo = __builtin_amdgcn_perm(t[1], t[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(t[3], t[2], 0x0C0C0400u);
+        return finite ? __builtin_amdgcn_perm(hi, lo, 0x05040100u) : 0u;
+    }
+};
+
+struct Kept {
+    uint2 q;
+    uint32_t exponent;
+};
+
+// The four lanes of a block bring its 32 values, zeros behind the row's end.
+__device__ __forceinline__ Kept keep(const float (&x)[kChunk]) {
+    float v[kChunk];
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) v[i] = x[i];
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    a = max(a, dpp<kSwapPairs>(a));
+    a = max(a, dpp<kSwapTwos>(a));
+    const BlockStep s(a);
+    s.saturate(v);
+    return {make_uint2(s.quantised(v), s.quantised(v + 4)), s.exponent};
+}
+
+// (255 gives an infinite step, and 0 times that the NaN)
+__device__ __forceinline__ float kept_step(uint32_t exponent) { return __uint_as_float(exponent << 23); }
+__device__ __forceinline__ void restore(uint2 q, uint32_t exponent, float (&v)[kChunk]) {
+    const float step = kept_step(exponent);
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) v[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? q.x : q.y) >> 8 * (i % 4))) * step;
+}
+
+// Where a checkpoint is, or null.
+struct KeptArray {
+    int8_t* values;
+    uint8_t* exponents;
+    int64_t pitch, blocks;
+
+    // The lane of the chunk that begins at channel `c` of a row; all four lanes of a block call it.
+    __device__ __forceinline__ void store(int64_t row, int c, const float (&v)[kChunk]) const {
+        const Kept k = keep(v);
+        if (c < pitch) *reinterpret_cast<uint2*>(values + row * pitch + c) = k.q;
+        if (c % kKeptBlock == 0 && c / kKeptBlock < blocks) exponents[row * blocks + c / kKeptBlock] = static_cast<uint8_t>(k.exponent);
+    }
+    __device__ __forceinline__ void load(int64_t row, int c, int valid, float (&v)[kChunk]) const {
+        if (valid > 0) {
+            restore(*reinterpret_cast<const uint2*>(values + row * pitch + c), exponents[row * blocks + c / kKeptBlock], v);
+            if (valid < kChunk) {
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i)
+                    if (i >= valid) v[i] = 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) v[i] = 0.0f;
+        }
+    }
+};
+
+inline KeptArray kept_array(const int8_t* values, const uint8_t* exponents, int64_t channels) {
+    return {const_cast<int8_t*>(values), const_cast<uint8_t*>(exponents), kept_pitch(channels), kept_blocks(channels)};
+}
+
+// Runs `f` with a value of the type that an entry point's `type` names.
+template <class F>
+int with_type(int type, F&& f) {
+    switch (type) {
+        case PENC_FP32: return f(float{});
+        case PENC_FP16: return f(half_t{});
+        case PENC_BF16: return f(bf16_t{});
+        default: return PENC_ERR_UNSUPPORTED_TYPE;
+    }
+}
+
+inline int launched() { return hipGetLastError() == hipSuccess ? PENC_OK : PENC_ERR_LAUNCH; }
+inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace penc

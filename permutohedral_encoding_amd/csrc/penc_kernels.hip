@@ -1689,11 +1689,14 @@ const char* penc_status_string(int status) {
         case PENC_ERR_BAD_SIZE: return "nr_positions, nr_levels and capacity must be positive and every array must stay below 2^31 elements";
         case PENC_ERR_UNSUPPORTED_POS_DIM: return "pos_dim must be 2,3,4,5,6,7 or 8";
         case PENC_ERR_UNSUPPORTED_NR_FEAT: return "nr_feat_per_level must be 2, 4 or 8";
-        case PENC_ERR_MISALIGNED: return "lattice_values must be aligned to one slot (at most 16 bytes), lattice_values_grad and gradient rows to 8 bytes";
+        case PENC_ERR_MISALIGNED: return "lattice_values must be aligned to one slot (at most 16 bytes), lattice_values_grad and gradient rows to 8 bytes, rows of a layer to a value, checkpoints to 16 bytes";
         case PENC_ERR_LAUNCH: return "the HIP runtime rejected a kernel launch";
-        case PENC_ERR_WORKSPACE_TOO_SMALL: return "the workspace cannot hold the level-major array the call needs (penc_backward_rowmajor_workspace_bytes, penc_forward_rowmajor_workspace_bytes)";
+        case PENC_ERR_WORKSPACE_TOO_SMALL: return "the workspace cannot hold the level-major array the call needs (penc_backward_rowmajor_workspace_bytes, penc_forward_rowmajor_workspace_bytes) or the layer's partial sums";
         case PENC_ERR_UNSUPPORTED_TABLE_FORMAT: return "table_format must be PENC_TABLE_FP16 or PENC_TABLE_BF16, with PENC_TABLE_CELLS for capacities that are powers of two and fill a line";
         case PENC_ERR_SCRATCH_TOO_SMALL: return "the problem is too large for the library's static scratch (penc_static_scratch_bytes): use penc_backward with a workspace";
+        case PENC_ERR_UNSUPPORTED_TYPE: return "a type must be PENC_FP32, PENC_FP16 or PENC_BF16, that of parameters and gates the rows' or PENC_FP32";
+        case PENC_ERR_UNSUPPORTED_KIND: return "no such activation or norm";
+        case PENC_ERR_BAD_LAYER_SIZE: return "rows must not be negative and a multiple of those of a gate, channels at least 1 and at most what the layer takes";
         default: return "unknown status";
     }
 }

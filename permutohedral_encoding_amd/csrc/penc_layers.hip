@@ -1,0 +1,399 @@
+// Checkpoints in 8 bits, and activations whose backward reads them.
+//
+//     y = act(x), or act(a) b of rows [a | b];     dx = g act'(x^), da = g b^ act'(a^), db = g act(a^)
+//     gelu  x Phi(x)                act' = Phi(x) + x phi(x)
+//     silu  x s, s = 1/(1+exp(-x))  act' = s (1 + x (1 - s))
+//     softplus  log(1 + exp(x))     act' = s
+//
+// All of them are one pass over their rows: bound by memory.  A lane has 8 channels, the lanes of a row are a power of two from 4 to 256,
+// so that a block of a checkpoint is always four neighbours of one wave, and a workgroup walks over the rows.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "penc_kept.hpp"
+#include "penc_norm.hpp"
+
+namespace penc {
+namespace {
+
+constexpr int kThreads = 256;
+
+// How lanes are laid over rows: 2^log2_lanes of them on a row, which takes `chunks` of eight channels (a multiple of four).
+struct Lanes {
+    int64_t rows;
+    int channels, chunks, log2_lanes;
+    unsigned grid;
+};
+
+Lanes lanes_for(int64_t rows, int64_t channels) {
+    Lanes l{rows, static_cast<int>(channels), static_cast<int>(4 * kept_blocks(channels)), 2, 0};
+    while (l.log2_lanes < 8 && (1 << l.log2_lanes) < l.chunks) ++l.log2_lanes;
+    const int64_t per_group = kThreads >> l.log2_lanes;
+    l.grid = static_cast<unsigned>(std::min<int64_t>((rows + per_group - 1) / per_group, 8192));
+    return l;
+}
+
+// f(row, first channel, channels in the row from there on, at most eight), four lanes of a block together
+template <class F>
+__device__ __forceinline__ void over_chunks(const Lanes& l, F&& f) {
+    const int lanes = 1 << l.log2_lanes, per_group = kThreads >> l.log2_lanes;
+    const int lane = threadIdx.x & (lanes - 1);
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * per_group + (threadIdx.x >> l.log2_lanes); row < l.rows;
+         row += static_cast<int64_t>(gridDim.x) * per_group)
+        for (int chunk = lane; chunk < l.chunks; chunk += lanes) f(row, chunk * kChunk, min(l.channels - chunk * kChunk, kChunk));
+}
+
+template <class E>
+__global__ __launch_bounds__(kThreads) void pack_kernel(Lanes l, const E* __restrict__ x, int64_t stride, KeptArray kept) {
+    over_chunks(l, [&](int64_t row, int c, int valid) {
+        float v[kChunk];
+        load_chunk(x + row * stride + c, valid, v);
+        kept.store(row, c, v);
+    });
+}
+
+// The encoding's own result: channels of consecutive rows next to each other.  A lane has a row and walks over its blocks, reading 32 channels,
+// each with the 63 lanes beside it.
+template <class E>
+__global__ __launch_bounds__(kThreads) void pack_channels_kernel(int64_t rows, int channels, const E* __restrict__ x, int64_t stride, KeptArray kept) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (row >= rows) return;
+    for (int first = 0; first < channels; first += kKeptBlock) {
+        float v[kKeptBlock];
+#pragma unroll
+        for (int i = 0; i < kKeptBlock; ++i) v[i] = first + i < channels ? static_cast<float>(x[(first + i) * stride + row]) : 0.0f;
+        uint32_t a = 0;
+#pragma unroll
+        for (int i = 0; i < kKeptBlock; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        const BlockStep s(a);
+        s.saturate(v);
+        int8_t* const to = kept.values + row * kept.pitch + first;
+#pragma unroll
+        for (int i = 0; i < kKeptBlock; i += 16) {
+            if (first + i >= kept.pitch) break;
+            uint4 q;
+            q.x = s.quantised(v + i), q.y = s.quantised(v + i + 4), q.z = s.quantised(v + i + 8), q.w = s.quantised(v + i + 12);
+            *reinterpret_cast<uint4*>(to + i) = q;
+        }
+        kept.exponents[row * kept.blocks + first / kKeptBlock] = static_cast<uint8_t>(s.exponent);
+    }
+}
+
+template <class E>
+__global__ __launch_bounds__(kThreads) void unpack_kernel(Lanes l, KeptArray kept, E* __restrict__ x) {
+    over_chunks(l, [&](int64_t row, int c, int valid) {
+        float v[kChunk];
+        kept.load(row, c, valid, v);
+        if constexpr (sizeof(E) == 2 && !std::is_same_v<E, bf16_t>) {
+            // (65520 and more round to 64 * 2^10 = 65536 in a block, which fp16 does not have)
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) v[i] = v[i] > 65504.0f ? 65504.0f : v[i] < -65504.0f ? -65504.0f : v[i];
+        }
+        if (valid > 0) store_chunk(x + row * l.channels + c, valid, v);
+    });
+}
+
+// act(x) and act'(x)
+template <int kKind>
+__device__ __forceinline__ void activate(float x, float& value, float& slope) {
+    if constexpr (kKind == PENC_GELU) {
+        const float below = 0.5f * (1.0f + erff(x * 0.70710678f));
+        value = x * below;
+        slope = below + x * (0.39894228f * expf(-0.5f * x * x));
+    } else if constexpr (kKind == PENC_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + expf(-x));
+        value = x * s;
+        slope = s * (1.0f + x * (1.0f - s));
+    } else {
+        const float e = expf(-fabsf(x)), r = __builtin_amdgcn_rcpf(1.0f + e);
+        value = fmaxf(x, 0.0f) + log1pf(e);
+        slope = x < 0.0f ? e * r : r;
+        if (x != x) value = slope = x;
+    }
+}
+
+template <class E, int kKind, bool kGated>
+__global__ __launch_bounds__(kThreads) void activation_kernel(Lanes l, const E* __restrict__ x, int64_t stride, E* __restrict__ y, KeptArray kept,
+                                                              KeptArray kept_gate) {
+    over_chunks(l, [&](int64_t row, int c, int valid) {
+        float a[kChunk], b[kChunk], unused;
+        load_chunk(x + row * stride + c, valid, a);
+        if constexpr (kGated) load_chunk(x + row * stride + l.channels + c, valid, b);
+        if (kept.values != nullptr) {
+            kept.store(row, c, a);
+            if constexpr (kGated) kept_gate.store(row, c, b);
+        }
+        if (valid <= 0) return;
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+            activate<kKind>(a[i], a[i], unused);
+            if constexpr (kGated) a[i] *= b[i];
+        }
+        store_chunk(y + row * l.channels + c, valid, a);
+    });
+}
+
+// x: the input itself, or null where it is kept in 8 bits
+template <class E, int kKind, bool kGated>
+__global__ __launch_bounds__(kThreads) void activation_backward_kernel(Lanes l, const E* __restrict__ x, int64_t stride, KeptArray kept,
+                                                                       KeptArray kept_gate, const E* __restrict__ grad, int64_t grad_stride,
+                                                                       E* __restrict__ dx) {
+    over_chunks(l, [&](int64_t row, int c, int valid) {
+        if (valid <= 0) return;
+        float a[kChunk], b[kChunk], g[kChunk], value, slope;
+        load_chunk(grad + row * grad_stride + c, valid, g);
+        if (x != nullptr) {
+            load_chunk(x + row * stride + c, valid, a);
+            if constexpr (kGated) load_chunk(x + row * stride + l.channels + c, valid, b);
+        } else {
+            kept.load(row, c, valid, a);
+            if constexpr (kGated) kept_gate.load(row, c, valid, b);
+        }
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+            activate<kKind>(a[i], value, slope);
+            if constexpr (kGated) {
+                a[i] = g[i] * b[i] * slope;
+                b[i] = g[i] * value;
+            } else {
+                a[i] = g[i] * slope;
+            }
+        }
+        E* const to = dx + row * l.channels * (kGated ? 2 : 1) + c;
+        store_chunk(to, valid, a);
+        if constexpr (kGated) store_chunk(to + l.channels, valid, b);
+    });
+}
+
+template <class F>
+int with_kind(int kind, int gated, F&& f) {
+    const auto with_gate = [&](auto k) { return gated ? f(k, std::true_type{}) : f(k, std::false_type{}); };
+    switch (kind) {
+        case PENC_GELU: return with_gate(std::integral_constant<int, PENC_GELU>{});
+        case PENC_SILU: return with_gate(std::integral_constant<int, PENC_SILU>{});
+        case PENC_SOFTPLUS: return with_gate(std::integral_constant<int, PENC_SOFTPLUS>{});
+        default: return PENC_ERR_UNSUPPORTED_KIND;
+    }
+}
+
+bool bad_size(int64_t rows, int64_t channels) { return rows < 0 || channels <= 0 || channels > PENC_MAX_CHANNELS; }
+bool misplaced(const int8_t* values) { return !aligned_to(values, kKeptPitch); }
+
+// How the backward of a norm is cut up: workgroups, pieces of a group of rows that share a gate, and the rows of partial sums they leave.
+struct NormPlan {
+    unsigned grid;
+    int64_t pieces, piece_rows, gate_rows;
+    bool gate_by_lanes;
+};
+NormPlan norm_plan(int64_t rows, int64_t channels, int64_t rows_per_gate) {
+    constexpr int64_t kMost = 512;  // workgroups: what the card holds of them at a time
+    const int64_t at_a_time = rows_at_a_time(static_cast<int>(channels));
+    const auto groups_of = [&](int64_t n) { return std::max<int64_t>(1, (n + at_a_time - 1) / at_a_time); };
+    NormPlan p{0, 1, rows_per_gate, 0, false};
+    if (rows_per_gate == 0) {
+        p.grid = static_cast<unsigned>(std::min(kMost, groups_of(rows)));
+        p.gate_rows = p.grid;
+    } else if (rows_per_gate < 2 * at_a_time) {
+        p.gate_by_lanes = true;
+        p.grid = static_cast<unsigned>(std::min(kMost, groups_of(rows / rows_per_gate)));
+    } else {
+        const int64_t groups = std::max<int64_t>(1, rows / rows_per_gate);
+        const int64_t wanted = std::min((2 * kMost + groups - 1) / groups, groups_of(rows_per_gate));
+        p.piece_rows = groups_of((rows_per_gate + wanted - 1) / wanted) * at_a_time;
+        p.pieces = (rows_per_gate + p.piece_rows - 1) / p.piece_rows;
+        p.grid = static_cast<unsigned>(std::min(kMost, groups * p.pieces));
+        p.gate_rows = p.pieces > 1 ? groups * p.pieces : 0;
+    }
+    return p;
+}
+
+// The checks and the kernels' arguments that the two directions share; false with `status` where there is nothing to launch.
+bool norm_args(const penc_norm* n, NormArgs& a, int& status) {
+    status = PENC_ERR_NULL_POINTER;
+    if (!n) return false;
+    status = PENC_ERR_UNSUPPORTED_KIND;
+    if (n->kind != PENC_RMS && n->kind != PENC_LAYER) return false;
+    status = PENC_ERR_UNSUPPORTED_TYPE;
+    if ((n->type != PENC_FP32 && n->type != PENC_FP16 && n->type != PENC_BF16) || (n->param_type != n->type && n->param_type != PENC_FP32) ||
+        (n->gate_type != n->type && n->gate_type != PENC_FP32))
+        return false;
+    status = PENC_ERR_BAD_LAYER_SIZE;
+    if (n->rows < 0 || n->channels <= 0 || n->channels > PENC_MAX_NORM_CHANNELS || n->rows_per_gate < 0 ||
+        (n->rows_per_gate > 0 && n->rows % n->rows_per_gate != 0))
+        return false;
+    status = PENC_ERR_NULL_POINTER;
+    if ((n->x_values == nullptr) != (n->x_exponents == nullptr) || (n->branch_values == nullptr) != (n->branch_exponents == nullptr)) return false;
+    status = PENC_ERR_MISALIGNED;
+    const size_t size = n->type == PENC_FP32 ? 4 : 2, param = n->param_type == PENC_FP32 ? 4 : 2, gate = n->gate_type == PENC_FP32 ? 4 : 2;
+    if (misplaced(n->x_values) || misplaced(n->branch_values) || !aligned_to(n->x, size) || !aligned_to(n->branch, size) || !aligned_to(n->gate, gate) ||
+        !aligned_to(n->post_weight, param) || !aligned_to(n->post_bias, param) || !aligned_to(n->pre_weight, param) || !aligned_to(n->pre_bias, param))
+        return false;
+    a = {n->rows, n->rows_per_gate, n->x_stride, n->branch_stride, static_cast<int>(n->channels), n->residual_scale, n->eps, n->kind == PENC_LAYER,
+         n->post_norm != 0, n->pre_norm != 0, n->has_branch != 0, n->param_type == PENC_FP32, n->gate_type == PENC_FP32, false, n->x, n->branch, n->gate,
+         n->post_weight, n->post_bias, n->pre_weight, n->pre_bias, kept_array(n->x_values, n->x_exponents, n->channels),
+         kept_array(n->branch_values, n->branch_exponents, n->channels)};
+    status = PENC_OK;
+    return true;
+}
+
+NormLaunches norm_launches_of(int type) {
+    return type == PENC_FP32 ? norm_launches<PENC_FP32>() : type == PENC_FP16 ? norm_launches<PENC_FP16>() : norm_launches<PENC_BF16>();
+}
+
+}  // namespace
+}  // namespace penc
+
+using namespace penc;
+
+extern "C" {
+
+int64_t penc_kept_pitch(int64_t channels) { return kept_pitch(channels); }
+int64_t penc_kept_blocks(int64_t channels) { return kept_blocks(channels); }
+
+int penc_keep(int type, int64_t rows, int64_t channels, const void* x, int64_t row_stride, int64_t channel_stride, int8_t* values,
+              uint8_t* exponents, void* stream) {
+    if (bad_size(rows, channels) || (channel_stride != 1 && row_stride != 1)) return PENC_ERR_BAD_LAYER_SIZE;
+    return with_type(type, [&](auto e) {
+        using E = decltype(e);
+        if (rows == 0) return PENC_OK;
+        if (!x || !values || !exponents) return PENC_ERR_NULL_POINTER;
+        if (misplaced(values) || !aligned_to(x, sizeof(E))) return PENC_ERR_MISALIGNED;
+        const KeptArray kept = kept_array(values, exponents, channels);
+        if (channel_stride == 1) {
+            const Lanes l = lanes_for(rows, channels);
+            hipLaunchKernelGGL(pack_kernel<E>, dim3(l.grid), dim3(kThreads), 0, static_cast<hipStream_t>(stream), l, static_cast<const E*>(x),
+                               row_stride, kept);
+        } else {
+            const int64_t groups = (rows + kThreads - 1) / kThreads;
+            if (groups > 0x7FFFFFFF) return PENC_ERR_BAD_LAYER_SIZE;
+            hipLaunchKernelGGL(pack_channels_kernel<E>, dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), rows,
+                               static_cast<int>(channels), static_cast<const E*>(x), channel_stride, kept);
+        }
+        return launched();
+    });
+}
+
+int penc_restore(int type, int64_t rows, int64_t channels, const int8_t* values, const uint8_t* exponents, void* x, void* stream) {
+    if (bad_size(rows, channels)) return PENC_ERR_BAD_LAYER_SIZE;
+    return with_type(type, [&](auto e) {
+        using E = decltype(e);
+        if (rows == 0) return PENC_OK;
+        if (!x || !values || !exponents) return PENC_ERR_NULL_POINTER;
+        if (misplaced(values) || !aligned_to(x, sizeof(E))) return PENC_ERR_MISALIGNED;
+        const Lanes l = lanes_for(rows, channels);
+        hipLaunchKernelGGL(unpack_kernel<E>, dim3(l.grid), dim3(kThreads), 0, static_cast<hipStream_t>(stream), l, kept_array(values, exponents, channels),
+                           static_cast<E*>(x));
+        return launched();
+    });
+}
+
+int penc_activation(int type, int kind, int gated, int64_t rows, int64_t channels, const void* x, int64_t row_stride, void* y, int8_t* values,
+                    uint8_t* exponents, void* stream) {
+    if (bad_size(rows, channels)) return PENC_ERR_BAD_LAYER_SIZE;
+    return with_type(type, [&](auto e) {
+        using E = decltype(e);
+        return with_kind(kind, gated, [&](auto k, auto g) {
+            if (rows == 0) return PENC_OK;
+            if (!x || !y || (values == nullptr) != (exponents == nullptr)) return PENC_ERR_NULL_POINTER;
+            if (misplaced(values) || !aligned_to(x, sizeof(E)) || !aligned_to(y, sizeof(E))) return PENC_ERR_MISALIGNED;
+            const Lanes l = lanes_for(rows, channels);
+            const KeptArray kept = kept_array(values, exponents, channels);
+            KeptArray kept_gate = kept;
+            if (values != nullptr) kept_gate.values += rows * kept.pitch, kept_gate.exponents += rows * kept.blocks;
+            hipLaunchKernelGGL((activation_kernel<E, decltype(k)::value, decltype(g)::value>), dim3(l.grid), dim3(kThreads), 0,
+                               static_cast<hipStream_t>(stream), l, static_cast<const E*>(x), row_stride, static_cast<E*>(y), kept, kept_gate);
+            return launched();
+        });
+    });
+}
+
+int penc_activation_backward(int type, int kind, int gated, int64_t rows, int64_t channels, const void* x, int64_t row_stride, const int8_t* values,
+                             const uint8_t* exponents, const void* grad, int64_t grad_row_stride, void* dx, void* stream) {
+    if (bad_size(rows, channels)) return PENC_ERR_BAD_LAYER_SIZE;
+    return with_type(type, [&](auto e) {
+        using E = decltype(e);
+        return with_kind(kind, gated, [&](auto k, auto g) {
+            if (rows == 0) return PENC_OK;
+            if (!grad || !dx || (!x && (!values || !exponents))) return PENC_ERR_NULL_POINTER;
+            if (misplaced(values) || !aligned_to(x, sizeof(E)) || !aligned_to(grad, sizeof(E)) || !aligned_to(dx, sizeof(E))) return PENC_ERR_MISALIGNED;
+            const Lanes l = lanes_for(rows, channels);
+            const KeptArray kept = kept_array(values, exponents, channels);
+            KeptArray kept_gate = kept;
+            if (values != nullptr) kept_gate.values += rows * kept.pitch, kept_gate.exponents += rows * kept.blocks;
+            hipLaunchKernelGGL((activation_backward_kernel<E, decltype(k)::value, decltype(g)::value>), dim3(l.grid), dim3(kThreads), 0,
+                               static_cast<hipStream_t>(stream), l, static_cast<const E*>(x), row_stride, kept, kept_gate, static_cast<const E*>(grad),
+                               grad_row_stride, static_cast<E*>(dx));
+            return launched();
+        });
+    });
+}
+
+int penc_residual_norm(const penc_norm* norm, void* y, void* n, void* stream) {
+    NormArgs a;
+    int status;
+    if (!norm_args(norm, a, status)) return status;
+    if (a.rows == 0) return PENC_OK;
+    if (!a.x || (a.pre_norm && !n) || (!a.pre_norm && !y) || (a.has_branch && !a.branch)) return PENC_ERR_NULL_POINTER;
+    if (!a.has_branch) a.kept_branch.values = nullptr;
+    const size_t size = norm->type == PENC_FP32 ? 4 : 2;
+    if (!aligned_to(y, size) || !aligned_to(n, size)) return PENC_ERR_MISALIGNED;
+    return norm_launches_of(norm->type).forward(a, y, n, static_cast<hipStream_t>(stream));
+}
+
+size_t penc_residual_norm_workspace_bytes(int64_t rows, int64_t channels, int64_t rows_per_gate) {
+    if (rows < 0 || channels <= 0 || channels > PENC_MAX_NORM_CHANNELS || rows_per_gate < 0) return 0;
+    const NormPlan p = norm_plan(rows, channels, rows_per_gate);
+    return 4 * static_cast<size_t>(channels) * (4 * static_cast<size_t>(p.grid) + static_cast<size_t>(p.gate_rows));
+}
+
+int penc_residual_norm_backward(const penc_norm* norm, const penc_norm_grads* grads, void* workspace, size_t workspace_bytes, void* stream) {
+    NormArgs a;
+    int status;
+    if (!norm_args(norm, a, status)) return status;
+    if (!grads || (grads->gate && !norm->has_branch)) return PENC_ERR_NULL_POINTER;
+    const bool kept = a.kept_x.values != nullptr;
+    if (a.rows > 0 && !kept && (!a.x || (a.has_branch && !a.branch))) return PENC_ERR_NULL_POINTER;
+    if (a.rows > 0 && kept && a.has_branch && !a.kept_branch.values) return PENC_ERR_NULL_POINTER;
+    const size_t size = norm->type == PENC_FP32 ? 4 : 2, param = norm->param_type == PENC_FP32 ? 4 : 2, gate = norm->gate_type == PENC_FP32 ? 4 : 2;
+    for (const void* p : {grads->y, grads->n, static_cast<const void*>(grads->x), static_cast<const void*>(grads->branch)})
+        if (!aligned_to(p, size)) return PENC_ERR_MISALIGNED;
+    for (const void* p : {grads->post_weight, grads->post_bias, grads->pre_weight, grads->pre_bias})
+        if (!aligned_to(p, param)) return PENC_ERR_MISALIGNED;
+    if (!aligned_to(grads->gate, gate) || !aligned_to(workspace, 16)) return PENC_ERR_MISALIGNED;
+    const NormPlan plan = norm_plan(a.rows, a.channels, a.rows_per_gate);
+    if (workspace_bytes < penc_residual_norm_workspace_bytes(a.rows, a.channels, a.rows_per_gate)) return PENC_ERR_WORKSPACE_TOO_SMALL;
+    if (!workspace) return PENC_ERR_NULL_POINTER;
+    a.gate_by_lanes = plan.gate_by_lanes;
+    NormGrads g{grads->y, a.pre_norm ? grads->n : nullptr, grads->y_stride, grads->n_stride, grads->x, a.has_branch ? grads->branch : nullptr, grads->gate,
+                nullptr, {}, plan.pieces, plan.piece_rows};
+    // partial sums of what is wanted, one array after the other
+    float* next = static_cast<float*>(workspace);
+    SumPartials sums{};
+    sums.channels = a.channels;
+    int n = 0;
+    const auto wanted = [&](void* to, int64_t groups, int64_t rows, bool fp32) {
+        if (!to || groups == 0) return static_cast<float*>(nullptr);
+        float* const from = next;
+        next += groups * rows * a.channels;
+        sums.sums[n++] = {from, to, groups, rows, fp32};
+        return from;
+    };
+    void* const to[4] = {grads->post_weight, grads->post_bias, grads->pre_weight, grads->pre_bias};
+    for (int i = 0; i < 4; ++i) g.sums[i] = wanted(to[i], 1, plan.grid, a.param_fp32);
+    if (a.rows_per_gate == 0) g.gate_sums = wanted(g.gate, 1, plan.grid, a.gate_fp32);
+    else if (plan.gate_rows > 0 && a.rows > 0) g.gate_sums = wanted(g.gate, a.rows / a.rows_per_gate, plan.pieces, a.gate_fp32);
+    const NormLaunches launches = norm_launches_of(norm->type);
+    // (without rows the workgroups leave sums of nothing)
+    if (a.rows > 0 || n > 0)
+        if (const int rc = launches.backward(a, g, plan.grid, static_cast<hipStream_t>(stream))) return rc;
+    if (n == 0) return PENC_OK;
+    int64_t groups = 1;
+    for (int i = 0; i < n; ++i) groups = std::max(groups, sums.sums[i].groups);
+    const int64_t grid = groups * ((a.channels + 31) / 32);
+    if (grid > 0x7FFFFFFF) return PENC_ERR_BAD_LAYER_SIZE;
+    return launches.sum_partials(sums, static_cast<unsigned>(grid), n, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

@@ -48,12 +48,14 @@
 #include <vector>
 
 #include "../../include/penc.h"
+#include "penc_torch.hpp"
 
 namespace {
 
 using at::Tensor;
 using torch::autograd::Node;
 using torch::autograd::variable_list;
+using namespace penc_torch;
 
 // ------------------------------------------------------------------------------------------
 // the C ABI
@@ -98,16 +100,10 @@ void check(int status, const char* what) {
     if (status != PENC_OK) TORCH_CHECK(false, what, ": ", api.status_string(status), " (status ", status, ")");
 }
 
-#define PENC_REQUIRE(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
-
 void require_f32_gpu(const Tensor& t, const char* name, int64_t ndim) {
     PENC_REQUIRE(t.is_cuda(), name, " should be in GPU memory. Please call .cuda() on the tensor");
     PENC_REQUIRE(t.scalar_type() == at::kFloat, name, " should be of type float");
     PENC_REQUIRE(t.dim() == ndim, name, " should have ", ndim, " dimensions, however it has sizes ", t.sizes());
-}
-
-void* current_stream(const at::Device& device) {
-    return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index()).stream();
 }
 
 // The capture that a stream takes part in, 0 where it takes part in none.
@@ -912,39 +908,6 @@ variable_list EncodeNode::apply(variable_list&& grads) {
 // ------------------------------------------------------------------------------------------
 // Python
 
-const Tensor& tensor_arg(PyObject* o, const char* name) {
-    PENC_REQUIRE(THPVariable_Check(o), name, " must be a torch.Tensor");
-    return THPVariable_Unpack(o);
-}
-
-// Runs `body` with C++ exceptions turned into Python ones.
-template <typename F>
-PyObject* guarded(F&& body) {
-    try {
-        return body();
-    } catch (python_error& e) {
-        e.restore();
-    } catch (const c10::ValueError& e) {
-        PyErr_SetString(PyExc_ValueError, e.what_without_backtrace());
-    } catch (const c10::OutOfMemoryError& e) {
-        PyObject* const torch_module = PyImport_ImportModule("torch");
-        PyObject* const type = torch_module != nullptr ? PyObject_GetAttrString(torch_module, "OutOfMemoryError") : nullptr;
-        PyErr_SetString(type != nullptr ? type : PyExc_RuntimeError, e.what_without_backtrace());
-        Py_XDECREF(type);
-        Py_XDECREF(torch_module);
-    } catch (const c10::Error& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-    }
-    return nullptr;
-}
-
-struct NoGil {
-    PyThreadState* state = PyEval_SaveThread();
-    ~NoGil() { PyEval_RestoreThread(state); }
-};
-
 // The checks of a call, in the order and with the words of _native.EncodingWrapper (reference: src/Encoding.cu:38-45, 57-66).
 void prepare_call(Call& c, const Tensor& positions, const Tensor& window) {
     require_f32_gpu(positions, "positions", 2);
@@ -1345,6 +1308,7 @@ PyObject* py_bind(PyObject*, PyObject* path) {
         PENC_FN(backward_positions_slopes);
         PENC_FN(grad_grad_slopes);
 #undef PENC_FN
+        bind_layers(lib);
         Py_RETURN_NONE;
     });
 }
@@ -1375,5 +1339,10 @@ PyMODINIT_FUNC PyInit__penc_torch() {
     const std::string key = "penc_slopes " + std::to_string(reinterpret_cast<uintptr_t>(&module));
     if (!c10::FreeHipMemoryCallbacksRegistry()->Has(key))
         c10::FreeHipMemoryCallbacksRegistry()->Register(key, []() -> std::unique_ptr<c10::FreeMemoryCallback> { return std::make_unique<GiveBackSlopes>(); });
-    return PyModule_Create(&module);
+    PyObject* const made = PyModule_Create(&module);
+    if (made != nullptr && !add_layer_functions(made)) {
+        Py_DECREF(made);
+        return nullptr;
+    }
+    return made;
 }
