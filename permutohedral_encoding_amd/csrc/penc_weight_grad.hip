@@ -36,42 +36,76 @@ struct Frag {
 __device__ __forceinline__ uint32_t low_halves(uint32_t first, uint32_t second) { return __builtin_amdgcn_perm(second, first, 0x05040100u); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t first, uint32_t second) { return __builtin_amdgcn_perm(second, first, 0x07060302u); }
 
-// What a lane has of the gradient: 8 rows of kWide columns, as they are in memory.
+// Where a lane's 8 rows of a step are.  The last step's lanes that would read behind `last` read the 8 rows before it instead, and `skip` of them count
+// for nothing: loads have no conditions.
+struct StepRows {
+    int64_t first;  // of the step, the same in every lane
+    uint32_t at;    // the lane's, from there on
+    int skip;
+
+    __device__ __forceinline__ StepRows(int64_t step, int row_at, int64_t last) {
+        const int64_t most = last - kLaneRows;
+        first = min(step, most);
+        const int64_t row = min(step + row_at, most);
+        at = static_cast<uint32_t>(row - first);
+        skip = static_cast<int>(step + row_at - row);
+    }
+};
+
+// Registers of a row.
+template <int kWords>
+using words_t = uint32_t __attribute__((ext_vector_type(kWords)));
+
+// Rows that count for nothing, after their loads have come.
+template <class W>
+__device__ __forceinline__ void skip_rows(W (&row)[kLaneRows], int skip) {
+    if (skip == 0) return;
+#pragma unroll
+    for (int j = 0; j < kLaneRows; ++j) row[j] = j < skip ? W{} : row[j];
+}
+
+// What a lane has of the gradient, 8 rows of kWide columns as they are in memory, in kWords registers a row.
 template <class E, int kWide>
 struct GradTile {
     static constexpr int kPieces = std::is_same_v<E, float> ? 3 : std::is_same_v<E, half_t> ? 2 : 1;
     static constexpr int kWords = kWide * sizeof(E) / 4;
     using Bits = std::conditional_t<sizeof(E) == 4, uint32_t, uint16_t>;
     using Vector = uint32_t __attribute__((ext_vector_type(kWords), aligned(sizeof(E))));
-    uint32_t row[kLaneRows][kWords];
 
-    __device__ __forceinline__ void load(const E* __restrict__ g, int64_t stride, int64_t rows_left, int valid) {
+    // The columns from which a lane reads: the last lane of a row, where it has fewer than kWide, takes some that its neighbour has too, and finds the same sums.
+    __device__ __forceinline__ static int column_of(int o, int outputs) { return min(o, outputs - kWide); }
+
+    template <class W>
+    __device__ __forceinline__ static void load(W (&row)[kLaneRows], const void* grad, int64_t stride, StepRows rows, int column) {
+        const char* const first = static_cast<const char*>(grad) + rows.first * stride * static_cast<int64_t>(sizeof(E));
+        const uint32_t at = (rows.at * static_cast<uint32_t>(stride) + static_cast<uint32_t>(column)) * static_cast<uint32_t>(sizeof(E));
 #pragma unroll
         for (int j = 0; j < kLaneRows; ++j) {
-            if (j < rows_left && valid >= kWide) {
-                const Vector v = *reinterpret_cast<const Vector*>(g + j * stride);
+            const Vector v = *reinterpret_cast<const Vector*>(first + j * stride * static_cast<int64_t>(sizeof(E)) + at);
 #pragma unroll
-                for (int w = 0; w < kWords; ++w) row[j][w] = v[w];
-            } else {
-                const auto bits = [&](int t) { return j < rows_left && t < valid ? static_cast<uint32_t>(__builtin_bit_cast(Bits, g[j * stride + t])) : 0u; };
-#pragma unroll
-                for (int w = 0; w < kWords; ++w) row[j][w] = sizeof(E) == 4 ? bits(w) : bits(2 * w) | bits(2 * w + 1) << 16;
-            }
+            for (int w = 0; w < kWords; ++w) row[j][w] = v[w];
         }
     }
-    __device__ __forceinline__ float value(int j, int t) const {
-        if constexpr (sizeof(E) == 4) return __uint_as_float(row[j][t]);
-        else return static_cast<float>(__builtin_bit_cast(E, static_cast<uint16_t>(row[j][t / 2] >> 16 * (t % 2))));
+    // for fewer rows or columns than a lane takes
+    template <class W>
+    __device__ __forceinline__ static void load_ragged(W (&row)[kLaneRows], const E* __restrict__ g, int64_t stride, int64_t rows_left, int valid) {
+#pragma unroll
+        for (int j = 0; j < kLaneRows; ++j) {
+            const auto bits = [&](int t) { return j < rows_left && t < valid ? static_cast<uint32_t>(__builtin_bit_cast(Bits, g[j * stride + t])) : 0u; };
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) row[j][w] = sizeof(E) == 4 ? bits(w) : bits(2 * w) | bits(2 * w + 1) << 16;
+        }
     }
     // column t in kPieces parts
-    __device__ __forceinline__ void column(int t, Frag (&f)[kPieces]) const {
+    template <class W>
+    __device__ __forceinline__ static void column(const W (&row)[kLaneRows], int t, Frag (&f)[kPieces]) {
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             if constexpr (kPieces == 1) {
                 const uint32_t a = row[2 * p][t / 2], b = row[2 * p + 1][t / 2];
                 f[0].d[p] = t % 2 == 0 ? low_halves(a, b) : high_halves(a, b);
             } else {
-                float a = value(2 * p, t), b = value(2 * p + 1, t);
+                float a = value(row[2 * p], t), b = value(row[2 * p + 1], t);
 #pragma unroll
                 for (int k = 0; k < kPieces; ++k) {
                     f[k].d[p] = high_halves(__float_as_uint(a), __float_as_uint(b));
@@ -80,6 +114,11 @@ struct GradTile {
             }
         }
     }
+    template <class W>
+    __device__ __forceinline__ static float value(const W& row, int t) {
+        if constexpr (sizeof(E) == 4) return __uint_as_float(row[t]);
+        else return static_cast<float>(__builtin_bit_cast(E, static_cast<uint16_t>(row[t / 2] >> 16 * (t % 2))));
+    }
     // x without its first 8 bits; nothing is left of an infinity, and a NaN stays one
     __device__ __forceinline__ static float rest(float x) {
         const float first = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
@@ -87,31 +126,51 @@ struct GradTile {
     }
 };
 
-// What a lane has of the checkpoint: 8 rows of kWide columns, all of one block.
+// What a lane has of the checkpoint: 8 rows of kWide columns, all of one block, and behind them the block's exponent.
 template <int kWide>
 struct KeptTile {
-    using Bytes = std::conditional_t<kWide == 8, uint2, uint32_t>;
-    Bytes row[kLaneRows];
-    uint32_t exponent[kLaneRows];
+    static constexpr int kWords = kWide / 4 + 1;
+    using Vector = uint32_t __attribute__((ext_vector_type(kWide / 4)));
 
-    __device__ __forceinline__ void load(const KeptArray& kept, int64_t first, int64_t rows_left, int c) {
+    // (columns behind a row's end are read from within it, for results that are not stored)
+    __device__ __forceinline__ static int column_of(int c, const KeptArray& kept) { return min(c, static_cast<int>(kept.pitch) - kWide); }
+
+    template <class W>
+    __device__ __forceinline__ static void load(W (&row)[kLaneRows], const KeptArray& kept, StepRows rows, int column) {
+        const int8_t* const values = kept.values + rows.first * kept.pitch;
+        const uint8_t* const exponents = kept.exponents + rows.first * kept.blocks;
+        const uint32_t at = rows.at * static_cast<uint32_t>(kept.pitch) + static_cast<uint32_t>(column);
+        const uint32_t block_at = rows.at * static_cast<uint32_t>(kept.blocks) + static_cast<uint32_t>(column / kKeptBlock);
 #pragma unroll
         for (int j = 0; j < kLaneRows; ++j) {
-            const bool there = j < rows_left && c < kept.pitch;
-            row[j] = there ? *reinterpret_cast<const Bytes*>(kept.values + (first + j) * kept.pitch + c) : Bytes{};
-            exponent[j] = there ? kept.exponents[(first + j) * kept.blocks + c / kKeptBlock] : 0;
+            const Vector v = *reinterpret_cast<const Vector*>(values + j * kept.pitch + at);
+#pragma unroll
+            for (int w = 0; w < kWide / 4; ++w) row[j][w] = v[w];
+            row[j][kWide / 4] = (exponents + j * kept.blocks)[block_at];
         }
     }
-    __device__ __forceinline__ float value(int j, int t) const {
-        uint32_t word;
-        if constexpr (kWide == 8) word = t < 4 ? row[j].x : row[j].y;
-        else word = row[j];
-        return static_cast<float>(static_cast<int8_t>(word >> 8 * (t % 4))) * kept_step(exponent[j]);
+    template <class W>
+    __device__ __forceinline__ static void load_ragged(W (&row)[kLaneRows], const KeptArray& kept, int64_t first, int64_t rows_left, int column) {
+#pragma unroll
+        for (int j = 0; j < kLaneRows; ++j) {
+            const bool there = j < rows_left;
+            const Vector v = there ? *reinterpret_cast<const Vector*>(kept.values + (first + j) * kept.pitch + column) : Vector{};
+#pragma unroll
+            for (int w = 0; w < kWide / 4; ++w) row[j][w] = v[w];
+            row[j][kWide / 4] = there ? kept.exponents[(first + j) * kept.blocks + column / kKeptBlock] : 0;
+        }
     }
-    __device__ __forceinline__ Frag column(int t) const {
+    // q 2^e as (q + 128) 2^e - 2^(e + 7), exact, of bytes that v_cvt_f32_ubyte takes where they are
+    template <class W>
+    __device__ __forceinline__ static uint32_t value(const W& row, int t) {
+        const float biased = static_cast<float>((row[t / 4] ^ 0x80808080u) >> 8 * (t % 4) & 0xFFu), step = kept_step(row[kWide / 4]);
+        return __float_as_uint(__builtin_fmaf(biased, step, -128.0f * step));
+    }
+    template <class W>
+    __device__ __forceinline__ static Frag column(const W (&row)[kLaneRows], int t) {
         Frag f;
 #pragma unroll
-        for (int p = 0; p < 4; ++p) f.d[p] = high_halves(__float_as_uint(value(2 * p, t)), __float_as_uint(value(2 * p + 1, t)));
+        for (int p = 0; p < 4; ++p) f.d[p] = high_halves(value(row[2 * p], t), value(row[2 * p + 1], t));
         return f;
     }
 };
@@ -124,33 +183,53 @@ struct WeightGrad {
     float *sums, *bias_sums;  // [splits][outputs][channels], [splits][outputs] or null
 };
 
+// The work of a workgroup.  Consecutive workgroups go to the 8 dies in turn: each of them gets neighbouring items, tiles of the same rows, which its cache
+// then holds.
+__device__ __forceinline__ int64_t item_of(const WeightGrad& a) {
+    constexpr unsigned kDies = 8;
+    const unsigned die = blockIdx.x % kDies, each = gridDim.x / kDies, rest = gridDim.x % kDies;
+    return die * each + min(die, rest) + blockIdx.x / kDies;
+}
+
 // 16 kWideO outputs by 16 kWideC channels.
-template <class E, int kWideO, int kWideC, int kWaves>
+template <class E, int kWideO, int kWideC, int kWaves, bool kRagged>
 __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) {
     constexpr int kPieces = GradTile<E, kWideO>::kPieces;
     __shared__ float lds[kWaves][16][16 * kWideC];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, column = lane % 16, rows_at = lane / 16 * kLaneRows;
-    const int tile = blockIdx.x % (a.channel_tiles * a.output_tiles), split = blockIdx.x / (a.channel_tiles * a.output_tiles);
+    const int64_t item = item_of(a);
+    const int tile = static_cast<int>(item % (a.channel_tiles * a.output_tiles));
+    const int64_t split = item / (a.channel_tiles * a.output_tiles);
     const int c0 = tile % a.channel_tiles * 16 * kWideC, o0 = tile / a.channel_tiles * 16 * kWideO;
-    const int c = c0 + column * kWideC, o = o0 + column * kWideO;
+    using G = GradTile<E, kWideO>;
+    using X = KeptTile<kWideC>;
+    const int c = X::column_of(c0 + column * kWideC, a.kept), o = kRagged ? o0 + column * kWideO : G::column_of(o0 + column * kWideO, a.outputs);
     const bool bias = a.bias_sums != nullptr && c0 == 0;
     const int64_t first = split * a.split_rows, last = min(first + a.split_rows, a.rows);
 
     acc_t acc[kWideO][kWideC] = {}, bias_acc[kWideO] = {};
     const Frag ones = {{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}};
     for (int64_t step = first + wave * kStep; step < last; step += kWaves * kStep) {
-        GradTile<E, kWideO> g;
-        KeptTile<kWideC> x;
-        const int64_t row = step + rows_at;
-        g.load(static_cast<const E*>(a.grad) + row * a.grad_stride + o, a.grad_stride, last - row, a.outputs - o);
-        x.load(a.kept, row, last - row, c);
+        words_t<G::kWords> g[kLaneRows];
+        words_t<X::kWords> x[kLaneRows];
+        if constexpr (kRagged) {
+            const int64_t row = step + rows_at;
+            G::load_ragged(g, static_cast<const E*>(a.grad) + row * a.grad_stride + o, a.grad_stride, last - row, a.outputs - o);
+            X::load_ragged(x, a.kept, row, last - row, c);
+        } else {
+            const StepRows rows(step, rows_at, a.rows);
+            G::load(g, a.grad, a.grad_stride, rows, o);
+            X::load(x, a.kept, rows, c);
+            skip_rows(g, rows.skip);
+            skip_rows(x, rows.skip);
+        }
         Frag fx[kWideC];
 #pragma unroll
-        for (int s = 0; s < kWideC; ++s) fx[s] = x.column(s);
+        for (int s = 0; s < kWideC; ++s) fx[s] = X::column(x, s);
 #pragma unroll
         for (int t = 0; t < kWideO; ++t) {
             Frag fg[kPieces];
-            g.column(t, fg);
+            G::column(g, t, fg);
 #pragma unroll
             for (int k = 0; k < kPieces; ++k) {
 #pragma unroll
@@ -160,7 +239,7 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
         }
     }
     // Lane (16 i + n) has rows 4 i .. 4 i + 3 of a result's column n.
-    float* const sums = a.sums + static_cast<int64_t>(split) * a.outputs * a.channels;
+    float* const sums = a.sums + split * a.outputs * a.channels;
 #pragma unroll
     for (int t = 0; t < kWideO; ++t) {
         if (t > 0) __syncthreads();
@@ -170,7 +249,9 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
             for (int s = 0; s < kWideC; ++s) lds[wave][lane / 16 * 4 + r][column * kWideC + s] = acc[t][s][r];
         __syncthreads();
         for (int i = threadIdx.x; i < 16 * 16 * kWideC; i += 64 * kWaves) {
-            const int m = i / (16 * kWideC), n = i % (16 * kWideC), to = o0 + m * kWideO + t;
+            const int m = i / (16 * kWideC), n = i % (16 * kWideC), from = o0 + m * kWideO;
+            if (from >= a.outputs) continue;
+            const int to = (kRagged ? from : G::column_of(from, a.outputs)) + t;
             float total = lds[0][m][n];
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) total += lds[w][m][n];
@@ -186,51 +267,194 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
             if (column == 0) lds[wave][lane / 16 * 4 + r][t] = bias_acc[t][r];
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * kWideO; i += 64 * kWaves) {
+        const int from = o0 + i / kWideO * kWideO, to = (kRagged ? from : G::column_of(from, a.outputs)) + i % kWideO;
         float total = lds[0][i / kWideO][i % kWideO];
         for (int w = 1; w < kWaves; ++w) total += lds[w][i / kWideO][i % kWideO];
-        if (o0 + i < a.outputs) a.bias_sums[static_cast<int64_t>(split) * a.outputs + o0 + i] = total;
+        if (from < a.outputs && to < a.outputs) a.bias_sums[split * a.outputs + to] = total;
     }
 }
 
-// The splits of `n` weights and, behind them, `n_bias` of the bias, in a fixed order: 64 results and 16 strands of splits to a workgroup.
-template <class To>
-__global__ __launch_bounds__(1024) void sum_splits_kernel(const float* __restrict__ sums, const float* __restrict__ bias_sums, int64_t n, int n_bias,
-                                                          int splits, To* __restrict__ weight, To* __restrict__ bias) {
-    __shared__ float lds[16][64];
-    const int lane = threadIdx.x % 64, strand = threadIdx.x / 64;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+// The same for products that the matrix cores bound: kBlockO outputs by kBlockC channels to a workgroup of 8 waves, which bring 32 kSteps rows at a time
+// into the LDS as the matrix instruction takes them, half of the waves the gradient and half the checkpoint (one of either kind on each SIMD), while all of
+// them multiply what was brought before.  Every value is converted once for the workgroup, and a wave's 4 x 8 tiles multiply a fragment 2.7 times.
+template <class E, int kBlockO, int kBlockC, int kSteps, int kWavesO>
+__global__ __launch_bounds__(512, 2) void weight_grad_lds_kernel(WeightGrad a) {
+    constexpr int kPieces = GradTile<E, 4>::kPieces, kWavesC = 8 / kWavesO;
+    constexpr int kWideO = kBlockO * kSteps / 64, kWideC = kBlockC * kSteps / 64;  // four waves bring each side
+    constexpr int kTilesO = kBlockO / 16 / kWavesO, kTilesC = kBlockC / 16 / kWavesC;
+    constexpr int kGrad = kSteps * kBlockO / 16 * kPieces, kKept = kSteps * kBlockC / 16;  // fragments of 64 lanes
+    __shared__ uint4 fragments[2 * (kGrad + kKept) * 64];                                   // those multiplied, and those brought
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int64_t item = item_of(a);
+    const int tiles = a.channel_tiles * a.output_tiles, tile = static_cast<int>(item % tiles);
+    const int64_t split = item / tiles;
+    const int c0 = tile % a.channel_tiles * kBlockC, o0 = tile / a.channel_tiles * kBlockO;
+    const int64_t first = split * a.split_rows, last = min(first + a.split_rows, a.rows);
+
+    // what this wave brings: 32 rows of 16 kWide columns
+    const bool brings_grad = wave < 4;
+    const int unit = wave % 4, unit_step = unit % kSteps, unit_column = unit / kSteps;
+    const int row_at = unit_step * kStep + lane / 16 * kLaneRows;
+    using G = GradTile<E, kWideO>;
+    using X = KeptTile<kWideC>;
+    const int o = G::column_of(o0 + unit_column * 16 * kWideO + lane % 16 * kWideO, a.outputs);
+    const int c = X::column_of(c0 + unit_column * 16 * kWideC + lane % 16 * kWideC, a.kept);
+    const auto fragment = [&](const uint4* from, int i) { return __builtin_bit_cast(frag_t, from[i * 64 + lane]); };
+    const int first_o = wave % kWavesO * kTilesO, first_c = wave / kWavesO * kTilesC;  // this wave's tiles
+    // the bias is one more column, of ones: the waves with the same outputs have some of them each
+    constexpr int kBias = (kTilesO + kWavesC - 1) / kWavesC;
+    const bool bias = a.bias_sums != nullptr && c0 == 0;
+    const int first_bias = wave / kWavesO * kBias;
+    const Frag ones = {{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}};
+    acc_t acc[kTilesO][kTilesC] = {}, bias_acc[kBias] = {};
+
+    // The loop of a wave that brings the gradient or the checkpoint: conversions and LDS between the products, without branches.  A step's rows are loaded
+    // when those before them have been brought, and have half a step to come.  (Behind the last step they are rows that are there, for fragments that
+    // nobody reads.)
+    const auto walk = [&](auto brings_grad, auto with_bias) {
+        constexpr bool kBringsGrad = decltype(brings_grad)::value;
+        using Side = std::conditional_t<kBringsGrad, G, X>;
+        constexpr int kColumns = kBringsGrad ? kWideO : kWideC, kSlots = kSteps * kPieces * kTilesC, kRows = kSteps * kStep;
+        static_assert(kColumns <= kSlots, "every column has its place between the products");
+        using Raw = words_t<Side::kWords>;
+        const auto load = [&](Raw(&raw)[kLaneRows], int64_t step) {
+            const StepRows rows(step, row_at, a.rows);
+            if constexpr (kBringsGrad) G::load(raw, a.grad, a.grad_stride, rows, o);
+            else X::load(raw, a.kept, rows, c);
+        };
+        const auto skip = [&](Raw(&raw)[kLaneRows], int64_t step) {
+            if (step + kRows > a.rows) skip_rows(raw, StepRows(step, row_at, a.rows).skip);
+        };
+        const auto bring = [&](const Raw(&raw)[kLaneRows], uint4* to, int t) {
+            if constexpr (kBringsGrad) {
+                Frag f[kPieces];
+                G::column(raw, t, f);
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k)
+                    to[((unit_step * kPieces + k) * (kBlockO / 16) + unit_column * kWideO + t) * 64 + lane] = make_uint4(f[k].d[0], f[k].d[1], f[k].d[2], f[k].d[3]);
+            } else {
+                const Frag f = X::column(raw, t);
+                to[(kGrad + unit_step * (kBlockC / 16) + unit_column * kWideC + t) * 64 + lane] = make_uint4(f.d[0], f.d[1], f.d[2], f.d[3]);
+            }
+        };
+        Raw raw[kLaneRows];
+        load(raw, first);
+        skip(raw, first);
+#pragma unroll
+        for (int t = 0; t < kColumns; ++t) bring(raw, fragments, t);
+        load(raw, first + kRows);
+        __syncthreads();
+        int turn = 0;
+        for (int64_t step = first; step < last; step += kRows) {
+            const uint4* const from = fragments + turn * (kGrad + kKept) * 64;
+            uint4* const to = fragments + (turn ^ 1) * (kGrad + kKept) * 64;
+            turn ^= 1;
+            frag_t fg[kTilesO], fx = fragment(from, kGrad + first_c);
+#pragma unroll
+            for (int z = 0; z < kSlots; ++z) {
+                const int s = z % kTilesC, part = z / kTilesC, more = z + 1;
+                if (s == 0) {
+#pragma unroll
+                    for (int t = 0; t < kTilesO; ++t) fg[t] = fragment(from, part * (kBlockO / 16) + first_o + t);
+                }
+                const frag_t now = fx;
+                if (more < kSlots) fx = fragment(from, kGrad + more / kTilesC / kPieces * (kBlockC / 16) + first_c + more % kTilesC);
+#pragma unroll
+                for (int t = 0; t < kTilesO; ++t) acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fg[t], now, acc[t][s], 0, 0, 0);
+                if (decltype(with_bias)::value && s == kTilesC - 1) {
+#pragma unroll
+                    for (int t = 0; t < kBias; ++t)
+                        bias_acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fragment(from, part * (kBlockO / 16) + first_o + first_bias + t), ones.get(), bias_acc[t], 0, 0, 0);
+                }
+                const int column = z - (kSlots - kColumns);
+                if (column == 0) skip(raw, step + kRows);
+                if (column >= 0) bring(raw, to, column);
+                __builtin_amdgcn_sched_barrier(0);  // (or all that is converted waits in registers that there are not)
+            }
+            load(raw, step + 2 * kRows);
+            __syncthreads();
+        }
+    };
+    // (a barrier counts waves, wherever in the code they are: all of them pass the same number)
+    if (brings_grad) {
+        if (bias) walk(std::true_type{}, std::true_type{});
+        else walk(std::true_type{}, std::false_type{});
+    } else {
+        if (bias) walk(std::false_type{}, std::true_type{});
+        else walk(std::false_type{}, std::false_type{});
+    }
+    // Lane (16 i + n) has rows 4 i .. 4 i + 3 of a result's column n; tile T's row m is output (T / kWide * 16 + m) * kWide + T % kWide.
+    float* const sums = a.sums + split * a.outputs * a.channels;
+#pragma unroll
+    for (int t = 0; t < kTilesO; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int big = first_o + t, from = o0 + (big / kWideO * 16 + lane / 16 * 4 + r) * kWideO, to = G::column_of(from, a.outputs) + big % kWideO;
+            if (from >= a.outputs) continue;
+#pragma unroll
+            for (int s = 0; s < kTilesC; ++s) {
+                const int wide = first_c + s, at = c0 + (wide / kWideC * 16 + lane % 16) * kWideC + wide % kWideC;
+                if (at < a.channels) sums[static_cast<int64_t>(to) * a.channels + at] = acc[t][s][r];
+            }
+        }
+    if (!bias || lane % 16 != 0) return;
+#pragma unroll
+    for (int t = 0; t < kBias; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int big = first_o + first_bias + t, from = o0 + (big / kWideO * 16 + lane / 16 * 4 + r) * kWideO;
+            if (from < a.outputs) a.bias_sums[split * a.outputs + G::column_of(from, a.outputs) + big % kWideO] = bias_acc[t][r];
+        }
+}
+
+// The splits of `n` weights and, behind them, `n_bias` of the bias, in a fixed order: 256 / kStrands results to a workgroup, each strand of threads
+// with every kStrands-th split.
+template <class To, int kStrands>
+__global__ __launch_bounds__(256) void sum_splits_kernel(const float* __restrict__ sums, const float* __restrict__ bias_sums, int64_t n, int n_bias,
+                                                         int splits, To* __restrict__ weight, To* __restrict__ bias) {
+    constexpr int kResults = 256 / kStrands;
+    __shared__ float lds[kStrands][kResults];
+    const int lane = threadIdx.x % kResults, strand = threadIdx.x / kResults;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kResults + lane;
     float total = 0.0f;
     if (i < n + n_bias) {
         const float* const from = i < n ? sums + i : bias_sums + (i - n);
         const int64_t stride = i < n ? n : n_bias;
-        for (int s = strand; s < splits; s += 16) total += from[s * stride];
+#pragma unroll 8
+        for (int s = strand; s < splits; s += kStrands) total += from[s * stride];
     }
-    lds[strand][lane] = total;
-    __syncthreads();
-    if (strand != 0 || i >= n + n_bias) return;
-    for (int s = 1; s < 16; ++s) total += lds[s][lane];
+    if constexpr (kStrands > 1) {
+        lds[strand][lane] = total;
+        __syncthreads();
+        if (strand != 0) return;
+        for (int s = 1; s < kStrands; ++s) total += lds[s][lane];
+    }
+    if (i >= n + n_bias) return;
     if (i < n) weight[i] = static_cast<To>(total);
     else bias[i - n] = static_cast<To>(total);
 }
 
-// How a product is cut up.  Tiles of 128 x 128 read each operand least often; where they would be half empty, or too few for the card even with the
-// rows split, 64 columns a side.
+constexpr int64_t kMostStride = 1 << 22;
+
+// How a product is cut up: into the tiles that are at most half empty.
 struct WeightPlan {
-    int wide_o, wide_c, waves, splits;
+    int block_o, block_c, at_a_time, splits;  // columns and rows of a workgroup
+    bool ragged;
     int64_t split_rows;
     int output_tiles, channel_tiles;
 };
-WeightPlan weight_plan(int64_t rows, int64_t channels, int64_t outputs) {
+WeightPlan weight_plan(int64_t rows, int64_t channels, int64_t outputs, int64_t grad_stride) {
     WeightPlan p{};
-    const bool large = channels > 64 && outputs > 64;
-    p.wide_o = p.wide_c = large ? 8 : 4;
-    p.waves = large ? 4 : 8;
-    p.output_tiles = static_cast<int>((outputs + 16 * p.wide_o - 1) / (16 * p.wide_o));
-    p.channel_tiles = static_cast<int>((channels + 16 * p.wide_c - 1) / (16 * p.wide_c));
-    const int64_t tiles = static_cast<int64_t>(p.output_tiles) * p.channel_tiles, at_a_time = p.waves * kStep;
-    const int64_t pieces = std::max<int64_t>(1, (rows + at_a_time - 1) / at_a_time);
-    const int64_t wanted = std::max<int64_t>(1, std::min(pieces, 512 / tiles));
-    p.split_rows = (pieces + wanted - 1) / wanted * at_a_time;
+    // (a lane takes 8 rows of 4 or 8 columns, at 32-bit offsets from a step's first row)
+    p.ragged = rows < kLaneRows || outputs < 4 || grad_stride > kMostStride;
+    p.block_o = p.block_c = p.ragged ? 64 : channels > 128 && outputs > 128 ? 256 : channels > 64 && outputs > 64 ? 128 : 64;
+    p.at_a_time = 8 * kStep;
+    p.output_tiles = static_cast<int>((outputs + p.block_o - 1) / p.block_o);
+    p.channel_tiles = static_cast<int>((channels + p.block_c - 1) / p.block_c);
+    const int64_t tiles = static_cast<int64_t>(p.output_tiles) * p.channel_tiles;
+    const int64_t pieces = std::max<int64_t>(1, (rows + p.at_a_time - 1) / p.at_a_time);
+    const int64_t wanted = std::max<int64_t>(1, std::min(pieces, (p.block_o == 64 ? 512 : 256) / tiles));
+    p.split_rows = (pieces + wanted - 1) / wanted * p.at_a_time;
     p.splits = static_cast<int>(std::max<int64_t>(1, (rows + p.split_rows - 1) / p.split_rows));
     return p;
 }
@@ -239,9 +463,14 @@ bool bad_size(int64_t rows, int64_t channels, int64_t outputs) {
     return rows < 0 || channels <= 0 || channels > PENC_MAX_CHANNELS || outputs <= 0 || outputs > PENC_MAX_CHANNELS || channels * outputs >= int64_t{1} << 31;
 }
 
-template <class E, int kWideO, int kWideC, int kWaves>
-void launch(const WeightGrad& a, unsigned grid, hipStream_t stream) {
-    hipLaunchKernelGGL((weight_grad_kernel<E, kWideO, kWideC, kWaves>), dim3(grid), dim3(64 * kWaves), 0, stream, a);
+template <class E>
+int launch(const WeightGrad& a, const WeightPlan& p, unsigned grid, hipStream_t stream) {
+    constexpr int kPieces = GradTile<E, 4>::kPieces, kSteps = kPieces == 1 ? 2 : 1;
+    if (p.ragged) hipLaunchKernelGGL((weight_grad_kernel<E, 4, 4, 8, true>), dim3(grid), dim3(512), 0, stream, a);
+    else if (p.block_o == 64) hipLaunchKernelGGL((weight_grad_kernel<E, 4, 4, 8, false>), dim3(grid), dim3(512), 0, stream, a);
+    else if (p.block_o == 128) hipLaunchKernelGGL((weight_grad_lds_kernel<E, 128, 128, 2 * kSteps, 4>), dim3(grid), dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((weight_grad_lds_kernel<E, 256, 256, kSteps, 4>), dim3(grid), dim3(512), 0, stream, a);
+    return launched();
 }
 
 }  // namespace
@@ -253,7 +482,7 @@ extern "C" {
 
 size_t penc_weight_grad_workspace_bytes(int64_t rows, int64_t channels, int64_t outputs) {
     if (bad_size(rows, channels, outputs)) return 0;
-    return static_cast<size_t>(weight_plan(rows, channels, outputs).splits) * static_cast<size_t>(channels + 1) * static_cast<size_t>(outputs) * 4;
+    return static_cast<size_t>(std::max(weight_plan(rows, channels, outputs, 0).splits, weight_plan(rows, channels, outputs, kMostStride + 1).splits)) * static_cast<size_t>(channels + 1) * static_cast<size_t>(outputs) * 4;
 }
 
 int penc_weight_grad(int type, int result_type, int64_t rows, int64_t channels, int64_t outputs, const int8_t* values, const uint8_t* exponents,
@@ -269,22 +498,22 @@ int penc_weight_grad(int type, int result_type, int64_t rows, int64_t channels, 
                 !aligned_to(workspace, 16))
                 return PENC_ERR_MISALIGNED;
             if (workspace_bytes < penc_weight_grad_workspace_bytes(rows, channels, outputs)) return PENC_ERR_WORKSPACE_TOO_SMALL;
-            const WeightPlan p = weight_plan(rows, channels, outputs);
+            const WeightPlan p = weight_plan(rows, channels, outputs, grad_row_stride);
             float* const sums = static_cast<float*>(workspace);
             const int64_t n = channels * outputs;
             const WeightGrad a{rows, grad_row_stride, p.split_rows, static_cast<int>(channels), static_cast<int>(outputs), p.channel_tiles,
                                p.output_tiles, kept_array(values, exponents, channels), grad, sums, bias_grad ? sums + p.splits * n : nullptr};
             const int64_t grid = static_cast<int64_t>(p.splits) * p.output_tiles * p.channel_tiles;
             const int n_bias = bias_grad ? static_cast<int>(outputs) : 0;
-            const int64_t sum_grid = (n + n_bias + 63) / 64;
             if (grid > 0x7FFFFFFF) return PENC_ERR_BAD_LAYER_SIZE;
             hipStream_t st = static_cast<hipStream_t>(stream);
-            if (p.wide_o == 8) launch<E, 8, 8, 4>(a, static_cast<unsigned>(grid), st);
-            else launch<E, 4, 4, 8>(a, static_cast<unsigned>(grid), st);
-            if (const int rc = launched()) return rc;
-            hipLaunchKernelGGL(sum_splits_kernel<To>, dim3(static_cast<unsigned>(sum_grid)), dim3(1024), 0, st, sums, a.bias_sums, n, n_bias, p.splits,
-                               static_cast<To*>(weight_grad), static_cast<To*>(bias_grad));
-            return launched();
+            if (const int rc = launch<E>(a, p, static_cast<unsigned>(grid), st)) return rc;
+            const auto sum = [&](auto kernel, int results) {
+                hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((n + n_bias + results - 1) / results)), dim3(256), 0, st, sums, a.bias_sums, n, n_bias,
+                                   p.splits, static_cast<To*>(weight_grad), static_cast<To*>(bias_grad));
+                return launched();
+            };
+            return p.splits < 16 ? sum(sum_splits_kernel<To, 1>, 256) : sum(sum_splits_kernel<To, 16>, 16);
         });
     });
 }

@@ -120,7 +120,8 @@ def test_checkpoint_behind_two_to_the_31_values():
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,channels,outputs", [(0, 5, 3), (1, 1, 1), (1, 48, 64), (31, 33, 65), (257, 48, 64), (300, 200, 130), (4097, 32, 64), (1000, 64, 3),
-                                                   (513, 8, 257), (70000, 48, 16), (2049, 129, 128)])
+                                                   (513, 8, 257), (70000, 48, 16), (2049, 129, 128),
+                                                   (7, 300, 300), (8, 257, 130), (9, 70, 66), (600, 300, 520), (40000, 129, 257), (20011, 72, 90)])
 def test_weight_grad(dtype, rows, channels, outputs):
     x = values(rows, channels, TYPES[dtype], wide=channels + 3)
     grad = values(rows, outputs, TYPES[dtype], seed=1, wide=outputs + 1)
