@@ -188,22 +188,22 @@ struct NormPlan {
     bool gate_by_lanes;
 };
 NormPlan norm_plan(int64_t rows, int64_t channels, int64_t rows_per_gate) {
-    constexpr int64_t kMost = 512;  // workgroups: what the card holds of them at a time
-    const int64_t at_a_time = rows_at_a_time(static_cast<int>(channels));
+    const int lanes = lanes_of_row(static_cast<int>(channels));
+    const int64_t at_a_time = row_threads(lanes) / lanes, most = std::min<int64_t>(most_groups(lanes), 1024);
     const auto groups_of = [&](int64_t n) { return std::max<int64_t>(1, (n + at_a_time - 1) / at_a_time); };
     NormPlan p{0, 1, rows_per_gate, 0, false};
     if (rows_per_gate == 0) {
-        p.grid = static_cast<unsigned>(std::min(kMost, groups_of(rows)));
+        p.grid = static_cast<unsigned>(std::min(most, groups_of(rows)));
         p.gate_rows = p.grid;
     } else if (rows_per_gate < 2 * at_a_time) {
         p.gate_by_lanes = true;
-        p.grid = static_cast<unsigned>(std::min(kMost, groups_of(rows / rows_per_gate)));
+        p.grid = static_cast<unsigned>(std::min(most, groups_of(rows / rows_per_gate)));
     } else {
         const int64_t groups = std::max<int64_t>(1, rows / rows_per_gate);
-        const int64_t wanted = std::min((2 * kMost + groups - 1) / groups, groups_of(rows_per_gate));
+        const int64_t wanted = groups >= most / 2 ? 1 : std::min((most + groups - 1) / groups, groups_of(rows_per_gate));
         p.piece_rows = groups_of((rows_per_gate + wanted - 1) / wanted) * at_a_time;
         p.pieces = (rows_per_gate + p.piece_rows - 1) / p.piece_rows;
-        p.grid = static_cast<unsigned>(std::min(kMost, groups * p.pieces));
+        p.grid = static_cast<unsigned>(std::min(most, groups * p.pieces));
         p.gate_rows = p.pieces > 1 ? groups * p.pieces : 0;
     }
     return p;

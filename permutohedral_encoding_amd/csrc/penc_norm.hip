@@ -8,8 +8,9 @@
 //     d = dp w_post, df = r_f (d - mean d - f~ mean(d f~))                                     (the "mean d" for "layer" alone)
 //     sums over rows: dgate = dY p, dw_post = dp f~, db_post = dp, dw_pre = dn y~, db_pre = dn
 //
-// One pass over the rows in either direction: a row stays in the registers of its lanes, 8 or 16 channels each, from its first load to its last
-// store, and the means go through the lanes (and, from 1025 channels on, through the LDS).  Bound by memory.
+// One pass over the rows in either direction, bound by memory: a row stays in the registers of its lanes, 8 channels each, from its first load to its
+// last store.  The means go through the lanes (and, from 513 channels on, through the LDS), each wait for them serving all sums that are known by
+// then: two on the way there, three back (rms; a mean has one more, before the squares around it).  The next row is loaded while a row is worked on.
 //
 // The sums over rows stay in registers while a workgroup walks over its rows; each workgroup leaves one row of partial sums, added up in a
 // fixed order by sum_partials_kernel.  No atomics: results are the same in every run.
@@ -35,15 +36,14 @@ __device__ __forceinline__ float across_halves(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-
-// The lanes of a workgroup, and the sum over those of a row.
+// The lanes of a workgroup, and sums over those of a row, the same in each of them.
 template <int kLanes>
 struct Row {
-    static constexpr int kThreads = kLanes > 256 ? kLanes : 256;
-    static constexpr int kRows = kThreads / kLanes;           // at a time
+    static constexpr int kThreads = row_threads(kLanes);
+    static constexpr int kRows = kThreads / kLanes;               // at a time
     static constexpr int kWaves = kLanes > 64 ? kLanes / 64 : 1;  // of one row
 
-    float2* exchange;  // [2][kWaves]: a reduction may begin while slow waves still read the one before it
+    float2* exchange;  // [2][kWaves]: a sum may begin while slow waves still read the one before it
     int turn = 0;
 
     __device__ __forceinline__ static float in_wave(float v) {
@@ -74,329 +74,357 @@ struct Row {
     }
 };
 
-template <int kVectors>
-struct Values {
-    float v[kVectors][kChunk];
-};
+using Values = float[kChunk];
 
-// What a lane has of a row: kVectors times 8 channels, kLanes chunks apart.
-template <class E, int kLanes, int kVectors>
+#define PENC_EACH _Pragma("unroll") for (int i = 0; i < kChunk; ++i)
+
+// The eight channels that a lane has of a row.  Loads have no conditions, so that they can be under way while something else is done: a lane
+// that would read behind the row reads its last eight channels, and `bring` moves those it has to the front.  kNarrow: rows of fewer than eight.
+template <class E, bool kNarrow>
 struct Place {
-    int channels, first;
+    int channels, first, valid;
     float per_channel;
-    __device__ __forceinline__ Place(int channels_, int lane) : channels(channels_), first(lane * kChunk), per_channel(1.0f / channels_) {}
-    __device__ __forceinline__ int channel(int j) const { return first + j * kLanes * kChunk; }
-    __device__ __forceinline__ int valid(int j) const { return min(channels - channel(j), kChunk); }
 
-    __device__ __forceinline__ void load(const E* row, Values<kVectors>& x) const {
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j) load_chunk(row + channel(j), valid(j), x.v[j]);
+    template <class T>
+    struct Fetched {
+        T __attribute__((ext_vector_type(kChunk))) v;
+    };
+    struct FetchedKept {
+        uint2 q;
+        uint32_t exponent;
+    };
+
+    __device__ __forceinline__ Place(int channels_, int lane)
+        : channels(channels_), first(lane * kChunk), valid(max(0, min(channels_ - lane * kChunk, kChunk))), per_channel(1.0f / channels_) {}
+
+    template <class T>
+    __device__ __forceinline__ Fetched<T> fetch(const T* __restrict__ row) const {
+        Fetched<T> f;
+        if constexpr (kNarrow) {
+            PENC_EACH f.v[i] = i < valid ? row[i] : static_cast<T>(0.0f);
+        } else {
+            f.v = *reinterpret_cast<const chunk_t<T>*>(row + min(first, channels - kChunk));
+        }
+        return f;
     }
-    __device__ __forceinline__ void load(const KeptArray& kept, int64_t row, Values<kVectors>& x) const {
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j) kept.load(row, channel(j), valid(j), x.v[j]);
+    __device__ __forceinline__ FetchedKept fetch(const KeptArray& kept, int64_t row) const {
+        const int c = min(first, static_cast<int>(kept.pitch) - kChunk);
+        return {*reinterpret_cast<const uint2*>(kept.values + row * kept.pitch + c), kept.exponents[row * kept.blocks + c / kKeptBlock]};
     }
-    __device__ __forceinline__ void keep(const KeptArray& kept, int64_t row, const Values<kVectors>& x) const {
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j) kept.store(row, channel(j), x.v[j]);
+    template <class T>
+    __device__ __forceinline__ void bring(const Fetched<T>& f, Values& x) const {
+        const float8 v = __builtin_convertvector(f.v, float8);
+        PENC_EACH x[i] = v[i];
+        if (kNarrow || (channels & 7) == 0) {
+            if (!kNarrow && valid == 0) PENC_EACH x[i] = 0.0f;
+            return;
+        }
+        // the row's last lane: forward by 8 - valid
+        Values moved;
+        const int by = kChunk - (channels & 7);
+        PENC_EACH moved[i] = x[i];
+        if (by & 4) PENC_EACH moved[i] = i + 4 < kChunk ? moved[i + 4 < kChunk ? i + 4 : 0] : 0.0f;
+        if (by & 2) PENC_EACH moved[i] = i + 2 < kChunk ? moved[i + 2 < kChunk ? i + 2 : 0] : 0.0f;
+        if (by & 1) PENC_EACH moved[i] = i + 1 < kChunk ? moved[i + 1 < kChunk ? i + 1 : 0] : 0.0f;
+        PENC_EACH x[i] = valid == kChunk ? x[i] : valid == 0 ? 0.0f : moved[i];
     }
-    __device__ __forceinline__ void store(E* row, const Values<kVectors>& x) const {
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j)
-            if (valid(j) > 0) store_chunk(row + channel(j), valid(j), x.v[j]);
+    __device__ __forceinline__ void bring(const FetchedKept& f, Values& x) const {
+        restore(valid > 0 ? f.q : make_uint2(0, 0), valid > 0 ? f.exponent : 0, x);
     }
-    __device__ __forceinline__ void load(const void* param, bool fp32, float none, Values<kVectors>& x, int64_t at = 0) const {
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j) {
-            if (param != nullptr) {
-                load_param<E>(param, fp32, at + channel(j), valid(j), x.v[j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) x.v[j][i] = none;
-            }
+    template <class T>
+    __device__ __forceinline__ void store(T* __restrict__ row, const Values& x) const {
+        if (valid > 0) store_part(row + first, x);
+    }
+    // (of a whole chunk at once, of a part in fours, twos and ones)
+    template <class T>
+    __device__ __forceinline__ void store_part(T* __restrict__ p, const Values& x) const {
+        float8 v;
+        PENC_EACH v[i] = x[i];
+        const auto y = __builtin_convertvector(v, T __attribute__((ext_vector_type(kChunk))));
+        if (valid == kChunk) {
+            *reinterpret_cast<chunk_t<T>*>(p) = y;
+            return;
+        }
+        using Four = T __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        using Two = T __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+        const int n = channels & 7;
+        if (n & 4) *reinterpret_cast<Four*>(p) = __builtin_shufflevector(y, y, 0, 1, 2, 3);
+        if (n & 2) {
+            if (n & 4) *reinterpret_cast<Two*>(p + 4) = __builtin_shufflevector(y, y, 4, 5);
+            else *reinterpret_cast<Two*>(p) = __builtin_shufflevector(y, y, 0, 1);
+        }
+        if (n & 1) {
+            if (n == 1) p[0] = y[0];
+            else if (n == 3) p[2] = y[2];
+            else if (n == 5) p[4] = y[4];
+            else p[6] = y[6];
         }
     }
-    // v becomes v~; returns r.  Channels behind the row's end stay zero.
-    __device__ __forceinline__ float normalise(Values<kVectors>& x, bool layer, float eps, Row<kLanes>& row) const {
-        if (layer) {
-            float s = 0.0f;
-#pragma unroll
-            for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) s += x.v[j][i];
-            const float mean = row.sum(s) * per_channel;
-#pragma unroll
-            for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) x.v[j][i] = i < valid(j) ? x.v[j][i] - mean : 0.0f;
-        }
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) s = __builtin_fmaf(x.v[j][i], x.v[j][i], s);
-        const float r = rsqrtf(row.sum(s) * per_channel + eps);
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) x.v[j][i] *= r;
-        return r;
+    // a parameter, or `none` for each channel
+    __device__ __forceinline__ void param(const void* p, bool fp32, float none, Values& x, int64_t at = 0) const {
+        if (p == nullptr) PENC_EACH x[i] = none;
+        else if (fp32) bring(fetch(static_cast<const float*>(p) + at), x);
+        else bring(fetch(static_cast<const E*>(p) + at), x);
     }
-    // d becomes r (d - mean d - v~ mean(d v~))
-    __device__ __forceinline__ void through_norm(Values<kVectors>& d, const Values<kVectors>& normed, float r, bool layer, Row<kLanes>& row) const {
-        float s = 0.0f, t = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) {
-                s += d.v[j][i];
-                t = __builtin_fmaf(d.v[j][i], normed.v[j][i], t);
-            }
-        const float2 sums = row.sums(s, t);
-        const float mean = layer ? sums.x * per_channel : 0.0f, along = sums.y * per_channel;
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) d.v[j][i] = r * (d.v[j][i] - mean - normed.v[j][i] * along);
+    // (a difference to the mean is zero behind the row's end)
+    __device__ __forceinline__ void centre(Values& x, float mean) const {
+        PENC_EACH x[i] = i < valid ? x[i] - mean : 0.0f;
     }
 };
 
-// The parameters of a lane's channels, loaded again for every row where a lane has more than 8 of them: they come from the caches, and
-// their registers would cost waves.
-template <class E, int kLanes, int kVectors>
-struct Params {
-    Values<kVectors> gate, post_weight, post_bias, pre_weight, pre_bias;
+__device__ __forceinline__ float total(const Values& x) {
+    float s = 0.0f;
+    PENC_EACH s += x[i];
+    return s;
+}
+__device__ __forceinline__ float dot(const Values& x, const Values& y) {
+    float s = 0.0f;
+    PENC_EACH s = __builtin_fmaf(x[i], y[i], s);
+    return s;
+}
 
-    __device__ __forceinline__ void load_shared(const NormArgs& a, const Place<E, kLanes, kVectors>& at) {
-        at.load(a.post_weight, a.param_fp32, 1.0f, post_weight);
-        at.load(a.post_bias, a.param_fp32, 0.0f, post_bias);
-        at.load(a.pre_weight, a.param_fp32, 1.0f, pre_weight);
-        at.load(a.pre_bias, a.param_fp32, 0.0f, pre_bias);
-    }
-    __device__ __forceinline__ void load_gate(const NormArgs& a, const Place<E, kLanes, kVectors>& at, int64_t group) {
-        at.load(a.gate, a.gate_fp32, 1.0f, gate, group * a.channels);
-    }
-};
+// v becomes v~; returns r.
+template <bool kFull, class P, class R>
+__device__ __forceinline__ float normalise(Values& x, const NormArgs& a, const P& at, R& row) {
+    if (kFull && a.layer) at.centre(x, row.sum(total(x)) * at.per_channel);
+    const float r = rsqrtf(row.sum(dot(x, x)) * at.per_channel + a.eps);
+    PENC_EACH x[i] *= r;
+    return r;
+}
 
-template <class E, int kLanes, int kVectors>
-__global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_kernel(NormArgs a, E* __restrict__ y_out, E* __restrict__ n_out) {
-    using R = Row<kLanes>;
-    __shared__ float2 exchange[2 * R::kWaves];
-    R across{exchange};
-    const Place<E, kLanes, kVectors> at(a.channels, threadIdx.x % kLanes);
-    Params<E, kLanes, kVectors> p;
-    if constexpr (kVectors == 1) {
-        p.load_shared(a, at);
-        if (a.rows_per_gate == 0) p.load_gate(a, at, 0);
-    }
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * R::kRows + threadIdx.x / kLanes; row < a.rows;
-         row += static_cast<int64_t>(gridDim.x) * R::kRows) {
-        Values<kVectors> x, f;
-        at.load(static_cast<const E*>(a.x) + row * a.x_stride, x);
-        if (a.has_branch) at.load(static_cast<const E*>(a.branch) + row * a.branch_stride, f);
-        if constexpr (kVectors > 1) p.load_shared(a, at);
-        if (a.rows_per_gate != 0) p.load_gate(a, at, group_of(row, a.rows_per_gate));
-        else if constexpr (kVectors > 1) p.load_gate(a, at, 0);
-        if (a.kept_x.values != nullptr) at.keep(a.kept_x, row, x);
-        if (a.kept_branch.values != nullptr) at.keep(a.kept_branch, row, f);
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) x.v[j][i] *= a.scale;
-        if (a.has_branch) {
-            if (a.post_norm) {
-                at.normalise(f, a.layer, a.eps, across);
-#pragma unroll
-                for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                    for (int i = 0; i < kChunk; ++i) f.v[j][i] = __builtin_fmaf(f.v[j][i], p.post_weight.v[j][i], p.post_bias.v[j][i]);
-            }
-#pragma unroll
-            for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) x.v[j][i] = __builtin_fmaf(p.gate.v[j][i], f.v[j][i], x.v[j][i]);
-        }
-        if (y_out != nullptr) at.store(y_out + row * a.channels, x);
-        if (a.pre_norm) {
-            // (of y before it is rounded)
-            at.normalise(x, a.layer, a.eps, across);
-#pragma unroll
-            for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) x.v[j][i] = __builtin_fmaf(x.v[j][i], p.pre_weight.v[j][i], p.pre_bias.v[j][i]);
-            at.store(n_out + row * a.channels, x);
-        }
+// The rows that the lanes of a row go through: `run` consecutive ones, then the next run `stride` runs on, up to `end`; body(row, the first of
+// its run, the last of its run, fetched).  `fetch` is called for a row while the one before it is worked on.
+template <class Fetch, class Body>
+__device__ __forceinline__ void walk(int64_t row, int64_t end, int64_t run, int64_t stride, Fetch&& fetch, Body&& body) {
+    if (row >= end) return;
+    auto now = fetch(row);
+    for (int64_t k = 0; row < end;) {
+        const bool ends = k + 1 == run;
+        const int64_t next = ends ? row + 1 + (stride - 1) * run : row + 1;
+        auto ahead = fetch(min(next, end - 1));
+        body(row, k == 0, ends, now);
+        now = ahead;
+        row = next;
+        k = ends ? 0 : k + 1;
     }
 }
 
-// The sums of one of a lane's accumulators over the rows that a workgroup has at a time: `store` gets them from the lanes of the first.
-template <int kLanes, int kVectors, class F>
-__device__ __forceinline__ void write_sum(const Values<kVectors>& sum, float (*__restrict__ lds)[kChunk], int channels, F&& store) {
-    constexpr int kRows = Row<kLanes>::kRows;
-    const int lane = threadIdx.x % kLanes;
-#pragma unroll
-    for (int j = 0; j < kVectors; ++j) {
-        float total[kChunk];
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i) total[i] = sum.v[j][i];
-        if constexpr (kRows > 1) {
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) lds[threadIdx.x][i] = total[i];
-            __syncthreads();
-            if (threadIdx.x < kLanes) {
-#pragma unroll 1
-                for (int r = 1; r < kRows; ++r)
-#pragma unroll
-                    for (int i = 0; i < kChunk; ++i) total[i] += lds[r * kLanes + lane][i];
-            }
-            __syncthreads();
-        }
-        const int c = (lane + j * kLanes) * kChunk;
-        if (threadIdx.x < kLanes && c < channels) store(c, min(channels - c, kChunk), total);
+// kFull: any kind of norm; else "rms" without biases, whose sums and parameters need 32 registers less.
+template <class E, int kLanes, bool kNarrow, bool kFull>
+__global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_kernel(NormArgs a, E* __restrict__ y_out, E* __restrict__ n_out) {
+    using R = Row<kLanes>;
+    using P = Place<E, kNarrow>;
+    __shared__ float2 exchange[2 * R::kWaves];
+    R across{exchange};
+    const P at(a.channels, threadIdx.x % kLanes);
+    Values gate, post_weight, post_bias, pre_weight, pre_bias;
+    at.param(a.post_weight, a.param_fp32, 1.0f, post_weight);
+    at.param(a.pre_weight, a.param_fp32, 1.0f, pre_weight);
+    if constexpr (kFull) {
+        at.param(a.post_bias, a.param_fp32, 0.0f, post_bias);
+        at.param(a.pre_bias, a.param_fp32, 0.0f, pre_bias);
     }
+    if (a.rows_per_gate == 0) at.param(a.gate, a.gate_fp32, 1.0f, gate);
+    struct Fetched {
+        typename P::template Fetched<E> x, f;
+    };
+    const auto fetch = [&](int64_t row) {
+        Fetched r;
+        r.x = at.fetch(static_cast<const E*>(a.x) + row * a.x_stride);
+        if (a.has_branch) r.f = at.fetch(static_cast<const E*>(a.branch) + row * a.branch_stride);
+        return r;
+    };
+    walk(static_cast<int64_t>(blockIdx.x) * R::kRows + threadIdx.x / kLanes, a.rows, 1, static_cast<int64_t>(gridDim.x) * R::kRows, fetch,
+         [&](int64_t row, bool, bool, const Fetched& fetched) {
+             Values x, f;
+             if (a.rows_per_gate != 0) at.param(a.gate, a.gate_fp32, 1.0f, gate, group_of(row, a.rows_per_gate) * a.channels);
+             at.bring(fetched.x, x);
+             if (a.kept_x.values != nullptr) a.kept_x.store(row, at.first, x);
+             PENC_EACH x[i] *= a.scale;
+             if (a.has_branch) {
+                 at.bring(fetched.f, f);
+                 if (a.kept_branch.values != nullptr) a.kept_branch.store(row, at.first, f);
+                 if (a.post_norm) {
+                     normalise<kFull>(f, a, at, across);
+                     PENC_EACH f[i] = kFull ? __builtin_fmaf(f[i], post_weight[i], post_bias[i]) : f[i] * post_weight[i];
+                 }
+                 PENC_EACH x[i] = __builtin_fmaf(gate[i], f[i], x[i]);
+             }
+             if (y_out != nullptr) at.store(y_out + row * a.channels, x);
+             if (a.pre_norm) {
+                 // (of y before it is rounded)
+                 normalise<kFull>(x, a, at, across);
+                 PENC_EACH x[i] = kFull ? __builtin_fmaf(x[i], pre_weight[i], pre_bias[i]) : x[i] * pre_weight[i];
+                 at.store(n_out + row * a.channels, x);
+             }
+         });
+}
+
+// The sums of one of a lane's accumulators over the rows that a workgroup has at a time: `store` gets them in the lanes of the first.
+template <int kLanes, class F>
+__device__ __forceinline__ void write_sum(const Values& sum, float (*__restrict__ lds)[kChunk], F&& store) {
+    constexpr int kRows = Row<kLanes>::kRows;
+    Values all;
+    PENC_EACH all[i] = sum[i];
+    if constexpr (kRows > 1) {
+        PENC_EACH lds[threadIdx.x][i] = all[i];
+        __syncthreads();
+        if (threadIdx.x < kLanes) {
+#pragma unroll 1
+            for (int r = 1; r < kRows; ++r) PENC_EACH all[i] += lds[r * kLanes + threadIdx.x][i];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x < kLanes) store(all);
 }
 
 // kKept: x and the branch are read from their checkpoints.
 //
 // Gates of groups of rows: with few rows in a group (a.gate_by_lanes) the lanes of a row take whole groups and write their sums themselves; else a
 // workgroup takes a piece of a group, `pieces` of them to a group, and leaves a row of partial sums.  One gate for all rows is one more sum over rows.
-template <class E, int kLanes, int kVectors, bool kKept>
+template <class E, int kLanes, bool kNarrow, bool kFull, bool kKept>
 __global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_backward_kernel(NormArgs a, NormGrads g) {
     using R = Row<kLanes>;
+    using P = Place<E, kNarrow>;
     __shared__ float2 exchange[2 * R::kWaves];
     __shared__ float lds[R::kRows > 1 ? R::kThreads : 1][kChunk];
     R across{exchange};
-    const Place<E, kLanes, kVectors> at(a.channels, threadIdx.x % kLanes);
-    Params<E, kLanes, kVectors> p;
-    if constexpr (kVectors == 1) {
-        p.load_shared(a, at);
-        p.load_gate(a, at, 0);
+    const P at(a.channels, threadIdx.x % kLanes);
+    Values gate, post_weight, post_bias, pre_weight, pre_bias;
+    at.param(a.post_weight, a.param_fp32, 1.0f, post_weight);
+    at.param(a.pre_weight, a.param_fp32, 1.0f, pre_weight);
+    if constexpr (kFull) {
+        at.param(a.post_bias, a.param_fp32, 0.0f, post_bias);
+        at.param(a.pre_bias, a.param_fp32, 0.0f, pre_bias);
     }
-    Values<kVectors> d_gate{}, d_post_weight{}, d_post_bias{}, d_pre_weight{}, d_pre_bias{};
+    at.param(a.gate, a.gate_fp32, 1.0f, gate);
+    Values d_gate{}, d_post_weight{}, d_post_bias{}, d_pre_weight{}, d_pre_bias{};
 
-    const auto one_row = [&](int64_t row, int64_t group, bool new_gate) {
-        Values<kVectors> x, f, dn, dy;
+    using Input = std::conditional_t<kKept, typename P::FetchedKept, typename P::template Fetched<E>>;
+    struct Fetched {
+        Input x, f;
+        typename P::template Fetched<E> dy, dn;
+    };
+    const auto fetch = [&](int64_t row) {
+        Fetched r;
         if constexpr (kKept) {
-            at.load(a.kept_x, row, x);
-            if (a.has_branch) at.load(a.kept_branch, row, f);
+            r.x = at.fetch(a.kept_x, row);
+            if (a.has_branch) r.f = at.fetch(a.kept_branch, row);
         } else {
-            at.load(static_cast<const E*>(a.x) + row * a.x_stride, x);
-            if (a.has_branch) at.load(static_cast<const E*>(a.branch) + row * a.branch_stride, f);
+            r.x = at.fetch(static_cast<const E*>(a.x) + row * a.x_stride);
+            if (a.has_branch) r.f = at.fetch(static_cast<const E*>(a.branch) + row * a.branch_stride);
         }
-        if (g.y != nullptr) at.load(static_cast<const E*>(g.y) + row * g.y_stride, dy);
-        else at.load(nullptr, false, 0.0f, dy);
-        if (g.n != nullptr) at.load(static_cast<const E*>(g.n) + row * g.n_stride, dn);
-        if constexpr (kVectors > 1) p.load_shared(a, at);
-        if (kVectors > 1 || new_gate) p.load_gate(a, at, group);
+        if (g.y != nullptr) r.dy = at.fetch(static_cast<const E*>(g.y) + row * g.y_stride);
+        if (g.n != nullptr) r.dn = at.fetch(static_cast<const E*>(g.n) + row * g.n_stride);
+        return r;
+    };
+    const auto one_row = [&](int64_t row, const Fetched& fetched) {
+        Values y, f, inner, dy;
         float r_f = 1.0f;
-        Values<kVectors> inner;
+        at.bring(fetched.x, y);
+        PENC_EACH y[i] *= a.scale;
         if (a.has_branch) {
-            if (a.post_norm) r_f = at.normalise(f, a.layer, a.eps, across);
-#pragma unroll
-            for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) {
-                    inner.v[j][i] = a.post_norm ? __builtin_fmaf(f.v[j][i], p.post_weight.v[j][i], p.post_bias.v[j][i]) : f.v[j][i];
-                    x.v[j][i] = __builtin_fmaf(p.gate.v[j][i], inner.v[j][i], a.scale * x.v[j][i]);
-                }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) x.v[j][i] *= a.scale;
+            at.bring(fetched.f, f);
+            if (a.post_norm) {
+                r_f = normalise<kFull>(f, a, at, across);
+                PENC_EACH inner[i] = kFull ? __builtin_fmaf(f[i], post_weight[i], post_bias[i]) : f[i] * post_weight[i];
+            } else {
+                PENC_EACH inner[i] = f[i];
+            }
+            PENC_EACH y[i] = __builtin_fmaf(gate[i], inner[i], y[i]);
         }
+        if (g.y != nullptr) at.bring(fetched.dy, dy);
+        else PENC_EACH dy[i] = 0.0f;
         if (g.n != nullptr) {
-            const float r_y = at.normalise(x, a.layer, a.eps, across);
-#pragma unroll
-            for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) {
-                    d_pre_weight.v[j][i] = __builtin_fmaf(dn.v[j][i], x.v[j][i], d_pre_weight.v[j][i]);
-                    d_pre_bias.v[j][i] += dn.v[j][i];
-                    dn.v[j][i] *= p.pre_weight.v[j][i];
-                }
-            at.through_norm(dn, x, r_y, a.layer, across);
-#pragma unroll
-            for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) dy.v[j][i] += dn.v[j][i];
+            Values dn, d;
+            at.bring(fetched.dn, dn);
+            PENC_EACH d[i] = dn[i] * pre_weight[i];
+            float mean = 0.0f;
+            if (kFull && a.layer) {
+                const float2 s = across.sums(total(y), total(d));
+                at.centre(y, s.x * at.per_channel);
+                mean = s.y * at.per_channel;
+            }
+            const float2 s = across.sums(dot(y, y), dot(d, y));
+            const float r_y = rsqrtf(s.x * at.per_channel + a.eps), along = s.y * at.per_channel * r_y;
+            PENC_EACH {
+                y[i] *= r_y;
+                d_pre_weight[i] = __builtin_fmaf(dn[i], y[i], d_pre_weight[i]);
+                if (kFull) d_pre_bias[i] += dn[i];
+                dy[i] = __builtin_fmaf(r_y, d[i] - mean - y[i] * along, dy[i]);
+            }
         }
         if (g.x != nullptr) {
-#pragma unroll
-            for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) x.v[j][i] = a.scale * dy.v[j][i];
-            at.store(static_cast<E*>(g.x) + row * a.channels, x);
+            Values dx;
+            PENC_EACH dx[i] = a.scale * dy[i];
+            at.store(static_cast<E*>(g.x) + row * a.channels, dx);
         }
         if (!a.has_branch) return;
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) {
-                d_gate.v[j][i] = __builtin_fmaf(dy.v[j][i], inner.v[j][i], d_gate.v[j][i]);
-                dy.v[j][i] *= p.gate.v[j][i];
-            }
+        PENC_EACH {
+            d_gate[i] = __builtin_fmaf(dy[i], inner[i], d_gate[i]);
+            dy[i] *= gate[i];
+        }
         if (a.post_norm) {
-#pragma unroll
-            for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) {
-                    d_post_weight.v[j][i] = __builtin_fmaf(dy.v[j][i], f.v[j][i], d_post_weight.v[j][i]);
-                    d_post_bias.v[j][i] += dy.v[j][i];
-                    dy.v[j][i] *= p.post_weight.v[j][i];
-                }
-            if (g.branch != nullptr) at.through_norm(dy, f, r_f, a.layer, across);
+            PENC_EACH {
+                d_post_weight[i] = __builtin_fmaf(dy[i], f[i], d_post_weight[i]);
+                if (kFull) d_post_bias[i] += dy[i];
+                dy[i] *= post_weight[i];
+            }
+            if (g.branch != nullptr) {
+                const float2 s = across.sums(dot(dy, f), kFull ? total(dy) : 0.0f);
+                const float along = s.x * at.per_channel, mean = kFull && a.layer ? s.y * at.per_channel : 0.0f;
+                PENC_EACH dy[i] = r_f * (dy[i] - mean - f[i] * along);
+            }
         }
         if (g.branch != nullptr) at.store(static_cast<E*>(g.branch) + row * a.channels, dy);
     };
 
-    const auto store_gate = [&](int64_t group, int c, int valid, const float(&v)[kChunk]) {
-        if (a.gate_fp32) store_chunk(static_cast<float*>(g.gate) + group * a.channels + c, valid, v);
-        else store_chunk(static_cast<E*>(g.gate) + group * a.channels + c, valid, v);
+    const auto store_gate = [&](int64_t group, const Values& v) {
+        if (a.gate_fp32) at.store(static_cast<float*>(g.gate) + group * a.channels, v);
+        else at.store(static_cast<E*>(g.gate) + group * a.channels, v);
     };
-    const auto leave = [&](float* sums, int64_t at_row, const Values<kVectors>& v) {
-        if (sums != nullptr)
-            write_sum<kLanes, kVectors>(v, lds, a.channels,
-                                        [&](int c, int valid, const float(&t)[kChunk]) { store_chunk(sums + at_row * a.channels + c, valid, t); });
+    const auto leave = [&](float* sums, int64_t at_row, const Values& v) {
+        if (sums != nullptr) write_sum<kLanes>(v, lds, [&](const Values& t) { at.store(sums + at_row * a.channels, t); });
     };
     const int sub = threadIdx.x / kLanes;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * R::kRows + sub, stride = static_cast<int64_t>(gridDim.x) * R::kRows;
     if (a.rows_per_gate == 0) {
-        for (int64_t row = static_cast<int64_t>(blockIdx.x) * R::kRows + sub; row < a.rows; row += static_cast<int64_t>(gridDim.x) * R::kRows)
-            one_row(row, 0, false);
+        walk(first, a.rows, 1, stride, fetch, [&](int64_t row, bool, bool, const Fetched& fetched) { one_row(row, fetched); });
     } else if (a.gate_by_lanes) {
-        const int64_t groups = a.rows / a.rows_per_gate;
-        for (int64_t group = static_cast<int64_t>(blockIdx.x) * R::kRows + sub; group < groups; group += static_cast<int64_t>(gridDim.x) * R::kRows) {
-            for (int64_t k = 0; k < a.rows_per_gate; ++k) one_row(group * a.rows_per_gate + k, group, k == 0);
-            if (g.gate != nullptr) {
-#pragma unroll
-                for (int j = 0; j < kVectors; ++j)
-                    if (at.valid(j) > 0) store_gate(group, at.channel(j), at.valid(j), d_gate.v[j]);
-            }
-            d_gate = Values<kVectors>{};
-        }
+        int64_t group = first;
+        walk(first * a.rows_per_gate, a.rows, a.rows_per_gate, stride, fetch, [&](int64_t row, bool begins, bool ends, const Fetched& fetched) {
+            if (begins) at.param(a.gate, a.gate_fp32, 1.0f, gate, group * a.channels);
+            one_row(row, fetched);
+            if (!ends) return;
+            if (g.gate != nullptr) store_gate(group, d_gate);
+            PENC_EACH d_gate[i] = 0.0f;
+            group += stride;
+        });
     } else {
         const int64_t units = a.rows / a.rows_per_gate * g.pieces;
         for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
             const int64_t group = unit / g.pieces, piece = unit % g.pieces;
-            const int64_t first = group * a.rows_per_gate + piece * g.piece_rows;
-            const int64_t last = min(first + g.piece_rows, (group + 1) * a.rows_per_gate);
-            p.load_gate(a, at, group);
-            for (int64_t row = first + sub; row < last; row += R::kRows) one_row(row, group, false);
+            const int64_t begin = group * a.rows_per_gate + piece * g.piece_rows;
+            at.param(a.gate, a.gate_fp32, 1.0f, gate, group * a.channels);
+            walk(begin + sub, min(begin + g.piece_rows, (group + 1) * a.rows_per_gate), 1, R::kRows, fetch,
+                 [&](int64_t row, bool, bool, const Fetched& fetched) { one_row(row, fetched); });
             if (g.gate != nullptr) {
-                if (g.pieces == 1)
-                    write_sum<kLanes, kVectors>(d_gate, lds, a.channels, [&](int c, int valid, const float(&v)[kChunk]) { store_gate(group, c, valid, v); });
-                else
-                    leave(g.gate_sums, unit, d_gate);
+                if (g.pieces == 1) write_sum<kLanes>(d_gate, lds, [&](const Values& v) { store_gate(group, v); });
+                else leave(g.gate_sums, unit, d_gate);
             }
-            d_gate = Values<kVectors>{};
+            PENC_EACH d_gate[i] = 0.0f;
         }
     }
     if (a.rows_per_gate == 0) leave(g.gate_sums, blockIdx.x, d_gate);
     leave(g.sums[0], blockIdx.x, d_post_weight);
-    leave(g.sums[1], blockIdx.x, d_post_bias);
     leave(g.sums[2], blockIdx.x, d_pre_weight);
-    leave(g.sums[3], blockIdx.x, d_pre_bias);
+    if constexpr (kFull) {
+        leave(g.sums[1], blockIdx.x, d_post_bias);
+        leave(g.sums[3], blockIdx.x, d_pre_bias);
+    }
 }
+
+#undef PENC_EACH
 
 // to[group][c] = the sum over `rows` rows of partial sums of a group, in a fixed order; 32 channels and 32 strands of rows to a workgroup.
 template <class E>
@@ -420,27 +448,35 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(SumPartials s) {
     else static_cast<E*>(sum.to)[group * s.channels + c] = static_cast<E>(total);
 }
 
+// "rms" without biases, also of gradients that nobody asked for
+bool is_full(const NormArgs& a, const NormGrads* g) {
+    return a.layer || a.post_bias != nullptr || a.pre_bias != nullptr || (g != nullptr && (g->sums[1] != nullptr || g->sums[3] != nullptr));
+}
+
 template <class E>
 int launch_norm(const NormArgs& a, void* y, void* n, hipStream_t stream) {
-    return with_row_shape(a.channels, [&](auto lanes, auto vectors) {
-        constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
-        const unsigned grid = static_cast<unsigned>(std::min<int64_t>((a.rows + Row<kLanes>::kRows - 1) / Row<kLanes>::kRows, 8192));
-        hipLaunchKernelGGL((norm_kernel<E, kLanes, kVectors>), dim3(grid), dim3(Row<kLanes>::kThreads), 0, stream, a, static_cast<E*>(y),
-                           static_cast<E*>(n));
+    return with_row_shape(a.channels, [&](auto lanes, auto narrow) {
+        constexpr int kLanes = decltype(lanes)::value;
+        constexpr bool kNarrow = decltype(narrow)::value;
+        const dim3 grid(static_cast<unsigned>(std::min<int64_t>((a.rows + Row<kLanes>::kRows - 1) / Row<kLanes>::kRows, most_groups(kLanes)))), threads(Row<kLanes>::kThreads);
+        if (is_full(a, nullptr)) hipLaunchKernelGGL((norm_kernel<E, kLanes, kNarrow, true>), grid, threads, 0, stream, a, static_cast<E*>(y), static_cast<E*>(n));
+        else hipLaunchKernelGGL((norm_kernel<E, kLanes, kNarrow, false>), grid, threads, 0, stream, a, static_cast<E*>(y), static_cast<E*>(n));
         return launched();
     });
 }
 
 template <class E>
 int launch_norm_backward(const NormArgs& a, const NormGrads& g, unsigned grid, hipStream_t stream) {
-    return with_row_shape(a.channels, [&](auto lanes, auto vectors) {
-        constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
-        const dim3 threads(Row<kLanes>::kThreads);
-        if (a.kept_x.values != nullptr)
-            hipLaunchKernelGGL((norm_backward_kernel<E, kLanes, kVectors, true>), dim3(grid), threads, 0, stream, a, g);
-        else
-            hipLaunchKernelGGL((norm_backward_kernel<E, kLanes, kVectors, false>), dim3(grid), threads, 0, stream, a, g);
-        return launched();
+    return with_row_shape(a.channels, [&](auto lanes, auto narrow) {
+        constexpr int kLanes = decltype(lanes)::value;
+        constexpr bool kNarrow = decltype(narrow)::value;
+        const auto launch = [&](auto full, auto kept) {
+            hipLaunchKernelGGL((norm_backward_kernel<E, kLanes, kNarrow, decltype(full)::value, decltype(kept)::value>), dim3(grid), dim3(Row<kLanes>::kThreads), 0,
+                               stream, a, g);
+            return launched();
+        };
+        const auto with_kept = [&](auto full) { return a.kept_x.values != nullptr ? launch(full, std::true_type{}) : launch(full, std::false_type{}); };
+        return is_full(a, &g) ? with_kept(std::true_type{}) : with_kept(std::false_type{});
     });
 }
 

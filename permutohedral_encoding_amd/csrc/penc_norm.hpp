@@ -44,30 +44,35 @@ __device__ __forceinline__ int64_t group_of(int64_t row, int64_t rows_per_gate) 
     return row / rows_per_gate;
 }
 
-// Lanes to a row and vectors of 8 channels to a lane.  A wave or less per row up to 1024 channels: nothing goes through the LDS.  From there on a
-// workgroup per row, wide before deep, so that a lane's sums over the rows (5 x 8 registers a vector) leave room for waves.
+// Lanes to a row, 8 channels each, and whether it has fewer than 8 channels.  A wave or less up to 512 channels: nothing goes through the LDS; from there on
+// a workgroup.
 template <class F>
 int with_row_shape(int channels, F&& f) {
-    const auto shape = [&](auto lanes, auto vectors) { return f(lanes, vectors); };
-#define PENC_SHAPE(most, lanes, vectors) \
-    if (channels <= most) return shape(std::integral_constant<int, lanes>{}, std::integral_constant<int, vectors>{})
-    PENC_SHAPE(32, 4, 1);
-    PENC_SHAPE(64, 8, 1);
-    PENC_SHAPE(128, 16, 1);
-    PENC_SHAPE(256, 32, 1);
-    PENC_SHAPE(512, 64, 1);
-    PENC_SHAPE(1024, 64, 2);
-    PENC_SHAPE(2048, 256, 1);
-    PENC_SHAPE(4096, 512, 1);
-    PENC_SHAPE(PENC_MAX_NORM_CHANNELS, 512, 2);
+    if (channels < kChunk) return f(std::integral_constant<int, 4>{}, std::true_type{});
+#define PENC_SHAPE(lanes) \
+    if (channels <= lanes * kChunk) return f(std::integral_constant<int, lanes>{}, std::false_type{})
+    PENC_SHAPE(4);
+    PENC_SHAPE(8);
+    PENC_SHAPE(16);
+    PENC_SHAPE(32);
+    PENC_SHAPE(64);
+    PENC_SHAPE(128);
+    PENC_SHAPE(256);
+    PENC_SHAPE(512);
+    PENC_SHAPE(1024);
 #undef PENC_SHAPE
     return PENC_ERR_BAD_LAYER_SIZE;
 }
+static_assert(PENC_MAX_NORM_CHANNELS == 1024 * kChunk, "the widest row");
 
-inline int rows_at_a_time(int channels) {
-    int rows = 1;
-    with_row_shape(channels, [&](auto lanes, auto) { return rows = decltype(lanes)::value < 256 ? 256 / decltype(lanes)::value : 1; });
-    return rows;
+__host__ __device__ constexpr int row_threads(int lanes) { return lanes > 64 ? lanes : 256; }
+// Workgroups that the card holds at a time, with 16 waves to each of its 256 compute units.
+inline int64_t most_groups(int lanes) { return 256 * 16 * 64 / row_threads(lanes); }
+
+inline int lanes_of_row(int channels) {
+    int n = 0;
+    with_row_shape(channels, [&](auto lanes, auto) { return n = decltype(lanes)::value; });
+    return n;
 }
 
 struct NormLaunches {
