@@ -136,8 +136,8 @@ __device__ __forceinline__ Kept keep(const float (&x)[kChunk]) {
 
 // (255 gives an infinite step, and 0 times that the NaN)
 __device__ __forceinline__ float kept_step(uint32_t exponent) { return __uint_as_float(exponent << 23); }
-__device__ __forceinline__ void restore(uint2 q, uint32_t exponent, float (&v)[kChunk]) {
-    const float step = kept_step(exponent);
+__device__ __forceinline__ void restore(uint2 q, uint32_t exponent, float (&v)[kChunk], float scale = 1.0f) {
+    const float step = kept_step(exponent) * scale;
 #pragma unroll
     for (int i = 0; i < kChunk; ++i) v[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? q.x : q.y) >> 8 * (i % 4))) * step;
 }

@@ -79,15 +79,16 @@ using Values = float[kChunk];
 #define PENC_EACH _Pragma("unroll") for (int i = 0; i < kChunk; ++i)
 
 // The eight channels that a lane has of a row.  Loads have no conditions, so that they can be under way while something else is done: a lane
-// that would read behind the row reads its last eight channels, and `bring` moves those it has to the front.  kNarrow: rows of fewer than eight.
-template <class E, bool kNarrow>
+// that would read behind the row reads its last eight channels, and `bring` moves those it has to the front.
+template <class E, int kEnd>
 struct Place {
+    static constexpr bool kNarrow = kEnd == kNarrowRow, kWhole = kEnd == kWholeChunks;
     int channels, first, valid;
     float per_channel;
 
     template <class T>
     struct Fetched {
-        T __attribute__((ext_vector_type(kChunk))) v;
+        uint32_t __attribute__((ext_vector_type(kChunk * sizeof(T) / 4))) w;
     };
     struct FetchedKept {
         uint2 q;
@@ -99,37 +100,57 @@ struct Place {
 
     template <class T>
     __device__ __forceinline__ Fetched<T> fetch(const T* __restrict__ row) const {
-        Fetched<T> f;
+        using Words = decltype(Fetched<T>::w);
         if constexpr (kNarrow) {
-            PENC_EACH f.v[i] = i < valid ? row[i] : static_cast<T>(0.0f);
+            T __attribute__((ext_vector_type(kChunk))) v;
+            PENC_EACH v[i] = i < valid ? row[i] : static_cast<T>(0.0f);
+            return {__builtin_bit_cast(Words, v)};
         } else {
-            f.v = *reinterpret_cast<const chunk_t<T>*>(row + min(first, channels - kChunk));
+            using Unaligned = uint32_t __attribute__((ext_vector_type(kChunk * sizeof(T) / 4), aligned(sizeof(T))));
+            return {*reinterpret_cast<const Unaligned*>(row + min(first, channels - kChunk))};
         }
-        return f;
     }
     __device__ __forceinline__ FetchedKept fetch(const KeptArray& kept, int64_t row) const {
         const int c = min(first, static_cast<int>(kept.pitch) - kChunk);
         return {*reinterpret_cast<const uint2*>(kept.values + row * kept.pitch + c), kept.exponents[row * kept.blocks + c / kKeptBlock]};
     }
+    // (with masks in place of conditions: of those the compiler makes a branch for each channel)
     template <class T>
     __device__ __forceinline__ void bring(const Fetched<T>& f, Values& x) const {
-        const float8 v = __builtin_convertvector(f.v, float8);
-        PENC_EACH x[i] = v[i];
-        if (kNarrow || (channels & 7) == 0) {
-            if (!kNarrow && valid == 0) PENC_EACH x[i] = 0.0f;
-            return;
+        constexpr int kWords = kChunk * sizeof(T) / 4;
+        auto w = f.w;
+        if constexpr (!kNarrow) {
+            const uint32_t whole = valid == kChunk ? ~0u : 0u;
+            if constexpr (kWhole) {
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) w[i] &= whole;
+            } else {
+                // the row's last lane: forward by 8 - valid
+                const int by = kChunk - (channels & 7);
+                const uint32_t part = ~whole & (valid > 0 ? ~0u : 0u), by4 = by & 4 ? ~0u : 0u, by2 = by & 2 ? ~0u : 0u, by1 = by & 1 ? ~0u : 0u;
+                auto m = w;
+                const auto forward = [&](int n, uint32_t mask) {
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) m[i] = (i + n < kWords ? m[i + n < kWords ? i + n : 0] & mask : 0u) | (m[i] & ~mask);
+                };
+                forward(kWords / 2, by4);
+                forward(kWords / 4, by2);
+                if constexpr (kWords == kChunk) {
+                    forward(1, by1);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) m[i] = __builtin_amdgcn_alignbit(i + 1 < kWords ? m[i + 1 < kWords ? i + 1 : 0] : 0u, m[i], by1 & 16u);
+                }
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) w[i] = (w[i] & whole) | (m[i] & part);
+            }
         }
-        // the row's last lane: forward by 8 - valid
-        Values moved;
-        const int by = kChunk - (channels & 7);
-        PENC_EACH moved[i] = x[i];
-        if (by & 4) PENC_EACH moved[i] = i + 4 < kChunk ? moved[i + 4 < kChunk ? i + 4 : 0] : 0.0f;
-        if (by & 2) PENC_EACH moved[i] = i + 2 < kChunk ? moved[i + 2 < kChunk ? i + 2 : 0] : 0.0f;
-        if (by & 1) PENC_EACH moved[i] = i + 1 < kChunk ? moved[i + 1 < kChunk ? i + 1 : 0] : 0.0f;
-        PENC_EACH x[i] = valid == kChunk ? x[i] : valid == 0 ? 0.0f : moved[i];
+        const float8 v = __builtin_convertvector(__builtin_bit_cast(T __attribute__((ext_vector_type(kChunk))), w), float8);
+        PENC_EACH x[i] = v[i];
     }
-    __device__ __forceinline__ void bring(const FetchedKept& f, Values& x) const {
-        restore(valid > 0 ? f.q : make_uint2(0, 0), valid > 0 ? f.exponent : 0, x);
+    __device__ __forceinline__ void bring(const FetchedKept& f, Values& x, float scale = 1.0f) const {
+        const uint32_t here = valid > 0 ? ~0u : 0u;
+        restore(make_uint2(f.q.x & here, f.q.y & here), f.exponent & here, x, scale);
     }
     template <class T>
     __device__ __forceinline__ void store(T* __restrict__ row, const Values& x) const {
@@ -141,7 +162,7 @@ struct Place {
         float8 v;
         PENC_EACH v[i] = x[i];
         const auto y = __builtin_convertvector(v, T __attribute__((ext_vector_type(kChunk))));
-        if (valid == kChunk) {
+        if (kWhole || valid == kChunk) {
             *reinterpret_cast<chunk_t<T>*>(p) = y;
             return;
         }
@@ -168,7 +189,7 @@ struct Place {
     }
     // (a difference to the mean is zero behind the row's end)
     __device__ __forceinline__ void centre(Values& x, float mean) const {
-        PENC_EACH x[i] = i < valid ? x[i] - mean : 0.0f;
+        PENC_EACH x[i] = __uint_as_float(__float_as_uint(x[i] - mean) & static_cast<uint32_t>((kWhole ? -valid : i - valid) >> 31));
     }
 };
 
@@ -183,6 +204,27 @@ __device__ __forceinline__ float dot(const Values& x, const Values& y) {
     return s;
 }
 
+// Parameters of all rows, in the LDS: read again for every row, where registers for them would cost waves.
+template <int kLanes, int kParams>
+struct Shared {
+    float4 v[kParams][2][kLanes];
+
+    // (by the lanes of the workgroup's first row; a barrier follows)
+    template <class P>
+    __device__ __forceinline__ void load(int k, const P& at, const void* param, bool fp32, float none) {
+        if (threadIdx.x >= kLanes) return;
+        Values x;
+        at.param(param, fp32, none, x);
+        v[k][0][threadIdx.x] = make_float4(x[0], x[1], x[2], x[3]);
+        v[k][1][threadIdx.x] = make_float4(x[4], x[5], x[6], x[7]);
+    }
+    __device__ __forceinline__ void get(int k, Values& x) const {
+        const int lane = threadIdx.x % kLanes;
+        const float4 a = v[k][0][lane], b = v[k][1][lane];
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    }
+};
+
 // v becomes v~; returns r.
 template <bool kFull, class P, class R>
 __device__ __forceinline__ float normalise(Values& x, const NormArgs& a, const P& at, R& row) {
@@ -194,13 +236,20 @@ __device__ __forceinline__ float normalise(Values& x, const NormArgs& a, const P
 
 // The rows that the lanes of a row go through: `run` consecutive ones, then the next run `stride` runs on, up to `end`; body(row, the first of
 // its run, the last of its run, fetched).  `fetch` is called for a row while the one before it is worked on.
-template <class Fetch, class Body>
+template <int kLanes, class Fetch, class Body>
 __device__ __forceinline__ void walk(int64_t row, int64_t end, int64_t run, int64_t stride, Fetch&& fetch, Body&& body) {
+    // (from a wave on, a row's number is that of all lanes: its addresses are computed once)
+    const auto same = [](int64_t v) {
+        if constexpr (kLanes < 64) return v;
+        return static_cast<int64_t>(static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32))) << 32 |
+                                    static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v))));
+    };
+    row = same(row);
     if (row >= end) return;
     auto now = fetch(row);
     for (int64_t k = 0; row < end;) {
         const bool ends = k + 1 == run;
-        const int64_t next = ends ? row + 1 + (stride - 1) * run : row + 1;
+        const int64_t next = same(ends ? row + 1 + (stride - 1) * run : row + 1);
         auto ahead = fetch(min(next, end - 1));
         body(row, k == 0, ends, now);
         now = ahead;
@@ -210,10 +259,10 @@ __device__ __forceinline__ void walk(int64_t row, int64_t end, int64_t run, int6
 }
 
 // kFull: any kind of norm; else "rms" without biases, whose sums and parameters need 32 registers less.
-template <class E, int kLanes, bool kNarrow, bool kFull>
+template <class E, int kLanes, int kEnd, bool kFull>
 __global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_kernel(NormArgs a, E* __restrict__ y_out, E* __restrict__ n_out) {
     using R = Row<kLanes>;
-    using P = Place<E, kNarrow>;
+    using P = Place<E, kEnd>;
     __shared__ float2 exchange[2 * R::kWaves];
     R across{exchange};
     const P at(a.channels, threadIdx.x % kLanes);
@@ -234,7 +283,7 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_kernel(NormArgs a,
         if (a.has_branch) r.f = at.fetch(static_cast<const E*>(a.branch) + row * a.branch_stride);
         return r;
     };
-    walk(static_cast<int64_t>(blockIdx.x) * R::kRows + threadIdx.x / kLanes, a.rows, 1, static_cast<int64_t>(gridDim.x) * R::kRows, fetch,
+    walk<kLanes>(static_cast<int64_t>(blockIdx.x) * R::kRows + threadIdx.x / kLanes, a.rows, 1, static_cast<int64_t>(gridDim.x) * R::kRows, fetch,
          [&](int64_t row, bool, bool, const Fetched& fetched) {
              Values x, f;
              if (a.rows_per_gate != 0) at.param(a.gate, a.gate_fp32, 1.0f, gate, group_of(row, a.rows_per_gate) * a.channels);
@@ -282,22 +331,25 @@ __device__ __forceinline__ void write_sum(const Values& sum, float (*__restrict_
 //
 // Gates of groups of rows: with few rows in a group (a.gate_by_lanes) the lanes of a row take whole groups and write their sums themselves; else a
 // workgroup takes a piece of a group, `pieces` of them to a group, and leaves a row of partial sums.  One gate for all rows is one more sum over rows.
-template <class E, int kLanes, bool kNarrow, bool kFull, bool kKept>
-__global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_backward_kernel(NormArgs a, NormGrads g) {
+template <class E, int kLanes, int kEnd, bool kFull, bool kKept>
+__global__ __launch_bounds__(Row<kLanes>::kThreads, !kFull ? 4 : kLanes == 512 ? 2 : 3) void norm_backward_kernel(NormArgs a, NormGrads g) {
     using R = Row<kLanes>;
-    using P = Place<E, kNarrow>;
+    using P = Place<E, kEnd>;
     __shared__ float2 exchange[2 * R::kWaves];
     __shared__ float lds[R::kRows > 1 ? R::kThreads : 1][kChunk];
+    __shared__ Shared<kLanes, kFull ? 4 : 2> params;
+    constexpr int kPostWeight = 0, kPreWeight = 1, kPostBias = 2, kPreBias = 3;
     R across{exchange};
     const P at(a.channels, threadIdx.x % kLanes);
-    Values gate, post_weight, post_bias, pre_weight, pre_bias;
-    at.param(a.post_weight, a.param_fp32, 1.0f, post_weight);
-    at.param(a.pre_weight, a.param_fp32, 1.0f, pre_weight);
+    params.load(kPostWeight, at, a.post_weight, a.param_fp32, 1.0f);
+    params.load(kPreWeight, at, a.pre_weight, a.param_fp32, 1.0f);
     if constexpr (kFull) {
-        at.param(a.post_bias, a.param_fp32, 0.0f, post_bias);
-        at.param(a.pre_bias, a.param_fp32, 0.0f, pre_bias);
+        params.load(kPostBias, at, a.post_bias, a.param_fp32, 0.0f);
+        params.load(kPreBias, at, a.pre_bias, a.param_fp32, 0.0f);
     }
+    Values gate;
     at.param(a.gate, a.gate_fp32, 1.0f, gate);
+    __syncthreads();
     Values d_gate{}, d_post_weight{}, d_post_bias{}, d_pre_weight{}, d_pre_bias{};
 
     using Input = std::conditional_t<kKept, typename P::FetchedKept, typename P::template Fetched<E>>;
@@ -319,26 +371,42 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_backward_kernel(No
         return r;
     };
     const auto one_row = [&](int64_t row, const Fetched& fetched) {
-        Values y, f, inner, dy;
+        Values y, f, dy;
         float r_f = 1.0f;
-        at.bring(fetched.x, y);
-        PENC_EACH y[i] *= a.scale;
+        // p, computed twice: its registers would be held all the way
+        const auto inner = [&](Values& p) {
+            PENC_EACH p[i] = f[i];
+            if (!a.post_norm) return;
+            Values w;
+            params.get(kPostWeight, w);
+            PENC_EACH p[i] *= w[i];
+            if constexpr (kFull) {
+                params.get(kPostBias, w);
+                PENC_EACH p[i] += w[i];
+            }
+        };
+        if constexpr (kKept) {
+            at.bring(fetched.x, y, a.scale);
+        } else {
+            at.bring(fetched.x, y);
+            PENC_EACH y[i] *= a.scale;
+        }
         if (a.has_branch) {
             at.bring(fetched.f, f);
             if (a.post_norm) {
                 r_f = normalise<kFull>(f, a, at, across);
-                PENC_EACH inner[i] = kFull ? __builtin_fmaf(f[i], post_weight[i], post_bias[i]) : f[i] * post_weight[i];
-            } else {
-                PENC_EACH inner[i] = f[i];
             }
-            PENC_EACH y[i] = __builtin_fmaf(gate[i], inner[i], y[i]);
+            Values p;
+            inner(p);
+            PENC_EACH y[i] = __builtin_fmaf(gate[i], p[i], y[i]);
         }
         if (g.y != nullptr) at.bring(fetched.dy, dy);
         else PENC_EACH dy[i] = 0.0f;
         if (g.n != nullptr) {
             Values dn, d;
             at.bring(fetched.dn, dn);
-            PENC_EACH d[i] = dn[i] * pre_weight[i];
+            params.get(kPreWeight, d);
+            PENC_EACH d[i] *= dn[i];
             float mean = 0.0f;
             if (kFull && a.layer) {
                 const float2 s = across.sums(total(y), total(d));
@@ -360,15 +428,18 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_backward_kernel(No
             at.store(static_cast<E*>(g.x) + row * a.channels, dx);
         }
         if (!a.has_branch) return;
+        Values p;
+        inner(p);
         PENC_EACH {
-            d_gate[i] = __builtin_fmaf(dy[i], inner[i], d_gate[i]);
+            d_gate[i] = __builtin_fmaf(dy[i], p[i], d_gate[i]);
             dy[i] *= gate[i];
         }
         if (a.post_norm) {
+            params.get(kPostWeight, p);
             PENC_EACH {
                 d_post_weight[i] = __builtin_fmaf(dy[i], f[i], d_post_weight[i]);
                 if (kFull) d_post_bias[i] += dy[i];
-                dy[i] *= post_weight[i];
+                dy[i] *= p[i];
             }
             if (g.branch != nullptr) {
                 const float2 s = across.sums(dot(dy, f), kFull ? total(dy) : 0.0f);
@@ -386,36 +457,33 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_backward_kernel(No
     const auto leave = [&](float* sums, int64_t at_row, const Values& v) {
         if (sums != nullptr) write_sum<kLanes>(v, lds, [&](const Values& t) { at.store(sums + at_row * a.channels, t); });
     };
-    const int sub = threadIdx.x / kLanes;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * R::kRows + sub, stride = static_cast<int64_t>(gridDim.x) * R::kRows;
-    if (a.rows_per_gate == 0) {
-        walk(first, a.rows, 1, stride, fetch, [&](int64_t row, bool, bool, const Fetched& fetched) { one_row(row, fetched); });
-    } else if (a.gate_by_lanes) {
-        int64_t group = first;
-        walk(first * a.rows_per_gate, a.rows, a.rows_per_gate, stride, fetch, [&](int64_t row, bool begins, bool ends, const Fetched& fetched) {
-            if (begins) at.param(a.gate, a.gate_fp32, 1.0f, gate, group * a.channels);
+    // one gate, or gates by lanes: a workgroup has one unit of rows; else it has pieces of groups, one after the other
+    const bool pieces = a.rows_per_gate != 0 && !a.gate_by_lanes;
+    const int64_t units = pieces ? a.rows / a.rows_per_gate * g.pieces : gridDim.x;
+    const int64_t run = a.gate_by_lanes ? a.rows_per_gate : 1;
+    for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        int64_t group = unit * R::kRows + threadIdx.x / kLanes, first = group * run, end = a.rows, stride = static_cast<int64_t>(gridDim.x) * R::kRows;
+        if (pieces) {
+            group = unit / g.pieces;
+            first = group * a.rows_per_gate + unit % g.pieces * g.piece_rows;
+            end = min(first + g.piece_rows, (group + 1) * a.rows_per_gate);
+            first += threadIdx.x / kLanes;
+            stride = R::kRows;
+            at.param(a.gate, a.gate_fp32, 1.0f, gate, group * a.channels);
+        }
+        walk<kLanes>(first, end, run, stride, fetch, [&](int64_t row, bool begins, bool ends, const Fetched& fetched) {
+            if (a.gate_by_lanes && begins) at.param(a.gate, a.gate_fp32, 1.0f, gate, group * a.channels);
             one_row(row, fetched);
-            if (!ends) return;
+            if (!a.gate_by_lanes || !ends) return;
             if (g.gate != nullptr) store_gate(group, d_gate);
             PENC_EACH d_gate[i] = 0.0f;
             group += stride;
         });
-    } else {
-        const int64_t units = a.rows / a.rows_per_gate * g.pieces;
-        for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-            const int64_t group = unit / g.pieces, piece = unit % g.pieces;
-            const int64_t begin = group * a.rows_per_gate + piece * g.piece_rows;
-            at.param(a.gate, a.gate_fp32, 1.0f, gate, group * a.channels);
-            walk(begin + sub, min(begin + g.piece_rows, (group + 1) * a.rows_per_gate), 1, R::kRows, fetch,
-                 [&](int64_t row, bool, bool, const Fetched& fetched) { one_row(row, fetched); });
-            if (g.gate != nullptr) {
-                if (g.pieces == 1) write_sum<kLanes>(d_gate, lds, [&](const Values& v) { store_gate(group, v); });
-                else leave(g.gate_sums, unit, d_gate);
-            }
-            PENC_EACH d_gate[i] = 0.0f;
-        }
+        if (a.gate_by_lanes) break;
+        if (pieces && g.pieces == 1 && g.gate != nullptr) write_sum<kLanes>(d_gate, lds, [&](const Values& v) { store_gate(group, v); });
+        else leave(g.gate_sums, unit, d_gate);
+        PENC_EACH d_gate[i] = 0.0f;
     }
-    if (a.rows_per_gate == 0) leave(g.gate_sums, blockIdx.x, d_gate);
     leave(g.sums[0], blockIdx.x, d_post_weight);
     leave(g.sums[2], blockIdx.x, d_pre_weight);
     if constexpr (kFull) {
@@ -455,23 +523,21 @@ bool is_full(const NormArgs& a, const NormGrads* g) {
 
 template <class E>
 int launch_norm(const NormArgs& a, void* y, void* n, hipStream_t stream) {
-    return with_row_shape(a.channels, [&](auto lanes, auto narrow) {
-        constexpr int kLanes = decltype(lanes)::value;
-        constexpr bool kNarrow = decltype(narrow)::value;
+    return with_row_shape(a.channels, [&](auto lanes, auto end) {
+        constexpr int kLanes = decltype(lanes)::value, kEnd = decltype(end)::value;
         const dim3 grid(static_cast<unsigned>(std::min<int64_t>((a.rows + Row<kLanes>::kRows - 1) / Row<kLanes>::kRows, most_groups(kLanes)))), threads(Row<kLanes>::kThreads);
-        if (is_full(a, nullptr)) hipLaunchKernelGGL((norm_kernel<E, kLanes, kNarrow, true>), grid, threads, 0, stream, a, static_cast<E*>(y), static_cast<E*>(n));
-        else hipLaunchKernelGGL((norm_kernel<E, kLanes, kNarrow, false>), grid, threads, 0, stream, a, static_cast<E*>(y), static_cast<E*>(n));
+        if (is_full(a, nullptr)) hipLaunchKernelGGL((norm_kernel<E, kLanes, kEnd, true>), grid, threads, 0, stream, a, static_cast<E*>(y), static_cast<E*>(n));
+        else hipLaunchKernelGGL((norm_kernel<E, kLanes, kEnd, false>), grid, threads, 0, stream, a, static_cast<E*>(y), static_cast<E*>(n));
         return launched();
     });
 }
 
 template <class E>
 int launch_norm_backward(const NormArgs& a, const NormGrads& g, unsigned grid, hipStream_t stream) {
-    return with_row_shape(a.channels, [&](auto lanes, auto narrow) {
-        constexpr int kLanes = decltype(lanes)::value;
-        constexpr bool kNarrow = decltype(narrow)::value;
+    return with_row_shape(a.channels, [&](auto lanes, auto end) {
+        constexpr int kLanes = decltype(lanes)::value, kEnd = decltype(end)::value;
         const auto launch = [&](auto full, auto kept) {
-            hipLaunchKernelGGL((norm_backward_kernel<E, kLanes, kNarrow, decltype(full)::value, decltype(kept)::value>), dim3(grid), dim3(Row<kLanes>::kThreads), 0,
+            hipLaunchKernelGGL((norm_backward_kernel<E, kLanes, kEnd, decltype(full)::value, decltype(kept)::value>), dim3(grid), dim3(Row<kLanes>::kThreads), 0,
                                stream, a, g);
             return launched();
         };

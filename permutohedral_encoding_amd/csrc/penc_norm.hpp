@@ -44,13 +44,18 @@ __device__ __forceinline__ int64_t group_of(int64_t row, int64_t rows_per_gate) 
     return row / rows_per_gate;
 }
 
-// Lanes to a row, 8 channels each, and whether it has fewer than 8 channels.  A wave or less up to 512 channels: nothing goes through the LDS; from there on
+// How a row ends: in a whole chunk of 8 channels, in a part of one, or before the first is whole.
+enum RowEnd { kWholeChunks, kPartOfChunk, kNarrowRow };
+
+// Lanes to a row, 8 channels each, and how it ends.  A wave or less up to 512 channels: nothing goes through the LDS; from there on
 // a workgroup.
 template <class F>
 int with_row_shape(int channels, F&& f) {
-    if (channels < kChunk) return f(std::integral_constant<int, 4>{}, std::true_type{});
-#define PENC_SHAPE(lanes) \
-    if (channels <= lanes * kChunk) return f(std::integral_constant<int, lanes>{}, std::false_type{})
+    if (channels < kChunk) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, kNarrowRow>{});
+#define PENC_SHAPE(lanes)                                                                                                                     \
+    if (channels <= lanes * kChunk)                                                                                                           \
+        return channels % kChunk == 0 ? f(std::integral_constant<int, lanes>{}, std::integral_constant<int, kWholeChunks>{})                  \
+                                      : f(std::integral_constant<int, lanes>{}, std::integral_constant<int, kPartOfChunk>{})
     PENC_SHAPE(4);
     PENC_SHAPE(8);
     PENC_SHAPE(16);
