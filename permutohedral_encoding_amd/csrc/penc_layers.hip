@@ -187,9 +187,9 @@ struct NormPlan {
     int64_t pieces, piece_rows, gate_rows;
     bool gate_by_lanes;
 };
-NormPlan norm_plan(int64_t rows, int64_t channels, int64_t rows_per_gate) {
+NormPlan norm_plan(int64_t rows, int64_t channels, int64_t rows_per_gate, bool full) {
     const int lanes = lanes_of_row(static_cast<int>(channels));
-    const int64_t at_a_time = row_threads(lanes) / lanes, most = std::min<int64_t>(most_groups(lanes), 1024);
+    const int64_t at_a_time = row_threads(lanes) / lanes, most = most_groups(lanes, full);
     const auto groups_of = [&](int64_t n) { return std::max<int64_t>(1, (n + at_a_time - 1) / at_a_time); };
     NormPlan p{0, 1, rows_per_gate, 0, false};
     if (rows_per_gate == 0) {
@@ -344,8 +344,12 @@ int penc_residual_norm(const penc_norm* norm, void* y, void* n, void* stream) {
 
 size_t penc_residual_norm_workspace_bytes(int64_t rows, int64_t channels, int64_t rows_per_gate) {
     if (rows < 0 || channels <= 0 || channels > PENC_MAX_NORM_CHANNELS || rows_per_gate < 0) return 0;
-    const NormPlan p = norm_plan(rows, channels, rows_per_gate);
-    return 4 * static_cast<size_t>(channels) * (4 * static_cast<size_t>(p.grid) + static_cast<size_t>(p.gate_rows));
+    size_t most = 0;
+    for (const bool full : {false, true}) {
+        const NormPlan p = norm_plan(rows, channels, rows_per_gate, full);
+        most = std::max(most, 4 * static_cast<size_t>(p.grid) + static_cast<size_t>(p.gate_rows));
+    }
+    return 4 * static_cast<size_t>(channels) * most;
 }
 
 int penc_residual_norm_backward(const penc_norm* norm, const penc_norm_grads* grads, void* workspace, size_t workspace_bytes, void* stream) {
@@ -362,7 +366,7 @@ int penc_residual_norm_backward(const penc_norm* norm, const penc_norm_grads* gr
     for (const void* p : {grads->post_weight, grads->post_bias, grads->pre_weight, grads->pre_bias})
         if (!aligned_to(p, param)) return PENC_ERR_MISALIGNED;
     if (!aligned_to(grads->gate, gate) || !aligned_to(workspace, 16)) return PENC_ERR_MISALIGNED;
-    const NormPlan plan = norm_plan(a.rows, a.channels, a.rows_per_gate);
+    const NormPlan plan = norm_plan(a.rows, a.channels, a.rows_per_gate, is_full(a) || grads->post_bias || grads->pre_bias);
     if (workspace_bytes < penc_residual_norm_workspace_bytes(a.rows, a.channels, a.rows_per_gate)) return PENC_ERR_WORKSPACE_TOO_SMALL;
     if (!workspace) return PENC_ERR_NULL_POINTER;
     a.gate_by_lanes = plan.gate_by_lanes;

@@ -46,30 +46,30 @@ struct Row {
     float2* exchange;  // [2][kWaves]: a sum may begin while slow waves still read the one before it
     int turn = 0;
 
+    template <int kOver>
     __device__ __forceinline__ static float in_wave(float v) {
-        v += __uint_as_float(dpp<kSwapPairs>(__float_as_uint(v)));
-        v += __uint_as_float(dpp<kSwapTwos>(__float_as_uint(v)));
-        if constexpr (kLanes >= 8) v += __uint_as_float(dpp<kMirrorHalfRow>(__float_as_uint(v)));
-        if constexpr (kLanes >= 16) v += __uint_as_float(dpp<kMirrorRow>(__float_as_uint(v)));
-        if constexpr (kLanes >= 32) v = across_rows(v);
-        if constexpr (kLanes >= 64) v = across_halves(v);
+        if constexpr (kOver >= 2) v += __uint_as_float(dpp<kSwapPairs>(__float_as_uint(v)));
+        if constexpr (kOver >= 4) v += __uint_as_float(dpp<kSwapTwos>(__float_as_uint(v)));
+        if constexpr (kOver >= 8) v += __uint_as_float(dpp<kMirrorHalfRow>(__float_as_uint(v)));
+        if constexpr (kOver >= 16) v += __uint_as_float(dpp<kMirrorRow>(__float_as_uint(v)));
+        if constexpr (kOver >= 32) v = across_rows(v);
+        if constexpr (kOver >= 64) v = across_halves(v);
         return v;
     }
     __device__ __forceinline__ float2 sums(float a, float b) {
-        float2 v = make_float2(in_wave(a), in_wave(b));
+        float2 v = make_float2(in_wave<kLanes>(a), in_wave<kLanes>(b));
         if constexpr (kWaves > 1) {
             float2* const e = exchange + turn * kWaves;
             turn ^= 1;
             if (threadIdx.x % 64 == 0) e[threadIdx.x / 64] = v;
             __syncthreads();
-            v = e[0];
-#pragma unroll
-            for (int i = 1; i < kWaves; ++i) v.x += e[i].x, v.y += e[i].y;
+            v = e[threadIdx.x % kWaves];
+            v.x = in_wave<kWaves>(v.x), v.y = in_wave<kWaves>(v.y);
         }
         return v;
     }
     __device__ __forceinline__ float sum(float a) {
-        if constexpr (kWaves == 1) return in_wave(a);
+        if constexpr (kWaves == 1) return in_wave<kLanes>(a);
         else return sums(a, 0.0f).x;
     }
 };
@@ -516,17 +516,12 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(SumPartials s) {
     else static_cast<E*>(sum.to)[group * s.channels + c] = static_cast<E>(total);
 }
 
-// "rms" without biases, also of gradients that nobody asked for
-bool is_full(const NormArgs& a, const NormGrads* g) {
-    return a.layer || a.post_bias != nullptr || a.pre_bias != nullptr || (g != nullptr && (g->sums[1] != nullptr || g->sums[3] != nullptr));
-}
-
 template <class E>
 int launch_norm(const NormArgs& a, void* y, void* n, hipStream_t stream) {
     return with_row_shape(a.channels, [&](auto lanes, auto end) {
         constexpr int kLanes = decltype(lanes)::value, kEnd = decltype(end)::value;
-        const dim3 grid(static_cast<unsigned>(std::min<int64_t>((a.rows + Row<kLanes>::kRows - 1) / Row<kLanes>::kRows, most_groups(kLanes)))), threads(Row<kLanes>::kThreads);
-        if (is_full(a, nullptr)) hipLaunchKernelGGL((norm_kernel<E, kLanes, kEnd, true>), grid, threads, 0, stream, a, static_cast<E*>(y), static_cast<E*>(n));
+        const dim3 grid(static_cast<unsigned>(std::min<int64_t>((a.rows + Row<kLanes>::kRows - 1) / Row<kLanes>::kRows, most_groups(kLanes, false)))), threads(Row<kLanes>::kThreads);
+        if (is_full(a)) hipLaunchKernelGGL((norm_kernel<E, kLanes, kEnd, true>), grid, threads, 0, stream, a, static_cast<E*>(y), static_cast<E*>(n));
         else hipLaunchKernelGGL((norm_kernel<E, kLanes, kEnd, false>), grid, threads, 0, stream, a, static_cast<E*>(y), static_cast<E*>(n));
         return launched();
     });
@@ -542,7 +537,7 @@ int launch_norm_backward(const NormArgs& a, const NormGrads& g, unsigned grid, h
             return launched();
         };
         const auto with_kept = [&](auto full) { return a.kept_x.values != nullptr ? launch(full, std::true_type{}) : launch(full, std::false_type{}); };
-        return is_full(a, &g) ? with_kept(std::true_type{}) : with_kept(std::false_type{});
+        return is_full(a) || g.sums[1] != nullptr || g.sums[3] != nullptr ? with_kept(std::true_type{}) : with_kept(std::false_type{});
     });
 }
 

@@ -19,6 +19,9 @@ struct NormArgs {
     KeptArray kept_x, kept_branch;
 };
 
+// Whether a norm is more than "rms" without biases.
+inline bool is_full(const NormArgs& a) { return a.layer || a.post_bias != nullptr || a.pre_bias != nullptr; }
+
 struct NormGrads {
     const void *y, *n;
     int64_t y_stride, n_stride;
@@ -71,8 +74,10 @@ int with_row_shape(int channels, F&& f) {
 static_assert(PENC_MAX_NORM_CHANNELS == 1024 * kChunk, "the widest row");
 
 __host__ __device__ constexpr int row_threads(int lanes) { return lanes > 64 ? lanes : 256; }
-// Workgroups that the card holds at a time, with 16 waves to each of its 256 compute units.
-inline int64_t most_groups(int lanes) { return 256 * 16 * 64 / row_threads(lanes); }
+// Workgroups that the card's 256 compute units hold at a time: 16 waves each, of the backward of any kind of norm 12, or 8 where a workgroup has as many.
+inline int64_t most_groups(int lanes, bool full_backward) {
+    return 256 * ((full_backward && lanes < 1024 ? lanes == 512 ? 8 : 12 : 16) * 64 / row_threads(lanes));
+}
 
 inline int lanes_of_row(int channels) {
     int n = 0;
