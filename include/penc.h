@@ -407,7 +407,7 @@ int penc_simplex_debug(int pos_dim, int64_t nr_positions, int nr_levels, int cap
  *
  * Rows of `channels` values of a type below; a row stride is counted in values, and channels of a row are adjacent
  * unless an entry point has a stride for them.  Arrays need the alignment of one value, checkpoints 16 bytes.  No rows is a valid call that
- * writes nothing (sums over the rows become zero).  Sums, statistics and steps are fp32, results are rounded once, to nearest, ties to even, and do not
+ * writes nothing (sums over the rows become zero).  Numbers of rows and row strides stay below 2^31.  Sums, statistics and steps are fp32, results are rounded once, to nearest, ties to even, and do not
  * depend on the order in which workgroups run.
  *
  * A checkpoint keeps rows in 8 bits, in blocks of 32 channels.  With a the largest magnitude of a block, e = the least integer of at least

@@ -142,21 +142,27 @@ __device__ __forceinline__ void restore(uint2 q, uint32_t exponent, float (&v)[k
     for (int i = 0; i < kChunk; ++i) v[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? q.x : q.y) >> 8 * (i % 4))) * step;
 }
 
+// Rows are numbered in 32 bits, and so are their strides: where a row begins takes one multiplication.
+using row_t = uint32_t;
+constexpr int64_t kMostRows = (int64_t{1} << 31) - 1;
+__device__ __forceinline__ uint64_t offset_of(row_t row, uint32_t stride) { return static_cast<uint64_t>(row) * stride; }
+
 // Where a checkpoint is, or null.
 struct KeptArray {
     int8_t* values;
     uint8_t* exponents;
-    int64_t pitch, blocks;
+    uint32_t pitch, blocks;
 
     // The lane of the chunk that begins at channel `c` of a row; all four lanes of a block call it.
-    __device__ __forceinline__ void store(int64_t row, int c, const float (&v)[kChunk]) const {
+    __device__ __forceinline__ void store(row_t row, int c, const float (&v)[kChunk]) const {
         const Kept k = keep(v);
-        if (c < pitch) *reinterpret_cast<uint2*>(values + row * pitch + c) = k.q;
-        if (c % kKeptBlock == 0 && c / kKeptBlock < blocks) exponents[row * blocks + c / kKeptBlock] = static_cast<uint8_t>(k.exponent);
+        const uint32_t at = static_cast<uint32_t>(c);
+        if (at < pitch) *reinterpret_cast<uint2*>(values + offset_of(row, pitch) + at) = k.q;
+        if (at % kKeptBlock == 0 && at / kKeptBlock < blocks) exponents[offset_of(row, blocks) + at / kKeptBlock] = static_cast<uint8_t>(k.exponent);
     }
-    __device__ __forceinline__ void load(int64_t row, int c, int valid, float (&v)[kChunk]) const {
+    __device__ __forceinline__ void load(row_t row, int c, int valid, float (&v)[kChunk]) const {
         if (valid > 0) {
-            restore(*reinterpret_cast<const uint2*>(values + row * pitch + c), exponents[row * blocks + c / kKeptBlock], v);
+            restore(*reinterpret_cast<const uint2*>(values + offset_of(row, pitch) + c), exponents[offset_of(row, blocks) + c / kKeptBlock], v);
             if (valid < kChunk) {
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i)
@@ -170,7 +176,8 @@ struct KeptArray {
 };
 
 inline KeptArray kept_array(const int8_t* values, const uint8_t* exponents, int64_t channels) {
-    return {const_cast<int8_t*>(values), const_cast<uint8_t*>(exponents), kept_pitch(channels), kept_blocks(channels)};
+    return {const_cast<int8_t*>(values), const_cast<uint8_t*>(exponents), static_cast<uint32_t>(kept_pitch(channels)),
+            static_cast<uint32_t>(kept_blocks(channels))};
 }
 
 // Runs `f` with a value of the type that an entry point's `type` names.
@@ -184,6 +191,8 @@ int with_type(int type, F&& f) {
     }
 }
 
+inline bool bad_rows(int64_t rows) { return rows < 0 || rows > kMostRows; }
+inline bool bad_stride(int64_t stride) { return stride < 0 || stride > kMostRows; }
 inline int launched() { return hipGetLastError() == hipSuccess ? PENC_OK : PENC_ERR_LAUNCH; }
 inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 

@@ -22,13 +22,13 @@ constexpr int kThreads = 256;
 
 // How lanes are laid over rows: 2^log2_lanes of them on a row, which takes `chunks` of eight channels (a multiple of four).
 struct Lanes {
-    int64_t rows;
+    row_t rows;
     int channels, chunks, log2_lanes;
     unsigned grid;
 };
 
 Lanes lanes_for(int64_t rows, int64_t channels) {
-    Lanes l{rows, static_cast<int>(channels), static_cast<int>(4 * kept_blocks(channels)), 2, 0};
+    Lanes l{static_cast<row_t>(rows), static_cast<int>(channels), static_cast<int>(4 * kept_blocks(channels)), 2, 0};
     while (l.log2_lanes < 8 && (1 << l.log2_lanes) < l.chunks) ++l.log2_lanes;
     const int64_t per_group = kThreads >> l.log2_lanes;
     l.grid = static_cast<unsigned>(std::min<int64_t>((rows + per_group - 1) / per_group, 8192));
@@ -40,16 +40,15 @@ template <class F>
 __device__ __forceinline__ void over_chunks(const Lanes& l, F&& f) {
     const int lanes = 1 << l.log2_lanes, per_group = kThreads >> l.log2_lanes;
     const int lane = threadIdx.x & (lanes - 1);
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * per_group + (threadIdx.x >> l.log2_lanes); row < l.rows;
-         row += static_cast<int64_t>(gridDim.x) * per_group)
+    for (row_t row = blockIdx.x * per_group + (threadIdx.x >> l.log2_lanes); row < l.rows; row += gridDim.x * per_group)
         for (int chunk = lane; chunk < l.chunks; chunk += lanes) f(row, chunk * kChunk, min(l.channels - chunk * kChunk, kChunk));
 }
 
 template <class E>
-__global__ __launch_bounds__(kThreads) void pack_kernel(Lanes l, const E* __restrict__ x, int64_t stride, KeptArray kept) {
-    over_chunks(l, [&](int64_t row, int c, int valid) {
+__global__ __launch_bounds__(kThreads) void pack_kernel(Lanes l, const E* __restrict__ x, uint32_t stride, KeptArray kept) {
+    over_chunks(l, [&](row_t row, int c, int valid) {
         float v[kChunk];
-        load_chunk(x + row * stride + c, valid, v);
+        load_chunk(x + offset_of(row, stride) + c, valid, v);
         kept.store(row, c, v);
     });
 }
@@ -57,8 +56,8 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(Lanes l, const E* __rest
 // The encoding's own result: channels of consecutive rows next to each other.  A lane has a row and walks over its blocks, reading 32 channels,
 // each with the 63 lanes beside it.
 template <class E>
-__global__ __launch_bounds__(kThreads) void pack_channels_kernel(int64_t rows, int channels, const E* __restrict__ x, int64_t stride, KeptArray kept) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+__global__ __launch_bounds__(kThreads) void pack_channels_kernel(row_t rows, int channels, const E* __restrict__ x, int64_t stride, KeptArray kept) {
+    const row_t row = blockIdx.x * kThreads + threadIdx.x;
     if (row >= rows) return;
     for (int first = 0; first < channels; first += kKeptBlock) {
         float v[kKeptBlock];
@@ -69,21 +68,21 @@ __global__ __launch_bounds__(kThreads) void pack_channels_kernel(int64_t rows, i
         for (int i = 0; i < kKeptBlock; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
         const BlockStep s(a);
         s.saturate(v);
-        int8_t* const to = kept.values + row * kept.pitch + first;
+        int8_t* const to = kept.values + offset_of(row, kept.pitch) + first;
 #pragma unroll
         for (int i = 0; i < kKeptBlock; i += 16) {
-            if (first + i >= kept.pitch) break;
+            if (first + i >= static_cast<int>(kept.pitch)) break;
             uint4 q;
             q.x = s.quantised(v + i), q.y = s.quantised(v + i + 4), q.z = s.quantised(v + i + 8), q.w = s.quantised(v + i + 12);
             *reinterpret_cast<uint4*>(to + i) = q;
         }
-        kept.exponents[row * kept.blocks + first / kKeptBlock] = static_cast<uint8_t>(s.exponent);
+        kept.exponents[offset_of(row, kept.blocks) + first / kKeptBlock] = static_cast<uint8_t>(s.exponent);
     }
 }
 
 template <class E>
 __global__ __launch_bounds__(kThreads) void unpack_kernel(Lanes l, KeptArray kept, E* __restrict__ x) {
-    over_chunks(l, [&](int64_t row, int c, int valid) {
+    over_chunks(l, [&](row_t row, int c, int valid) {
         float v[kChunk];
         kept.load(row, c, valid, v);
         if constexpr (sizeof(E) == 2 && !std::is_same_v<E, bf16_t>) {
@@ -91,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void unpack_kernel(Lanes l, KeptArray kep
 #pragma unroll
             for (int i = 0; i < kChunk; ++i) v[i] = v[i] > 65504.0f ? 65504.0f : v[i] < -65504.0f ? -65504.0f : v[i];
         }
-        if (valid > 0) store_chunk(x + row * l.channels + c, valid, v);
+        if (valid > 0) store_chunk(x + offset_of(row, l.channels) + c, valid, v);
     });
 }
 
@@ -115,12 +114,12 @@ __device__ __forceinline__ void activate(float x, float& value, float& slope) {
 }
 
 template <class E, int kKind, bool kGated>
-__global__ __launch_bounds__(kThreads) void activation_kernel(Lanes l, const E* __restrict__ x, int64_t stride, E* __restrict__ y, KeptArray kept,
+__global__ __launch_bounds__(kThreads) void activation_kernel(Lanes l, const E* __restrict__ x, uint32_t stride, E* __restrict__ y, KeptArray kept,
                                                               KeptArray kept_gate) {
-    over_chunks(l, [&](int64_t row, int c, int valid) {
+    over_chunks(l, [&](row_t row, int c, int valid) {
         float a[kChunk], b[kChunk], unused;
-        load_chunk(x + row * stride + c, valid, a);
-        if constexpr (kGated) load_chunk(x + row * stride + l.channels + c, valid, b);
+        load_chunk(x + offset_of(row, stride) + c, valid, a);
+        if constexpr (kGated) load_chunk(x + offset_of(row, stride) + l.channels + c, valid, b);
         if (kept.values != nullptr) {
             kept.store(row, c, a);
             if constexpr (kGated) kept_gate.store(row, c, b);
@@ -131,22 +130,22 @@ __global__ __launch_bounds__(kThreads) void activation_kernel(Lanes l, const E* 
             activate<kKind>(a[i], a[i], unused);
             if constexpr (kGated) a[i] *= b[i];
         }
-        store_chunk(y + row * l.channels + c, valid, a);
+        store_chunk(y + offset_of(row, l.channels) + c, valid, a);
     });
 }
 
 // x: the input itself, or null where it is kept in 8 bits
 template <class E, int kKind, bool kGated>
-__global__ __launch_bounds__(kThreads) void activation_backward_kernel(Lanes l, const E* __restrict__ x, int64_t stride, KeptArray kept,
-                                                                       KeptArray kept_gate, const E* __restrict__ grad, int64_t grad_stride,
+__global__ __launch_bounds__(kThreads) void activation_backward_kernel(Lanes l, const E* __restrict__ x, uint32_t stride, KeptArray kept,
+                                                                       KeptArray kept_gate, const E* __restrict__ grad, uint32_t grad_stride,
                                                                        E* __restrict__ dx) {
-    over_chunks(l, [&](int64_t row, int c, int valid) {
+    over_chunks(l, [&](row_t row, int c, int valid) {
         if (valid <= 0) return;
         float a[kChunk], b[kChunk], g[kChunk], value, slope;
-        load_chunk(grad + row * grad_stride + c, valid, g);
+        load_chunk(grad + offset_of(row, grad_stride) + c, valid, g);
         if (x != nullptr) {
-            load_chunk(x + row * stride + c, valid, a);
-            if constexpr (kGated) load_chunk(x + row * stride + l.channels + c, valid, b);
+            load_chunk(x + offset_of(row, stride) + c, valid, a);
+            if constexpr (kGated) load_chunk(x + offset_of(row, stride) + l.channels + c, valid, b);
         } else {
             kept.load(row, c, valid, a);
             if constexpr (kGated) kept_gate.load(row, c, valid, b);
@@ -161,7 +160,7 @@ __global__ __launch_bounds__(kThreads) void activation_backward_kernel(Lanes l, 
                 a[i] = g[i] * slope;
             }
         }
-        E* const to = dx + row * l.channels * (kGated ? 2 : 1) + c;
+        E* const to = dx + offset_of(row, l.channels * (kGated ? 2 : 1)) + c;
         store_chunk(to, valid, a);
         if constexpr (kGated) store_chunk(to + l.channels, valid, b);
     });
@@ -178,7 +177,7 @@ int with_kind(int kind, int gated, F&& f) {
     }
 }
 
-bool bad_size(int64_t rows, int64_t channels) { return rows < 0 || channels <= 0 || channels > PENC_MAX_CHANNELS; }
+bool bad_size(int64_t rows, int64_t channels) { return bad_rows(rows) || channels <= 0 || channels > PENC_MAX_CHANNELS; }
 bool misplaced(const int8_t* values) { return !aligned_to(values, kKeptPitch); }
 
 // How the backward of a norm is cut up: workgroups, pieces of a group of rows that share a gate, and the rows of partial sums they leave.
@@ -220,7 +219,7 @@ bool norm_args(const penc_norm* n, NormArgs& a, int& status) {
         (n->gate_type != n->type && n->gate_type != PENC_FP32))
         return false;
     status = PENC_ERR_BAD_LAYER_SIZE;
-    if (n->rows < 0 || n->channels <= 0 || n->channels > PENC_MAX_NORM_CHANNELS || n->rows_per_gate < 0 ||
+    if (bad_rows(n->rows) || bad_stride(n->x_stride) || bad_stride(n->branch_stride) || n->channels <= 0 || n->channels > PENC_MAX_NORM_CHANNELS || n->rows_per_gate < 0 ||
         (n->rows_per_gate > 0 && n->rows % n->rows_per_gate != 0))
         return false;
     status = PENC_ERR_NULL_POINTER;
@@ -230,7 +229,8 @@ bool norm_args(const penc_norm* n, NormArgs& a, int& status) {
     if (misplaced(n->x_values) || misplaced(n->branch_values) || !aligned_to(n->x, size) || !aligned_to(n->branch, size) || !aligned_to(n->gate, gate) ||
         !aligned_to(n->post_weight, param) || !aligned_to(n->post_bias, param) || !aligned_to(n->pre_weight, param) || !aligned_to(n->pre_bias, param))
         return false;
-    a = {n->rows, n->rows_per_gate, n->x_stride, n->branch_stride, static_cast<int>(n->channels), n->residual_scale, n->eps, n->kind == PENC_LAYER,
+    a = {static_cast<row_t>(n->rows), static_cast<row_t>(n->rows_per_gate), static_cast<uint32_t>(n->x_stride), static_cast<uint32_t>(n->branch_stride),
+         static_cast<int>(n->channels), n->residual_scale, n->eps, n->kind == PENC_LAYER,
          n->post_norm != 0, n->pre_norm != 0, n->has_branch != 0, n->param_type == PENC_FP32, n->gate_type == PENC_FP32, false, n->x, n->branch, n->gate,
          n->post_weight, n->post_bias, n->pre_weight, n->pre_bias, kept_array(n->x_values, n->x_exponents, n->channels),
          kept_array(n->branch_values, n->branch_exponents, n->channels)};
@@ -254,7 +254,8 @@ int64_t penc_kept_blocks(int64_t channels) { return kept_blocks(channels); }
 
 int penc_keep(int type, int64_t rows, int64_t channels, const void* x, int64_t row_stride, int64_t channel_stride, int8_t* values,
               uint8_t* exponents, void* stream) {
-    if (bad_size(rows, channels) || (channel_stride != 1 && row_stride != 1)) return PENC_ERR_BAD_LAYER_SIZE;
+    if (bad_size(rows, channels) || (channel_stride != 1 && row_stride != 1) || (channel_stride == 1 && bad_stride(row_stride)) || channel_stride < 0)
+        return PENC_ERR_BAD_LAYER_SIZE;
     return with_type(type, [&](auto e) {
         using E = decltype(e);
         if (rows == 0) return PENC_OK;
@@ -264,11 +265,10 @@ int penc_keep(int type, int64_t rows, int64_t channels, const void* x, int64_t r
         if (channel_stride == 1) {
             const Lanes l = lanes_for(rows, channels);
             hipLaunchKernelGGL(pack_kernel<E>, dim3(l.grid), dim3(kThreads), 0, static_cast<hipStream_t>(stream), l, static_cast<const E*>(x),
-                               row_stride, kept);
+                               static_cast<uint32_t>(row_stride), kept);
         } else {
             const int64_t groups = (rows + kThreads - 1) / kThreads;
-            if (groups > 0x7FFFFFFF) return PENC_ERR_BAD_LAYER_SIZE;
-            hipLaunchKernelGGL(pack_channels_kernel<E>, dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), rows,
+            hipLaunchKernelGGL(pack_channels_kernel<E>, dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), static_cast<row_t>(rows),
                                static_cast<int>(channels), static_cast<const E*>(x), channel_stride, kept);
         }
         return launched();
@@ -291,7 +291,7 @@ int penc_restore(int type, int64_t rows, int64_t channels, const int8_t* values,
 
 int penc_activation(int type, int kind, int gated, int64_t rows, int64_t channels, const void* x, int64_t row_stride, void* y, int8_t* values,
                     uint8_t* exponents, void* stream) {
-    if (bad_size(rows, channels)) return PENC_ERR_BAD_LAYER_SIZE;
+    if (bad_size(rows, channels) || bad_stride(row_stride)) return PENC_ERR_BAD_LAYER_SIZE;
     return with_type(type, [&](auto e) {
         using E = decltype(e);
         return with_kind(kind, gated, [&](auto k, auto g) {
@@ -303,7 +303,7 @@ int penc_activation(int type, int kind, int gated, int64_t rows, int64_t channel
             KeptArray kept_gate = kept;
             if (values != nullptr) kept_gate.values += rows * kept.pitch, kept_gate.exponents += rows * kept.blocks;
             hipLaunchKernelGGL((activation_kernel<E, decltype(k)::value, decltype(g)::value>), dim3(l.grid), dim3(kThreads), 0,
-                               static_cast<hipStream_t>(stream), l, static_cast<const E*>(x), row_stride, static_cast<E*>(y), kept, kept_gate);
+                               static_cast<hipStream_t>(stream), l, static_cast<const E*>(x), static_cast<uint32_t>(row_stride), static_cast<E*>(y), kept, kept_gate);
             return launched();
         });
     });
@@ -311,7 +311,7 @@ int penc_activation(int type, int kind, int gated, int64_t rows, int64_t channel
 
 int penc_activation_backward(int type, int kind, int gated, int64_t rows, int64_t channels, const void* x, int64_t row_stride, const int8_t* values,
                              const uint8_t* exponents, const void* grad, int64_t grad_row_stride, void* dx, void* stream) {
-    if (bad_size(rows, channels)) return PENC_ERR_BAD_LAYER_SIZE;
+    if (bad_size(rows, channels) || bad_stride(row_stride) || bad_stride(grad_row_stride)) return PENC_ERR_BAD_LAYER_SIZE;
     return with_type(type, [&](auto e) {
         using E = decltype(e);
         return with_kind(kind, gated, [&](auto k, auto g) {
@@ -323,8 +323,8 @@ int penc_activation_backward(int type, int kind, int gated, int64_t rows, int64_
             KeptArray kept_gate = kept;
             if (values != nullptr) kept_gate.values += rows * kept.pitch, kept_gate.exponents += rows * kept.blocks;
             hipLaunchKernelGGL((activation_backward_kernel<E, decltype(k)::value, decltype(g)::value>), dim3(l.grid), dim3(kThreads), 0,
-                               static_cast<hipStream_t>(stream), l, static_cast<const E*>(x), row_stride, kept, kept_gate, static_cast<const E*>(grad),
-                               grad_row_stride, static_cast<E*>(dx));
+                               static_cast<hipStream_t>(stream), l, static_cast<const E*>(x), static_cast<uint32_t>(row_stride), kept, kept_gate, static_cast<const E*>(grad),
+                               static_cast<uint32_t>(grad_row_stride), static_cast<E*>(dx));
             return launched();
         });
     });
@@ -343,7 +343,7 @@ int penc_residual_norm(const penc_norm* norm, void* y, void* n, void* stream) {
 }
 
 size_t penc_residual_norm_workspace_bytes(int64_t rows, int64_t channels, int64_t rows_per_gate) {
-    if (rows < 0 || channels <= 0 || channels > PENC_MAX_NORM_CHANNELS || rows_per_gate < 0) return 0;
+    if (bad_rows(rows) || channels <= 0 || channels > PENC_MAX_NORM_CHANNELS || rows_per_gate < 0) return 0;
     size_t most = 0;
     for (const bool full : {false, true}) {
         const NormPlan p = norm_plan(rows, channels, rows_per_gate, full);
@@ -366,12 +366,13 @@ int penc_residual_norm_backward(const penc_norm* norm, const penc_norm_grads* gr
     for (const void* p : {grads->post_weight, grads->post_bias, grads->pre_weight, grads->pre_bias})
         if (!aligned_to(p, param)) return PENC_ERR_MISALIGNED;
     if (!aligned_to(grads->gate, gate) || !aligned_to(workspace, 16)) return PENC_ERR_MISALIGNED;
+    if (bad_stride(grads->y_stride) || bad_stride(grads->n_stride)) return PENC_ERR_BAD_LAYER_SIZE;
     const NormPlan plan = norm_plan(a.rows, a.channels, a.rows_per_gate, is_full(a) || grads->post_bias || grads->pre_bias);
     if (workspace_bytes < penc_residual_norm_workspace_bytes(a.rows, a.channels, a.rows_per_gate)) return PENC_ERR_WORKSPACE_TOO_SMALL;
     if (!workspace) return PENC_ERR_NULL_POINTER;
     a.gate_by_lanes = plan.gate_by_lanes;
-    NormGrads g{grads->y, a.pre_norm ? grads->n : nullptr, grads->y_stride, grads->n_stride, grads->x, a.has_branch ? grads->branch : nullptr, grads->gate,
-                nullptr, {}, plan.pieces, plan.piece_rows};
+    NormGrads g{grads->y, a.pre_norm ? grads->n : nullptr, static_cast<uint32_t>(grads->y_stride), static_cast<uint32_t>(grads->n_stride), grads->x, a.has_branch ? grads->branch : nullptr, grads->gate,
+                nullptr, {}, static_cast<uint32_t>(plan.pieces), static_cast<row_t>(plan.piece_rows)};
     // partial sums of what is wanted, one array after the other
     float* next = static_cast<float*>(workspace);
     SumPartials sums{};

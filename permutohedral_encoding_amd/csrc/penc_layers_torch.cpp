@@ -113,8 +113,9 @@ Rows rows_of(const Tensor& t, const char* name) {
     PENC_REQUIRE(r.channels >= 1, name, " should have at least one channel, however it has sizes ", t.sizes());
     r.n = t.numel() / r.channels;
     r.values = t;
-    if (r.n == 0) r.stride = r.channels;
-    else if (!rows_in_place(t, r.stride)) {
+    if (r.n == 0) {
+        r.stride = r.channels;
+    } else if (!rows_in_place(t, r.stride) || r.stride >= (int64_t{1} << 31)) {
         r.values = t.contiguous();
         r.stride = r.channels;
     }

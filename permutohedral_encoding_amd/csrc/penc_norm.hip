@@ -110,9 +110,9 @@ struct Place {
             return {*reinterpret_cast<const Unaligned*>(row + min(first, channels - kChunk))};
         }
     }
-    __device__ __forceinline__ FetchedKept fetch(const KeptArray& kept, int64_t row) const {
+    __device__ __forceinline__ FetchedKept fetch(const KeptArray& kept, row_t row) const {
         const int c = min(first, static_cast<int>(kept.pitch) - kChunk);
-        return {*reinterpret_cast<const uint2*>(kept.values + row * kept.pitch + c), kept.exponents[row * kept.blocks + c / kKeptBlock]};
+        return {*reinterpret_cast<const uint2*>(kept.values + offset_of(row, kept.pitch) + c), kept.exponents[offset_of(row, kept.blocks) + c / kKeptBlock]};
     }
     // (with masks in place of conditions: of those the compiler makes a branch for each channel)
     template <class T>
@@ -182,7 +182,7 @@ struct Place {
         }
     }
     // a parameter, or `none` for each channel
-    __device__ __forceinline__ void param(const void* p, bool fp32, float none, Values& x, int64_t at = 0) const {
+    __device__ __forceinline__ void param(const void* p, bool fp32, float none, Values& x, uint64_t at = 0) const {
         if (p == nullptr) PENC_EACH x[i] = none;
         else if (fp32) bring(fetch(static_cast<const float*>(p) + at), x);
         else bring(fetch(static_cast<const E*>(p) + at), x);
@@ -237,19 +237,15 @@ __device__ __forceinline__ float normalise(Values& x, const NormArgs& a, const P
 // The rows that the lanes of a row go through: `run` consecutive ones, then the next run `stride` runs on, up to `end`; body(row, the first of
 // its run, the last of its run, fetched).  `fetch` is called for a row while the one before it is worked on.
 template <int kLanes, class Fetch, class Body>
-__device__ __forceinline__ void walk(int64_t row, int64_t end, int64_t run, int64_t stride, Fetch&& fetch, Body&& body) {
+__device__ __forceinline__ void walk(row_t row, row_t end, row_t run, row_t stride, Fetch&& fetch, Body&& body) {
     // (from a wave on, a row's number is that of all lanes: its addresses are computed once)
-    const auto same = [](int64_t v) {
-        if constexpr (kLanes < 64) return v;
-        return static_cast<int64_t>(static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32))) << 32 |
-                                    static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v))));
-    };
+    const auto same = [](row_t v) { return kLanes < 64 ? v : static_cast<row_t>(__builtin_amdgcn_readfirstlane(v)); };
     row = same(row);
     if (row >= end) return;
     auto now = fetch(row);
-    for (int64_t k = 0; row < end;) {
+    for (row_t k = 0; row < end;) {
         const bool ends = k + 1 == run;
-        const int64_t next = same(ends ? row + 1 + (stride - 1) * run : row + 1);
+        const row_t next = same(ends ? row + 1 + (stride - 1) * run : row + 1);
         auto ahead = fetch(min(next, end - 1));
         body(row, k == 0, ends, now);
         now = ahead;
@@ -277,36 +273,45 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_kernel(NormArgs a,
     struct Fetched {
         typename P::template Fetched<E> x, f;
     };
-    const auto fetch = [&](int64_t row) {
+    const auto fetch = [&](row_t row) {
         Fetched r;
-        r.x = at.fetch(static_cast<const E*>(a.x) + row * a.x_stride);
-        if (a.has_branch) r.f = at.fetch(static_cast<const E*>(a.branch) + row * a.branch_stride);
+        r.x = at.fetch(static_cast<const E*>(a.x) + offset_of(row, a.x_stride));
+        if (a.has_branch) r.f = at.fetch(static_cast<const E*>(a.branch) + offset_of(row, a.branch_stride));
         return r;
     };
-    walk<kLanes>(static_cast<int64_t>(blockIdx.x) * R::kRows + threadIdx.x / kLanes, a.rows, 1, static_cast<int64_t>(gridDim.x) * R::kRows, fetch,
-         [&](int64_t row, bool, bool, const Fetched& fetched) {
-             Values x, f;
-             if (a.rows_per_gate != 0) at.param(a.gate, a.gate_fp32, 1.0f, gate, group_of(row, a.rows_per_gate) * a.channels);
-             at.bring(fetched.x, x);
-             if (a.kept_x.values != nullptr) a.kept_x.store(row, at.first, x);
-             PENC_EACH x[i] *= a.scale;
-             if (a.has_branch) {
-                 at.bring(fetched.f, f);
-                 if (a.kept_branch.values != nullptr) a.kept_branch.store(row, at.first, f);
-                 if (a.post_norm) {
-                     normalise<kFull>(f, a, at, across);
-                     PENC_EACH f[i] = kFull ? __builtin_fmaf(f[i], post_weight[i], post_bias[i]) : f[i] * post_weight[i];
-                 }
-                 PENC_EACH x[i] = __builtin_fmaf(gate[i], f[i], x[i]);
-             }
-             if (y_out != nullptr) at.store(y_out + row * a.channels, x);
-             if (a.pre_norm) {
-                 // (of y before it is rounded)
-                 normalise<kFull>(x, a, at, across);
-                 PENC_EACH x[i] = kFull ? __builtin_fmaf(x[i], pre_weight[i], pre_bias[i]) : x[i] * pre_weight[i];
-                 at.store(n_out + row * a.channels, x);
-             }
-         });
+    // One gate: workgroups take rows in turn.  Else each takes rows that follow each other, and the gate changes seldom.
+    row_t first = blockIdx.x * R::kRows + threadIdx.x / kLanes, end = a.rows, stride = gridDim.x * R::kRows, gate_until = 0;
+    if (a.rows_per_gate != 0) {
+        const row_t each = ((a.rows - 1) / stride + 1) * R::kRows, begin = min(blockIdx.x * each, a.rows);
+        first = begin + threadIdx.x / kLanes, end = min(begin + each, a.rows), stride = R::kRows;
+    }
+    walk<kLanes>(first, end, 1, stride, fetch, [&](row_t row, bool, bool, const Fetched& fetched) {
+        Values x, f;
+        if (a.rows_per_gate != 0 && row >= gate_until) {
+            const row_t group = row / a.rows_per_gate;
+            gate_until = (group + 1) * a.rows_per_gate;
+            at.param(a.gate, a.gate_fp32, 1.0f, gate, offset_of(group, a.channels));
+        }
+        at.bring(fetched.x, x);
+        if (a.kept_x.values != nullptr) a.kept_x.store(row, at.first, x);
+        PENC_EACH x[i] *= a.scale;
+        if (a.has_branch) {
+            at.bring(fetched.f, f);
+            if (a.kept_branch.values != nullptr) a.kept_branch.store(row, at.first, f);
+            if (a.post_norm) {
+                normalise<kFull>(f, a, at, across);
+                PENC_EACH f[i] = kFull ? __builtin_fmaf(f[i], post_weight[i], post_bias[i]) : f[i] * post_weight[i];
+            }
+            PENC_EACH x[i] = __builtin_fmaf(gate[i], f[i], x[i]);
+        }
+        if (y_out != nullptr) at.store(y_out + offset_of(row, a.channels), x);
+        if (a.pre_norm) {
+            // (of y before it is rounded)
+            normalise<kFull>(x, a, at, across);
+            PENC_EACH x[i] = kFull ? __builtin_fmaf(x[i], pre_weight[i], pre_bias[i]) : x[i] * pre_weight[i];
+            at.store(n_out + offset_of(row, a.channels), x);
+        }
+    });
 }
 
 // The sums of one of a lane's accumulators over the rows that a workgroup has at a time: `store` gets them in the lanes of the first.
@@ -357,20 +362,20 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads, !kFull ? 4 : kLanes == 512 ?
         Input x, f;
         typename P::template Fetched<E> dy, dn;
     };
-    const auto fetch = [&](int64_t row) {
+    const auto fetch = [&](row_t row) {
         Fetched r;
         if constexpr (kKept) {
             r.x = at.fetch(a.kept_x, row);
             if (a.has_branch) r.f = at.fetch(a.kept_branch, row);
         } else {
-            r.x = at.fetch(static_cast<const E*>(a.x) + row * a.x_stride);
-            if (a.has_branch) r.f = at.fetch(static_cast<const E*>(a.branch) + row * a.branch_stride);
+            r.x = at.fetch(static_cast<const E*>(a.x) + offset_of(row, a.x_stride));
+            if (a.has_branch) r.f = at.fetch(static_cast<const E*>(a.branch) + offset_of(row, a.branch_stride));
         }
-        if (g.y != nullptr) r.dy = at.fetch(static_cast<const E*>(g.y) + row * g.y_stride);
-        if (g.n != nullptr) r.dn = at.fetch(static_cast<const E*>(g.n) + row * g.n_stride);
+        if (g.y != nullptr) r.dy = at.fetch(static_cast<const E*>(g.y) + offset_of(row, g.y_stride));
+        if (g.n != nullptr) r.dn = at.fetch(static_cast<const E*>(g.n) + offset_of(row, g.n_stride));
         return r;
     };
-    const auto one_row = [&](int64_t row, const Fetched& fetched) {
+    const auto one_row = [&](row_t row, const Fetched& fetched) {
         Values y, f, dy;
         float r_f = 1.0f;
         // p, computed twice: its registers would be held all the way
@@ -425,7 +430,7 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads, !kFull ? 4 : kLanes == 512 ?
         if (g.x != nullptr) {
             Values dx;
             PENC_EACH dx[i] = a.scale * dy[i];
-            at.store(static_cast<E*>(g.x) + row * a.channels, dx);
+            at.store(static_cast<E*>(g.x) + offset_of(row, a.channels), dx);
         }
         if (!a.has_branch) return;
         Values p;
@@ -447,32 +452,32 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads, !kFull ? 4 : kLanes == 512 ?
                 PENC_EACH dy[i] = r_f * (dy[i] - mean - f[i] * along);
             }
         }
-        if (g.branch != nullptr) at.store(static_cast<E*>(g.branch) + row * a.channels, dy);
+        if (g.branch != nullptr) at.store(static_cast<E*>(g.branch) + offset_of(row, a.channels), dy);
     };
 
-    const auto store_gate = [&](int64_t group, const Values& v) {
-        if (a.gate_fp32) at.store(static_cast<float*>(g.gate) + group * a.channels, v);
-        else at.store(static_cast<E*>(g.gate) + group * a.channels, v);
+    const auto store_gate = [&](row_t group, const Values& v) {
+        if (a.gate_fp32) at.store(static_cast<float*>(g.gate) + offset_of(group, a.channels), v);
+        else at.store(static_cast<E*>(g.gate) + offset_of(group, a.channels), v);
     };
-    const auto leave = [&](float* sums, int64_t at_row, const Values& v) {
-        if (sums != nullptr) write_sum<kLanes>(v, lds, [&](const Values& t) { at.store(sums + at_row * a.channels, t); });
+    const auto leave = [&](float* sums, row_t at_row, const Values& v) {
+        if (sums != nullptr) write_sum<kLanes>(v, lds, [&](const Values& t) { at.store(sums + offset_of(at_row, a.channels), t); });
     };
     // one gate, or gates by lanes: a workgroup has one unit of rows; else it has pieces of groups, one after the other
     const bool pieces = a.rows_per_gate != 0 && !a.gate_by_lanes;
-    const int64_t units = pieces ? a.rows / a.rows_per_gate * g.pieces : gridDim.x;
-    const int64_t run = a.gate_by_lanes ? a.rows_per_gate : 1;
-    for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-        int64_t group = unit * R::kRows + threadIdx.x / kLanes, first = group * run, end = a.rows, stride = static_cast<int64_t>(gridDim.x) * R::kRows;
+    const row_t units = pieces ? a.rows / a.rows_per_gate * g.pieces : gridDim.x;
+    const row_t run = a.gate_by_lanes ? a.rows_per_gate : 1;
+    for (row_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        row_t group = unit * R::kRows + threadIdx.x / kLanes, first = group * run, end = a.rows, stride = gridDim.x * R::kRows;
         if (pieces) {
             group = unit / g.pieces;
             first = group * a.rows_per_gate + unit % g.pieces * g.piece_rows;
             end = min(first + g.piece_rows, (group + 1) * a.rows_per_gate);
             first += threadIdx.x / kLanes;
             stride = R::kRows;
-            at.param(a.gate, a.gate_fp32, 1.0f, gate, group * a.channels);
+            at.param(a.gate, a.gate_fp32, 1.0f, gate, offset_of(group, a.channels));
         }
-        walk<kLanes>(first, end, run, stride, fetch, [&](int64_t row, bool begins, bool ends, const Fetched& fetched) {
-            if (a.gate_by_lanes && begins) at.param(a.gate, a.gate_fp32, 1.0f, gate, group * a.channels);
+        walk<kLanes>(first, end, run, stride, fetch, [&](row_t row, bool begins, bool ends, const Fetched& fetched) {
+            if (a.gate_by_lanes && begins) at.param(a.gate, a.gate_fp32, 1.0f, gate, offset_of(group, a.channels));
             one_row(row, fetched);
             if (!a.gate_by_lanes || !ends) return;
             if (g.gate != nullptr) store_gate(group, d_gate);

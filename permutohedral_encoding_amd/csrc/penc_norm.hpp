@@ -11,7 +11,8 @@
 namespace penc {
 
 struct NormArgs {
-    int64_t rows, rows_per_gate, x_stride, branch_stride;
+    row_t rows, rows_per_gate;
+    uint32_t x_stride, branch_stride;
     int channels;
     float scale, eps;
     bool layer, post_norm, pre_norm, has_branch, param_fp32, gate_fp32, gate_by_lanes;
@@ -24,11 +25,12 @@ inline bool is_full(const NormArgs& a) { return a.layer || a.post_bias != nullpt
 
 struct NormGrads {
     const void *y, *n;
-    int64_t y_stride, n_stride;
+    uint32_t y_stride, n_stride;
     void *x, *branch, *gate;
     float* gate_sums;              // a row for each workgroup (one gate) or piece of a group
     float* sums[4];                // a row for each workgroup: post weight, post bias, pre weight, pre bias; null where not wanted
-    int64_t pieces, piece_rows;    // of a group of rows that share a gate
+    uint32_t pieces;               // of a group of rows that share a gate
+    row_t piece_rows;
 };
 
 struct Sum {
@@ -41,11 +43,6 @@ struct SumPartials {
     Sum sums[5];
     int channels;
 };
-
-__device__ __forceinline__ int64_t group_of(int64_t row, int64_t rows_per_gate) {
-    if (((row | rows_per_gate) >> 32) == 0) return static_cast<uint32_t>(row) / static_cast<uint32_t>(rows_per_gate);
-    return row / rows_per_gate;
-}
 
 // How a row ends: in a whole chunk of 8 channels, in a part of one, or before the first is whole.
 enum RowEnd { kWholeChunks, kPartOfChunk, kNarrowRow };

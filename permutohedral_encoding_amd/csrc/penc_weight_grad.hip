@@ -460,7 +460,7 @@ WeightPlan weight_plan(int64_t rows, int64_t channels, int64_t outputs, int64_t 
 }
 
 bool bad_size(int64_t rows, int64_t channels, int64_t outputs) {
-    return rows < 0 || channels <= 0 || channels > PENC_MAX_CHANNELS || outputs <= 0 || outputs > PENC_MAX_CHANNELS || channels * outputs >= int64_t{1} << 31;
+    return bad_rows(rows) || channels <= 0 || channels > PENC_MAX_CHANNELS || outputs <= 0 || outputs > PENC_MAX_CHANNELS || channels * outputs >= int64_t{1} << 31;
 }
 
 template <class E>
