@@ -195,7 +195,7 @@ __device__ __forceinline__ int64_t item_of(const WeightGrad& a) {
 template <class E, int kWideO, int kWideC, int kWaves, bool kRagged>
 __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) {
     constexpr int kPieces = GradTile<E, kWideO>::kPieces;
-    __shared__ float lds[kWaves][16][16 * kWideC];
+    __shared__ float lds[kWaves][16 * kWideO][16 * kWideC];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, column = lane % 16, rows_at = lane / 16 * kLaneRows;
     const int64_t item = item_of(a);
     const int tile = static_cast<int>(item % (a.channel_tiles * a.output_tiles));
@@ -209,17 +209,28 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
 
     acc_t acc[kWideO][kWideC] = {}, bias_acc[kWideO] = {};
     const Frag ones = {{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}};
-    for (int64_t step = first + wave * kStep; step < last; step += kWaves * kStep) {
-        words_t<G::kWords> g[kLaneRows];
-        words_t<X::kWords> x[kLaneRows];
+    words_t<G::kWords> g[kLaneRows], g_ahead[kLaneRows];
+    words_t<X::kWords> x[kLaneRows], x_ahead[kLaneRows];
+    // (behind the last step: rows that are there)
+    const auto load = [&](int64_t step) {
         if constexpr (kRagged) {
             const int64_t row = step + rows_at;
-            G::load_ragged(g, static_cast<const E*>(a.grad) + row * a.grad_stride + o, a.grad_stride, last - row, a.outputs - o);
-            X::load_ragged(x, a.kept, row, last - row, c);
+            G::load_ragged(g_ahead, static_cast<const E*>(a.grad) + row * a.grad_stride + o, a.grad_stride, last - row, a.outputs - o);
+            X::load_ragged(x_ahead, a.kept, row, last - row, c);
         } else {
             const StepRows rows(step, rows_at, a.rows);
-            G::load(g, a.grad, a.grad_stride, rows, o);
-            X::load(x, a.kept, rows, c);
+            G::load(g_ahead, a.grad, a.grad_stride, rows, o);
+            X::load(x_ahead, a.kept, rows, c);
+        }
+    };
+    int64_t step = first + wave * kStep;
+    if (step < last) load(step);
+    for (; step < last; step += kWaves * kStep) {
+#pragma unroll
+        for (int j = 0; j < kLaneRows; ++j) g[j] = g_ahead[j], x[j] = x_ahead[j];
+        load(step + kWaves * kStep);
+        if (!kRagged && step + kStep > a.rows) {
+            const StepRows rows(step, rows_at, a.rows);
             skip_rows(g, rows.skip);
             skip_rows(x, rows.skip);
         }
@@ -241,22 +252,20 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
     // Lane (16 i + n) has rows 4 i .. 4 i + 3 of a result's column n.
     float* const sums = a.sums + split * a.outputs * a.channels;
 #pragma unroll
-    for (int t = 0; t < kWideO; ++t) {
-        if (t > 0) __syncthreads();
+    for (int t = 0; t < kWideO; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int s = 0; s < kWideC; ++s) lds[wave][lane / 16 * 4 + r][column * kWideC + s] = acc[t][s][r];
-        __syncthreads();
-        for (int i = threadIdx.x; i < 16 * 16 * kWideC; i += 64 * kWaves) {
-            const int m = i / (16 * kWideC), n = i % (16 * kWideC), from = o0 + m * kWideO;
-            if (from >= a.outputs) continue;
-            const int to = (kRagged ? from : G::column_of(from, a.outputs)) + t;
-            float total = lds[0][m][n];
+            for (int s = 0; s < kWideC; ++s) lds[wave][(lane / 16 * 4 + r) * kWideO + t][column * kWideC + s] = acc[t][s][r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256 * kWideO * kWideC; i += 64 * kWaves) {
+        const int m = i / (16 * kWideC), n = i % (16 * kWideC), from = o0 + m / kWideO * kWideO;
+        if (from >= a.outputs) break;
+        const int to = (kRagged ? from : G::column_of(from, a.outputs)) + m % kWideO;
+        float total = lds[0][m][n];
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) total += lds[w][m][n];
-            if (to < a.outputs && c0 + n < a.channels) sums[static_cast<int64_t>(to) * a.channels + c0 + n] = total;
-        }
+        for (int w = 1; w < kWaves; ++w) total += lds[w][m][n];
+        if (to < a.outputs && c0 + n < a.channels) sums[static_cast<int64_t>(to) * a.channels + c0 + n] = total;
     }
     if (!bias) return;
     __syncthreads();
@@ -264,12 +273,12 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
     for (int t = 0; t < kWideO; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            if (column == 0) lds[wave][lane / 16 * 4 + r][t] = bias_acc[t][r];
+            if (column == 0) lds[wave][0][(lane / 16 * 4 + r) * kWideO + t] = bias_acc[t][r];
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * kWideO; i += 64 * kWaves) {
         const int from = o0 + i / kWideO * kWideO, to = (kRagged ? from : G::column_of(from, a.outputs)) + i % kWideO;
-        float total = lds[0][i / kWideO][i % kWideO];
-        for (int w = 1; w < kWaves; ++w) total += lds[w][i / kWideO][i % kWideO];
+        float total = lds[0][0][i];
+        for (int w = 1; w < kWaves; ++w) total += lds[w][0][i];
         if (from < a.outputs && to < a.outputs) a.bias_sums[split * a.outputs + to] = total;
     }
 }
@@ -453,7 +462,7 @@ WeightPlan weight_plan(int64_t rows, int64_t channels, int64_t outputs, int64_t 
     p.channel_tiles = static_cast<int>((channels + p.block_c - 1) / p.block_c);
     const int64_t tiles = static_cast<int64_t>(p.output_tiles) * p.channel_tiles;
     const int64_t pieces = std::max<int64_t>(1, (rows + p.at_a_time - 1) / p.at_a_time);
-    const int64_t wanted = std::max<int64_t>(1, std::min(pieces, (p.block_o == 64 ? 512 : 256) / tiles));
+    const int64_t wanted = std::max<int64_t>(1, std::min(pieces, 256 / tiles));
     p.split_rows = (pieces + wanted - 1) / wanted * p.at_a_time;
     p.splits = static_cast<int>(std::max<int64_t>(1, (rows + p.split_rows - 1) / p.split_rows));
     return p;
