@@ -131,16 +131,20 @@ Tensor empty_rows(const Tensor& like, int64_t channels) {
 // ------------------------------------------------------------------------------------------
 // checkpoints
 
+// `count` checkpoints of rows in one piece of memory: the values of each, one behind the other, then the exponents of each.
 struct Checkpoint {
-    Tensor values, exponents;  // undefined: none
-    int8_t* q() const { return values.defined() ? static_cast<int8_t*>(values.data_ptr()) : nullptr; }
-    uint8_t* e() const { return exponents.defined() ? static_cast<uint8_t*>(exponents.data_ptr()) : nullptr; }
+    Tensor bytes;  // int8; undefined: none
+    int64_t rows = 0, channels = 0, count = 1;
+
+    int8_t* q(int64_t k = 0) const { return bytes.defined() ? static_cast<int8_t*>(bytes.data_ptr()) + k * rows * api.kept_pitch(channels) : nullptr; }
+    uint8_t* e(int64_t k = 0) const {
+        return bytes.defined() ? reinterpret_cast<uint8_t*>(q(count)) + k * rows * api.kept_blocks(channels) : nullptr;
+    }
+    static int64_t size(int64_t rows, int64_t channels, int64_t count) { return count * rows * (api.kept_pitch(channels) + api.kept_blocks(channels)); }
 };
 
-// Room for `count` checkpoints of rows, one behind the other.
 Checkpoint room_for(const Tensor& like, int64_t rows, int64_t channels, int64_t count = 1) {
-    return {at::empty({count * rows, api.kept_pitch(channels)}, like.options().dtype(at::kChar)),
-            at::empty({count * rows, api.kept_blocks(channels)}, like.options().dtype(at::kByte))};
+    return {at::empty({Checkpoint::size(rows, channels, count)}, like.options().dtype(at::kChar)), rows, channels, count};
 }
 
 Checkpoint keep(const Tensor& x, const char* name) {
@@ -158,7 +162,7 @@ Checkpoint keep(const Tensor& x, const char* name) {
 std::pair<Tensor, Tensor> weight_grad(const Checkpoint& kept, int64_t channels, const Tensor& grad, at::ScalarType result, bool bias) {
     const int type = type_of(grad.scalar_type(), "grad");
     const Rows g = rows_of(grad, "grad");
-    PENC_REQUIRE(g.n == kept.values.size(0), "grad should have a row for each of the ", kept.values.size(0), " rows kept, however it has sizes ", grad.sizes());
+    PENC_REQUIRE(g.n == kept.rows, "grad should have a row for each of the ", kept.rows, " rows kept, however it has sizes ", grad.sizes());
     const auto options = grad.options().dtype(result);
     Tensor weight = at::empty({g.channels, channels}, options), b;
     if (bias) b = at::empty({g.channels}, options);
@@ -249,7 +253,7 @@ struct LinearNode : public LayerNode {
 
     std::string name() const override { return "LayersLinearBackward"; }
     variable_list gradients(const variable_list& grads) override {
-        const std::vector<Tensor> t = unpacked();  // weight, values, exponents
+        const std::vector<Tensor> t = unpacked();  // weight, the checkpoint of x
         const Tensor g = (grads[0].scalar_type() == type ? grads[0] : grads[0].to(type)).reshape({-1, grads[0].size(-1)});
         const c10::DeviceGuard device(g.device());
         c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
@@ -257,7 +261,7 @@ struct LinearNode : public LayerNode {
         if (task_should_compute_output(0)) out[0] = at::mm(g, t[0]).view(x_sizes);
         const bool want_bias = has_bias && task_should_compute_output(2);
         if (task_should_compute_output(1) && t[1].defined())
-            std::tie(out[1], out[2]) = weight_grad({t[1], t[2]}, channels, g, type, want_bias);
+            std::tie(out[1], out[2]) = weight_grad({t[1], g.size(0), channels}, channels, g, type, want_bias);
         else if (want_bias)
             out[2] = at::sum(g, {0});
         return out;
@@ -289,7 +293,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const Tensor& bias) {
     node->x_sizes = x.sizes().vec();
     node->type = x.scalar_type();
     node->has_bias = bias.defined();
-    node->save({&weight, &kept.values, &kept.exponents});
+    node->save({&weight, &kept.bytes});
     torch::autograd::set_history(y, node);
     return y;
 }
@@ -303,7 +307,7 @@ struct ActivationNode : public LayerNode {
 
     std::string name() const override { return "LayersActivationBackward"; }
     variable_list gradients(const variable_list& grads) override {
-        const std::vector<Tensor> t = unpacked();  // x, or values and exponents
+        const std::vector<Tensor> t = unpacked();  // x, or its checkpoint
         const c10::DeviceGuard device(grads[0].device());
         variable_list out(1);
         out[0] = at::empty(sizes, grads[0].options().dtype(scalar_type_of(type)));
@@ -312,7 +316,7 @@ struct ActivationNode : public LayerNode {
         Rows x;
         Checkpoint kept;
         if (t[0].defined()) x = rows_of(t[0], "x");
-        else kept = {t[1], t[2]};
+        else kept = {t[1], rows, channels, gated ? 2 : 1};
         check(api.activation_backward(type, kind, gated, rows, channels, t[0].defined() ? x.data() : nullptr, x.stride, kept.q(), kept.e(), g.data(),
                                       g.stride, out[0].data_ptr(), current_stream(out[0].device())),
               "activation");
@@ -347,7 +351,7 @@ Tensor activation(const Tensor& x, int kind, bool gated, bool keep_8bit) {
     node->rows = rows, node->channels = channels;
     node->sizes = x.sizes().vec();
     const Tensor none;
-    node->save({keep_8bit ? &none : &x, &kept.values, &kept.exponents});
+    node->save({keep_8bit ? &none : &x, &kept.bytes});
     torch::autograd::set_history(y, node);
     return y;
 }
@@ -413,13 +417,13 @@ struct NormNode : public LayerNode {
 
     std::string name() const override { return "LayersResidualNormBackward"; }
     variable_list gradients(const variable_list& grads) override {
-        // x, branch (undefined where kept), their checkpoints, gate, post weight and bias, pre weight and bias
+        // x and branch, or (undefined) the checkpoints of both, gate, post weight and bias, pre weight and bias
         const std::vector<Tensor> t = unpacked();
         const auto scalar = scalar_type_of(type);
-        const Tensor gate = t[6].defined() ? t[6].contiguous() : Tensor();
+        const Tensor gate = t[3].defined() ? t[3].contiguous() : Tensor();
         Tensor params[4];
         for (int i = 0; i < 4; ++i)
-            if (t[7 + i].defined()) params[i] = t[7 + i].contiguous();
+            if (t[4 + i].defined()) params[i] = t[4 + i].contiguous();
         const Tensor& any = grads[0].defined() ? grads[0] : grads[1];
         const c10::DeviceGuard device(any.device());
         variable_list out(7);
@@ -427,7 +431,7 @@ struct NormNode : public LayerNode {
         if (task_should_compute_output(0)) out[0] = at::empty(sizes, options_of_rows);
         if (has_branch && task_should_compute_output(1)) out[1] = at::empty(sizes, options_of_rows);
         for (int i = 0; i < 5; ++i)
-            if (t[6 + i].defined() && task_should_compute_output(2 + i)) out[2 + i] = at::empty(t[6 + i].sizes(), t[6 + i].options());
+            if (t[3 + i].defined() && task_should_compute_output(2 + i)) out[2 + i] = at::empty(t[3 + i].sizes(), t[3 + i].options());
         if (rows == 0) {
             for (Tensor& o : out)
                 if (o.defined()) o.zero_();
@@ -437,9 +441,9 @@ struct NormNode : public LayerNode {
         n.has_branch = has_branch;
         Rows x, branch, gy, gn;
         if (options.keep_8bit) {
-            const auto q = [](const Tensor& v) { return v.defined() ? static_cast<int8_t*>(v.data_ptr()) : nullptr; };
-            const auto e = [](const Tensor& v) { return v.defined() ? static_cast<uint8_t*>(v.data_ptr()) : nullptr; };
-            n.x_values = q(t[2]), n.x_exponents = e(t[3]), n.branch_values = q(t[4]), n.branch_exponents = e(t[5]);
+            const Checkpoint kept{t[2], rows, channels, has_branch ? 2 : 1};
+            n.x_values = kept.q(), n.x_exponents = kept.e();
+            if (has_branch) n.branch_values = kept.q(1), n.branch_exponents = kept.e(1);
         } else {
             x = rows_of(t[0], "x");
             n.x = x.data(), n.x_stride = x.stride;
@@ -475,7 +479,7 @@ std::pair<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& branch, c
     const c10::DeviceGuard device(x.device());
     const bool differentiable = any_requires_grad({&x, &branch, &gate, &params[0], &params[1], &params[2], &params[3]});
     Tensor y, n;
-    Checkpoint kept_x, kept_branch;
+    Checkpoint kept;
     int64_t rows, channels, per_gate = 0;
     {
         at::NoGradGuard no_grad;
@@ -520,12 +524,9 @@ std::pair<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& branch, c
             a.x = r.data(), a.x_stride = r.stride;
             if (has_branch) a.branch = b.data(), a.branch_stride = b.stride;
             if (differentiable && o.keep_8bit) {
-                kept_x = room_for(x, rows, channels);
-                a.x_values = kept_x.q(), a.x_exponents = kept_x.e();
-                if (has_branch) {
-                    kept_branch = room_for(x, rows, channels);
-                    a.branch_values = kept_branch.q(), a.branch_exponents = kept_branch.e();
-                }
+                kept = room_for(x, rows, channels, has_branch ? 2 : 1);
+                a.x_values = kept.q(), a.x_exponents = kept.e();
+                if (has_branch) a.branch_values = kept.q(1), a.branch_exponents = kept.e(1);
             }
             check(api.residual_norm(&a, has_branch ? y.data_ptr() : nullptr, o.pre_norm ? n.data_ptr() : nullptr, current_stream(x.device())),
                   "residual_norm");
@@ -540,8 +541,7 @@ std::pair<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& branch, c
     node->has_branch = has_branch, node->has_y = has_branch;
     node->sizes = x.sizes().vec();
     const Tensor none;
-    node->save({o.keep_8bit ? &none : &x, o.keep_8bit ? &none : &branch, &kept_x.values, &kept_x.exponents, &kept_branch.values, &kept_branch.exponents,
-                &gate, &params[0], &params[1], &params[2], &params[3]});
+    node->save({o.keep_8bit ? &none : &x, o.keep_8bit ? &none : &branch, &kept.bytes, &gate, &params[0], &params[1], &params[2], &params[3]});
     if (y.defined()) torch::autograd::set_history(y, node);
     if (n.defined()) torch::autograd::set_history(n, node);
     return {y, n};
@@ -552,7 +552,7 @@ std::pair<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& branch, c
 
 Tensor optional_arg(PyObject* o, const char* name) { return o == Py_None ? Tensor() : tensor_arg(o, name); }
 
-// layers_keep(x) -> (values, exponents)
+// layers_keep(x) -> the checkpoint: int8, values and behind them exponents
 PyObject* py_keep(PyObject*, PyObject* x_arg) {
     return guarded([&]() -> PyObject* {
         TORCH_CHECK(api.keep != nullptr, "bind() has not been called");
@@ -565,47 +565,47 @@ PyObject* py_keep(PyObject*, PyObject* x_arg) {
             const c10::DeviceGuard device(x.device());
             kept = keep(x.detach(), "x");
         }
-        return Py_BuildValue("NN", THPVariable_Wrap(std::move(kept.values)), THPVariable_Wrap(std::move(kept.exponents)));
+        return THPVariable_Wrap(std::move(kept.bytes));
     });
 }
 
-void require_checkpoint(const Tensor& values, const Tensor& exponents, int64_t channels) {
-    require_plain({&values, &exponents});
-    PENC_REQUIRE(channels >= 1 && channels <= PENC_MAX_CHANNELS && values.scalar_type() == at::kChar && exponents.scalar_type() == at::kByte &&
-                     values.dim() == 2 && exponents.dim() == 2 && values.is_contiguous() && exponents.is_contiguous() &&
-                     values.size(0) == exponents.size(0) && values.size(1) == api.kept_pitch(channels) && exponents.size(1) == api.kept_blocks(channels),
-                 "not a checkpoint of rows of ", channels, " channels");
+Checkpoint checkpoint_of(const Tensor& bytes, int64_t rows, int64_t channels) {
+    require_plain({&bytes});
+    PENC_REQUIRE(rows >= 0 && channels >= 1 && channels <= PENC_MAX_CHANNELS && bytes.scalar_type() == at::kChar && bytes.dim() == 1 && bytes.is_contiguous() &&
+                     bytes.numel() == Checkpoint::size(rows, channels, 1),
+                 "not a checkpoint of ", rows, " rows of ", channels, " channels");
+    return {bytes, rows, channels};
 }
 
-// layers_restore(values, exponents, channels, type) -> (rows, channels)
+// layers_restore(checkpoint, rows, channels, type) -> (rows, channels)
 PyObject* py_restore(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
         TORCH_CHECK(n_args == 4, "layers_restore takes 4 arguments");
         TORCH_CHECK(api.keep != nullptr, "bind() has not been called");
-        const Checkpoint kept{tensor_arg(args[0], "values"), tensor_arg(args[1], "exponents")};
-        const int64_t channels = PyLong_AsLongLong(args[2]);
+        const Tensor& bytes = tensor_arg(args[0], "checkpoint");
+        const int64_t rows = PyLong_AsLongLong(args[1]), channels = PyLong_AsLongLong(args[2]);
         const long type = PyLong_AsLong(args[3]);
         if (PyErr_Occurred()) return nullptr;
         Tensor x;
         {
             NoGil no_gil;
             at::NoGradGuard no_grad;
-            require_checkpoint(kept.values, kept.exponents, channels);
-            const c10::DeviceGuard device(kept.values.device());
-            x = at::empty({kept.values.size(0), channels}, kept.values.options().dtype(scalar_type_of(type)));
-            check(api.restore(static_cast<int>(type), x.size(0), channels, kept.q(), kept.e(), x.data_ptr(), current_stream(x.device())), "unpack");
+            const Checkpoint kept = checkpoint_of(bytes, rows, channels);
+            const c10::DeviceGuard device(bytes.device());
+            x = at::empty({rows, channels}, bytes.options().dtype(scalar_type_of(type)));
+            check(api.restore(static_cast<int>(type), rows, channels, kept.q(), kept.e(), x.data_ptr(), current_stream(x.device())), "unpack");
         }
         return THPVariable_Wrap(std::move(x));
     });
 }
 
-// layers_weight_grad(values, exponents, channels, grad, bias, type) -> (weight gradient, bias gradient or None)
+// layers_weight_grad(checkpoint, rows, channels, grad, bias, type) -> (weight gradient, bias gradient or None)
 PyObject* py_weight_grad(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
         TORCH_CHECK(n_args == 6, "layers_weight_grad takes 6 arguments");
         TORCH_CHECK(api.keep != nullptr, "bind() has not been called");
-        const Checkpoint kept{tensor_arg(args[0], "values"), tensor_arg(args[1], "exponents")};
-        const int64_t channels = PyLong_AsLongLong(args[2]);
+        const Tensor& bytes = tensor_arg(args[0], "checkpoint");
+        const int64_t rows = PyLong_AsLongLong(args[1]), channels = PyLong_AsLongLong(args[2]);
         const Tensor& grad = tensor_arg(args[3], "grad");
         const int bias = PyObject_IsTrue(args[4]);
         const long type = PyLong_AsLong(args[5]);
@@ -614,8 +614,8 @@ PyObject* py_weight_grad(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         {
             NoGil no_gil;
             at::NoGradGuard no_grad;
-            require_checkpoint(kept.values, kept.exponents, channels);
-            require_plain({&kept.values, &grad});
+            const Checkpoint kept = checkpoint_of(bytes, rows, channels);
+            require_plain({&bytes, &grad});
             const c10::DeviceGuard device(grad.device());
             out = weight_grad(kept, channels, grad.detach(), scalar_type_of(type), bias != 0);
         }

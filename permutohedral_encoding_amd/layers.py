@@ -25,6 +25,10 @@ _ACTIVATIONS = {"gelu": 0, "silu": 1, "softplus": 2}
 _NORMS = {"rms": 0, "layer": 1}
 
 
+def _bridge():
+    return _native._bridge or _native.bridge()
+
+
 def _code(table, key, what):
     try:
         return table[key]
@@ -35,18 +39,31 @@ def _code(table, key, what):
 class Checkpoint:
     """A tensor ``(..., C)`` in 8 bits, made by :func:`checkpoint`.
 
-    ``values`` (int8, rows of C rounded up to 16) and ``exponents`` (uint8, one for each block of 32 channels): a value stands for
-    ``values * 2 ** (exponents - 127)``.  It is off by at most half a step, 1/127 of the largest magnitude in its block or less, and a block
-    with an infinity or a NaN comes back as NaN."""
+    A value stands for ``values * 2 ** (exponents - 127)``, with one exponent for each block of 32 channels of a row.  It is off by at most half a step, and a
+    step is at most 1/63 of the largest magnitude in the block; a block with an infinity or a NaN comes back as NaN."""
 
-    def __init__(self, values, exponents, shape, dtype):
-        self.values, self.exponents, self.shape, self.dtype = values, exponents, torch.Size(shape), dtype
+    __slots__ = ("data", "rows", "shape", "dtype")
+
+    def __init__(self, data, shape, dtype):
+        self.data, self.shape, self.dtype = data, shape, dtype
+        self.rows = shape.numel() // shape[-1]
+
+    @property
+    def values(self):
+        """int8, rows of C rounded up to 16 (the rest zero)."""
+        pitch = -(-self.shape[-1] // 16) * 16
+        return self.data[: self.rows * pitch].view(self.rows, pitch)
+
+    @property
+    def exponents(self):
+        """uint8, one for each block; 255 for one that is not finite."""
+        blocks = -(-self.shape[-1] // 32)
+        return self.data[self.data.numel() - self.rows * blocks:].view(torch.uint8).view(self.rows, blocks)
 
     def unpack(self, dtype=None):
         """The values that the checkpoint stands for, of the type of the tensor it was made of or of ``dtype`` (float16: at most 65504 in magnitude)."""
-        dtype = self.dtype if dtype is None else dtype
-        rows = _native.bridge().layers_restore(self.values, self.exponents, self.shape[-1], _code(_TYPES, dtype, "dtype"))
-        return rows.view(self.shape)
+        rows = _bridge().layers_restore(self.data, self.rows, self.shape[-1], _code(_TYPES, self.dtype if dtype is None else dtype, "dtype"))
+        return rows if len(self.shape) == 2 else rows.view(self.shape)
 
     def weight_grad(self, grad, bias=False, dtype=None):
         """What a linear layer with this input needs of the gradient ``(..., O)`` of its result: the gradient of its weight ``(O, C)``, the sum over the
@@ -54,20 +71,19 @@ class Checkpoint:
         if grad.shape[:-1] != self.shape[:-1]:
             raise ValueError(f"grad should have the rows of the tensor kept, {tuple(self.shape)}, however it has sizes {tuple(grad.shape)}")
         code = _code(_TYPES, grad.dtype if dtype is None else dtype, "dtype")
-        weight_grad, bias_grad = _native.bridge().layers_weight_grad(self.values, self.exponents, self.shape[-1], grad, bool(bias), code)
-        return (weight_grad, bias_grad) if bias else weight_grad
+        both = _bridge().layers_weight_grad(self.data, self.rows, self.shape[-1], grad, bias, code)
+        return both if bias else both[0]
 
 
 def checkpoint(x):
     """Keeps ``x`` in 8 bits: blocks of 32 channels of a row share a power of two as their step.  Outside of autograd: the
     functions below call it where they need it."""
-    values, exponents = _native.bridge().layers_keep(x)
-    return Checkpoint(values, exponents, x.shape, x.dtype)
+    return Checkpoint(_bridge().layers_keep(x), x.shape, x.dtype)
 
 
 def linear(x, weight, bias=None):
     """``torch.nn.functional.linear`` that keeps its input in 8 bits for the weight gradient.  ``x``, ``weight`` (O, C) and ``bias`` (O,) are of one type."""
-    return _native.bridge().layers_linear(x, weight, bias)
+    return _bridge().layers_linear(x, weight, bias)
 
 
 def activation(x, kind="gelu", gated=False, keep_8bit=True):
@@ -75,13 +91,13 @@ def activation(x, kind="gelu", gated=False, keep_8bit=True):
 
     ``kind``: "gelu" (``x Phi(x)``), "silu" (``x / (1 + exp(-x))``) or "softplus" (``log(1 + exp(x))``).  ``keep_8bit=False`` keeps ``x`` itself for the
     backward."""
-    return _native.bridge().layers_activation(x, _code(_ACTIVATIONS, kind, "kind"), gated, keep_8bit)
+    return _bridge().layers_activation(x, _code(_ACTIVATIONS, kind, "kind"), gated, keep_8bit)
 
 
 def norm(x, weight=None, bias=None, kind="rms", eps=1e-6, keep_8bit=True):
     """``x / sqrt(mean(x^2) + eps) * weight + bias`` over the channels ("rms"), or that of ``x - mean(x)`` ("layer").  At most 8192 channels; parameters
     are of the type of ``x`` or float32."""
-    return _native.bridge().layers_residual_norm(x, None, None, None, None, weight, bias, 1.0, False, True, _code(_NORMS, kind, "kind"), eps, keep_8bit)[1]
+    return _bridge().layers_residual_norm(x, None, None, None, None, weight, bias, 1.0, False, True, _code(_NORMS, kind, "kind"), eps, keep_8bit)[1]
 
 
 def residual_norm(x, branch, gate=None, residual_scale=1.0, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, post_norm=True, pre_norm=True,
@@ -94,6 +110,6 @@ def residual_norm(x, branch, gate=None, residual_scale=1.0, post_weight=None, po
     ``rows / groups`` consecutive rows.  The norms are those of :func:`norm`, ``n`` is of ``y`` before it is rounded."""
     if branch is None:
         raise ValueError("residual_norm should have a branch (layers.norm is the norm of a tensor alone)")
-    y, n = _native.bridge().layers_residual_norm(x, branch, gate, post_weight, post_bias, pre_weight, pre_bias, residual_scale, post_norm, pre_norm,
+    y, n = _bridge().layers_residual_norm(x, branch, gate, post_weight, post_bias, pre_weight, pre_bias, residual_scale, post_norm, pre_norm,
                                                  _code(_NORMS, kind, "kind"), eps, keep_8bit)
     return (y, n) if pre_norm else y
