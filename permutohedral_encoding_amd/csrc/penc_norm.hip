@@ -511,6 +511,7 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(SumPartials s) {
     float total = 0.0f;
     if (c < s.channels) {
         const float* const from = sum.from + group * sum.rows * s.channels + c;
+#pragma unroll 8
         for (int64_t r = strand; r < sum.rows; r += 32) total += from[r * s.channels];
     }
     lds[strand][threadIdx.x % 32] = total;
