@@ -78,7 +78,7 @@ void require_plain(std::initializer_list<const Tensor*> tensors) {
         if (!t->defined()) continue;
         TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), "forward-mode differentiation of the layers is not implemented");
         PENC_REQUIRE(t->is_cuda(), "the layers' tensors should be in GPU memory. Please call .cuda() on the tensor");
-        PENC_REQUIRE(t->layout() == at::kStrided, "the layers take dense tensors");
+        PENC_REQUIRE(t->layout() == at::kStrided && !t->is_neg() && !t->_is_zerotensor(), "the layers take dense tensors that are in memory as they are");
         if (first == nullptr) first = t;
         PENC_REQUIRE(t->device() == first->device(), "the layers' tensors must be on the same device");
     }
@@ -240,6 +240,17 @@ std::shared_ptr<N> make_node() {
     return std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
 }
 
+// What hooks on saved tensors may have brought back in another form.
+Checkpoint saved_checkpoint(const Tensor& bytes, int64_t rows, int64_t channels, int64_t count) {
+    TORCH_CHECK(bytes.defined() && bytes.is_cuda() && bytes.scalar_type() == at::kChar && bytes.is_contiguous() &&
+                    bytes.numel() == Checkpoint::size(rows, channels, count),
+                "a checkpoint saved for the backward has come back in another form");
+    return {bytes, rows, channels, count};
+}
+void require_saved(const Tensor& t, c10::IntArrayRef sizes, at::ScalarType type) {
+    TORCH_CHECK(t.defined() && t.is_cuda() && t.sizes() == sizes && t.scalar_type() == type, "a tensor saved for the backward has come back in another form");
+}
+
 // The gradient of a result as rows of the result's type (autograd has brought it to the result's sizes).
 Rows grad_rows(const Tensor& g, at::ScalarType type) { return rows_of(g.scalar_type() == type ? g.detach() : g.detach().to(type), "the gradient"); }
 
@@ -260,10 +271,8 @@ struct LinearNode : public LayerNode {
         variable_list out(3);
         if (task_should_compute_output(0)) out[0] = at::mm(g, t[0]).view(x_sizes);
         const bool want_bias = has_bias && task_should_compute_output(2);
-        if (task_should_compute_output(1) && t[1].defined())
-            std::tie(out[1], out[2]) = weight_grad({t[1], g.size(0), channels}, channels, g, type, want_bias);
-        else if (want_bias)
-            out[2] = at::sum(g, {0});
+        if (t[1].defined() && (task_should_compute_output(1) || want_bias))
+            std::tie(out[1], out[2]) = weight_grad(saved_checkpoint(t[1], g.size(0), channels, 1), channels, g, type, want_bias);
         return out;
     }
 };
@@ -284,7 +293,8 @@ Tensor linear(const Tensor& x, const Tensor& weight, const Tensor& bias) {
         at::NoGradGuard no_grad;
         c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
         y = at::linear(x, weight, bias);
-        if (differentiable && weight.requires_grad()) kept = keep(x.detach(), "x");
+        // (for the bias alone too: its sum comes with the weight's)
+        if (differentiable && (weight.requires_grad() || (bias.defined() && bias.requires_grad()))) kept = keep(x.detach(), "x");
     }
     if (!differentiable) return y;
     auto node = make_node<LinearNode>();
@@ -302,6 +312,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const Tensor& bias) {
 
 struct ActivationNode : public LayerNode {
     int kind = 0, type = 0, gated = 0;
+    bool keep_8bit = true;
     int64_t rows = 0, channels = 0;
     std::vector<int64_t> sizes;  // of x
 
@@ -315,9 +326,13 @@ struct ActivationNode : public LayerNode {
         const Rows g = grad_rows(grads[0], scalar_type_of(type));
         Rows x;
         Checkpoint kept;
-        if (t[0].defined()) x = rows_of(t[0], "x");
-        else kept = {t[1], rows, channels, gated ? 2 : 1};
-        check(api.activation_backward(type, kind, gated, rows, channels, t[0].defined() ? x.data() : nullptr, x.stride, kept.q(), kept.e(), g.data(),
+        if (keep_8bit) {
+            kept = saved_checkpoint(t[1], rows, channels, gated ? 2 : 1);
+        } else {
+            require_saved(t[0], sizes, scalar_type_of(type));
+            x = rows_of(t[0], "x");
+        }
+        check(api.activation_backward(type, kind, gated, rows, channels, keep_8bit ? nullptr : x.data(), x.stride, kept.q(), kept.e(), g.data(),
                                       g.stride, out[0].data_ptr(), current_stream(out[0].device())),
               "activation");
         return out;
@@ -347,7 +362,7 @@ Tensor activation(const Tensor& x, int kind, bool gated, bool keep_8bit) {
     if (!differentiable) return y;
     auto node = make_node<ActivationNode>();
     node->set_next_edges(torch::autograd::collect_next_edges(x));
-    node->kind = kind, node->type = type, node->gated = gated;
+    node->kind = kind, node->type = type, node->gated = gated, node->keep_8bit = keep_8bit;
     node->rows = rows, node->channels = channels;
     node->sizes = x.sizes().vec();
     const Tensor none;
@@ -413,13 +428,18 @@ struct NormNode : public LayerNode {
     int type = 0;
     int64_t rows = 0, channels = 0, per_gate = 0;
     bool has_branch = false, has_y = false;
-    std::vector<int64_t> sizes;
+    std::vector<int64_t> sizes, param_sizes[5];  // of x; of the gate, weights and biases
+    at::ScalarType param_types[5] = {};
 
     std::string name() const override { return "LayersResidualNormBackward"; }
     variable_list gradients(const variable_list& grads) override {
         // x and branch, or (undefined) the checkpoints of both, gate, post weight and bias, pre weight and bias
         const std::vector<Tensor> t = unpacked();
         const auto scalar = scalar_type_of(type);
+        for (int i = 0; i < 5; ++i) {
+            TORCH_CHECK(t[3 + i].defined() == (param_sizes[i].size() != 0), "a parameter saved for the backward has not come back");
+            if (t[3 + i].defined()) require_saved(t[3 + i], param_sizes[i], param_types[i]);
+        }
         const Tensor gate = t[3].defined() ? t[3].contiguous() : Tensor();
         Tensor params[4];
         for (int i = 0; i < 4; ++i)
@@ -441,10 +461,12 @@ struct NormNode : public LayerNode {
         n.has_branch = has_branch;
         Rows x, branch, gy, gn;
         if (options.keep_8bit) {
-            const Checkpoint kept{t[2], rows, channels, has_branch ? 2 : 1};
+            const Checkpoint kept = saved_checkpoint(t[2], rows, channels, has_branch ? 2 : 1);
             n.x_values = kept.q(), n.x_exponents = kept.e();
             if (has_branch) n.branch_values = kept.q(1), n.branch_exponents = kept.e(1);
         } else {
+            require_saved(t[0], sizes, scalar);
+            if (has_branch) require_saved(t[1], sizes, scalar);
             x = rows_of(t[0], "x");
             n.x = x.data(), n.x_stride = x.stride;
             if (has_branch) {
@@ -540,6 +562,10 @@ std::pair<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& branch, c
     node->rows = rows, node->channels = channels, node->per_gate = per_gate;
     node->has_branch = has_branch, node->has_y = has_branch;
     node->sizes = x.sizes().vec();
+    for (int i = 0; i < 5; ++i) {
+        const Tensor& p = i == 0 ? gate : params[i - 1];
+        if (p.defined()) node->param_sizes[i] = p.sizes().vec(), node->param_types[i] = p.scalar_type();
+    }
     const Tensor none;
     node->save({o.keep_8bit ? &none : &x, o.keep_8bit ? &none : &branch, &kept.bytes, &gate, &params[0], &params[1], &params[2], &params[3]});
     if (y.defined()) torch::autograd::set_history(y, node);
@@ -667,6 +693,7 @@ PyObject* py_residual_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) 
         const Tensor params[4] = {optional_arg(args[3], "post_weight"), optional_arg(args[4], "post_bias"), optional_arg(args[5], "pre_weight"),
                                   optional_arg(args[6], "pre_bias")};
         NormOptions o;
+        PENC_REQUIRE(!THPVariable_Check(args[7]) && !THPVariable_Check(args[11]), "residual_scale and eps should be numbers: they have no gradient");
         o.scale = PyFloat_AsDouble(args[7]);
         o.post_norm = PyObject_IsTrue(args[8]) == 1, o.pre_norm = PyObject_IsTrue(args[9]) == 1;
         o.kind = static_cast<int>(PyLong_AsLong(args[10]));

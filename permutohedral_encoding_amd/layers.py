@@ -12,7 +12,7 @@ needs in 8 bits a value (a quarter of fp32) and are one pass over memory in eith
 All of them take float32, float16 or bfloat16 tensors ``(..., C)`` in GPU memory, on the current stream of the tensor's device, of any strides (rows whose
 channels are adjacent are read in place, as is the encoding's own result).  Sums and statistics are float32, results are rounded once, and
 every call gives the same result for the same inputs.  Every backward is the gradient of the forward at the values that the checkpoint stands for; it can
-be captured in a graph, and cannot be differentiated again (an eikonal loss needs layers that can).  There is no CPU path.
+be captured in a graph, and cannot be differentiated again (an eikonal loss needs layers that can).  Autocast does not apply to them.  There is no CPU path.
 """
 import torch
 
@@ -82,7 +82,7 @@ def checkpoint(x):
 
 
 def linear(x, weight, bias=None):
-    """``torch.nn.functional.linear`` that keeps its input in 8 bits for the weight gradient.  ``x``, ``weight`` (O, C) and ``bias`` (O,) are of one type."""
+    """``torch.nn.functional.linear`` that keeps its input in 8 bits for the gradients of weight and bias.  ``x``, ``weight`` (O, C) and ``bias`` (O,) are of one type."""
     return _bridge().layers_linear(x, weight, bias)
 
 
@@ -104,7 +104,7 @@ def residual_norm(x, branch, gate=None, residual_scale=1.0, post_weight=None, po
                   kind="rms", eps=1e-6, keep_8bit=True):
     """What stands between a block and the next one, in one pass: ``y = residual_scale * x + gate * norm(branch)`` and ``n = norm(y)``.
 
-    ``x`` is the residual stream, ``branch`` (same sizes and type) what the block made of it; the result is ``(y, n)``, or ``y`` with ``pre_norm=False``.
+    ``x`` is the residual stream, ``branch`` (same sizes and type) what the block made of it, ``residual_scale`` a number; the result is ``(y, n)``, or ``y`` with ``pre_norm=False``.
     ``post_norm=False`` takes the branch as it is.  ``gate`` (None: 1) has sizes ``(C,)`` for all rows, those of ``x`` with trailing ones before the channels
     (a gate for each row, or for each ray of ``(rays, samples, C)``: ``(rays, 1, C)``), or ``(groups, C)`` for ``x`` of ``(rows, C)``, each for
     ``rows / groups`` consecutive rows.  The norms are those of :func:`norm`, ``n`` is of ``y`` before it is rounded."""

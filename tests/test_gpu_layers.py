@@ -205,7 +205,7 @@ def test_activations_far_out():
 
 # ------------------------------------------------------------------------------------------ norms
 
-NORM_SHAPES = [(1, 1), (3, 8), (7, 31), (129, 64), (65, 100), (33, 203), (50, 512), (9, 1000), (5, 1024), (6, 2048), (3, 2051), (5, 4096), (4, 8192), (2, 8191)]
+NORM_SHAPES = [(1, 1), (5, 3), (300, 7), (3, 8), (2, 9), (7, 31), (129, 64), (65, 100), (33, 203), (50, 512), (9, 1000), (5, 1024), (6, 2048), (3, 2051), (5, 4096), (4, 8192), (2, 8191)]
 
 
 def norm_case(rows, channels, dtype, params, kind, gate, seed=0):
@@ -355,6 +355,7 @@ def test_what_a_norm_refuses():
                  lambda: layers.residual_norm(x, f, gate=w.half()), lambda: layers.norm(x, w.view(1, 24)), lambda: layers.norm(torch.zeros(2, 8193, device="cuda")),
                  lambda: layers.norm(x, w.cpu()), lambda: layers.activation(x[:, :23], gated=True), lambda: layers.linear(x, torch.ones(3, 24, device="cuda")),
                  lambda: layers.linear(x, x[:, :23]), lambda: layers.linear(x, x, x[0, :5]), lambda: layers.checkpoint(x).weight_grad(f[:3]),
+                 lambda: layers.residual_norm(x, f, residual_scale=w[0]), lambda: layers.norm(x, eps=w[0]), lambda: layers.norm(torch._neg_view(x)),
                  lambda: layers.checkpoint(x).unpack(torch.float64), lambda: layers.checkpoint(x).weight_grad(f, dtype=torch.int8)):
         with pytest.raises(ValueError):
             call()
@@ -533,6 +534,12 @@ def test_what_autograd_checks():
     with torch.autograd.graph.saved_tensors_hooks(lambda t: (seen.append(t.dtype), t.cpu())[1], lambda t: t.cuda()):
         y = layers.norm(x, w).sum()
     assert torch.int8 in seen and all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, (x, w))))
+    for back in (lambda t: t.cuda()[:-1], lambda t: t.cuda().to(torch.float64)):  # a hook that brings something else back
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), back):
+            ys = layers.norm(x, w).sum(), layers.activation(x).sum(), layers.activation(x, keep_8bit=False).sum()
+        for y in ys:
+            with pytest.raises(RuntimeError, match="another form"):
+                y.backward()
     # gradients of broadcast results
     a = torch.autograd.grad(layers.activation(x).sum(), x)[0]
     assert torch.equal(a, torch.autograd.grad(layers.activation(x), x, torch.ones(20, 32, device="cuda"))[0])
