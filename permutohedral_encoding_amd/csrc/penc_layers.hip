@@ -53,19 +53,21 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(Lanes l, const E* __rest
     });
 }
 
-// The encoding's own result: channels of consecutive rows next to each other.  A lane has a row and walks over its blocks, reading 32 channels,
-// each with the 63 lanes beside it.  kStaged: rows of up to 128 channels wait in the LDS and are written whole, one after the other: 1000003 x 48 fp32
-// 48.7 us without, 38.6 with; 2^20 x 48 54 and 50 (channels 4 MiB apart meet in the same memory channels).
-constexpr int kMostStaged = 128;
-template <class E, bool kStaged>
+// The encoding's own result: channels of consecutive rows next to each other.  A workgroup has kThreads rows and up to 128 of their channels: a lane has a
+// row and walks over its blocks, reading 32 channels, each with the 63 lanes beside it, and what it makes of them waits in the LDS until all rows' can be
+// written one after the other.  (Written by the lanes themselves, 16 bytes a row: 1000003 x 48 fp32 48.7 us instead of 38.6; 2^20 x 48 54 instead of 50, where
+// channels 4 MiB apart meet in the same memory channels.)
+constexpr int kPiece = 128;
+template <class E>
 __global__ __launch_bounds__(kThreads) void pack_channels_kernel(row_t rows, int channels, const E* __restrict__ x, int64_t stride, KeptArray kept) {
     extern __shared__ uint4 staged[];  // the rows, and behind them their exponents
-    uint8_t* const staged_exponents = reinterpret_cast<uint8_t*>(staged) + kThreads * kept.pitch;
+    const int begin = blockIdx.y * kPiece;
+    const uint32_t pitch = min(static_cast<uint32_t>(kPiece), kept.pitch - begin), blocks = min(static_cast<uint32_t>(kPiece / kKeptBlock), kept.blocks - begin / kKeptBlock);
+    uint8_t* const exponents = reinterpret_cast<uint8_t*>(staged) + kThreads * pitch;
     const row_t row0 = blockIdx.x * kThreads, row = row0 + threadIdx.x;
-    int8_t* const values = kStaged ? reinterpret_cast<int8_t*>(staged) + threadIdx.x * kept.pitch : kept.values + offset_of(row, kept.pitch);
-    uint8_t* const exponents = kStaged ? staged_exponents + threadIdx.x * kept.blocks : kept.exponents + offset_of(row, kept.blocks);
     if (row < rows) {
-        for (int first = 0; first < channels; first += kKeptBlock) {
+        for (uint32_t block = 0; block < blocks; ++block) {
+            const int first = begin + block * kKeptBlock;
             float v[kKeptBlock];
 #pragma unroll
             for (int i = 0; i < kKeptBlock; ++i) v[i] = first + i < channels ? static_cast<float>(x[(first + i) * stride + row]) : 0.0f;
@@ -76,21 +78,20 @@ __global__ __launch_bounds__(kThreads) void pack_channels_kernel(row_t rows, int
             s.saturate(v);
 #pragma unroll
             for (int i = 0; i < kKeptBlock; i += 16) {
-                if (first + i >= static_cast<int>(kept.pitch)) break;
+                if (block * kKeptBlock + i >= pitch) break;
                 uint4 q;
                 q.x = s.quantised(v + i), q.y = s.quantised(v + i + 4), q.z = s.quantised(v + i + 8), q.w = s.quantised(v + i + 12);
-                *reinterpret_cast<uint4*>(values + first + i) = q;
+                staged[(threadIdx.x * pitch + block * kKeptBlock + i) / 16] = q;
             }
-            exponents[first / kKeptBlock] = static_cast<uint8_t>(s.exponent);
+            exponents[threadIdx.x * blocks + block] = static_cast<uint8_t>(s.exponent);
         }
     }
-    if constexpr (kStaged) {
-        __syncthreads();
-        const uint32_t n = min(static_cast<uint32_t>(kThreads), rows - row0);
-        uint4* const to = reinterpret_cast<uint4*>(kept.values + offset_of(row0, kept.pitch));
-        for (uint32_t i = threadIdx.x; i < n * kept.pitch / 16; i += kThreads) to[i] = staged[i];
-        for (uint32_t i = threadIdx.x; i < n * kept.blocks; i += kThreads) kept.exponents[offset_of(row0, kept.blocks) + i] = staged_exponents[i];
-    }
+    __syncthreads();
+    const uint32_t n = min(static_cast<uint32_t>(kThreads), rows - row0), vectors = pitch / 16;
+    for (uint32_t i = threadIdx.x; i < n * vectors; i += kThreads)
+        *reinterpret_cast<uint4*>(kept.values + offset_of(row0 + i / vectors, kept.pitch) + begin + i % vectors * 16) = staged[i];
+    for (uint32_t i = threadIdx.x; i < n * blocks; i += kThreads)
+        kept.exponents[offset_of(row0 + i / blocks, kept.blocks) + begin / kKeptBlock + i % blocks] = exponents[i];
 }
 
 template <class E>
@@ -280,13 +281,12 @@ int penc_keep(int type, int64_t rows, int64_t channels, const void* x, int64_t r
             hipLaunchKernelGGL(pack_kernel<E>, dim3(l.grid), dim3(kThreads), 0, static_cast<hipStream_t>(stream), l, static_cast<const E*>(x),
                                static_cast<uint32_t>(row_stride), kept);
         } else {
-            const int64_t groups = (rows + kThreads - 1) / kThreads;
-            const auto launch = [&](auto kernel, uint32_t lds) {
-                hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(kThreads), lds, static_cast<hipStream_t>(stream), static_cast<row_t>(rows),
-                                   static_cast<int>(channels), static_cast<const E*>(x), channel_stride, kept);
-            };
-            if (kept.pitch <= kMostStaged) launch(pack_channels_kernel<E, true>, kThreads * (kept.pitch + kept.blocks));
-            else launch(pack_channels_kernel<E, false>, 0);
+            const int64_t groups = (rows + kThreads - 1) / kThreads, pieces = (channels + kPiece - 1) / kPiece;
+            if (pieces > 0xFFFF) return PENC_ERR_BAD_LAYER_SIZE;
+            const uint32_t lds = kThreads * (std::min<uint32_t>(kPiece, kept.pitch) + std::min<uint32_t>(kPiece / kKeptBlock, kept.blocks));
+            hipLaunchKernelGGL(pack_channels_kernel<E>, dim3(static_cast<unsigned>(groups), static_cast<unsigned>(pieces)), dim3(kThreads), lds,
+                               static_cast<hipStream_t>(stream), static_cast<row_t>(rows), static_cast<int>(channels), static_cast<const E*>(x), channel_stride,
+                               kept);
         }
         return launched();
     });

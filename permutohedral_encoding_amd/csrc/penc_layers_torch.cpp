@@ -152,7 +152,7 @@ Checkpoint keep(const Tensor& x, const char* name) {
     PENC_REQUIRE(x.dim() >= 1 && x.size(-1) >= 1, name, " should have at least one channel, however it has sizes ", x.sizes());
     PENC_REQUIRE(x.size(-1) <= PENC_MAX_CHANNELS, name, " has more than ", PENC_MAX_CHANNELS, " channels");
     // the encoding's own result: channels of consecutive rows side by side
-    const bool by_channels = x.dim() == 2 && x.size(0) > 1 && x.size(1) > 1 && x.stride(0) == 1 && x.stride(1) >= x.size(0);
+    const bool by_channels = x.dim() == 2 && x.size(0) > 1 && x.size(1) > 1 && x.size(1) <= (1 << 22) && x.stride(0) == 1 && x.stride(1) >= x.size(0);
     const Rows r = by_channels ? Rows{x, x.size(0), x.size(1), 1} : rows_of(x, name);
     Checkpoint kept = room_for(x, r.n, r.channels);
     check(api.keep(type, r.n, r.channels, r.data(), r.stride, by_channels ? x.stride(1) : 1, kept.q(), kept.e(), current_stream(x.device())), "checkpoint");
