@@ -23,6 +23,7 @@ namespace penc {
 namespace {
 
 constexpr int kStep = 32;  // rows of a matrix instruction
+constexpr int kLargeBlock = 256;
 constexpr int kLaneRows = 8;
 
 using frag_t = bf16_t __attribute__((ext_vector_type(8)));
@@ -181,7 +182,23 @@ struct WeightGrad {
     KeptArray kept;
     const void* grad;
     float *sums, *bias_sums;  // [splits][outputs][channels], [splits][outputs] or null
+    void *weight, *bias;      // where the rows are not split, the results themselves (else null), of `type`
+    int type;
 };
+
+// A workgroup's sum of result `at`, of the weight or the bias.
+__device__ __forceinline__ void leave(float* sums, void* result, int type, int64_t n, int64_t split, int64_t at, float total) {
+    if (result == nullptr) sums[split * n + at] = total;
+    else if (type == PENC_FP32) static_cast<float*>(result)[at] = total;
+    else if (type == PENC_FP16) static_cast<half_t*>(result)[at] = static_cast<half_t>(total);
+    else static_cast<bf16_t*>(result)[at] = static_cast<bf16_t>(total);
+}
+__device__ __forceinline__ void leave_weight(const WeightGrad& a, int64_t split, int output, int channel, float total) {
+    leave(a.sums, a.weight, a.type, static_cast<int64_t>(a.outputs) * a.channels, split, static_cast<int64_t>(output) * a.channels + channel, total);
+}
+__device__ __forceinline__ void leave_bias(const WeightGrad& a, int64_t split, int output, float total) {
+    leave(a.bias_sums, a.bias, a.type, a.outputs, split, output, total);
+}
 
 // The work of a workgroup.  Consecutive workgroups go to the 8 dies in turn: each of them gets neighbouring items, tiles of the same rows, which its cache
 // then holds.
@@ -204,7 +221,7 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
     using G = GradTile<E, kWideO>;
     using X = KeptTile<kWideC>;
     const int c = X::column_of(c0 + column * kWideC, a.kept), o = kRagged ? o0 + column * kWideO : G::column_of(o0 + column * kWideO, a.outputs);
-    const bool bias = a.bias_sums != nullptr && c0 == 0;
+    const bool bias = (a.bias_sums != nullptr || a.bias != nullptr) && c0 == 0;
     const int64_t first = split * a.split_rows, last = min(first + a.split_rows, a.rows);
 
     acc_t acc[kWideO][kWideC] = {}, bias_acc[kWideO] = {};
@@ -250,7 +267,6 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
         }
     }
     // Lane (16 i + n) has rows 4 i .. 4 i + 3 of a result's column n.
-    float* const sums = a.sums + split * a.outputs * a.channels;
 #pragma unroll
     for (int t = 0; t < kWideO; ++t)
 #pragma unroll
@@ -265,7 +281,7 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
         float total = lds[0][m][n];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) total += lds[w][m][n];
-        if (to < a.outputs && c0 + n < a.channels) sums[static_cast<int64_t>(to) * a.channels + c0 + n] = total;
+        if (to < a.outputs && c0 + n < a.channels) leave_weight(a, split, to, c0 + n, total);
     }
     if (!bias) return;
     __syncthreads();
@@ -279,15 +295,16 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
         const int from = o0 + i / kWideO * kWideO, to = (kRagged ? from : G::column_of(from, a.outputs)) + i % kWideO;
         float total = lds[0][0][i];
         for (int w = 1; w < kWaves; ++w) total += lds[w][0][i];
-        if (from < a.outputs && to < a.outputs) a.bias_sums[split * a.outputs + to] = total;
+        if (from < a.outputs && to < a.outputs) leave_bias(a, split, to, total);
     }
 }
 
-// The same for products that the matrix cores bound: kBlockO outputs by kBlockC channels to a workgroup of 8 waves, which bring 32 kSteps rows at a time
+// The same for products that the matrix cores bound: 256 outputs by 256 channels to a workgroup of 8 waves, which bring 32 kSteps rows at a time
 // into the LDS as the matrix instruction takes them, half of the waves the gradient and half the checkpoint (one of either kind on each SIMD), while all of
 // them multiply what was brought before.  Every value is converted once for the workgroup, and a wave's 4 x 8 tiles multiply a fragment 2.7 times.
-template <class E, int kBlockO, int kBlockC, int kSteps, int kWavesO>
+template <class E, int kSteps>
 __global__ __launch_bounds__(512, 2) void weight_grad_lds_kernel(WeightGrad a) {
+    constexpr int kBlockO = kLargeBlock, kBlockC = kLargeBlock, kWavesO = 4;
     constexpr int kPieces = GradTile<E, 4>::kPieces, kWavesC = 8 / kWavesO;
     constexpr int kWideO = kBlockO * kSteps / 64, kWideC = kBlockC * kSteps / 64;  // four waves bring each side
     constexpr int kTilesO = kBlockO / 16 / kWavesO, kTilesC = kBlockC / 16 / kWavesC;
@@ -312,7 +329,7 @@ __global__ __launch_bounds__(512, 2) void weight_grad_lds_kernel(WeightGrad a) {
     const int first_o = wave % kWavesO * kTilesO, first_c = wave / kWavesO * kTilesC;  // this wave's tiles
     // the bias is one more column, of ones: the waves with the same outputs have some of them each
     constexpr int kBias = (kTilesO + kWavesC - 1) / kWavesC;
-    const bool bias = a.bias_sums != nullptr && c0 == 0;
+    const bool bias = (a.bias_sums != nullptr || a.bias != nullptr) && c0 == 0;
     const int first_bias = wave / kWavesO * kBias;
     const Frag ones = {{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}};
     acc_t acc[kTilesO][kTilesC] = {}, bias_acc[kBias] = {};
@@ -392,28 +409,47 @@ __global__ __launch_bounds__(512, 2) void weight_grad_lds_kernel(WeightGrad a) {
         if (bias) walk(std::false_type{}, std::true_type{});
         else walk(std::false_type{}, std::false_type{});
     }
-    // Lane (16 i + n) has rows 4 i .. 4 i + 3 of a result's column n; tile T's row m is output (T / kWide * 16 + m) * kWide + T % kWide.
-    float* const sums = a.sums + split * a.outputs * a.channels;
+    // Lane (16 i + n) has rows 4 i .. 4 i + 3 of a result's column n; tile T's row m is output (T / kWide * 16 + m) * kWide + T % kWide, and kWideC tiles
+    // have neighbouring channels.
+    static_assert(kTilesC % kWideC == 0, "a wave has whole groups of neighbouring channels");
+    const auto write = [&](auto* to, auto* to_bias) {
+        using To = std::remove_pointer_t<decltype(to)>;
+        using Wide = To __attribute__((ext_vector_type(kWideC), aligned(sizeof(To))));
 #pragma unroll
-    for (int t = 0; t < kTilesO; ++t)
+        for (int t = 0; t < kTilesO; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int big = first_o + t, from = o0 + (big / kWideO * 16 + lane / 16 * 4 + r) * kWideO, to = G::column_of(from, a.outputs) + big % kWideO;
-            if (from >= a.outputs) continue;
+            for (int r = 0; r < 4; ++r) {
+                const int big = first_o + t, from = o0 + (big / kWideO * 16 + lane / 16 * 4 + r) * kWideO;
+                if (from >= a.outputs) continue;
+                To* const row = to + static_cast<int64_t>(G::column_of(from, a.outputs) + big % kWideO) * a.channels;
 #pragma unroll
-            for (int s = 0; s < kTilesC; ++s) {
-                const int wide = first_c + s, at = c0 + (wide / kWideC * 16 + lane % 16) * kWideC + wide % kWideC;
-                if (at < a.channels) sums[static_cast<int64_t>(to) * a.channels + at] = acc[t][s][r];
+                for (int group = 0; group < kTilesC; group += kWideC) {
+                    const int at = c0 + ((first_c + group) / kWideC * 16 + lane % 16) * kWideC;
+                    Wide v;
+#pragma unroll
+                    for (int s = 0; s < kWideC; ++s) v[s] = static_cast<To>(acc[t][group + s][r]);
+                    if (at + kWideC <= a.channels) {
+                        *reinterpret_cast<Wide*>(row + at) = v;
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < kWideC; ++s)
+                            if (at + s < a.channels) row[at + s] = v[s];
+                    }
+                }
             }
-        }
-    if (!bias || lane % 16 != 0) return;
+        if (!bias || lane % 16 != 0) return;
 #pragma unroll
-    for (int t = 0; t < kBias; ++t)
+        for (int t = 0; t < kBias; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int big = first_o + first_bias + t, from = o0 + (big / kWideO * 16 + lane / 16 * 4 + r) * kWideO;
-            if (from < a.outputs) a.bias_sums[split * a.outputs + G::column_of(from, a.outputs) + big % kWideO] = bias_acc[t][r];
-        }
+            for (int r = 0; r < 4; ++r) {
+                const int big = first_o + first_bias + t, from = o0 + (big / kWideO * 16 + lane / 16 * 4 + r) * kWideO;
+                if (from < a.outputs) to_bias[G::column_of(from, a.outputs) + big % kWideO] = static_cast<To>(bias_acc[t][r]);
+            }
+    };
+    if (a.weight == nullptr) write(a.sums + split * a.outputs * a.channels, a.bias_sums + split * a.outputs);
+    else if (a.type == PENC_FP32) write(static_cast<float*>(a.weight), static_cast<float*>(a.bias));
+    else if (a.type == PENC_FP16) write(static_cast<half_t*>(a.weight), static_cast<half_t*>(a.bias));
+    else write(static_cast<bf16_t*>(a.weight), static_cast<bf16_t*>(a.bias));
 }
 
 // The splits of `n` weights and, behind them, `n_bias` of the bias, in a fixed order: 256 / kStrands results to a workgroup, each strand of threads
@@ -444,26 +480,31 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(const float* __restrict
 }
 
 constexpr int64_t kMostStride = 1 << 22;
+// Products of as many multiplications (three or two for one of a gradient in parts) go by the larger tiles.  us by 64 columns a side -> by 256:
+// 1024 x 1024 bf16, 4096 rows 27 -> 55, 16384 86 -> 80, 131072 658 -> 331; 256 x 1545 bf16, 16384 rows 51 -> 50; 256 x 256 fp32, 131072 rows 102 -> 85,
+// 1024 x 1024 fp32, 4096 rows 51 -> 65, 16384 178 -> 131.  Fewer rows do not fill the card with large tiles; one row of 1024 x 1024 7 -> 9.
+constexpr int64_t kLargeProduct = int64_t{1} << 34;
 
-// How a product is cut up: into the tiles that are at most half empty.
+// How a product is cut up.
 struct WeightPlan {
-    int block_o, block_c, at_a_time, splits;  // columns and rows of a workgroup
+    int block, splits;  // columns of a workgroup either way; workgroups of a tile
     bool ragged;
     int64_t split_rows;
     int output_tiles, channel_tiles;
 };
-WeightPlan weight_plan(int64_t rows, int64_t channels, int64_t outputs, int64_t grad_stride) {
+WeightPlan weight_plan(int type, int64_t rows, int64_t channels, int64_t outputs, int64_t grad_stride) {
     WeightPlan p{};
     // (a lane takes 8 rows of 4 or 8 columns, at 32-bit offsets from a step's first row)
     p.ragged = rows < kLaneRows || outputs < 4 || grad_stride > kMostStride;
-    p.block_o = p.block_c = p.ragged ? 64 : channels > 128 && outputs > 128 ? 256 : channels > 64 && outputs > 64 ? 128 : 64;
-    p.at_a_time = 8 * kStep;
-    p.output_tiles = static_cast<int>((outputs + p.block_o - 1) / p.block_o);
-    p.channel_tiles = static_cast<int>((channels + p.block_c - 1) / p.block_c);
-    const int64_t tiles = static_cast<int64_t>(p.output_tiles) * p.channel_tiles;
-    const int64_t pieces = std::max<int64_t>(1, (rows + p.at_a_time - 1) / p.at_a_time);
+    const int64_t pieces_of_a_value = type == PENC_FP32 ? 3 : type == PENC_FP16 ? 2 : 1;
+    const bool large = !p.ragged && channels > 128 && outputs > 128 && rows * channels * outputs * pieces_of_a_value >= kLargeProduct;
+    p.block = large ? kLargeBlock : 64;
+    p.output_tiles = static_cast<int>((outputs + p.block - 1) / p.block);
+    p.channel_tiles = static_cast<int>((channels + p.block - 1) / p.block);
+    const int64_t tiles = static_cast<int64_t>(p.output_tiles) * p.channel_tiles, at_a_time = 8 * kStep;
+    const int64_t pieces = std::max<int64_t>(1, (rows + at_a_time - 1) / at_a_time);
     const int64_t wanted = std::max<int64_t>(1, std::min(pieces, 256 / tiles));
-    p.split_rows = (pieces + wanted - 1) / wanted * p.at_a_time;
+    p.split_rows = (pieces + wanted - 1) / wanted * at_a_time;
     p.splits = static_cast<int>(std::max<int64_t>(1, (rows + p.split_rows - 1) / p.split_rows));
     return p;
 }
@@ -476,9 +517,8 @@ template <class E>
 int launch(const WeightGrad& a, const WeightPlan& p, unsigned grid, hipStream_t stream) {
     constexpr int kPieces = GradTile<E, 4>::kPieces, kSteps = kPieces == 1 ? 2 : 1;
     if (p.ragged) hipLaunchKernelGGL((weight_grad_kernel<E, 4, 4, 8, true>), dim3(grid), dim3(512), 0, stream, a);
-    else if (p.block_o == 64) hipLaunchKernelGGL((weight_grad_kernel<E, 4, 4, 8, false>), dim3(grid), dim3(512), 0, stream, a);
-    else if (p.block_o == 128) hipLaunchKernelGGL((weight_grad_lds_kernel<E, 128, 128, 2 * kSteps, 4>), dim3(grid), dim3(512), 0, stream, a);
-    else hipLaunchKernelGGL((weight_grad_lds_kernel<E, 256, 256, kSteps, 4>), dim3(grid), dim3(512), 0, stream, a);
+    else if (p.block != kLargeBlock) hipLaunchKernelGGL((weight_grad_kernel<E, 4, 4, 8, false>), dim3(grid), dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((weight_grad_lds_kernel<E, kSteps>), dim3(grid), dim3(512), 0, stream, a);
     return launched();
 }
 
@@ -491,7 +531,10 @@ extern "C" {
 
 size_t penc_weight_grad_workspace_bytes(int64_t rows, int64_t channels, int64_t outputs) {
     if (bad_size(rows, channels, outputs)) return 0;
-    return static_cast<size_t>(std::max(weight_plan(rows, channels, outputs, 0).splits, weight_plan(rows, channels, outputs, kMostStride + 1).splits)) * static_cast<size_t>(channels + 1) * static_cast<size_t>(outputs) * 4;
+    int splits = 1;  // the most of any type and stride
+    for (const int type : {PENC_FP32, PENC_FP16, PENC_BF16})
+        for (const int64_t stride : {int64_t{0}, kMostStride + 1}) splits = std::max(splits, weight_plan(type, rows, channels, outputs, stride).splits);
+    return static_cast<size_t>(splits) * static_cast<size_t>(channels + 1) * static_cast<size_t>(outputs) * 4;
 }
 
 int penc_weight_grad(int type, int result_type, int64_t rows, int64_t channels, int64_t outputs, const int8_t* values, const uint8_t* exponents,
@@ -507,16 +550,18 @@ int penc_weight_grad(int type, int result_type, int64_t rows, int64_t channels, 
                 !aligned_to(workspace, 16))
                 return PENC_ERR_MISALIGNED;
             if (workspace_bytes < penc_weight_grad_workspace_bytes(rows, channels, outputs)) return PENC_ERR_WORKSPACE_TOO_SMALL;
-            const WeightPlan p = weight_plan(rows, channels, outputs, grad_row_stride);
+            const WeightPlan p = weight_plan(type, rows, channels, outputs, grad_row_stride);
             float* const sums = static_cast<float*>(workspace);
             const int64_t n = channels * outputs;
             const WeightGrad a{rows, grad_row_stride, p.split_rows, static_cast<int>(channels), static_cast<int>(outputs), p.channel_tiles,
-                               p.output_tiles, kept_array(values, exponents, channels), grad, sums, bias_grad ? sums + p.splits * n : nullptr};
+                               p.output_tiles, kept_array(values, exponents, channels), grad, sums, bias_grad ? sums + p.splits * n : nullptr,
+                               p.splits == 1 ? weight_grad : nullptr, p.splits == 1 ? bias_grad : nullptr, result_type};
             const int64_t grid = static_cast<int64_t>(p.splits) * p.output_tiles * p.channel_tiles;
             const int n_bias = bias_grad ? static_cast<int>(outputs) : 0;
             if (grid > 0x7FFFFFFF) return PENC_ERR_BAD_LAYER_SIZE;
             hipStream_t st = static_cast<hipStream_t>(stream);
             if (const int rc = launch<E>(a, p, static_cast<unsigned>(grid), st)) return rc;
+            if (p.splits == 1) return PENC_OK;
             const auto sum = [&](auto kernel, int results) {
                 hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((n + n_bias + results - 1) / results)), dim3(256), 0, st, sums, a.bias_sums, n, n_bias,
                                    p.splits, static_cast<To*>(weight_grad), static_cast<To*>(bias_grad));
