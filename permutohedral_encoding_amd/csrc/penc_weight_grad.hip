@@ -40,15 +40,15 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t first, uint32_t second)
 // Where a lane's 8 rows of a step are.  The last step's lanes that would read behind `last` read the 8 rows before it instead, and `skip` of them count
 // for nothing: loads have no conditions.
 struct StepRows {
-    int64_t first;  // of the step, the same in every lane
-    uint32_t at;    // the lane's, from there on
+    row_t first;  // of the step, the same in every lane
+    uint32_t at;  // the lane's, from there on
     int skip;
 
-    __device__ __forceinline__ StepRows(int64_t step, int row_at, int64_t last) {
-        const int64_t most = last - kLaneRows;
+    __device__ __forceinline__ StepRows(row_t step, uint32_t row_at, row_t rows) {
+        const row_t most = rows - kLaneRows;
         first = min(step, most);
-        const int64_t row = min(step + row_at, most);
-        at = static_cast<uint32_t>(row - first);
+        const row_t row = min(step + row_at, most);
+        at = row - first;
         skip = static_cast<int>(step + row_at - row);
     }
 };
@@ -78,7 +78,7 @@ struct GradTile {
 
     template <class W>
     __device__ __forceinline__ static void load(W (&row)[kLaneRows], const void* grad, int64_t stride, StepRows rows, int column) {
-        const char* const first = static_cast<const char*>(grad) + rows.first * stride * static_cast<int64_t>(sizeof(E));
+        const char* const first = static_cast<const char*>(grad) + static_cast<int64_t>(rows.first) * stride * static_cast<int64_t>(sizeof(E));
         const uint32_t at = (rows.at * static_cast<uint32_t>(stride) + static_cast<uint32_t>(column)) * static_cast<uint32_t>(sizeof(E));
 #pragma unroll
         for (int j = 0; j < kLaneRows; ++j) {
@@ -138,8 +138,8 @@ struct KeptTile {
 
     template <class W>
     __device__ __forceinline__ static void load(W (&row)[kLaneRows], const KeptArray& kept, StepRows rows, int column) {
-        const int8_t* const values = kept.values + rows.first * kept.pitch;
-        const uint8_t* const exponents = kept.exponents + rows.first * kept.blocks;
+        const int8_t* const values = kept.values + offset_of(rows.first, kept.pitch);
+        const uint8_t* const exponents = kept.exponents + offset_of(rows.first, kept.blocks);
         const uint32_t at = rows.at * static_cast<uint32_t>(kept.pitch) + static_cast<uint32_t>(column);
         const uint32_t block_at = rows.at * static_cast<uint32_t>(kept.blocks) + static_cast<uint32_t>(column / kKeptBlock);
 #pragma unroll
@@ -177,7 +177,8 @@ struct KeptTile {
 };
 
 struct WeightGrad {
-    int64_t rows, grad_stride, split_rows;  // split_rows: of a workgroup, a multiple of its waves' steps
+    row_t rows, split_rows;  // split_rows: of a workgroup, a multiple of its waves' steps
+    int64_t grad_stride;
     int channels, outputs, channel_tiles, output_tiles;
     KeptArray kept;
     const void* grad;
@@ -222,25 +223,25 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
     using X = KeptTile<kWideC>;
     const int c = X::column_of(c0 + column * kWideC, a.kept), o = kRagged ? o0 + column * kWideO : G::column_of(o0 + column * kWideO, a.outputs);
     const bool bias = (a.bias_sums != nullptr || a.bias != nullptr) && c0 == 0;
-    const int64_t first = split * a.split_rows, last = min(first + a.split_rows, a.rows);
+    const row_t first = static_cast<row_t>(split) * a.split_rows, last = min(first + a.split_rows, a.rows);
 
     acc_t acc[kWideO][kWideC] = {}, bias_acc[kWideO] = {};
     const Frag ones = {{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}};
     words_t<G::kWords> g[kLaneRows], g_ahead[kLaneRows];
     words_t<X::kWords> x[kLaneRows], x_ahead[kLaneRows];
     // (behind the last step: rows that are there)
-    const auto load = [&](int64_t step) {
+    const auto load = [&](row_t step) {
         if constexpr (kRagged) {
-            const int64_t row = step + rows_at;
-            G::load_ragged(g_ahead, static_cast<const E*>(a.grad) + row * a.grad_stride + o, a.grad_stride, last - row, a.outputs - o);
-            X::load_ragged(x_ahead, a.kept, row, last - row, c);
+            const int64_t row = static_cast<int64_t>(step) + rows_at;
+            G::load_ragged(g_ahead, static_cast<const E*>(a.grad) + row * a.grad_stride + o, a.grad_stride, static_cast<int64_t>(last) - row, a.outputs - o);
+            X::load_ragged(x_ahead, a.kept, row, static_cast<int64_t>(last) - row, c);
         } else {
             const StepRows rows(step, rows_at, a.rows);
             G::load(g_ahead, a.grad, a.grad_stride, rows, o);
             X::load(x_ahead, a.kept, rows, c);
         }
     };
-    int64_t step = first + wave * kStep;
+    row_t step = first + wave * kStep;
     if (step < last) load(step);
     for (; step < last; step += kWaves * kStep) {
 #pragma unroll
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(512, 2) void weight_grad_lds_kernel(WeightGrad a) {
     const int tiles = a.channel_tiles * a.output_tiles, tile = static_cast<int>(item % tiles);
     const int64_t split = item / tiles;
     const int c0 = tile % a.channel_tiles * kBlockC, o0 = tile / a.channel_tiles * kBlockO;
-    const int64_t first = split * a.split_rows, last = min(first + a.split_rows, a.rows);
+    const row_t first = static_cast<row_t>(split) * a.split_rows, last = min(first + a.split_rows, a.rows);
 
     // what this wave brings: 32 rows of 16 kWide columns
     const bool brings_grad = wave < 4;
@@ -343,12 +344,12 @@ __global__ __launch_bounds__(512, 2) void weight_grad_lds_kernel(WeightGrad a) {
         constexpr int kColumns = kBringsGrad ? kWideO : kWideC, kSlots = kSteps * kPieces * kTilesC, kRows = kSteps * kStep;
         static_assert(kColumns <= kSlots, "every column has its place between the products");
         using Raw = words_t<Side::kWords>;
-        const auto load = [&](Raw(&raw)[kLaneRows], int64_t step) {
+        const auto load = [&](Raw(&raw)[kLaneRows], row_t step) {
             const StepRows rows(step, row_at, a.rows);
             if constexpr (kBringsGrad) G::load(raw, a.grad, a.grad_stride, rows, o);
             else X::load(raw, a.kept, rows, c);
         };
-        const auto skip = [&](Raw(&raw)[kLaneRows], int64_t step) {
+        const auto skip = [&](Raw(&raw)[kLaneRows], row_t step) {
             if (step + kRows > a.rows) skip_rows(raw, StepRows(step, row_at, a.rows).skip);
         };
         const auto bring = [&](const Raw(&raw)[kLaneRows], uint4* to, int t) {
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(512, 2) void weight_grad_lds_kernel(WeightGrad a) {
         load(raw, first + kRows);
         __syncthreads();
         int turn = 0;
-        for (int64_t step = first; step < last; step += kRows) {
+        for (row_t step = first; step < last; step += kRows) {
             const uint4* const from = fragments + turn * (kGrad + kKept) * 64;
             uint4* const to = fragments + (turn ^ 1) * (kGrad + kKept) * 64;
             turn ^= 1;
@@ -553,7 +554,7 @@ int penc_weight_grad(int type, int result_type, int64_t rows, int64_t channels, 
             const WeightPlan p = weight_plan(type, rows, channels, outputs, grad_row_stride);
             float* const sums = static_cast<float*>(workspace);
             const int64_t n = channels * outputs;
-            const WeightGrad a{rows, grad_row_stride, p.split_rows, static_cast<int>(channels), static_cast<int>(outputs), p.channel_tiles,
+            const WeightGrad a{static_cast<row_t>(rows), static_cast<row_t>(p.split_rows), grad_row_stride, static_cast<int>(channels), static_cast<int>(outputs), p.channel_tiles,
                                p.output_tiles, kept_array(values, exponents, channels), grad, sums, bias_grad ? sums + p.splits * n : nullptr,
                                p.splits == 1 ? weight_grad : nullptr, p.splits == 1 ? bias_grad : nullptr, result_type};
             const int64_t grid = static_cast<int64_t>(p.splits) * p.output_tiles * p.channel_tiles;
