@@ -67,13 +67,6 @@ __device__ __forceinline__ void store_chunk(E* __restrict__ p, int valid, const 
     }
 }
 
-// A parameter: fp32, or of the type of the rows it is applied to.
-template <class E>
-__device__ __forceinline__ void load_param(const void* p, bool fp32, int64_t at, int valid, float (&v)[kChunk]) {
-    if (fp32) load_chunk(static_cast<const float*>(p) + at, valid, v);
-    else load_chunk(static_cast<const E*>(p) + at, valid, v);
-}
-
 template <int kControl>
 __device__ __forceinline__ uint32_t dpp(uint32_t x) {
     return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kControl, 0xF, 0xF, true));

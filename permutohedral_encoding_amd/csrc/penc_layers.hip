@@ -6,7 +6,13 @@
 //     softplus  log(1 + exp(x))     act' = s
 //
 // All of them are one pass over their rows: bound by memory.  A lane has 8 channels, the lanes of a row are a power of two from 4 to 256,
-// so that a block of a checkpoint is always four neighbours of one wave, and a workgroup walks over the rows.
+// so that a block of a checkpoint is always four neighbours of one wave, and a workgroup walks over the rows.  Measured, us and bytes read and
+// written (a copy on this card reaches 5.5 TB/s; what fits the 256 MB cache in front of the memory, more):
+//
+//     pack, channels adjacent     65536 x 1024 bf16  38, 5.3 TB/s      1048576 x 48 fp32  44, 5.8 TB/s
+//     pack, rows adjacent                                              1048576 x 48 fp32  62, 4.1 TB/s
+//     unpack                      65536 x 1024 bf16  31, 6.6 TB/s      1048576 x 48 fp32  42, 6.1 TB/s
+//     gated silu                  32765 x 2 2048 bf16: forward with its checkpoints 98, 5.5 TB/s; backward from them 98, 5.5 TB/s
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -56,7 +62,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(Lanes l, const E* __rest
 // The encoding's own result: channels of consecutive rows next to each other.  A workgroup has kThreads rows and up to 128 of their channels: a lane has a
 // row and walks over its blocks, reading 32 channels, each with the 63 lanes beside it, and what it makes of them waits in the LDS until all rows' can be
 // written one after the other.  (Written by the lanes themselves, 16 bytes a row: 1000003 x 48 fp32 48.7 us instead of 38.6; 2^20 x 48 54 instead of 50, where
-// channels 4 MiB apart meet in the same memory channels.)
+// channels 4 MiB apart meet in the same memory channels.  All 8192 channels of 10 rows by one workgroup: 515 us instead of 7.)
 constexpr int kPiece = 128;
 template <class E>
 __global__ __launch_bounds__(kThreads) void pack_channels_kernel(row_t rows, int channels, const E* __restrict__ x, int64_t stride, KeptArray kept) {
@@ -388,6 +394,7 @@ int penc_residual_norm_backward(const penc_norm* norm, const penc_norm_grads* gr
     if (workspace_bytes < penc_residual_norm_workspace_bytes(a.rows, a.channels, a.rows_per_gate)) return PENC_ERR_WORKSPACE_TOO_SMALL;
     if (!workspace) return PENC_ERR_NULL_POINTER;
     a.gate_by_lanes = plan.gate_by_lanes;
+    if (a.rows == 0) a.gate = nullptr;  // (there may be no group's gate either)
     NormGrads g{grads->y, a.pre_norm ? grads->n : nullptr, static_cast<uint32_t>(grads->y_stride), static_cast<uint32_t>(grads->n_stride), grads->x, a.has_branch ? grads->branch : nullptr, grads->gate,
                 nullptr, {}, static_cast<uint32_t>(plan.pieces), static_cast<row_t>(plan.piece_rows)};
     // partial sums of what is wanted, one array after the other

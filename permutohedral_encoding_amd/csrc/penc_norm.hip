@@ -14,6 +14,15 @@
 //
 // The sums over rows stay in registers while a workgroup walks over its rows; each workgroup leaves one row of partial sums, added up in a
 // fixed order by sum_partials_kernel.  No atomics: results are the same in every run.
+//
+// Measured, with the checkpoints of x and f written and read (us, and the rate of the bytes that this takes; a copy on this card reaches 5.5 TB/s):
+//
+//     1048576 x 64 fp32 "rms"                              forward 234, 5.2 TB/s      backward 252, 4.8 TB/s
+//     16384 x 4096 bf16 "rms"                                      121, 5.5                    156, 4.3
+//     130944 x 203 fp16 "layer", a gate per 128 rows                66, 4.0                    102, 2.6
+//
+// The last is bound by instructions: 570 of the vector units for 8 channels of the backward, 60% of its time, in the three waves a SIMD has
+// registers for.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -254,7 +263,8 @@ __device__ __forceinline__ void walk(row_t row, row_t end, row_t run, row_t stri
     }
 }
 
-// kFull: any kind of norm; else "rms" without biases, whose sums and parameters need 32 registers less.
+// kFull: any kind of norm; else "rms" without biases, whose sums and parameters need 32 registers less (backward of 16384 x 4096 bf16 as "layer": 232 us
+// instead of 156).
 template <class E, int kLanes, int kEnd, bool kFull>
 __global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_kernel(NormArgs a, E* __restrict__ y_out, E* __restrict__ n_out) {
     using R = Row<kLanes>;
@@ -333,6 +343,9 @@ __device__ __forceinline__ void write_sum(const Values& sum, float (*__restrict_
 }
 
 // kKept: x and the branch are read from their checkpoints.
+//
+// Waves to a SIMD, by what the kernel needs in registers: 128 do for "rms" without biases, 168 for the others, and more where a workgroup is eight waves,
+// of which a compute unit holds one or two and not one and a half.  (Four waves of "layer" with 4096 channels spill: 331 us instead of 232.)
 //
 // Gates of groups of rows: with few rows in a group (a.gate_by_lanes) the lanes of a row take whole groups and write their sums themselves; else a
 // workgroup takes a piece of a group, `pieces` of them to a group, and leaves a row of partial sums.  One gate for all rows is one more sum over rows.
@@ -499,7 +512,8 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads, !kFull ? 4 : kLanes == 512 ?
 
 #undef PENC_EACH
 
-// to[group][c] = the sum over `rows` rows of partial sums of a group, in a fixed order; 32 channels and 32 strands of rows to a workgroup.
+// to[group][c] = the sum over `rows` rows of partial sums of a group, in a fixed order; 32 channels and 32 strands of rows to a workgroup, which waits
+// for memory and not for its bytes: 5 us behind the backward of 1048576 x 64.
 template <class E>
 __global__ __launch_bounds__(1024) void sum_partials_kernel(SumPartials s) {
     __shared__ float lds[32][33];

@@ -209,7 +209,8 @@ __device__ __forceinline__ int64_t item_of(const WeightGrad& a) {
     return die * each + min(die, rest) + blockIdx.x / kDies;
 }
 
-// 16 kWideO outputs by 16 kWideC channels.
+// 16 kWideO outputs by 16 kWideC channels.  Bound by memory: each operand is read once for 64 columns of the other.  1048576 x 48 by 64 outputs fp32 74 us,
+// 4.3 TB/s (a wave's next rows are on their way while it multiplies; without that 82).
 template <class E, int kWideO, int kWideC, int kWaves, bool kRagged>
 __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) {
     constexpr int kPieces = GradTile<E, kWideO>::kPieces;
@@ -303,6 +304,8 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
 // The same for products that the matrix cores bound: 256 outputs by 256 channels to a workgroup of 8 waves, which bring 32 kSteps rows at a time
 // into the LDS as the matrix instruction takes them, half of the waves the gradient and half the checkpoint (one of either kind on each SIMD), while all of
 // them multiply what was brought before.  Every value is converted once for the workgroup, and a wave's 4 x 8 tiles multiply a fragment 2.7 times.
+// Bound by the matrix cores and what goes on between their instructions: 16384 x 1024 by 4096 outputs bf16 150 us, 0.92 PFLOP/s (the library's product of
+// bf16 operands of these sizes 197 us, and of 8192^3, its best, 1.28 PFLOP/s; the 64-column kernel 495).
 template <class E, int kSteps>
 __global__ __launch_bounds__(512, 2) void weight_grad_lds_kernel(WeightGrad a) {
     constexpr int kBlockO = kLargeBlock, kBlockC = kLargeBlock, kWavesO = 4;
@@ -454,7 +457,7 @@ __global__ __launch_bounds__(512, 2) void weight_grad_lds_kernel(WeightGrad a) {
 }
 
 // The splits of `n` weights and, behind them, `n_bias` of the bias, in a fixed order: 256 / kStrands results to a workgroup, each strand of threads
-// with every kStrands-th split.
+// with every kStrands-th split.  16 us for the 4 splits of 4096 x 1024, 4.7 TB/s; 5 us for the 256 of 64 x 48.
 template <class To, int kStrands>
 __global__ __launch_bounds__(256) void sum_splits_kernel(const float* __restrict__ sums, const float* __restrict__ bias_sums, int64_t n, int n_bias,
                                                          int splits, To* __restrict__ weight, To* __restrict__ bias) {
@@ -541,7 +544,7 @@ size_t penc_weight_grad_workspace_bytes(int64_t rows, int64_t channels, int64_t 
 int penc_weight_grad(int type, int result_type, int64_t rows, int64_t channels, int64_t outputs, const int8_t* values, const uint8_t* exponents,
                      const void* grad, int64_t grad_row_stride, void* weight_grad, void* bias_grad, void* workspace, size_t workspace_bytes,
                      void* stream) {
-    if (bad_size(rows, channels, outputs)) return PENC_ERR_BAD_LAYER_SIZE;
+    if (bad_size(rows, channels, outputs) || grad_row_stride < 0) return PENC_ERR_BAD_LAYER_SIZE;
     return with_type(type, [&](auto e) {
         using E = decltype(e);
         return with_type(result_type, [&](auto r) -> int {

@@ -590,3 +590,119 @@ def test_a_step_in_a_graph():
         torch.cuda.synchronize()
         for a, b in zip(out, step(leaf)):
             torch.testing.assert_close(a, b)
+
+
+def block(x, p):
+    f = layers.linear(layers.activation(x, "silu"), p["w1"], p["b1"])
+    y, n = layers.residual_norm(x, f, gate=p["gate"], post_weight=p["post"], pre_weight=p["pre"], kind="layer")
+    return layers.activation(layers.linear(n, p["w2"]), "gelu", gated=True) + y
+
+
+def block_step(x, p, grad, names=("w1", "b1", "gate", "post", "pre", "w2")):
+    out = block(x, p)
+    return [out, *torch.autograd.grad(out, [x, *(p[k] for k in names)], grad)]
+
+
+def captured(call):
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    return graph, out
+
+
+def test_two_graphs_in_turn_and_at_once():
+    """Each has its own workspaces: replays of one, also while the other runs, leave the other's results as they are."""
+    cases = []
+    for seed, points in ((0, 256), (1, 4097)):
+        p = decoder(points - points % 16, 32, 16)[1]
+        p["gate"] = p["gate"][:1].detach().clone().requires_grad_(True)
+        cases.append((values(points, 32, torch.float32, seed).requires_grad_(True), p, values(points, 32, torch.float32, seed + 2)))
+    want = [[t.detach().clone() for t in block_step(*c)] for c in cases]
+    graphs = [captured(lambda c=c: block_step(*c)) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+
+    def compare():
+        torch.cuda.synchronize()
+        for (_, out), expected in zip(graphs, want):
+            for a, b in zip(out, expected):
+                torch.testing.assert_close(a, b)
+                a.detach().zero_()
+        torch.cuda.synchronize()
+
+    for _ in range(3):
+        for graph, _ in graphs:
+            graph.replay()
+        compare()
+        for (graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        compare()
+
+
+def test_two_steps_at_once_on_two_streams():
+    p = decoder(2048, 64, 16)[1]
+    inputs = [(values(2048, 64, torch.float32, k).requires_grad_(True), values(2048, 64, torch.float32, k + 2)) for k in range(2)]
+    want = [block_step(x, p, grad) for x, grad in inputs]
+    streams, got = [torch.cuda.Stream() for _ in inputs], [None, None]
+    for _ in range(3):
+        for k, stream in enumerate(streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                got[k] = block_step(inputs[k][0], p, inputs[k][1])
+        for stream in streams:
+            torch.cuda.current_stream().wait_stream(stream)
+        for one, expected in zip(got, want):
+            for a, b in zip(one, expected):
+                torch.testing.assert_close(a, b)
+        torch.cuda.synchronize()
+
+
+def test_a_bias_alone_in_a_graph():
+    x, w = values(5000, 48, torch.float32), values(64, 48, torch.float32, seed=1)
+    b = torch.zeros(64, device="cuda", requires_grad=True)
+    grad = values(5000, 64, torch.float32, seed=2)
+    graph, out = captured(lambda: torch.autograd.grad(layers.linear(x, w, b), b, grad))
+    want, magnitude = grad.double().sum(0), grad.double().abs().sum(0)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert_near(out[0], want, magnitude, 5000, "bias")
+        out[0].zero_()
+
+
+def test_one_tensor_in_several_places():
+    """As the residual and the branch, as the weight of both norms; parameters that are views: every place adds to the same gradient."""
+    x, w, s = values(40, 56, torch.float32), values(1, 112, torch.float32, seed=1)[0], torch.tensor(0.5, device="cuda")
+    grad_y, grad_n = values(40, 56, torch.float32, seed=2), values(40, 56, torch.float32, seed=3)
+
+    def run(x_of, branch_of, post_of, pre_of, gate_of):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, s)]
+        out = layers.residual_norm(x_of(leaves[0]), branch_of(leaves[0]), gate=gate_of(leaves[2]), post_weight=post_of(leaves[1]), pre_weight=pre_of(leaves[1]))
+        return [*out, *torch.autograd.grad(out, leaves, (grad_y, grad_n))]
+
+    same = run(lambda t: t, lambda t: t, lambda t: t[::2], lambda t: t[::2], lambda t: t.expand(56))
+    apart = run(lambda t: t.clone(), lambda t: t.clone(), lambda t: t[::2].clone(), lambda t: t[::2].clone(), lambda t: t.expand(56).clone())
+    for a, b in zip(same, apart):
+        assert torch.equal(a, b)
+
+
+def test_inference_mode_and_autocast_change_nothing():
+    p = decoder(64, 32, 16)[1]
+    x, grad = values(64, 32, torch.float32).requires_grad_(True), values(64, 32, torch.float32, seed=1)
+    want = block_step(x, p, grad)
+    with torch.inference_mode():
+        got = block(x, p)
+        inside = values(64, 32, torch.float32)
+    assert torch.equal(got, want[0]) and not got.requires_grad
+    for t in (torch.bfloat16, torch.float16):
+        with torch.autocast("cuda", dtype=t):
+            got = block_step(x, p, grad)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # a tensor made in inference mode is an input like any other: what is kept of it is not the tensor
+    got = torch.autograd.grad(block(inside, p), p["w1"], grad)
+    assert torch.equal(got[0], want[2])

@@ -66,6 +66,7 @@ def test_the_entry_points_refuse_before_they_launch():
     assert lib.penc_weight_grad(0, 0, 100, 48, 64, p, p, p, 64, p, z, z, need, z) == 1
     assert lib.penc_weight_grad(0, 4, 100, 48, 64, p, p, p, 64, p, z, p, need, z) == 10
     assert lib.penc_weight_grad(0, 0, 100, 48, 0, p, p, p, 64, p, z, p, need, z) == 12
+    assert lib.penc_weight_grad(0, 0, 100, 48, 64, p, p, p, -64, p, z, p, need, z) == 12
     for status in (10, 11, 12):
         assert lib.penc_status_string(status) != lib.penc_status_string(99)
 
