@@ -14,7 +14,7 @@ Unlike the kernel benchmark (``bench.py``) these figures include everything a us
 pays: output allocation, the loss, the gradient layout change and the optimiser walking the whole
 table.
 
-    python -m permutohedral_encoding_amd.perf_sweep [--dims 2 3 4 5 6] [--points 524288] [--iters 300] [--fused-optimizer] [--contiguous-output]
+    python -m permutohedral_encoding_amd.perf_sweep [--dims 2 3 4 5 6] [--points 524288] [--iters 300] [--fused-optimizer] [--contiguous-output] [--decoder]
 
 ``--consumers`` instead runs what the layer after the encoding does with the (N, 48) result of 2^20 points,
 a few times each and meant to be run under a kernel trace: ``torch.nn.Linear``, ``torch.cat`` with
@@ -27,6 +27,10 @@ levels, 2^18 slots, 2^20 points) on the same number of points in different order
 (the benchmark), consecutive samples along rays (64, 128 and 512 per ray), and the uniform points sorted
 along a Z-order curve; then the table backward of every level on its own (all other levels masked by the
 window) for three of them.  A renderer delivers the second kind, a caller who sorts for locality the third.
+
+``--decoder`` trains the encoding of ``--points`` points and a decoder of residual blocks behind it (``--width`` channels, ``--blocks`` blocks of a gated
+layer and a layer back, normed before and after) once with torch's layers and once with those of ``layers.py``, and reports points per second and the memory
+that a step adds at its peak.  The steps are those of training: forward, loss, backward, AdamW on the table and the decoder.
 """
 import argparse
 import json
@@ -176,6 +180,73 @@ def point_orders(repeats=25):
         print(f"| {name} | " + " | ".join(f"{x:.0f}" for x in row) + " |", flush=True)
 
 
+def decoder(nr_points, iters, warmup, width=64, blocks=2, dtype=torch.float32, pos_dim=3, levels=24, log2_capacity=18):
+    """One row for torch's layers and one for those of layers.py, on the same parameters and points."""
+    import torch.nn.functional as F
+
+    from . import layers
+    from .optim import AdamW
+
+    def torch_norm(x, weight):
+        return F.rms_norm(x, x.shape[-1:], weight, 1e-6)
+
+    def with_torch(x, p):
+        h = F.linear(x, p["in"])
+        n = torch_norm(h, p["norm"])
+        for b in p["blocks"]:
+            a, gate = F.linear(n, b["up"]).chunk(2, dim=-1)
+            h = h + b["gate"] * torch_norm(F.linear(F.silu(a) * gate, b["down"]), b["post"])
+            n = torch_norm(h, b["pre"])
+        return F.linear(n, p["out"])
+
+    def with_layers(x, p):
+        h = layers.linear(x, p["in"])
+        n = layers.norm(h, p["norm"])
+        for b in p["blocks"]:
+            f = layers.linear(layers.activation(layers.linear(n, b["up"]), "silu", gated=True), b["down"])
+            h, n = layers.residual_norm(h, f, gate=b["gate"], post_weight=b["post"], pre_weight=b["pre"])
+        return layers.linear(n, p["out"])
+
+    rows = []
+    for name, forward in (("torch", with_torch), ("layers", with_layers)):
+        torch.manual_seed(0)
+        enc = PermutoEncoding(pos_dim, 1 << log2_capacity, levels, 2, np.geomspace(1.0, 1e-4, num=levels))
+
+        def weight(outputs, channels):
+            return (torch.randn(outputs, channels, device="cuda") / channels ** 0.5).to(dtype).requires_grad_(True)
+
+        def ones(scale=1.0):
+            return torch.full((width,), scale, device="cuda", dtype=dtype, requires_grad=True)
+
+        p = {"in": weight(width, enc.output_dims()), "norm": ones(), "out": weight(3, width),
+             "blocks": [{"up": weight(4 * width, width), "down": weight(width, 2 * width), "gate": ones(0.1), "post": ones(), "pre": ones()}
+                        for _ in range(blocks)]}
+        decoder_parameters = [p["in"], p["norm"], p["out"], *(t for b in p["blocks"] for t in b.values())]
+        table_step = AdamW(enc.parameters(), betas=(0.9, 0.99), eps=1e-15, weight_decay=0.0, lr=1e-3)
+        decoder_step = torch.optim.AdamW(decoder_parameters, lr=1e-3, weight_decay=0.0)
+        points = torch.rand(nr_points, pos_dim, device="cuda") - 0.5
+
+        def step():
+            loss = ((forward(enc(points).to(dtype), p).float() - 0.5) ** 2).mean()
+            for opt in (table_step, decoder_step):
+                opt.zero_grad()
+            loss.backward()
+            for opt in (table_step, decoder_step):
+                opt.step()
+
+        for _ in range(2):
+            step()
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        step()
+        peak = torch.cuda.max_memory_allocated() - before
+        rows.append({"layers": name, "points": nr_points, "width": width, "blocks": blocks, "dtype": str(dtype).split(".")[-1],
+                     "train": _timed(step, nr_points, iters, warmup), "peak_bytes": peak})
+        print(f"| {name} | {rows[-1]['train']:.3g} | {peak / 2 ** 20:.0f} |", flush=True)
+    return rows
+
+
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--dims", type=int, nargs="+", default=[2, 3, 4, 5, 6])
@@ -188,6 +259,10 @@ def main():
                     help="build the module with contiguous_output=True: dense (N, F*L) rows instead of the strided view")
     ap.add_argument("--consumers", action="store_true", help="run the consumers of the forward result instead (for a kernel trace)")
     ap.add_argument("--point-orders", action="store_true", help="time forward and table backward on unordered, ray-ordered and Z-ordered points instead")
+    ap.add_argument("--decoder", action="store_true", help="train encoding and decoder with torch's layers and with those of layers.py instead")
+    ap.add_argument("--width", type=int, default=64, help="channels of the decoder")
+    ap.add_argument("--blocks", type=int, default=2, help="residual blocks of the decoder")
+    ap.add_argument("--dtype", choices=("float32", "bfloat16"), default="float32", help="type of the decoder")
     args = ap.parse_args()
     if not torch.cuda.is_available():
         raise SystemExit("perf_sweep: no GPU visible; the encoding has no CPU path")
@@ -196,6 +271,11 @@ def main():
         return
     if args.point_orders:
         point_orders()
+        return
+    if args.decoder:
+        print("| layers | training (points/s) | memory of a step (MiB) |")
+        print("|---|---|---|")
+        print(json.dumps(decoder(args.points, args.iters, args.warmup, args.width, args.blocks, getattr(torch, args.dtype))))
         return
     print("| pos_dim | inference (points/s) | training, table grad (points/s) | training, table + position grad (points/s) |")
     print("|---|---|---|---|")

@@ -706,3 +706,11 @@ def test_inference_mode_and_autocast_change_nothing():
     # a tensor made in inference mode is an input like any other: what is kept of it is not the tensor
     got = torch.autograd.grad(block(inside, p), p["w1"], grad)
     assert torch.equal(got[0], want[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_sweep_trains_a_decoder_with_both(dtype):
+    from permutohedral_encoding_amd import perf_sweep
+    rows = perf_sweep.decoder(1000, 3, 1, width=40, blocks=1, dtype=dtype, levels=6, log2_capacity=10)
+    assert [r["layers"] for r in rows] == ["torch", "layers"] and all(r["train"] > 0 for r in rows)
+    assert rows[1]["peak_bytes"] < rows[0]["peak_bytes"]
