@@ -7,8 +7,9 @@
 // rest exactly), so that every product is exact and the sums are those of fp32.
 //
 // The matrix instruction wants 8 consecutive rows of one column in a lane.  A lane loads them for kWide neighbouring columns (16 bytes of a row in
-// one load), and v_perm pairs two rows' halves; lane m of 16 then has columns kWide m .. kWide m + kWide - 1, one for each of kWide tiles, whose
-// columns are kWide apart.  Which column a lane of a tile stands for is free, so nothing goes through the LDS on the way in.
+// one load; one or two columns where there are few), and v_perm pairs two rows' halves; lane m of 16 then has columns kWide m .. kWide m + kWide - 1,
+// one for each of kWide tiles, whose columns are kWide apart.  Which column a lane of a tile stands for is free, so nothing goes through the LDS on the
+// way in.
 //
 // A wave walks over rows 32 at a time, the waves of a workgroup and the workgroups of a tile each over their own, and the partial sums are added in
 // a fixed order: the waves' in the LDS, the workgroups' by sum_splits_kernel.
@@ -69,7 +70,7 @@ __device__ __forceinline__ void skip_rows(W (&row)[kLaneRows], int skip) {
 template <class E, int kWide>
 struct GradTile {
     static constexpr int kPieces = std::is_same_v<E, float> ? 3 : std::is_same_v<E, half_t> ? 2 : 1;
-    static constexpr int kWords = kWide * sizeof(E) / 4;
+    static constexpr int kWords = kWide == 1 ? 1 : kWide * sizeof(E) / 4;
     using Bits = std::conditional_t<sizeof(E) == 4, uint32_t, uint16_t>;
     using Vector = uint32_t __attribute__((ext_vector_type(kWords), aligned(sizeof(E))));
 
@@ -82,9 +83,14 @@ struct GradTile {
         const uint32_t at = (rows.at * static_cast<uint32_t>(stride) + static_cast<uint32_t>(column)) * static_cast<uint32_t>(sizeof(E));
 #pragma unroll
         for (int j = 0; j < kLaneRows; ++j) {
-            const Vector v = *reinterpret_cast<const Vector*>(first + j * stride * static_cast<int64_t>(sizeof(E)) + at);
+            const char* const p = first + j * stride * static_cast<int64_t>(sizeof(E)) + at;
+            if constexpr (kWide == 1) {
+                row[j][0] = *reinterpret_cast<const Bits*>(p);
+            } else {
+                const Vector v = *reinterpret_cast<const Vector*>(p);
 #pragma unroll
-            for (int w = 0; w < kWords; ++w) row[j][w] = v[w];
+                for (int w = 0; w < kWords; ++w) row[j][w] = v[w];
+            }
         }
     }
     // for fewer rows or columns than a lane takes
@@ -210,7 +216,8 @@ __device__ __forceinline__ int64_t item_of(const WeightGrad& a) {
 }
 
 // 16 kWideO outputs by 16 kWideC channels.  Bound by memory: each operand is read once for 64 columns of the other.  1048576 x 48 by 64 outputs fp32 74 us,
-// 4.3 TB/s (a wave's next rows are on their way while it multiplies; without that 82).
+// 4.3 TB/s (a wave's next rows are on their way while it multiplies; without that 82).  kWideO is 4, or 1 or 2 for 16 or 32 outputs and fewer, which leave the
+// registers and LDS of a second workgroup: 1048576 x 64 by 1 output fp32 64 -> 25 us, by 16 51 -> 28, by 32 52 -> 43; bf16 by 3 53 -> 18, by 32 27 -> 28.
 template <class E, int kWideO, int kWideC, int kWaves, bool kRagged>
 __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) {
     constexpr int kPieces = GradTile<E, kWideO>::kPieces;
@@ -491,15 +498,17 @@ constexpr int64_t kLargeProduct = int64_t{1} << 34;
 
 // How a product is cut up.
 struct WeightPlan {
-    int block, splits;  // columns of a workgroup either way; workgroups of a tile
+    int block, splits;  // columns of a workgroup, channels and (but where they are few) outputs; workgroups of a tile
     bool ragged;
+    int wide;  // sixteens of outputs of a workgroup with 64 channels
     int64_t split_rows;
     int output_tiles, channel_tiles;
 };
 WeightPlan weight_plan(int type, int64_t rows, int64_t channels, int64_t outputs, int64_t grad_stride) {
     WeightPlan p{};
-    // (a lane takes 8 rows of 4 or 8 columns, at 32-bit offsets from a step's first row)
-    p.ragged = rows < kLaneRows || outputs < 4 || grad_stride > kMostStride;
+    // (a lane takes 8 rows, at 32-bit offsets from a step's first row)
+    p.ragged = rows < kLaneRows || grad_stride > kMostStride;
+    p.wide = p.ragged || outputs > 32 ? 4 : outputs > 16 ? 2 : 1;
     const int64_t pieces_of_a_value = type == PENC_FP32 ? 3 : type == PENC_FP16 ? 2 : 1;
     const bool large = !p.ragged && channels > 128 && outputs > 128 && rows * channels * outputs * pieces_of_a_value >= kLargeProduct;
     p.block = large ? kLargeBlock : 64;
@@ -507,7 +516,7 @@ WeightPlan weight_plan(int type, int64_t rows, int64_t channels, int64_t outputs
     p.channel_tiles = static_cast<int>((channels + p.block - 1) / p.block);
     const int64_t tiles = static_cast<int64_t>(p.output_tiles) * p.channel_tiles, at_a_time = 8 * kStep;
     const int64_t pieces = std::max<int64_t>(1, (rows + at_a_time - 1) / at_a_time);
-    const int64_t wanted = std::max<int64_t>(1, std::min(pieces, 256 / tiles));
+    const int64_t wanted = std::max<int64_t>(1, std::min(pieces, (p.wide < 4 ? 512 : 256) / tiles));
     p.split_rows = (pieces + wanted - 1) / wanted * at_a_time;
     p.splits = static_cast<int>(std::max<int64_t>(1, (rows + p.split_rows - 1) / p.split_rows));
     return p;
@@ -521,6 +530,8 @@ template <class E>
 int launch(const WeightGrad& a, const WeightPlan& p, unsigned grid, hipStream_t stream) {
     constexpr int kPieces = GradTile<E, 4>::kPieces, kSteps = kPieces == 1 ? 2 : 1;
     if (p.ragged) hipLaunchKernelGGL((weight_grad_kernel<E, 4, 4, 8, true>), dim3(grid), dim3(512), 0, stream, a);
+    else if (p.wide == 1) hipLaunchKernelGGL((weight_grad_kernel<E, 1, 4, 8, false>), dim3(grid), dim3(512), 0, stream, a);
+    else if (p.wide == 2) hipLaunchKernelGGL((weight_grad_kernel<E, 2, 4, 8, false>), dim3(grid), dim3(512), 0, stream, a);
     else if (p.block != kLargeBlock) hipLaunchKernelGGL((weight_grad_kernel<E, 4, 4, 8, false>), dim3(grid), dim3(512), 0, stream, a);
     else hipLaunchKernelGGL((weight_grad_lds_kernel<E, kSteps>), dim3(grid), dim3(512), 0, stream, a);
     return launched();

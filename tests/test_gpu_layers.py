@@ -140,6 +140,23 @@ def test_weight_grad(dtype, rows, channels, outputs):
     assert torch.equal(kept.weight_grad(grad), weight)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("outputs", [1, 2, 3, 4, 15, 16, 17, 18, 31, 32, 33])
+@pytest.mark.parametrize("rows,channels", [(8, 1), (9, 33), (265, 64), (5000, 130)])
+def test_weight_grad_of_few_outputs(dtype, outputs, rows, channels):
+    x = values(rows, channels, TYPES[dtype], seed=2)
+    wide = values(rows, outputs, TYPES[dtype], seed=3, wide=outputs + 2).clone()
+    storage = torch.full((rows, outputs + 2), math.nan, dtype=TYPES[dtype], device="cuda")  # what is beside the gradient is not read
+    storage[:, 1:-1] = wide
+    grad = storage[:, 1:-1]
+    weight, bias = layers.checkpoint(x).weight_grad(grad, bias=True, dtype=torch.float32)
+    back, g = ref.kept(x), wide.double()
+    chain = 2 * (rows / 64 + 2048)  # (as above)
+    assert_near(weight, g.t().contiguous() @ back, g.abs().t().contiguous() @ back.abs(), chain, "weight")
+    assert_near(bias, g.sum(0), g.abs().sum(0), chain, "bias")
+    assert torch.equal(weight, layers.checkpoint(x).weight_grad(wide, dtype=torch.float32))
+
+
 def test_weight_grad_takes_gradients_whole():
     """Single rows: a product has to come back as it is, whatever the bits and the magnitude of the gradient; infinities and NaN stay in their row and column."""
     for dtype in TYPES.values():
