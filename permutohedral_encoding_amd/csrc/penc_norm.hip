@@ -123,35 +123,18 @@ struct Place {
         const int c = min(first, static_cast<int>(kept.pitch) - kChunk);
         return {*reinterpret_cast<const uint2*>(kept.values + offset_of(row, kept.pitch) + c), kept.exponents[offset_of(row, kept.blocks) + c / kKeptBlock]};
     }
-    // (with masks in place of conditions: of those the compiler makes a branch for each channel)
     template <class T>
     __device__ __forceinline__ void bring(const Fetched<T>& f, Values& x) const {
-        constexpr int kWords = kChunk * sizeof(T) / 4;
         auto w = f.w;
         if constexpr (!kNarrow) {
             const uint32_t whole = valid == kChunk ? ~0u : 0u;
             if constexpr (kWhole) {
+                w &= whole;
+            } else {  // the row's last lane
+                const auto m = to_front<T>(w, kChunk - (channels & 7));
+                const uint32_t part = ~whole & (valid > 0 ? ~0u : 0u);
 #pragma unroll
-                for (int i = 0; i < kWords; ++i) w[i] &= whole;
-            } else {
-                // the row's last lane: forward by 8 - valid
-                const int by = kChunk - (channels & 7);
-                const uint32_t part = ~whole & (valid > 0 ? ~0u : 0u), by4 = by & 4 ? ~0u : 0u, by2 = by & 2 ? ~0u : 0u, by1 = by & 1 ? ~0u : 0u;
-                auto m = w;
-                const auto forward = [&](int n, uint32_t mask) {
-#pragma unroll
-                    for (int i = 0; i < kWords; ++i) m[i] = (i + n < kWords ? m[i + n < kWords ? i + n : 0] & mask : 0u) | (m[i] & ~mask);
-                };
-                forward(kWords / 2, by4);
-                forward(kWords / 4, by2);
-                if constexpr (kWords == kChunk) {
-                    forward(1, by1);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kWords; ++i) m[i] = __builtin_amdgcn_alignbit(i + 1 < kWords ? m[i + 1 < kWords ? i + 1 : 0] : 0u, m[i], by1 & 16u);
-                }
-#pragma unroll
-                for (int i = 0; i < kWords; ++i) w[i] = (w[i] & whole) | (m[i] & part);
+                for (int i = 0; i < static_cast<int>(kChunk * sizeof(T) / 4); ++i) w[i] = (w[i] & whole) | (m[i] & part);
             }
         }
         const float8 v = __builtin_convertvector(__builtin_bit_cast(T __attribute__((ext_vector_type(kChunk))), w), float8);
@@ -163,32 +146,10 @@ struct Place {
     }
     template <class T>
     __device__ __forceinline__ void store(T* __restrict__ row, const Values& x) const {
-        if (valid > 0) store_part(row + first, x);
-    }
-    // (of a whole chunk at once, of a part in fours, twos and ones)
-    template <class T>
-    __device__ __forceinline__ void store_part(T* __restrict__ p, const Values& x) const {
-        float8 v;
-        PENC_EACH v[i] = x[i];
-        const auto y = __builtin_convertvector(v, T __attribute__((ext_vector_type(kChunk))));
-        if (kWhole || valid == kChunk) {
-            *reinterpret_cast<chunk_t<T>*>(p) = y;
-            return;
-        }
-        using Four = T __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-        using Two = T __attribute__((ext_vector_type(2), aligned(sizeof(T))));
-        const int n = channels & 7;
-        if (n & 4) *reinterpret_cast<Four*>(p) = __builtin_shufflevector(y, y, 0, 1, 2, 3);
-        if (n & 2) {
-            if (n & 4) *reinterpret_cast<Two*>(p + 4) = __builtin_shufflevector(y, y, 4, 5);
-            else *reinterpret_cast<Two*>(p) = __builtin_shufflevector(y, y, 0, 1);
-        }
-        if (n & 1) {
-            if (n == 1) p[0] = y[0];
-            else if (n == 3) p[2] = y[2];
-            else if (n == 5) p[4] = y[4];
-            else p[6] = y[6];
-        }
+        if (valid <= 0) return;
+        const auto y = rounded<T>(x);
+        if (kWhole || valid == kChunk) store_whole(row + first, y);
+        else store_part(row + first, channels & 7, y);
     }
     // a parameter, or `none` for each channel
     __device__ __forceinline__ void param(const void* p, bool fp32, float none, Values& x, uint64_t at = 0) const {

@@ -206,6 +206,40 @@ def test_activation(dtype, kind, gated, rows, channels):
         assert torch.equal(layers.activation(x, kind, gated=gated), y)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels", [(7, 24), (50, 70), (41, 96), (1, 130), (33, 200), (3, 2100), (2, 2080), (5, 5000), (2, 66001)])
+def test_rows_of_any_length_share_lanes(dtype, rows, channels):
+    """Lanes of a row that are no power of two, and rows that take several turns of a workgroup: a row's results are those of the row alone."""
+    x = values(rows, channels, TYPES[dtype], seed=4, wide=channels + 3)
+    kept = layers.checkpoint(x)
+    q, e = ref.kept_arrays(x)
+    assert torch.equal(kept.values[:, :channels].double(), q[:, :channels]) and torch.equal(kept.exponents.double(), e + 127)
+    assert not kept.values[:, channels:].any() and torch.equal(kept.unpack(torch.float32).double(), ref.kept(x))
+    x = x.detach().requires_grad_(True)
+    y = layers.activation(x, "gelu")
+    grad = values(rows, channels, TYPES[dtype], seed=5)
+    dx, = torch.autograd.grad(y, x, grad)
+    back = ref.kept(x.detach())
+    assert_near(y, ref.act(x.detach().double(), "gelu"), x.detach().double().abs() + 1, 64, "y")
+    assert_near(dx, grad.double() * ref.act_slope(back, "gelu"), grad.double().abs() * (back.abs() + 1), 64, "dx")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels", [(1, 7), (1, 8), (2047, 1), (2049, 1), (683, 3), (686, 3), (2048, 5), (29, 212), (1 << 17, 33)])
+def test_dense_rows_without_a_checkpoint_are_one_after_the_other(dtype, rows, channels):
+    x, grad = values(rows, channels, TYPES[dtype], seed=6).contiguous(), values(rows, channels, TYPES[dtype], seed=7).contiguous()
+    apart, grad_apart = (torch.full((rows, channels + 1), math.nan, dtype=t.dtype, device="cuda")[:, :channels].copy_(t) for t in (x, grad))
+    for kind in ("silu", "softplus"):
+        out = []
+        for a, g in ((x, grad), (apart, grad_apart), (x, grad_apart)):
+            leaf = a.detach().requires_grad_(True)
+            y = layers.activation(leaf, kind, keep_8bit=False)
+            out.append((y, layers.activation(a, kind), *torch.autograd.grad(y, leaf, g)))
+        for y, alone, dx in out:
+            assert torch.equal(y, out[1][0]) and torch.equal(alone, y) and torch.equal(dx, out[1][2])
+        assert_near(out[0][0], ref.act(x.double(), kind), x.double().abs() + 1, 64, "y")
+
+
 def test_activations_far_out():
     x = torch.tensor([[-1e30, -200.0, -90.0, -20.0, -0.0, 0.0, 20.0, 90.0, 200.0, 1e30]], device="cuda")
     for kind, below in (("gelu", 0.0), ("silu", 0.0), ("softplus", 0.0)):
