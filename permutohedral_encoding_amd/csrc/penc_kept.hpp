@@ -71,7 +71,8 @@ __device__ __forceinline__ void load_chunk(const E* __restrict__ row, int c, int
         chunk_words<E> w = *reinterpret_cast<const Unaligned*>(row + min(c, channels - kChunk));
         const uint32_t whole = c + kChunk <= channels ? ~0u : 0u;
         if (channels % kChunk == 0) {
-            w &= whole;
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(kChunk * sizeof(E) / 4); ++i) w[i] &= whole;
         } else {
             const chunk_words<E> m = to_front<E>(w, kChunk - channels % kChunk);
             const uint32_t part = ~whole & (c < channels ? ~0u : 0u);

@@ -128,8 +128,9 @@ struct Place {
         auto w = f.w;
         if constexpr (!kNarrow) {
             const uint32_t whole = valid == kChunk ? ~0u : 0u;
-            if constexpr (kWhole) {
-                w &= whole;
+            if constexpr (kWhole) {  // (word by word: of the vectors' own operators the backward spills, 16384 x 4096 bf16 156 -> 165 us)
+#pragma unroll
+                for (int i = 0; i < static_cast<int>(kChunk * sizeof(T) / 4); ++i) w[i] &= whole;
             } else {  // the row's last lane
                 const auto m = to_front<T>(w, kChunk - (channels & 7));
                 const uint32_t part = ~whole & (valid > 0 ? ~0u : 0u);
