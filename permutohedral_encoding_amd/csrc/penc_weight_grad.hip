@@ -216,7 +216,7 @@ __device__ __forceinline__ int64_t item_of(const WeightGrad& a) {
 }
 
 // 16 kWideO outputs by 16 kWideC channels.  Bound by memory: each operand is read once for 64 columns of the other.  1048576 x 48 by 64 outputs fp32 74 us,
-// 4.3 TB/s (a wave's next rows are on their way while it multiplies; without that 82).  kWideO is 4, or 1 or 2 for 16 or 32 outputs and fewer, which leave the
+// 4.3 TB/s (a wave's next rows are on their way while it multiplies; without that 82).  kWideO is 4, or 1 or 2 for 16 or 32 outputs and fewer (and for few rows), which leave the
 // registers and LDS of a second workgroup: 1048576 x 64 by 1 output fp32 64 -> 25 us, by 16 51 -> 28, by 32 52 -> 43; bf16 by 3 53 -> 18, by 32 27 -> 28.
 template <class E, int kWideO, int kWideC, int kWaves, bool kRagged>
 __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) {
@@ -496,11 +496,15 @@ constexpr int64_t kMostStride = 1 << 22;
 // 1024 x 1024 fp32, 4096 rows 51 -> 65, 16384 178 -> 131.  Fewer rows do not fill the card with large tiles; one row of 1024 x 1024 7 -> 9.
 constexpr int64_t kLargeProduct = int64_t{1} << 34;
 
+// Of few rows the tiles are narrower, until there are as many workgroups.  us, fp32 by 64 outputs: 200 x 1024 8.5 -> 6.8,
+// 1000 x 64 11.0 -> 9.4, 16384 x 32 12.1 -> 9.7; bf16 1000 x 32 10.0 -> 9.4.
+constexpr int64_t kFewGroups = 128;
+
 // How a product is cut up.
 struct WeightPlan {
     int block, splits;  // columns of a workgroup, channels and (but where they are few) outputs; workgroups of a tile
     bool ragged;
-    int wide;  // sixteens of outputs of a workgroup with 64 channels
+    int wide;  // sixteens of outputs of a workgroup that has 64 channels
     int64_t split_rows;
     int output_tiles, channel_tiles;
 };
@@ -508,14 +512,16 @@ WeightPlan weight_plan(int type, int64_t rows, int64_t channels, int64_t outputs
     WeightPlan p{};
     // (a lane takes 8 rows, at 32-bit offsets from a step's first row)
     p.ragged = rows < kLaneRows || grad_stride > kMostStride;
-    p.wide = p.ragged || outputs > 32 ? 4 : outputs > 16 ? 2 : 1;
     const int64_t pieces_of_a_value = type == PENC_FP32 ? 3 : type == PENC_FP16 ? 2 : 1;
     const bool large = !p.ragged && channels > 128 && outputs > 128 && rows * channels * outputs * pieces_of_a_value >= kLargeProduct;
     p.block = large ? kLargeBlock : 64;
-    p.output_tiles = static_cast<int>((outputs + p.block - 1) / p.block);
     p.channel_tiles = static_cast<int>((channels + p.block - 1) / p.block);
-    const int64_t tiles = static_cast<int64_t>(p.output_tiles) * p.channel_tiles, at_a_time = 8 * kStep;
-    const int64_t pieces = std::max<int64_t>(1, (rows + at_a_time - 1) / at_a_time);
+    const int64_t at_a_time = 8 * kStep, pieces = std::max<int64_t>(1, (rows + at_a_time - 1) / at_a_time);
+    const auto tiles_of = [&](int outputs_of_tile) { return static_cast<int>((outputs + outputs_of_tile - 1) / outputs_of_tile); };
+    p.wide = p.ragged || outputs > 32 ? 4 : outputs > 16 ? 2 : 1;
+    while (!p.ragged && !large && p.wide > 1 && tiles_of(16 * p.wide) * p.channel_tiles * pieces < kFewGroups) p.wide /= 2;
+    p.output_tiles = tiles_of(large ? kLargeBlock : 16 * p.wide);
+    const int64_t tiles = static_cast<int64_t>(p.output_tiles) * p.channel_tiles;
     const int64_t wanted = std::max<int64_t>(1, std::min(pieces, (p.wide < 4 ? 512 : 256) / tiles));
     p.split_rows = (pieces + wanted - 1) / wanted * at_a_time;
     p.splits = static_cast<int>(std::max<int64_t>(1, (rows + p.split_rows - 1) / p.split_rows));
