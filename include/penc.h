@@ -406,9 +406,10 @@ int penc_simplex_debug(int pos_dim, int64_t nr_positions, int nr_levels, int cap
  * The layers behind the encoding.  No counterpart in the reference, whose scripts take them from torch.
  *
  * Rows of `channels` values of a type below; a row stride is counted in values, and channels of a row are adjacent
- * unless an entry point has a stride for them.  Arrays need the alignment of one value, checkpoints 16 bytes.  No rows is a valid call that
- * writes nothing (sums over the rows become zero).  Numbers of rows and row strides stay below 2^31.  Sums, statistics and steps are fp32, results are rounded once, to nearest, ties to even, and do not
- * depend on the order in which workgroups run.
+ * unless an entry point has a stride for them.  Arrays need the alignment of one value, checkpoints 16 bytes, and no array that is written
+ * overlaps another.  No rows is a valid call that writes nothing (sums over the rows become zero).  Numbers of rows and row strides stay below
+ * 2^31.  Sums, statistics and steps are fp32, results are rounded once, to nearest, ties to even, and do not depend on the order in which
+ * workgroups run.
  *
  * A checkpoint keeps rows in 8 bits, in blocks of 32 channels.  With a the largest magnitude of a block, e = the least integer of at least
  * -126 with a / 2^e < 127.5, and q = x / 2^e rounded, ties to even (e at most 121, q at most 127: values from 127.5 * 2^121 on come back as 127 * 2^121):
@@ -443,7 +444,7 @@ int penc_activation_backward(int type, int kind, int gated, int64_t rows, int64_
                              const uint8_t* exponents, const void* grad, int64_t grad_row_stride, void* dx, void* stream);
 
 /* weight_grad[o][c] = sum over the rows of grad[row][o] * x^[row][c] and (may be NULL) bias_grad[o] = sum of grad[row][o], both of result_type: what a
- * linear layer with `outputs` outputs needs of its kept input.  `workspace` holds partial sums (penc_weight_grad_workspace_bytes, 0: none needed). */
+ * linear layer with `outputs` outputs needs of its kept input.  `workspace` holds partial sums (penc_weight_grad_workspace_bytes; 0 for sizes that are refused). */
 size_t penc_weight_grad_workspace_bytes(int64_t rows, int64_t channels, int64_t outputs);
 int penc_weight_grad(int type, int result_type, int64_t rows, int64_t channels, int64_t outputs, const int8_t* values, const uint8_t* exponents,
                      const void* grad, int64_t grad_row_stride, void* weight_grad, void* bias_grad, void* workspace, size_t workspace_bytes,
@@ -463,13 +464,13 @@ typedef struct penc_norm {
     float residual_scale, eps;
     int64_t rows, channels;
     int64_t rows_per_gate;   /* 0: one gate of `channels` values for all rows; else this many consecutive rows (rows is a multiple) share one */
-    const void* x;           /* backward: NULL where x is kept */
+    const void* x;           /* backward: not read where x is kept */
     int64_t x_stride;
-    const void* branch;      /* forward: NULL: y = residual_scale * x; backward: NULL where it is kept or there is none */
+    const void* branch;      /* read with has_branch (without: y = residual_scale * x); backward: not read where it is kept */
     int64_t branch_stride;
     int has_branch;
     const void *gate, *post_weight, *post_bias, *pre_weight, *pre_bias; /* each may be NULL: 1, or 0 for a bias */
-    int8_t* x_values;        /* checkpoints of x and branch, written by the forward where not NULL, read by the backward where x, branch are NULL */
+    int8_t* x_values;        /* checkpoints of x and branch, written by the forward and read by the backward where not NULL */
     uint8_t* x_exponents;
     int8_t* branch_values;
     uint8_t* branch_exponents;

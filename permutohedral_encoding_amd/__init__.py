@@ -3,6 +3,7 @@
 from .modules import PermutoEncoding, Coarse2Fine
 from .funcs import PermutoEncodingFunc, PermutoEncodingFuncBack
 from .utils import map_range_val, cosine_easing_window
+from . import layers
 
 __all__ = ["PermutoEncoding", "Coarse2Fine", "PermutoEncodingFunc", "PermutoEncodingFuncBack", "map_range_val",
-           "cosine_easing_window"]
+           "cosine_easing_window", "layers"]
