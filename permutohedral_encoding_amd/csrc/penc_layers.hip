@@ -144,8 +144,10 @@ __device__ __forceinline__ void activate(float x, float& value, float& slope) {
         value = x * s;
         slope = s * (1.0f + x * (1.0f - s));
     } else {
-        const float e = expf(-fabsf(x)), r = __builtin_amdgcn_rcpf(1.0f + e);
-        value = fmaxf(x, 0.0f) + log1pf(e);
+        // log(1 + e) with e in 0..1: u = 1 + e leaves c = e - (u - 1) of e behind, both differences exact, and log(u + c) = log(u) + c / u up to c^2.
+        // (69757 x 2 161 fp16 gated, forward and back: log1pf 54 and 61 us, this 23 and 24)
+        const float e = expf(-fabsf(x)), u = 1.0f + e, c = e - (u - 1.0f), r = __builtin_amdgcn_rcpf(u);
+        value = fmaxf(x, 0.0f) + __builtin_fmaf(c, r, 0.69314718f * __builtin_amdgcn_logf(u));
         slope = x < 0.0f ? e * r : r;
         if (x != x) value = slope = x;
     }

@@ -206,6 +206,16 @@ def test_activation(dtype, kind, gated, rows, channels):
         assert torch.equal(layers.activation(x, kind, gated=gated), y)
 
 
+def test_softplus_of_small_results():
+    """Relative to the result, down to where it is exp(x): exp 2 units, the logarithm 1, two products and a sum of half a unit each, the reciprocal's share
+    far below: 5 units of 2^-23 at most, here 8.  (Left of 88 the sum is x and less than a unit more.)"""
+    x = torch.cat([torch.linspace(-85.0, 88.0, 1 << 20, device="cuda"), torch.linspace(-18.0, -14.0, 1 << 18, device="cuda"),
+                   torch.linspace(-1e-3, 1e-3, 1 << 16, device="cuda")])[None]
+    want = ref.act(x.double(), "softplus")
+    error = (layers.activation(x, "softplus").double() - want).abs() / want
+    assert float(error.max()) <= 8 * 2.0 ** -23, float(error.max() * 2 ** 23)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,channels", [(7, 24), (50, 70), (41, 96), (1, 130), (33, 200), (3, 2100), (2, 2080), (5, 5000), (2, 66001)])
 def test_rows_of_any_length_share_lanes(dtype, rows, channels):
