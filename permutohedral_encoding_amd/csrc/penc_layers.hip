@@ -10,9 +10,9 @@
 // written (a copy on this card reaches 5.5 TB/s; what fits the 256 MB cache in front of the memory, more):
 //
 //     pack, channels adjacent     65536 x 1024 bf16  38, 5.3 TB/s      1048576 x 48 fp32  44, 5.8 TB/s
-//     pack, rows adjacent                                              1048576 x 48 fp32  62, 4.1 TB/s
-//     unpack                      65536 x 1024 bf16  31, 6.6 TB/s      1048576 x 48 fp32  42, 6.1 TB/s
-//     gated silu                  32765 x 2 2048 bf16: forward with its checkpoints 98, 5.5 TB/s; backward from them 98, 5.5 TB/s
+//     pack, rows adjacent                                              1048576 x 48 fp32  60, 4.2 TB/s
+//     unpack                      65536 x 1024 bf16  31, 6.6 TB/s      1048576 x 48 fp32  38, 6.7 TB/s
+//     gated silu                  32765 x 2 2048 bf16: forward with its checkpoints 93, 5.8 TB/s; backward from them 93, 5.8 TB/s
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
