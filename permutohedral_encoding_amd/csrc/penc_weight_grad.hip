@@ -216,8 +216,9 @@ __device__ __forceinline__ int64_t item_of(const WeightGrad& a) {
 }
 
 // 16 kWideO outputs by 16 kWideC channels.  Bound by memory: each operand is read once for 64 columns of the other.  1048576 x 48 by 64 outputs fp32 74 us,
-// 4.3 TB/s (a wave's next rows are on their way while it multiplies; without that 82).  kWideO is 4, or 1 or 2 for 16 or 32 outputs and fewer (and for few rows), which leave the
-// registers and LDS of a second workgroup: 1048576 x 64 by 1 output fp32 64 -> 25 us, by 16 51 -> 28, by 32 52 -> 43; bf16 by 3 53 -> 18, by 32 27 -> 28.
+// 4.3 TB/s (a wave's next rows are on their way while it multiplies; without that 82).  kWideO is 4, or 1 or 2 for 16 or 32 outputs and fewer (and for few
+// rows), which leave the registers and LDS of a second workgroup: 1048576 x 64 by 1 output fp32 64 -> 25 us, by 16 51 -> 28, by 32 52 -> 43; bf16 by 3
+// 53 -> 18, by 32 27 -> 28.
 template <class E, int kWideO, int kWideC, int kWaves, bool kRagged>
 __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) {
     constexpr int kPieces = GradTile<E, kWideO>::kPieces;
