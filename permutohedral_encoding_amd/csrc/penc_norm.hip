@@ -152,9 +152,9 @@ struct Place {
         if (kWhole || valid == kChunk) store_whole(row + first, y);
         else store_part(row + first, channels & 7, y);
     }
-    // a parameter, or `none` for each channel
+    // a parameter, or `none` for each channel; behind the row's end 0 in either case, which takes away what the mean of a "layer" leaves there of a gradient
     __device__ __forceinline__ void param(const void* p, bool fp32, float none, Values& x, uint64_t at = 0) const {
-        if (p == nullptr) PENC_EACH x[i] = none;
+        if (p == nullptr) PENC_EACH x[i] = i < valid ? none : 0.0f;
         else if (fp32) bring(fetch(static_cast<const float*>(p) + at), x);
         else bring(fetch(static_cast<const E*>(p) + at), x);
     }

@@ -370,6 +370,25 @@ def test_parts_of_a_residual_norm(kind):
         assert_near(got, *want[name], K + 37, name)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("given", ["", "gate", "post_weight", "post_bias", "pre_weight", "post_weight pre_weight", "post_bias pre_bias", "gate post_bias",
+                                   "gate post_weight post_bias pre_weight pre_bias"])
+def test_parameters_that_are_not_given(dtype, kind, given):
+    """They count as 1 (a bias: 0) in the row, and for nothing in the lanes behind its end; with upstream gradients whose mean is not zero."""
+    for rows, channels in ((5, 3), (9, 8), (2, 9), (7, 48), (33, 64), (33, 72), (33, 203), (9, 520), (9, 1000), (5, 1024), (2, 2051), (3, 5000)):
+        s = norm_case(rows, channels, dtype, "fp32", kind, gate=0)
+        generator = torch.Generator(device="cuda").manual_seed(8)
+        for name in ("gate", "post_weight", "post_bias", "pre_weight", "pre_bias"):
+            if name not in given.split():
+                s[name] = None
+            elif s[name] is None:
+                s[name] = 0.1 * torch.randn(channels, generator=generator, device="cuda")
+        s["grad_y"], s["grad_n"] = s["grad_y"] + 0.5, s["grad_n"] + 1.0
+        for keep_8bit in (True, False):
+            check_norm(s, kind=kind, keep_8bit=keep_8bit)
+
+
 def test_a_row_of_zeros_has_a_norm():
     x = torch.zeros(4, 64, device="cuda", requires_grad=True)
     f = torch.zeros(4, 64, device="cuda", requires_grad=True)
