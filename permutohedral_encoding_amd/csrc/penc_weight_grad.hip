@@ -167,11 +167,10 @@ struct KeptTile {
             row[j][kWide / 4] = there ? kept.exponents[(first + j) * kept.blocks + column / kKeptBlock] : 0;
         }
     }
-    // q 2^e as (q + 128) 2^e - 2^(e + 7), exact, of bytes that v_cvt_f32_ubyte takes where they are
+    // q 2^e, exact
     template <class W>
     __device__ __forceinline__ static uint32_t value(const W& row, int t) {
-        const float biased = static_cast<float>((row[t / 4] ^ 0x80808080u) >> 8 * (t % 4) & 0xFFu), step = kept_step(row[kWide / 4]);
-        return __float_as_uint(__builtin_fmaf(biased, step, -128.0f * step));
+        return __float_as_uint(static_cast<float>(static_cast<int8_t>(row[t / 4] >> 8 * (t % 4))) * kept_step(row[kWide / 4]));
     }
     template <class W>
     __device__ __forceinline__ static Frag column(const W (&row)[kLaneRows], int t) {

@@ -177,6 +177,27 @@ def test_weight_grad_takes_gradients_whole():
     assert torch.isnan(weight[0, :32]).all() and torch.equal(weight[0, 32:], torch.full((8,), 2.0, device="cuda"))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels,outputs", [(3, 40, 5), (300, 70, 3), (40000, 48, 20), (40000, 48, 64), (150001, 300, 390)])
+def test_weight_grad_of_blocks_at_the_top_of_the_range(dtype, rows, channels, outputs):
+    """The largest step there is, beside zeros and ordinary rows: values as `unpack` has them, for gradients of every type in tiles of every size.  (Gradients
+    are so small that no sum overflows: 1600 rows of 3.4e38 times at most 2^-24 * 128.)"""
+    x = values(rows, channels, torch.float32, seed=4)
+    top = torch.zeros(channels, device="cuda")
+    top[:6] = torch.tensor([3.4028234e38, -3.4028234e38, 1.7e38, 0.0, -1e30, 1.0], device="cuda")
+    top[-1] = -3.4e38
+    x[::97] = top
+    x[-1] = top
+    grad = (values(rows, outputs, torch.float32, seed=5).clamp(-128, 128) * 2.0 ** -24).to(TYPES[dtype])
+    kept = layers.checkpoint(x)
+    back, g = kept.unpack().double(), grad.double()
+    assert torch.isfinite(back).all() and torch.equal(back, ref.kept(x))
+    weight = kept.weight_grad(grad, dtype=torch.float32)
+    # A wave adds at most the rows of a workgroup, rows / 64 and the rest of a unit of 256, three times over where a gradient is in three parts, and their
+    # sums are one more chain of at most 256; a factor of two for additions that do not round to nearest.
+    assert_near(weight, g.t().contiguous() @ back, g.abs().t().contiguous() @ back.abs(), 2 * (3 * (rows / 64 + 256) + 256), "weight")
+
+
 # ------------------------------------------------------------------------------------------ activations
 
 @pytest.mark.parametrize("dtype", TYPES)
