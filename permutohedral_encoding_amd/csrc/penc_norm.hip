@@ -152,11 +152,15 @@ struct Place {
         if (kWhole || valid == kChunk) store_whole(row + first, y);
         else store_part(row + first, channels & 7, y);
     }
-    // a parameter, or `none` for each channel; behind the row's end 0 in either case, which takes away what the mean of a "layer" leaves there of a gradient
-    __device__ __forceinline__ void param(const void* p, bool fp32, float none, Values& x, uint64_t at = 0) const {
-        if (p == nullptr) PENC_EACH x[i] = i < valid ? none : 0.0f;
-        else if (fp32) bring(fetch(static_cast<const float*>(p) + at), x);
+    // a parameter, 0 behind the row's end
+    __device__ __forceinline__ void given(const void* p, bool fp32, Values& x, uint64_t at = 0) const {
+        if (fp32) bring(fetch(static_cast<const float*>(p) + at), x);
         else bring(fetch(static_cast<const E*>(p) + at), x);
+    }
+    // the same, or `none` for each channel; 0 behind the row's end takes away what the mean of a "layer" leaves there of a gradient
+    __device__ __forceinline__ void param(const void* p, bool fp32, float none, Values& x) const {
+        if (p != nullptr) given(p, fp32, x);
+        else PENC_EACH x[i] = i < valid ? none : 0.0f;
     }
     // (a difference to the mean is zero behind the row's end)
     __device__ __forceinline__ void centre(Values& x, float mean) const {
@@ -241,7 +245,7 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_kernel(NormArgs a,
         at.param(a.post_bias, a.param_fp32, 0.0f, post_bias);
         at.param(a.pre_bias, a.param_fp32, 0.0f, pre_bias);
     }
-    if (a.rows_per_gate == 0) at.param(a.gate, a.gate_fp32, 1.0f, gate);
+    at.param(a.gate, a.gate_fp32, 1.0f, gate);
     struct Fetched {
         typename P::template Fetched<E> x, f;
     };
@@ -262,7 +266,7 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads) void norm_kernel(NormArgs a,
         if (a.rows_per_gate != 0 && row >= gate_until) {
             const row_t group = row / a.rows_per_gate;
             gate_until = (group + 1) * a.rows_per_gate;
-            at.param(a.gate, a.gate_fp32, 1.0f, gate, offset_of(group, a.channels));
+            if (a.gate != nullptr) at.given(a.gate, a.gate_fp32, gate, offset_of(group, a.channels));
         }
         at.bring(fetched.x, x);
         if (a.kept_x.values != nullptr) a.kept_x.store(row, at.first, x);
@@ -449,10 +453,10 @@ __global__ __launch_bounds__(Row<kLanes>::kThreads, !kFull ? 4 : kLanes == 512 ?
             end = min(first + g.piece_rows, (group + 1) * a.rows_per_gate);
             first += threadIdx.x / kLanes;
             stride = R::kRows;
-            at.param(a.gate, a.gate_fp32, 1.0f, gate, offset_of(group, a.channels));
+            if (a.gate != nullptr) at.given(a.gate, a.gate_fp32, gate, offset_of(group, a.channels));
         }
         walk<kLanes>(first, end, run, stride, fetch, [&](row_t row, bool begins, bool ends, const Fetched& fetched) {
-            if (a.gate_by_lanes && begins) at.param(a.gate, a.gate_fp32, 1.0f, gate, offset_of(group, a.channels));
+            if (a.gate_by_lanes && begins && a.gate != nullptr) at.given(a.gate, a.gate_fp32, gate, offset_of(group, a.channels));
             one_row(row, fetched);
             if (!a.gate_by_lanes || !ends) return;
             if (g.gate != nullptr) store_gate(group, d_gate);

@@ -410,6 +410,29 @@ def test_parameters_that_are_not_given(dtype, kind, given):
             check_norm(s, kind=kind, keep_8bit=keep_8bit)
 
 
+@pytest.mark.parametrize("per_gate", [1, 4, 300])
+def test_groups_of_rows_without_a_gate(per_gate):
+    """Through the C ABI: rows_per_gate and no gate is a gate of ones."""
+    import ctypes
+
+    from permutohedral_encoding_amd import _native
+    from test_layers import Norm, NormGrads
+    lib, stream = _native.lib(), torch.cuda.current_stream().cuda_stream
+    s = norm_case(600, 72, "fp32", "fp32", "layer", gate=None)
+    x, f = s["x"].contiguous(), s["f"].contiguous()
+    want = layers.residual_norm(x.requires_grad_(True), f.requires_grad_(True), kind="layer", keep_8bit=False)
+    want += torch.autograd.grad(want, (x, f), (s["grad_y"], s["grad_n"]))
+    y, n, dx, df = got = [torch.empty_like(x) for _ in range(4)]
+    dy, dn = s["grad_y"].contiguous(), s["grad_n"].contiguous()
+    norm = Norm(0, 0, 0, 1, 1, 1, 1.0, 1e-6, 600, 72, per_gate, x.data_ptr(), 72, f.data_ptr(), 72, 1)
+    grads = NormGrads(dy.data_ptr(), 72, dn.data_ptr(), 72, dx.data_ptr(), df.data_ptr())
+    nbytes = lib.penc_residual_norm_workspace_bytes(600, 72, per_gate)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    assert lib.penc_residual_norm(ctypes.byref(norm), y.data_ptr(), n.data_ptr(), stream) == 0
+    assert lib.penc_residual_norm_backward(ctypes.byref(norm), ctypes.byref(grads), workspace.data_ptr(), nbytes, stream) == 0
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_a_row_of_zeros_has_a_norm():
     x = torch.zeros(4, 64, device="cuda", requires_grad=True)
     f = torch.zeros(4, 64, device="cuda", requires_grad=True)
