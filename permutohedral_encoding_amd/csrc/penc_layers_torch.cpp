@@ -292,9 +292,17 @@ Tensor linear(const Tensor& x, const Tensor& weight, const Tensor& bias) {
     {
         at::NoGradGuard no_grad;
         c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
-        y = at::linear(x, weight, bias);
+        // (as rows: of leading dimensions that are not one, at::linear makes a batched product whose right operand is a transposed view, and in 16 bits those
+        // have faulted the GPU)
+        const Tensor rows = x.dim() == 2 ? x.detach() : x.detach().reshape({-1, x.size(-1)});
+        y = at::linear(rows, weight, bias);
+        if (x.dim() != 2) {
+            std::vector<int64_t> sizes = x.sizes().vec();
+            sizes.back() = weight.size(0);
+            y = at::_unsafe_view(y, sizes);  // (a result of its own, and no view of one made without gradients)
+        }
         // (for the bias alone too: its sum comes with the weight's)
-        if (differentiable && (weight.requires_grad() || (bias.defined() && bias.requires_grad()))) kept = keep(x.detach(), "x");
+        if (differentiable && (weight.requires_grad() || (bias.defined() && bias.requires_grad()))) kept = keep(rows, "x");
     }
     if (!differentiable) return y;
     auto node = make_node<LinearNode>();

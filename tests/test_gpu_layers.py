@@ -524,6 +524,42 @@ def test_linear(dtype):
         torch.testing.assert_close(got.reshape(-1), (dx.reshape(-1), dw.reshape(-1), db)[wanted])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_of_any_strides_is_one_product_of_rows(dtype):
+    """Never a batched product (of a transposed right operand in 16 bits: those have faulted the GPU), also where no weight wants a gradient."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Products(TorchDispatchMode):
+        seen = ()
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen += (func.overloadpacket.__name__,)
+            return func(*args, **(kwargs or {}))
+
+    w, b = values(64, 48, TYPES[dtype], seed=1), values(1, 64, TYPES[dtype], seed=2)[0]
+    x = values(120, 48, TYPES[dtype])
+    given = (x, x[7], x.view(2, 60, 48), x.view(4, 30, 48).transpose(0, 1), x.view(5, 24, 48)[:, ::3], x.view(2, 3, 20, 48).transpose(1, 2), x[:40].expand(3, 40, 48),
+             x[:, :1].expand(120, 48).view(4, 30, 48), x.view(2, 60, 48)[:, :0], x.view(3, 40, 48).permute(1, 0, 2)[:1])
+    for t in given:
+        want = torch.nn.functional.linear(t.contiguous().view(-1, 48), w, b).view(*t.shape[:-1], 64)
+        for bias in (b, None):
+            with Products() as products:
+                y = layers.linear(t, w, bias)
+            assert not {"bmm", "baddbmm"} & set(products.seen) and {"mm", "addmm", "linear"} & set(products.seen), products.seen
+            assert y.shape == want.shape and y.is_contiguous()
+            if bias is not None:
+                torch.testing.assert_close(y, want)
+        leaves = [v.detach().requires_grad_(True) for v in (t, w, b)]
+        y = layers.linear(*leaves)
+        y.add_(0)  # (a result like any other: it may be changed in place)
+        grad = values(max(1, y[..., 0].numel()), 64, TYPES[dtype], seed=3)[: y[..., 0].numel()].view(y.shape)
+        dx, dw, db = torch.autograd.grad(y, leaves, grad)
+        kept = layers.checkpoint(t.reshape(-1, 48))
+        weight, bias = kept.weight_grad(grad.reshape(-1, 64), bias=True)
+        torch.testing.assert_close(dx, (grad.reshape(-1, 64) @ w).view(t.shape))
+        assert torch.equal(dw, weight) and torch.equal(db, bias)
+
+
 def decoder(points, width, samples):
     """An encoding and what stands behind it."""
     import numpy as np
