@@ -264,7 +264,7 @@ struct LinearNode : public LayerNode {
 
     std::string name() const override { return "LayersLinearBackward"; }
     variable_list gradients(const variable_list& grads) override {
-        const std::vector<Tensor> t = unpacked();  // weight, the checkpoint of x
+        const std::vector<Tensor> t = unpacked();  // the weight, where x wants a gradient, and the checkpoint of x
         const Tensor g = (grads[0].scalar_type() == type ? grads[0] : grads[0].to(type)).reshape({-1, grads[0].size(-1)});
         const c10::DeviceGuard device(g.device());
         c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
@@ -311,7 +311,9 @@ Tensor linear(const Tensor& x, const Tensor& weight, const Tensor& bias) {
     node->x_sizes = x.sizes().vec();
     node->type = x.scalar_type();
     node->has_bias = bias.defined();
-    node->save({&weight, &kept.bytes});
+    // (the weight for the gradient of x alone: where x wants none, it may be changed before the backward, as with torch's own layer)
+    const Tensor none;
+    node->save({x.requires_grad() ? &weight : &none, &kept.bytes});
     torch::autograd::set_history(y, node);
     return y;
 }

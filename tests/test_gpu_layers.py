@@ -560,6 +560,26 @@ def test_linear_of_any_strides_is_one_product_of_rows(dtype):
         assert torch.equal(dw, weight) and torch.equal(db, bias)
 
 
+def test_linear_keeps_its_weight_for_the_gradient_of_x_alone():
+    """As torch.nn.functional.linear: where x wants no gradient, the weight may be changed before the backward, and hooks do not see it."""
+    x, w, grad = values(50, 48, torch.float32), values(64, 48, torch.float32, seed=1), values(50, 64, torch.float32, seed=2)
+    want, bias = layers.checkpoint(x).weight_grad(grad, bias=True)
+    w, b = w.requires_grad_(True), torch.zeros(64, device="cuda", requires_grad=True)
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (seen.append(t.dtype), t)[1], lambda t: t):
+        y = layers.linear(x, w, b)
+    with torch.no_grad():
+        w.mul_(2)
+    dw, db = torch.autograd.grad(y, (w, b), grad)
+    assert torch.equal(dw, want) and torch.equal(db, bias) and seen == [torch.int8]
+    given = x.detach().requires_grad_(True)
+    y = layers.linear(given, w)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, given, grad)
+
+
 def decoder(points, width, samples):
     """An encoding and what stands behind it."""
     import numpy as np
