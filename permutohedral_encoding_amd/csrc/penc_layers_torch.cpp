@@ -207,9 +207,13 @@ struct LayerNode : public Node {
     }
     variable_list apply(variable_list&& grads) override {
         bool any = false;
-        for (const Tensor& g : grads) {
+        for (Tensor& g : grads) {
             if (!g.defined()) continue;
             any = true;
+            if (g.is_neg()) {  // (the imaginary part of a conjugated gradient, for instance: negated when it is read)
+                at::NoGradGuard no_grad;
+                g = g.resolve_neg();
+            }
             require_plain({&g});
         }
         if (!any) return variable_list(num_outputs());

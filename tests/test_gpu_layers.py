@@ -729,6 +729,21 @@ def test_what_autograd_checks():
         layers.activation(torch.autograd.forward_ad.make_dual(x.detach(), x.detach()))
 
 
+def test_gradients_that_are_negated_when_they_are_read():
+    """What comes back through the imaginary part of a conjugated number."""
+    x, w = values(20, 32, torch.float32).requires_grad_(True), values(16, 32, torch.float32, seed=1)
+    for layer in (layers.activation, layers.norm, lambda t: layers.residual_norm(t, t)[0], lambda t: layers.linear(t, w)):
+        out = []
+        for through_complex in (True, False):
+            y = layer(x)
+            met = []
+            y.register_hook(lambda g: met.append(g.is_neg()))
+            z = (torch.complex(torch.zeros_like(y), y).conj() * (1 + 2j)).real if through_complex else 2 * y
+            out.append(torch.autograd.grad(z.sum(), x)[0])
+            assert met == [through_complex]
+        torch.testing.assert_close(*out)
+
+
 def test_a_step_on_another_stream():
     enc, p, positions = decoder(512, 32, 16)
     grad = values(512, 3, torch.float32)
