@@ -178,6 +178,32 @@ def test_weight_grad_takes_gradients_whole():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("products,channels,outputs", [(150001, 300, 390), (1040001, 129, 129), (280009, 208, 300), (100003, 512, 336), (2205, 2900, 2700)])
+def test_weight_grad_of_large_products(dtype, products, channels, outputs):
+    """The tiles of 256 x 256, from 2^34 multiplications on (a value of fp32 counts three times, of fp16 twice): columns that fill no tile, rows that fill no step,
+    split over workgroups and not (the last), results of each type, with and without a bias."""
+    parts = {"fp32": 3, "fp16": 2, "bf16": 1}[dtype]
+    rows = -(-products // parts)
+    assert parts * rows * channels * outputs >= 1 << 34
+    x = values(rows, channels, TYPES[dtype], wide=channels + 3)
+    grad = (values(rows, outputs + 1, TYPES[dtype], seed=1) / math.sqrt(rows))[:, :outputs]
+    kept = layers.checkpoint(x)
+    back, g = ref.kept(x), grad.double()
+    want = g.t().contiguous() @ back, g.sum(0)
+    magnitude = g.abs().t().contiguous() @ back.abs(), g.abs().sum(0)
+    # A wave adds all the rows of its workgroup, a row as often as it has parts: they are dealt out in units of 256 to as many workgroups of a tile as 256 in all
+    # allow, whose sums are one more chain.  A factor of two for additions that do not round to nearest.
+    splits = max(1, 256 // (-(-channels // 256) * -(-outputs // 256)))
+    chain = 2 * (parts * (rows // splits + 512) + splits)
+    for result in TYPES.values():
+        weight, bias = kept.weight_grad(grad, bias=True, dtype=result)
+        for got, value, m, what in zip((weight, bias), want, magnitude, ("weight", "bias")):
+            assert got.dtype == result
+            assert_near(got, value, m, chain, what)
+        assert torch.equal(weight, kept.weight_grad(grad, dtype=result))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,channels,outputs", [(3, 40, 5), (300, 70, 3), (40000, 48, 20), (40000, 48, 64), (150001, 300, 390)])
 def test_weight_grad_of_blocks_at_the_top_of_the_range(dtype, rows, channels, outputs):
     """The largest step there is, beside zeros and ordinary rows: values as `unpack` has them, for gradients of every type in tiles of every size.  (Gradients

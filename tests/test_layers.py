@@ -71,6 +71,14 @@ def test_the_entry_points_refuse_before_they_launch():
         assert lib.penc_status_string(status) != lib.penc_status_string(99)
 
 
+def test_the_products_that_the_gpu_tests_call_large_are():
+    """The rows of a product of 300 channels by 390 outputs are split over 64 workgroups in tiles of 256 x 256 and over 7 in those of 64 x 64, so that the
+    workspace says which of them fp32 takes from 2^34 multiplications on (three for each of its own)."""
+    lib = _native.lib()
+    splits = lambda rows: lib.penc_weight_grad_workspace_bytes(rows, 300, 390) // (4 * 301 * 390)  # noqa: E731
+    assert splits(50001) > 40 and splits(48000) <= 7
+
+
 def test_the_norms_refuse_before_they_launch():
     lib = _native.lib()
     block, p = _memory()
