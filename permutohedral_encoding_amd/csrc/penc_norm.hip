@@ -128,7 +128,7 @@ struct Place {
         auto w = f.w;
         if constexpr (!kNarrow) {
             const uint32_t whole = valid == kChunk ? ~0u : 0u;
-            if constexpr (kWhole) {  // (word by word: of the vectors' own operators the backward spills, 16384 x 4096 bf16 156 -> 165 us)
+            if constexpr (kWhole) {  // (word by word: of the vectors' own operators the backward spills 38 registers and not 4, 16384 x 4096 bf16 156 -> 165 us)
 #pragma unroll
                 for (int i = 0; i < static_cast<int>(kChunk * sizeof(T) / 4); ++i) w[i] &= whole;
             } else {  // the row's last lane
@@ -310,8 +310,10 @@ __device__ __forceinline__ void write_sum(const Values& sum, float (*__restrict_
 
 // kKept: x and the branch are read from their checkpoints.
 //
-// Waves to a SIMD, by what the kernel needs in registers: 128 do for "rms" without biases, 168 for the others, and more where a workgroup is eight waves,
-// of which a compute unit holds one or two and not one and a half.  (Four waves of "layer" with 4096 channels spill: 331 us instead of 232.)
+// Waves to a SIMD, by what the kernel needs in registers: four, of 128, for "rms" without biases, which 16-bit rows of up to 512 channels fit, wider ones but for 2 to
+// 4 registers that are spilled, fp32 but for up to 14; three, of 168, for the others, which spill none; and two where a workgroup is eight waves, of which a
+// compute unit holds one or two and not one and a half.  Rows of more than 4096 channels are workgroups of 16 waves, which have 128 registers and no choice:
+// "layer" spills 18 to 64 there.  (Four waves of "layer" with 4096 channels spill: 331 us instead of 232.)
 //
 // Gates of groups of rows: with few rows in a group (a.gate_by_lanes) the lanes of a row take whole groups and write their sums themselves; else a
 // workgroup takes a piece of a group, `pieces` of them to a group, and leaves a row of partial sums.  One gate for all rows is one more sum over rows.

@@ -4,7 +4,8 @@
 //
 // A product over the rows, which are the strides of both operands, by v_mfma_f32_16x16x32_bf16.  x^ = q 2^e has at most 7 bits and is exact in
 // bfloat16; a gradient is taken whole: bfloat16 as it is, fp16 as a sum of two and fp32 as a sum of three bfloat16 values (8 bits each, the
-// rest exactly), so that every product is exact and the sums are those of fp32.
+// rest exactly), so that every product is exact and the sums are those of fp32.  (Of fp32 gradients under 2^-110 the last bits would be under bfloat16's
+// least value, 2^-133, and are dropped.)
 //
 // The matrix instruction wants 8 consecutive rows of one column in a lane.  A lane loads them for kWide neighbouring columns (16 bytes of a row in
 // one load; one or two columns where there are few), and v_perm pairs two rows' halves; lane m of 16 then has columns kWide m .. kWide m + kWide - 1,
@@ -311,8 +312,9 @@ __global__ __launch_bounds__(64 * kWaves) void weight_grad_kernel(WeightGrad a) 
 // The same for products that the matrix cores bound: 256 outputs by 256 channels to a workgroup of 8 waves, which bring 32 kSteps rows at a time
 // into the LDS as the matrix instruction takes them, half of the waves the gradient and half the checkpoint (one of either kind on each SIMD), while all of
 // them multiply what was brought before.  Every value is converted once for the workgroup, and a wave's 4 x 8 tiles multiply a fragment 2.7 times.
-// Bound by the matrix cores and what goes on between their instructions: 16384 x 1024 by 4096 outputs bf16 150 us, 0.92 PFLOP/s (the library's product of
-// bf16 operands of these sizes 197 us, and of 8192^3, its best, 1.28 PFLOP/s; the 64-column kernel 495).
+// Bound by the matrix cores and the LDS, which have as much to do: of bf16, 64 rows take the matrix cores 2060 clocks at their peak, and the 192 KB read and
+// 64 KB written 2050 at 128 bytes a clock.  16384 x 1024 by 4096 outputs bf16 145 us with the sum of its splits, 0.95 PFLOP/s (the library's product of bf16
+// operands of these sizes 197 us, and of 8192^3, its best, 1.28 PFLOP/s; the 64-column kernel 286).
 template <class E, int kSteps>
 __global__ __launch_bounds__(512, 2) void weight_grad_lds_kernel(WeightGrad a) {
     constexpr int kBlockO = kLargeBlock, kBlockC = kLargeBlock, kWavesO = 4;
@@ -492,8 +494,8 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(const float* __restrict
 
 constexpr int64_t kMostStride = 1 << 22;
 // Products of as many multiplications (three or two for one of a gradient in parts) go by the larger tiles.  us by 64 columns a side -> by 256:
-// 1024 x 1024 bf16, 4096 rows 27 -> 55, 16384 86 -> 80, 131072 658 -> 331; 256 x 1545 bf16, 16384 rows 51 -> 50; 256 x 256 fp32, 131072 rows 102 -> 85,
-// 1024 x 1024 fp32, 4096 rows 51 -> 65, 16384 178 -> 131.  Fewer rows do not fill the card with large tiles; one row of 1024 x 1024 7 -> 9.
+// 1024 x 1024 bf16, 4096 rows 26 -> 54, 16384 84 -> 75, 131072 643 -> 294; 256 x 1545 bf16, 16384 rows 50 -> 48; 256 x 256 fp32, 131072 rows 90 -> 76,
+// 1024 x 1024 fp32, 4096 rows 47 -> 59, 16384 166 -> 115.  Fewer rows do not fill the card with large tiles; 8 rows of 1024 x 1024 7 -> 9.
 constexpr int64_t kLargeProduct = int64_t{1} << 34;
 
 // Of few rows the tiles are narrower, until there are as many workgroups.  us, fp32 by 64 outputs: 200 x 1024 8.5 -> 6.8,
