@@ -11,9 +11,12 @@ needs in 8 bits a value (a quarter of fp32) and are one pass over memory in eith
 
 All of them take float32, float16 or bfloat16 tensors ``(..., C)`` in GPU memory, on the current stream of the tensor's device, of any strides (rows whose
 channels are adjacent are read in place, as is the encoding's own result).  Sums and statistics are float32, results are rounded once, and
-every call gives the same result for the same inputs.  Every backward is the gradient of the forward at the values that the checkpoint stands for; it
-cannot be differentiated again (an eikonal loss needs layers that can).  Forward and backward can be captured in a graph, under torch's own condition: no graph
-of autograd that was built outside of the capture on the same leaves is still alive.  Autocast does not apply to them.  There is no CPU path.
+every call gives the same result for the same inputs.  Every backward is the gradient of the forward at the values that the checkpoint stands for.  Forward and
+backward can be captured in a graph, under torch's own condition: no graph of autograd that was built outside of the capture on the same leaves is still alive.
+Autocast does not apply to them.  There is no CPU path.
+
+There is no second derivative either: differentiating a gradient of these layers again raises an error.  An eikonal loss, and whatever else is made of the
+gradient with respect to the positions, needs torch's own layers behind the encoding, which itself can be differentiated twice.
 """
 import torch
 
