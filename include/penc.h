@@ -490,6 +490,38 @@ typedef struct penc_norm_grads {
 size_t penc_residual_norm_workspace_bytes(int64_t rows, int64_t channels, int64_t rows_per_gate);
 int penc_residual_norm_backward(const penc_norm* norm, const penc_norm_grads* grads, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Rows that go to experts.  No counterpart in the reference.  A row has `choices` experts, numbered from 0; any other number is no expert.  Choice i of
+ * rows * choices (row i / choices) stands at positions[i] when choices are sorted by expert: those of one expert in their order, those of none behind all others.
+ * offsets[e] is where expert e's begin, offsets[experts] how many choices have one ("routed"): plans as penc_plan makes them.  Rows behind the routed ones are
+ * not read, and zero where they are written.  What is said above of strides, alignment, overlap, rounding and order holds here too. */
+#define PENC_MAX_EXPERTS 1024
+#define PENC_MAX_ROUTED 8     /* choices that penc_route makes */
+#define PENC_MAX_CHOICES 1024 /* choices of a row in a plan */
+
+/* The `choices` largest logits of each row (a NaN is the largest; the lowest index first among equal ones; -inf is never chosen: where nothing else is left,
+ * expert -1 with weight 0) and their weights exp(l - top) / sum of exp(l - top), over the chosen (normalise) or over all. */
+int penc_route(int type, int64_t rows, int experts, int choices, int normalise, const void* logits, int64_t row_stride, float* weights, int32_t* chosen,
+               void* stream);
+/* dlogits (dense rows of `type`) from the gradient of the weights; `logits` is read without `normalise` alone. */
+int penc_route_backward(int type, int64_t rows, int experts, int choices, int normalise, const void* logits, int64_t row_stride, const float* weights,
+                        const int32_t* chosen, const float* grad, void* dlogits, void* stream);
+
+/* positions[items] and offsets[experts + 1] of `items` choices, numbers of index_bytes (4 or 8) bytes. */
+size_t penc_plan_workspace_bytes(int64_t items, int experts);
+int penc_plan(int index_bytes, int64_t items, int experts, const void* chosen, int32_t* positions, int32_t* offsets, void* workspace, size_t workspace_bytes,
+              void* stream);
+
+/* sorted[positions[i]] = x[i / choices] (dense rows).  `routed` is a device pointer, offsets + experts of the plan.  Its backward is penc_combine without weights. */
+int penc_dispatch(int type, int64_t rows, int choices, int64_t channels, const void* x, int64_t row_stride, const int32_t* positions, const int32_t* routed,
+                  void* sorted, void* stream);
+/* out[t] (dense rows) = sum over j of weights[t][j] (of weight_type: `type` or PENC_FP32; NULL: 1) * y[positions[t * choices + j]]. */
+int penc_combine(int type, int weight_type, int64_t rows, int choices, int64_t channels, const void* y, int64_t row_stride, const void* weights,
+                 const int32_t* positions, const int32_t* routed, void* out, void* stream);
+/* dy (dense rows; may be NULL) and dweights (dense, of weight_type; may be NULL, y is then not read). */
+int penc_combine_backward(int type, int weight_type, int64_t rows, int choices, int64_t channels, const void* grad, int64_t grad_row_stride, const void* y,
+                          int64_t row_stride, const void* weights, const int32_t* positions, const int32_t* routed, void* dy, void* dweights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

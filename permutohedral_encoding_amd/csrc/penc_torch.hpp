@@ -16,6 +16,9 @@ using at::Tensor;
 // penc_layers_torch.cpp: takes its entry points from the library; adds its functions to the module.
 void bind_layers(void* library);
 bool add_layer_functions(PyObject* module);
+// penc_experts_torch.cpp, likewise
+void bind_experts(void* library);
+bool add_expert_functions(PyObject* module);
 
 #define PENC_REQUIRE(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
 

@@ -22,7 +22,7 @@ import torch
 
 from . import _native
 
-__all__ = ["Checkpoint", "checkpoint", "linear", "activation", "norm", "residual_norm"]
+__all__ = ["Checkpoint", "checkpoint", "linear", "activation", "norm", "residual_norm", "Routing", "route", "routing", "dispatch", "combine"]
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # PENC_FP32, PENC_FP16, PENC_BF16 (include/penc.h)
 _ACTIVATIONS = {"gelu": 0, "silu": 1, "softplus": 2}
@@ -118,3 +118,40 @@ def residual_norm(x, branch, gate=None, residual_scale=1.0, post_weight=None, po
     y, n = _bridge().layers_residual_norm(x, branch, gate, post_weight, post_bias, pre_weight, pre_bias, residual_scale, post_norm, pre_norm,
                                                  _code(_NORMS, kind, "kind"), eps, keep_8bit)
     return (y, n) if pre_norm else y
+
+
+class Routing:
+    """Which experts rows go to, made by :func:`route` or :func:`routing`: ``experts`` (..., k) of ``number``, and where the k choices of each row stand when the
+    choices of all rows are sorted by expert: ``positions`` (..., k) int32, those of one expert in their order, expert by expert from ``offsets`` (number + 1,) int32
+    on, and those without an expert last."""
+
+    __slots__ = ("experts", "number", "positions", "offsets")
+
+    def __init__(self, experts, number, positions, offsets):
+        self.experts, self.number, self.positions, self.offsets = experts, number, positions, offsets
+
+
+def route(logits, choices=1, normalise=True):
+    """The experts of rows: the ``choices`` (at most 8) largest of each row's logits ``(..., experts)``, at most 1024.  Returns ``(weights, routing)``, weights (..., choices) in
+    float32: the softmax over the chosen experts or, with ``normalise=False``, their share of the softmax over all.
+
+    Of equal logits the lowest expert's is first, a NaN is the largest, and -inf is never chosen: a row with nothing else has no expert (-1) and weights of zero."""
+    weights, experts, positions, offsets = _bridge().layers_route(logits, choices, normalise)
+    return weights, Routing(experts, logits.shape[-1], positions, offsets)
+
+
+def routing(experts, number):
+    """The :class:`Routing` of experts that are given, integers (..., choices); one outside of 0 to ``number - 1`` is no expert."""
+    positions, offsets = _bridge().layers_plan(experts, number)
+    return Routing(experts, number, positions, offsets)
+
+
+def dispatch(x, routing):
+    """The rows of ``x`` (..., C), one for each choice, sorted by expert: ``(rows * choices, C)``.  Choices without an expert are zeros, behind all others."""
+    return _bridge().layers_dispatch(x, routing.positions, routing.offsets)
+
+
+def combine(y, weights, routing):
+    """What the experts made of the sorted rows, brought back: the sum over a row's choices of ``weights`` (..., choices) times the choice's row of ``y`` (rows * choices, C).
+    ``weights`` are of the type of ``y`` or float32.  Choices without an expert are left out, and so is what stands in their rows."""
+    return _bridge().layers_combine(y, weights, routing.positions, routing.offsets)

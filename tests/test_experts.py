@@ -1,0 +1,51 @@
+"""Rows that go to experts without a GPU: what the entry points refuse."""
+import numpy as np
+import pytest
+import torch
+
+from permutohedral_encoding_amd import _native, layers
+
+
+def _memory():
+    block = np.zeros(4096, np.uint8)
+    return block, block.ctypes.data + (-block.ctypes.data) % 64
+
+
+def test_the_entry_points_refuse_before_they_launch():
+    lib = _native.lib()
+    block, p = _memory()
+    z = None
+    assert lib.penc_route(3, 4, 8, 2, 1, p, 8, p, p, z) == 10
+    for bad in ((-1, 8, 2), (1 << 31, 8, 2), (4, 0, 1), (4, 1025, 1), (4, 8, 0), (4, 8, 9), (4, 1, 2), (1 << 30, 8, 2)):
+        assert lib.penc_route(0, *bad, 1, p, 8, p, p, z) == 12 == lib.penc_route_backward(0, *bad, 1, p, 8, p, p, p, p, z)
+    assert lib.penc_route(0, 4, 8, 2, 1, p, -1, p, p, z) == 12
+    assert lib.penc_route(0, 4, 8, 2, 1, z, 8, p, p, z) == 1 and lib.penc_route(0, 4, 8, 2, 1, p, 8, z, p, z) == 1 and lib.penc_route(0, 4, 8, 2, 1, p, 8, p, z, z) == 1
+    assert lib.penc_route(1, 4, 8, 2, 1, p + 1, 8, p, p, z) == 5 and lib.penc_route(0, 4, 8, 2, 1, p, 8, p + 2, p, z) == 5
+    assert lib.penc_route(0, 0, 8, 2, 1, z, 8, z, z, z) == 0
+    assert lib.penc_route_backward(0, 4, 8, 2, 0, z, 8, p, p, p, p, z) == 1 and lib.penc_route_backward(0, 4, 8, 2, 1, z, 8, p, p, z, p, z) == 1
+    # plans: one chunk needs no workspace
+    assert lib.penc_plan_workspace_bytes(4096, 8) == 0 == lib.penc_plan_workspace_bytes(-1, 8) == lib.penc_plan_workspace_bytes(10000, 1025)
+    need = lib.penc_plan_workspace_bytes(10000, 8)
+    assert need == 4 * 9 * (3 + 1)
+    assert lib.penc_plan(2, 10, 8, p, p, p, z, 0, z) == 10 and lib.penc_plan(4, -1, 8, p, p, p, z, 0, z) == 12 and lib.penc_plan(4, 10, 0, p, p, p, z, 0, z) == 12
+    assert lib.penc_plan(4, 10, 8, z, p, p, z, 0, z) == 1 and lib.penc_plan(4, 10, 8, p, p, z, z, 0, z) == 1 and lib.penc_plan(8, 10, 8, p + 4, p, p, z, 0, z) == 5
+    assert lib.penc_plan(4, 10000, 8, p, p, p, p, need - 1, z) == 8 and lib.penc_plan(4, 10000, 8, p, p, p, z, need, z) == 1
+    # rows there and back
+    assert lib.penc_dispatch(3, 4, 2, 8, p, 8, p, p, p, z) == 10
+    for bad in ((-1, 2, 8), (4, 0, 8), (4, 1025, 8), (4, 2, 0), (4, 2, (1 << 24) + 1), (1 << 30, 2, 8)):
+        assert lib.penc_dispatch(0, *bad, p, 8, p, p, p, z) == 12 == lib.penc_combine(0, 0, *bad, p, 8, p, p, p, p, z)
+        assert lib.penc_combine_backward(0, 0, *bad, p, 8, p, 8, p, p, p, p, p, z) == 12
+    assert lib.penc_dispatch(0, 4, 2, 8, z, 8, p, p, p, z) == 1 and lib.penc_dispatch(0, 4, 2, 8, p, 8, z, p, p, z) == 1 and lib.penc_dispatch(0, 4, 2, 8, p, 8, p, z, p, z) == 1
+    assert lib.penc_dispatch(0, 4, 2, 8, p + 2, 8, p, p, p, z) == 5 and lib.penc_dispatch(1, 0, 2, 8, z, 8, z, z, z, z) == 0
+    assert lib.penc_combine(1, 2, 4, 2, 8, p, 8, p, p, p, p, z) == 10 and lib.penc_combine(1, 1, 4, 2, 8, p, 8, p + 1, p, p, p, z) == 5
+    assert lib.penc_combine(0, 0, 4, 2, 8, z, 8, p, p, p, p, z) == 1
+    assert lib.penc_combine_backward(0, 0, 4, 2, 8, p, 8, z, 8, p, p, p, z, p, z) == 1  # the weights' gradient needs y
+    assert lib.penc_combine_backward(0, 0, 4, 2, 8, p, 8, z, 8, p, p, p, z, z, z) == 0  # nothing is wanted
+
+
+def test_tensors_in_host_memory_are_refused():
+    x, experts = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int64)
+    plan = layers.Routing(experts, 3, experts.int(), torch.zeros(4, dtype=torch.int32))
+    for call in (lambda: layers.route(x), lambda: layers.routing(experts, 3), lambda: layers.dispatch(x, plan), lambda: layers.combine(x, x, plan)):
+        with pytest.raises(ValueError, match="GPU memory"):
+            call()

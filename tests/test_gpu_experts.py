@@ -1,0 +1,279 @@
+"""Rows that go to experts, on the GPU, against their definitions in 64 bits (expert_reference.py).
+
+Tolerances: indices, positions and copied rows have to be equal.  An exponential of l - top is off by |l - top| 2^-24 for the rounded difference and two steps of
+its own, a sum over a row's experts adds 16 roundings in a lane and 6 over the lanes, a quotient one: (|l - top| + 64) 2^-24 of a weight and, with a few more products
+and sums over the choices, of the terms of a gradient.  A weighted sum of k rows makes 2 k roundings, a dot product of C channels at most C + 8."""
+import math
+
+import pytest
+import torch
+
+import expert_reference as ref
+from permutohedral_encoding_amd import layers
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def random(shape, seed=0, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(dtype)
+
+
+def chosen_experts(rows, choices, number, seed=0, none=0.1, dtype=torch.int64):
+    generator = torch.Generator(device="cuda").manual_seed(seed)
+    e = torch.randint(0, number, (rows, choices), generator=generator, device="cuda")
+    return torch.where(torch.rand((rows, choices), generator=generator, device="cuda") < none, -1, e).to(dtype)
+
+
+def assert_within(got, want, bound, what):
+    assert got.shape == want.shape, what
+    error = (got.detach().double() - want).abs()
+    assert bool((error <= bound).all()), f"{what}: worst error/bound {float((error / bound).max()):.3g}"
+
+
+# ------------------------------------------------------------------------------------------ route
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("normalise", [True, False])
+@pytest.mark.parametrize("rows,number,choices", [(1, 1, 1), (5, 2, 2), (1000, 7, 2), (257, 8, 8), (4097, 9, 3), (300, 16, 1), (300, 33, 5), (1000, 64, 2), (70, 100, 4),
+                                                 (65, 256, 8), (33, 257, 2), (17, 512, 6), (9, 513, 2), (19, 1000, 8), (3, 1024, 4)])
+def test_route(dtype, normalise, rows, number, choices):
+    logits = random((rows, number + 3), 1, TYPES[dtype])[:, :number]
+    closed = torch.rand(rows, number, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda") < 0.3
+    if rows > 4:
+        logits = torch.where(closed, -math.inf, logits)
+        logits[3] = -math.inf
+    logits.requires_grad_(True)
+    weights, routing = layers.route(logits, choices, normalise=normalise)
+    grad = random((rows, choices), 3)
+    chosen, w, d, m, far = ref.route(logits, choices, normalise, grad)
+    assert weights.dtype == torch.float32 and routing.experts.dtype == torch.int32 and routing.number == number
+    assert torch.equal(routing.experts.long(), chosen)
+    assert_within(weights, w, (far + 64) * ref.U * w + 2.0 ** -126, "weights")
+    positions, offsets = ref.plan(chosen, number)
+    assert torch.equal(routing.positions.cpu(), positions) and torch.equal(routing.offsets.cpu(), offsets)
+    dl, = torch.autograd.grad(weights, logits, grad)
+    assert dl.dtype == logits.dtype
+    assert_within(dl, d, (far + 64) * ref.U * m + ref.half_step(d, dl.dtype) + 2.0 ** -126, "dlogits")
+
+
+def test_equal_logits_go_to_the_lowest_experts():
+    for dtype in TYPES.values():
+        for number in (5, 8, 64, 300, 1000):
+            logits = torch.zeros(9, number, device="cuda", dtype=dtype)
+            logits[:, ::2] = -0.0
+            logits[4, number // 2:] = 1.0
+            weights, routing = layers.route(logits, 4)
+            assert torch.equal(routing.experts[:4].cpu(), torch.arange(4, dtype=torch.int32).expand(4, 4))
+            first = number // 2
+            expected = [e if e < number else e - number for e in range(first, first + 4)]
+            assert routing.experts[4].tolist() == expected
+            assert bool((weights[0] == 0.25).all())
+
+
+def test_logits_that_are_not_finite():
+    inf, nan = math.inf, math.nan
+    logits = torch.tensor([[1.0, nan, 2.0, 0.0], [inf, 1.0, 0.0, 0.0], [-inf, -inf, -inf, 3.0], [-inf] * 4, [nan, nan, 1.0, inf]], device="cuda", requires_grad=True)
+    for normalise in (True, False):
+        weights, routing = layers.route(logits, 2, normalise=normalise)
+        assert routing.experts.tolist() == [[1, 2], [0, 1], [3, -1], [-1, -1], [0, 1]]
+        assert bool(torch.isnan(weights[0]).all()) and bool(torch.isnan(weights[1]).any()) and bool(torch.isnan(weights[4]).all())
+        assert weights[2].tolist() == [1.0, 0.0] and weights[3].tolist() == [0.0, 0.0]
+        dl, = torch.autograd.grad(weights.sum(), logits)
+        assert dl[2].tolist() == [0.0] * 4 and dl[3].tolist() == [0.0] * 4
+
+
+def test_route_of_other_shapes():
+    logits = random((4, 6, 10))
+    weights, routing = layers.route(logits, 3)
+    flat, flat_routing = layers.route(logits.view(24, 10), 3)
+    assert weights.shape == routing.experts.shape == routing.positions.shape == (4, 6, 3)
+    assert torch.equal(weights.view(24, 3), flat) and torch.equal(routing.positions.view(24, 3), flat_routing.positions)
+    weights, routing = layers.route(logits.transpose(0, 1), 3)
+    assert torch.equal(weights, flat.view(4, 6, 3).transpose(0, 1))
+    weights, routing = layers.route(logits[:0], 2)
+    assert weights.shape == (0, 6, 2) and routing.offsets.tolist() == [0] * 11
+    weights, routing = layers.route(logits[0, 0], 2)
+    assert weights.shape == (2,) and sorted(routing.positions.tolist()) == [0, 1]
+
+
+@pytest.mark.parametrize("normalise", [True, False])
+def test_the_gradient_of_route_against_differences(normalise):
+    logits = random((6, 9), 5).requires_grad_(True)
+    grad = random((6, 3), 6)
+    weights, _ = layers.route(logits, 3, normalise=normalise)
+    dl, = torch.autograd.grad(weights, logits, grad)
+    step = 2.0 ** -8
+    for e in range(9):
+        moved = [logits.detach().clone() for _ in range(2)]
+        for m, sign in zip(moved, (1.0, -1.0)):
+            m[:, e] += sign * step
+        plus, minus = (layers.route(m, 3, normalise=normalise) for m in moved)
+        same = (plus[1].experts == minus[1].experts).all(1)
+        assert bool(same.any())
+        difference = ((plus[0] - minus[0]).double() * grad).sum(1) / (2 * step)
+        # a third derivative of a share is at most 1, and each of the 2 * 3 weights is off by 64 2^-24
+        bound = step ** 2 * grad.abs().sum(1) + 6 * 64 * ref.U * grad.abs().amax(1) / step
+        assert bool(((dl[:, e].double() - difference).abs() <= bound)[same].all())
+
+
+# ------------------------------------------------------------------------------------------ plans
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("rows,choices,number", [(0, 2, 5), (1, 1, 1), (1, 2, 64), (63, 1, 3), (64, 3, 7), (1000, 2, 8), (4096, 1, 1024), (4097, 1, 2), (2049, 2, 1000),
+                                                 (30000, 4, 63), (30000, 1, 64), (5, 1000, 17), (1 << 18, 2, 13)])
+def test_plan(dtype, rows, choices, number):
+    for none in (0.0, 0.2, 1.0):
+        experts = chosen_experts(rows, choices, number, none=none, dtype=dtype)
+        routing = layers.routing(experts, number)
+        positions, offsets = ref.plan(experts, number)
+        assert torch.equal(routing.positions.cpu(), positions) and torch.equal(routing.offsets.cpu(), offsets)
+
+
+def test_plan_of_experts_that_are_none_and_of_one_alone():
+    experts = torch.tensor([[5, -7], [1 << 40, 2], [3, 3], [2, -1]], device="cuda")
+    routing = layers.routing(experts, 5)
+    assert routing.positions.tolist() == [[4, 5], [6, 0], [2, 3], [1, 7]] and routing.offsets.tolist() == [0, 0, 0, 2, 4, 4]
+    routing = layers.routing(torch.full((10000, 1), 3, device="cuda"), 9)
+    assert torch.equal(routing.positions[:, 0].cpu(), torch.arange(10000, dtype=torch.int32)) and routing.offsets.tolist() == [0] * 4 + [10000] * 6
+    strided = chosen_experts(50, 6, 4)[:, ::2]
+    assert torch.equal(layers.routing(strided, 4).positions.cpu(), ref.plan(strided, 4)[0])
+
+
+# ------------------------------------------------------------------------------------------ rows there and back
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,choices,channels", [(0, 2, 5), (1, 1, 1), (1, 2, 1024), (100, 2, 3), (257, 1, 8), (300, 3, 64), (65, 4, 203), (33, 5, 7), (20, 9, 130),
+                                                   (4097, 2, 48), (7, 2, 4100)])
+def test_rows_there_and_back(dtype, rows, choices, channels):
+    dtype, number = TYPES[dtype], 7
+    for none, weight_dtype in ((0.2, torch.float32), (0.0, dtype), (1.0, torch.float32)):
+        experts = chosen_experts(rows, choices, number, seed=rows, none=none)
+        routing = layers.routing(experts, number)
+        at, there = routing.positions.long(), (experts >= 0)[:, :, None]
+        x = random((rows, channels + 3), 1, dtype)[:, :channels].requires_grad_(True)
+        y = random((rows * choices, channels + 1), 2, dtype)[:, :channels]
+        total = int(routing.offsets[-1])
+        y[total:] = math.nan  # (what stands in rows without an expert is not read)
+        y.requires_grad_(True)
+        weights = random((rows, choices), 3, weight_dtype).requires_grad_(True)
+
+        rows_there = layers.dispatch(x, routing)
+        want = torch.zeros((rows * choices, channels), dtype=dtype, device="cuda")
+        want[at] = torch.where(there, x.detach()[:, None], 0)
+        assert torch.equal(rows_there, want)
+
+        out = layers.combine(y, weights, routing)
+        back = torch.where(there, y.detach().double()[at], 0.0)
+        w = weights.detach().double()[:, :, None]
+        assert out.dtype == dtype and out.shape == (rows, channels)
+        value, size = (back * w).sum(1), (back * w).abs().sum(1)
+        assert_within(out, value, 2 * choices * ref.U * size + ref.half_step(value, dtype), "out")
+
+        grad_there, grad_out = random((rows * choices, channels), 4, dtype), random((rows, channels + 2), 5, dtype)[:, :channels]
+        grad_there[total:] = math.nan
+        dx, dy, dw = torch.autograd.grad((rows_there, out), (x, y, weights), (grad_there, grad_out))
+        g = torch.where(there, grad_there.double()[at], 0.0)
+        assert dx.dtype == dtype and dw.dtype == weight_dtype
+        assert_within(dx, g.sum(1), choices * ref.U * g.abs().sum(1) + ref.half_step(g.sum(1), dtype), "dx")
+        want = torch.zeros((rows * choices, channels), dtype=torch.float64, device="cuda")
+        want[at] = torch.where(there, grad_out.double()[:, None] * w, 0.0)
+        assert_within(dy, want, ref.U * want.abs() + ref.half_step(want, dtype), "dy")
+        terms = grad_out.double()[:, None] * back
+        assert_within(dw, terms.sum(2), (channels + 8) * ref.U * terms.abs().sum(2) + ref.half_step(terms.sum(2), weight_dtype), "dweights")
+
+
+def test_rows_of_other_shapes_and_partial_gradients():
+    experts = chosen_experts(24, 2, 5, none=0.1).view(4, 6, 2)
+    routing = layers.routing(experts, 5)
+    x = random((6, 4, 40)).transpose(0, 1).requires_grad_(True)
+    flat_routing = layers.routing(experts.view(24, 2), 5)
+    there = layers.dispatch(x, routing)
+    assert torch.equal(there, layers.dispatch(x.detach().reshape(24, 40), flat_routing))
+    weights = random((4, 6, 2), 1)
+    out = layers.combine(there, weights, routing)
+    assert out.shape == (4, 6, 40)
+    dx, = torch.autograd.grad(out, x, torch.ones(1, 1, 40, device="cuda").expand(4, 6, 40))
+    assert_within(dx, torch.where(experts >= 0, weights.double(), 0.0).sum(2, keepdim=True).expand(4, 6, 40), 8 * ref.U * weights.abs().sum(2, keepdim=True).double() + 1e-30, "dx")
+    # the weights alone, and y alone
+    y, w = there.detach().requires_grad_(True), weights.clone().requires_grad_(True)
+    both = torch.autograd.grad(layers.combine(y, w, routing).sum(), (y, w))
+    assert torch.equal(torch.autograd.grad(layers.combine(y.detach(), w, routing).sum(), w)[0], both[1])
+    assert torch.equal(torch.autograd.grad(layers.combine(y, w.detach(), routing).sum(), y)[0], both[0])
+    # a row that goes to the same expert twice
+    twice = layers.routing(torch.tensor([[1, 1], [0, 1]], device="cuda"), 2)
+    rows = layers.dispatch(x.detach()[0, :2], twice)
+    assert torch.equal(rows, x.detach()[0][[1, 0, 0, 1]])
+
+
+def test_rows_behind_two_to_the_31_values():
+    rows, channels = (1 << 20) + 3, 2080
+    x = torch.zeros(rows, channels, dtype=torch.bfloat16, device="cuda")
+    x[-5:] = random((5, channels), 1, torch.bfloat16)
+    experts = torch.zeros(rows, 1, dtype=torch.int32, device="cuda")
+    experts[-5:] = 2
+    experts[0] = 1
+    routing = layers.routing(experts, 3)
+    there = layers.dispatch(x, routing)
+    assert torch.equal(there[-5:], x[-5:]) and not bool(there[:-5].any())
+    assert torch.equal(layers.combine(there, torch.ones(rows, 1, device="cuda"), routing), x)
+
+
+# ------------------------------------------------------------------------------------------ refusals
+
+def test_refusals():
+    x, routing = random((6, 8)), layers.routing(chosen_experts(6, 2, 4), 4)
+    logits = random((6, 4))
+    cpu = layers.Routing(routing.experts, 4, routing.positions.cpu(), routing.offsets)
+    for call, message in [(lambda: layers.route(logits, 5), "choose"), (lambda: layers.route(logits, 0), "choose"),
+                          (lambda: layers.route(random((2, 100)), 9), "choose"), (lambda: layers.route(random((2, 1025)), 1), "experts"),
+                          (lambda: layers.route(logits.double(), 1), "type"), (lambda: layers.routing(logits, 4), "int32 or int64"),
+                          (lambda: layers.routing(routing.experts, 0), "experts"), (lambda: layers.routing(routing.experts, 1025), "experts"),
+                          (lambda: layers.dispatch(x[:5], routing), "rows"), (lambda: layers.dispatch(x, cpu), "GPU memory"),
+                          (lambda: layers.dispatch(x.long(), routing), "type"), (lambda: layers.combine(x, torch.ones(6, 2, device="cuda"), routing), "choices"),
+                          (lambda: layers.combine(random((12, 8)), torch.ones(6, 1, device="cuda"), routing), "each choice"),
+                          (lambda: layers.combine(random((12, 8), dtype=torch.bfloat16), torch.ones(6, 2, device="cuda", dtype=torch.float16), routing), "weights"),
+                          (lambda: layers.dispatch(x, layers.Routing(None, 4, routing.positions.long(), routing.offsets)), "routing")]:
+        with pytest.raises(ValueError, match=message):
+            call()
+    weights, _ = layers.route(logits.requires_grad_(True), 2)
+    first, = torch.autograd.grad(weights.square().sum(), logits, create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        first.sum().backward()
+
+
+# ------------------------------------------------------------------------------------------ streams and graphs
+
+def test_on_another_stream_and_in_a_graph():
+    logits, x = random((500, 16)), random((500, 48), 1)
+
+    def forward(logits, x):
+        weights, routing = layers.route(logits, 2)
+        return layers.combine(2.0 * layers.dispatch(x, routing), weights, routing), routing.positions
+
+    want, want_at = forward(logits, x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got, got_at = forward(logits, x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want) and torch.equal(got_at, want_at)
+
+    given = [logits.clone().requires_grad_(True), x.clone().requires_grad_(True)]
+    grad = random((500, 48), 2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = forward(*given)
+        grads = torch.autograd.grad(out, given, grad)
+    for seed in range(3):
+        new = [random((500, 16), 10 + seed), random((500, 48), 20 + seed)]
+        with torch.no_grad():
+            for t, n in zip(given, new):
+                t.copy_(n)
+        graph.replay()
+        eager = [t.clone().requires_grad_(True) for t in new]
+        want, _ = forward(*eager)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(want, eager, grad)))
