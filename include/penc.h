@@ -522,6 +522,20 @@ int penc_combine(int type, int weight_type, int64_t rows, int choices, int64_t c
 int penc_combine_backward(int type, int weight_type, int64_t rows, int choices, int64_t channels, const void* grad, int64_t grad_row_stride, const void* y,
                           int64_t row_stride, const void* weights, const int32_t* positions, const int32_t* routed, void* dy, void* dweights, void* stream);
 
+/* A linear layer of each expert on its own rows, of rows sorted by expert: y[r] (dense rows) = weight[e] x[r] + bias[e] for offsets[e] <= r < offsets[e + 1], weight dense
+ * [experts][outputs][channels], bias [experts][outputs] or NULL, of one type.  Rows that are read are at least as far apart as they are long. */
+#define PENC_MAX_EXPERT_CHANNELS (1 << 18)
+#define PENC_MAX_EXPERT_STRIDE (1 << 20)
+int penc_expert_linear(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t row_stride, const void* weight,
+                       const void* bias, const int32_t* offsets, void* y, void* stream);
+int penc_expert_linear_input_grad(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* grad, int64_t grad_row_stride,
+                                  const void* weight, const int32_t* offsets, void* dx, void* stream);
+/* The gradients of the weights and (may be NULL) biases; zero for an expert without rows.  `workspace` holds partial sums. */
+size_t penc_expert_weight_grad_workspace_bytes(int type, int64_t rows, int experts, int64_t channels, int64_t outputs);
+int penc_expert_weight_grad(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t row_stride, const void* grad,
+                            int64_t grad_row_stride, const int32_t* offsets, void* weight_grad, void* bias_grad, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,287 @@
+// A linear layer of each expert on its own rows, of rows sorted by expert: for offsets[e] <= r < offsets[e + 1]
+//
+//     y[r][o] = sum over c of W[e][o][c] x[r][c] + b[e][o],      dx[r][c] = sum over o of W[e][o][c] dy[r][o],
+//     dW[e][o][c] = sum over these r of dy[r][o] x[r][c],        db[e][o] = sum of dy[r][o].
+//
+// Which rows a workgroup has it finds from the offsets, which are on the device: tiles of rows do not cross from one expert to the next, and the grid has room for one
+// tile of each expert that is not full.  Rows behind the last expert's are zero in y and dx and not read otherwise.
+//
+// The type of values (PENC_TYPE: those of penc.h) is one compilation each.
+#include <algorithm>
+
+#include "penc_expert_linear.hpp"
+#include "penc_product.hpp"
+
+#ifndef PENC_TYPE
+#error "PENC_TYPE: PENC_FP32, PENC_FP16 or PENC_BF16"
+#endif
+
+namespace penc {
+namespace {
+
+using Value = std::conditional_t<PENC_TYPE == PENC_FP32, float, std::conditional_t<PENC_TYPE == PENC_FP16, half_t, bf16_t>>;
+constexpr int kSize = sizeof(Value);
+
+// Tile `t` of rows: those of an expert (`experts`: the rows behind the last one's), cut every `most` rows.
+struct RowTile {
+    int expert, first, rows, of_expert, tiles;  // of_expert: which of the expert's tiles it is; tiles: the expert's; expert < 0: there is no such tile
+};
+
+// All lanes of a wave call it.  kWhole: tiles of the rows behind the last expert's too; else each expert has a tile at least, be it one of no rows.
+template <bool kWhole>
+__device__ __forceinline__ RowTile row_tile(const int32_t* __restrict__ offsets, int experts, int rows, uint32_t t, int most) {
+    const int lane = threadIdx.x % 64;
+    uint32_t before = 0;
+    for (int base = 0; base < experts + (kWhole ? 1 : 0); base += 64) {
+        const int e = base + lane;
+        int from = 0, to = 0;
+        if (e <= experts) from = min(max(offsets[e], 0), rows);
+        if (e < experts) to = min(max(offsets[e + 1], 0), rows);
+        else if (kWhole && e == experts) to = rows;
+        const int n = max(to - from, 0);
+        uint32_t tiles = (static_cast<uint32_t>(n) + most - 1) / most;
+        if (!kWhole && e < experts) tiles = max(tiles, 1u);
+        if (e > experts || (!kWhole && e == experts)) tiles = 0;
+        uint32_t sum = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t other = __shfl_up(sum, d);
+            sum += lane >= d ? other : 0u;
+        }
+        const uint64_t behind = __ballot(t < before + sum);
+        if (behind != 0) {
+            const int found = __builtin_ctzll(behind);
+            const int first = __shfl(from, found), count = __shfl(n, found);
+            const uint32_t its = __shfl(tiles, found), at = t - before - (__shfl(sum, found) - its);
+            const int skip = static_cast<int>(at) * most;
+            return {__builtin_amdgcn_readfirstlane(base + found), __builtin_amdgcn_readfirstlane(first + skip),
+                    __builtin_amdgcn_readfirstlane(min(count - skip, most)), __builtin_amdgcn_readfirstlane(static_cast<int>(at)),
+                    __builtin_amdgcn_readfirstlane(static_cast<int>(its))};
+        }
+        before += __shfl(sum, 63);
+    }
+    return {-1, 0, 0, 0, 0};
+}
+
+struct RowsArgs {
+    const void *rows_in, *weight, *bias;
+    void* rows_out;
+    int64_t stride;                // of rows_in, in values
+    const int32_t* offsets;
+    int experts, rows, wide, deep; // wide: values of a row of the result; deep: of the operand
+    uint32_t items, tiles;         // tiles: of a row of the result
+    bool aligned;                  // whether four results can be stored at once
+};
+
+// y (kBack false: weights by rows of k) or dx.
+template <bool kBack, class P>
+__global__ __launch_bounds__(P::kThreads) void expert_rows_kernel(RowsArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
+    const uint32_t item = item_of(a.items);
+    const RowTile t = row_tile<true>(a.offsets, a.experts, a.rows, item / a.tiles, P::kN);
+    if (t.expert < 0) return;
+    const int m0 = static_cast<int>(item % a.tiles) * P::kM;
+    P p;
+    if (t.expert == a.experts) {
+        p.run(lds, {}, {}, 0, [](const char*, int) {});
+    } else {
+        const char* const weight = static_cast<const char*>(a.weight) + static_cast<int64_t>(t.expert) * a.wide * a.deep * kSize;
+        const int m_rows = min(a.wide - m0, P::kM);
+        const Operand m = kBack ? Operand{weight + static_cast<int64_t>(m0) * kSize, static_cast<int64_t>(a.wide) * kSize, a.deep, m_rows * kSize}
+                                : Operand{weight + static_cast<int64_t>(m0) * a.deep * kSize, static_cast<int64_t>(a.deep) * kSize, m_rows, a.deep * kSize};
+        const Operand n{static_cast<const char*>(a.rows_in) + static_cast<int64_t>(t.first) * a.stride * kSize, a.stride * kSize, t.rows, a.deep * kSize};
+        p.run(lds, m, n, a.deep, [](const char*, int) {});
+    }
+    const Value* const bias = !kBack && a.bias != nullptr && t.expert < a.experts ? static_cast<const Value*>(a.bias) + static_cast<int64_t>(t.expert) * a.wide : nullptr;
+    Value* const out = static_cast<Value*>(a.rows_out) + static_cast<int64_t>(t.first) * a.wide;
+    p.each([&](int m, int n, tile_acc v) {
+        const int valid = a.wide - m0 - m;
+        if (n >= t.rows || valid <= 0) return;
+        if (!kBack && bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < valid) v[i] += static_cast<float>(bias[m0 + m + i]);
+        }
+        store_four(out + static_cast<int64_t>(n) * a.wide + m0 + m, v, valid, a.aligned);
+    });
+}
+
+struct WeightArgs {
+    const void *x, *grad;
+    int64_t x_stride, grad_stride;
+    const int32_t* offsets;
+    int experts, rows, channels, outputs, most;  // most: rows of a piece
+    uint32_t items, channel_tiles, tiles;
+    void *weight, *bias;  // results, written where an expert's rows are one piece
+    float* sums;          // [pieces][outputs][channels], and behind them [pieces][outputs]
+    int64_t pieces;
+    bool aligned;
+};
+
+// dW and db of a piece of an expert's rows.
+template <class P>
+__global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
+    const uint32_t item = item_of(a.items), piece = item / a.tiles, tile = item % a.tiles;
+    const RowTile t = row_tile<false>(a.offsets, a.experts, a.rows, piece, a.most);
+    if (t.expert < 0) return;
+    const int c0 = static_cast<int>(tile % a.channel_tiles) * P::kM, o0 = static_cast<int>(tile / a.channel_tiles) * P::kN;
+    const bool bias = a.bias != nullptr && c0 == 0 && P::wave_m() == 0;
+    const Operand m{static_cast<const char*>(a.x) + (static_cast<int64_t>(t.first) * a.x_stride + c0) * kSize, a.x_stride * kSize, t.rows, min(a.channels - c0, P::kM) * kSize};
+    const Operand n{static_cast<const char*>(a.grad) + (static_cast<int64_t>(t.first) * a.grad_stride + o0) * kSize, a.grad_stride * kSize, t.rows,
+                    min(a.outputs - o0, P::kN) * kSize};
+    P p;
+    // the sums of dy itself are its products with ones
+    tile_acc bias_acc[P::kTilesN] = {};
+    const uint32_t one = PENC_TYPE == PENC_FP32 ? 0x3F800000u : PENC_TYPE == PENC_FP16 ? 0x3C003C00u : 0x3F803F80u;
+    const chunk16 ones = {one, one, one, one};
+    p.run(lds, m, n, t.rows, [&](const char* step, int) {
+        if (!bias) return;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int j = 0; j < P::kTilesN; ++j)
+                bias_acc[j] = multiply<Value>(ones, P::TileN::fragment(step + P::TileM::kSize, P::wave_n() + 16 * j, q), bias_acc[j]);
+    });
+    const int64_t n_weights = static_cast<int64_t>(a.outputs) * a.channels;
+    const bool whole = t.tiles == 1;
+    p.each([&](int c, int o, tile_acc v) {
+        const int valid = a.channels - c0 - c;
+        if (o0 + o >= a.outputs || valid <= 0) return;
+        const int64_t at = static_cast<int64_t>(o0 + o) * a.channels + c0 + c;
+        if (whole) store_four(static_cast<Value*>(a.weight) + t.expert * n_weights + at, v, valid, a.aligned);
+        else store_four(a.sums + piece * n_weights + at, v, valid, a.channels % 4 == 0);
+    });
+    if (!bias) return;
+    const int lane = threadIdx.x % 64;
+#pragma unroll
+    for (int j = 0; j < P::kTilesN; ++j) {
+        const int o = o0 + P::wave_n() + 16 * j + lane;
+        if (lane >= 16 || o >= a.outputs) continue;
+        if (whole) static_cast<Value*>(a.bias)[static_cast<int64_t>(t.expert) * a.outputs + o] = static_cast<Value>(bias_acc[j][0]);
+        else a.sums[a.pieces * n_weights + static_cast<int64_t>(piece) * a.outputs + o] = bias_acc[j][0];
+    }
+}
+
+constexpr int kSumThreads = 256;
+
+// The sums of experts whose rows are several pieces, piece by piece.
+__global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, uint32_t blocks) {
+    const int e = static_cast<int>(blockIdx.x / blocks);
+    // the first of the expert's pieces, and how many there are
+    uint32_t first = 0, mine = 0;
+    for (int i = static_cast<int>(threadIdx.x) % 64; i <= e; i += 64) {
+        const int from = min(max(a.offsets[i], 0), a.rows), to = min(max(a.offsets[i + 1], 0), a.rows);
+        const uint32_t n = max((static_cast<uint32_t>(max(to - from, 0)) + a.most - 1) / a.most, 1u);
+        if (i < e) first += n;
+        else mine = n;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) first += __shfl_xor(first, d), mine = max(mine, static_cast<uint32_t>(__shfl_xor(mine, d)));
+    if (mine <= 1) return;
+    const int64_t weights = static_cast<int64_t>(a.outputs) * a.channels, n = weights + (a.bias != nullptr ? a.outputs : 0);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x % blocks) * kSumThreads + threadIdx.x; i < n; i += static_cast<int64_t>(blocks) * kSumThreads) {
+        const bool weight = i < weights;
+        const int64_t each = weight ? weights : a.outputs, at = weight ? i : i - weights;
+        const float* const from = a.sums + (weight ? 0 : a.pieces * weights) + first * each + at;
+        float sum = 0.0f;
+        for (uint32_t k = 0; k < mine; ++k) sum += from[k * each];
+        static_cast<Value*>(weight ? a.weight : a.bias)[e * each + at] = static_cast<Value>(sum);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// which kernel
+
+// Whether chunks of 16 bytes are on 16 bytes.
+bool chunked(const void* p, int64_t stride, int64_t bytes) { return aligned_to(p, 16) && stride * kSize % 16 == 0 && bytes * kSize % 16 == 0; }
+
+template <bool kBack, class P>
+int launch_rows(RowsArgs a, hipStream_t stream) {
+    a.tiles = static_cast<uint32_t>((a.wide + P::kM - 1) / P::kM);
+    const int64_t items = (a.rows / P::kN + static_cast<int64_t>(a.experts) + 1) * a.tiles;
+    if (items * P::kThreads >= int64_t{1} << 32) return PENC_ERR_BAD_LAYER_SIZE;
+    a.items = static_cast<uint32_t>(items);
+    expert_rows_kernel<kBack, P><<<a.items, P::kThreads, 0, stream>>>(a);
+    return launched();
+}
+
+template <bool kBack, bool kDirect>
+int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
+    if (a.wide <= 64) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kDirect>>(a, stream);
+    return launch_rows<kBack, Product<Value, kBack, false, 128, 128, 2, 2, kDirect>>(a, stream);
+}
+
+// How the rows of the weights' gradient are cut.
+struct WeightPlan {
+    bool small;    // tiles of 64 x 64, else of 128 x 128
+    int64_t tiles; // of an expert
+    int64_t most;  // rows of a piece
+    int64_t pieces;
+};
+WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
+    WeightPlan p;
+    p.small = channels <= 64 || outputs <= 64;
+    const int64_t side = p.small ? 64 : 128;
+    p.tiles = ((channels + side - 1) / side) * ((outputs + side - 1) / side);
+    const int64_t wanted = (1024 + p.tiles - 1) / p.tiles;  // pieces for four workgroups to a compute unit
+    int64_t most = experts >= wanted ? 2 * ((rows + experts - 1) / experts) : (rows + wanted - 1) / wanted;
+    most = std::max<int64_t>((most + 63) / 64 * 64, 512);
+    p.most = std::min<int64_t>(most, (int64_t{1} << 30));
+    p.pieces = rows / p.most + experts;
+    return p;
+}
+
+template <class P>
+int launch_weights(WeightArgs a, const WeightPlan& plan, hipStream_t stream) {
+    a.channel_tiles = static_cast<uint32_t>((a.channels + P::kM - 1) / P::kM);
+    a.tiles = static_cast<uint32_t>(plan.tiles);
+    const int64_t items = plan.pieces * plan.tiles;
+    if (items * P::kThreads >= int64_t{1} << 32) return PENC_ERR_BAD_LAYER_SIZE;
+    a.items = static_cast<uint32_t>(items);
+    expert_weights_kernel<P><<<a.items, P::kThreads, 0, stream>>>(a);
+    return launched();
+}
+
+template <bool kDirect>
+int weights_of_experts(const WeightArgs& a, const WeightPlan& plan, hipStream_t stream) {
+    if (plan.small) return launch_weights<Product<Value, true, true, 64, 64, 2, 2, kDirect>>(a, plan, stream);
+    return launch_weights<Product<Value, true, true, 128, 128, 2, 2, kDirect>>(a, plan, stream);
+}
+
+}  // namespace
+
+template <>
+int expert_rows<PENC_TYPE>(bool back, int64_t rows, int experts, int64_t wide, int64_t deep, const void* in, int64_t stride, const void* weight, const void* bias,
+                           const int32_t* offsets, void* out, hipStream_t stream) {
+    if (rows == 0) return PENC_OK;
+    RowsArgs a{in, weight, bias, out, stride, offsets, experts, static_cast<int>(rows), static_cast<int>(wide), static_cast<int>(deep), 0, 0,
+               aligned_to(out, 4 * kSize) && wide % 4 == 0};
+    const bool direct = chunked(in, stride, deep) && chunked(weight, back ? wide : deep, back ? wide : deep);
+    if (back) return direct ? rows_of_experts<true, true>(a, stream) : rows_of_experts<true, false>(a, stream);
+    return direct ? rows_of_experts<false, true>(a, stream) : rows_of_experts<false, false>(a, stream);
+}
+
+template <>
+size_t expert_weights_workspace<PENC_TYPE>(int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
+    const WeightPlan p = weight_plan(rows, experts, channels, outputs);
+    if (rows <= p.most) return 0;  // no expert's rows are cut
+    return 4 * static_cast<size_t>(p.pieces) * static_cast<size_t>(outputs) * (static_cast<size_t>(channels) + 1);
+}
+
+template <>
+int expert_weights<PENC_TYPE>(int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t x_stride, const void* grad, int64_t grad_stride,
+                              const int32_t* offsets, void* weight, void* bias, void* workspace, hipStream_t stream) {
+    const WeightPlan plan = weight_plan(rows, experts, channels, outputs);
+    WeightArgs a{x, grad, x_stride, grad_stride, offsets, experts, static_cast<int>(rows), static_cast<int>(channels), static_cast<int>(outputs),
+                 static_cast<int>(plan.most), 0, 0, 0, weight, bias, static_cast<float*>(workspace), plan.pieces, aligned_to(weight, 4 * kSize) && channels % 4 == 0};
+    const bool direct = chunked(x, x_stride, channels) && chunked(grad, grad_stride, outputs);
+    if (const int rc = direct ? weights_of_experts<true>(a, plan, stream) : weights_of_experts<false>(a, plan, stream)) return rc;
+    if (rows <= plan.most) return PENC_OK;
+    const int64_t results = outputs * (channels + 1);
+    const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>((results + kSumThreads - 1) / kSumThreads, std::max<int64_t>(1, 65536 / experts)));
+    expert_sums_kernel<<<static_cast<uint32_t>(experts) * blocks, kSumThreads, 0, stream>>>(a, blocks);
+    return launched();
+}
+
+}  // namespace penc

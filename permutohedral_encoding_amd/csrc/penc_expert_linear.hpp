@@ -1,0 +1,19 @@
+// The products of penc_expert_linear.hip, one compilation for each type of include/penc.h.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace penc {
+
+// y of `deep` channels and `wide` outputs, or (back) dx of `deep` outputs and `wide` channels; weight [experts][outputs][channels].
+template <int kType>
+int expert_rows(bool back, int64_t rows, int experts, int64_t wide, int64_t deep, const void* in, int64_t stride, const void* weight, const void* bias,
+                const int32_t* offsets, void* out, hipStream_t stream);
+template <int kType>
+size_t expert_weights_workspace(int64_t rows, int64_t experts, int64_t channels, int64_t outputs);
+template <int kType>
+int expert_weights(int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t x_stride, const void* grad, int64_t grad_stride,
+                   const int32_t* offsets, void* weight, void* bias, void* workspace, hipStream_t stream);
+
+}  // namespace penc

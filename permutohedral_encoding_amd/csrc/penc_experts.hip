@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "penc_expert_linear.hpp"
 #include "penc_kept.hpp"
 
 namespace penc {
@@ -668,6 +669,93 @@ int penc_combine_backward(int type, int weight_type, int64_t rows, int choices, 
                 return weight_type == PENC_FP32 ? launch(float{}) : launch(e);
             });
         });
+    });
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------
+// the experts' products (penc_expert_linear.hip)
+
+namespace {
+
+// Runs f with the type as a constant.
+template <class F>
+int with_constant_type(int type, F&& f) {
+    switch (type) {
+        case PENC_FP32: return f(std::integral_constant<int, PENC_FP32>{});
+        case PENC_FP16: return f(std::integral_constant<int, PENC_FP16>{});
+        case PENC_BF16: return f(std::integral_constant<int, PENC_BF16>{});
+        default: return PENC_ERR_UNSUPPORTED_TYPE;
+    }
+}
+
+bool bad_layer(int64_t rows, int experts, int64_t channels, int64_t outputs) {
+    return bad_rows(rows) || experts < 1 || experts > PENC_MAX_EXPERTS || channels < 1 || channels > PENC_MAX_EXPERT_CHANNELS || outputs < 1 ||
+           outputs > PENC_MAX_EXPERT_CHANNELS;
+}
+// (rows that overlap would not end where one is told that they do)
+bool bad_row_stride(int64_t rows, int64_t stride, int64_t values) { return rows > 1 && (stride < values || stride > PENC_MAX_EXPERT_STRIDE); }
+
+}  // namespace
+
+extern "C" {
+
+int penc_expert_linear(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t row_stride, const void* weight,
+                       const void* bias, const int32_t* offsets, void* y, void* stream) {
+    return with_constant_type(type, [&](auto constant) -> int {
+        constexpr int kType = decltype(constant)::value;
+        if (bad_layer(rows, experts, channels, outputs) || bad_row_stride(rows, row_stride, channels)) return PENC_ERR_BAD_LAYER_SIZE;
+        if (rows == 0) return PENC_OK;
+        if (!x || !weight || !offsets || !y) return PENC_ERR_NULL_POINTER;
+        const size_t size = kType == PENC_FP32 ? 4 : 2;
+        if (!aligned_to(x, size) || !aligned_to(weight, size) || !aligned_to(bias, size) || !aligned_to(y, size) || !aligned_to(offsets, 4))
+            return PENC_ERR_MISALIGNED;
+        return expert_rows<kType>(false, rows, experts, outputs, channels, x, rows > 1 ? row_stride : channels, weight, bias, offsets, y,
+                                  static_cast<hipStream_t>(stream));
+    });
+}
+
+int penc_expert_linear_input_grad(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* grad, int64_t grad_row_stride,
+                                  const void* weight, const int32_t* offsets, void* dx, void* stream) {
+    return with_constant_type(type, [&](auto constant) -> int {
+        constexpr int kType = decltype(constant)::value;
+        if (bad_layer(rows, experts, channels, outputs) || bad_row_stride(rows, grad_row_stride, outputs)) return PENC_ERR_BAD_LAYER_SIZE;
+        if (rows == 0) return PENC_OK;
+        if (!grad || !weight || !offsets || !dx) return PENC_ERR_NULL_POINTER;
+        const size_t size = kType == PENC_FP32 ? 4 : 2;
+        if (!aligned_to(grad, size) || !aligned_to(weight, size) || !aligned_to(dx, size) || !aligned_to(offsets, 4)) return PENC_ERR_MISALIGNED;
+        return expert_rows<kType>(true, rows, experts, channels, outputs, grad, rows > 1 ? grad_row_stride : outputs, weight, nullptr, offsets, dx,
+                                  static_cast<hipStream_t>(stream));
+    });
+}
+
+size_t penc_expert_weight_grad_workspace_bytes(int type, int64_t rows, int experts, int64_t channels, int64_t outputs) {
+    if (bad_layer(rows, experts, channels, outputs)) return 0;
+    switch (type) {
+        case PENC_FP32: return expert_weights_workspace<PENC_FP32>(rows, experts, channels, outputs);
+        case PENC_FP16: return expert_weights_workspace<PENC_FP16>(rows, experts, channels, outputs);
+        case PENC_BF16: return expert_weights_workspace<PENC_BF16>(rows, experts, channels, outputs);
+        default: return 0;
+    }
+}
+
+int penc_expert_weight_grad(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t row_stride, const void* grad,
+                            int64_t grad_row_stride, const int32_t* offsets, void* weight_grad, void* bias_grad, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+    return with_constant_type(type, [&](auto constant) -> int {
+        constexpr int kType = decltype(constant)::value;
+        if (bad_layer(rows, experts, channels, outputs) || bad_row_stride(rows, row_stride, channels) || bad_row_stride(rows, grad_row_stride, outputs))
+            return PENC_ERR_BAD_LAYER_SIZE;
+        if ((rows > 0 && (!x || !grad)) || !offsets || !weight_grad) return PENC_ERR_NULL_POINTER;
+        const size_t size = kType == PENC_FP32 ? 4 : 2, need = penc_expert_weight_grad_workspace_bytes(type, rows, experts, channels, outputs);
+        if (!aligned_to(x, size) || !aligned_to(grad, size) || !aligned_to(weight_grad, size) || !aligned_to(bias_grad, size) || !aligned_to(offsets, 4) ||
+            !aligned_to(workspace, 16))
+            return PENC_ERR_MISALIGNED;
+        if (workspace_bytes < need) return PENC_ERR_WORKSPACE_TOO_SMALL;
+        if (need > 0 && !workspace) return PENC_ERR_NULL_POINTER;
+        return expert_weights<kType>(rows, experts, channels, outputs, x, rows > 1 ? row_stride : channels, grad, rows > 1 ? grad_row_stride : outputs, offsets,
+                                     weight_grad, bias_grad, workspace, static_cast<hipStream_t>(stream));
     });
 }
 

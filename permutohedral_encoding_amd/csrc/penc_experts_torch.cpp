@@ -17,6 +17,10 @@ struct Api {
     PENC_FN(dispatch);
     PENC_FN(combine);
     PENC_FN(combine_backward);
+    PENC_FN(expert_linear);
+    PENC_FN(expert_linear_input_grad);
+    PENC_FN(expert_weight_grad_workspace_bytes);
+    PENC_FN(expert_weight_grad);
 #undef PENC_FN
 } api;
 
@@ -290,6 +294,100 @@ Tensor combine(const Tensor& y, const Tensor& weights, const Tensor& positions, 
 }
 
 // ------------------------------------------------------------------------------------------
+// expert_linear
+
+// Rows as the products read them: none overlaps another, and none is further from it than a tile's offsets reach.
+Rows product_rows(Rows r) {
+    if (r.n > 1 && (r.stride < r.channels || r.stride > PENC_MAX_EXPERT_STRIDE)) {
+        r.values = r.values.clone(at::MemoryFormat::Contiguous);
+        r.stride = r.channels;
+    }
+    return r;
+}
+
+struct ExpertLinearNode : public ExpertNode {
+    int type = 0, experts = 0;
+    int64_t rows = 0;
+    std::vector<int64_t> sizes, weight_sizes;
+    bool has_bias = false;
+
+    std::string name() const override { return "LayersExpertLinearBackward"; }
+    variable_list gradients(const variable_list& grads) override {
+        const std::vector<Tensor> t = unpacked();  // x (where a parameter wants a gradient), weight (where x does), offsets
+        const auto scalar = scalar_type_of(type);
+        const c10::DeviceGuard device(grads[0].device());
+        TORCH_CHECK(t[2].defined() && t[2].is_cuda() && t[2].scalar_type() == at::kInt && t[2].is_contiguous() && t[2].numel() == experts + 1,
+                    "a routing saved for the backward has come back in another form");
+        const int32_t* const offsets = static_cast<const int32_t*>(t[2].const_data_ptr());
+        const int64_t outputs = weight_sizes[1], channels = weight_sizes[2];
+        const Rows g = product_rows(grad_rows(grads[0], scalar));
+        const auto options = grads[0].options().dtype(scalar);
+        void* const stream = current_stream(grads[0].device());
+        variable_list out(3);
+        if (t[1].defined() && task_should_compute_output(0)) {
+            require_saved(t[1], weight_sizes, scalar);
+            const Tensor weight = t[1].contiguous();
+            out[0] = at::empty(sizes, options);
+            check(api.expert_linear_input_grad(type, rows, experts, channels, outputs, g.data(), g.stride, weight.const_data_ptr(), offsets, out[0].data_ptr(),
+                                               stream),
+                  "expert_linear");
+        }
+        const bool want_bias = has_bias && task_should_compute_output(2);
+        if (t[0].defined() && (task_should_compute_output(1) || want_bias)) {
+            require_saved(t[0], sizes, scalar);
+            const Rows x = product_rows(rows_of(t[0], "x"));
+            Tensor weight = at::empty(weight_sizes, options);
+            if (want_bias) out[2] = at::empty({weight_sizes[0], outputs}, options);
+            const size_t n = api.expert_weight_grad_workspace_bytes(type, rows, experts, channels, outputs);
+            const Tensor ws = at::empty({static_cast<int64_t>(n)}, options.dtype(at::kByte));
+            check(api.expert_weight_grad(type, rows, experts, channels, outputs, x.data(), x.stride, g.data(), g.stride, offsets, weight.data_ptr(),
+                                         want_bias ? out[2].data_ptr() : nullptr, ws.data_ptr(), n, stream),
+                  "expert_linear");
+            if (task_should_compute_output(1)) out[1] = std::move(weight);
+        }
+        return out;
+    }
+};
+
+Tensor expert_linear(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& positions, const Tensor& offsets) {
+    require_plain({&x, &weight, &bias, &positions, &offsets});
+    const Plan plan = plan_of(positions, offsets);
+    const int type = type_of(x.scalar_type(), "x");
+    PENC_REQUIRE(weight.scalar_type() == x.scalar_type() && (!bias.defined() || bias.scalar_type() == x.scalar_type()),
+                 "x, weight and bias of expert_linear should be of one type");
+    PENC_REQUIRE(weight.dim() == 3 && weight.size(0) == plan.experts && weight.size(1) >= 1 && weight.size(2) >= 1, "weight should have sizes (", plan.experts,
+                 ", outputs, channels), however they are ", weight.sizes());
+    const int64_t outputs = weight.size(1), channels = weight.size(2);
+    PENC_REQUIRE(x.dim() == 2 && x.size(1) == channels, "expert_linear should have rows of ", channels, " channels, however x has sizes ", x.sizes());
+    PENC_REQUIRE(outputs <= PENC_MAX_EXPERT_CHANNELS && channels <= PENC_MAX_EXPERT_CHANNELS, "an expert should have at most ", PENC_MAX_EXPERT_CHANNELS,
+                 " channels and outputs");
+    PENC_REQUIRE(!bias.defined() || (bias.dim() == 2 && bias.size(0) == plan.experts && bias.size(1) == outputs),
+                 "expert_linear should have a bias for each expert and output");
+    const c10::DeviceGuard device(x.device());
+    const bool differentiable = any_requires_grad({&x, &weight, &bias});
+    Tensor y;
+    {
+        at::NoGradGuard no_grad;
+        const Rows r = product_rows(sorted_rows(x.detach(), plan, "x"));
+        const Tensor w = weight.detach().contiguous(), b = bias.defined() ? bias.detach().contiguous() : Tensor();
+        y = at::empty({x.size(0), outputs}, x.options());
+        check(api.expert_linear(type, r.n, plan.experts, channels, outputs, r.data(), r.stride, w.const_data_ptr(), b.defined() ? b.const_data_ptr() : nullptr,
+                                plan.begins(), y.data_ptr(), current_stream(x.device())),
+              "expert_linear");
+    }
+    if (!differentiable) return y;
+    auto node = make_node<ExpertLinearNode>();
+    node->set_next_edges(torch::autograd::collect_next_edges(x, weight, bias));
+    node->type = type, node->experts = plan.experts, node->rows = x.size(0);
+    node->sizes = x.sizes().vec(), node->weight_sizes = weight.sizes().vec();
+    node->has_bias = bias.defined();
+    const Tensor none;
+    node->save({weight.requires_grad() || (bias.defined() && bias.requires_grad()) ? &x : &none, x.requires_grad() ? &weight : &none, &offsets});
+    torch::autograd::set_history(y, node);
+    return y;
+}
+
+// ------------------------------------------------------------------------------------------
 // Python
 
 void require_bound() { TORCH_CHECK(api.route != nullptr, "bind() has not been called"); }
@@ -364,10 +462,27 @@ PyObject* py_combine(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     });
 }
 
+// layers_expert_linear(x, weight, bias or None, positions, offsets)
+PyObject* py_expert_linear(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        TORCH_CHECK(n_args == 5, "layers_expert_linear takes 5 arguments");
+        require_bound();
+        const Tensor &x = tensor_arg(args[0], "x"), &weight = tensor_arg(args[1], "weight"), bias = optional_arg(args[2], "bias"),
+                     &positions = tensor_arg(args[3], "positions"), &offsets = tensor_arg(args[4], "offsets");
+        Tensor out;
+        {
+            NoGil no_gil;
+            out = expert_linear(x, weight, bias, positions, offsets);
+        }
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
 PyMethodDef methods[] = {fast<py_route>("layers_route", "the experts of rows, their weights, and where the choices stand when they are sorted by expert"),
                          fast<py_plan>("layers_plan", "where given choices stand"),
                          fast<py_dispatch>("layers_dispatch", "rows sorted by expert"),
                          fast<py_combine>("layers_combine", "weighted sums of sorted rows"),
+                         fast<py_expert_linear>("layers_expert_linear", "a linear layer of each expert on its own rows"),
                          {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace
@@ -385,6 +500,10 @@ void bind_experts(void* library) {
     PENC_FN(dispatch);
     PENC_FN(combine);
     PENC_FN(combine_backward);
+    PENC_FN(expert_linear);
+    PENC_FN(expert_linear_input_grad);
+    PENC_FN(expert_weight_grad_workspace_bytes);
+    PENC_FN(expert_weight_grad);
     PENC_FN(route);
 #undef PENC_FN
 }

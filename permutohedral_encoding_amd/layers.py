@@ -22,7 +22,7 @@ import torch
 
 from . import _native
 
-__all__ = ["Checkpoint", "checkpoint", "linear", "activation", "norm", "residual_norm", "Routing", "route", "routing", "dispatch", "combine"]
+__all__ = ["Checkpoint", "checkpoint", "linear", "activation", "norm", "residual_norm", "Routing", "route", "routing", "dispatch", "expert_linear", "combine"]
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # PENC_FP32, PENC_FP16, PENC_BF16 (include/penc.h)
 _ACTIVATIONS = {"gelu": 0, "silu": 1, "softplus": 2}
@@ -149,6 +149,12 @@ def routing(experts, number):
 def dispatch(x, routing):
     """The rows of ``x`` (..., C), one for each choice, sorted by expert: ``(rows * choices, C)``.  Choices without an expert are zeros, behind all others."""
     return _bridge().layers_dispatch(x, routing.positions, routing.offsets)
+
+
+def expert_linear(x, weight, bias, routing):
+    """A linear layer of each expert on its own rows: ``x`` (rows * choices, C) is sorted by expert, as :func:`dispatch` makes it, ``weight`` (experts, O, C) and ``bias``
+    (experts, O) or None are of its type.  Rows without an expert are zeros in the result and in the gradient, and not read.  Its input is kept as it is for the backward."""
+    return _bridge().layers_expert_linear(x, weight, bias, routing.positions, routing.offsets)
 
 
 def combine(y, weights, routing):

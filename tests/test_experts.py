@@ -43,9 +43,33 @@ def test_the_entry_points_refuse_before_they_launch():
     assert lib.penc_combine_backward(0, 0, 4, 2, 8, p, 8, z, 8, p, p, p, z, z, z) == 0  # nothing is wanted
 
 
+def test_the_products_refuse_before_they_launch():
+    lib = _native.lib()
+    block, p = _memory()
+    z = None
+    assert lib.penc_expert_linear(3, 4, 2, 8, 8, p, 8, p, p, p, p, z) == 10 == lib.penc_expert_linear_input_grad(-1, 4, 2, 8, 8, p, 8, p, p, p, z)
+    assert lib.penc_expert_weight_grad(7, 4, 2, 8, 8, p, 8, p, 8, p, p, p, p, 0, z) == 10
+    for bad in ((-1, 2, 8, 8), (1 << 31, 2, 8, 8), (4, 0, 8, 8), (4, 1025, 8, 8), (4, 2, 0, 8), (4, 2, 8, 0), (4, 2, (1 << 18) + 1, 8), (4, 2, 8, (1 << 18) + 1)):
+        assert lib.penc_expert_linear(0, *bad, p, 1 << 19, p, p, p, p, z) == 12 == lib.penc_expert_linear_input_grad(0, *bad, p, 1 << 19, p, p, p, z)
+        assert lib.penc_expert_weight_grad(0, *bad, p, 1 << 19, p, 1 << 19, p, p, p, p, 0, z) == 12 and lib.penc_expert_weight_grad_workspace_bytes(0, *bad) == 0
+    # rows that overlap, and rows too far apart
+    for stride in (7, -8, (1 << 20) + 1):
+        assert lib.penc_expert_linear(0, 4, 2, 8, 8, p, stride, p, p, p, p, z) == 12 == lib.penc_expert_linear_input_grad(0, 4, 2, 8, 8, p, stride, p, p, p, z)
+        assert lib.penc_expert_weight_grad(0, 4, 2, 8, 8, p, 8, p, stride, p, p, p, p, 0, z) == 12 == lib.penc_expert_weight_grad(0, 4, 2, 8, 8, p, stride, p, 8, p, p, p, p, 0, z)
+    assert lib.penc_expert_linear(0, 4, 2, 8, 8, z, 8, p, p, p, p, z) == 1 == lib.penc_expert_linear(0, 4, 2, 8, 8, p, 8, p, p, z, p, z)
+    assert lib.penc_expert_linear(0, 4, 2, 8, 8, p + 2, 8, p, p, p, p, z) == 5 and lib.penc_expert_linear(1, 4, 2, 8, 8, p, 8, p, p + 1, p, p, z) == 5
+    assert lib.penc_expert_linear(0, 0, 2, 8, 8, z, 8, z, z, z, z, z) == 0 == lib.penc_expert_linear_input_grad(0, 0, 2, 8, 8, z, 8, z, z, z, z)
+    need = lib.penc_expert_weight_grad_workspace_bytes(0, 1 << 20, 8, 64, 64)
+    assert 4 * 65 * 64 * 8 < need < 1 << 26 and lib.penc_expert_weight_grad_workspace_bytes(0, 100, 8, 64, 64) == 0
+    assert lib.penc_expert_weight_grad(0, 1 << 20, 8, 64, 64, p, 64, p, 64, p, p, p, p, need - 1, z) == 8
+    assert lib.penc_expert_weight_grad(0, 1 << 20, 8, 64, 64, p, 64, p, 64, p, p, p, z, need, z) == 1
+    assert lib.penc_expert_weight_grad(0, 4, 8, 64, 64, p, 64, p, 64, p, z, p, p, need, z) == 1
+
+
 def test_tensors_in_host_memory_are_refused():
     x, experts = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int64)
     plan = layers.Routing(experts, 3, experts.int(), torch.zeros(4, dtype=torch.int32))
-    for call in (lambda: layers.route(x), lambda: layers.routing(experts, 3), lambda: layers.dispatch(x, plan), lambda: layers.combine(x, x, plan)):
+    for call in (lambda: layers.route(x), lambda: layers.routing(experts, 3), lambda: layers.dispatch(x, plan), lambda: layers.combine(x, x, plan),
+                 lambda: layers.expert_linear(x, x[None], None, plan)):
         with pytest.raises(ValueError, match="GPU memory"):
             call()

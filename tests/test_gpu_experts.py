@@ -220,6 +220,171 @@ def test_rows_behind_two_to_the_31_values():
     assert torch.equal(layers.combine(there, torch.ones(rows, 1, device="cuda"), routing), x)
 
 
+# ------------------------------------------------------------------------------------------ the experts' products
+# A result is one chain of additions: of its channels, or of an expert's rows; twice 2^-24 of the terms' magnitudes for each, for additions that do not round to
+# nearest.  Products of 16-bit values are exact, those of float32 round once: another 2^-24.
+
+def products(x, weight, bias, grad, offsets):
+    """{name: (value, magnitude, length of the chain)} in 64 bits."""
+    x, weight, grad = x.detach().double(), weight.detach().double(), grad.double()
+    number, outputs, channels = weight.shape
+    out = {k: [torch.zeros(s, dtype=torch.float64, device="cuda") for _ in range(2)]
+           for k, s in (("y", (x.shape[0], outputs)), ("dx", x.shape), ("dweight", weight.shape), ("dbias", (number, outputs)))}
+    longest = 1
+    for e in range(number):
+        at = slice(int(offsets[e]), int(offsets[e + 1]))
+        longest = max(longest, at.stop - at.start)
+        for k, f in enumerate((lambda t: t, torch.abs)):
+            a, w, g = f(x[at]), f(weight[e]), f(grad[at])
+            out["y"][k][at] = a @ w.t() + (f(bias[e].detach().double()) if bias is not None else 0.0)
+            out["dx"][k][at] = g @ w
+            out["dweight"][k][e] = g.t() @ a
+            out["dbias"][k][e] = g.sum(0)
+    chain = {"y": channels + 1, "dx": outputs, "dweight": longest, "dbias": longest}
+    return {k: (*v, 2 * chain[k] + 8) for k, v in out.items()}
+
+
+def check_products(rows, number, channels, outputs, dtype, bias=True, none=0.1, extra=0, seed=0, empty=()):
+    experts = chosen_experts(rows, 1, number, seed=seed, none=none)
+    for e in empty:
+        experts[experts == e] = (e + 1) % number
+    routing = layers.routing(experts, number)
+    total = int(routing.offsets[-1])
+    x, grad = random((rows, channels + extra), 1, dtype)[:, :channels], random((rows, outputs + extra), 2, dtype)[:, :outputs]
+    x[total:] = math.nan  # (what stands in rows without an expert is not read)
+    grad[total:] = math.nan
+    x.requires_grad_(True)
+    weight = random((number, outputs, channels), 3, dtype).requires_grad_(True)
+    b = random((number, outputs), 4, dtype).requires_grad_(True) if bias else None
+    y = layers.expert_linear(x, weight, b, routing)
+    given = [t for t in (x, weight, b) if t is not None]
+    grads = dict(zip(("dx", "dweight", "dbias"), torch.autograd.grad(y, given, grad)))
+    want = products(x, weight, b, grad, routing.offsets.tolist())
+    for name, got in {"y": y, **grads}.items():
+        value, magnitude, chain = want[name]
+        assert got.dtype == dtype
+        assert_within(got, value, chain * ref.U * magnitude + ref.half_step(value, dtype), name)
+    return y, grads
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,channels,outputs", [(0, 3, 5, 7), (1, 1, 1, 1), (1, 8, 64, 64), (7, 3, 3, 2), (65, 2, 64, 64), (300, 5, 8, 24), (257, 4, 40, 72),
+                                                          (300, 7, 72, 200), (1000, 3, 130, 65), (513, 2, 203, 130), (130, 70, 48, 16), (2000, 1, 128, 256),
+                                                          (900, 4, 264, 136), (40, 1024, 16, 8), (5000, 2, 64, 3), (3000, 3, 512, 264), (700, 6, 100, 300)])
+def test_expert_linear(dtype, rows, number, channels, outputs):
+    check_products(rows, number, channels, outputs, TYPES[dtype])
+    check_products(rows, number, channels, outputs, TYPES[dtype], bias=False, none=0.0, extra=8, empty=(0,) if number > 1 else ())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_expert_linear_of_rows_that_begin_anywhere(dtype):
+    for extra in (1, 2, 3, 5):
+        check_products(401, 3, 64, 136, TYPES[dtype], extra=extra)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,channels,outputs", [(70001, 2, 64, 64), (50000, 1, 48, 130), (40000, 3, 128, 128), (20000, 300, 32, 64)])
+def test_expert_linear_of_many_rows(dtype, rows, number, channels, outputs):
+    """(the rows of an expert are cut for its weights' gradient)"""
+    first = check_products(rows, number, channels, outputs, TYPES[dtype])
+    second = check_products(rows, number, channels, outputs, TYPES[dtype])
+    assert torch.equal(first[0], second[0]) and all(torch.equal(first[1][k], second[1][k]) for k in first[1])
+
+
+def test_what_is_not_finite_stays_with_its_expert():
+    for dtype in TYPES.values():
+        for channels in (64, 67):
+            experts = torch.arange(5, device="cuda").repeat_interleave(50)[:, None]
+            routing = layers.routing(experts, 5)
+            x, weight, grad = random((250, channels), 1, dtype), random((5, 70, channels), 2, dtype), random((250, 70), 3, dtype)
+            clean = layers.expert_linear(x.requires_grad_(True), weight.requires_grad_(True), None, routing)
+            clean = [clean.detach(), *torch.autograd.grad(clean, (x, weight), grad)]
+            with torch.no_grad():
+                x[100:150], grad[100:150] = math.inf, math.nan
+                weight[3] = math.nan
+            y = layers.expert_linear(x, weight, None, routing)
+            got = [y.detach(), *torch.autograd.grad(y, (x, weight), grad)]
+            rows = torch.cat([torch.arange(100), torch.arange(200, 250)]).cuda()
+            assert all(torch.equal(a[rows], b[rows]) for a, b in zip(got[:2], clean[:2]))
+            assert torch.equal(got[2][[0, 1, 3, 4]], clean[2][[0, 1, 3, 4]])
+            assert not bool(torch.isfinite(got[2][2]).any()) and not bool(torch.isfinite(got[0][150:200]).any())
+
+
+def test_expert_linear_takes_what_it_says():
+    routing = layers.routing(torch.zeros(6, 2, dtype=torch.int64, device="cuda"), 3)
+    x, weight, bias = random((12, 8)), random((3, 5, 8), 1), random((3, 5), 2)
+    want = layers.expert_linear(x, weight, bias, routing)
+    assert torch.equal(layers.expert_linear(x, weight.transpose(1, 2).contiguous().transpose(1, 2), bias, routing), want)
+    wide = random((12, 8), 3).repeat(1, 2)
+    assert torch.equal(layers.expert_linear(wide[:, ::2], weight, bias, routing), layers.expert_linear(wide[:, ::2].contiguous(), weight, bias, routing))
+    row = random((1, 8), 4)
+    assert torch.equal(layers.expert_linear(row.expand(12, 8), weight, bias, routing), layers.expert_linear(row.repeat(12, 1), weight, bias, routing))
+    # gradients that autograd broadcasts, and each parameter alone
+    given = [t.clone().requires_grad_(True) for t in (x, weight, bias)]
+    all_of_them = torch.autograd.grad(layers.expert_linear(*given, routing).sum(), given)
+    for i in range(3):
+        alone = [t.detach().requires_grad_(k == i) for k, t in enumerate(given)]
+        assert torch.equal(torch.autograd.grad(layers.expert_linear(*alone, routing).sum(), alone[i])[0], all_of_them[i])
+    assert bool((all_of_them[2][0] == 12.0).all()) and not bool(all_of_them[1][1:].any())
+    for bad, message in [((x[:11], weight, bias), "choices"), ((x[:, :7], weight, bias), "channels"), ((x, weight[:2], bias), "sizes"),
+                         ((x, weight, bias[:, :4]), "bias"), ((x, weight.half(), bias), "one type"), ((x.double(), weight, bias), "type"),
+                         ((x, weight, bias.cpu()), "GPU memory")]:
+        with pytest.raises(ValueError, match=message):
+            layers.expert_linear(*bad, routing)
+
+
+def test_expert_linear_behind_two_to_the_31_values():
+    rows, channels = (1 << 20) + 3, 2080
+    x = torch.zeros(rows, channels, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = random((3, channels), 1, torch.bfloat16)
+    experts = torch.zeros(rows, 1, dtype=torch.int32, device="cuda")
+    experts[-3:] = 1
+    routing = layers.routing(experts, 2)
+    weight = random((2, 8, channels), 2, torch.bfloat16).requires_grad_(True)
+    y = layers.expert_linear(x.requires_grad_(True), weight, None, routing)
+    grad = torch.zeros(rows, 8, dtype=torch.bfloat16, device="cuda")
+    grad[-1, 3] = 1.0
+    dx, dw = torch.autograd.grad(y, (x, weight), grad)
+    want = x.detach()[-3:].double() @ weight.detach()[1].double().t()
+    size = x.detach()[-3:].double().abs() @ weight.detach()[1].double().abs().t()
+    assert_within(y[-3:], want, (2 * channels + 8) * ref.U * size + ref.half_step(want, torch.bfloat16), "y")
+    assert not bool(y[:-3].any()) and torch.equal(dx[-1], weight.detach()[1, 3]) and not bool(dx[:-1].any())
+    assert torch.equal(dw[1, 3], x.detach()[-1]) and not bool(dw[0].any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_layers_of_experts_together(dtype):
+    """A decoder of experts, forward and backward, against its formula with the experts that were chosen."""
+    dtype, rows, number, choices, channels, hidden = TYPES[dtype], 700, 5, 2, 48, 64
+    x = random((rows, channels), 1, dtype)
+    router = random((number, channels), 2, dtype)
+    up, bias, down = random((number, hidden, channels), 3, dtype) / 7, random((number, hidden), 4, dtype), random((number, 3, hidden), 5, dtype) / 8
+    given = [t.requires_grad_(True) for t in (x, router, up, bias, down)]
+    weights, routing = layers.route(layers.linear(x, router), choices)
+    h = layers.expert_linear(layers.dispatch(x, routing), up, bias, routing)
+    h = layers.activation(h, "silu", keep_8bit=False)
+    out = layers.combine(layers.expert_linear(h, down, None, routing), weights, routing)
+    grad = random((rows, 3), 6, dtype)
+    grads = torch.autograd.grad(out, given, grad)
+
+    at = [t.detach().double().requires_grad_(True) for t in given]
+    xd, rd, ud, bd, dd = at
+    w = torch.softmax((xd @ rd.t()).gather(1, routing.experts.long()), 1)
+    want = 0.0
+    for j in range(choices):
+        e = routing.experts[:, j].long()
+        hj = torch.nn.functional.silu((ud[e] @ xd[:, :, None])[:, :, 0] + bd[e])
+        want = want + w[:, j:j + 1] * (dd[e] @ hj[:, :, None])[:, :, 0]
+    wanted = torch.autograd.grad(want, at, grad.double())
+    # Seven results are rounded to the type on the way of a value, twelve on that of a gradient, and the checkpoint of x has steps of 1/126 of a block's
+    # largest value for the router's weight; relative to the whole, with a factor of four for values that cancel.
+    eps = torch.finfo(dtype).eps
+    assert float((out.detach().double() - want).norm()) <= 4 * (7 * eps + 2 * channels * ref.U) * float(want.detach().norm())
+    for name, g, v in zip(("x", "router", "up", "bias", "down"), grads, wanted):
+        bound = 4 * (12 * eps + 2 * rows * ref.U) + (0.02 if name == "router" else 0.0)
+        assert float((g.double() - v).norm()) <= bound * float(v.norm()), name
+
+
 # ------------------------------------------------------------------------------------------ refusals
 
 def test_refusals():
