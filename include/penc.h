@@ -536,6 +536,23 @@ int penc_expert_weight_grad(int type, int64_t rows, int experts, int64_t channel
                             int64_t grad_row_stride, const int32_t* offsets, void* weight_grad, void* bias_grad, void* workspace, size_t workspace_bytes,
                             void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Nearly orthogonal matrices from updates (penc_orthogonal.hip).  No counterpart in the reference.  Of each of `matrices` dense rows x columns matrices of a type
+ * X = update / (its Frobenius norm + eps), and `steps` times X = a X + (b S + c S S) X with S = X X^T.  A matrix of zeros stays one, one with an infinity or
+ * a NaN becomes NaN.  Coefficients that make more than 3 of a singular value, or more than 15 of the factor, are refused (PENC_ERR_UNSUPPORTED_KIND).  `result` is dense, of the same
+ * type, aligned to four values; `workspace` is aligned to 256 bytes. */
+#define PENC_MAX_MATRICES (1 << 20)
+#define PENC_MAX_MATRIX_SIDE (1 << 16)
+#define PENC_MAX_ORTHOGONAL_STEPS 64
+size_t penc_orthogonalise_workspace_bytes(int type, int64_t matrices, int64_t rows, int64_t columns);
+int penc_orthogonalise(int type, int64_t matrices, int64_t rows, int64_t columns, int steps, float a, float b, float c, float eps, const void* update, void* result,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* The rest of an optimiser's step, of n values: average += (1 - momentum) (grad - average), update = grad + momentum (average - grad) (nesterov) or average;
+ * params = decay params - rate orthogonal.  Values are of `type`, the average is fp32. */
+int penc_muon_momentum(int type, int64_t n, const void* grad, float* average, float momentum, int nesterov, void* update, void* stream);
+int penc_muon_apply(int type, int64_t n, void* params, const void* orthogonal, float decay, float rate, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

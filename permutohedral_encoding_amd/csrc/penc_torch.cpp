@@ -1310,6 +1310,7 @@ PyObject* py_bind(PyObject*, PyObject* path) {
 #undef PENC_FN
         bind_layers(lib);
         bind_experts(lib);
+        bind_orthogonal(lib);
         Py_RETURN_NONE;
     });
 }
@@ -1341,7 +1342,7 @@ PyMODINIT_FUNC PyInit__penc_torch() {
     if (!c10::FreeHipMemoryCallbacksRegistry()->Has(key))
         c10::FreeHipMemoryCallbacksRegistry()->Register(key, []() -> std::unique_ptr<c10::FreeMemoryCallback> { return std::make_unique<GiveBackSlopes>(); });
     PyObject* const made = PyModule_Create(&module);
-    if (made != nullptr && !(add_layer_functions(made) && add_expert_functions(made))) {
+    if (made != nullptr && !(add_layer_functions(made) && add_expert_functions(made) && add_orthogonal_functions(made))) {
         Py_DECREF(made);
         return nullptr;
     }

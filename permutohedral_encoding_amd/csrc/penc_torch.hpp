@@ -19,6 +19,9 @@ bool add_layer_functions(PyObject* module);
 // penc_experts_torch.cpp, likewise
 void bind_experts(void* library);
 bool add_expert_functions(PyObject* module);
+// penc_orthogonal_torch.cpp, likewise
+void bind_orthogonal(void* library);
+bool add_orthogonal_functions(PyObject* module);
 
 #define PENC_REQUIRE(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
 

@@ -1,4 +1,4 @@
-"""A fused AdamW for the encoding's table (``penc_adamw_step``).
+"""A fused AdamW for the encoding's table (``penc_adamw_step``), and Muon for the matrices behind it (``penc_orthogonalise``).
 
 The reference library has no optimiser; its scripts step the table with ``torch.optim.AdamW``
 (examples/performance.py:161), which walks the whole table with several elementwise kernels per
@@ -7,9 +7,23 @@ one kernel per parameter, and can leave entries whose gradient is exactly zero u
 (``skip_zero_gradients``), the usual way to train hash tables most of whose slots see no point in a
 step.
 """
+import math
+
 import torch
 
 from . import _native
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # a s + b s^3 + c s^5 takes small singular values up fastest (K. Jordan et al., "Muon", 2024)
+
+
+def orthogonalise(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    """Nearly orthogonal matrices from those of ``update`` (..., rows, columns), float32, float16 or bfloat16 in GPU memory: ``X = G / (|G| + eps)`` with the Frobenius norm, and
+    ``steps`` times ``X = a X + (b S + c S S) X`` with ``S = X X^T``, which takes each singular value s of X to ``a s + b s^3 + c s^5``.
+
+    The products are of float16 twice (22 bits) for float32 and float16, of float16 for bfloat16, sums in float32.  Zeros stay zeros, a matrix with an infinity or a NaN becomes NaN.
+    Coefficients that make more than 3 of a singular value, or more than 15 of the factor, are refused.  No gradient is recorded."""
+    a, b, c = coefficients
+    return _native.bridge().orthogonalise(update, steps, a, b, c, eps)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -109,4 +123,62 @@ class SparseTableAdamW(torch.optim.Optimizer):
                 _native.bridge().adamw_step_sparse(p, sparse.grad, state["exp_avg"], state["exp_avg_sq"], sparse.touched,
                                                    float(group["lr"]), float(beta1), float(beta2), float(group["eps"]),
                                                    float(group["weight_decay"]), int(state["step"]))
+        return loss
+
+
+class Muon(torch.optim.Optimizer):
+    """Steps along orthogonalised momentum, for the weights of hidden layers: matrices, or stacks of them such as those of
+    :func:`layers.expert_linear` (..., rows, columns), float32, float16 or bfloat16 in GPU memory.  As ``torch.optim.Muon`` ::
+
+        m = m + (1 - momentum) (g - m);    u = g + momentum (m - g) with nesterov, else m
+        p = (1 - lr weight_decay) p - lr scale orthogonalise(u)
+
+    with ``scale`` sqrt(max(1, rows / columns)), or 0.2 sqrt(max(rows, columns)) with ``match_rms_adamw``.  The average m is float32, u of the parameter's type; parameters of one
+    size go through the products together.  Tables, norms and biases take another optimiser.  (A captured step keeps the ``lr`` that it was captured with.)
+    """
+
+    def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, steps=5, coefficients=COEFFICIENTS, eps=1e-7, match_rms_adamw=False):
+        if lr < 0.0 or weight_decay < 0.0 or not 0.0 <= momentum < 1.0:
+            raise ValueError("Muon: lr and weight_decay must be non-negative and momentum in [0, 1)")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=bool(nesterov), weight_decay=weight_decay, steps=steps, coefficients=tuple(coefficients), eps=eps,
+                                      match_rms_adamw=bool(match_rms_adamw)))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() < 2:
+                    raise ValueError(f"Muon: parameters must be matrices or stacks of them, not of sizes {tuple(p.shape)}")
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # (which brings floating-point state to the parameters' type: the averages stay float32)
+        params = [p for group in self.param_groups for p in group["params"]]
+        numbers = [n for group in state_dict["param_groups"] for n in group["params"]]
+        for p, n in zip(params, numbers):
+            if n in state_dict["state"]:
+                self.state[p]["momentum_buffer"] = state_dict["state"][n]["momentum_buffer"].to(device=p.device, dtype=torch.float32, copy=True)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            together = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if not (p.is_cuda and p.is_contiguous()):
+                    raise RuntimeError("Muon: parameters must be contiguous tensors in GPU memory")
+                if p.grad.layout != torch.strided or p.grad.dtype != p.dtype:
+                    raise RuntimeError("Muon: gradients must be dense and of the parameter's type")
+                state = self.state[p]
+                if not state:
+                    state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                together.setdefault((tuple(p.shape), p.dtype, p.device), []).append((p, p.grad.contiguous(), state["momentum_buffer"]))
+            for (shape, _, _), members in together.items():
+                rows, columns = shape[-2:]
+                scale = 0.2 * math.sqrt(max(rows, columns)) if group["match_rms_adamw"] else math.sqrt(max(1.0, rows / columns))
+                params, grads, averages = map(list, zip(*members))
+                _native.bridge().muon_step(params, grads, averages, group["steps"], *group["coefficients"], group["eps"], group["momentum"], group["nesterov"],
+                                           1.0 - group["lr"] * group["weight_decay"], group["lr"] * scale)
         return loss

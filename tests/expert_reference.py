@@ -52,3 +52,27 @@ def plan(chosen, number):
     counts = torch.bincount(flat, minlength=number + 1)
     offsets = torch.cat([counts.new_zeros(1), counts[:number].cumsum(0)])
     return positions.view(chosen.shape).int(), offsets.int()
+
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalise(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, stored=lambda t: t, dtype=torch.float64):
+    """The steps in ``dtype``, X, S and the factor going through ``stored``."""
+    a, b, c = coefficients
+    g = update.to(dtype)
+    tall = g.shape[-2] > g.shape[-1]
+    g = g.transpose(-1, -2).contiguous() if tall else g
+    norm = g.double().square().sum((-1, -2), keepdim=True).sqrt().to(dtype)
+    x = stored(g / (norm + eps))
+    for step in range(steps):
+        s = stored(x @ x.transpose(-1, -2).contiguous())
+        f = stored(b * s + c * (s @ s))
+        x = a * x + f @ x
+        x = stored(x) if step + 1 < steps else x
+    return x.transpose(-1, -2).contiguous() if tall else x
+
+
+def in_float16(t):
+    """As 64-bit numbers, what float16 holds of them times 2^12."""
+    return (t * 4096.0).half().double() / 4096.0

@@ -73,3 +73,26 @@ def test_tensors_in_host_memory_are_refused():
                  lambda: layers.expert_linear(x, x[None], None, plan)):
         with pytest.raises(ValueError, match="GPU memory"):
             call()
+
+
+def test_orthogonalise_refuses_before_it_launches():
+    lib = _native.lib()
+    block, p = _memory()
+    p += (-p) % 256
+    z, good = None, (3.4445, -4.7750, 2.0315)
+    call = lambda t=0, m=1, r=8, c=9, steps=5, k=good, eps=1e-7, g=p, to=p + 1024, ws=p, n=1 << 30: lib.penc_orthogonalise(t, m, r, c, steps, *k, eps, g, to, ws, n, z)  # noqa: E731
+    assert call(t=3) == 10 and call(m=-1) == 12 and call(m=(1 << 20) + 1) == 12 and call(r=0) == 12 and call(c=(1 << 16) + 1) == 12 and call(steps=0) == 12 and call(steps=65) == 12
+    assert call(eps=0.0) == 11 and call(eps=float("nan")) == 11 and call(eps=float("inf")) == 11
+    # singular values over 3 and factors over 15 are refused, wherever on the way they come up
+    for k in ((4.0, 0.0, 0.0), (float("nan"), 0.0, 0.0), (1.0, 16.0, -16.0), (2.0, 1.5, 0.0), (0.0, 0.0, float("inf"))):
+        assert call(k=k) == 11
+    assert call(k=(2.0, 0.0, 0.0), steps=1, g=z) == 1 and call(k=(2.0, 0.0, 0.0), steps=2) == 11
+    assert call(k=(1.5, -0.5, 0.0), steps=64, g=z) == 1 and call(steps=64, g=z) == 1
+    assert call(g=z) == 1 and call(to=z) == 1 and call(g=p + 2) == 5 and call(to=p + 4) == 5 and call(ws=p + 16) == 5 and call(m=0, g=z, to=z) == 0
+    # small matrices need no workspace
+    assert lib.penc_orthogonalise_workspace_bytes(0, 100, 64, 256) == 0 == lib.penc_orthogonalise_workspace_bytes(0, 1, 0, 4)
+    need = lib.penc_orthogonalise_workspace_bytes(2, 2, 1000, 203)
+    assert need >= 2 * (2 * 1000 * 256 + 2 * 203 * 256) * 2 and lib.penc_orthogonalise_workspace_bytes(0, 2, 1000, 203) > need
+    assert call(t=2, m=2, r=1000, c=203, n=need - 1) == 8 and call(t=2, m=2, r=1000, c=203, ws=z) == 1
+    assert lib.penc_muon_momentum(0, -1, p, p, 0.9, 1, p, z) == 12 and lib.penc_muon_momentum(0, 4, z, p, 0.9, 1, p, z) == 1 and lib.penc_muon_momentum(0, 0, z, z, 0.9, 1, z, z) == 0
+    assert lib.penc_muon_apply(4, 4, p, p, 1.0, 0.1, z) == 10 and lib.penc_muon_apply(0, 4, p, p + 2, 1.0, 0.1, z) == 5 and lib.penc_muon_apply(0, 4, p, z, 1.0, 0.1, z) == 1

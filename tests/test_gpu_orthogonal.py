@@ -1,0 +1,239 @@
+"""Orthogonalised updates on the GPU against the same steps in 64 bits (expert_reference.py).
+
+Tolerances, of a matrix's Frobenius norm.  An error of a step is taken up by the steps behind it, by factors that depend on the matrix, so that the measure is what the same steps
+make of roundings of the same kind: in float32 for float32 and float16, where a stored number is off by up to 2^-22 instead of 2^-24 (a factor of four) and a product leaves out
+as much again (two); with X, S and the factor in float16 for bfloat16 (a factor of two for another order of the sums, and as much for the luck of single roundings).  The result's own
+rounding comes on top.  A single value is off by at most 16 times the mean of that (of 10^6 normally distributed errors the largest is 5)."""
+import math
+
+import pytest
+import torch
+
+import expert_reference as ref
+from permutohedral_encoding_amd import layers, optim
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def updates(matrices, rows, columns, dtype, seed=0, scale=1e-3):
+    """Channels of different sizes, and a few directions that carry much."""
+    kw = dict(generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+    rank = min(3, rows, columns)
+    g = torch.randn((matrices, rows, columns), **kw) * torch.exp(0.5 * torch.randn((matrices, 1, columns), **kw))
+    return (scale * (g + torch.randn((matrices, rows, rank), **kw) @ torch.randn((matrices, rank, columns), **kw))).to(dtype)
+
+
+def norms(t):
+    return t.double().square().sum((-1, -2)).sqrt()
+
+
+def assert_orthogonalised(got, update, **given):
+    want = ref.orthogonalise(update, **given)
+    assert got.shape == update.shape and got.dtype == update.dtype
+    if got.dtype == torch.bfloat16:
+        allowed = 4 * norms(ref.orthogonalise(update, stored=ref.in_float16, **given) - want)
+    else:
+        allowed = 8 * norms(ref.orthogonalise(update, dtype=torch.float32, **given).double() - want)
+    # (a matrix of few values may have them all right in float32 by luck: 16 roundings of a value of 1, each taken up threefold by two steps)
+    allowed = allowed + 144 * ref.U * norms(want) + norms(ref.half_step(want, got.dtype))
+    error = (got.double() - want).abs()
+    assert bool((norms(error) <= allowed).all()), f"worst error/bound {float((norms(error) / allowed).max()):.3g}"
+    worst = 16 * allowed / math.sqrt(want.shape[-1] * want.shape[-2]) + 2 * ref.half_step(want, got.dtype).amax((-1, -2))
+    assert bool((error.amax((-1, -2)) <= worst).all()), f"worst single error/bound {float((error.amax((-1, -2)) / worst).max()):.3g}"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("matrices,rows,columns", [(1, 1, 1), (2, 1, 5), (2, 7, 1), (3, 2, 2), (3, 16, 16), (2, 31, 33), (3, 64, 64), (16, 256, 64), (2, 65, 300), (1, 128, 128),
+                                                   (2, 160, 128), (1, 100, 250), (300, 20, 24), (1, 127, 190), (1, 64, 500), (2, 33, 1000)])
+def test_matrices_that_stay_in_the_lds_or_nearly(dtype, matrices, rows, columns):
+    update = updates(matrices, rows, columns, TYPES[dtype])
+    assert_orthogonalised(optim.orthogonalise(update), update)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("matrices,rows,columns", [(1, 130, 130), (1, 203, 1000), (1, 1000, 203), (2, 257, 513), (1, 129, 3), (3, 1, 5000), (2, 4097, 2), (1, 512, 512), (3, 300, 700),
+                                                   (1, 2100, 161), (40, 520, 530), (33, 531, 390), (20, 260, 1030)])
+def test_larger_matrices(dtype, matrices, rows, columns):
+    update = updates(matrices, rows, columns, TYPES[dtype])
+    assert_orthogonalised(optim.orthogonalise(update), update)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_steps_coefficients_and_eps(dtype):
+    for shape in ((3, 40, 60), (2, 140, 200)):
+        update = updates(*shape, TYPES[dtype])
+        for given in (dict(steps=1), dict(steps=2), dict(steps=8), dict(coefficients=(1.5, -0.5, 0.0), steps=6), dict(coefficients=(1.875, -1.25, 0.375), steps=4),
+                      dict(eps=1e-2), dict(eps=1.0)):
+            assert_orthogonalised(optim.orthogonalise(update, **given), update, **given)
+
+
+def test_updates_of_any_size():
+    """Squares that float32 does not have, above and below."""
+    for shape in ((2, 24, 40), (2, 140, 150)):
+        for scale in (2.0 ** 116, 2.0 ** -110):
+            update = updates(*shape, torch.float32, scale=scale)
+            assert_orthogonalised(optim.orthogonalise(update, eps=1e-30), update, eps=1e-30)
+
+
+def test_zeros_and_what_is_not_finite_stay_with_their_matrix():
+    for dtype in TYPES.values():
+        for shape in ((5, 30, 50), (5, 140, 133)):
+            update = updates(*shape, dtype)
+            want = optim.orthogonalise(update)
+            update[1] = 0.0
+            update[2, 3, 4] = math.nan
+            update[3, 7, 8] = math.inf
+            got = optim.orthogonalise(update)
+            assert torch.equal(got[[0, 4]], want[[0, 4]]) and not bool(got[1].any()) and bool(torch.isnan(got[2:4]).all())
+
+
+def test_updates_of_other_shapes():
+    update = updates(6, 40, 30, torch.float32)
+    want = optim.orthogonalise(update)
+    assert torch.equal(optim.orthogonalise(update.view(2, 3, 40, 30)), want.view(2, 3, 40, 30))
+    assert torch.equal(optim.orthogonalise(update[2]), want[2])
+    assert torch.equal(optim.orthogonalise(update[:, ::2].contiguous()), optim.orthogonalise(update[:, ::2]))
+    assert optim.orthogonalise(update[:0]).shape == (0, 40, 30)
+    turned = optim.orthogonalise(update.transpose(1, 2)).transpose(1, 2)
+    assert float((turned - want).norm()) <= 1e-5 * float(want.norm())
+    required = update.clone().requires_grad_(True)
+    assert not optim.orthogonalise(required).requires_grad
+    assert torch.equal(optim.orthogonalise(required), want)
+
+
+def test_refusals():
+    update = updates(1, 8, 9, torch.float32)
+    for call, message in [(lambda: optim.orthogonalise(update, steps=0), "steps"), (lambda: optim.orthogonalise(update, steps=65), "steps"),
+                          (lambda: optim.orthogonalise(update, eps=0.0), "eps"), (lambda: optim.orthogonalise(update, eps=math.nan), "eps"),
+                          (lambda: optim.orthogonalise(update, coefficients=(4.0, 0.0, 0.0)), "coefficients"),
+                          (lambda: optim.orthogonalise(update, coefficients=(math.nan, 0.0, 0.0)), "coefficients"),
+                          (lambda: optim.orthogonalise(update, coefficients=(1.0, 16.0, -16.0)), "coefficients"),
+                          (lambda: optim.orthogonalise(update[0, 0]), "matrices"), (lambda: optim.orthogonalise(update.double()), "type"),
+                          (lambda: optim.orthogonalise(update[:, :0]), "matrices"), (lambda: optim.orthogonalise(update.cpu()), "GPU memory"),
+                          (lambda: optim.Muon([torch.zeros(3, requires_grad=True, device="cuda")]), "stacks"), (lambda: optim.Muon([update], lr=-1.0), "lr")]:
+        with pytest.raises(ValueError, match=message):
+            call()
+
+
+def test_on_another_stream_and_in_a_graph():
+    for shape in ((4, 64, 96), (2, 150, 200)):
+        given = updates(*shape, torch.bfloat16)
+        want = optim.orthogonalise(given)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = optim.orthogonalise(given)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = optim.orthogonalise(given)
+        for seed in range(3):
+            given.copy_(updates(*shape, torch.bfloat16, seed=seed + 1))
+            graph.replay()
+            want = optim.orthogonalise(given)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------------------------------ the optimiser
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nesterov,match", [(True, False), (False, True)])
+def test_muon_follows_its_formula(dtype, nesterov, match):
+    dtype = TYPES[dtype]
+    shapes = [(64, 48), (3, 40, 30), (64, 48), (140, 150)]
+    params = [torch.nn.Parameter(updates(1, s[-2] * (s[0] if len(s) == 3 else 1), s[-1], dtype, seed=i, scale=0.1).view(s)) for i, s in enumerate(shapes)]
+    lr, momentum, decay = 0.02, 0.9, 0.1
+    opt = optim.Muon(params, lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=decay, match_rms_adamw=match)
+    averages = [torch.zeros(s, dtype=torch.float64, device="cuda") for s in shapes]
+    for step in range(3):
+        for i, p in enumerate(params):
+            p.grad = updates(1, *p.shape[-2:], dtype, seed=10 * step + i).expand(p.shape if p.dim() == 3 else (1, *p.shape)).reshape(p.shape).clone() if step != 1 or i != 1 else None
+        before, versions = [p.detach().double() for p in params], [p._version for p in params]
+        opt.step()
+        for i, (p, m) in enumerate(zip(params, averages)):
+            if p.grad is None:
+                assert torch.equal(p.double(), before[i]) and p._version == versions[i]
+                continue
+            assert p._version > versions[i]
+            g = p.grad.double()
+            m += (1 - momentum) * (g - m)
+            # two roundings of a value or average a step, three steps
+            assert bool((opt.state[p]["momentum_buffer"].double() - m).abs().max() <= 6 * ref.U * (g.abs().max() + m.abs().max()) + 1e-30)
+            assert opt.state[p]["momentum_buffer"].dtype == torch.float32
+            u = (g + momentum * (m - g) if nesterov else m).to(dtype)
+            rows, columns = p.shape[-2:]
+            rate = lr * (0.2 * math.sqrt(max(rows, columns)) if match else math.sqrt(max(1.0, rows / columns)))
+            want = (1 - lr * decay) * before[i] - rate * ref.orthogonalise(u)
+            # the update's own rounding can fall to the other side, and is taken up by the steps; then the direction's rounding and the parameter's
+            loose = {torch.float32: 1e-4, torch.float16: 2e-2, torch.bfloat16: 6e-2}[dtype]
+            assert bool((norms(p.detach().double() - want) <= loose * rate * norms(ref.orthogonalise(u)) + norms(ref.half_step(want, dtype))).all())
+
+
+def test_muon_and_torchs():
+    p, q = (torch.nn.Parameter(updates(1, 96, 64, torch.float32, seed=1, scale=0.1)[0]) for _ in range(2))
+    ours, theirs = optim.Muon([p], lr=0.02), torch.optim.Muon([q], lr=0.02)
+    start = p.detach().clone()
+    for step in range(3):
+        p.grad = updates(1, 96, 64, torch.float32, seed=step + 2)[0]
+        q.grad = p.grad.clone()
+        ours.step()
+        theirs.step()
+    # (theirs takes its products in bfloat16, which are off by 1e-2 of the step)
+    assert float((p - q).detach().norm()) <= 0.05 * float((p - start).detach().norm())
+
+
+def test_muon_comes_back_from_a_checkpoint():
+    def steps(opt, p, seeds):
+        for seed in seeds:
+            p.grad = updates(1, 40, 50, p.dtype, seed=seed)[0]
+            opt.step()
+
+    for dtype in TYPES.values():
+        p = torch.nn.Parameter(updates(1, 40, 50, dtype, seed=1, scale=0.1)[0])
+        opt = optim.Muon([p], lr=0.02)
+        steps(opt, p, (2, 3))
+        q = torch.nn.Parameter(p.detach().clone())
+        again = optim.Muon([q], lr=0.5)
+        again.load_state_dict(opt.state_dict())
+        assert again.state[q]["momentum_buffer"].dtype == torch.float32
+        assert torch.equal(again.state[q]["momentum_buffer"], opt.state[p]["momentum_buffer"])
+        steps(opt, p, (4,))
+        steps(again, q, (4,))
+        assert torch.equal(p, q)
+
+
+def test_muon_refuses():
+    p = torch.nn.Parameter(torch.zeros(8, 6, device="cuda").t())
+    p.grad = torch.ones_like(p)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        optim.Muon([p]).step()
+    p = torch.nn.Parameter(torch.zeros(8, 6, device="cuda"))
+    p.grad = torch.ones_like(p).to_sparse()
+    with pytest.raises(RuntimeError, match="dense"):
+        optim.Muon([p]).step()
+
+
+def test_a_decoder_of_experts_trains_with_muon():
+    """Every piece together: rows go to experts, come back, and the stacks of weights take a step against the gradient."""
+    generator = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(2000, 32, generator=generator, device="cuda")
+    stacks = [torch.nn.Parameter(torch.randn(s, generator=generator, device="cuda") / math.sqrt(s[-1])) for s in ((4, 64, 32), (4, 32, 64))]
+    router = torch.nn.Parameter(torch.randn(4, 32, generator=generator, device="cuda") / 6)
+    opt = optim.Muon([*stacks, router], lr=1e-3, weight_decay=0.0)
+
+    def loss():
+        weights, routing = layers.route(layers.linear(x, router), 2)
+        h = layers.activation(layers.expert_linear(layers.dispatch(x, routing), stacks[0], None, routing), "gelu")
+        return layers.combine(layers.expert_linear(h, stacks[1], None, routing), weights, routing).square().mean()
+
+    for _ in range(3):
+        opt.zero_grad()
+        loss().backward()
+        before = [p.detach().clone() for p in opt.param_groups[0]["params"]]
+        opt.step()
+        for p, b in zip(opt.param_groups[0]["params"], before):
+            assert float(((p - b) * p.grad).sum()) < 0.0  # (a matrix and what its singular values are made equal of have a positive product)
