@@ -22,6 +22,21 @@ namespace {
 using Value = std::conditional_t<PENC_TYPE == PENC_FP32, float, std::conditional_t<PENC_TYPE == PENC_FP16, half_t, bf16_t>>;
 constexpr int kSize = sizeof(Value);
 
+// The sum of a wave's values up to each lane.
+__device__ __forceinline__ uint32_t sum_to_lane(uint32_t v) {
+    const auto moved = [](uint32_t x, auto control, auto rows) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(control)::value, decltype(rows)::value, 0xF, false));
+    };
+    constexpr std::integral_constant<int, 0xF> all{};
+    v += moved(v, std::integral_constant<int, 0x111>{}, all);  // from 1, 2, 4 and 8 lanes before, of 16
+    v += moved(v, std::integral_constant<int, 0x112>{}, all);
+    v += moved(v, std::integral_constant<int, 0x114>{}, all);
+    v += moved(v, std::integral_constant<int, 0x118>{}, all);
+    v += moved(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // the last of 16 lanes to the next 16
+    v += moved(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // the last of 32 to the others
+    return v;
+}
+
 // Tile `t` of rows: those of an expert (`experts`: the rows behind the last one's), cut every `most` rows.
 struct RowTile {
     int expert, first, rows, of_expert, tiles;  // of_expert: which of the expert's tiles it is; tiles: the expert's; expert < 0: there is no such tile
@@ -42,23 +57,18 @@ __device__ __forceinline__ RowTile row_tile(const int32_t* __restrict__ offsets,
         uint32_t tiles = (static_cast<uint32_t>(n) + most - 1) / most;
         if (!kWhole && e < experts) tiles = max(tiles, 1u);
         if (e > experts || (!kWhole && e == experts)) tiles = 0;
-        uint32_t sum = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t other = __shfl_up(sum, d);
-            sum += lane >= d ? other : 0u;
-        }
+        const uint32_t sum = sum_to_lane(tiles);
         const uint64_t behind = __ballot(t < before + sum);
         if (behind != 0) {
             const int found = __builtin_ctzll(behind);
-            const int first = __shfl(from, found), count = __shfl(n, found);
-            const uint32_t its = __shfl(tiles, found), at = t - before - (__shfl(sum, found) - its);
-            const int skip = static_cast<int>(at) * most;
-            return {__builtin_amdgcn_readfirstlane(base + found), __builtin_amdgcn_readfirstlane(first + skip),
-                    __builtin_amdgcn_readfirstlane(min(count - skip, most)), __builtin_amdgcn_readfirstlane(static_cast<int>(at)),
-                    __builtin_amdgcn_readfirstlane(static_cast<int>(its))};
+            const auto its_own = [&](int v) { return __builtin_amdgcn_readlane(v, found); };
+            const int first = its_own(from), count = its_own(n);
+            const uint32_t its = its_own(tiles), at = t - before - (its_own(sum) - its);
+            // (tiles of rows are full but for the last one; pieces for the weights' gradient are alike)
+            const int each = kWhole ? most : (count / static_cast<int>(its) / 64 + 1) * 64, skip = min(static_cast<int>(at) * each, count);
+            return {base + found, first + skip, min(count - skip, each), static_cast<int>(at), static_cast<int>(its)};
         }
-        before += __shfl(sum, 63);
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
     return {-1, 0, 0, 0, 0};
 }
@@ -69,41 +79,46 @@ struct RowsArgs {
     int64_t stride;                // of rows_in, in values
     const int32_t* offsets;
     int experts, rows, wide, deep; // wide: values of a row of the result; deep: of the operand
-    uint32_t items, tiles;         // tiles: of a row of the result
-    bool aligned;                  // whether four results can be stored at once
+    Spread spread;
+    uint32_t tiles;                // of a row of the result
+    bool aligned;                  // whether rows of the result begin on 16 bytes
 };
+
+constexpr uint32_t kGroup = 8;
 
 // y (kBack false: weights by rows of k) or dx.
 template <bool kBack, class P>
 __global__ __launch_bounds__(P::kThreads) void expert_rows_kernel(RowsArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
-    const uint32_t item = item_of(a.items);
-    const RowTile t = row_tile<true>(a.offsets, a.experts, a.rows, item / a.tiles, P::kN);
+    // eight tiles of rows to each tile of weights, one after the other: what a die works on at a time fits its cache
+    const uint32_t item = a.spread.item(), of_group = kGroup * a.tiles, group = item / of_group, in_group = item % of_group;
+    if (item >= a.spread.items) return;
+    const uint32_t grouped = min(kGroup, a.spread.items / a.tiles - group * kGroup);
+    const RowTile t = row_tile<true>(a.offsets, a.experts, a.rows, group * kGroup + in_group % grouped, P::kN);
     if (t.expert < 0) return;
-    const int m0 = static_cast<int>(item % a.tiles) * P::kM;
+    const int m0 = static_cast<int>(in_group / grouped) * P::kM;
     P p;
+    const int columns = a.wide - m0;
     if (t.expert == a.experts) {
-        p.run(lds, {}, {}, 0, [](const char*, int) {});
+        p.start(P::kZero);
     } else {
+        const Value* const bias = !kBack && a.bias != nullptr ? static_cast<const Value*>(a.bias) + static_cast<int64_t>(t.expert) * a.wide + m0 : nullptr;
         const char* const weight = static_cast<const char*>(a.weight) + static_cast<int64_t>(t.expert) * a.wide * a.deep * kSize;
-        const int m_rows = min(a.wide - m0, P::kM);
+        const int m_rows = min(columns, P::kM);
         const Operand m = kBack ? Operand{weight + static_cast<int64_t>(m0) * kSize, static_cast<int64_t>(a.wide) * kSize, a.deep, m_rows * kSize}
                                 : Operand{weight + static_cast<int64_t>(m0) * a.deep * kSize, static_cast<int64_t>(a.deep) * kSize, m_rows, a.deep * kSize};
         const Operand n{static_cast<const char*>(a.rows_in) + static_cast<int64_t>(t.first) * a.stride * kSize, a.stride * kSize, t.rows, a.deep * kSize};
-        p.run(lds, m, n, a.deep, [](const char*, int) {});
-    }
-    const Value* const bias = !kBack && a.bias != nullptr && t.expert < a.experts ? static_cast<const Value*>(a.bias) + static_cast<int64_t>(t.expert) * a.wide : nullptr;
-    Value* const out = static_cast<Value*>(a.rows_out) + static_cast<int64_t>(t.first) * a.wide;
-    p.each([&](int m, int n, tile_acc v) {
-        const int valid = a.wide - m0 - m;
-        if (n >= t.rows || valid <= 0) return;
-        if (!kBack && bias != nullptr) {
+        const auto first = [&](int m) {
+            tile_acc v{};
+            if (bias != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < valid) v[i] += static_cast<float>(bias[m0 + m + i]);
-        }
-        store_four(out + static_cast<int64_t>(n) * a.wide + m0 + m, v, valid, a.aligned);
-    });
+                for (int k = 0; k < 4; ++k) v[k] = m + k < columns ? static_cast<float>(bias[m + k]) : 0.0f;
+            }
+            return v;
+        };
+        p.run(lds, m, n, a.deep, first, P::kNothing);
+    }
+    store_rows(p, static_cast<Value*>(a.rows_out) + static_cast<int64_t>(t.first) * a.wide + m0, a.wide, t.rows, columns, a.aligned);
 }
 
 struct WeightArgs {
@@ -111,7 +126,8 @@ struct WeightArgs {
     int64_t x_stride, grad_stride;
     const int32_t* offsets;
     int experts, rows, channels, outputs, most;  // most: rows of a piece
-    uint32_t items, channel_tiles, tiles;
+    Spread spread;
+    uint32_t channel_tiles, tiles;
     void *weight, *bias;  // results, written where an expert's rows are one piece
     float* sums;          // [pieces][outputs][channels], and behind them [pieces][outputs]
     int64_t pieces;
@@ -122,7 +138,8 @@ struct WeightArgs {
 template <class P>
 __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
-    const uint32_t item = item_of(a.items), piece = item / a.tiles, tile = item % a.tiles;
+    const uint32_t item = a.spread.item(), piece = item / a.tiles, tile = item % a.tiles;
+    if (item >= a.spread.items) return;
     const RowTile t = row_tile<false>(a.offsets, a.experts, a.rows, piece, a.most);
     if (t.expert < 0) return;
     const int c0 = static_cast<int>(tile % a.channel_tiles) * P::kM, o0 = static_cast<int>(tile / a.channel_tiles) * P::kN;
@@ -135,23 +152,16 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
     tile_acc bias_acc[P::kTilesN] = {};
     const uint32_t one = PENC_TYPE == PENC_FP32 ? 0x3F800000u : PENC_TYPE == PENC_FP16 ? 0x3C003C00u : 0x3F803F80u;
     const chunk16 ones = {one, one, one, one};
-    p.run(lds, m, n, t.rows, [&](const char* step, int) {
+    p.run(lds, m, n, t.rows, P::kZero, [&](const chunk16 (&grad)[P::kTilesN]) {
         if (!bias) return;
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int j = 0; j < P::kTilesN; ++j)
-                bias_acc[j] = multiply<Value>(ones, P::TileN::fragment(step + P::TileM::kSize, P::wave_n() + 16 * j, q), bias_acc[j]);
+        for (int j = 0; j < P::kTilesN; ++j) bias_acc[j] = multiply<Value>(ones, grad[j], bias_acc[j]);
     });
     const int64_t n_weights = static_cast<int64_t>(a.outputs) * a.channels;
     const bool whole = t.tiles == 1;
-    p.each([&](int c, int o, tile_acc v) {
-        const int valid = a.channels - c0 - c;
-        if (o0 + o >= a.outputs || valid <= 0) return;
-        const int64_t at = static_cast<int64_t>(o0 + o) * a.channels + c0 + c;
-        if (whole) store_four(static_cast<Value*>(a.weight) + t.expert * n_weights + at, v, valid, a.aligned);
-        else store_four(a.sums + piece * n_weights + at, v, valid, a.channels % 4 == 0);
-    });
+    const int64_t at = static_cast<int64_t>(o0) * a.channels + c0;
+    if (whole) store_rows(p, static_cast<Value*>(a.weight) + t.expert * n_weights + at, a.channels, a.outputs - o0, a.channels - c0, a.aligned);
+    else store_rows(p, a.sums + piece * n_weights + at, a.channels, a.outputs - o0, a.channels - c0, a.channels % 4 == 0);
     if (!bias) return;
     const int lane = threadIdx.x % 64;
 #pragma unroll
@@ -196,35 +206,41 @@ __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, 
 // Whether chunks of 16 bytes are on 16 bytes.
 bool chunked(const void* p, int64_t stride, int64_t bytes) { return aligned_to(p, 16) && stride * kSize % 16 == 0 && bytes * kSize % 16 == 0; }
 
+// (a launch has less than 2^32 threads, and a spread rounds up)
+constexpr int64_t kMostThreads = (int64_t{1} << 32) - (1 << 18);
+
 template <bool kBack, class P>
 int launch_rows(RowsArgs a, hipStream_t stream) {
     a.tiles = static_cast<uint32_t>((a.wide + P::kM - 1) / P::kM);
     const int64_t items = (a.rows / P::kN + static_cast<int64_t>(a.experts) + 1) * a.tiles;
-    if (items * P::kThreads >= int64_t{1} << 32) return PENC_ERR_BAD_LAYER_SIZE;
-    a.items = static_cast<uint32_t>(items);
-    expert_rows_kernel<kBack, P><<<a.items, P::kThreads, 0, stream>>>(a);
+    if (items * P::kThreads >= kMostThreads) return PENC_ERR_BAD_LAYER_SIZE;
+    a.spread = Spread(items, 32);
+    expert_rows_kernel<kBack, P><<<a.spread.grid(), P::kThreads, 0, stream>>>(a);
     return launched();
 }
 
 template <bool kBack, bool kDirect>
 int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
     if (a.wide <= 64) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kDirect>>(a, stream);
+    if constexpr (kDirect && kSize == 2) {
+        if (static_cast<int64_t>(a.rows / 256 + a.experts) * ((a.wide + 255) / 256) >= 512) return launch_rows<kBack, Product<Value, kBack, false, 256, 256, 4, 2, true>>(a, stream);
+    }
     return launch_rows<kBack, Product<Value, kBack, false, 128, 128, 2, 2, kDirect>>(a, stream);
 }
 
 // How the rows of the weights' gradient are cut.
 struct WeightPlan {
-    bool small;    // tiles of 64 x 64, else of 128 x 128
+    int side;      // of a tile
     int64_t tiles; // of an expert
     int64_t most;  // rows of a piece
     int64_t pieces;
 };
 WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
     WeightPlan p;
-    p.small = channels <= 64 || outputs <= 64;
-    const int64_t side = p.small ? 64 : 128;
+    p.side = channels <= 64 || outputs <= 64 ? 64 : kSize == 2 && channels >= 256 && outputs >= 256 && rows * channels * outputs >= int64_t{1} << 34 ? 256 : 128;
+    const int64_t side = p.side;
     p.tiles = ((channels + side - 1) / side) * ((outputs + side - 1) / side);
-    const int64_t wanted = (1024 + p.tiles - 1) / p.tiles;  // pieces for four workgroups to a compute unit
+    const int64_t wanted = ((side == 256 ? 512 : 1024) + p.tiles - 1) / p.tiles;  // pieces for four workgroups to a compute unit
     int64_t most = experts >= wanted ? 2 * ((rows + experts - 1) / experts) : (rows + wanted - 1) / wanted;
     most = std::max<int64_t>((most + 63) / 64 * 64, 512);
     p.most = std::min<int64_t>(most, (int64_t{1} << 30));
@@ -237,15 +253,19 @@ int launch_weights(WeightArgs a, const WeightPlan& plan, hipStream_t stream) {
     a.channel_tiles = static_cast<uint32_t>((a.channels + P::kM - 1) / P::kM);
     a.tiles = static_cast<uint32_t>(plan.tiles);
     const int64_t items = plan.pieces * plan.tiles;
-    if (items * P::kThreads >= int64_t{1} << 32) return PENC_ERR_BAD_LAYER_SIZE;
-    a.items = static_cast<uint32_t>(items);
-    expert_weights_kernel<P><<<a.items, P::kThreads, 0, stream>>>(a);
+    if (items * P::kThreads >= kMostThreads) return PENC_ERR_BAD_LAYER_SIZE;
+    // (pieces take different times: all dies work on the same ones)
+    a.spread = Spread(items, plan.tiles / 8);
+    expert_weights_kernel<P><<<a.spread.grid(), P::kThreads, 0, stream>>>(a);
     return launched();
 }
 
 template <bool kDirect>
 int weights_of_experts(const WeightArgs& a, const WeightPlan& plan, hipStream_t stream) {
-    if (plan.small) return launch_weights<Product<Value, true, true, 64, 64, 2, 2, kDirect>>(a, plan, stream);
+    if (plan.side == 64) return launch_weights<Product<Value, true, true, 64, 64, 2, 2, kDirect>>(a, plan, stream);
+    if constexpr (kSize == 2) {
+        if (plan.side == 256) return launch_weights<Product<Value, true, true, 256, 256, 2, 4, kDirect>>(a, plan, stream);
+    }
     return launch_weights<Product<Value, true, true, 128, 128, 2, 2, kDirect>>(a, plan, stream);
 }
 
@@ -255,8 +275,8 @@ template <>
 int expert_rows<PENC_TYPE>(bool back, int64_t rows, int experts, int64_t wide, int64_t deep, const void* in, int64_t stride, const void* weight, const void* bias,
                            const int32_t* offsets, void* out, hipStream_t stream) {
     if (rows == 0) return PENC_OK;
-    RowsArgs a{in, weight, bias, out, stride, offsets, experts, static_cast<int>(rows), static_cast<int>(wide), static_cast<int>(deep), 0, 0,
-               aligned_to(out, 4 * kSize) && wide % 4 == 0};
+    RowsArgs a{in, weight, bias, out, stride, offsets, experts, static_cast<int>(rows), static_cast<int>(wide), static_cast<int>(deep), {}, 0,
+               aligned_to(out, 16) && wide * kSize % 16 == 0};
     const bool direct = chunked(in, stride, deep) && chunked(weight, back ? wide : deep, back ? wide : deep);
     if (back) return direct ? rows_of_experts<true, true>(a, stream) : rows_of_experts<true, false>(a, stream);
     return direct ? rows_of_experts<false, true>(a, stream) : rows_of_experts<false, false>(a, stream);
@@ -274,7 +294,7 @@ int expert_weights<PENC_TYPE>(int64_t rows, int experts, int64_t channels, int64
                               const int32_t* offsets, void* weight, void* bias, void* workspace, hipStream_t stream) {
     const WeightPlan plan = weight_plan(rows, experts, channels, outputs);
     WeightArgs a{x, grad, x_stride, grad_stride, offsets, experts, static_cast<int>(rows), static_cast<int>(channels), static_cast<int>(outputs),
-                 static_cast<int>(plan.most), 0, 0, 0, weight, bias, static_cast<float*>(workspace), plan.pieces, aligned_to(weight, 4 * kSize) && channels % 4 == 0};
+                 static_cast<int>(plan.most), {}, 0, 0, weight, bias, static_cast<float*>(workspace), plan.pieces, aligned_to(weight, 16) && channels * kSize % 16 == 0};
     const bool direct = chunked(x, x_stride, channels) && chunked(grad, grad_stride, outputs);
     if (const int rc = direct ? weights_of_experts<true>(a, plan, stream) : weights_of_experts<false>(a, plan, stream)) return rc;
     if (rows <= plan.most) return PENC_OK;

@@ -131,7 +131,8 @@ struct StepArgs {
     char* out;
     void* result;           // of the last step: [matrices][rows][columns]
     int rows, columns, padded, small, small_padded;
-    uint32_t items, each, tiles_m;  // each: of a matrix
+    Spread spread;
+    uint32_t each, tiles_m;  // each: items of a matrix
     float a, b, c;
 };
 
@@ -147,22 +148,22 @@ template <Stage kStage, bool kTall, class E, class Result, class P>
 __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
     constexpr int kBytes = ProductType<E>::kBytes;
-    const uint32_t item = item_of(a.items), t = item % a.each;
+    const uint32_t item = a.spread.item(), t = item % a.each;
+    if (item >= a.spread.items) return;
     const int64_t matrix = item / a.each;
     const int64_t stride = static_cast<int64_t>(a.padded) * kBytes, small_stride = static_cast<int64_t>(a.small_padded) * kBytes;
     const char *const x = a.x + matrix * a.rows * stride, *const s = a.s + matrix * a.small * small_stride, *const f = a.f + matrix * a.small * small_stride;
     uint32_t i = t % a.tiles_m, j = t / a.tiles_m;
     if constexpr (kStage != kUpdate) pair_of(t, i, j);
-    const int m0 = static_cast<int>(i) * P::kM, n0 = static_cast<int>(j) * P::kN;
+    const int m0 = uniform(static_cast<int>(i)) * P::kM, n0 = uniform(static_cast<int>(j)) * P::kN;
     const auto rows_from = [&](const char* p, int64_t row_bytes, int rows, int first, int most) { return Operand{p + first * row_bytes, row_bytes, min(rows - first, most), static_cast<int>(row_bytes)}; };
     const auto columns_from = [&](int first, int most) { return Operand{x + first * kBytes, stride, a.rows, min(a.padded - first, most) * kBytes}; };
     P p;
-    const auto nothing = [](const char*, int) {};
-    if constexpr (kStage == kGram && !kTall) p.run(lds, rows_from(x, stride, a.rows, m0, P::kM), rows_from(x, stride, a.rows, n0, P::kN), a.padded, nothing);
-    else if constexpr (kStage == kGram) p.run(lds, columns_from(m0, P::kM), columns_from(n0, P::kN), a.rows, nothing);
-    else if constexpr (kStage == kSquare) p.run(lds, rows_from(s, small_stride, a.small, m0, P::kM), rows_from(s, small_stride, a.small, n0, P::kN), a.small_padded, nothing);
-    else if constexpr (!kTall) p.run(lds, columns_from(m0, P::kM), rows_from(f, small_stride, a.small, n0, P::kN), a.small, nothing);
-    else p.run(lds, rows_from(f, small_stride, a.small, m0, P::kM), rows_from(x, stride, a.rows, n0, P::kN), a.padded, nothing);
+    if constexpr (kStage == kGram && !kTall) p.run(lds, rows_from(x, stride, a.rows, m0, P::kM), rows_from(x, stride, a.rows, n0, P::kN), a.padded, P::kZero, P::kNothing);
+    else if constexpr (kStage == kGram) p.run(lds, columns_from(m0, P::kM), columns_from(n0, P::kN), a.rows, P::kZero, P::kNothing);
+    else if constexpr (kStage == kSquare) p.run(lds, rows_from(s, small_stride, a.small, m0, P::kM), rows_from(s, small_stride, a.small, n0, P::kN), a.small_padded, P::kZero, P::kNothing);
+    else if constexpr (!kTall) p.run(lds, columns_from(m0, P::kM), rows_from(f, small_stride, a.small, n0, P::kN), a.small, P::kZero, P::kNothing);
+    else p.run(lds, rows_from(f, small_stride, a.small, m0, P::kM), rows_from(x, stride, a.rows, n0, P::kN), a.padded, P::kZero, P::kNothing);
     if constexpr (kStage != kUpdate) {
         char* const out = a.out + matrix * a.small * small_stride;
         p.each([&](int m, int n, tile_acc v) {
@@ -204,12 +205,12 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
 constexpr int kResidentThreads = 512, kResidentWaves = kResidentThreads / 64;
 constexpr int kMostSmall = 128;
 
-// A matrix of Split numbers in the LDS, rows of an odd number of 128 bytes; chunks of a row's 128 bytes are permuted as those of an operand's tile.
+// A matrix of Split numbers in the LDS.  Chunks of a row's 128 bytes are permuted by the row, so that neither 8 rows of one chunk nor 4 rows of two chunks meet in a bank.
 struct Resident {
     char* first;
     int pitch;
 
-    __device__ __forceinline__ char* chunk(int row, int byte) const { return first + row * pitch + (byte & ~127) + ((byte >> 4 & 7) ^ (row >> 1 & 7)) * 16 + (byte & 15); }
+    __device__ __forceinline__ char* chunk(int row, int byte) const { return first + row * pitch + (byte & ~127) + ((byte >> 4 & 7) ^ ((row & 3) << 1 | (row >> 2 & 1))) * 16 + (byte & 15); }
     // 16 rows from `row` on, 32 k from 32 `line` on
     __device__ __forceinline__ chunk16 across(int row, int line, int q) const {
         const int lane = threadIdx.x % 64;
@@ -254,7 +255,7 @@ __device__ __forceinline__ tile_acc multiply_split(chunk16 a, chunk16 a_low, chu
     return multiply<half_t>(a, b, c);
 }
 
-__host__ __device__ constexpr int resident_pitch(int padded) { return (padded / 32 | 1) * 128; }
+__host__ __device__ constexpr int resident_pitch(int padded) { return padded * 4; }
 __host__ __device__ constexpr int round_to_32(int n) { return (n + 31) / 32 * 32; }
 
 // One matrix to a workgroup, X as `small` rows of `large` numbers whichever way it lies in memory.  A wave has 16 x 32 results of S and of F, and 16 columns of X, which it
@@ -425,14 +426,18 @@ int launch_step(StepArgs a, int64_t matrices, hipStream_t stream) {
             each = static_cast<int64_t>(a.tiles_m) * ((a.rows + P::kN - 1) / P::kN);
         }
         const int64_t items = each * matrices;
-        if (items * P::kThreads >= int64_t{1} << 32) return PENC_ERR_BAD_LAYER_SIZE;
-        a.each = static_cast<uint32_t>(each), a.items = static_cast<uint32_t>(items);
-        step_kernel<kStage, kTall, E, Result, P><<<a.items, P::kThreads, 0, stream>>>(a);
+        if (items * P::kThreads >= (int64_t{1} << 32) - (1 << 18)) return PENC_ERR_BAD_LAYER_SIZE;
+        a.each = static_cast<uint32_t>(each), a.spread = Spread(items, 32);
+        step_kernel<kStage, kTall, E, Result, P><<<a.spread.grid(), P::kThreads, 0, stream>>>(a);
         return launched();
     };
     // tiles of 64 x 64 where there would not be a workgroup of 128 x 128 for each compute unit
     const int64_t side_m = kStage == kUpdate ? a.columns : a.small, side_n = kStage == kUpdate ? a.rows : a.small;
     const int64_t large = matrices * ((side_m + 127) / 128) * ((side_n + 127) / 128) / (kStage == kUpdate ? 1 : 2);
+    const int64_t huge = matrices * ((side_m + 255) / 256) * ((side_n + 255) / 256) / (kStage == kUpdate ? 1 : 2);
+    if constexpr (std::is_same_v<E, half_t>) {
+        if (huge >= 128) return launch(std::common_type<Product<E, kAlongM, kAlongN, 256, 256, 4, 2, true>>{});
+    }
     if (large < 256) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, true>>{});
     return launch(std::common_type<Product<E, kAlongM, kAlongN, 128, 128, 2, 2, true>>{});
 }
@@ -451,7 +456,7 @@ int orthogonalise(int64_t matrices, int64_t rows, int64_t columns, int steps, Co
     if (const int rc = launched()) return rc;
     for (int step = 0; step < steps; ++step) {
         StepArgs a{x, s, f, s, nullptr, static_cast<int>(rows), static_cast<int>(columns), static_cast<int>(l.padded), static_cast<int>(l.small),
-                   static_cast<int>(l.small_padded), 0, 0, 0, k.a, k.b, k.c};
+                   static_cast<int>(l.small_padded), {}, 0, 0, k.a, k.b, k.c};
         const auto all = [&](auto tall) -> int {
             constexpr bool kTall = decltype(tall)::value;
             if (const int rc = launch_step<kGram, kTall, E, G>(a, matrices, stream)) return rc;

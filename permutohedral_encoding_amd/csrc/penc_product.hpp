@@ -1,26 +1,29 @@
 // Matrix products of a workgroup: D[m][n] = sum over k of A[m][k] B[n][k], for a tile of kM x kN results that stay in the registers of its waves.
 //
-// Operands come in steps of k through the LDS, one step on its way while the one before is multiplied.  An operand is
+// Operands come in steps of k through the LDS, up to three steps on their way while one is multiplied, and its fragments are read from the LDS while the one before is.
+// An operand is
 //
-//     Across   rows of adjacent k: 128 bytes of each row in a step, 64 k of a 16-bit type and 32 of fp32
+//     Across   rows of adjacent k: 64 bytes of each row in a step, 32 k of a 16-bit type and 16 of fp32
 //     Along    rows of one k, adjacent in m (or n): as many k in a step, transposed on the way from the LDS into registers
 //
 // 16-bit types are multiplied by v_mfma_f32_16x16x32, fp32 by v_mfma_f32_16x16x4_f32.  A Split number is two halves, hi = the nearest to x and lo = the nearest to x - hi
-// (22 bits of x together, where x - hi is no less than 2^-14): of every 32 numbers the hi and behind them the lo, so that a row has 4 bytes for each; a product is
+// (22 bits of x together, where x - hi is no less than 2^-14): of every 32 numbers the hi and behind them the lo, 128 bytes in a step; a product is
 // hi hi + hi lo + lo hi, and what is left out is 2^-22 of it.
 //
-// Chunks of 16 bytes go from memory into the LDS directly, where rows and their ends are on 16 bytes, each lane its own: where a chunk stands in the LDS is fixed by the lane that brings it, so
+// Chunks of 16 bytes go from memory into the LDS directly, where rows and their ends are on 16 bytes.  Where a chunk stands in the LDS is fixed by the lane that brings it, so
 // a lane brings the chunk that belongs there.  Addresses behind an operand's end (rows, k, or columns) read zeros, which the buffer's bounds see to.  Of operands that
 // begin anywhere, lanes load what is there into registers and write it into the LDS.
 //
-// Where a chunk stands: fragments are read by 16 lanes at a time, which should meet 64 banks of 4 bytes each once.  Across: lanes read one chunk c of 16 rows of 128 bytes; c
-// stands at c ^ (row / 2 mod 8).  Along: 16 lanes read 32 bytes (fp32: 64) of 4 neighbouring k, and 16 more those of the k 8 (fp32: 4) behind; pieces of 32 (64)
-// bytes are permuted by these bits of k.
+// Where a chunk stands: a read of 16 bytes takes 8 lanes at a time, one of 8 bytes 16 and one of 4 bytes 32, which should meet the 32 banks of 4 bytes once.  Across: lanes read one chunk c
+// of 8 rows; c stands at c ^ (row / 2 mod 4) (of 128 bytes: row mod 8).  Along: 16 lanes read 32 bytes (fp32: 64) of each of 4 neighbouring k (fp32: 32 lanes of two k, 4 apart);
+// pieces of 32 (64) bytes are permuted by these bits of k.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "penc_kept.hpp"
 
@@ -32,18 +35,21 @@ struct split_t {
 
 template <class E>
 struct ProductType {
-    static constexpr int kBytes = 2;  // of a number
-    static constexpr int kDepth = 64; // k of a step
+    static constexpr int kBytes = 2;   // of a number
+    static constexpr int kDepth = 32;  // k of a step
+    static constexpr int kParts = 1;   // fragments of 16 rows of a step
 };
 template <>
 struct ProductType<float> {
     static constexpr int kBytes = 4;
-    static constexpr int kDepth = 32;
+    static constexpr int kDepth = 16;
+    static constexpr int kParts = 1;
 };
 template <>
 struct ProductType<split_t> {
     static constexpr int kBytes = 4;
     static constexpr int kDepth = 32;
+    static constexpr int kParts = 2;
 };
 
 using tile_acc = float __attribute__((ext_vector_type(4)));
@@ -78,44 +84,43 @@ constexpr int kMostOperandStride = 1 << 24;  // bytes: 256 rows are within a buf
 template <class E, bool kAlong, int kWide>
 struct OperandTile {
     using T = ProductType<E>;
-    static constexpr int kRowBytes = kAlong ? kWide * T::kBytes : 128;
+    static constexpr int kLine = T::kDepth * T::kBytes;
+    static constexpr int kRowBytes = kAlong ? kWide * T::kBytes : kLine;
     static constexpr int kRows = kAlong ? T::kDepth : kWide;
     static constexpr int kSize = kRows * kRowBytes;
     static constexpr int kChunks = kSize / 16, kRowChunks = kRowBytes / 16;
 
     // where chunk c of a row stands in it
     __device__ __forceinline__ static int place(int row, int c) {
-        if constexpr (!kAlong) return c ^ (row >> 1 & 7);
+        if constexpr (!kAlong) return kLine == 64 ? c ^ (row >> 1 & 3) : c ^ (row & 7);
         else if constexpr (std::is_same_v<E, float>) return c ^ (row >> 2 & 3) << 2;
         else if constexpr (kRowBytes >= 256) return c ^ ((row & 3) | (row >> 3 & 1) << 2) << 1;
         else return c ^ ((row >> 1 & 1) | (row >> 3 & 1) << 1) << 1;
     }
 
-    // 16 rows (columns) from `at` on, as the matrix instruction takes them: lane 16 g + i has row i; half q of a step (Split: hi or lo).
-    __device__ __forceinline__ static chunk16 fragment(const char* lds, int at, int q) {
+    // 16 rows (columns) from `at` on, as the matrix instruction takes them: lane 16 g + i has row i.  Split: hi (part 0) or lo.
+    __device__ __forceinline__ static chunk16 fragment(const char* lds, int at, int part) {
         const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
         if constexpr (!kAlong) {
             const int row = at + i;
-            return *reinterpret_cast<const chunk16*>(lds + row * 128 + place(row, q * 4 + g) * 16);
+            return *reinterpret_cast<const chunk16*>(lds + row * kLine + place(row, part * 4 + g) * 16);
         } else if constexpr (std::is_same_v<E, float>) {
             chunk16 f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int row = q * 16 + g * 4 + j, column = at + i;
+                const int row = g * 4 + j, column = at + i;
                 f[j] = *reinterpret_cast<const uint32_t*>(lds + row * kRowBytes + place(row, column / 4) * 16 + column % 4 * 4);
             }
             return f;
         } else {
-            constexpr bool kSplit = std::is_same_v<E, split_t>;
-            const int byte = (kSplit ? at / 32 * 128 + at % 32 * 2 + q * 64 : at * 2) + i % 4 * 8;
+            const int byte = (std::is_same_v<E, split_t> ? at / 32 * 128 + at % 32 * 2 + part * 64 : at * 2) + i % 4 * 8;
             using V = short __attribute__((ext_vector_type(4)));
             using Lds = __attribute__((address_space(3))) V;
             chunk16 f;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int row = (kSplit ? 0 : q * 32) + g * 8 + h * 4 + i / 4;
-                const char* const p = lds + row * kRowBytes + place(row, byte / 16) * 16 + byte % 16;
-                const V v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p));
+                const int row = g * 8 + h * 4 + i / 4;
+                const V v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(lds + row * kRowBytes + place(row, byte / 16) * 16 + byte % 16));
                 const uint2 w = __builtin_bit_cast(uint2, v);
                 f[2 * h] = w.x, f[2 * h + 1] = w.y;
             }
@@ -124,67 +129,88 @@ struct OperandTile {
     }
 };
 
-// Brings an operand's steps into the LDS.
+// 16 bytes to each lane from buffer + at, to the LDS from `to` on, lane after lane.  (Not the builtin: of that the compiler knows that it writes to the LDS, but not where, and has every
+// read of the LDS wait for it.  It has no result: what it brings is waited for by wait_for_loads.  The wait states are those that a scalar register written by a vector
+// instruction needs before it is an address, and M0 before it is used.)
+__device__ __forceinline__ void load_to_lds(__attribute__((ext_vector_type(4))) uint32_t buffer, int at, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(to), "v"(at), "s"(buffer) : "memory");
+}
+
+// What is the same in all lanes, in a scalar register (the compiler does not see it of all that is computed from a division).
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    const uint32_t low = static_cast<uint32_t>(uniform(static_cast<int>(x)));
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(x >> 32)))) << 32 | low);
+}
+
+// Brings an operand's steps into the LDS, one after the other.
 template <class E, bool kAlong, int kWide, int kThreads, bool kDirect>
 struct Loader {
     using Tile = OperandTile<E, kAlong, kWide>;
     using T = ProductType<E>;
     static constexpr int kEach = Tile::kChunks / kThreads;
-    static_assert(Tile::kChunks % kThreads == 0);
+    static_assert(Tile::kChunks % kThreads == 0 && kThreads % 128 == 0);
 
-    Operand o;
-    int row[kEach], byte[kEach];  // of the chunks that this lane brings
+    const char* first;  // of the next step
+    int64_t step_bytes;
+    int left;           // Across: bytes of a row, Along: rows
+    int stride, rest;   // rest: what the buffer has beside: Across: the rows before the last, Along: how much longer a row is than they are apart
+    int rows;
+    int at[kEach];      // of this lane's chunks from `first` on
+    int byte;           // Across: in a row
     chunk16 held[kDirect ? 1 : kEach];
 
-    __device__ __forceinline__ explicit Loader(const Operand& operand) : o(operand) {
+    __device__ __forceinline__ explicit Loader(const Operand& o)
+        : first(reinterpret_cast<const char*>(uniform(reinterpret_cast<int64_t>(o.first)))), step_bytes(kAlong ? T::kDepth * uniform(o.stride) : Tile::kLine),
+          left(uniform(kAlong ? o.rows : o.bytes)), stride(uniform(static_cast<int>(o.stride))), rest(kAlong ? uniform(o.bytes) - stride : uniform(o.rows - 1) * stride),
+          rows(o.rows) {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            const int slot = j * kThreads + static_cast<int>(threadIdx.x);
-            row[j] = slot / Tile::kRowChunks;
-            byte[j] = Tile::place(row[j], slot % Tile::kRowChunks) * 16;
+            const int slot = j * kThreads + static_cast<int>(threadIdx.x), row = slot / Tile::kRowChunks;
+            const int in_row = Tile::place(row, slot % Tile::kRowChunks) * 16;
+            at[j] = row * stride + in_row;
+            if (!kAlong) byte = in_row;  // (the same for all of them: kThreads / kRowChunks rows are a whole number of permutations)
+            if (kAlong && in_row >= o.bytes) at[j] = -1;
         }
     }
 
-    // The chunks of a step are on their way, into the LDS or into registers.
-    __device__ __forceinline__ void begin(char* lds, int step) {
-        // (rows, bytes of a row, and the first of them that this step has)
-        const int64_t past = kAlong ? static_cast<int64_t>(step) * T::kDepth * o.stride : static_cast<int64_t>(step) * 128;
-        const char* const first = o.first + past;
-        const int rows = kAlong ? o.rows - step * T::kDepth : o.rows, bytes = kAlong ? o.bytes : o.bytes - step * 128;
+    // The chunks of the next step are on their way, into the LDS or into registers.
+    __device__ __forceinline__ void begin(uint32_t lds) {
         if constexpr (kDirect) {
-            const int64_t there = rows > 0 && bytes > 0 ? (rows - 1) * o.stride + bytes : 0;
-            const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(first), 0, static_cast<int>(there < 0x7FFFFFFF ? there : 0x7FFFFFFF), 0x00020000);
-            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+            const int there = left <= 0 ? 0 : kAlong ? min(left, T::kDepth) * stride + rest : rest + left;
+            const uint64_t p = reinterpret_cast<uint64_t>(first);
+            const __attribute__((ext_vector_type(4))) uint32_t buffer = {static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xFFFFu, static_cast<uint32_t>(there), 0x00020000u};
+            const uint32_t to = lds + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * 1024;
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) {
-                const int at = byte[j] < bytes ? row[j] * static_cast<int>(o.stride) + byte[j] : -1;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (__attribute__((address_space(3))) void*)(lds + (j * kThreads + wave * 64) * 16), 16, at, 0, 0, 0);
-            }
+            for (int j = 0; j < kEach; ++j) load_to_lds(buffer, kAlong || byte < left ? at[j] : -1, to + j * kThreads * 16);
         } else {
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
-                const char* const p = first + row[j] * o.stride + byte[j];
-                const int left = row[j] < rows ? bytes - byte[j] : 0;
+                const int slot = j * kThreads + static_cast<int>(threadIdx.x), row = slot / Tile::kRowChunks;
+                const int in_row = Tile::place(row, slot % Tile::kRowChunks) * 16, n = kAlong ? (row < left ? rest + stride - in_row : 0) : (row < rows ? left - in_row : 0);
+                const char* const p = first + static_cast<int64_t>(row) * stride + in_row;
                 chunk16 v{};
-                if (left >= 16) {
+                if (n >= 16) {
                     using Unaligned = uint32_t __attribute__((ext_vector_type(4), aligned(T::kBytes == 2 ? 2 : 4)));
                     v = *reinterpret_cast<const Unaligned*>(p);
-                } else if (left > 0) {
+                } else if (n > 0) {
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         if constexpr (T::kBytes == 4) {
-                            if (4 * w < left) v[w] = *reinterpret_cast<const uint32_t*>(p + 4 * w);
+                            if (4 * w < n) v[w] = *reinterpret_cast<const uint32_t*>(p + 4 * w);
                         } else {
-                            if (4 * w < left) v[w] = *reinterpret_cast<const uint16_t*>(p + 4 * w);
-                            if (4 * w + 2 < left) v[w] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + 4 * w + 2)) << 16;
+                            if (4 * w < n) v[w] = *reinterpret_cast<const uint16_t*>(p + 4 * w);
+                            if (4 * w + 2 < n) v[w] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + 4 * w + 2)) << 16;
                         }
                     }
                 }
                 held[j] = v;
             }
         }
+        first += step_bytes;
+        left -= kAlong ? T::kDepth : Tile::kLine;
     }
-    // What was on its way is in the LDS (of this wave; a barrier makes it so for the others).
+    // What is held goes into the LDS (a barrier makes it so for the other waves).
     __device__ __forceinline__ void end(char* lds) {
         if constexpr (!kDirect) {
 #pragma unroll
@@ -193,16 +219,52 @@ struct Loader {
     }
 };
 
-// A workgroup of kWavesM x kWavesN waves, each with kM / kWavesM x kN / kWavesN results.
-template <class E, bool kAlongM, bool kAlongN, int kM_, int kN_, int kWavesM, int kWavesN, bool kDirect>
+// Until all but kLoads of this wave's loads have come (they come in order), and it has read what it asked the LDS for.
+template <int kLoads>
+__device__ __forceinline__ void wait_for_loads() {
+    static_assert(kLoads < 64);
+    __builtin_amdgcn_s_waitcnt((kLoads & 15) | 7 << 4 | (kLoads >> 4) << 14);
+}
+
+// A workgroup of kWavesM x kWavesN waves, each with kM / kWavesM x kN / kWavesN results; kRing steps have room in the LDS.
+template <class E, bool kAlongM, bool kAlongN, int kM_, int kN_, int kWavesM, int kWavesN, bool kDirect, int kRing = 4>
 struct Product {
     static constexpr int kM = kM_, kN = kN_, kThreads = 64 * kWavesM * kWavesN;
     static constexpr int kTilesM = kM / kWavesM / 16, kTilesN = kN / kWavesN / 16;
     using TileM = OperandTile<E, kAlongM, kM>;
     using TileN = OperandTile<E, kAlongN, kN>;
+    using LoadM = Loader<E, kAlongM, kM, kThreads, kDirect>;
+    using LoadN = Loader<E, kAlongN, kN, kThreads, kDirect>;
     static constexpr int kStage = TileM::kSize + TileN::kSize;
-    static constexpr int kLds = 2 * kStage;
-    static constexpr int kDepth = ProductType<E>::kDepth;
+    static constexpr int kLds = kRing * kStage;
+    static constexpr int kDepth = ProductType<E>::kDepth, kParts = ProductType<E>::kParts;
+    static constexpr int kLoads = LoadM::kEach + LoadN::kEach;  // of a lane, for a step
+
+    // What a wave multiplies in a step.
+    struct Fragments {
+        chunk16 m[kParts][kTilesM], n[kParts][kTilesN];
+
+        __device__ __forceinline__ void read(const char* lds) {
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+#pragma unroll
+                for (int j = 0; j < kTilesN; ++j) n[p][j] = TileN::fragment(lds + TileM::kSize, wave_n() + 16 * j, p);
+#pragma unroll
+                for (int i = 0; i < kTilesM; ++i) m[p][i] = TileM::fragment(lds, wave_m() + 16 * i, p);
+            }
+        }
+    };
+
+    // Reads of the LDS of a step, and products.
+    template <bool kAlong>
+    static constexpr int kReadsOf = !kAlong ? 1 : std::is_same_v<E, float> ? 4 : 2;
+    static constexpr int kReads = kParts * (kTilesM * kReadsOf<kAlongM> + kTilesN * kReadsOf<kAlongN>);
+    static constexpr int kProducts = kTilesM * kTilesN * (kParts == 2 ? 3 : std::is_same_v<E, float> ? 4 : 1);
+    // A wave issues in order: reads of the LDS, which all waves begin at the same time, are spread over the products, which go on meanwhile.
+    template <size_t... kRead>
+    __device__ __forceinline__ static void alternate(std::index_sequence<kRead...>) {
+        ((__builtin_amdgcn_sched_group_barrier(0x008, (kRead + 1) * kProducts / kReads - kRead * kProducts / kReads, 0), __builtin_amdgcn_sched_group_barrier(0x100, 1, 0)), ...);
+    }
 
     tile_acc acc[kTilesM][kTilesN];
 
@@ -210,73 +272,103 @@ struct Product {
     __device__ __forceinline__ static int wave_m() { return wave() / kWavesN * (kM / kWavesM); }
     __device__ __forceinline__ static int wave_n() { return wave() % kWavesN * (kN / kWavesN); }
 
-    __device__ __forceinline__ void multiply_step(const char* lds) {
-        const char *const m = lds, *const n = lds + TileM::kSize;
-        if constexpr (std::is_same_v<E, split_t>) {
-            chunk16 a[kTilesM], b[kTilesN], low[kTilesN];
-#pragma unroll
-            for (int i = 0; i < kTilesM; ++i) a[i] = TileM::fragment(m, wave_m() + 16 * i, 0);
-#pragma unroll
-            for (int j = 0; j < kTilesN; ++j) b[j] = TileN::fragment(n, wave_n() + 16 * j, 0);
-#pragma unroll
-            for (int j = 0; j < kTilesN; ++j) low[j] = TileN::fragment(n, wave_n() + 16 * j, 1);
-#pragma unroll
-            for (int i = 0; i < kTilesM; ++i)
-#pragma unroll
-                for (int j = 0; j < kTilesN; ++j) acc[i][j] = multiply<half_t>(a[i], low[j], acc[i][j]);
-#pragma unroll
-            for (int i = 0; i < kTilesM; ++i) {
-                const chunk16 a_low = TileM::fragment(m, wave_m() + 16 * i, 1);
-#pragma unroll
-                for (int j = 0; j < kTilesN; ++j) acc[i][j] = multiply<half_t>(a_low, b[j], acc[i][j]);
-            }
-#pragma unroll
-            for (int i = 0; i < kTilesM; ++i)
-#pragma unroll
-                for (int j = 0; j < kTilesN; ++j) acc[i][j] = multiply<half_t>(a[i], b[j], acc[i][j]);
-        } else {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                chunk16 a[kTilesM], b[kTilesN];
-#pragma unroll
-                for (int i = 0; i < kTilesM; ++i) a[i] = TileM::fragment(m, wave_m() + 16 * i, q);
-#pragma unroll
-                for (int j = 0; j < kTilesN; ++j) b[j] = TileN::fragment(n, wave_n() + 16 * j, q);
-#pragma unroll
-                for (int i = 0; i < kTilesM; ++i)
-#pragma unroll
-                    for (int j = 0; j < kTilesN; ++j) acc[i][j] = multiply<E>(a[i], b[j], acc[i][j]);
-            }
-        }
-    }
-
-    // `also(lds, step)` may look at each step while it is there.
-    template <class F>
-    __device__ __forceinline__ void run(char* lds, const Operand& m, const Operand& n, int depth, F&& also) {
+    __device__ __forceinline__ void multiply_all(const chunk16 (&m)[kTilesM], const chunk16 (&n)[kTilesN]) {
+        using Part = std::conditional_t<std::is_same_v<E, split_t>, half_t, E>;
 #pragma unroll
         for (int i = 0; i < kTilesM; ++i)
 #pragma unroll
-            for (int j = 0; j < kTilesN; ++j) acc[i][j] = tile_acc{};
-        const int steps = (depth + kDepth - 1) / kDepth;
-        if (steps == 0) return;
-        Loader<E, kAlongM, kM, kThreads, kDirect> load_m(m);
-        Loader<E, kAlongN, kN, kThreads, kDirect> load_n(n);
-        load_m.begin(lds, 0);
-        load_n.begin(lds + TileM::kSize, 0);
-        for (int step = 0; step < steps; ++step) {
-            char* const here = lds + (step & 1) * kStage;
-            char* const next = lds + ((step & 1) ^ 1) * kStage;
-            load_m.end(here);
-            load_n.end(here + TileM::kSize);
-            if constexpr (kDirect) __builtin_amdgcn_s_waitcnt(0x0F70);  // (what this wave's loads bring is there)
-            __syncthreads();  // so it is for all of them, and none still reads the other half
-            if (step + 1 < steps) {
-                load_m.begin(next, step + 1);
-                load_n.begin(next + TileM::kSize, step + 1);
-            }
-            multiply_step(here);
-            also(here, step);
+            for (int j = 0; j < kTilesN; ++j) acc[i][j] = multiply<Part>(m[i], n[j], acc[i][j]);
+    }
+    __device__ __forceinline__ void multiply_step(const Fragments& f) {
+        if constexpr (kParts == 2) {
+            multiply_all(f.m[0], f.n[1]);
+            multiply_all(f.m[1], f.n[0]);
         }
+        multiply_all(f.m[0], f.n[0]);
+    }
+
+    // Where the sums begin: f(m), for the four results from m on, of every n.
+    template <class F>
+    __device__ __forceinline__ void start(F&& f) {
+#pragma unroll
+        for (int i = 0; i < kTilesM; ++i) {
+            const tile_acc v = f(wave_m() + 16 * i + static_cast<int>(threadIdx.x) % 64 / 16 * 4);
+#pragma unroll
+            for (int j = 0; j < kTilesN; ++j) acc[i][j] = v;
+        }
+    }
+    static constexpr auto kZero = [](int) { return tile_acc{}; };
+    static constexpr auto kNothing = [](const auto&) {};
+
+    // The sums begin at first(m).  `also(n)` may look at the fragments of N of each step.
+    template <class First, class F>
+    __device__ __forceinline__ void run(char* lds, const Operand& m, const Operand& n, int depth, First&& first, F&& also) {
+        const int steps = (depth + kDepth - 1) / kDepth;
+        if (steps == 0) return start(first);
+        LoadM load_m(m);
+        LoadN load_n(n);
+        // Steps behind the last one are loaded too, and are zeros: each wave always has as many loads on their way.
+        constexpr int kAhead = kRing - 1;
+        const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+        int room = 0, read = 0;  // where the next step goes, and where the next fragments are
+        const auto begin = [&] {
+            load_m.begin(lds_at + room);
+            load_n.begin(lds_at + room + TileM::kSize);
+            if constexpr (kDirect) room = room + kStage == kLds ? 0 : room + kStage;
+        };
+        const auto end = [&] {
+            load_m.end(lds + room);
+            load_n.end(lds + room + TileM::kSize);
+            if constexpr (!kDirect) room = room + kStage == kLds ? 0 : room + kStage;
+        };
+        const auto fragments = [&](Fragments& f) {
+            f.read(lds + read);
+            read = read + kStage == kLds ? 0 : read + kStage;
+        };
+        const auto meet = [&] {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        };
+        if constexpr (kDirect) {
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) begin();
+            start(first);
+            wait_for_loads<kLoads * (kAhead - 1)>();
+        } else {
+            start(first);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                begin();
+                if (k + 1 < kAhead) end();
+            }
+        }
+        meet();
+        Fragments even, odd;
+        fragments(even);
+        // In step i: what is brought for step i + 1 is there for all waves, and the fragments of step i - 1, whose room step i + kAhead takes, have been read.
+        const auto turn = [&](const Fragments& now, Fragments& next) {
+            if constexpr (kDirect) wait_for_loads<kLoads * (kAhead - 2)>();
+            meet();
+            if constexpr (!kDirect) end();
+            begin();
+            __builtin_amdgcn_sched_barrier(0);
+            fragments(next);
+            multiply_step(now);
+            also(now.n[0]);
+            alternate(std::make_index_sequence<kReads>{});
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        int i = 0;
+        for (; i + 1 < steps; i += 2) {
+            turn(even, odd);
+            turn(odd, even);
+        }
+        if (i < steps) {
+            multiply_step(even);
+            also(even.n[0]);
+        }
+        if constexpr (kDirect) wait_for_loads<0>();  // (nothing is on its way into the LDS when the workgroup ends)
     }
 
     // Calls f(m, n, v) for the results of this lane: v of m .. m + 3 and n, within the tile.
@@ -304,11 +396,46 @@ __device__ __forceinline__ void store_four(E* p, tile_acc v, int valid, bool ali
     }
 }
 
-// The work of a workgroup of `items`.  Consecutive workgroups go to the 8 dies in turn: each die gets neighbouring items, whose operands its cache then holds.
-__device__ __forceinline__ uint32_t item_of(uint32_t items) {
-    constexpr uint32_t kDies = 8;
-    const uint32_t die = blockIdx.x % kDies, each = items / kDies, rest = items % kDies;
-    return die * each + min(die, rest) + blockIdx.x / kDies;
+// Stores a workgroup's results as rows of n, `stride` values apart: `rows` of them and `columns` of m, rounded once.  aligned: rows begin on 16 bytes.
+// 16-bit results: lanes 16 apart have four neighbouring m each, of one n; they exchange those of two tiles, and each stores eight of one of them.
+template <class E, class P>
+__device__ __forceinline__ void store_rows(const P& p, E* out, int64_t stride, int rows, int columns, bool aligned) {
+    if constexpr (sizeof(E) == 2 && P::kTilesM % 2 == 0) {
+        if (aligned) {
+            const int lane = threadIdx.x % 64, g = lane / 16;
+#pragma unroll
+            for (int j = 0; j < P::kTilesN; ++j) {
+                const int n = P::wave_n() + 16 * j + lane % 16;
+#pragma unroll
+                for (int i = 0; i < P::kTilesM; i += 2) {
+                    using Four = E __attribute__((ext_vector_type(4)));
+                    const uint2 a = __builtin_bit_cast(uint2, __builtin_convertvector(p.acc[i][j], Four)), b = __builtin_bit_cast(uint2, __builtin_convertvector(p.acc[i + 1][j], Four));
+                    const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+                    const int m = P::wave_m() + 16 * (i + g % 2) + g / 2 * 8;
+                    if (n < rows && m < columns) *reinterpret_cast<uint4*>(out + n * stride + m) = make_uint4(x[0], y[0], x[1], y[1]);
+                }
+            }
+            return;
+        }
+    }
+    p.each([&](int m, int n, tile_acc v) {
+        if (n < rows && m < columns) store_four(out + n * stride + m, v, columns - m, aligned);
+    });
 }
+
+// How items are spread over a launch.  Consecutive workgroups go to the 8 dies in turn; each die gets `run` neighbouring items at a time, whose operands its cache then holds,
+// and all of them go through the items alike: items take different times, and of some there is nothing to do.
+struct Spread {
+    uint32_t items, run;
+    static constexpr uint32_t kDies = 8;
+
+    Spread() = default;
+    Spread(int64_t n, int64_t most) : items(static_cast<uint32_t>(n)), run(static_cast<uint32_t>(std::max<int64_t>(1, std::min((n + kDies - 1) / kDies, most)))) {}
+    uint32_t grid() const { return (items + kDies * run - 1) / (kDies * run) * (kDies * run); }
+    __device__ __forceinline__ uint32_t item() const {
+        const uint32_t at = blockIdx.x / kDies;
+        return (at / run * kDies + blockIdx.x % kDies) * run + at % run;
+    }
+};
 
 }  // namespace penc
