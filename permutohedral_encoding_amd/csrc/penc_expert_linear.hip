@@ -81,7 +81,6 @@ struct RowsArgs {
     int experts, rows, wide, deep; // wide: values of a row of the result; deep: of the operand
     Spread spread;
     uint32_t tiles;                // of a row of the result
-    bool aligned;                  // whether rows of the result begin on 16 bytes
 };
 
 constexpr uint32_t kGroup = 8;
@@ -118,7 +117,7 @@ __global__ __launch_bounds__(P::kThreads) void expert_rows_kernel(RowsArgs a) {
         };
         p.run(lds, m, n, a.deep, first, P::kNothing);
     }
-    store_rows(p, static_cast<Value*>(a.rows_out) + static_cast<int64_t>(t.first) * a.wide + m0, a.wide, t.rows, columns, a.aligned);
+    store_rows(p, static_cast<Value*>(a.rows_out) + static_cast<int64_t>(t.first) * a.wide + m0, a.wide, t.rows, columns);
 }
 
 struct WeightArgs {
@@ -131,7 +130,6 @@ struct WeightArgs {
     void *weight, *bias;  // results, written where an expert's rows are one piece
     float* sums;          // [pieces][outputs][channels], and behind them [pieces][outputs]
     int64_t pieces;
-    bool aligned;
 };
 
 // dW and db of a piece of an expert's rows.
@@ -160,8 +158,8 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
     const int64_t n_weights = static_cast<int64_t>(a.outputs) * a.channels;
     const bool whole = t.tiles == 1;
     const int64_t at = static_cast<int64_t>(o0) * a.channels + c0;
-    if (whole) store_rows(p, static_cast<Value*>(a.weight) + t.expert * n_weights + at, a.channels, a.outputs - o0, a.channels - c0, a.aligned);
-    else store_rows(p, a.sums + piece * n_weights + at, a.channels, a.outputs - o0, a.channels - c0, a.channels % 4 == 0);
+    if (whole) store_rows(p, static_cast<Value*>(a.weight) + t.expert * n_weights + at, a.channels, a.outputs - o0, a.channels - c0);
+    else store_rows(p, a.sums + piece * n_weights + at, a.channels, a.outputs - o0, a.channels - c0);
     if (!bias) return;
     const int lane = threadIdx.x % 64;
 #pragma unroll
@@ -175,8 +173,11 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
 
 constexpr int kSumThreads = 256;
 
-// The sums of experts whose rows are several pieces, piece by piece.
+// The sums of experts whose rows are several pieces: kSlices lanes share a result's pieces, each taking every kSlices-th in order, and their sums are added in order.
+template <int kSlices>
 __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, uint32_t blocks) {
+    constexpr int kResults = kSumThreads / kSlices;
+    __shared__ float lds[kSlices][kResults];
     const int e = static_cast<int>(blockIdx.x / blocks);
     // the first of the expert's pieces, and how many there are
     uint32_t first = 0, mine = 0;
@@ -190,21 +191,37 @@ __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, 
     for (int d = 1; d < 64; d *= 2) first += __shfl_xor(first, d), mine = max(mine, static_cast<uint32_t>(__shfl_xor(mine, d)));
     if (mine <= 1) return;
     const int64_t weights = static_cast<int64_t>(a.outputs) * a.channels, n = weights + (a.bias != nullptr ? a.outputs : 0);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x % blocks) * kSumThreads + threadIdx.x; i < n; i += static_cast<int64_t>(blocks) * kSumThreads) {
-        const bool weight = i < weights;
+    const int slice = static_cast<int>(threadIdx.x) / kResults, result = static_cast<int>(threadIdx.x) % kResults;
+    for (int64_t begin = static_cast<int64_t>(blockIdx.x % blocks) * kResults; begin < n; begin += static_cast<int64_t>(blocks) * kResults) {
+        const int64_t i = begin + result;
+        const bool there = i < n, weight = i < weights;
         const int64_t each = weight ? weights : a.outputs, at = weight ? i : i - weights;
-        const float* const from = a.sums + (weight ? 0 : a.pieces * weights) + first * each + at;
         float sum = 0.0f;
-        for (uint32_t k = 0; k < mine; ++k) sum += from[k * each];
-        static_cast<Value*>(weight ? a.weight : a.bias)[e * each + at] = static_cast<Value>(sum);
+        if (there) {
+            const float* const from = a.sums + (weight ? 0 : a.pieces * weights) + first * each + at;
+#pragma unroll 4
+            for (uint32_t k = slice; k < mine; k += kSlices) sum += from[k * each];
+        }
+        if constexpr (kSlices > 1) {
+            lds[slice][result] = sum;
+            __syncthreads();
+            sum = lds[0][result];
+#pragma unroll
+            for (int k = 1; k < kSlices; ++k) sum += lds[k][result];
+            __syncthreads();
+        }
+        if (there && slice == 0) static_cast<Value*>(weight ? a.weight : a.bias)[e * each + at] = static_cast<Value>(sum);
     }
 }
 
 // ------------------------------------------------------------------------------------------
 // which kernel
 
-// Whether chunks of 16 bytes are on 16 bytes.
-bool chunked(const void* p, int64_t stride, int64_t bytes) { return aligned_to(p, 16) && stride * kSize % 16 == 0 && bytes * kSize % 16 == 0; }
+// How chunks of rows of `values` values, `stride` apart, come.
+Chunks chunks_of(const void* p, int64_t stride, int64_t values) {
+    if (aligned_to(p, 16) && stride * kSize % 16 == 0 && values * kSize % 16 == 0) return Chunks::kDirect;
+    return values * kSize >= 16 ? Chunks::kHeld : Chunks::kSingle;
+}
 
 // (a launch has less than 2^32 threads, and a spread rounds up)
 constexpr int64_t kMostThreads = (int64_t{1} << 32) - (1 << 18);
@@ -219,13 +236,24 @@ int launch_rows(RowsArgs a, hipStream_t stream) {
     return launched();
 }
 
-template <bool kBack, bool kDirect>
+template <bool kBack, Chunks kChunks>
 int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
-    if (a.wide <= 64) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kDirect>>(a, stream);
-    if constexpr (kDirect && kSize == 2) {
-        if (static_cast<int64_t>(a.rows / 256 + a.experts) * ((a.wide + 255) / 256) >= 512) return launch_rows<kBack, Product<Value, kBack, false, 256, 256, 4, 2, true>>(a, stream);
+    // (129 to 192 results: three tiles of 64, not two of 128)
+    if (a.wide <= 64 || (a.wide > 128 && a.wide <= 192) || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks>>(a, stream);
+    if constexpr (kChunks != Chunks::kSingle) {
+        if constexpr (kChunks == Chunks::kDirect && kSize == 2) {
+            if (static_cast<int64_t>(a.rows / 256 + a.experts) * ((a.wide + 255) / 256) >= 512)
+                return launch_rows<kBack, Product<Value, kBack, false, 256, 256, 4, 2, kChunks>>(a, stream);
+        }
+        return launch_rows<kBack, Product<Value, kBack, false, 128, 128, 2, 2, kChunks>>(a, stream);
     }
-    return launch_rows<kBack, Product<Value, kBack, false, 128, 128, 2, 2, kDirect>>(a, stream);
+}
+
+template <bool kBack>
+int rows_of_experts(const RowsArgs& a, Chunks chunks, hipStream_t stream) {
+    if (chunks == Chunks::kDirect) return rows_of_experts<kBack, Chunks::kDirect>(a, stream);
+    if (chunks == Chunks::kHeld) return rows_of_experts<kBack, Chunks::kHeld>(a, stream);
+    return rows_of_experts<kBack, Chunks::kSingle>(a, stream);
 }
 
 // How the rows of the weights' gradient are cut.
@@ -237,10 +265,10 @@ struct WeightPlan {
 };
 WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
     WeightPlan p;
-    p.side = channels <= 64 || outputs <= 64 ? 64 : kSize == 2 && channels >= 256 && outputs >= 256 && rows * channels * outputs >= int64_t{1} << 34 ? 256 : 128;
+    p.side = channels <= 64 || outputs <= 64 ? 64 : kSize == 2 && channels % 8 == 0 && outputs % 8 == 0 && channels >= 256 && outputs >= 256 && rows * channels * outputs >= int64_t{1} << 34 ? 256 : 128;
     const int64_t side = p.side;
     p.tiles = ((channels + side - 1) / side) * ((outputs + side - 1) / side);
-    const int64_t wanted = ((side == 256 ? 512 : 1024) + p.tiles - 1) / p.tiles;  // pieces for four workgroups to a compute unit
+    const int64_t wanted = ((side == 256 ? 512 : side == 128 ? 1024 : 2048) + p.tiles - 1) / p.tiles;  // pieces for four workgroups to a compute unit
     int64_t most = experts >= wanted ? 2 * ((rows + experts - 1) / experts) : (rows + wanted - 1) / wanted;
     most = std::max<int64_t>((most + 63) / 64 * 64, 512);
     p.most = std::min<int64_t>(most, (int64_t{1} << 30));
@@ -251,22 +279,25 @@ WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t 
 template <class P>
 int launch_weights(WeightArgs a, const WeightPlan& plan, hipStream_t stream) {
     a.channel_tiles = static_cast<uint32_t>((a.channels + P::kM - 1) / P::kM);
-    a.tiles = static_cast<uint32_t>(plan.tiles);
-    const int64_t items = plan.pieces * plan.tiles;
+    a.tiles = a.channel_tiles * static_cast<uint32_t>((a.outputs + P::kN - 1) / P::kN);
+    const int64_t items = plan.pieces * a.tiles;
     if (items * P::kThreads >= kMostThreads) return PENC_ERR_BAD_LAYER_SIZE;
     // (pieces take different times: all dies work on the same ones)
-    a.spread = Spread(items, plan.tiles / 8);
+    a.spread = Spread(items, a.tiles / 8);
     expert_weights_kernel<P><<<a.spread.grid(), P::kThreads, 0, stream>>>(a);
     return launched();
 }
 
-template <bool kDirect>
+template <Chunks kChunks>
 int weights_of_experts(const WeightArgs& a, const WeightPlan& plan, hipStream_t stream) {
-    if (plan.side == 64) return launch_weights<Product<Value, true, true, 64, 64, 2, 2, kDirect>>(a, plan, stream);
-    if constexpr (kSize == 2) {
-        if (plan.side == 256) return launch_weights<Product<Value, true, true, 256, 256, 2, 4, kDirect>>(a, plan, stream);
+    if (plan.side == 64) return launch_weights<Product<Value, true, true, 64, 64, 2, 2, kChunks>>(a, plan, stream);
+    if constexpr (kChunks != Chunks::kSingle) {
+        if constexpr (kChunks == Chunks::kDirect && kSize == 2) {
+            if (plan.side == 256) return launch_weights<Product<Value, true, true, 256, 256, 2, 4, kChunks>>(a, plan, stream);
+        }
+        return launch_weights<Product<Value, true, true, 128, 128, 2, 2, kChunks>>(a, plan, stream);
     }
-    return launch_weights<Product<Value, true, true, 128, 128, 2, 2, kDirect>>(a, plan, stream);
+    return PENC_ERR_BAD_LAYER_SIZE;  // (not reached: rows of less than 16 bytes have less than 64 values)
 }
 
 }  // namespace
@@ -275,11 +306,9 @@ template <>
 int expert_rows<PENC_TYPE>(bool back, int64_t rows, int experts, int64_t wide, int64_t deep, const void* in, int64_t stride, const void* weight, const void* bias,
                            const int32_t* offsets, void* out, hipStream_t stream) {
     if (rows == 0) return PENC_OK;
-    RowsArgs a{in, weight, bias, out, stride, offsets, experts, static_cast<int>(rows), static_cast<int>(wide), static_cast<int>(deep), {}, 0,
-               aligned_to(out, 16) && wide * kSize % 16 == 0};
-    const bool direct = chunked(in, stride, deep) && chunked(weight, back ? wide : deep, back ? wide : deep);
-    if (back) return direct ? rows_of_experts<true, true>(a, stream) : rows_of_experts<true, false>(a, stream);
-    return direct ? rows_of_experts<false, true>(a, stream) : rows_of_experts<false, false>(a, stream);
+    RowsArgs a{in, weight, bias, out, stride, offsets, experts, static_cast<int>(rows), static_cast<int>(wide), static_cast<int>(deep), {}, 0};
+    const Chunks chunks = std::max(chunks_of(in, stride, deep), chunks_of(weight, back ? wide : deep, back ? wide : deep));
+    return back ? rows_of_experts<true>(a, chunks, stream) : rows_of_experts<false>(a, chunks, stream);
 }
 
 template <>
@@ -294,14 +323,22 @@ int expert_weights<PENC_TYPE>(int64_t rows, int experts, int64_t channels, int64
                               const int32_t* offsets, void* weight, void* bias, void* workspace, hipStream_t stream) {
     const WeightPlan plan = weight_plan(rows, experts, channels, outputs);
     WeightArgs a{x, grad, x_stride, grad_stride, offsets, experts, static_cast<int>(rows), static_cast<int>(channels), static_cast<int>(outputs),
-                 static_cast<int>(plan.most), {}, 0, 0, weight, bias, static_cast<float*>(workspace), plan.pieces, aligned_to(weight, 16) && channels * kSize % 16 == 0};
-    const bool direct = chunked(x, x_stride, channels) && chunked(grad, grad_stride, outputs);
-    if (const int rc = direct ? weights_of_experts<true>(a, plan, stream) : weights_of_experts<false>(a, plan, stream)) return rc;
+                 static_cast<int>(plan.most), {}, 0, 0, weight, bias, static_cast<float*>(workspace), plan.pieces};
+    const Chunks chunks = std::max(chunks_of(x, x_stride, channels), chunks_of(grad, grad_stride, outputs));
+    if (const int rc = chunks == Chunks::kDirect ? weights_of_experts<Chunks::kDirect>(a, plan, stream)
+                       : chunks == Chunks::kHeld ? weights_of_experts<Chunks::kHeld>(a, plan, stream)
+                                                 : weights_of_experts<Chunks::kSingle>(a, plan, stream))
+        return rc;
     if (rows <= plan.most) return PENC_OK;
     const int64_t results = outputs * (channels + 1);
-    const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>((results + kSumThreads - 1) / kSumThreads, std::max<int64_t>(1, 65536 / experts)));
-    expert_sums_kernel<<<static_cast<uint32_t>(experts) * blocks, kSumThreads, 0, stream>>>(a, blocks);
-    return launched();
+    // (many pieces: a few results, and lanes that share them)
+    const auto sum = [&](auto slices) -> int {
+        constexpr int kSlices = decltype(slices)::value, kResults = kSumThreads / kSlices;
+        const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>((results + kResults - 1) / kResults, std::max<int64_t>(1, 65536 / experts)));
+        expert_sums_kernel<kSlices><<<static_cast<uint32_t>(experts) * blocks, kSumThreads, 0, stream>>>(a, blocks);
+        return launched();
+    };
+    return plan.pieces >= 32 * static_cast<int64_t>(experts) ? sum(std::integral_constant<int, 16>{}) : sum(std::integral_constant<int, 1>{});
 }
 
 }  // namespace penc

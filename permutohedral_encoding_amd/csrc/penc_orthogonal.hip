@@ -187,14 +187,14 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
         }
     } else {
         char* const out = a.out + matrix * a.rows * stride;
+        using result_four = Result __attribute__((ext_vector_type(4)));
         Result* const result = static_cast<Result*>(a.result) + matrix * a.rows * a.columns;
-        const bool aligned = a.columns % 4 == 0;
         p.each([&](int m, int n, tile_acc v) {
             m += m0, n += n0;
             if (n >= a.rows || m >= a.padded) return;
             v = a.a * load_stored<E>(x + n * stride, m) + v * kPerScale;
             if (a.result == nullptr) store_stored<E>(out + n * stride, m, v);
-            else if (m < a.columns) store_four(result + static_cast<int64_t>(n) * a.columns + m, v * kPerScale, a.columns - m, aligned);
+            else if (m < a.columns) store_values<Result, 4>(result + static_cast<int64_t>(n) * a.columns + m, __builtin_convertvector(v * kPerScale, result_four), a.columns - m);
         });
     }
 }
@@ -436,10 +436,10 @@ int launch_step(StepArgs a, int64_t matrices, hipStream_t stream) {
     const int64_t large = matrices * ((side_m + 127) / 128) * ((side_n + 127) / 128) / (kStage == kUpdate ? 1 : 2);
     const int64_t huge = matrices * ((side_m + 255) / 256) * ((side_n + 255) / 256) / (kStage == kUpdate ? 1 : 2);
     if constexpr (std::is_same_v<E, half_t>) {
-        if (huge >= 128) return launch(std::common_type<Product<E, kAlongM, kAlongN, 256, 256, 4, 2, true>>{});
+        if (huge >= 128) return launch(std::common_type<Product<E, kAlongM, kAlongN, 256, 256, 4, 2, Chunks::kDirect>>{});
     }
-    if (large < 256) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, true>>{});
-    return launch(std::common_type<Product<E, kAlongM, kAlongN, 128, 128, 2, 2, true>>{});
+    if (large < 256) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, Chunks::kDirect>>{});
+    return launch(std::common_type<Product<E, kAlongM, kAlongN, 128, 128, 2, 2, Chunks::kDirect>>{});
 }
 
 template <class E, class G>

@@ -11,8 +11,8 @@
 // hi hi + hi lo + lo hi, and what is left out is 2^-22 of it.
 //
 // Chunks of 16 bytes go from memory into the LDS directly, where rows and their ends are on 16 bytes.  Where a chunk stands in the LDS is fixed by the lane that brings it, so
-// a lane brings the chunk that belongs there.  Addresses behind an operand's end (rows, k, or columns) read zeros, which the buffer's bounds see to.  Of operands that
-// begin anywhere, lanes load what is there into registers and write it into the LDS.
+// a lane brings the chunk that belongs there.  Addresses behind an operand's end (rows, k, or columns) read zeros, which the buffer's bounds see to.  Of rows that begin anywhere,
+// lanes load chunks into registers and write them into the LDS two steps later; where a row ends, its last 16 bytes, of which what the chunk does not have is moved out then.
 //
 // Where a chunk stands: a read of 16 bytes takes 8 lanes at a time, one of 8 bytes 16 and one of 4 bytes 32, which should meet the 32 banks of 4 bytes once.  Across: lanes read one chunk c
 // of 8 rows; c stands at c ^ (row / 2 mod 4) (of 128 bytes: row mod 8).  Along: 16 lanes read 32 bytes (fp32: 64) of each of 4 neighbouring k (fp32: 32 lanes of two k, 4 apart);
@@ -143,9 +143,22 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
     return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(x >> 32)))) << 32 | low);
 }
 
+// How chunks come: directly, through registers, or (rows of less than 16 bytes) value by value.
+enum class Chunks { kDirect, kHeld, kSingle };
+
+// The last 16 - by of 16 bytes, and zeros behind them (by: a multiple of two).
+__device__ __forceinline__ chunk16 to_front(chunk16 m, int by) {
+    const bool eight = by & 8, four = by & 4, two = by & 2;
+    m = {eight ? m[2] : m[0], eight ? m[3] : m[1], eight ? 0u : m[2], eight ? 0u : m[3]};
+    m = {four ? m[1] : m[0], four ? m[2] : m[1], four ? m[3] : m[2], four ? 0u : m[3]};
+    if (two) m = {m[0] >> 16 | m[1] << 16, m[1] >> 16 | m[2] << 16, m[2] >> 16 | m[3] << 16, m[3] >> 16};
+    return by >= 16 ? chunk16{} : m;
+}
+
 // Brings an operand's steps into the LDS, one after the other.
-template <class E, bool kAlong, int kWide, int kThreads, bool kDirect>
+template <class E, bool kAlong, int kWide, int kThreads, Chunks kChunksCome>
 struct Loader {
+    static constexpr bool kDirect = kChunksCome == Chunks::kDirect;
     using Tile = OperandTile<E, kAlong, kWide>;
     using T = ProductType<E>;
     static constexpr int kEach = Tile::kChunks / kThreads;
@@ -155,27 +168,27 @@ struct Loader {
     int64_t step_bytes;
     int left;           // Across: bytes of a row, Along: rows
     int stride, rest;   // rest: what the buffer has beside: Across: the rows before the last, Along: how much longer a row is than they are apart
-    int rows;
-    int at[kEach];      // of this lane's chunks from `first` on
-    int byte;           // Across: in a row
-    chunk16 held[kDirect ? 1 : kEach];
+    int rows, wide;     // of the operand; bytes of a row (Along)
+    int at[kDirect ? kEach : 1];  // of this lane's chunks from `first` on
+    int byte;                     // Across: in a row
+    chunk16 held[kDirect ? 1 : 2][kDirect ? 1 : kEach];  // two steps
+
+    __device__ __forceinline__ static int slot_of(int j) { return j * kThreads + static_cast<int>(threadIdx.x); }
+    __device__ __forceinline__ static int row_of(int j) { return slot_of(j) / Tile::kRowChunks; }
+    __device__ __forceinline__ static int byte_of(int j) { return Tile::place(row_of(j), slot_of(j) % Tile::kRowChunks) * 16; }
 
     __device__ __forceinline__ explicit Loader(const Operand& o)
         : first(reinterpret_cast<const char*>(uniform(reinterpret_cast<int64_t>(o.first)))), step_bytes(kAlong ? T::kDepth * uniform(o.stride) : Tile::kLine),
           left(uniform(kAlong ? o.rows : o.bytes)), stride(uniform(static_cast<int>(o.stride))), rest(kAlong ? uniform(o.bytes) - stride : uniform(o.rows - 1) * stride),
-          rows(o.rows) {
+          rows(uniform(o.rows)), wide(uniform(o.bytes)), byte(byte_of(0)) {  // (byte: the same for all chunks: kThreads / kRowChunks rows are a whole number of permutations)
+        if constexpr (kDirect) {
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const int slot = j * kThreads + static_cast<int>(threadIdx.x), row = slot / Tile::kRowChunks;
-            const int in_row = Tile::place(row, slot % Tile::kRowChunks) * 16;
-            at[j] = row * stride + in_row;
-            if (!kAlong) byte = in_row;  // (the same for all of them: kThreads / kRowChunks rows are a whole number of permutations)
-            if (kAlong && in_row >= o.bytes) at[j] = -1;
+            for (int j = 0; j < kEach; ++j) at[j] = kAlong && byte_of(j) >= wide ? -1 : row_of(j) * stride + byte_of(j);
         }
     }
 
-    // The chunks of the next step are on their way, into the LDS or into registers.
-    __device__ __forceinline__ void begin(uint32_t lds) {
+    // The chunks of the next step are on their way, into the LDS or into registers (`hold`: which).
+    __device__ __forceinline__ void begin(uint32_t lds, int hold) {
         if constexpr (kDirect) {
             const int there = left <= 0 ? 0 : kAlong ? min(left, T::kDepth) * stride + rest : rest + left;
             const uint64_t p = reinterpret_cast<uint64_t>(first);
@@ -183,38 +196,50 @@ struct Loader {
             const uint32_t to = lds + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * 1024;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) load_to_lds(buffer, kAlong || byte < left ? at[j] : -1, to + j * kThreads * 16);
+        } else if constexpr (kChunksCome == Chunks::kHeld) {
+            // (loads have no conditions: where there is nothing, the operand's last row or a row's last 16 bytes are read)
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                using Unaligned = uint32_t __attribute__((ext_vector_type(4), aligned(T::kBytes == 2 ? 2 : 4)));
+                const int row = min(row_of(j), (kAlong ? left : rows) - 1), in_row = min(byte_of(j), (kAlong ? wide : left) - 16);
+                held[hold][j] = *reinterpret_cast<const Unaligned*>(first + (static_cast<int64_t>(row) * stride + in_row));
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
-                const int slot = j * kThreads + static_cast<int>(threadIdx.x), row = slot / Tile::kRowChunks;
-                const int in_row = Tile::place(row, slot % Tile::kRowChunks) * 16, n = kAlong ? (row < left ? rest + stride - in_row : 0) : (row < rows ? left - in_row : 0);
-                const char* const p = first + static_cast<int64_t>(row) * stride + in_row;
+                const int row = row_of(j), n = (row < (kAlong ? left : rows) ? (kAlong ? wide : left) : 0) - byte_of(j);
+                const char* const p = first + static_cast<int64_t>(row) * stride + byte_of(j);
                 chunk16 v{};
-                if (n >= 16) {
-                    using Unaligned = uint32_t __attribute__((ext_vector_type(4), aligned(T::kBytes == 2 ? 2 : 4)));
-                    v = *reinterpret_cast<const Unaligned*>(p);
-                } else if (n > 0) {
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        if constexpr (T::kBytes == 4) {
-                            if (4 * w < n) v[w] = *reinterpret_cast<const uint32_t*>(p + 4 * w);
-                        } else {
-                            if (4 * w < n) v[w] = *reinterpret_cast<const uint16_t*>(p + 4 * w);
-                            if (4 * w + 2 < n) v[w] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + 4 * w + 2)) << 16;
-                        }
+                for (int w = 0; w < 4; ++w) {
+                    if constexpr (T::kBytes == 4) {
+                        if (4 * w < n) v[w] = *reinterpret_cast<const uint32_t*>(p + 4 * w);
+                    } else {
+                        if (4 * w < n) v[w] = *reinterpret_cast<const uint16_t*>(p + 4 * w);
+                        if (4 * w + 2 < n) v[w] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + 4 * w + 2)) << 16;
                     }
                 }
-                held[j] = v;
+                held[hold][j] = v;
             }
         }
         first += step_bytes;
         left -= kAlong ? T::kDepth : Tile::kLine;
     }
-    // What is held goes into the LDS (a barrier makes it so for the other waves).
-    __device__ __forceinline__ void end(char* lds) {
+    // What was held two steps ago goes into the LDS (a barrier makes it so for the other waves).
+    __device__ __forceinline__ void end(char* lds, int hold) {
         if constexpr (!kDirect) {
+            if constexpr (kChunksCome == Chunks::kHeld) {
+                const int there = left + 2 * (kAlong ? T::kDepth : Tile::kLine);  // as it was
+                if (kAlong ? there < T::kDepth || wide < Tile::kRowBytes : there < Tile::kLine) {
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) *reinterpret_cast<chunk16*>(lds + (j * kThreads + static_cast<int>(threadIdx.x)) * 16) = held[j];
+                    for (int j = 0; j < kEach; ++j) {
+                        const int in_row = (kAlong ? wide : there) - byte_of(j);
+                        held[hold][j] = to_front(held[hold][j], kAlong && row_of(j) >= there ? 16 : min(max(16 - in_row, 0), 16));
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) *reinterpret_cast<chunk16*>(lds + slot_of(j) * 16) = held[hold][j];
         }
     }
 };
@@ -227,14 +252,15 @@ __device__ __forceinline__ void wait_for_loads() {
 }
 
 // A workgroup of kWavesM x kWavesN waves, each with kM / kWavesM x kN / kWavesN results; kRing steps have room in the LDS.
-template <class E, bool kAlongM, bool kAlongN, int kM_, int kN_, int kWavesM, int kWavesN, bool kDirect, int kRing = 4>
+template <class E, bool kAlongM, bool kAlongN, int kM_, int kN_, int kWavesM, int kWavesN, Chunks kChunksCome, int kRing = 4>
 struct Product {
     static constexpr int kM = kM_, kN = kN_, kThreads = 64 * kWavesM * kWavesN;
     static constexpr int kTilesM = kM / kWavesM / 16, kTilesN = kN / kWavesN / 16;
     using TileM = OperandTile<E, kAlongM, kM>;
     using TileN = OperandTile<E, kAlongN, kN>;
-    using LoadM = Loader<E, kAlongM, kM, kThreads, kDirect>;
-    using LoadN = Loader<E, kAlongN, kN, kThreads, kDirect>;
+    static constexpr bool kDirect = kChunksCome == Chunks::kDirect;
+    using LoadM = Loader<E, kAlongM, kM, kThreads, kChunksCome>;
+    using LoadN = Loader<E, kAlongN, kN, kThreads, kChunksCome>;
     static constexpr int kStage = TileM::kSize + TileN::kSize;
     static constexpr int kLds = kRing * kStage;
     static constexpr int kDepth = ProductType<E>::kDepth, kParts = ProductType<E>::kParts;
@@ -311,14 +337,14 @@ struct Product {
         constexpr int kAhead = kRing - 1;
         const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
         int room = 0, read = 0;  // where the next step goes, and where the next fragments are
-        const auto begin = [&] {
-            load_m.begin(lds_at + room);
-            load_n.begin(lds_at + room + TileM::kSize);
+        const auto begin = [&](int hold) {
+            load_m.begin(lds_at + room, hold);
+            load_n.begin(lds_at + room + TileM::kSize, hold);
             if constexpr (kDirect) room = room + kStage == kLds ? 0 : room + kStage;
         };
-        const auto end = [&] {
-            load_m.end(lds + room);
-            load_n.end(lds + room + TileM::kSize);
+        const auto end = [&](int hold) {
+            load_m.end(lds + room, hold);
+            load_n.end(lds + room + TileM::kSize, hold);
             if constexpr (!kDirect) room = room + kStage == kLds ? 0 : room + kStage;
         };
         const auto fragments = [&](Fragments& f) {
@@ -332,26 +358,29 @@ struct Product {
         };
         if constexpr (kDirect) {
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) begin();
+            for (int k = 0; k < kAhead; ++k) begin(0);
             start(first);
             wait_for_loads<kLoads * (kAhead - 1)>();
         } else {
+            static_assert(kRing == 4);
+            begin(0);
+            begin(1);
             start(first);
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                begin();
-                if (k + 1 < kAhead) end();
-            }
+            end(0);
+            begin(0);
+            end(1);
+            begin(1);
         }
         meet();
         Fragments even, odd;
         fragments(even);
         // In step i: what is brought for step i + 1 is there for all waves, and the fragments of step i - 1, whose room step i + kAhead takes, have been read.
-        const auto turn = [&](const Fragments& now, Fragments& next) {
+        // (Held in registers: steps i + 2, which goes into the LDS, and i + 3, and then i + 3 and i + 4.)
+        const auto turn = [&](const Fragments& now, Fragments& next, int hold) {
             if constexpr (kDirect) wait_for_loads<kLoads * (kAhead - 2)>();
             meet();
-            if constexpr (!kDirect) end();
-            begin();
+            if constexpr (!kDirect) end(hold);
+            begin(hold);
             __builtin_amdgcn_sched_barrier(0);
             fragments(next);
             multiply_step(now);
@@ -361,8 +390,8 @@ struct Product {
         };
         int i = 0;
         for (; i + 1 < steps; i += 2) {
-            turn(even, odd);
-            turn(odd, even);
+            turn(even, odd, 0);
+            turn(odd, even, 1);
         }
         if (i < steps) {
             multiply_step(even);
@@ -382,45 +411,43 @@ struct Product {
     }
 };
 
-// Stores v, of m .. m + 3 of `valid`, rounded once.
-template <class E>
-__device__ __forceinline__ void store_four(E* p, tile_acc v, int valid, bool aligned) {
-    using Four = E __attribute__((ext_vector_type(4)));
-    const Four y = __builtin_convertvector(v, Four);
-    if (valid >= 4 && aligned) {
-        *reinterpret_cast<Four*>(p) = y;
+// Stores the first `valid` of kWide values, wherever they are.
+template <class E, int kWide>
+__device__ __forceinline__ void store_values(E* p, E __attribute__((ext_vector_type(kWide))) v, int valid) {
+    using Unaligned = E __attribute__((ext_vector_type(kWide), aligned(sizeof(E))));
+    if (valid >= kWide) {
+        *reinterpret_cast<Unaligned*>(p) = v;
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < valid) p[i] = y[i];
+        for (int i = 0; i < kWide; ++i)
+            if (i < valid) p[i] = v[i];
     }
 }
 
-// Stores a workgroup's results as rows of n, `stride` values apart: `rows` of them and `columns` of m, rounded once.  aligned: rows begin on 16 bytes.
+// Stores a workgroup's results as rows of n, `stride` values apart: `rows` of them and `columns` of m, rounded once.
 // 16-bit results: lanes 16 apart have four neighbouring m each, of one n; they exchange those of two tiles, and each stores eight of one of them.
 template <class E, class P>
-__device__ __forceinline__ void store_rows(const P& p, E* out, int64_t stride, int rows, int columns, bool aligned) {
+__device__ __forceinline__ void store_rows(const P& p, E* out, int64_t stride, int rows, int columns) {
+    using Four = E __attribute__((ext_vector_type(4)));
     if constexpr (sizeof(E) == 2 && P::kTilesM % 2 == 0) {
-        if (aligned) {
-            const int lane = threadIdx.x % 64, g = lane / 16;
+        using Eight = E __attribute__((ext_vector_type(8)));
+        const int lane = threadIdx.x % 64, g = lane / 16;
 #pragma unroll
-            for (int j = 0; j < P::kTilesN; ++j) {
-                const int n = P::wave_n() + 16 * j + lane % 16;
+        for (int j = 0; j < P::kTilesN; ++j) {
+            const int n = P::wave_n() + 16 * j + lane % 16;
 #pragma unroll
-                for (int i = 0; i < P::kTilesM; i += 2) {
-                    using Four = E __attribute__((ext_vector_type(4)));
-                    const uint2 a = __builtin_bit_cast(uint2, __builtin_convertvector(p.acc[i][j], Four)), b = __builtin_bit_cast(uint2, __builtin_convertvector(p.acc[i + 1][j], Four));
-                    const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
-                    const int m = P::wave_m() + 16 * (i + g % 2) + g / 2 * 8;
-                    if (n < rows && m < columns) *reinterpret_cast<uint4*>(out + n * stride + m) = make_uint4(x[0], y[0], x[1], y[1]);
-                }
+            for (int i = 0; i < P::kTilesM; i += 2) {
+                const uint2 a = __builtin_bit_cast(uint2, __builtin_convertvector(p.acc[i][j], Four)), b = __builtin_bit_cast(uint2, __builtin_convertvector(p.acc[i + 1][j], Four));
+                const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+                const int m = P::wave_m() + 16 * (i + g % 2) + g / 2 * 8;
+                if (n < rows && m < columns) store_values<E, 8>(out + n * stride + m, __builtin_bit_cast(Eight, make_uint4(x[0], y[0], x[1], y[1])), columns - m);
             }
-            return;
         }
+    } else {
+        p.each([&](int m, int n, tile_acc v) {
+            if (n < rows && m < columns) store_values<E, 4>(out + n * stride + m, __builtin_convertvector(v, Four), columns - m);
+        });
     }
-    p.each([&](int m, int n, tile_acc v) {
-        if (n < rows && m < columns) store_four(out + n * stride + m, v, columns - m, aligned);
-    });
 }
 
 // How items are spread over a launch.  Consecutive workgroups go to the 8 dies in turn; each die gets `run` neighbouring items at a time, whose operands its cache then holds,
