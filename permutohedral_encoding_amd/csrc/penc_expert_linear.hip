@@ -120,6 +120,183 @@ __global__ __launch_bounds__(P::kThreads) void expert_rows_kernel(RowsArgs a) {
     store_rows(p, static_cast<Value*>(a.rows_out) + static_cast<int64_t>(t.first) * a.wide + m0, a.wide, t.rows, columns);
 }
 
+// ------------------------------------------------------------------------------------------
+// narrow layers, and few rows
+
+// 16 bytes of a buffer, zeros behind its end.
+__device__ __forceinline__ chunk16 load_chunk16(__amdgpu_buffer_rsrc_t buffer, int at) {
+    return __builtin_bit_cast(chunk16, __builtin_amdgcn_raw_buffer_load_b128(buffer, at, 0, 0));
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const char* first, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(first), 0, static_cast<int>(min(max(bytes, int64_t{0}), int64_t{0x7FFFFFFF})), 0x00020000);
+}
+
+// Stores what a wave has of 16 rows (v[t]: four of 16 results to a lane), `columns` of each.
+template <class E, int kTiles>
+__device__ __forceinline__ void store_sixteen_rows(const tile_acc (&v)[kTiles], E* out, int64_t stride, int rows, int columns) {
+    using Four = E __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x % 64, n = lane % 16, g = lane / 16;
+    if constexpr (sizeof(E) == 2 && kTiles % 2 == 0) {
+        using Eight = E __attribute__((ext_vector_type(8)));
+#pragma unroll
+        for (int t = 0; t < kTiles; t += 2) {
+            const uint2 a = __builtin_bit_cast(uint2, __builtin_convertvector(v[t], Four)), b = __builtin_bit_cast(uint2, __builtin_convertvector(v[t + 1], Four));
+            const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+            const int m = 16 * (t + g % 2) + g / 2 * 8;
+            if (n < rows && m < columns) store_values<E, 8>(out + n * stride + m, __builtin_bit_cast(Eight, make_uint4(x[0], y[0], x[1], y[1])), columns - m);
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const int m = 16 * t + g * 4;
+            if (n < rows && m < columns) store_values<E, 4>(out + n * stride + m, __builtin_convertvector(v[t], Four), columns - m);
+        }
+    }
+}
+
+constexpr int kNarrowThreads = 256, kNarrowLines = 4, kNarrowTiles = 4;  // 64 results of 256 bytes
+constexpr int kNarrowGroups = kSize == 2 ? 2 : 1;                       // of 16 rows that a wave has at a time
+
+// Layers whose weights fit a wave's registers: at most 64 results of rows of at most 256 bytes.  The weights come through the LDS once; then waves walk over rows, 16 (or twice 16) at a
+// time, straight from memory into the fragments' registers, the next ones on their way.
+template <bool kBack, int kLines, int kTiles>
+__global__ __launch_bounds__(kNarrowThreads) void expert_narrow_kernel(RowsArgs a, int most) {
+    using Load = Loader<Value, kBack, 64, kNarrowThreads, Chunks::kDirect>;
+    using Tile = typename Load::Tile;
+    __shared__ __attribute__((aligned(1024))) char lds[kLines * Tile::kSize];
+    const uint32_t item = a.spread.item();
+    if (item >= a.spread.items) return;
+    const RowTile t = row_tile<true>(a.offsets, a.experts, a.rows, item, most);
+    if (t.expert < 0) return;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    Value* const out = static_cast<Value*>(a.rows_out) + static_cast<int64_t>(t.first) * a.wide;
+    constexpr int kStep = 16 * kNarrowGroups * kNarrowThreads / 64;
+    if (t.expert == a.experts) {
+        const tile_acc zero[kTiles] = {};
+        for (int row = wave * 16; row < t.rows; row += 16 * kNarrowThreads / 64) store_sixteen_rows(zero, out + static_cast<int64_t>(row) * a.wide, a.wide, t.rows - row, a.wide);
+        return;
+    }
+    const char* const weight = static_cast<const char*>(a.weight) + static_cast<int64_t>(t.expert) * a.wide * a.deep * kSize;
+    Load load(kBack ? Operand{weight, static_cast<int64_t>(a.wide) * kSize, a.deep, a.wide * kSize} : Operand{weight, static_cast<int64_t>(a.deep) * kSize, a.wide, a.deep * kSize});
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+#pragma unroll
+    for (int l = 0; l < kLines; ++l) load.begin(lds_at + l * Tile::kSize, 0);
+
+    // this lane's chunks of a row, and of the rows of a group
+    const int deep_bytes = a.deep * kSize, stride = static_cast<int>(a.stride) * kSize;
+    int at[kLines];
+#pragma unroll
+    for (int l = 0; l < kLines; ++l) {
+        const int byte = l * 64 + lane / 16 * 16;
+        at[l] = byte < deep_bytes ? lane % 16 * stride + byte : -1;
+    }
+    const char* const in = static_cast<const char*>(a.rows_in) + static_cast<int64_t>(t.first) * a.stride * kSize;
+    chunk16 rows[kNarrowGroups][kLines], next[kNarrowGroups][kLines];
+    const auto begin = [&](chunk16 (&r)[kNarrowGroups][kLines], int row) {
+#pragma unroll
+        for (int k = 0; k < kNarrowGroups; ++k) {
+            const int first = row + 16 * k, left = t.rows - first;
+            const auto buffer = buffer_of(in + static_cast<int64_t>(first) * stride, left <= 0 ? 0 : static_cast<int64_t>(left - 1) * stride + deep_bytes);
+#pragma unroll
+            for (int l = 0; l < kLines; ++l) r[k][l] = load_chunk16(buffer, at[l]);
+        }
+    };
+    int row = wave * 16 * kNarrowGroups;
+    begin(next, row);
+    tile_acc bias[kTiles] = {};
+    if (!kBack && a.bias != nullptr) {
+        const Value* const from = static_cast<const Value*>(a.bias) + static_cast<int64_t>(t.expert) * a.wide;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int m = 16 * i + lane / 16 * 4 + k;
+                bias[i][k] = m < a.wide ? static_cast<float>(from[m]) : 0.0f;
+            }
+    }
+    wait_for_loads<0>();
+    __syncthreads();
+    chunk16 w[kTiles][kLines];
+#pragma unroll
+    for (int l = 0; l < kLines; ++l)
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) w[i][l] = Tile::fragment(lds + l * Tile::kSize, 16 * i, 0);
+    for (; row < t.rows; row += kStep) {
+#pragma unroll
+        for (int k = 0; k < kNarrowGroups; ++k)
+#pragma unroll
+            for (int l = 0; l < kLines; ++l) rows[k][l] = next[k][l];
+        begin(next, row + kStep);
+#pragma unroll
+        for (int k = 0; k < kNarrowGroups; ++k) {
+            tile_acc acc[kTiles];
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) acc[i] = bias[i];
+#pragma unroll
+            for (int l = 0; l < kLines; ++l)
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) acc[i] = multiply<Value>(w[i][l], rows[k][l], acc[i]);
+            const int first = row + 16 * k;
+            store_sixteen_rows(acc, out + static_cast<int64_t>(first) * a.wide, a.wide, t.rows - first, a.wide);
+        }
+    }
+}
+
+constexpr int kFewRows = 16, kFewOutputs = 64, kFewThreads = 256, kFewWaves = kFewThreads / 64;
+
+// A few rows of an expert, whose weights are what there is to read: 64 outputs of 16 rows to a workgroup, whose waves take each fourth line of 64 bytes of all of them straight into the
+// fragments' registers, four lines on their way, and add their sums in order.
+__global__ __launch_bounds__(kFewThreads) void expert_few_kernel(RowsArgs a) {
+    constexpr int kTiles = kFewOutputs / 16, kAhead = 4;
+    __shared__ tile_acc lds[kFewWaves - 1][kTiles][64];
+    const uint32_t item = a.spread.item();
+    if (item >= a.spread.items) return;
+    const RowTile t = row_tile<true>(a.offsets, a.experts, a.rows, item / a.tiles, kFewRows);
+    if (t.expert < 0) return;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), m0 = static_cast<int>(item % a.tiles) * kFewOutputs, columns = a.wide - m0;
+    tile_acc acc[kTiles] = {};
+    if (t.expert < a.experts) {
+        const int deep_bytes = a.deep * kSize, stride = static_cast<int>(a.stride) * kSize;
+        const auto weights = buffer_of(static_cast<const char*>(a.weight) + (static_cast<int64_t>(t.expert) * a.wide + m0) * deep_bytes, static_cast<int64_t>(min(columns, kFewOutputs)) * deep_bytes);
+        const auto rows = buffer_of(static_cast<const char*>(a.rows_in) + static_cast<int64_t>(t.first) * stride, static_cast<int64_t>(t.rows - 1) * stride + deep_bytes);
+        const int w_at = lane % 16 * deep_bytes + lane / 16 * 16, x_at = lane % 16 * stride + lane / 16 * 16;
+        for (int first = wave * 64; first < deep_bytes; first += kAhead * kFewWaves * 64) {
+            chunk16 w[kAhead][kTiles], x[kAhead];
+#pragma unroll
+            for (int l = 0; l < kAhead; ++l) {
+                const int byte = first + l * kFewWaves * 64;
+                const bool there = byte + lane / 16 * 16 < deep_bytes;
+                x[l] = load_chunk16(rows, there ? x_at + byte : -1);
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) w[l][i] = load_chunk16(weights, there ? w_at + 16 * i * deep_bytes + byte : -1);
+            }
+#pragma unroll
+            for (int l = 0; l < kAhead; ++l)
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) acc[i] = multiply<Value>(w[l][i], x[l], acc[i]);
+        }
+    }
+    if (wave > 0) {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) lds[wave - 1][i][lane] = acc[i];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+        for (int k = 0; k < kFewWaves - 1; ++k) acc[i] += lds[k][i][lane];
+        if (a.bias != nullptr && t.expert < a.experts) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int m = m0 + 16 * i + lane / 16 * 4 + k;
+                if (m < a.wide) acc[i][k] += static_cast<float>(static_cast<const Value*>(a.bias)[static_cast<int64_t>(t.expert) * a.wide + m]);
+            }
+        }
+    }
+    store_sixteen_rows(acc, static_cast<Value*>(a.rows_out) + static_cast<int64_t>(t.first) * a.wide + m0, a.wide, t.rows, columns);
+}
+
 struct WeightArgs {
     const void *x, *grad;
     int64_t x_stride, grad_stride;
@@ -146,15 +323,31 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
     const Operand n{static_cast<const char*>(a.grad) + (static_cast<int64_t>(t.first) * a.grad_stride + o0) * kSize, a.grad_stride * kSize, t.rows,
                     min(a.outputs - o0, P::kN) * kSize};
     P p;
-    // the sums of dy itself are its products with ones
+    // the sums of dy itself: of 16-bit types its products with ones, of fp32, whose products take eight times as long, each lane's own k
     tile_acc bias_acc[P::kTilesN] = {};
-    const uint32_t one = PENC_TYPE == PENC_FP32 ? 0x3F800000u : PENC_TYPE == PENC_FP16 ? 0x3C003C00u : 0x3F803F80u;
+    const uint32_t one = PENC_TYPE == PENC_FP16 ? 0x3C003C00u : 0x3F803F80u;
     const chunk16 ones = {one, one, one, one};
     p.run(lds, m, n, t.rows, P::kZero, [&](const chunk16 (&grad)[P::kTilesN]) {
         if (!bias) return;
 #pragma unroll
-        for (int j = 0; j < P::kTilesN; ++j) bias_acc[j] = multiply<Value>(ones, grad[j], bias_acc[j]);
+        for (int j = 0; j < P::kTilesN; ++j) {
+            if constexpr (PENC_TYPE == PENC_FP32) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) bias_acc[j][k] += __uint_as_float(grad[j][k]);
+            } else {
+                bias_acc[j] = multiply<Value>(ones, grad[j], bias_acc[j]);
+            }
+        }
     });
+    if constexpr (PENC_TYPE == PENC_FP32) {
+#pragma unroll
+        for (int j = 0; j < P::kTilesN; ++j) {
+            float sum = (bias_acc[j][0] + bias_acc[j][1]) + (bias_acc[j][2] + bias_acc[j][3]);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            bias_acc[j][0] = sum;
+        }
+    }
     const int64_t n_weights = static_cast<int64_t>(a.outputs) * a.channels;
     const bool whole = t.tiles == 1;
     const int64_t at = static_cast<int64_t>(o0) * a.channels + c0;
@@ -226,18 +419,51 @@ Chunks chunks_of(const void* p, int64_t stride, int64_t values) {
 // (a launch has less than 2^32 threads, and a spread rounds up)
 constexpr int64_t kMostThreads = (int64_t{1} << 32) - (1 << 18);
 
+// The most tiles of `most` rows that there are.
+int64_t row_tiles(const RowsArgs& a, int most) { return a.rows / most + std::min(a.experts, a.rows) + 1; }
+
 template <bool kBack, class P>
 int launch_rows(RowsArgs a, hipStream_t stream) {
     a.tiles = static_cast<uint32_t>((a.wide + P::kM - 1) / P::kM);
-    const int64_t items = (a.rows / P::kN + static_cast<int64_t>(a.experts) + 1) * a.tiles;
+    const int64_t items = row_tiles(a, P::kN) * a.tiles;
     if (items * P::kThreads >= kMostThreads) return PENC_ERR_BAD_LAYER_SIZE;
     a.spread = Spread(items, 32);
     expert_rows_kernel<kBack, P><<<a.spread.grid(), P::kThreads, 0, stream>>>(a);
     return launched();
 }
 
+template <bool kBack>
+int launch_narrow(RowsArgs a, hipStream_t stream) {
+    // (1024 workgroups, as many as the card holds, have some that begin late: 2^20 x 64 by 64 fp32 140 us, 4096 of them 125)
+    const int most = static_cast<int>(std::min<int64_t>(std::max<int64_t>((a.rows / 4096 + 63) / 64 * 64, 256), 1 << 16));
+    a.spread = Spread(row_tiles(a, most), 1);
+    const auto launch = [&](auto lines, auto tiles) -> int {
+        expert_narrow_kernel<kBack, decltype(lines)::value, decltype(tiles)::value><<<a.spread.grid(), kNarrowThreads, 0, stream>>>(a, most);
+        return launched();
+    };
+    const auto with_tiles = [&](auto lines) -> int {
+        if (a.wide <= 16) return launch(lines, std::integral_constant<int, 1>{});
+        if (a.wide <= 32) return launch(lines, std::integral_constant<int, 2>{});
+        return launch(lines, std::integral_constant<int, 4>{});
+    };
+    return a.deep * kSize <= 128 ? with_tiles(std::integral_constant<int, 2>{}) : with_tiles(std::integral_constant<int, 4>{});
+}
+
+int launch_few(RowsArgs a, hipStream_t stream) {
+    a.tiles = static_cast<uint32_t>((a.wide + kFewOutputs - 1) / kFewOutputs);
+    const int64_t items = row_tiles(a, kFewRows) * a.tiles;
+    if (items * kFewThreads >= kMostThreads) return PENC_ERR_BAD_LAYER_SIZE;
+    a.spread = Spread(items, 32);
+    expert_few_kernel<<<a.spread.grid(), kFewThreads, 0, stream>>>(a);
+    return launched();
+}
+
 template <bool kBack, Chunks kChunks>
 int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
+    if constexpr (kChunks == Chunks::kDirect) {
+        if (a.wide <= 16 * kNarrowTiles && a.deep * kSize <= 64 * kNarrowLines && a.stride * kSize * 64 < 1 << 30) return launch_narrow<kBack>(a, stream);
+        if (!kBack && a.rows <= kFewRows * static_cast<int64_t>(a.experts)) return launch_few(a, stream);
+    }
     // (129 to 192 results: three tiles of 64, not two of 128)
     if (a.wide <= 64 || (a.wide > 128 && a.wide <= 192) || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks>>(a, stream);
     if constexpr (kChunks != Chunks::kSingle) {

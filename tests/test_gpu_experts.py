@@ -277,6 +277,15 @@ def test_expert_linear(dtype, rows, number, channels, outputs):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,channels,outputs", [(1000, 3, 64, 64), (1000, 4, 8, 3), (999, 2, 16, 17), (700, 3, 128, 40), (513, 5, 32, 33), (2000, 2, 24, 64),
+                                                          (5, 8, 264, 200), (40, 16, 512, 130), (16, 1, 1032, 65), (3, 300, 64, 100), (100, 9, 2048, 80)])
+def test_expert_linear_of_narrow_layers_and_of_few_rows(dtype, rows, number, channels, outputs):
+    for none in (0.0, 0.3, 1.0):
+        check_products(rows, number, channels, outputs, TYPES[dtype], none=none, extra=8, empty=(1,) if number > 1 else ())
+        check_products(rows, number, outputs, channels, TYPES[dtype], none=none, bias=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_expert_linear_of_rows_that_begin_anywhere(dtype):
     for extra in (1, 2, 3, 5):
         check_products(401, 3, 64, 136, TYPES[dtype], extra=extra)
