@@ -30,33 +30,35 @@ struct Coefficients {
     float a, b, c, eps;
 };
 
-// Four numbers at `column` of a stored row.
+// Where `column` of a stored row is.
 template <class E>
 __device__ __forceinline__ int column_at(int column) {
     if constexpr (std::is_same_v<E, split_t>) return column / 32 * 128 + column % 32 * 2;
     else return column * 2;
 }
-using half_four = half_t __attribute__((ext_vector_type(4)));
+template <int kWide>
+using halves = half_t __attribute__((ext_vector_type(kWide)));
+template <int kWide>
+using floats = float __attribute__((ext_vector_type(kWide)));
+
+// What of v the second half holds.
+template <int kWide>
+__device__ __forceinline__ halves<kWide> rest_of(floats<kWide> v, halves<kWide> hi) {
+    return __builtin_convertvector(v - __builtin_convertvector(hi, floats<kWide>), halves<kWide>);
+}
 template <class E>
-__device__ __forceinline__ tile_acc load_stored(const char* row, int column) {
+__device__ __forceinline__ floats<8> load_stored(const char* row, int column) {
     const char* const p = row + column_at<E>(column);
-    tile_acc v = __builtin_convertvector(*reinterpret_cast<const half_four*>(p), tile_acc);
-    if constexpr (std::is_same_v<E, split_t>) v += __builtin_convertvector(*reinterpret_cast<const half_four*>(p + 64), tile_acc);
+    floats<8> v = __builtin_convertvector(*reinterpret_cast<const halves<8>*>(p), floats<8>);
+    if constexpr (std::is_same_v<E, split_t>) v += __builtin_convertvector(*reinterpret_cast<const halves<8>*>(p + 64), floats<8>);
     return v;
 }
 template <class E>
-__device__ __forceinline__ void store_stored(char* row, int column, tile_acc v) {
+__device__ __forceinline__ void store_stored(char* row, int column, floats<8> v) {
     char* const p = row + column_at<E>(column);
-    const half_four hi = __builtin_convertvector(v, half_four);
-    *reinterpret_cast<half_four*>(p) = hi;
-    if constexpr (std::is_same_v<E, split_t>) *reinterpret_cast<half_four*>(p + 64) = __builtin_convertvector(v - __builtin_convertvector(hi, tile_acc), half_four);
-}
-template <class E>
-__device__ __forceinline__ void store_stored(char* row, int column, float v) {
-    char* const p = row + column_at<E>(column);
-    const half_t hi = static_cast<half_t>(v);
-    *reinterpret_cast<half_t*>(p) = hi;
-    if constexpr (std::is_same_v<E, split_t>) *reinterpret_cast<half_t*>(p + 64) = static_cast<half_t>(v - static_cast<float>(hi));
+    const halves<8> hi = __builtin_convertvector(v, halves<8>);
+    *reinterpret_cast<halves<8>*>(p) = hi;
+    if constexpr (std::is_same_v<E, split_t>) *reinterpret_cast<halves<8>*>(p + 64) = rest_of<8>(v, hi);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -84,18 +86,29 @@ __device__ __forceinline__ double per_norm(double squares, float eps) { return s
 template <class G>
 __device__ __forceinline__ float scaled(G g, double factor) { return static_cast<float>(static_cast<double>(static_cast<float>(g)) * factor); }
 
+// 16 x 4096 x 1024 bf16 28 us, 4.8 TB/s.
 template <class G>
 __global__ __launch_bounds__(kThreads) void squares_kernel(int64_t values, int pieces, const G* __restrict__ g, double* __restrict__ sums) {
-    const int64_t each = (values + pieces - 1) / pieces, piece = blockIdx.x % pieces;
-    const int64_t first = piece * each, last = min(first + each, values);
-    const G* const from = g + blockIdx.x / pieces * values;
-    double sum = 0.0;
-    for (int64_t i = first + threadIdx.x; i < last; i += kThreads) {
-        const double v = static_cast<double>(static_cast<float>(from[i]));
-        sum += v * v;
+    constexpr int kWide = 16 / sizeof(G);
+    using Unaligned = G __attribute__((ext_vector_type(kWide), aligned(sizeof(G))));
+    const int64_t each = ((values + pieces - 1) / pieces + kWide - 1) / kWide * kWide, piece = blockIdx.x % pieces;
+    const int64_t first = piece * each, last = min(first + each, values), whole = max(last - first, int64_t{0}) / kWide;
+    const G* const from = g + blockIdx.x / pieces * values + first;
+    double sum[kWide] = {};
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < whole; i += kThreads) {
+        const Unaligned v = *reinterpret_cast<const Unaligned*>(from + i * kWide);
+#pragma unroll
+        for (int k = 0; k < kWide; ++k) sum[k] = __builtin_fma(static_cast<double>(static_cast<float>(v[k])), static_cast<double>(static_cast<float>(v[k])), sum[k]);
     }
-    sum = workgroup_sum<kThreads>(sum);
-    if (threadIdx.x == 0) sums[blockIdx.x] = sum;
+    for (int64_t i = whole * kWide + threadIdx.x; i < last - first; i += kThreads) {
+        const double v = static_cast<double>(static_cast<float>(from[i]));
+        sum[0] += v * v;
+    }
+#pragma unroll
+    for (int k = 1; k < kWide; ++k) sum[0] += sum[k];
+    sum[0] = workgroup_sum<kThreads>(sum[0]);
+    if (threadIdx.x == 0) sums[blockIdx.x] = sum[0];
 }
 
 // X 2^12 as it is stored, zeros behind each row's end.
@@ -110,13 +123,22 @@ __global__ __launch_bounds__(kThreads) void stage_kernel(int rows, int columns, 
     const G* const from = g + matrix * rows * columns;
     const int64_t stride = static_cast<int64_t>(padded) * ProductType<E>::kBytes;
     char* const to = x + matrix * rows * stride;
-    const int64_t fours = static_cast<int64_t>(rows) * (padded / 4);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x % blocks) * kThreads + threadIdx.x; i < fours; i += static_cast<int64_t>(blocks) * kThreads) {
-        const int64_t row = i / (padded / 4);
-        const int column = static_cast<int>(i % (padded / 4)) * 4;
-        tile_acc v;
+    using Unaligned = G __attribute__((ext_vector_type(8), aligned(sizeof(G))));
+    const uint32_t per_row = padded / 8, eights = static_cast<uint32_t>(rows) * per_row;  // (below 2^30: sides are at most 2^16)
+    for (uint32_t i = blockIdx.x % blocks * kThreads + threadIdx.x; i < eights; i += blocks * kThreads) {
+        const uint32_t row = i / per_row;
+        const int column = static_cast<int>(i % per_row) * 8;
+        const G* const p = from + static_cast<int64_t>(row) * columns + column;
+        floats<8> v{};
+        if (column + 8 <= columns) {
+            const Unaligned u = *reinterpret_cast<const Unaligned*>(p);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = column + k < columns ? scaled(from[row * columns + column + k], factor) : 0.0f;
+            for (int k = 0; k < 8; ++k) v[k] = scaled(u[k], factor);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (column + k < columns) v[k] = scaled(p[k], factor);
+        }
         store_stored<E>(to + row * stride, column, v);
     }
 }
@@ -144,6 +166,13 @@ __device__ __forceinline__ void pair_of(uint32_t t, uint32_t& i, uint32_t& j) {
     i = t - j * (j + 1) / 2;
 }
 
+// Where eight halves from m on stand in row n of a tile that is to be turned: neighbouring rows of eight lanes, and four rows of 32 bytes, meet no bank twice.
+template <int kWideM>
+__device__ __forceinline__ int turned_place(int n, int m) {
+    constexpr int kChunks = kWideM / 8;
+    return (m / 8 ^ (kChunks >= 8 ? (n & 3) << 1 | (n >> 2 & 1) : n >> 1 & 3)) * 16;
+}
+
 template <Stage kStage, bool kTall, class E, class Result, class P>
 __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
@@ -166,35 +195,55 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
     else p.run(lds, rows_from(f, small_stride, a.small, m0, P::kM), rows_from(x, stride, a.rows, n0, P::kN), a.padded, P::kZero, P::kNothing);
     if constexpr (kStage != kUpdate) {
         char* const out = a.out + matrix * a.small * small_stride;
-        p.each([&](int m, int n, tile_acc v) {
+        constexpr int kWideM = P::kM / P::kWavesM, kWideN = P::kN / P::kWavesN, kParts = ProductType<E>::kParts;
+        // The other side of the diagonal: a wave's results as halves in the LDS, rows of n, and read back by columns.
+        static_assert(kParts * P::kThreads / 64 * kWideM * kWideN * 2 <= P::kLds);
+        char* const turned = lds + P::wave() * (kParts * kWideM * kWideN * 2);
+        if (m0 != n0) __syncthreads();
+        p.each_eight([&](int m, int n, floats<8> v) {
+            const int lm = m - P::wave_m(), ln = n - P::wave_n();
             m += m0, n += n0;
-            if (n >= a.small || m >= a.small_padded) return;
             v *= kPerScale;
-            if constexpr (kStage == kSquare) v = a.b * load_stored<E>(s + n * small_stride, m) + a.c * v;
-            store_stored<E>(out + n * small_stride, m, v);
-            if (i == j) return;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (m + k < a.small) store_stored<E>(out + (m + k) * small_stride, n, v[k]);
+            const bool there = n < a.small && m < a.small_padded;
+            if constexpr (kStage == kSquare) v = a.b * (there ? load_stored<E>(s + n * small_stride, m) : floats<8>{}) + a.c * v;
+            if (there) store_stored<E>(out + n * small_stride, m, v);
+            if (m0 == n0) return;
+            const halves<8> hi = __builtin_convertvector(v, halves<8>);
+            *reinterpret_cast<halves<8>*>(turned + ln * (kWideM * 2) + turned_place<kWideM>(ln, lm)) = hi;
+            if constexpr (kParts == 2) *reinterpret_cast<halves<8>*>(turned + (kWideN + ln) * (kWideM * 2) + turned_place<kWideM>(ln, lm)) = rest_of<8>(v, hi);
         });
-        // (columns behind the last one, of rows that only the other side of the diagonal has)
-        if (i != j && n0 + P::kN >= a.small) {
-            const int behind = a.small_padded - a.small;
-            for (int k = static_cast<int>(threadIdx.x); k < behind * P::kM; k += P::kThreads) {
-                const int row = m0 + k / behind;
-                if (row < a.small) store_stored<E>(out + row * small_stride, a.small + k % behind, 0.0f);
-            }
-        }
+        if (m0 == n0) return;
+        // lane 16 g + i: row m + i of the other side, eight columns from n + 8 g on
+        const int lane = threadIdx.x % 64, g = lane / 16, l16 = lane % 16;
+        using V = short __attribute__((ext_vector_type(4)));
+        using Lds = __attribute__((address_space(3))) V;
+#pragma unroll
+        for (int m = 0; m < kWideM; m += 16)
+#pragma unroll
+            for (int n = 0; n < kWideN; n += 32)
+#pragma unroll
+                for (int part = 0; part < kParts; ++part) {
+                    uint2 w[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int ln = n + g * 8 + h * 4 + l16 / 4, lm = m + l16 % 4 * 4;
+                        w[h] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                             (Lds*)(turned + (part * kWideN + ln) * (kWideM * 2) + turned_place<kWideM>(ln, lm & ~7) + lm % 8 * 2)));
+                    }
+                    const int row = m0 + P::wave_m() + m + l16, column = n0 + P::wave_n() + n + g * 8;
+                    if (row < a.small && column < a.small_padded)
+                        *reinterpret_cast<uint4*>(out + row * small_stride + column_at<E>(column) + part * 64) = make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
+                }
     } else {
         char* const out = a.out + matrix * a.rows * stride;
-        using result_four = Result __attribute__((ext_vector_type(4)));
         Result* const result = static_cast<Result*>(a.result) + matrix * a.rows * a.columns;
-        p.each([&](int m, int n, tile_acc v) {
+        using Eight = Result __attribute__((ext_vector_type(8)));
+        p.each_eight([&](int m, int n, floats<8> v) {
             m += m0, n += n0;
             if (n >= a.rows || m >= a.padded) return;
             v = a.a * load_stored<E>(x + n * stride, m) + v * kPerScale;
             if (a.result == nullptr) store_stored<E>(out + n * stride, m, v);
-            else if (m < a.columns) store_values<Result, 4>(result + static_cast<int64_t>(n) * a.columns + m, __builtin_convertvector(v * kPerScale, result_four), a.columns - m);
+            else if (m < a.columns) store_values<Result, 8>(result + static_cast<int64_t>(n) * a.columns + m, __builtin_convertvector(v * kPerScale, Eight), a.columns - m);
         });
     }
 }
@@ -204,6 +253,7 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
 
 constexpr int kResidentThreads = 512, kResidentWaves = kResidentThreads / 64;
 constexpr int kMostSmall = 128;
+constexpr int kMostResident = 160 * 1024 - 256;  // bytes of the LDS
 
 // A matrix of Split numbers in the LDS.  Chunks of a row's 128 bytes are permuted by the row, so that neither 8 rows of one chunk nor 4 rows of two chunks meet in a bank.
 struct Resident {
@@ -230,22 +280,12 @@ struct Resident {
         }
         return f;
     }
-    __device__ __forceinline__ tile_acc load(int row, int column) const {
+    template <int kWide>
+    __device__ __forceinline__ void store(int row, int column, floats<kWide> v) const {
         const int byte = column_at<split_t>(column);
-        return __builtin_convertvector(*reinterpret_cast<const half_four*>(chunk(row, byte)), tile_acc) +
-               __builtin_convertvector(*reinterpret_cast<const half_four*>(chunk(row, byte + 64)), tile_acc);
-    }
-    __device__ __forceinline__ void store(int row, int column, tile_acc v) const {
-        const int byte = column_at<split_t>(column);
-        const half_four hi = __builtin_convertvector(v, half_four);
-        *reinterpret_cast<half_four*>(chunk(row, byte)) = hi;
-        *reinterpret_cast<half_four*>(chunk(row, byte + 64)) = __builtin_convertvector(v - __builtin_convertvector(hi, tile_acc), half_four);
-    }
-    __device__ __forceinline__ void store(int row, int column, float v) const {
-        const int byte = column_at<split_t>(column);
-        const half_t hi = static_cast<half_t>(v);
-        *reinterpret_cast<half_t*>(chunk(row, byte)) = hi;
-        *reinterpret_cast<half_t*>(chunk(row, byte + 64)) = static_cast<half_t>(v - static_cast<float>(hi));
+        const halves<kWide> hi = __builtin_convertvector(v, halves<kWide>);
+        *reinterpret_cast<halves<kWide>*>(chunk(row, byte)) = hi;
+        *reinterpret_cast<halves<kWide>*>(chunk(row, byte + 64)) = rest_of<kWide>(v, hi);
     }
 };
 
@@ -258,57 +298,80 @@ __device__ __forceinline__ tile_acc multiply_split(chunk16 a, chunk16 a_low, chu
 __host__ __device__ constexpr int resident_pitch(int padded) { return padded * 4; }
 __host__ __device__ constexpr int round_to_32(int n) { return (n + 31) / 32 * 32; }
 
-// One matrix to a workgroup, X as `small` rows of `large` numbers whichever way it lies in memory.  A wave has 16 x 32 results of S and of F, and 16 columns of X, which it
-// overwrites when it has them all.
-template <class G, int kLds>
+// One matrix to a workgroup, X as `small` rows (at most 16 kTiles) of `large` numbers whichever way it lies in memory.  A wave has 16 x 32 results of S and of F, and up to kBlocks times 16
+// columns of X, which are its own: in fp32 in its registers, for a X, and as operands in the LDS, which it overwrites when it has read them.
+template <class G, int kTiles, int kBlocks>
 __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, int columns, int steps, Coefficients k, const G* __restrict__ g, G* __restrict__ result) {
-    __shared__ __attribute__((aligned(1024))) char lds[kLds];
+    __shared__ __attribute__((aligned(1024))) char lds[kMostResident];
+    constexpr int kPadded = 16 * kTiles, kLines = kPadded / 32;
     const bool tall = rows > columns;
-    const int small = min(rows, columns), large = max(rows, columns), small_padded = round_to_32(small), large_padded = round_to_32(large);
-    const Resident x{lds, resident_pitch(large_padded)}, s{lds + small_padded * x.pitch, resident_pitch(small_padded)};
+    const int small = min(rows, columns), large = max(rows, columns), large_padded = (large + 63) / 64 * 64;
+    const Resident x{lds, resident_pitch(large_padded)}, s{lds + kPadded * x.pitch, resident_pitch(kPadded)};
     const int64_t values = static_cast<int64_t>(rows) * columns;
     const G* const from = g + blockIdx.x * values;
+    // (where number `column` of row `row` is in memory)
+    const int row_step = tall ? 1 : columns, column_step = tall ? columns : 1;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), q4 = lane / 16 * 4, l16 = lane % 16;
     double squares = 0.0;
+#pragma unroll 8
     for (int i = static_cast<int>(threadIdx.x); i < values; i += kResidentThreads) {
         const double v = static_cast<double>(static_cast<float>(from[i]));
         squares += v * v;
     }
     const double factor = per_norm(workgroup_sum<kResidentThreads>(squares), k.eps);
-    for (int i = static_cast<int>(threadIdx.x); i < small_padded * large_padded; i += kResidentThreads) {
-        // (neighbouring lanes read neighbours in memory)
-        const int row = tall ? i % small_padded : i / large_padded, column = tall ? i / small_padded : i % large_padded;
-        const bool there = row < small && column < large;
-        x.store(row, column, there ? scaled(from[tall ? column * columns + row : row * columns + column], factor) : 0.0f);
+    // (a lane has eight numbers of a row; neighbouring lanes are neighbours in memory)
+    const int eights = large_padded / 8;
+#pragma unroll 2
+    for (int i = static_cast<int>(threadIdx.x); i < kPadded * eights; i += kResidentThreads) {
+        const int row = tall ? i % kPadded : i / eights, column = (tall ? i / kPadded : i % eights) * 8;
+        floats<8> v{};
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+            if (row < small && column + n < large) v[n] = scaled(from[row * row_step + (column + n) * column_step], factor);
+        x.store<8>(row, column, v);
     }
+    tile_acc own[kBlocks][kTiles];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+            const int row = n * 16 + l16, column = (b * kResidentWaves + wave) * 16 + q4;
+            own[b][n] = tile_acc{};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (row < small && column + i < large) own[b][n][i] = scaled(from[row * row_step + (column + i) * column_step], factor);
+        }
     __syncthreads();
-    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), q4 = lane / 16 * 4, l16 = lane % 16;
-    const int units_m = small_padded / 16, units = units_m * (small_padded / 32);
-    constexpr int kMostUnits = kMostSmall / 16 * (kMostSmall / 32) / kResidentWaves;
+    constexpr int kUnits = kTiles * kTiles / 2, kMostUnits = (kUnits + kResidentWaves - 1) / kResidentWaves;
     for (int step = 0; step < steps; ++step) {
         tile_acc of_s[kMostUnits][2];
 #pragma unroll
         for (int u = 0; u < kMostUnits; ++u) {
-            const int unit = u * kResidentWaves + wave, m = unit % units_m * 16, n = unit / units_m * 32;
-            if (unit >= units) continue;
+            const int unit = u * kResidentWaves + wave, m = unit % kTiles * 16, n = unit / kTiles * 32;
+            if (unit >= kUnits) continue;
             of_s[u][0] = of_s[u][1] = tile_acc{};
-            for (int line = 0; line < large_padded / 32; ++line) {
-                const chunk16 a = x.across(m, line, 0), a_low = x.across(m, line, 1);
+            for (int first = 0; first < large_padded / 32; first += 2) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) of_s[u][h] = multiply_split(a, a_low, x.across(n + 16 * h, line, 0), x.across(n + 16 * h, line, 1), of_s[u][h]);
+                for (int line = first; line < first + 2; ++line) {
+                    const chunk16 a = x.across(m, line, 0), a_low = x.across(m, line, 1);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) of_s[u][h] = multiply_split(a, a_low, x.across(n + 16 * h, line, 0), x.across(n + 16 * h, line, 1), of_s[u][h]);
+                }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 of_s[u][h] *= kPerScale;
-                s.store(n + 16 * h + l16, m + q4, of_s[u][h]);
+                s.store<4>(n + 16 * h + l16, m + q4, of_s[u][h]);
             }
         }
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < kMostUnits; ++u) {
-            const int unit = u * kResidentWaves + wave, m = unit % units_m * 16, n = unit / units_m * 32;
-            if (unit >= units) continue;
+            const int unit = u * kResidentWaves + wave, m = unit % kTiles * 16, n = unit / kTiles * 32;
+            if (unit >= kUnits) continue;
             tile_acc square[2] = {};
-            for (int line = 0; line < small_padded / 32; ++line) {
+#pragma unroll
+            for (int line = 0; line < kLines; ++line) {
                 const chunk16 a = s.across(m, line, 0), a_low = s.across(m, line, 1);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) square[h] = multiply_split(a, a_low, s.across(n + 16 * h, line, 0), s.across(n + 16 * h, line, 1), square[h]);
@@ -319,41 +382,49 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < kMostUnits; ++u) {
-            const int unit = u * kResidentWaves + wave, m = unit % units_m * 16, n = unit / units_m * 32;
-            if (unit >= units) continue;
+            const int unit = u * kResidentWaves + wave, m = unit % kTiles * 16, n = unit / kTiles * 32;
+            if (unit >= kUnits) continue;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) s.store(n + 16 * h + l16, m + q4, of_s[u][h]);
+            for (int h = 0; h < 2; ++h) s.store<4>(n + 16 * h + l16, m + q4, of_s[u][h]);
         }
         __syncthreads();
         const bool last = step + 1 == steps;
-        for (int m = wave * 16; m < large_padded; m += kResidentWaves * 16) {
-            constexpr int kMostTiles = kMostSmall / 16;
-            tile_acc acc[kMostTiles];
 #pragma unroll
-            for (int n = 0; n < kMostTiles; ++n) acc[n] = tile_acc{};
-            for (int line = 0; line < small_padded / 32; ++line) {
+        for (int b = 0; b < kBlocks; ++b) {
+            const int m = (b * kResidentWaves + wave) * 16;
+            if (m >= large_padded) continue;
+            tile_acc acc[kTiles] = {};
+#pragma unroll
+            for (int line = 0; line < kLines; ++line) {
                 const chunk16 a = x.along(line * 32, m, 0), a_low = x.along(line * 32, m, 1);
 #pragma unroll
-                for (int n = 0; n < kMostTiles; ++n)
-                    if (n * 16 < small_padded) acc[n] = multiply_split(a, a_low, s.across(n * 16, line, 0), s.across(n * 16, line, 1), acc[n]);
+                for (int n = 0; n < kTiles; ++n) acc[n] = multiply_split(a, a_low, s.across(n * 16, line, 0), s.across(n * 16, line, 1), acc[n]);
             }
 #pragma unroll
-            for (int n = 0; n < kMostTiles; ++n) {
-                if (n * 16 >= small_padded) continue;
-                const int row = n * 16 + l16, column = m + q4;
-                const tile_acc v = k.a * x.load(row, column) + acc[n] * kPerScale;
-                if (!last) {
-                    x.store(row, column, v);
-                } else if (row < small) {
-                    G* const to = result + blockIdx.x * values;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (column + i < large) to[tall ? (column + i) * columns + row : row * columns + column + i] = static_cast<G>(v[i] * kPerScale);
-                }
+            for (int n = 0; n < kTiles; ++n) {
+                own[b][n] = k.a * own[b][n] + acc[n] * kPerScale;
+                if (!last) x.store<4>(n * 16 + l16, m + q4, own[b][n]);
             }
         }
         __syncthreads();
     }
+    G* const to = result + blockIdx.x * values;
+    using Four = G __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+            const int row = n * 16 + l16, column = (b * kResidentWaves + wave) * 16 + q4;
+            const Four y = __builtin_convertvector(own[b][n] * kPerScale, Four);
+            if (row >= small || column >= large) continue;
+            if (!tall) {
+                store_values<G, 4>(to + row * columns + column, y, large - column);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (column + i < large) to[(column + i) * columns + row] = y[i];
+            }
+        }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -382,12 +453,31 @@ unsigned grid_of(int64_t n) { return static_cast<unsigned>(std::min<int64_t>((n 
 // ------------------------------------------------------------------------------------------
 // which kernels
 
-int64_t resident_bytes(int64_t small, int64_t large) {
-    if (small > kMostSmall || large > 1 << 12) return int64_t{1} << 40;
-    const int s = round_to_32(static_cast<int>(small)), l = round_to_32(static_cast<int>(large));
-    return static_cast<int64_t>(s) * (resident_pitch(l) + resident_pitch(s));
+// How many times 16 columns of X a wave may have, for 16 kTiles rows: what fits the LDS.
+template <int kTiles>
+constexpr int kMostBlocks = ((kMostResident / (16 * kTiles) - 16 * kTiles * 4) / 256 * 4 + kResidentWaves - 1) / kResidentWaves;
+
+bool is_resident(int64_t rows, int64_t columns) {
+    const int64_t small = std::min(rows, columns), large = std::max(rows, columns);
+    if (small > kMostSmall || large > 1 << 12) return false;
+    const int s = round_to_32(static_cast<int>(small)), l = (static_cast<int>(large) + 63) / 64 * 64;
+    return static_cast<int64_t>(s) * (resident_pitch(l) + resident_pitch(s)) <= kMostResident;
 }
-constexpr int kMostResident = 160 * 1024 - 256;
+
+template <class G>
+int resident(int64_t matrices, int64_t rows, int64_t columns, int steps, Coefficients k, const G* g, G* result, hipStream_t stream) {
+    const auto launch = [&](auto tiles) -> int {
+        constexpr int kTiles = decltype(tiles)::value;
+        resident_kernel<G, kTiles, kMostBlocks<kTiles>><<<static_cast<unsigned>(matrices), kResidentThreads, 0, stream>>>(static_cast<int>(rows), static_cast<int>(columns), steps,
+                                                                                                                          k, g, result);
+        return launched();
+    };
+    const int64_t small = std::min(rows, columns);
+    if (small <= 32) return launch(std::integral_constant<int, 2>{});
+    if (small <= 64) return launch(std::integral_constant<int, 4>{});
+    if (small <= 96) return launch(std::integral_constant<int, 6>{});
+    return launch(std::integral_constant<int, 8>{});
+}
 
 // The workspace of matrices that do not stay in the LDS.
 struct Layout {
@@ -438,7 +528,7 @@ int launch_step(StepArgs a, int64_t matrices, hipStream_t stream) {
     if constexpr (std::is_same_v<E, half_t>) {
         if (huge >= 128) return launch(std::common_type<Product<E, kAlongM, kAlongN, 256, 256, 4, 2, Chunks::kDirect>>{});
     }
-    if (large < 256) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, Chunks::kDirect>>{});
+    if (large < 256) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, Chunks::kDirect, 8>>{});
     return launch(std::common_type<Product<E, kAlongM, kAlongN, 128, 128, 2, 2, Chunks::kDirect>>{});
 }
 
@@ -449,8 +539,8 @@ int orthogonalise(int64_t matrices, int64_t rows, int64_t columns, int steps, Co
     double* const sums = reinterpret_cast<double*>(f + l.s);
     squares_kernel<G><<<static_cast<unsigned>(matrices * l.pieces), kThreads, 0, stream>>>(rows * columns, l.pieces, g, sums);
     if (const int rc = launched()) return rc;
-    const int64_t fours = rows * (l.padded / 4);
-    const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>((fours + kThreads - 1) / kThreads, std::max<int64_t>(1, 4096 / matrices)));
+    const int64_t eights = rows * (l.padded / 8);
+    const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>((eights + kThreads - 1) / kThreads, std::max<int64_t>(1, 4096 / matrices)));
     stage_kernel<E, G><<<static_cast<unsigned>(matrices * blocks), kThreads, 0, stream>>>(static_cast<int>(rows), static_cast<int>(columns), static_cast<int>(l.padded),
                                                                                          l.pieces, g, sums, k.eps, x, blocks);
     if (const int rc = launched()) return rc;
@@ -509,7 +599,7 @@ using namespace penc;
 extern "C" {
 
 size_t penc_orthogonalise_workspace_bytes(int type, int64_t matrices, int64_t rows, int64_t columns) {
-    if (bad_matrices(matrices, rows, columns) || resident_bytes(std::min(rows, columns), std::max(rows, columns)) <= kMostResident) return 0;
+    if (bad_matrices(matrices, rows, columns) || is_resident(rows, columns)) return 0;
     return type == PENC_BF16 ? layout_of<half_t>(matrices, rows, columns).total : layout_of<split_t>(matrices, rows, columns).total;
 }
 
@@ -529,17 +619,7 @@ int penc_orthogonalise(int type, int64_t matrices, int64_t rows, int64_t columns
         const hipStream_t s = static_cast<hipStream_t>(stream);
         const G* const from = static_cast<const G*>(update);
         G* const to = static_cast<G*>(result);
-        if (need == 0) {
-            const int64_t bytes = resident_bytes(std::min(rows, columns), std::max(rows, columns));
-            const auto launch = [&](auto size) -> int {
-                resident_kernel<G, decltype(size)::value><<<static_cast<unsigned>(matrices), kResidentThreads, 0, s>>>(static_cast<int>(rows), static_cast<int>(columns),
-                                                                                                                    steps, k, from, to);
-                return launched();
-            };
-            // (two workgroups to a compute unit, where they fit)
-            if (bytes <= kMostResident / 2) return launch(std::integral_constant<int, kMostResident / 2>{});
-            return launch(std::integral_constant<int, kMostResident>{});
-        }
+        if (need == 0) return resident<G>(matrices, rows, columns, steps, k, from, to, s);
         using E = std::conditional_t<std::is_same_v<G, bf16_t>, half_t, split_t>;
         return orthogonalise<E, G>(matrices, rows, columns, steps, k, from, to, static_cast<char*>(workspace), s);
     });

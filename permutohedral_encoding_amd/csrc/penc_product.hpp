@@ -252,8 +252,9 @@ __device__ __forceinline__ void wait_for_loads() {
 }
 
 // A workgroup of kWavesM x kWavesN waves, each with kM / kWavesM x kN / kWavesN results; kRing steps have room in the LDS.
-template <class E, bool kAlongM, bool kAlongN, int kM_, int kN_, int kWavesM, int kWavesN, Chunks kChunksCome, int kRing = 4>
+template <class E, bool kAlongM, bool kAlongN, int kM_, int kN_, int kWavesM_, int kWavesN_, Chunks kChunksCome, int kRing = 4>
 struct Product {
+    static constexpr int kWavesM = kWavesM_, kWavesN = kWavesN_;
     static constexpr int kM = kM_, kN = kN_, kThreads = 64 * kWavesM * kWavesN;
     static constexpr int kTilesM = kM / kWavesM / 16, kTilesN = kN / kWavesN / 16;
     using TileM = OperandTile<E, kAlongM, kM>;
@@ -398,6 +399,26 @@ struct Product {
             also(even.n[0]);
         }
         if constexpr (kDirect) wait_for_loads<0>();  // (nothing is on its way into the LDS when the workgroup ends)
+    }
+
+    // Calls f(m, n, v) for eight results m .. m + 7 of n at a time: lanes 16 apart have four neighbouring m each, and exchange those of two tiles.
+    template <class F>
+    __device__ __forceinline__ void each_eight(F&& f) const {
+        static_assert(kTilesM % 2 == 0);
+        using Eight = float __attribute__((ext_vector_type(8)));
+        const int lane = threadIdx.x % 64, g = lane / 16;
+#pragma unroll
+        for (int j = 0; j < kTilesN; ++j)
+#pragma unroll
+            for (int i = 0; i < kTilesM; i += 2) {
+                Eight v;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][j][r]), __float_as_uint(acc[i + 1][j][r]), false, false);
+                    v[r] = __uint_as_float(x[0]), v[4 + r] = __uint_as_float(x[1]);
+                }
+                f(wave_m() + 16 * (i + g % 2) + g / 2 * 8, wave_n() + 16 * j + lane % 16, v);
+            }
     }
 
     // Calls f(m, n, v) for the results of this lane: v of m .. m + 3 and n, within the tile.
