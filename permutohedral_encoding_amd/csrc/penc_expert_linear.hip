@@ -163,7 +163,8 @@ template <bool kBack, int kLines, int kTiles>
 __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_kernel(RowsArgs a, int most) {
     using Load = Loader<Value, kBack, 64, kNarrowThreads, Chunks::kDirect>;
     using Tile = typename Load::Tile;
-    __shared__ __attribute__((aligned(1024))) char lds[kLines * Tile::kSize];
+    static_assert(kLines % 2 == 0);
+    __shared__ __attribute__((aligned(1024))) char lds[kLines / 2 * Tile::kSize];
     const uint32_t item = a.spread.item();
     if (item >= a.spread.items) return;
     const RowTile t = row_tile<true>(a.offsets, a.experts, a.rows, item, most);
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_kernel(RowsArgs 
     Load load(kBack ? Operand{weight, static_cast<int64_t>(a.wide) * kSize, a.deep, a.wide * kSize} : Operand{weight, static_cast<int64_t>(a.deep) * kSize, a.wide, a.deep * kSize});
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
 #pragma unroll
-    for (int l = 0; l < kLines; ++l) load.begin(lds_at + l * Tile::kSize, 0);
+    for (int l = 0; l < kLines / 2; ++l) load.begin(lds_at + l * Tile::kSize);
 
     // this lane's chunks of a row, and of the rows of a group
     const int deep_bytes = a.deep * kSize, stride = static_cast<int>(a.stride) * kSize;
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_kernel(RowsArgs 
 #pragma unroll
     for (int l = 0; l < kLines; ++l)
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) w[i][l] = Tile::fragment(lds + l * Tile::kSize, 16 * i, 0);
+        for (int i = 0; i < kTiles; ++i) w[i][l] = Tile::fragment(lds + l / 2 * Tile::kSize, 16 * i, l % 2, 0);
     for (; row < t.rows; row += kStep) {
 #pragma unroll
         for (int k = 0; k < kNarrowGroups; ++k)

@@ -528,7 +528,7 @@ int launch_step(StepArgs a, int64_t matrices, hipStream_t stream) {
     if constexpr (std::is_same_v<E, half_t>) {
         if (huge >= 128) return launch(std::common_type<Product<E, kAlongM, kAlongN, 256, 256, 4, 2, Chunks::kDirect>>{});
     }
-    if (large < 256) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, Chunks::kDirect, 8>>{});
+    if (large < 256) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, Chunks::kDirect, 4>>{});
     return launch(std::common_type<Product<E, kAlongM, kAlongN, 128, 128, 2, 2, Chunks::kDirect>>{});
 }
 

@@ -1,21 +1,21 @@
 // Matrix products of a workgroup: D[m][n] = sum over k of A[m][k] B[n][k], for a tile of kM x kN results that stay in the registers of its waves.
 //
-// Operands come in steps of k through the LDS, up to three steps on their way while one is multiplied, and its fragments are read from the LDS while the one before is.
-// An operand is
+// Operands come in steps of k through the LDS; one or more steps are on their way while one is multiplied, and the fragments of each half of a step are read from the LDS while the half
+// before is.  An operand is
 //
-//     Across   rows of adjacent k: 64 bytes of each row in a step, 32 k of a 16-bit type and 16 of fp32
+//     Across   rows of adjacent k: 128 bytes of each row in a step, 64 k of a 16-bit type and 32 of fp32
 //     Along    rows of one k, adjacent in m (or n): as many k in a step, transposed on the way from the LDS into registers
 //
 // 16-bit types are multiplied by v_mfma_f32_16x16x32, fp32 by v_mfma_f32_16x16x4_f32.  A Split number is two halves, hi = the nearest to x and lo = the nearest to x - hi
-// (22 bits of x together, where x - hi is no less than 2^-14): of every 32 numbers the hi and behind them the lo, 128 bytes in a step; a product is
+// (22 bits of x together, where x - hi is no less than 2^-14): of every 32 numbers the hi and behind them the lo, twice 128 bytes in a step; a product is
 // hi hi + hi lo + lo hi, and what is left out is 2^-22 of it.
 //
 // Chunks of 16 bytes go from memory into the LDS directly, where rows and their ends are on 16 bytes.  Where a chunk stands in the LDS is fixed by the lane that brings it, so
 // a lane brings the chunk that belongs there.  Addresses behind an operand's end (rows, k, or columns) read zeros, which the buffer's bounds see to.  Of rows that begin anywhere,
-// lanes load chunks into registers and write them into the LDS two steps later; where a row ends, its last 16 bytes, of which what the chunk does not have is moved out then.
+// lanes load chunks into registers and write them into the LDS a step later; where a row ends, its last 16 bytes, of which what the chunk does not have is moved out then.
 //
 // Where a chunk stands: a read of 16 bytes takes 8 lanes at a time, one of 8 bytes 16 and one of 4 bytes 32, which should meet the 32 banks of 4 bytes once.  Across: lanes read one chunk c
-// of 8 rows; c stands at c ^ (row / 2 mod 4) (of 128 bytes: row mod 8).  Along: 16 lanes read 32 bytes (fp32: 64) of each of 4 neighbouring k (fp32: 32 lanes of two k, 4 apart);
+// of 8 rows; c stands at c ^ (row mod 8).  Along: 16 lanes read 32 bytes (fp32: 64) of each of 4 neighbouring k (fp32: 32 lanes of two k, 4 apart);
 // pieces of 32 (64) bytes are permuted by these bits of k.
 #pragma once
 
@@ -36,19 +36,19 @@ struct split_t {
 template <class E>
 struct ProductType {
     static constexpr int kBytes = 2;   // of a number
-    static constexpr int kDepth = 32;  // k of a step
-    static constexpr int kParts = 1;   // fragments of 16 rows of a step
+    static constexpr int kDepth = 64;  // k of a step
+    static constexpr int kParts = 1;   // fragments of 16 rows and half a step
 };
 template <>
 struct ProductType<float> {
     static constexpr int kBytes = 4;
-    static constexpr int kDepth = 16;
+    static constexpr int kDepth = 32;
     static constexpr int kParts = 1;
 };
 template <>
 struct ProductType<split_t> {
     static constexpr int kBytes = 4;
-    static constexpr int kDepth = 32;
+    static constexpr int kDepth = 64;
     static constexpr int kParts = 2;
 };
 
@@ -92,23 +92,23 @@ struct OperandTile {
 
     // where chunk c of a row stands in it
     __device__ __forceinline__ static int place(int row, int c) {
-        if constexpr (!kAlong) return kLine == 64 ? c ^ (row >> 1 & 3) : c ^ (row & 7);
+        if constexpr (!kAlong) return c ^ (row & 7);
         else if constexpr (std::is_same_v<E, float>) return c ^ (row >> 2 & 3) << 2;
         else if constexpr (kRowBytes >= 256) return c ^ ((row & 3) | (row >> 3 & 1) << 2) << 1;
         else return c ^ ((row >> 1 & 1) | (row >> 3 & 1) << 1) << 1;
     }
 
-    // 16 rows (columns) from `at` on, as the matrix instruction takes them: lane 16 g + i has row i.  Split: hi (part 0) or lo.
-    __device__ __forceinline__ static chunk16 fragment(const char* lds, int at, int part) {
+    // 16 rows (columns) from `at` on, of half a step, as the matrix instruction takes them: lane 16 g + i has row i.  Split: hi (part 0) or lo.
+    __device__ __forceinline__ static chunk16 fragment(const char* lds, int at, int half, int part) {
         const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
         if constexpr (!kAlong) {
             const int row = at + i;
-            return *reinterpret_cast<const chunk16*>(lds + row * kLine + place(row, part * 4 + g) * 16);
+            return *reinterpret_cast<const chunk16*>(lds + row * kLine + place(row, half * (4 * T::kParts) + part * 4 + g) * 16);
         } else if constexpr (std::is_same_v<E, float>) {
             chunk16 f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int row = g * 4 + j, column = at + i;
+                const int row = half * 16 + g * 4 + j, column = at + i;
                 f[j] = *reinterpret_cast<const uint32_t*>(lds + row * kRowBytes + place(row, column / 4) * 16 + column % 4 * 4);
             }
             return f;
@@ -119,7 +119,7 @@ struct OperandTile {
             chunk16 f;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int row = g * 8 + h * 4 + i / 4;
+                const int row = half * 32 + g * 8 + h * 4 + i / 4;
                 const V v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(lds + row * kRowBytes + place(row, byte / 16) * 16 + byte % 16));
                 const uint2 w = __builtin_bit_cast(uint2, v);
                 f[2 * h] = w.x, f[2 * h + 1] = w.y;
@@ -171,7 +171,7 @@ struct Loader {
     int rows, wide;     // of the operand; bytes of a row (Along)
     int at[kDirect ? kEach : 1];  // of this lane's chunks from `first` on
     int byte;                     // Across: in a row
-    chunk16 held[kDirect ? 1 : 2][kDirect ? 1 : kEach];  // two steps
+    chunk16 held[kDirect ? 1 : kEach];
 
     __device__ __forceinline__ static int slot_of(int j) { return j * kThreads + static_cast<int>(threadIdx.x); }
     __device__ __forceinline__ static int row_of(int j) { return slot_of(j) / Tile::kRowChunks; }
@@ -187,8 +187,8 @@ struct Loader {
         }
     }
 
-    // The chunks of the next step are on their way, into the LDS or into registers (`hold`: which).
-    __device__ __forceinline__ void begin(uint32_t lds, int hold) {
+    // The chunks of the next step are on their way, into the LDS or into registers.
+    __device__ __forceinline__ void begin(uint32_t lds) {
         if constexpr (kDirect) {
             const int there = left <= 0 ? 0 : kAlong ? min(left, T::kDepth) * stride + rest : rest + left;
             const uint64_t p = reinterpret_cast<uint64_t>(first);
@@ -202,7 +202,7 @@ struct Loader {
             for (int j = 0; j < kEach; ++j) {
                 using Unaligned = uint32_t __attribute__((ext_vector_type(4), aligned(T::kBytes == 2 ? 2 : 4)));
                 const int row = min(row_of(j), (kAlong ? left : rows) - 1), in_row = min(byte_of(j), (kAlong ? wide : left) - 16);
-                held[hold][j] = *reinterpret_cast<const Unaligned*>(first + (static_cast<int64_t>(row) * stride + in_row));
+                held[j] = *reinterpret_cast<const Unaligned*>(first + (static_cast<int64_t>(row) * stride + in_row));
             }
         } else {
 #pragma unroll
@@ -219,27 +219,27 @@ struct Loader {
                         if (4 * w + 2 < n) v[w] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + 4 * w + 2)) << 16;
                     }
                 }
-                held[hold][j] = v;
+                held[j] = v;
             }
         }
         first += step_bytes;
         left -= kAlong ? T::kDepth : Tile::kLine;
     }
-    // What was held two steps ago goes into the LDS (a barrier makes it so for the other waves).
-    __device__ __forceinline__ void end(char* lds, int hold) {
+    // What is held goes into the LDS (a barrier makes it so for the other waves).
+    __device__ __forceinline__ void end(char* lds) {
         if constexpr (!kDirect) {
             if constexpr (kChunksCome == Chunks::kHeld) {
-                const int there = left + 2 * (kAlong ? T::kDepth : Tile::kLine);  // as it was
+                const int there = left + (kAlong ? T::kDepth : Tile::kLine);  // as it was
                 if (kAlong ? there < T::kDepth || wide < Tile::kRowBytes : there < Tile::kLine) {
 #pragma unroll
                     for (int j = 0; j < kEach; ++j) {
                         const int in_row = (kAlong ? wide : there) - byte_of(j);
-                        held[hold][j] = to_front(held[hold][j], kAlong && row_of(j) >= there ? 16 : min(max(16 - in_row, 0), 16));
+                        held[j] = to_front(held[j], kAlong && row_of(j) >= there ? 16 : min(max(16 - in_row, 0), 16));
                     }
                 }
             }
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) *reinterpret_cast<chunk16*>(lds + slot_of(j) * 16) = held[hold][j];
+            for (int j = 0; j < kEach; ++j) *reinterpret_cast<chunk16*>(lds + slot_of(j) * 16) = held[j];
         }
     }
 };
@@ -252,7 +252,7 @@ __device__ __forceinline__ void wait_for_loads() {
 }
 
 // A workgroup of kWavesM x kWavesN waves, each with kM / kWavesM x kN / kWavesN results; kRing steps have room in the LDS.
-template <class E, bool kAlongM, bool kAlongN, int kM_, int kN_, int kWavesM_, int kWavesN_, Chunks kChunksCome, int kRing = 4>
+template <class E, bool kAlongM, bool kAlongN, int kM_, int kN_, int kWavesM_, int kWavesN_, Chunks kChunksCome, int kRing = 2>
 struct Product {
     static constexpr int kWavesM = kWavesM_, kWavesN = kWavesN_;
     static constexpr int kM = kM_, kN = kN_, kThreads = 64 * kWavesM * kWavesN;
@@ -267,22 +267,22 @@ struct Product {
     static constexpr int kDepth = ProductType<E>::kDepth, kParts = ProductType<E>::kParts;
     static constexpr int kLoads = LoadM::kEach + LoadN::kEach;  // of a lane, for a step
 
-    // What a wave multiplies in a step.
+    // What a wave multiplies in half a step.
     struct Fragments {
         chunk16 m[kParts][kTilesM], n[kParts][kTilesN];
 
-        __device__ __forceinline__ void read(const char* lds) {
+        __device__ __forceinline__ void read(const char* lds, int half) {
 #pragma unroll
             for (int p = 0; p < kParts; ++p) {
 #pragma unroll
-                for (int j = 0; j < kTilesN; ++j) n[p][j] = TileN::fragment(lds + TileM::kSize, wave_n() + 16 * j, p);
+                for (int j = 0; j < kTilesN; ++j) n[p][j] = TileN::fragment(lds + TileM::kSize, wave_n() + 16 * j, half, p);
 #pragma unroll
-                for (int i = 0; i < kTilesM; ++i) m[p][i] = TileM::fragment(lds, wave_m() + 16 * i, p);
+                for (int i = 0; i < kTilesM; ++i) m[p][i] = TileM::fragment(lds, wave_m() + 16 * i, half, p);
             }
         }
     };
 
-    // Reads of the LDS of a step, and products.
+    // Reads of the LDS of half a step, and products.
     template <bool kAlong>
     static constexpr int kReadsOf = !kAlong ? 1 : std::is_same_v<E, float> ? 4 : 2;
     static constexpr int kReads = kParts * (kTilesM * kReadsOf<kAlongM> + kTilesN * kReadsOf<kAlongN>);
@@ -306,7 +306,7 @@ struct Product {
 #pragma unroll
             for (int j = 0; j < kTilesN; ++j) acc[i][j] = multiply<Part>(m[i], n[j], acc[i][j]);
     }
-    __device__ __forceinline__ void multiply_step(const Fragments& f) {
+    __device__ __forceinline__ void multiply_half(const Fragments& f) {
         if constexpr (kParts == 2) {
             multiply_all(f.m[0], f.n[1]);
             multiply_all(f.m[1], f.n[0]);
@@ -335,22 +335,18 @@ struct Product {
         LoadM load_m(m);
         LoadN load_n(n);
         // Steps behind the last one are loaded too, and are zeros: each wave always has as many loads on their way.
-        constexpr int kAhead = kRing - 1;
         const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-        int room = 0, read = 0;  // where the next step goes, and where the next fragments are
-        const auto begin = [&](int hold) {
-            load_m.begin(lds_at + room, hold);
-            load_n.begin(lds_at + room + TileM::kSize, hold);
-            if constexpr (kDirect) room = room + kStage == kLds ? 0 : room + kStage;
+        int room = 0, here = 0;  // where the next step goes, and the present one is
+        const auto behind = [](int at) { return at + kStage == kLds ? 0 : at + kStage; };
+        const auto begin = [&] {
+            load_m.begin(lds_at + room);
+            load_n.begin(lds_at + room + TileM::kSize);
+            if constexpr (kDirect) room = behind(room);
         };
-        const auto end = [&](int hold) {
-            load_m.end(lds + room, hold);
-            load_n.end(lds + room + TileM::kSize, hold);
-            if constexpr (!kDirect) room = room + kStage == kLds ? 0 : room + kStage;
-        };
-        const auto fragments = [&](Fragments& f) {
-            f.read(lds + read);
-            read = read + kStage == kLds ? 0 : read + kStage;
+        const auto end = [&] {
+            load_m.end(lds + room);
+            load_n.end(lds + room + TileM::kSize);
+            room = behind(room);
         };
         const auto meet = [&] {
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -359,45 +355,40 @@ struct Product {
         };
         if constexpr (kDirect) {
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) begin(0);
+            for (int k = 0; k < kRing; ++k) begin();
             start(first);
-            wait_for_loads<kLoads * (kAhead - 1)>();
+            wait_for_loads<kLoads * (kRing - 1)>();
         } else {
-            static_assert(kRing == 4);
-            begin(0);
-            begin(1);
+            static_assert(kRing == 2);
+            begin();
             start(first);
-            end(0);
-            begin(0);
-            end(1);
-            begin(1);
+            end();
+            begin();
         }
         meet();
         Fragments even, odd;
-        fragments(even);
-        // In step i: what is brought for step i + 1 is there for all waves, and the fragments of step i - 1, whose room step i + kAhead takes, have been read.
-        // (Held in registers: steps i + 2, which goes into the LDS, and i + 3, and then i + 3 and i + 4.)
-        const auto turn = [&](const Fragments& now, Fragments& next, int hold) {
-            if constexpr (kDirect) wait_for_loads<kLoads * (kAhead - 2)>();
-            meet();
-            if constexpr (!kDirect) end(hold);
-            begin(hold);
+        even.read(lds, 0);
+        const auto turn = [&](const Fragments& now, Fragments& next, const char* from, int half) {
             __builtin_amdgcn_sched_barrier(0);
-            fragments(next);
-            multiply_step(now);
+            next.read(from, half);
+            multiply_half(now);
             also(now.n[0]);
             alternate(std::make_index_sequence<kReads>{});
             __builtin_amdgcn_sched_barrier(0);
         };
-        int i = 0;
-        for (; i + 1 < steps; i += 2) {
-            turn(even, odd, 0);
-            turn(odd, even, 1);
+        for (int step = 1; step < steps; ++step) {
+            turn(even, odd, lds + here, 1);
+            // What is brought for the next step is there for all waves, and all have read the second half of this one, whose room the step kRing behind it takes.
+            if constexpr (kDirect) wait_for_loads<kLoads * (kRing - 2)>();
+            else end();
+            meet();
+            begin();
+            here = behind(here);
+            turn(odd, even, lds + here, 0);
         }
-        if (i < steps) {
-            multiply_step(even);
-            also(even.n[0]);
-        }
+        turn(even, odd, lds + here, 1);
+        multiply_half(odd);
+        also(odd.n[0]);
         if constexpr (kDirect) wait_for_loads<0>();  // (nothing is on its way into the LDS when the workgroup ends)
     }
 
