@@ -21,6 +21,7 @@ namespace {
 
 using Value = std::conditional_t<PENC_TYPE == PENC_FP32, float, std::conditional_t<PENC_TYPE == PENC_FP16, half_t, bf16_t>>;
 constexpr int kSize = sizeof(Value);
+static_assert(PENC_MAX_EXPERT_STRIDE * kSize <= kMostOperandStride && PENC_MAX_EXPERT_CHANNELS * kSize <= kMostOperandStride);
 
 // The sum of a wave's values up to each lane.
 __device__ __forceinline__ uint32_t sum_to_lane(uint32_t v) {
@@ -73,6 +74,19 @@ __device__ __forceinline__ RowTile row_tile(const int32_t* __restrict__ offsets,
     return {-1, 0, 0, 0, 0};
 }
 
+// How many tiles row_tile<true> has.
+__device__ __forceinline__ uint32_t row_tiles(const int32_t* __restrict__ offsets, int experts, int rows, int most) {
+    const int lane = threadIdx.x % 64;
+    uint32_t tiles = 0;
+    for (int e = lane; e <= experts; e += 64) {
+        const int from = min(max(offsets[e], 0), rows), to = e < experts ? min(max(offsets[e + 1], 0), rows) : rows;
+        tiles += (static_cast<uint32_t>(max(to - from, 0)) + most - 1) / most;
+    }
+    return __builtin_amdgcn_readlane(sum_to_lane(tiles), 63);
+}
+
+constexpr uint32_t kUnits = 256;  // compute units
+
 struct RowsArgs {
     const void *rows_in, *weight, *bias;
     void* rows_out;
@@ -85,19 +99,11 @@ struct RowsArgs {
 
 constexpr uint32_t kGroup = 8;
 
-// y (kBack false: weights by rows of k) or dx.
+// A tile of results: those of P::kN rows from `skip` rows into t on, and P::kM columns from m0 on.
 template <bool kBack, class P>
-__global__ __launch_bounds__(P::kThreads) void expert_rows_kernel(RowsArgs a) {
-    __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
-    // eight tiles of rows to each tile of weights, one after the other: what a die works on at a time fits its cache
-    const uint32_t item = a.spread.item(), of_group = kGroup * a.tiles, group = item / of_group, in_group = item % of_group;
-    if (item >= a.spread.items) return;
-    const uint32_t grouped = min(kGroup, a.spread.items / a.tiles - group * kGroup);
-    const RowTile t = row_tile<true>(a.offsets, a.experts, a.rows, group * kGroup + in_group % grouped, P::kN);
-    if (t.expert < 0) return;
-    const int m0 = static_cast<int>(in_group / grouped) * P::kM;
+__device__ __forceinline__ void rows_tile(const RowsArgs& a, char* lds, const RowTile& t, int skip, int m0) {
     P p;
-    const int columns = a.wide - m0;
+    const int columns = a.wide - m0, first_row = t.first + skip, rows = t.rows - skip;
     if (t.expert == a.experts) {
         p.start(P::kZero);
     } else {
@@ -106,7 +112,7 @@ __global__ __launch_bounds__(P::kThreads) void expert_rows_kernel(RowsArgs a) {
         const int m_rows = min(columns, P::kM);
         const Operand m = kBack ? Operand{weight + static_cast<int64_t>(m0) * kSize, static_cast<int64_t>(a.wide) * kSize, a.deep, m_rows * kSize}
                                 : Operand{weight + static_cast<int64_t>(m0) * a.deep * kSize, static_cast<int64_t>(a.deep) * kSize, m_rows, a.deep * kSize};
-        const Operand n{static_cast<const char*>(a.rows_in) + static_cast<int64_t>(t.first) * a.stride * kSize, a.stride * kSize, t.rows, a.deep * kSize};
+        const Operand n{static_cast<const char*>(a.rows_in) + static_cast<int64_t>(first_row) * a.stride * kSize, a.stride * kSize, min(rows, P::kN), a.deep * kSize};
         const auto first = [&](int m) {
             tile_acc v{};
             if (bias != nullptr) {
@@ -117,7 +123,40 @@ __global__ __launch_bounds__(P::kThreads) void expert_rows_kernel(RowsArgs a) {
         };
         p.run(lds, m, n, a.deep, first, P::kNothing);
     }
-    store_rows(p, static_cast<Value*>(a.rows_out) + static_cast<int64_t>(t.first) * a.wide + m0, a.wide, t.rows, columns);
+    store_rows(p, static_cast<Value*>(a.rows_out) + static_cast<int64_t>(first_row) * a.wide + m0, a.wide, rows, columns);
+}
+
+// kSplit: with as many tiles as compute units, or twice or three times as many, and a few more, those few take as long as all before them; where the last round has at most half of the compute
+// units, its tiles go in quarters, which then are one round or two of a third of the time (32768 x 4096 by 1024 bf16, 544 tiles: 310 -> 250 us).
+template <bool kBack, class P, class Quarter>
+__global__ __launch_bounds__(P::kThreads) void expert_rows_kernel(RowsArgs a) {
+    constexpr bool kSplit = !std::is_same_v<P, Quarter>;
+    __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
+    const uint32_t item = a.spread.item();
+    if (item >= a.spread.items) return;
+    uint32_t tile = item, quarter = 0, tiles = a.spread.items;
+    bool whole = true;
+    if constexpr (kSplit) {
+        static_assert(Quarter::kM * 2 == P::kM && Quarter::kN * 2 == P::kN && Quarter::kThreads == P::kThreads && Quarter::kLds <= P::kLds);
+        tiles = row_tiles(a.offsets, a.experts, a.rows, P::kN) * a.tiles;
+        const uint32_t last = tiles % kUnits;
+        if (last <= kUnits / 2 && item >= tiles - last) {
+            whole = false;
+            tile = tiles - last + (item - (tiles - last)) / 4, quarter = (item - (tiles - last)) % 4;
+        }
+        if (tile >= tiles) return;
+    }
+    // eight tiles of rows to each tile of weights, one after the other: what a die works on at a time fits its cache
+    const uint32_t of_group = kGroup * a.tiles, group = tile / of_group, in_group = tile % of_group, grouped = min(kGroup, tiles / a.tiles - group * kGroup);
+    const RowTile t = row_tile<true>(a.offsets, a.experts, a.rows, group * kGroup + in_group % grouped, P::kN);
+    if (t.expert < 0) return;
+    const int m0 = static_cast<int>(in_group / grouped) * P::kM;
+    if (whole) {
+        rows_tile<kBack, P>(a, lds, t, 0, m0);
+    } else {
+        const int skip = static_cast<int>(quarter / 2) * Quarter::kN, m1 = m0 + static_cast<int>(quarter % 2) * Quarter::kM;
+        if (skip < t.rows && m1 < a.wide) rows_tile<kBack, Quarter>(a, lds, t, skip, m1);
+    }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -189,7 +228,7 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_kernel(RowsArgs 
 #pragma unroll
     for (int l = 0; l < kLines; ++l) {
         const int byte = l * 64 + lane / 16 * 16;
-        at[l] = byte < deep_bytes ? lane % 16 * stride + byte : -1;
+        at[l] = byte < deep_bytes ? lane % 16 * stride + byte : kNowhere;
     }
     const char* const in = static_cast<const char*>(a.rows_in) + static_cast<int64_t>(t.first) * a.stride * kSize;
     chunk16 rows[kNarrowGroups][kLines], next[kNarrowGroups][kLines];
@@ -267,9 +306,9 @@ __global__ __launch_bounds__(kFewThreads) void expert_few_kernel(RowsArgs a) {
             for (int l = 0; l < kAhead; ++l) {
                 const int byte = first + l * kFewWaves * 64;
                 const bool there = byte + lane / 16 * 16 < deep_bytes;
-                x[l] = load_chunk16(rows, there ? x_at + byte : -1);
+                x[l] = load_chunk16(rows, there ? x_at + byte : kNowhere);
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i) w[l][i] = load_chunk16(weights, there ? w_at + 16 * i * deep_bytes + byte : -1);
+                for (int i = 0; i < kTiles; ++i) w[l][i] = load_chunk16(weights, there ? w_at + 16 * i * deep_bytes + byte : kNowhere);
             }
 #pragma unroll
             for (int l = 0; l < kAhead; ++l)
@@ -386,7 +425,20 @@ __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, 
     if (mine <= 1) return;
     const int64_t weights = static_cast<int64_t>(a.outputs) * a.channels, n = weights + (a.bias != nullptr ? a.outputs : 0);
     const int slice = static_cast<int>(threadIdx.x) / kResults, result = static_cast<int>(threadIdx.x) % kResults;
-    for (int64_t begin = static_cast<int64_t>(blockIdx.x % blocks) * kResults; begin < n; begin += static_cast<int64_t>(blocks) * kResults) {
+    // (a lane has kWide results: with one slice four, where those of every piece and expert begin on four)
+    constexpr int kWide = kSlices == 1 ? 4 : 1;
+    const bool fours = kWide == 4 && weights % 4 == 0;
+    if (fours) {
+        using Four = float __attribute__((ext_vector_type(4)));
+        for (int64_t i = (static_cast<int64_t>(blockIdx.x % blocks) * kResults + result) * 4; i < weights; i += static_cast<int64_t>(blocks) * kResults * 4) {
+            const float* const from = a.sums + first * weights + i;
+            Four sum{};
+#pragma unroll 4
+            for (uint32_t k = 0; k < mine; ++k) sum += *reinterpret_cast<const Four*>(from + k * weights);
+            store_values<Value, 4>(static_cast<Value*>(a.weight) + e * weights + i, __builtin_convertvector(sum, Value __attribute__((ext_vector_type(4)))), 4);
+        }
+    }
+    for (int64_t begin = static_cast<int64_t>(blockIdx.x % blocks) * kResults + (fours ? weights : 0); begin < n; begin += static_cast<int64_t>(blocks) * kResults) {
         const int64_t i = begin + result;
         const bool there = i < n, weight = i < weights;
         const int64_t each = weight ? weights : a.outputs, at = weight ? i : i - weights;
@@ -423,13 +475,13 @@ constexpr int64_t kMostThreads = (int64_t{1} << 32) - (1 << 18);
 // The most tiles of `most` rows that there are.
 int64_t row_tiles(const RowsArgs& a, int most) { return a.rows / most + std::min(a.experts, a.rows) + 1; }
 
-template <bool kBack, class P>
+template <bool kBack, class P, class Quarter = P>
 int launch_rows(RowsArgs a, hipStream_t stream) {
     a.tiles = static_cast<uint32_t>((a.wide + P::kM - 1) / P::kM);
-    const int64_t items = row_tiles(a, P::kN) * a.tiles;
+    const int64_t items = row_tiles(a, P::kN) * a.tiles + (std::is_same_v<P, Quarter> ? 0 : 3 * kUnits / 2);
     if (items * P::kThreads >= kMostThreads) return PENC_ERR_BAD_LAYER_SIZE;
     a.spread = Spread(items, 32);
-    expert_rows_kernel<kBack, P><<<a.spread.grid(), P::kThreads, 0, stream>>>(a);
+    expert_rows_kernel<kBack, P, Quarter><<<a.spread.grid(), P::kThreads, 0, stream>>>(a);
     return launched();
 }
 
@@ -470,7 +522,7 @@ int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
     if constexpr (kChunks != Chunks::kSingle) {
         if constexpr (kChunks == Chunks::kDirect && kSize == 2) {
             if (static_cast<int64_t>(a.rows / 256 + a.experts) * ((a.wide + 255) / 256) >= 512)
-                return launch_rows<kBack, Product<Value, kBack, false, 256, 256, 4, 2, kChunks>>(a, stream);
+                return launch_rows<kBack, Product<Value, kBack, false, 256, 256, 4, 2, kChunks>, Product<Value, kBack, false, 128, 128, 4, 2, kChunks>>(a, stream);
         }
         return launch_rows<kBack, Product<Value, kBack, false, 128, 128, 2, 2, kChunks>>(a, stream);
     }
@@ -561,7 +613,7 @@ int expert_weights<PENC_TYPE>(int64_t rows, int experts, int64_t channels, int64
     // (many pieces: a few results, and lanes that share them)
     const auto sum = [&](auto slices) -> int {
         constexpr int kSlices = decltype(slices)::value, kResults = kSumThreads / kSlices;
-        const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>((results + kResults - 1) / kResults, std::max<int64_t>(1, 65536 / experts)));
+        const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>((results + kResults - 1) / kResults, std::max<int64_t>(16, 8192 / experts)));
         expert_sums_kernel<kSlices><<<static_cast<uint32_t>(experts) * blocks, kSumThreads, 0, stream>>>(a, blocks);
         return launched();
     };

@@ -78,7 +78,8 @@ struct Operand {
     int bytes;       // of a row from `first` on: Across: of k; Along: of columns
 };
 
-constexpr int kMostOperandStride = 1 << 24;  // bytes: 256 rows are within a buffer's 2^32
+constexpr int kMostOperandStride = 1 << 22;  // bytes: 256 rows end before kNowhere
+constexpr int kNowhere = 1 << 30;            // behind every buffer's end
 
 // kAlong; kWide: rows (Across) or columns (Along) of the tile.
 template <class E, bool kAlong, int kWide>
@@ -129,11 +130,11 @@ struct OperandTile {
     }
 };
 
-// 16 bytes to each lane from buffer + at, to the LDS from `to` on, lane after lane.  (Not the builtin: of that the compiler knows that it writes to the LDS, but not where, and has every
+// 16 bytes to each lane from buffer + at + more, to the LDS from `to` on, lane after lane.  (Not the builtin: of that the compiler knows that it writes to the LDS, but not where, and has every
 // read of the LDS wait for it.  It has no result: what it brings is waited for by wait_for_loads.  The wait states are those that a scalar register written by a vector
 // instruction needs before it is an address, and M0 before it is used.)
-__device__ __forceinline__ void load_to_lds(__attribute__((ext_vector_type(4))) uint32_t buffer, int at, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(to), "v"(at), "s"(buffer) : "memory");
+__device__ __forceinline__ void load_to_lds(__attribute__((ext_vector_type(4))) uint32_t buffer, int at, int more, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(to), "v"(at), "s"(buffer), "s"(more) : "memory");
 }
 
 // What is the same in all lanes, in a scalar register (the compiler does not see it of all that is computed from a division).
@@ -169,8 +170,11 @@ struct Loader {
     int left;           // Across: bytes of a row, Along: rows
     int stride, rest;   // rest: what the buffer has beside: Across: the rows before the last, Along: how much longer a row is than they are apart
     int rows, wide;     // of the operand; bytes of a row (Along)
-    int at[kDirect ? kEach : 1];  // of this lane's chunks from `first` on
-    int byte;                     // Across: in a row
+    // this lane's chunks from `first` on: rows kSameRows apart, where a chunk stands alike in those (else each has its own)
+    static constexpr int kSameRows = kThreads / Tile::kRowChunks;
+    static constexpr bool kSame = kSameRows % 16 == 0;
+    int at[kDirect && !kSame ? kEach : 1];
+    int byte;  // Across: in a row
     chunk16 held[kDirect ? 1 : kEach];
 
     __device__ __forceinline__ static int slot_of(int j) { return j * kThreads + static_cast<int>(threadIdx.x); }
@@ -180,10 +184,11 @@ struct Loader {
     __device__ __forceinline__ explicit Loader(const Operand& o)
         : first(reinterpret_cast<const char*>(uniform(reinterpret_cast<int64_t>(o.first)))), step_bytes(kAlong ? T::kDepth * uniform(o.stride) : Tile::kLine),
           left(uniform(kAlong ? o.rows : o.bytes)), stride(uniform(static_cast<int>(o.stride))), rest(kAlong ? uniform(o.bytes) - stride : uniform(o.rows - 1) * stride),
-          rows(uniform(o.rows)), wide(uniform(o.bytes)), byte(byte_of(0)) {  // (byte: the same for all chunks: kThreads / kRowChunks rows are a whole number of permutations)
+          rows(uniform(o.rows)), wide(uniform(o.bytes)), byte(byte_of(0)) {
+        static_assert(kAlong || kSameRows % 8 == 0);
         if constexpr (kDirect) {
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) at[j] = kAlong && byte_of(j) >= wide ? -1 : row_of(j) * stride + byte_of(j);
+            for (int j = 0; j < (kSame ? 1 : kEach); ++j) at[j] = kAlong && byte_of(j) >= wide ? kNowhere : row_of(j) * stride + byte_of(j);
         }
     }
 
@@ -195,7 +200,10 @@ struct Loader {
             const __attribute__((ext_vector_type(4))) uint32_t buffer = {static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xFFFFu, static_cast<uint32_t>(there), 0x00020000u};
             const uint32_t to = lds + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * 1024;
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) load_to_lds(buffer, kAlong || byte < left ? at[j] : -1, to + j * kThreads * 16);
+            for (int j = 0; j < kEach; ++j) {
+                const int from = at[kSame ? 0 : j];
+                load_to_lds(buffer, kAlong || byte < left ? from : kNowhere, kSame ? j * kSameRows * stride : 0, to + j * kThreads * 16);
+            }
         } else if constexpr (kChunksCome == Chunks::kHeld) {
             // (loads have no conditions: where there is nothing, the operand's last row or a row's last 16 bytes are read)
 #pragma unroll
