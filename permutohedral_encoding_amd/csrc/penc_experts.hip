@@ -19,7 +19,7 @@
 namespace penc {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kLog2Threads = 8;
 constexpr int kWave = 64;
 
 // ------------------------------------------------------------------------------------------
@@ -51,20 +51,47 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return key == 0xFFFFFFFFu ? __builtin_nanf("") : __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-// A lane of kLanes has 8 kChunks consecutive logits of a row.
+// A lane of kLanes has 8 kChunks logits of a row, in pieces of 16 bytes: neighbouring lanes have neighbouring pieces.
 template <class E, int kLanes, int kChunks>
 struct LogitRow {
-    static constexpr int kValues = kChunk * kChunks;
+    static constexpr int kWide = 16 / sizeof(E), kPieces = kChunk * kChunks / kWide, kValues = kWide * kPieces;
+    using Unaligned = E __attribute__((ext_vector_type(kWide), aligned(sizeof(E))));
     float v[kValues];
-    int first;
 
-    __device__ __forceinline__ LogitRow(const E* __restrict__ row, int experts) : first(static_cast<int>(threadIdx.x) % kLanes * kValues) {
+    // where value i is in the row
+    __device__ __forceinline__ static int index_of(int i) { return (i / kWide * kLanes + static_cast<int>(threadIdx.x) % kLanes) * kWide + i % kWide; }
+
+    __device__ __forceinline__ LogitRow(const E* __restrict__ row, int experts) {
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            float part[kChunk];
-            load_chunk(row, first + c * kChunk, experts, part);
+        for (int p = 0; p < kPieces; ++p) {
+            const int at = index_of(p * kWide);
+            if (at + kWide <= experts) {
+                const Unaligned piece = *reinterpret_cast<const Unaligned*>(row + at);
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) v[c * kChunk + i] = first + c * kChunk + i < experts ? part[i] : -__builtin_inff();
+                for (int i = 0; i < kWide; ++i) v[p * kWide + i] = static_cast<float>(piece[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kWide; ++i) v[p * kWide + i] = at + i < experts ? static_cast<float>(row[at + i]) : -__builtin_inff();
+            }
+        }
+    }
+    // Stores results as the logits lie.
+    __device__ __forceinline__ static void store(E* __restrict__ row, int experts, const float (&out)[kValues]) {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+            const int at = index_of(p * kWide);
+            using Floats = float __attribute__((ext_vector_type(kWide)));
+            Floats f;
+#pragma unroll
+            for (int i = 0; i < kWide; ++i) f[i] = out[p * kWide + i];
+            const auto y = __builtin_convertvector(f, E __attribute__((ext_vector_type(kWide))));
+            if (at + kWide <= experts) {
+                *reinterpret_cast<Unaligned*>(row + at) = y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kWide; ++i)
+                    if (at + i < experts) row[at + i] = y[i];
+            }
         }
     }
     // exp(l - top) of all of them (top: the largest, and not -inf)
@@ -94,15 +121,15 @@ __global__ __launch_bounds__(kThreads) void route_kernel(row_t rows, int experts
             best[j] = 0, at[j] = -1;
             if (j >= choices) continue;
             uint32_t key = keys[0];
-            int index = 0;
+            int index = Row::index_of(0);
 #pragma unroll
             for (int i = 1; i < Row::kValues; ++i)
-                if (keys[i] > key) key = keys[i], index = i;
+                if (keys[i] > key) key = keys[i], index = Row::index_of(i);
             best[j] = over_lanes<kLanes>(key, [](uint32_t a, uint32_t b) { return max(a, b); });
-            const uint32_t mine = key == best[j] ? static_cast<uint32_t>(r.first + index) : 0x7FFFFFFFu;
+            const uint32_t mine = key == best[j] ? static_cast<uint32_t>(index) : 0x7FFFFFFFu;
             at[j] = static_cast<int>(over_lanes<kLanes>(mine, [](uint32_t a, uint32_t b) { return min(a, b); }));
 #pragma unroll
-            for (int i = 0; i < Row::kValues; ++i) keys[i] = at[j] == r.first + i ? 0u : keys[i];
+            for (int i = 0; i < Row::kValues; ++i) keys[i] = at[j] == Row::index_of(i) ? 0u : keys[i];
         }
         const float top = logit_of(best[0]);
         float w[kMost], sum = 0.0f;
@@ -129,8 +156,8 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(row_t rows, in
                                                                   uint32_t stride, const float* __restrict__ weights, const int32_t* __restrict__ chosen,
                                                                   const float* __restrict__ grad, E* __restrict__ dlogits) {
     for (row_t row = blockIdx.x * static_cast<row_t>(kThreads / kLanes) + threadIdx.x / kLanes; row < rows; row += gridDim.x * static_cast<row_t>(kThreads / kLanes)) {
-        constexpr int kValues = kChunk * kChunks;
-        const int first = static_cast<int>(threadIdx.x) % kLanes * kValues;
+        using Row = LogitRow<E, kLanes, kChunks>;
+        constexpr int kValues = Row::kValues;
         float d[kMost], w[kMost], mean = 0.0f;
         int at[kMost];
 #pragma unroll
@@ -149,7 +176,7 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(row_t rows, in
 #pragma unroll
             for (int j = 0; j < kMost; ++j) d[j] -= w[j] * mean;
         } else {
-            const LogitRow<E, kLanes, kChunks> r(logits + offset_of(row, stride), experts);
+            const Row r(logits + offset_of(row, stride), experts);
             uint32_t key = 0;
 #pragma unroll
             for (int i = 0; i < kValues; ++i) key = max(key, key_of(r.v[i]));
@@ -160,16 +187,8 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(row_t rows, in
 #pragma unroll
         for (int j = 0; j < kMost; ++j)
 #pragma unroll
-            for (int i = 0; i < kValues; ++i) out[i] += at[j] == first + i ? d[j] : 0.0f;
-        E* const to = dlogits + offset_of(row, static_cast<uint32_t>(experts));
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            float part[kChunk];
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) part[i] = out[c * kChunk + i];
-            const int begin = first + c * kChunk;
-            if (begin < experts) store_chunk(to + begin, experts - begin, part);
-        }
+            for (int i = 0; i < kValues; ++i) out[i] += at[j] == Row::index_of(i) ? d[j] : 0.0f;
+        Row::store(dlogits + offset_of(row, static_cast<uint32_t>(experts)), experts, out);
     }
 }
 
@@ -200,9 +219,9 @@ unsigned grid_of(int64_t rows, int per_workgroup) { return static_cast<unsigned>
 // ------------------------------------------------------------------------------------------
 // plan
 
-constexpr int kPlanItems = 16;                          // of a lane
+constexpr int kPlanItems = 4;                           // of a lane
 constexpr int kPlanChunk = kThreads * kPlanItems;       // of a workgroup
-constexpr int kPlanWaves = kThreads / kWave;
+constexpr int kPlanAlone = 1024, kPlanMost = 16;        // one workgroup alone: its lanes, and the most items of a lane
 constexpr int kClasses = PENC_MAX_EXPERTS + 1;          // the experts, and none
 
 template <class I>
@@ -218,17 +237,24 @@ __global__ __launch_bounds__(kThreads) void plan_count_kernel(int64_t items, int
     for (int e = threadIdx.x; e <= experts; e += kThreads) lds[e] = 0;
     __syncthreads();
     const int64_t first = static_cast<int64_t>(blockIdx.x) * kPlanChunk;
+    int expert[kPlanItems];
+    bool there[kPlanItems];
 #pragma unroll
     for (int i = 0; i < kPlanItems; ++i) {
         const int64_t item = first + i * kThreads + threadIdx.x;
-        if (item < items) atomicAdd(&lds[class_of(chosen, item, experts)], 1u);
+        expert[i] = class_of(chosen, min(item, items - 1), experts);
+        there[i] = item < items;
     }
+#pragma unroll
+    for (int i = 0; i < kPlanItems; ++i)
+        if (there[i]) atomicAdd(&lds[expert[i]], 1u);
     __syncthreads();
     for (int e = threadIdx.x; e <= experts; e += kThreads) counts[static_cast<int64_t>(e) * gridDim.x + blockIdx.x] = lds[e];
 }
 
-// The exclusive sums of kThreads lanes' values, and their total.
-__device__ __forceinline__ uint32_t sums_before(uint32_t v, uint32_t (&of_waves)[kPlanWaves], uint32_t& total) {
+// The exclusive sums of kWaves waves' lanes' values, and their total.
+template <int kWaves>
+__device__ __forceinline__ uint32_t sums_before(uint32_t v, uint32_t (&of_waves)[kWaves], uint32_t& total) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     uint32_t sum = v;
 #pragma unroll
@@ -242,7 +268,7 @@ __device__ __forceinline__ uint32_t sums_before(uint32_t v, uint32_t (&of_waves)
     uint32_t before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
         before += w < wave ? of_waves[w] : 0u;
         total += of_waves[w];
     }
@@ -251,7 +277,7 @@ __device__ __forceinline__ uint32_t sums_before(uint32_t v, uint32_t (&of_waves)
 
 // A workgroup to an expert: each chunk's count becomes the sum of those before it; totals[expert].
 __global__ __launch_bounds__(kThreads) void plan_scan_kernel(int64_t chunks, uint32_t* __restrict__ counts, uint32_t* __restrict__ totals) {
-    __shared__ uint32_t of_waves[kPlanWaves];
+    __shared__ uint32_t of_waves[kThreads / kWave];
     uint32_t* const mine = counts + blockIdx.x * chunks;
     uint32_t before = 0;
     for (int64_t first = 0; first < chunks; first += kThreads) {
@@ -267,28 +293,32 @@ __global__ __launch_bounds__(kThreads) void plan_scan_kernel(int64_t chunks, uin
 
 // Where each choice of a chunk stands.  A wave takes 64 consecutive choices after the other; lanes of one expert find each other by a ballot for each bit of its
 // number, and each stands behind those of the wave's choices before.  Without `counts` there is one chunk, which counts for itself.
-template <class I>
-__global__ __launch_bounds__(kThreads) void plan_place_kernel(int64_t items, int experts, int bits, const I* __restrict__ chosen,
+template <class I, int kLanes, int kItems>
+__global__ __launch_bounds__(kLanes) void plan_place_kernel(int64_t items, int experts, int bits, const I* __restrict__ chosen,
                                                               const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
                                                               int32_t* __restrict__ positions, int32_t* __restrict__ offsets) {
-    __shared__ uint32_t lds[kPlanWaves][kClasses];
-    __shared__ uint32_t of_waves[kPlanWaves];
+    constexpr int kWaves = kLanes / kWave;
+    __shared__ uint32_t lds[kWaves][kClasses];
+    __shared__ uint32_t of_waves[kWaves];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    for (int e = threadIdx.x; e <= experts; e += kThreads)
+    for (int e = threadIdx.x; e <= experts; e += kLanes)
 #pragma unroll
-        for (int w = 0; w < kPlanWaves; ++w) lds[w][e] = 0;
+        for (int w = 0; w < kWaves; ++w) lds[w][e] = 0;
     __syncthreads();
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kPlanChunk + wave * (kPlanChunk / kPlanWaves) + lane;
-    int expert[kPlanItems];
-    uint32_t rank[kPlanItems];
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kLanes * kItems) + wave * (kWave * kItems) + lane;
+    int expert[kItems];
+    uint32_t rank[kItems];
 #pragma unroll
-    for (int i = 0; i < kPlanItems; ++i) {
+    for (int i = 0; i < kItems; ++i) {
+        // (read without a condition: a branch for each would have them come one after the other)
         const int64_t item = first + i * kWave;
-        expert[i] = item < items ? class_of(chosen, item, experts) : -1;
+        const int e = items > 0 ? class_of(chosen, min(item, items - 1), experts) : 0;
+        expert[i] = item < items ? e : -1;
     }
 #pragma unroll
-    for (int i = 0; i < kPlanItems; ++i) {
+    for (int i = 0; i < kItems; ++i) {
         uint64_t same = __ballot(expert[i] >= 0);
+        if (same == 0) break;  // (nothing behind it either)
         for (int b = 0; b < bits; ++b) {
             const bool set = expert[i] >> b & 1;
             const uint64_t those = __ballot(set);
@@ -305,7 +335,7 @@ __global__ __launch_bounds__(kThreads) void plan_place_kernel(int64_t items, int
     __syncthreads();
     // what stands before each wave's choices of an expert: the experts before, the chunks before, the waves before
     uint32_t of_experts = 0;
-    for (int begin = 0; begin <= experts; begin += kThreads) {
+    for (int begin = 0; begin <= experts; begin += kLanes) {
         const int e = begin + static_cast<int>(threadIdx.x);
         uint32_t mine = 0;
         if (e <= experts) {
@@ -313,7 +343,7 @@ __global__ __launch_bounds__(kThreads) void plan_place_kernel(int64_t items, int
                 mine = totals[e];
             } else {
 #pragma unroll
-                for (int w = 0; w < kPlanWaves; ++w) mine += lds[w][e];
+                for (int w = 0; w < kWaves; ++w) mine += lds[w][e];
             }
         }
         uint32_t total;
@@ -323,7 +353,7 @@ __global__ __launch_bounds__(kThreads) void plan_place_kernel(int64_t items, int
             if (blockIdx.x == 0) offsets[e] = static_cast<int32_t>(at);
             if (counts != nullptr) at += counts[static_cast<int64_t>(e) * gridDim.x + blockIdx.x];
 #pragma unroll
-            for (int w = 0; w < kPlanWaves; ++w) {
+            for (int w = 0; w < kWaves; ++w) {
                 const uint32_t n = lds[w][e];
                 lds[w][e] = at;
                 at += n;
@@ -332,7 +362,7 @@ __global__ __launch_bounds__(kThreads) void plan_place_kernel(int64_t items, int
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kPlanItems; ++i) {
+    for (int i = 0; i < kItems; ++i) {
         const int64_t item = first + i * kWave;
         if (item < items) positions[item] = static_cast<int32_t>(lds[wave][expert[i]] + rank[i]);
     }
@@ -378,7 +408,7 @@ struct Single {
     __device__ __forceinline__ static Vector rounded(Floats v) { return Vector{static_cast<E>(v[0])}; }
 };
 
-// A row to neighbouring lanes, a power of two of them up to a wave, and from there on every `step`-th.
+// A row to neighbouring lanes, a power of two of them, and from there on every `step`-th.
 struct Group {
     row_t first, step;
     int lane;
@@ -406,35 +436,46 @@ __global__ __launch_bounds__(kThreads) void dispatch_kernel(RowPlan plan, int lo
     }
 }
 
-// out[t] = the sum, with weights or without, of the rows at t's choices; kMost at a time are on their way.
+// out[t] = the sum, with weights or without, of the rows at t's choices; kMost at a time are on their way, of kAhead pieces each.
 template <class P, class E, class W, int kMost>
 __global__ __launch_bounds__(kThreads) void gather_kernel(RowPlan plan, int log2_lanes, const E* __restrict__ y, uint32_t stride, const W* __restrict__ weights,
                                                           E* __restrict__ out) {
+    constexpr int kAhead = 1;
     const Group g(log2_lanes);
     const uint32_t most = plan.most();
+    const int step = P::kWide << log2_lanes;
     for (row_t row = g.first; row < plan.rows; row += g.step) {
-        for (int c = g.lane * P::kWide; c < plan.channels; c += P::kWide << log2_lanes) {
-            const int at = min(c, plan.channels - P::kWide);
-            typename P::Floats sum{};
-            for (int first = 0; first < plan.choices; first += kMost) {
-                typename P::Vector v[kMost];
-                float w[kMost];
-                bool there[kMost];
-    #pragma unroll
-                for (int j = 0; j < kMost; ++j) {
-                    there[j] = first + j < plan.choices;
-                    const uint32_t from = there[j] ? plan.position(row, first + j) : 0u;
-                    there[j] = there[j] && from < most;
-                    if (there[j]) {
-                        v[j] = P::load(y + offset_of(from, stride) + at);
-                        w[j] = weights != nullptr ? static_cast<float>(weights[offset_of(row, static_cast<uint32_t>(plan.choices)) + first + j]) : 1.0f;
-                    }
-                }
-    #pragma unroll
-                for (int j = 0; j < kMost; ++j)
-                    if (there[j]) sum += P::floats(v[j]) * w[j];
+        const E* from[kMost];
+        float w[kMost];
+        const auto choose = [&](int first) {
+#pragma unroll
+            for (int j = 0; j < kMost; ++j) {
+                const bool there = first + j < plan.choices;
+                const uint32_t at = there ? plan.position(row, first + j) : most;
+                from[j] = at < most ? y + offset_of(at, stride) : nullptr;
+                w[j] = from[j] != nullptr && weights != nullptr ? static_cast<float>(weights[offset_of(row, static_cast<uint32_t>(plan.choices)) + first + j]) : 1.0f;
             }
-            P::store(out + offset_of(row, plan.channels) + at, P::rounded(sum));
+        };
+        choose(0);
+        for (int c = g.lane * P::kWide; c < plan.channels; c += kAhead * step) {
+            typename P::Floats sum[kAhead] = {};
+            for (int first = 0; first < plan.choices; first += kMost) {
+                if (plan.choices > kMost) choose(first);
+                typename P::Vector v[kAhead][kMost];
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+                    for (int j = 0; j < kMost; ++j)
+                        if (from[j] != nullptr) v[a][j] = P::load(from[j] + min(c + a * step, plan.channels - P::kWide));
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+                    for (int j = 0; j < kMost; ++j)
+                        if (from[j] != nullptr) sum[a] += P::floats(v[a][j]) * w[j];
+            }
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a)
+                if (c + a * step < plan.channels) P::store(out + offset_of(row, plan.channels) + min(c + a * step, plan.channels - P::kWide), P::rounded(sum[a]));
         }
     }
 }
@@ -491,13 +532,13 @@ bool bad_plan(int64_t rows, int choices, int64_t channels) {
     return bad_rows(rows) || choices < 1 || choices > PENC_MAX_CHOICES || bad_rows(rows * choices) || channels < 1 || channels > PENC_MAX_CHANNELS;
 }
 
-// Runs f with the kind of piece that a row takes, and the lanes of a row.
+// Runs f with the kind of piece that a row takes, and the lanes of a row, at most 2^most.
 template <class E, class F>
-int with_pieces(int64_t channels, F&& f) {
+int with_pieces(int64_t channels, int most, F&& f) {
     constexpr int kWide = Piece<E>::kWide;
-    const auto log2_lanes = [](int64_t pieces) {
+    const auto log2_lanes = [most](int64_t pieces) {
         int n = 0;
-        while (n < 6 && (1 << n) < pieces) ++n;
+        while (n < most && (1 << n) < pieces) ++n;
         return n;
     };
     if (channels >= kWide) return f(Piece<E>{}, log2_lanes((channels + kWide - 1) / kWide));
@@ -565,7 +606,7 @@ int penc_route_backward(int type, int64_t rows, int experts, int choices, int no
 }
 
 size_t penc_plan_workspace_bytes(int64_t items, int experts) {
-    if (bad_rows(items) || experts < 1 || experts > PENC_MAX_EXPERTS || items <= kPlanChunk) return 0;
+    if (bad_rows(items) || experts < 1 || experts > PENC_MAX_EXPERTS || items <= kPlanAlone * kPlanMost) return 0;
     return 4 * (static_cast<size_t>(experts) + 1) * (static_cast<size_t>((items + kPlanChunk - 1) / kPlanChunk) + 1);
 }
 
@@ -579,22 +620,27 @@ int penc_plan(int index_bytes, int64_t items, int experts, const void* chosen, i
     if (workspace_bytes < need) return PENC_ERR_WORKSPACE_TOO_SMALL;
     if (need > 0 && !workspace) return PENC_ERR_NULL_POINTER;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const int64_t chunks = std::max<int64_t>(1, (items + kPlanChunk - 1) / kPlanChunk);
     int bits = 1;
     while ((1 << bits) <= experts) ++bits;
     const auto plan = [&](auto index) -> int {
         using I = decltype(index);
         const I* const from = static_cast<const I*>(chosen);
-        uint32_t *counts = nullptr, *totals = nullptr;
-        if (chunks > 1) {
-            totals = static_cast<uint32_t*>(workspace);
-            counts = totals + experts + 1;
-            plan_count_kernel<I><<<static_cast<unsigned>(chunks), kThreads, 0, s>>>(items, experts, from, counts);
-            if (const int rc = launched()) return rc;
-            plan_scan_kernel<<<static_cast<unsigned>(experts + 1), kThreads, 0, s>>>(chunks, counts, totals);
-            if (const int rc = launched()) return rc;
-        }
-        plan_place_kernel<I><<<static_cast<unsigned>(chunks), kThreads, 0, s>>>(items, experts, bits, from, counts, totals, positions, offsets);
+        // up to 16384 choices: one workgroup, one launch
+        const auto alone = [&](auto n) -> int {
+            plan_place_kernel<I, kPlanAlone, decltype(n)::value><<<1, kPlanAlone, 0, s>>>(items, experts, bits, from, nullptr, nullptr, positions, offsets);
+            return launched();
+        };
+        if (items <= kPlanAlone) return alone(std::integral_constant<int, 1>{});
+        if (items <= kPlanAlone * 4) return alone(std::integral_constant<int, 4>{});
+        if (items <= kPlanAlone * kPlanMost) return alone(std::integral_constant<int, kPlanMost>{});
+        const int64_t chunks = (items + kPlanChunk - 1) / kPlanChunk;
+        uint32_t* const totals = static_cast<uint32_t*>(workspace);
+        uint32_t* const counts = totals + experts + 1;
+        plan_count_kernel<I><<<static_cast<unsigned>(chunks), kThreads, 0, s>>>(items, experts, from, counts);
+        if (const int rc = launched()) return rc;
+        plan_scan_kernel<<<static_cast<unsigned>(experts + 1), kThreads, 0, s>>>(chunks, counts, totals);
+        if (const int rc = launched()) return rc;
+        plan_place_kernel<I, kThreads, kPlanItems><<<static_cast<unsigned>(chunks), kThreads, 0, s>>>(items, experts, bits, from, counts, totals, positions, offsets);
         return launched();
     };
     return index_bytes == 4 ? plan(int32_t{}) : plan(int64_t{});
@@ -609,7 +655,7 @@ int penc_dispatch(int type, int64_t rows, int choices, int64_t channels, const v
     const auto copy = [&](auto e) -> int {
         using E = decltype(e);
         if (!aligned_to(x, sizeof(E)) || !aligned_to(sorted, sizeof(E)) || !aligned_to(positions, 4) || !aligned_to(routed, 4)) return PENC_ERR_MISALIGNED;
-        return with_pieces<E>(channels, [&](auto piece, int log2_lanes) -> int {
+        return with_pieces<E>(channels, kLog2Threads, [&](auto piece, int log2_lanes) -> int {
             dispatch_kernel<decltype(piece)><<<grid_of(rows, kThreads >> log2_lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
                 row_plan(rows, choices, channels, positions, routed), log2_lanes, static_cast<const E*>(x), static_cast<uint32_t>(row_stride), static_cast<E*>(sorted));
             return launched();
@@ -629,7 +675,7 @@ int penc_combine(int type, int weight_type, int64_t rows, int choices, int64_t c
         if (!aligned_to(y, sizeof(E)) || !aligned_to(out, sizeof(E)) || !aligned_to(weights, weight_type == PENC_FP32 ? 4 : 2) || !aligned_to(positions, 4) ||
             !aligned_to(routed, 4))
             return PENC_ERR_MISALIGNED;
-        return with_pieces<E>(channels, [&](auto piece, int log2_lanes) -> int {
+        return with_pieces<E>(channels, kLog2Threads, [&](auto piece, int log2_lanes) -> int {
             return with_most(choices, [&](auto most) -> int {
                 const auto launch = [&](auto w) -> int {
                     using W = decltype(w);
@@ -656,7 +702,7 @@ int penc_combine_backward(int type, int weight_type, int64_t rows, int choices, 
         if (!aligned_to(y, sizeof(E)) || !aligned_to(grad, sizeof(E)) || !aligned_to(dy, sizeof(E)) || !aligned_to(weights, weight) ||
             !aligned_to(dweights, weight) || !aligned_to(positions, 4) || !aligned_to(routed, 4))
             return PENC_ERR_MISALIGNED;
-        return with_pieces<E>(channels, [&](auto piece, int log2_lanes) -> int {
+        return with_pieces<E>(channels, 6, [&](auto piece, int log2_lanes) -> int {
             return with_most(choices, [&](auto most) -> int {
                 const auto launch = [&](auto w) -> int {
                     using W = decltype(w);

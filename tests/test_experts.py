@@ -23,13 +23,13 @@ def test_the_entry_points_refuse_before_they_launch():
     assert lib.penc_route(1, 4, 8, 2, 1, p + 1, 8, p, p, z) == 5 and lib.penc_route(0, 4, 8, 2, 1, p, 8, p + 2, p, z) == 5
     assert lib.penc_route(0, 0, 8, 2, 1, z, 8, z, z, z) == 0
     assert lib.penc_route_backward(0, 4, 8, 2, 0, z, 8, p, p, p, p, z) == 1 and lib.penc_route_backward(0, 4, 8, 2, 1, z, 8, p, p, z, p, z) == 1
-    # plans: one chunk needs no workspace
-    assert lib.penc_plan_workspace_bytes(4096, 8) == 0 == lib.penc_plan_workspace_bytes(-1, 8) == lib.penc_plan_workspace_bytes(10000, 1025)
-    need = lib.penc_plan_workspace_bytes(10000, 8)
-    assert need == 4 * 9 * (3 + 1)
+    # plans: a few choices need no workspace
+    assert lib.penc_plan_workspace_bytes(16384, 8) == 0 == lib.penc_plan_workspace_bytes(-1, 8) == lib.penc_plan_workspace_bytes(10000, 1025)
+    need = lib.penc_plan_workspace_bytes(20000, 8)
+    assert need == 4 * 9 * (20 + 1)
     assert lib.penc_plan(2, 10, 8, p, p, p, z, 0, z) == 10 and lib.penc_plan(4, -1, 8, p, p, p, z, 0, z) == 12 and lib.penc_plan(4, 10, 0, p, p, p, z, 0, z) == 12
     assert lib.penc_plan(4, 10, 8, z, p, p, z, 0, z) == 1 and lib.penc_plan(4, 10, 8, p, p, z, z, 0, z) == 1 and lib.penc_plan(8, 10, 8, p + 4, p, p, z, 0, z) == 5
-    assert lib.penc_plan(4, 10000, 8, p, p, p, p, need - 1, z) == 8 and lib.penc_plan(4, 10000, 8, p, p, p, z, need, z) == 1
+    assert lib.penc_plan(4, 20000, 8, p, p, p, p, need - 1, z) == 8 and lib.penc_plan(4, 20000, 8, p, p, p, z, need, z) == 1
     # rows there and back
     assert lib.penc_dispatch(3, 4, 2, 8, p, 8, p, p, p, z) == 10
     for bad in ((-1, 2, 8), (4, 0, 8), (4, 1025, 8), (4, 2, 0), (4, 2, (1 << 24) + 1), (1 << 30, 2, 8)):

@@ -122,7 +122,7 @@ def test_the_gradient_of_route_against_differences(normalise):
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("rows,choices,number", [(0, 2, 5), (1, 1, 1), (1, 2, 64), (63, 1, 3), (64, 3, 7), (1000, 2, 8), (4096, 1, 1024), (4097, 1, 2), (2049, 2, 1000),
-                                                 (30000, 4, 63), (30000, 1, 64), (5, 1000, 17), (1 << 18, 2, 13)])
+                                                 (16384, 1, 9), (16385, 1, 9), (8000, 2, 1024), (30000, 4, 63), (30000, 1, 64), (5, 1000, 17), (1 << 18, 2, 13)])
 def test_plan(dtype, rows, choices, number):
     for none in (0.0, 0.2, 1.0):
         experts = chosen_experts(rows, choices, number, none=none, dtype=dtype)
