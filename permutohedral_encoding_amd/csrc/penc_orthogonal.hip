@@ -155,6 +155,8 @@ struct StepArgs {
     int rows, columns, padded, small, small_padded;
     Spread spread;
     uint32_t each, tiles_m;  // each: items of a matrix
+    int splits;              // kGram: workgroups that share a tile's k, each of which leaves its sums in `partial`
+    float* partial;
     float a, b, c;
 };
 
@@ -177,8 +179,9 @@ template <Stage kStage, bool kTall, class E, class Result, class P>
 __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
     constexpr int kBytes = ProductType<E>::kBytes;
-    const uint32_t item = a.spread.item(), t = item % a.each;
-    if (item >= a.spread.items) return;
+    const uint32_t of_launch = a.spread.item();
+    if (of_launch >= a.spread.items) return;
+    const uint32_t item = kStage == kGram ? of_launch / a.splits : of_launch, split = kStage == kGram ? of_launch % a.splits : 0, t = item % a.each;
     const int64_t matrix = item / a.each;
     const int64_t stride = static_cast<int64_t>(a.padded) * kBytes, small_stride = static_cast<int64_t>(a.small_padded) * kBytes;
     const char *const x = a.x + matrix * a.rows * stride, *const s = a.s + matrix * a.small * small_stride, *const f = a.f + matrix * a.small * small_stride;
@@ -188,11 +191,23 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
     const auto rows_from = [&](const char* p, int64_t row_bytes, int rows, int first, int most) { return Operand{p + first * row_bytes, row_bytes, min(rows - first, most), static_cast<int>(row_bytes)}; };
     const auto columns_from = [&](int first, int most) { return Operand{x + first * kBytes, stride, a.rows, min(a.padded - first, most) * kBytes}; };
     P p;
-    if constexpr (kStage == kGram && !kTall) p.run(lds, rows_from(x, stride, a.rows, m0, P::kM), rows_from(x, stride, a.rows, n0, P::kN), a.padded, P::kZero, P::kNothing);
-    else if constexpr (kStage == kGram) p.run(lds, columns_from(m0, P::kM), columns_from(n0, P::kN), a.rows, P::kZero, P::kNothing);
-    else if constexpr (kStage == kSquare) p.run(lds, rows_from(s, small_stride, a.small, m0, P::kM), rows_from(s, small_stride, a.small, n0, P::kN), a.small_padded, P::kZero, P::kNothing);
-    else if constexpr (!kTall) p.run(lds, columns_from(m0, P::kM), rows_from(f, small_stride, a.small, n0, P::kN), a.small, P::kZero, P::kNothing);
-    else p.run(lds, rows_from(f, small_stride, a.small, m0, P::kM), rows_from(x, stride, a.rows, n0, P::kN), a.padded, P::kZero, P::kNothing);
+    if constexpr (kStage == kGram) {
+        const int all = kTall ? a.rows : a.padded, each = ((all + P::kDepth - 1) / P::kDepth + a.splits - 1) / a.splits * P::kDepth;
+        const int k0 = min(static_cast<int>(split) * each, all), depth = min(all - k0, each);
+        Operand m = kTall ? columns_from(m0, P::kM) : rows_from(x, stride, a.rows, m0, P::kM), n = kTall ? columns_from(n0, P::kN) : rows_from(x, stride, a.rows, n0, P::kN);
+        m.first += k0 * (kTall ? stride : kBytes), n.first += k0 * (kTall ? stride : kBytes);
+        if constexpr (kTall) m.rows = n.rows = depth;
+        else m.bytes = n.bytes = depth * kBytes;
+        p.run(lds, m, n, depth, P::kZero, P::kNothing);
+        if (a.partial != nullptr) {
+            float* const to = a.partial + static_cast<int64_t>(of_launch) * (P::kM * P::kN);
+            p.each([&](int m, int n, tile_acc v) { *reinterpret_cast<tile_acc*>(to + n * P::kM + m) = v; });
+            return;
+        }
+    }
+    if constexpr (kStage == kSquare) p.run(lds, rows_from(s, small_stride, a.small, m0, P::kM), rows_from(s, small_stride, a.small, n0, P::kN), a.small_padded, P::kZero, P::kNothing);
+    if constexpr (kStage == kUpdate && !kTall) p.run(lds, columns_from(m0, P::kM), rows_from(f, small_stride, a.small, n0, P::kN), a.small, P::kZero, P::kNothing);
+    if constexpr (kStage == kUpdate && kTall) p.run(lds, rows_from(f, small_stride, a.small, m0, P::kM), rows_from(x, stride, a.rows, n0, P::kN), a.padded, P::kZero, P::kNothing);
     if constexpr (kStage != kUpdate) {
         char* const out = a.out + matrix * a.small * small_stride;
         constexpr int kWideM = P::kM / P::kWavesM, kWideN = P::kN / P::kWavesN, kParts = ProductType<E>::kParts;
@@ -245,6 +260,40 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
             if (a.result == nullptr) store_stored<E>(out + n * stride, m, v);
             else if (m < a.columns) store_values<Result, 8>(result + static_cast<int64_t>(n) * a.columns + m, __builtin_convertvector(v * kPerScale, Eight), a.columns - m);
         });
+    }
+}
+
+constexpr int kSumSide = 64, kSumThreads = 512;
+
+// S from the sums of the workgroups that shared its tiles, of 64 x 64, in their order, and the other side of the diagonal.
+template <class E>
+__global__ __launch_bounds__(kSumThreads) void gram_sum_kernel(StepArgs a) {
+    __shared__ float lds[kSumSide][kSumSide + 1];
+    const uint32_t t = blockIdx.x % a.each;
+    const int64_t matrix = blockIdx.x / a.each, stride = static_cast<int64_t>(a.small_padded) * ProductType<E>::kBytes;
+    uint32_t i, j;
+    pair_of(t, i, j);
+    char* const out = a.out + matrix * a.small * stride;
+    const float* const from = a.partial + static_cast<int64_t>(blockIdx.x) * a.splits * (kSumSide * kSumSide);
+    const int m0 = static_cast<int>(i) * kSumSide, n0 = static_cast<int>(j) * kSumSide;
+    for (int at = static_cast<int>(threadIdx.x) * 8; at < kSumSide * kSumSide; at += kSumThreads * 8) {
+        floats<8> v{};
+#pragma unroll 8
+        for (int k = 0; k < a.splits; ++k) v += *reinterpret_cast<const floats<8>*>(from + k * (kSumSide * kSumSide) + at);
+        v *= kPerScale;
+        const int n = at / kSumSide, m = at % kSumSide;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) lds[m + k][n] = v[k];
+        if (n0 + n < a.small && m0 + m < a.small_padded) store_stored<E>(out + (n0 + n) * stride, m0 + m, v);
+    }
+    if (i == j) return;
+    __syncthreads();
+    for (int at = static_cast<int>(threadIdx.x) * 8; at < kSumSide * kSumSide; at += kSumThreads * 8) {
+        const int m = at / kSumSide, n = at % kSumSide;
+        floats<8> v;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = lds[m][n + k];
+        if (m0 + m < a.small && n0 + n < a.small_padded) store_stored<E>(out + (m0 + m) * stride, n0 + n, v);
     }
 }
 
@@ -303,7 +352,7 @@ __host__ __device__ constexpr int round_to_32(int n) { return (n + 31) / 32 * 32
 template <class G, int kTiles, int kBlocks>
 __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, int columns, int steps, Coefficients k, const G* __restrict__ g, G* __restrict__ result) {
     __shared__ __attribute__((aligned(1024))) char lds[kMostResident];
-    constexpr int kPadded = 16 * kTiles, kLines = kPadded / 32;
+    constexpr int kPadded = 16 * kTiles, kLines = kPadded / 32, kTogether = kBlocks > 1 ? 2 : 1;
     const bool tall = rows > columns;
     const int small = min(rows, columns), large = max(rows, columns), large_padded = (large + 63) / 64 * 64;
     const Resident x{lds, resident_pitch(large_padded)}, s{lds + kPadded * x.pitch, resident_pitch(kPadded)};
@@ -312,31 +361,50 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
     // (where number `column` of row `row` is in memory)
     const int row_step = tall ? 1 : columns, column_step = tall ? columns : 1;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), q4 = lane / 16 * 4, l16 = lane % 16;
-    double squares = 0.0;
-#pragma unroll 8
-    for (int i = static_cast<int>(threadIdx.x); i < values; i += kResidentThreads) {
-        const double v = static_cast<double>(static_cast<float>(from[i]));
-        squares += v * v;
-    }
-    const double factor = per_norm(workgroup_sum<kResidentThreads>(squares), k.eps);
-    // (a lane has eight numbers of a row; neighbouring lanes are neighbours in memory)
-    const int eights = large_padded / 8;
-#pragma unroll 2
-    for (int i = static_cast<int>(threadIdx.x); i < kPadded * eights; i += kResidentThreads) {
-        const int row = tall ? i % kPadded : i / eights, column = (tall ? i / kPadded : i % eights) * 8;
-        floats<8> v{};
+    // The matrix once from memory: eight numbers of a row to a lane, neighbouring lanes neighbours in memory.
+    constexpr int kEights = (kMostResident / 4 / 8 + kResidentThreads - 1) / kResidentThreads;
+    const int eights = large_padded / 8, all = kPadded * eights;
+    floats<8> read[kEights];
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-            if (row < small && column + n < large) v[n] = scaled(from[row * row_step + (column + n) * column_step], factor);
-        x.store<8>(row, column, v);
+    for (int e = 0; e < kEights; ++e) {
+        read[e] = floats<8>{};
+        const int i = e * kResidentThreads + static_cast<int>(threadIdx.x);
+        if (e * kResidentThreads >= all) continue;
+        const int row = tall ? i % kPadded : i / eights, column = (tall ? i / kPadded : i % eights) * 8;
+        const G* const p = from + row * row_step + column * column_step;
+        if (row < small && !tall && column + 8 <= large) {
+            using Unaligned = G __attribute__((ext_vector_type(8), aligned(sizeof(G))));
+            read[e] = __builtin_convertvector(*reinterpret_cast<const Unaligned*>(p), floats<8>);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if (row < small && column + n < large) read[e][n] = static_cast<float>(p[n * column_step]);
+        }
     }
-    tile_acc own[kBlocks][kTiles];
+    double squares = 0.0;
+#pragma unroll
+    for (int e = 0; e < kEights; ++e)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) squares = __builtin_fma(static_cast<double>(read[e][n]), static_cast<double>(read[e][n]), squares);
+    const double factor = per_norm(workgroup_sum<kResidentThreads>(squares), k.eps);
+#pragma unroll
+    for (int e = 0; e < kEights; ++e) {
+        const int i = e * kResidentThreads + static_cast<int>(threadIdx.x);
+        if (i >= all) continue;
+        floats<8> v;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) v[n] = scaled(read[e][n], factor);
+        x.store<8>(tall ? i % kPadded : i / eights, (tall ? i / kPadded : i % eights) * 8, v);
+    }
+    // What this wave has of X as results.
+    floats<4> own[kBlocks][kTiles];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
             const int row = n * 16 + l16, column = (b * kResidentWaves + wave) * 16 + q4;
-            own[b][n] = tile_acc{};
+            own[b][n] = floats<4>{};
+            if ((b * kResidentWaves + wave) * 16 >= large) continue;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (row < small && column + i < large) own[b][n][i] = scaled(from[row * row_step + (column + i) * column_step], factor);
@@ -389,21 +457,36 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
         }
         __syncthreads();
         const bool last = step + 1 == steps;
+        // (two blocks of columns at a time: each fragment of F is read once for both)
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            const int m = (b * kResidentWaves + wave) * 16;
-            if (m >= large_padded) continue;
-            tile_acc acc[kTiles] = {};
+        for (int b = 0; b < kBlocks; b += kTogether) {
+            if ((b * kResidentWaves + wave) * 16 >= large_padded) continue;
+            tile_acc acc[kTogether][kTiles] = {};
 #pragma unroll
             for (int line = 0; line < kLines; ++line) {
-                const chunk16 a = x.along(line * 32, m, 0), a_low = x.along(line * 32, m, 1);
+                chunk16 a[kTogether][2];
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n) acc[n] = multiply_split(a, a_low, s.across(n * 16, line, 0), s.across(n * 16, line, 1), acc[n]);
+                for (int t = 0; t < kTogether; ++t) {
+                    // (where there is no second block: the first one's, for results that are not taken)
+                    const int m = ((b + t) * kResidentWaves + wave) * 16, at = m < large_padded ? m : (b * kResidentWaves + wave) * 16;
+                    a[t][0] = x.along(line * 32, at, 0), a[t][1] = x.along(line * 32, at, 1);
+                }
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) {
+                    const chunk16 f = s.across(n * 16, line, 0), f_low = s.across(n * 16, line, 1);
+#pragma unroll
+                    for (int t = 0; t < kTogether; ++t) acc[t][n] = multiply_split(a[t][0], a[t][1], f, f_low, acc[t][n]);
+                }
             }
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n) {
-                own[b][n] = k.a * own[b][n] + acc[n] * kPerScale;
-                if (!last) x.store<4>(n * 16 + l16, m + q4, own[b][n]);
+            for (int t = 0; t < kTogether; ++t) {
+                const int m = ((b + t) * kResidentWaves + wave) * 16;
+                if (b + t >= kBlocks || m >= large_padded) continue;
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) {
+                    own[b + t][n] = k.a * own[b + t][n] + acc[t][n] * kPerScale;
+                    if (!last) x.store<4>(n * 16 + l16, m + q4, own[b + t][n]);
+                }
             }
         }
         __syncthreads();
@@ -479,10 +562,26 @@ int resident(int64_t matrices, int64_t rows, int64_t columns, int steps, Coeffic
     return launch(std::integral_constant<int, 8>{});
 }
 
+// Whether a launch takes tiles of 64 x 64: where there would not be a workgroup of 128 x 128 for each compute unit.
+bool small_tiles(int64_t matrices, int64_t side_m, int64_t side_n, bool half) {
+    return matrices * ((side_m + 127) / 128) * ((side_n + 127) / 128) / (half ? 2 : 1) < 256;
+}
+int64_t pairs_of(int64_t small, int side) {
+    const int64_t tiles = (small + side - 1) / side;
+    return tiles * (tiles + 1) / 2;
+}
+// How many workgroups share the k of a tile of S: up to one for each compute unit, each with two steps at least (1000 x 203 fp16: 14 us without, 4 and 3 for the sums).
+int gram_splits(int64_t matrices, int64_t small, int64_t depth, int step) {
+    const int64_t items = matrices * pairs_of(small, kSumSide);
+    if (!small_tiles(matrices, small, small, true) || items > 64) return 1;
+    return static_cast<int>(std::max<int64_t>(1, std::min({256 / items, depth / (2 * step), int64_t{16}})));
+}
+
 // The workspace of matrices that do not stay in the LDS.
 struct Layout {
     int64_t padded, small, small_padded, x, s;  // x, s: bytes of all matrices'
-    int pieces;
+    int pieces, splits;
+    int64_t partial;  // bytes of the sums of workgroups that share tiles
     size_t total;
 };
 template <class E>
@@ -495,9 +594,11 @@ Layout layout_of(int64_t matrices, int64_t rows, int64_t columns) {
     l.x = matrices * rows * l.padded * kBytes;
     l.s = matrices * l.small * l.small_padded * kBytes;
     l.pieces = static_cast<int>(std::min<int64_t>(kMostPieces, (rows * columns + 16383) / 16384));
+    l.splits = gram_splits(matrices, l.small, std::max(rows, columns), kDepth);
     const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     l.x = up(l.x), l.s = up(l.s);
-    l.total = static_cast<size_t>(2 * l.x + 2 * l.s + up(8 * matrices * l.pieces));
+    l.partial = l.splits > 1 ? matrices * pairs_of(l.small, kSumSide) * l.splits * (4 * kSumSide * kSumSide) : 0;
+    l.total = static_cast<size_t>(2 * l.x + 2 * l.s + l.partial + up(8 * matrices * l.pieces));
     return l;
 }
 
@@ -508,27 +609,24 @@ int launch_step(StepArgs a, int64_t matrices, hipStream_t stream) {
         using P = typename decltype(product)::type;
         int64_t each;
         if (kStage != kUpdate) {
-            const int64_t tiles = (a.small + P::kM - 1) / P::kM;
-            each = tiles * (tiles + 1) / 2;
+            each = pairs_of(a.small, P::kM);
             a.tiles_m = 1;
         } else {
             a.tiles_m = static_cast<uint32_t>((a.columns + P::kM - 1) / P::kM);
             each = static_cast<int64_t>(a.tiles_m) * ((a.rows + P::kN - 1) / P::kN);
         }
-        const int64_t items = each * matrices;
+        const int64_t items = each * matrices * (kStage == kGram ? a.splits : 1);
         if (items * P::kThreads >= (int64_t{1} << 32) - (1 << 18)) return PENC_ERR_BAD_LAYER_SIZE;
         a.each = static_cast<uint32_t>(each), a.spread = Spread(items, 32);
         step_kernel<kStage, kTall, E, Result, P><<<a.spread.grid(), P::kThreads, 0, stream>>>(a);
         return launched();
     };
-    // tiles of 64 x 64 where there would not be a workgroup of 128 x 128 for each compute unit
     const int64_t side_m = kStage == kUpdate ? a.columns : a.small, side_n = kStage == kUpdate ? a.rows : a.small;
-    const int64_t large = matrices * ((side_m + 127) / 128) * ((side_n + 127) / 128) / (kStage == kUpdate ? 1 : 2);
     const int64_t huge = matrices * ((side_m + 255) / 256) * ((side_n + 255) / 256) / (kStage == kUpdate ? 1 : 2);
     if constexpr (std::is_same_v<E, half_t>) {
         if (huge >= 128) return launch(std::common_type<Product<E, kAlongM, kAlongN, 256, 256, 4, 2, Chunks::kDirect>>{});
     }
-    if (large < 256) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, Chunks::kDirect, 4>>{});
+    if (small_tiles(matrices, side_m, side_n, kStage != kUpdate)) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, Chunks::kDirect, 4>>{});
     return launch(std::common_type<Product<E, kAlongM, kAlongN, 128, 128, 2, 2, Chunks::kDirect>>{});
 }
 
@@ -536,7 +634,8 @@ template <class E, class G>
 int orthogonalise(int64_t matrices, int64_t rows, int64_t columns, int steps, Coefficients k, const G* g, G* result, char* workspace, hipStream_t stream) {
     const Layout l = layout_of<E>(matrices, rows, columns);
     char *x = workspace, *next = x + l.x, *const s = next + l.x, *const f = s + l.s;
-    double* const sums = reinterpret_cast<double*>(f + l.s);
+    float* const partial = reinterpret_cast<float*>(f + l.s);
+    double* const sums = reinterpret_cast<double*>(f + l.s + l.partial);
     squares_kernel<G><<<static_cast<unsigned>(matrices * l.pieces), kThreads, 0, stream>>>(rows * columns, l.pieces, g, sums);
     if (const int rc = launched()) return rc;
     const int64_t eights = rows * (l.padded / 8);
@@ -546,10 +645,15 @@ int orthogonalise(int64_t matrices, int64_t rows, int64_t columns, int steps, Co
     if (const int rc = launched()) return rc;
     for (int step = 0; step < steps; ++step) {
         StepArgs a{x, s, f, s, nullptr, static_cast<int>(rows), static_cast<int>(columns), static_cast<int>(l.padded), static_cast<int>(l.small),
-                   static_cast<int>(l.small_padded), {}, 0, 0, k.a, k.b, k.c};
+                   static_cast<int>(l.small_padded), {}, 0, 0, l.splits, l.splits > 1 ? partial : nullptr, k.a, k.b, k.c};
         const auto all = [&](auto tall) -> int {
             constexpr bool kTall = decltype(tall)::value;
             if (const int rc = launch_step<kGram, kTall, E, G>(a, matrices, stream)) return rc;
+            if (l.splits > 1) {
+                a.each = static_cast<uint32_t>(pairs_of(l.small, kSumSide));
+                gram_sum_kernel<E><<<static_cast<unsigned>(matrices * a.each), kSumThreads, 0, stream>>>(a);
+                if (const int rc = launched()) return rc;
+            }
             a.out = f;
             if (const int rc = launch_step<kSquare, false, E, G>(a, matrices, stream)) return rc;
             a.out = next;
