@@ -338,10 +338,11 @@ struct Resident {
     }
 };
 
-__device__ __forceinline__ tile_acc multiply_split(chunk16 a, chunk16 a_low, chunk16 b, chunk16 b_low, tile_acc c) {
-    c = multiply<half_t>(a, b_low, c);
-    c = multiply<half_t>(a_low, b, c);
-    return multiply<half_t>(a, b, c);
+// (the products with a lo have sums of their own: see Product::low)
+__device__ __forceinline__ void multiply_split(chunk16 a, chunk16 a_low, chunk16 b, chunk16 b_low, tile_acc& high, tile_acc& low) {
+    low = multiply<half_t>(a, b_low, low);
+    low = multiply<half_t>(a_low, b, low);
+    high = multiply<half_t>(a, b, high);
 }
 
 __host__ __device__ constexpr int resident_pitch(int padded) { return padded * 4; }
@@ -352,7 +353,8 @@ __host__ __device__ constexpr int round_to_32(int n) { return (n + 31) / 32 * 32
 template <class G, int kTiles, int kBlocks>
 __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, int columns, int steps, Coefficients k, const G* __restrict__ g, G* __restrict__ result) {
     __shared__ __attribute__((aligned(1024))) char lds[kMostResident];
-    constexpr int kPadded = 16 * kTiles, kLines = kPadded / 32, kTogether = kBlocks > 1 ? 2 : 1;
+    constexpr int kPadded = 16 * kTiles, kLines = kPadded / 32, kTogether = kBlocks > 1 && kTiles <= 4 ? 2 : 1;
+    constexpr int kUnroll = kTiles <= 4 ? kLines : 1;  // (more would not fit the registers)
     const bool tall = rows > columns;
     const int small = min(rows, columns), large = max(rows, columns), large_padded = (large + 63) / 64 * 64;
     const Resident x{lds, resident_pitch(large_padded)}, s{lds + kPadded * x.pitch, resident_pitch(kPadded)};
@@ -417,18 +419,18 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
         for (int u = 0; u < kMostUnits; ++u) {
             const int unit = u * kResidentWaves + wave, m = unit % kTiles * 16, n = unit / kTiles * 32;
             if (unit >= kUnits) continue;
-            of_s[u][0] = of_s[u][1] = tile_acc{};
+            tile_acc high[2] = {}, low[2] = {};
             for (int first = 0; first < large_padded / 32; first += 2) {
 #pragma unroll
                 for (int line = first; line < first + 2; ++line) {
                     const chunk16 a = x.across(m, line, 0), a_low = x.across(m, line, 1);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) of_s[u][h] = multiply_split(a, a_low, x.across(n + 16 * h, line, 0), x.across(n + 16 * h, line, 1), of_s[u][h]);
+                    for (int h = 0; h < 2; ++h) multiply_split(a, a_low, x.across(n + 16 * h, line, 0), x.across(n + 16 * h, line, 1), high[h], low[h]);
                 }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                of_s[u][h] *= kPerScale;
+                of_s[u][h] = (high[h] + low[h]) * kPerScale;
                 s.store<4>(n + 16 * h + l16, m + q4, of_s[u][h]);
             }
         }
@@ -437,15 +439,15 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
         for (int u = 0; u < kMostUnits; ++u) {
             const int unit = u * kResidentWaves + wave, m = unit % kTiles * 16, n = unit / kTiles * 32;
             if (unit >= kUnits) continue;
-            tile_acc square[2] = {};
-#pragma unroll
+            tile_acc high[2] = {}, low[2] = {};
+#pragma unroll kUnroll
             for (int line = 0; line < kLines; ++line) {
                 const chunk16 a = s.across(m, line, 0), a_low = s.across(m, line, 1);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) square[h] = multiply_split(a, a_low, s.across(n + 16 * h, line, 0), s.across(n + 16 * h, line, 1), square[h]);
+                for (int h = 0; h < 2; ++h) multiply_split(a, a_low, s.across(n + 16 * h, line, 0), s.across(n + 16 * h, line, 1), high[h], low[h]);
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) of_s[u][h] = k.b * of_s[u][h] + (k.c * kPerScale) * square[h];
+            for (int h = 0; h < 2; ++h) of_s[u][h] = k.b * of_s[u][h] + (k.c * kPerScale) * (high[h] + low[h]);
         }
         __syncthreads();
 #pragma unroll
@@ -461,8 +463,8 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
 #pragma unroll
         for (int b = 0; b < kBlocks; b += kTogether) {
             if ((b * kResidentWaves + wave) * 16 >= large_padded) continue;
-            tile_acc acc[kTogether][kTiles] = {};
-#pragma unroll
+            tile_acc high[kTogether][kTiles] = {}, low[kTogether][kTiles] = {};
+#pragma unroll kUnroll
             for (int line = 0; line < kLines; ++line) {
                 chunk16 a[kTogether][2];
 #pragma unroll
@@ -475,7 +477,7 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
                 for (int n = 0; n < kTiles; ++n) {
                     const chunk16 f = s.across(n * 16, line, 0), f_low = s.across(n * 16, line, 1);
 #pragma unroll
-                    for (int t = 0; t < kTogether; ++t) acc[t][n] = multiply_split(a[t][0], a[t][1], f, f_low, acc[t][n]);
+                    for (int t = 0; t < kTogether; ++t) multiply_split(a[t][0], a[t][1], f, f_low, high[t][n], low[t][n]);
                 }
             }
 #pragma unroll
@@ -484,7 +486,7 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
                 if (b + t >= kBlocks || m >= large_padded) continue;
 #pragma unroll
                 for (int n = 0; n < kTiles; ++n) {
-                    own[b + t][n] = k.a * own[b + t][n] + acc[t][n] * kPerScale;
+                    own[b + t][n] = k.a * own[b + t][n] + (high[t][n] + low[t][n]) * kPerScale;
                     if (!last) x.store<4>(n * 16 + l16, m + q4, own[b + t][n]);
                 }
             }
@@ -588,9 +590,9 @@ template <class E>
 Layout layout_of(int64_t matrices, int64_t rows, int64_t columns) {
     constexpr int kBytes = ProductType<E>::kBytes, kDepth = ProductType<E>::kDepth;
     Layout l;
-    l.padded = (columns + kDepth - 1) / kDepth * kDepth;
+    l.padded = (columns + 31) / 32 * 32;
     l.small = std::min(rows, columns);
-    l.small_padded = (l.small + kDepth - 1) / kDepth * kDepth;
+    l.small_padded = (l.small + 31) / 32 * 32;
     l.x = matrices * rows * l.padded * kBytes;
     l.s = matrices * l.small * l.small_padded * kBytes;
     l.pieces = static_cast<int>(std::min<int64_t>(kMostPieces, (rows * columns + 16383) / 16384));
@@ -626,7 +628,12 @@ int launch_step(StepArgs a, int64_t matrices, hipStream_t stream) {
     if constexpr (std::is_same_v<E, half_t>) {
         if (huge >= 128) return launch(std::common_type<Product<E, kAlongM, kAlongN, 256, 256, 4, 2, Chunks::kDirect>>{});
     }
-    if (small_tiles(matrices, side_m, side_n, kStage != kUpdate)) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, Chunks::kDirect, 4>>{});
+    if (small_tiles(matrices, side_m, side_n, kStage != kUpdate)) {
+        // (of a few workgroups each has a compute unit's LDS to itself, for loads ahead; of many, two share it)
+        const int64_t items = matrices * (kStage == kUpdate ? ((side_m + 63) / 64) * ((side_n + 63) / 64) : pairs_of(a.small, 64)) * (kStage == kGram ? a.splits : 1);
+        if (items > 256) return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, Chunks::kDirect, 2>>{});
+        return launch(std::common_type<Product<E, kAlongM, kAlongN, 64, 64, 2, 2, Chunks::kDirect, 4>>{});
+    }
     return launch(std::common_type<Product<E, kAlongM, kAlongN, 128, 128, 2, 2, Chunks::kDirect>>{});
 }
 

@@ -307,19 +307,31 @@ struct Product {
     __device__ __forceinline__ static int wave_m() { return wave() / kWavesN * (kM / kWavesM); }
     __device__ __forceinline__ static int wave_n() { return wave() % kWavesN * (kN / kWavesN); }
 
-    __device__ __forceinline__ void multiply_all(const chunk16 (&m)[kTilesM], const chunk16 (&n)[kTilesN]) {
+    // Sums of products with a lo, 2^-11 of the others: on their own they round as much less, and the others a third as often.
+    tile_acc low[kParts == 2 ? kTilesM : 1][kParts == 2 ? kTilesN : 1];
+
+    template <int kI, int kJ>
+    __device__ __forceinline__ static void multiply_all(const chunk16 (&m)[kTilesM], const chunk16 (&n)[kTilesN], tile_acc (&to)[kI][kJ]) {
         using Part = std::conditional_t<std::is_same_v<E, split_t>, half_t, E>;
 #pragma unroll
         for (int i = 0; i < kTilesM; ++i)
 #pragma unroll
-            for (int j = 0; j < kTilesN; ++j) acc[i][j] = multiply<Part>(m[i], n[j], acc[i][j]);
+            for (int j = 0; j < kTilesN; ++j) to[i][j] = multiply<Part>(m[i], n[j], to[i][j]);
     }
     __device__ __forceinline__ void multiply_half(const Fragments& f) {
         if constexpr (kParts == 2) {
-            multiply_all(f.m[0], f.n[1]);
-            multiply_all(f.m[1], f.n[0]);
+            multiply_all(f.m[0], f.n[1], low);
+            multiply_all(f.m[1], f.n[0], low);
         }
-        multiply_all(f.m[0], f.n[0]);
+        multiply_all(f.m[0], f.n[0], acc);
+    }
+    __device__ __forceinline__ void add_low() {
+        if constexpr (kParts == 2) {
+#pragma unroll
+            for (int i = 0; i < kTilesM; ++i)
+#pragma unroll
+                for (int j = 0; j < kTilesN; ++j) acc[i][j] += low[i][j];
+        }
     }
 
     // Where the sums begin: f(m), for the four results from m on, of every n.
@@ -329,7 +341,10 @@ struct Product {
         for (int i = 0; i < kTilesM; ++i) {
             const tile_acc v = f(wave_m() + 16 * i + static_cast<int>(threadIdx.x) % 64 / 16 * 4);
 #pragma unroll
-            for (int j = 0; j < kTilesN; ++j) acc[i][j] = v;
+            for (int j = 0; j < kTilesN; ++j) {
+                acc[i][j] = v;
+                if constexpr (kParts == 2) low[i][j] = tile_acc{};
+            }
         }
     }
     static constexpr auto kZero = [](int) { return tile_acc{}; };
@@ -397,6 +412,7 @@ struct Product {
         turn(even, odd, lds + here, 1);
         multiply_half(odd);
         also(odd.n[0]);
+        add_low();
         if constexpr (kDirect) wait_for_loads<0>();  // (nothing is on its way into the LDS when the workgroup ends)
     }
 
