@@ -236,7 +236,7 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_kernel(RowsArgs 
 #pragma unroll
         for (int k = 0; k < kNarrowGroups; ++k) {
             const int first = row + 16 * k, left = t.rows - first;
-            const auto buffer = buffer_of(in + static_cast<int64_t>(first) * stride, left <= 0 ? 0 : static_cast<int64_t>(left - 1) * stride + deep_bytes);
+            const auto buffer = buffer_of(in + static_cast<int64_t>(first) * stride, left <= 0 ? 0 : (min(left, 16) - 1) * stride + deep_bytes);
 #pragma unroll
             for (int l = 0; l < kLines; ++l) r[k][l] = load_chunk16(buffer, at[l]);
         }
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, 
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) first += __shfl_xor(first, d), mine = max(mine, static_cast<uint32_t>(__shfl_xor(mine, d)));
-    if (mine <= 1) return;
+    if (mine <= 1 || first + mine > a.pieces) return;  // (the second: offsets that no plan has)
     const int64_t weights = static_cast<int64_t>(a.outputs) * a.channels, n = weights + (a.bias != nullptr ? a.outputs : 0);
     const int slice = static_cast<int>(threadIdx.x) / kResults, result = static_cast<int>(threadIdx.x) % kResults;
     // (a lane has kWide results: with one slice four, where those of every piece and expert begin on four)
@@ -544,7 +544,7 @@ struct WeightPlan {
 };
 WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
     WeightPlan p;
-    p.side = channels <= 64 || outputs <= 64 ? 64 : kSize == 2 && channels % 8 == 0 && outputs % 8 == 0 && channels >= 256 && outputs >= 256 && rows * channels * outputs >= int64_t{1} << 34 ? 256 : 128;
+    p.side = channels <= 64 || outputs <= 64 ? 64 : kSize == 2 && channels % 8 == 0 && outputs % 8 == 0 && channels >= 256 && outputs >= 256 && static_cast<double>(rows) * static_cast<double>(channels * outputs) >= 0x1p34 ? 256 : 128;
     const int64_t side = p.side;
     p.tiles = ((channels + side - 1) / side) * ((outputs + side - 1) / side);
     const int64_t wanted = ((side == 256 ? 512 : side == 128 ? 1024 : 2048) + p.tiles - 1) / p.tiles;  // pieces for four workgroups to a compute unit

@@ -134,7 +134,7 @@ class Muon(torch.optim.Optimizer):
         p = (1 - lr weight_decay) p - lr scale orthogonalise(u)
 
     with ``scale`` sqrt(max(1, rows / columns)), or 0.2 sqrt(max(rows, columns)) with ``match_rms_adamw``.  The average m is float32, u of the parameter's type; parameters of one
-    size go through the products together.  Tables, norms and biases take another optimiser.  (A captured step keeps the ``lr`` that it was captured with.)
+    size go through the products together.  Tables, norms and biases take another optimiser.  (A captured step keeps the ``lr`` that it was captured with, and is not a parameter's first.)
     """
 
     def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, steps=5, coefficients=COEFFICIENTS, eps=1e-7, match_rms_adamw=False):
@@ -173,6 +173,8 @@ class Muon(torch.optim.Optimizer):
                     raise RuntimeError("Muon: gradients must be dense and of the parameter's type")
                 state = self.state[p]
                 if not state:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("Muon: a step has to be taken before one is captured (a graph would begin the averages anew each time)")
                     state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 together.setdefault((tuple(p.shape), p.dtype, p.device), []).append((p, p.grad.contiguous(), state["momentum_buffer"]))
             for (shape, _, _), members in together.items():

@@ -14,7 +14,7 @@ Unlike the kernel benchmark (``bench.py``) these figures include everything a us
 pays: output allocation, the loss, the gradient layout change and the optimiser walking the whole
 table.
 
-    python -m permutohedral_encoding_amd.perf_sweep [--dims 2 3 4 5 6] [--points 524288] [--iters 300] [--fused-optimizer] [--contiguous-output] [--decoder]
+    python -m permutohedral_encoding_amd.perf_sweep [--dims 2 3 4 5 6] [--points 524288] [--iters 300] [--fused-optimizer] [--contiguous-output] [--decoder] [--experts]
 
 ``--consumers`` instead runs what the layer after the encoding does with the (N, 48) result of 2^20 points,
 a few times each and meant to be run under a kernel trace: ``torch.nn.Linear``, ``torch.cat`` with
@@ -31,6 +31,10 @@ window) for three of them.  A renderer delivers the second kind, a caller who so
 ``--decoder`` trains the encoding of ``--points`` points and a decoder of residual blocks behind it (``--width`` channels, ``--blocks`` blocks of a gated
 layer and a layer back, normed before and after) once with torch's layers and once with those of ``layers.py``, and reports points per second and the memory
 that a step adds at its peak.  The steps are those of training: forward, loss, backward, AdamW on the table and the decoder.
+
+``--experts`` does the same with a decoder of experts: each point goes to 2 of ``--number`` experts by a learned router, an expert is a layer to ``--width``
+channels, gelu and a layer back to 32, and the experts' stacked weights are stepped by Muon.  torch's row sorts the choices, multiplies expert by expert and
+orthogonalises in torch's products.
 """
 import argparse
 import json
@@ -247,6 +251,94 @@ def decoder(nr_points, iters, warmup, width=64, blocks=2, dtype=torch.float32, p
     return rows
 
 
+def experts(nr_points, iters, warmup, width=64, number=16, dtype=torch.float32, pos_dim=3, levels=24, log2_capacity=18):
+    """One row for torch's operations and one for those of layers.py and optim.py, on the same parameters and points."""
+    import torch.nn.functional as F
+
+    from . import layers
+    from .optim import COEFFICIENTS, AdamW, Muon
+
+    choices, channels = 2, 32
+
+    def with_torch(x, p):
+        logits, chosen = torch.topk(F.linear(x, p["router"]).float(), choices, dim=-1)
+        weights = F.softmax(logits, dim=-1).to(x.dtype)
+        order = torch.argsort(chosen.flatten(), stable=True)
+        counts = torch.bincount(chosen.flatten(), minlength=number).tolist()
+        rows = x[order // choices].split(counts)
+        y = torch.cat([F.linear(F.gelu(F.linear(r, p["up"][e], p["up_bias"][e])), p["down"][e], p["down_bias"][e]) for e, r in enumerate(rows)])
+        back = torch.empty_like(order)
+        back[order] = torch.arange(order.numel(), device=order.device)
+        return F.linear((y[back].view(-1, choices, channels) * weights[..., None]).sum(1), p["out"])
+
+    def with_layers(x, p):
+        weights, routing = layers.route(layers.linear(x, p["router"]), choices)
+        h = layers.expert_linear(layers.dispatch(x, routing), p["up"], p["up_bias"], routing)
+        y = layers.expert_linear(layers.activation(h), p["down"], p["down_bias"], routing)
+        return layers.linear(layers.combine(y, weights, routing), p["out"])
+
+    class TorchMuon(torch.optim.Optimizer):
+        def __init__(self, params, lr, momentum=0.95):
+            super().__init__(params, dict(lr=lr, momentum=momentum))
+
+        @torch.no_grad()
+        def step(self):
+            a, b, c = COEFFICIENTS
+            for group in self.param_groups:
+                for w in group["params"]:
+                    if w.grad is None:
+                        continue
+                    kept = self.state[w].setdefault("momentum", torch.zeros_like(w, dtype=torch.float32))
+                    grad = w.grad.float()
+                    kept.lerp_(grad, 1 - group["momentum"])
+                    x = grad.lerp(kept, group["momentum"])
+                    tall = x.shape[-2] > x.shape[-1]
+                    x = x.transpose(-2, -1).contiguous() if tall else x
+                    x = x / (x.norm(dim=(-2, -1), keepdim=True) + 1e-7)
+                    for _ in range(5):
+                        s = x @ x.transpose(-2, -1).contiguous()
+                        x = a * x + (b * s + c * (s @ s)) @ x
+                    x = x.transpose(-2, -1) if tall else x
+                    w.add_(x.to(w.dtype), alpha=-group["lr"] * max(1.0, w.shape[-2] / w.shape[-1]) ** 0.5)
+
+    rows = []
+    for name, forward, stacks in (("torch", with_torch, TorchMuon), ("layers", with_layers, Muon)):
+        torch.manual_seed(0)
+        enc = PermutoEncoding(pos_dim, 1 << log2_capacity, levels, 2, np.geomspace(1.0, 1e-4, num=levels))
+
+        def weight(*sizes):
+            return (torch.randn(*sizes, device="cuda") / sizes[-1] ** 0.5).to(dtype).requires_grad_(True)
+
+        def zeros(*sizes):
+            return torch.zeros(*sizes, device="cuda", dtype=dtype, requires_grad=True)
+
+        p = {"router": weight(number, enc.output_dims()), "up": weight(number, width, enc.output_dims()), "up_bias": zeros(number, width),
+             "down": weight(number, channels, width), "down_bias": zeros(number, channels), "out": weight(3, channels)}
+        steps = (AdamW(enc.parameters(), betas=(0.9, 0.99), eps=1e-15, weight_decay=0.0, lr=1e-3), stacks([p["up"], p["down"]], lr=1e-2),
+                 torch.optim.AdamW([p["router"], p["up_bias"], p["down_bias"], p["out"]], lr=1e-3, weight_decay=0.0))
+        points = torch.rand(nr_points, pos_dim, device="cuda") - 0.5
+
+        def step():
+            loss = ((forward(enc(points).to(dtype), p).float() - 0.5) ** 2).mean()
+            for opt in steps:
+                opt.zero_grad()
+            loss.backward()
+            for opt in steps:
+                opt.step()
+
+        for _ in range(2):
+            step()
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        step()
+        peak = torch.cuda.max_memory_allocated() - before
+        rows.append({"layers": name, "points": nr_points, "width": width, "experts": number, "dtype": str(dtype).split(".")[-1],
+                     "train": _timed(step, nr_points, iters, warmup), "peak_bytes": peak})
+        print(f"| {name} | {rows[-1]['train']:.3g} | {peak / 2 ** 20:.0f} |", flush=True)
+    return rows
+
+
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--dims", type=int, nargs="+", default=[2, 3, 4, 5, 6])
@@ -260,7 +352,9 @@ def main():
     ap.add_argument("--consumers", action="store_true", help="run the consumers of the forward result instead (for a kernel trace)")
     ap.add_argument("--point-orders", action="store_true", help="time forward and table backward on unordered, ray-ordered and Z-ordered points instead")
     ap.add_argument("--decoder", action="store_true", help="train encoding and decoder with torch's layers and with those of layers.py instead")
-    ap.add_argument("--width", type=int, default=64, help="channels of the decoder")
+    ap.add_argument("--experts", action="store_true", help="train encoding and a decoder of experts with torch's operations and with those of layers.py and optim.py instead")
+    ap.add_argument("--number", type=int, default=16, help="experts of the decoder")
+    ap.add_argument("--width", type=int, default=64, help="channels of the decoder, or of an expert between its layers")
     ap.add_argument("--blocks", type=int, default=2, help="residual blocks of the decoder")
     ap.add_argument("--dtype", choices=("float32", "bfloat16"), default="float32", help="type of the decoder")
     args = ap.parse_args()
@@ -276,6 +370,11 @@ def main():
         print("| layers | training (points/s) | memory of a step (MiB) |")
         print("|---|---|---|")
         print(json.dumps(decoder(args.points, args.iters, args.warmup, args.width, args.blocks, getattr(torch, args.dtype))))
+        return
+    if args.experts:
+        print("| layers | training (points/s) | memory of a step (MiB) |")
+        print("|---|---|---|")
+        print(json.dumps(experts(args.points, args.iters, args.warmup, args.width, args.number, getattr(torch, args.dtype))))
         return
     print("| pos_dim | inference (points/s) | training, table grad (points/s) | training, table + position grad (points/s) |")
     print("|---|---|---|---|")

@@ -451,3 +451,135 @@ def test_on_another_stream_and_in_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(want, eager, grad)))
+
+
+def decoder(x, logits, up, bias, down):
+    weights, routing = layers.route(logits, 2)
+    h = layers.activation(layers.expert_linear(layers.dispatch(x, routing), up, bias, routing), keep_8bit=False)
+    return layers.combine(layers.expert_linear(h, down, None, routing), weights, routing)
+
+
+def decoder_inputs(rows, number, seed, dtype=torch.float32):
+    return [random(s, seed + i, t) / 4 for i, (s, t) in enumerate((((rows, 40), dtype), ((rows, number), torch.float32), ((number, 72, 40), dtype), ((number, 72), dtype),
+                                                                   ((number, 40, 72), dtype)))]
+
+
+def test_two_graphs_of_a_decoder_at_once():
+    """Plans of several launches and weight gradients of several pieces have workspaces: two graphs, and eager work beside them, share none."""
+    rows, number = 20000, 3
+    grad = random((rows, 40), 9)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    given = [[t.requires_grad_(True) for t in decoder_inputs(rows, number, 100 * k)] for k in range(2)]
+    graphs, results = [], []
+    for g, s in zip(given, streams):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            out = decoder(*g)
+            results.append([out, *torch.autograd.grad(out, g, grad)])
+    for seed in range(3):
+        new = [decoder_inputs(rows, number, 1000 * seed + 50 * k) for k in range(2)]
+        with torch.no_grad():
+            for g, n in zip(given, new):
+                for a, b in zip(g, n):
+                    a.copy_(b)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        wanted = []
+        for n in new:  # (on the current stream, meanwhile)
+            eager = [t.clone().requires_grad_(True) for t in n]
+            out = decoder(*eager)
+            wanted.append([out, *torch.autograd.grad(out, eager, grad)])
+        torch.cuda.synchronize()
+        for got, want in zip(results, wanted):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_padded_batch():
+    """Rows of padding have logits of -inf alone: nothing of what stands in them goes anywhere."""
+    rows, padding, number = 300, 77, 4
+    given = decoder_inputs(rows, number, 1)
+    full = [torch.cat([given[0], torch.full((padding, 40), math.nan, device="cuda")]), torch.cat([given[1], torch.full((padding, number), -math.inf, device="cuda")]), *given[2:]]
+    grad = random((rows, 40), 9)
+    results = []
+    for tensors, g in ((given, grad), (full, torch.cat([grad, torch.full((padding, 40), math.nan, device="cuda")]))):
+        tensors = [t.clone().requires_grad_(True) for t in tensors]
+        out = decoder(*tensors)
+        results.append([out.detach(), *torch.autograd.grad(out, tensors, g)])
+    (out, dx, dlogits, *dw), (all_out, all_dx, all_dlogits, *all_dw) = results
+    assert torch.equal(all_out[:rows], out) and torch.equal(all_dx[:rows], dx) and torch.equal(all_dlogits[:rows], dlogits)
+    assert not any(bool(t[rows:].any()) for t in (all_out, all_dx, all_dlogits))
+    # (the rows of each expert are the same, in the same order)
+    assert all(torch.equal(a, b) for a, b in zip(dw, all_dw))
+
+
+def test_an_expert_twice_in_a_row():
+    rows = 130
+    experts = torch.randint(0, 3, (rows, 1), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").repeat(1, 3)
+    routing = layers.routing(experts, 3)
+    assert sorted(routing.positions.flatten().tolist()) == list(range(3 * rows))
+    x, weights = random((rows, 24), 1).requires_grad_(True), random((rows, 3), 2).requires_grad_(True)
+    out = layers.combine(layers.dispatch(x, routing), weights, routing)
+    grad = random((rows, 24), 3)
+    dx, dw = torch.autograd.grad(out, (x, weights), grad)
+    xd, wd, gd = x.detach().double(), weights.detach().double(), grad.double()
+    bound = 16 * ref.U * wd.abs().sum(1, keepdim=True)
+    assert_within(out, xd * wd.sum(1, keepdim=True), bound * xd.abs(), "out")
+    assert_within(dx, gd * wd.sum(1, keepdim=True), bound * gd.abs(), "dx")
+    assert_within(dw, (xd * gd).sum(1, keepdim=True).expand(-1, 3), 64 * ref.U * (xd * gd).abs().sum(1, keepdim=True).expand(-1, 3), "dw")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_expert_linear_of_wide_layers(dtype):
+    """Tiles of 256 x 256 in each direction, the last of them in quarters; experts of no row, of one, and of nearly all; rows without an expert; rows that are further apart, on
+    16 bytes and not."""
+    rows, number, channels, outputs = 100000, 7, 384, 520
+    generator = torch.Generator(device="cuda").manual_seed(5)
+    experts = torch.randint(0, 4, (rows, 1), generator=generator, device="cuda").clamp_(max=2)  # (half of them to expert 2)
+    experts[:300] = -1
+    experts[1000] = 5
+    experts[2000:2300] = 6
+    routing = layers.routing(experts, number)
+    total = int(routing.offsets[-1])
+    assert total == rows - 300
+    weight = random((number, outputs, channels), 3, TYPES[dtype]).requires_grad_(True)
+    bias = random((number, outputs), 4, TYPES[dtype]).requires_grad_(True)
+    for extra in (0, 8, 3):
+        x, grad = random((rows, channels + extra), 1, TYPES[dtype])[:, :channels], random((rows, outputs + extra), 2, TYPES[dtype])[:, :outputs]
+        x[total:] = math.nan
+        grad[total:] = math.nan
+        x.requires_grad_(True)
+        y = layers.expert_linear(x, weight, bias, routing)
+        grads = dict(zip(("dx", "dweight", "dbias"), torch.autograd.grad(y, (x, weight, bias), grad)))
+        want = products(x, weight, bias, grad, routing.offsets.tolist())
+        for name, got in {"y": y, **grads}.items():
+            value, magnitude, chain = want[name]
+            assert_within(got, value, chain * ref.U * magnitude + ref.half_step(value, TYPES[dtype]), name)
+
+
+def test_without_gradients_and_under_autocast():
+    given = decoder_inputs(200, 4, 1, torch.bfloat16)
+    want = decoder(*given)
+    for context in (torch.no_grad(), torch.inference_mode(), torch.autocast("cuda", dtype=torch.float16)):
+        with context:
+            assert torch.equal(decoder(*given), want)
+    # a routing made in inference mode is saved like any other tensor made there: not at all
+    leaf = given[0].clone().requires_grad_(True)
+    with torch.inference_mode():
+        _, routing = layers.route(given[1], 2)
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        layers.dispatch(leaf, routing)
+    # what the backward reads is not to be changed before
+    weights, routing = layers.route(given[1].clone().requires_grad_(True), 2)
+    total = weights.sum()
+    routing.experts.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        total.backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_sweep_trains_a_decoder_of_experts_with_both(dtype):
+    from permutohedral_encoding_amd import perf_sweep
+    rows = perf_sweep.experts(1000, 3, 1, width=40, number=5, dtype=dtype, levels=6, log2_capacity=10)
+    assert [r["layers"] for r in rows] == ["torch", "layers"] and all(r["train"] > 0 for r in rows)

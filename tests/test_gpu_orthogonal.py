@@ -237,3 +237,29 @@ def test_a_decoder_of_experts_trains_with_muon():
         opt.step()
         for p, b in zip(opt.param_groups[0]["params"], before):
             assert float(((p - b) * p.grad).sum()) < 0.0  # (a matrix and what its singular values are made equal of have a positive product)
+
+
+def test_a_captured_step_is_not_the_first():
+    start = updates(3, 40, 24, torch.float32, seed=1, scale=1.0)
+    p, q = (torch.nn.Parameter(start.clone()) for _ in range(2))
+    p.grad, q.grad = (torch.empty_like(start) for _ in range(2))
+    eager, captured = optim.Muon([p]), optim.Muon([q])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), pytest.raises(RuntimeError, match="before one is captured"):
+        captured.step()
+    graphs = []
+    for seed in range(5):
+        grad = updates(3, 40, 24, torch.float32, seed=10 + seed)
+        p.grad.copy_(grad)
+        q.grad.copy_(grad)
+        eager.step()
+        if seed == 0:
+            captured.step()
+        elif seed == 1:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[0]):
+                captured.step()
+        if graphs:
+            graphs[0].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q)
