@@ -349,36 +349,25 @@ struct WeightArgs {
     int64_t pieces;
 };
 
-// dW and db of a piece of an expert's rows.
-template <class P>
-__global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs a) {
-    __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
-    const uint32_t item = a.spread.item(), piece = item / a.tiles, tile = item % a.tiles;
-    if (item >= a.spread.items) return;
-    const RowTile t = row_tile<false>(a.offsets, a.experts, a.rows, piece, a.most);
-    if (t.expert < 0) return;
-    const int c0 = static_cast<int>(tile % a.channel_tiles) * P::kM, o0 = static_cast<int>(tile / a.channel_tiles) * P::kN;
-    const bool bias = a.bias != nullptr && c0 == 0 && P::wave_m() == 0;
-    const Operand m{static_cast<const char*>(a.x) + (static_cast<int64_t>(t.first) * a.x_stride + c0) * kSize, a.x_stride * kSize, t.rows, min(a.channels - c0, P::kM) * kSize};
-    const Operand n{static_cast<const char*>(a.grad) + (static_cast<int64_t>(t.first) * a.grad_stride + o0) * kSize, a.grad_stride * kSize, t.rows,
-                    min(a.outputs - o0, P::kN) * kSize};
-    P p;
-    // the sums of dy itself: of 16-bit types its products with ones, of fp32, whose products take eight times as long, each lane's own k
-    tile_acc bias_acc[P::kTilesN] = {};
+// Adds what a step has of dy to a wave's sums of dy itself: of 16-bit types its products with ones, of fp32, whose products take eight times as long, each lane's own k.
+template <int kTilesN>
+__device__ __forceinline__ void add_bias_grads(const chunk16 (&grad)[kTilesN], tile_acc (&bias_acc)[kTilesN]) {
     const uint32_t one = PENC_TYPE == PENC_FP16 ? 0x3C003C00u : 0x3F803F80u;
     const chunk16 ones = {one, one, one, one};
-    p.run(lds, m, n, t.rows, P::kZero, [&](const chunk16 (&grad)[P::kTilesN]) {
-        if (!bias) return;
 #pragma unroll
-        for (int j = 0; j < P::kTilesN; ++j) {
-            if constexpr (PENC_TYPE == PENC_FP32) {
+    for (int j = 0; j < kTilesN; ++j) {
+        if constexpr (PENC_TYPE == PENC_FP32) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) bias_acc[j][k] += __uint_as_float(grad[j][k]);
-            } else {
-                bias_acc[j] = multiply<Value>(ones, grad[j], bias_acc[j]);
-            }
+            for (int k = 0; k < 4; ++k) bias_acc[j][k] += __uint_as_float(grad[j][k]);
+        } else {
+            bias_acc[j] = multiply<Value>(ones, grad[j], bias_acc[j]);
         }
-    });
+    }
+}
+
+// Stores what a workgroup has of dW, and the waves with `bias` of db: the results where the expert's rows are one piece, else the piece's sums.
+template <class P>
+__device__ __forceinline__ void store_weight_grads(const WeightArgs& a, const RowTile& t, uint32_t piece, int c0, int o0, const P& p, bool bias, tile_acc (&bias_acc)[P::kTilesN]) {
     if constexpr (PENC_TYPE == PENC_FP32) {
 #pragma unroll
         for (int j = 0; j < P::kTilesN; ++j) {
@@ -402,6 +391,117 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
         if (whole) static_cast<Value*>(a.bias)[static_cast<int64_t>(t.expert) * a.outputs + o] = static_cast<Value>(bias_acc[j][0]);
         else a.sums[a.pieces * n_weights + static_cast<int64_t>(piece) * a.outputs + o] = bias_acc[j][0];
     }
+}
+
+// dW and db of a piece of an expert's rows.
+template <class P>
+__global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
+    const uint32_t item = a.spread.item(), piece = item / a.tiles, tile = item % a.tiles;
+    if (item >= a.spread.items) return;
+    const RowTile t = row_tile<false>(a.offsets, a.experts, a.rows, piece, a.most);
+    if (t.expert < 0) return;
+    const int c0 = static_cast<int>(tile % a.channel_tiles) * P::kM, o0 = static_cast<int>(tile / a.channel_tiles) * P::kN;
+    const bool bias = a.bias != nullptr && c0 == 0 && P::wave_m() == 0;
+    const Operand m{static_cast<const char*>(a.x) + (static_cast<int64_t>(t.first) * a.x_stride + c0) * kSize, a.x_stride * kSize, t.rows, min(a.channels - c0, P::kM) * kSize};
+    const Operand n{static_cast<const char*>(a.grad) + (static_cast<int64_t>(t.first) * a.grad_stride + o0) * kSize, a.grad_stride * kSize, t.rows,
+                    min(a.outputs - o0, P::kN) * kSize};
+    P p;
+    tile_acc bias_acc[P::kTilesN] = {};
+    p.run(lds, m, n, t.rows, P::kZero, [&](const chunk16 (&grad)[P::kTilesN]) {
+        if (bias) add_bias_grads(grad, bias_acc);
+    });
+    store_weight_grads(a, t, piece, c0, o0, p, bias, bias_acc);
+}
+
+constexpr int kNarrowRing = 3, kTailBlocks = 256;
+
+// All gradients of a narrow layer, of at most 64 channels and outputs: x and dy are read once, where dx and dW on their own read dy twice.  A wave has the weights for some of dx's
+// columns in registers and reads, of each step that the workgroup brings into the LDS, the fragments for both products.  Workgroups behind those of the pieces clear dx behind the
+// last expert's rows.  2^20 x 64 by 64 fp32 (8 experts): 175 us, 4.7 TB/s, and 8 for the sums; dx and dW on their own 119 and 136, and 13.
+__global__ __launch_bounds__(kNarrowThreads) void expert_narrow_grads_kernel(WeightArgs a, const void* weight, void* dx) {
+    using P = Product<Value, true, true, 64, 64, 2, 2, Chunks::kDirect, kNarrowRing>;
+    using Load = Loader<Value, true, 64, kNarrowThreads, Chunks::kDirect>;
+    using Tile = typename Load::Tile;
+    constexpr int kDepth = P::kDepth, kWeightSteps = 64 / kDepth;
+    constexpr int kRowTiles = kDepth / 16, kShare = 4 / kRowTiles, kTiles = 4 / kShare;  // of a step; waves to each; tiles of 16 columns that a wave has
+    constexpr int kLines = 64 * kSize / 64;                                             // 64 bytes of a row of dy
+    // the weights, until all waves have read them, have the room of the step that is loaded first in the loop
+    constexpr int kWeightsAt = (kNarrowRing - 1) * P::kStage;
+    static_assert(P::kThreads == kNarrowThreads && kWeightSteps * Tile::kSize <= P::kStage);
+    __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
+    if (blockIdx.x >= gridDim.x - kTailBlocks) {
+        const int routed = min(max(a.offsets[a.experts], 0), a.rows);
+        const int64_t chunks = static_cast<int64_t>(a.rows - routed) * a.channels * kSize / 16;
+        chunk16* const to = reinterpret_cast<chunk16*>(static_cast<Value*>(dx) + static_cast<int64_t>(routed) * a.channels);
+        for (int64_t i = static_cast<int64_t>(blockIdx.x - (gridDim.x - kTailBlocks)) * kNarrowThreads + threadIdx.x; i < chunks; i += kTailBlocks * kNarrowThreads) to[i] = chunk16{};
+        return;
+    }
+    const uint32_t piece = a.spread.item();
+    if (piece >= a.spread.items) return;
+    const RowTile t = row_tile<false>(a.offsets, a.experts, a.rows, piece, a.most);
+    if (t.expert < 0) return;
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+    const int64_t row_bytes = static_cast<int64_t>(a.channels) * kSize;
+    Load load_w(Operand{static_cast<const char*>(weight) + t.expert * a.outputs * row_bytes, row_bytes, a.outputs, static_cast<int>(row_bytes)});
+    Load load_m(Operand{static_cast<const char*>(a.x) + t.first * a.x_stride * kSize, a.x_stride * kSize, t.rows, static_cast<int>(row_bytes)});
+    Load load_n(Operand{static_cast<const char*>(a.grad) + t.first * a.grad_stride * kSize, a.grad_stride * kSize, t.rows, a.outputs * kSize});
+#pragma unroll
+    for (int k = 0; k < kWeightSteps; ++k) load_w.begin(lds_at + kWeightsAt + k * Tile::kSize);
+    int room = 0, here = 0;
+    const auto behind = [](int at) { return at + P::kStage == P::kLds ? 0 : at + P::kStage; };
+    const auto begin = [&] {
+        load_m.begin(lds_at + room);
+        load_n.begin(lds_at + room + Tile::kSize);
+        room = behind(room);
+    };
+    const auto meet = [&] {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    };
+#pragma unroll
+    for (int k = 0; k < kNarrowRing - 1; ++k) begin();
+    const int lane = threadIdx.x % 64, wave = P::wave(), row16 = wave / kShare * 16, m0 = wave % kShare * (16 * kTiles);
+    P p;
+    p.start(P::kZero);
+    const bool bias = a.bias != nullptr && P::wave_m() == 0;
+    tile_acc bias_acc[P::kTilesN] = {};
+    wait_for_loads<P::kLoads * (kNarrowRing - 1)>();
+    meet();
+    chunk16 w[kTiles][kLines];
+#pragma unroll
+    for (int l = 0; l < kLines; ++l)
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) w[i][l] = Tile::fragment(lds + kWeightsAt + l / 2 * Tile::kSize, m0 + 16 * i, l % 2, 0);
+    Value* const out = static_cast<Value*>(dx) + static_cast<int64_t>(t.first) * a.channels;
+    for (int first = 0; first < t.rows; first += kDepth) {
+        // This step is there for all waves, and all have read the one before, whose room the step kNarrowRing - 1 behind this one takes.
+        wait_for_loads<P::kLoads * (kNarrowRing - 2)>();
+        meet();
+        begin();
+        typename P::Fragments f[2];
+        f[0].read(lds + here, 0);
+        f[1].read(lds + here, 1);
+        chunk16 rows[kLines];
+#pragma unroll
+        for (int l = 0; l < kLines; ++l) rows[l] = *reinterpret_cast<const chunk16*>(lds + here + Tile::kSize + (row16 + lane % 16) * Tile::kRowBytes + Tile::place(row16 + lane % 16, l * 4 + lane / 16) * 16);
+        here = behind(here);
+        tile_acc acc[kTiles] = {};
+#pragma unroll
+        for (int l = 0; l < kLines; ++l)
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) acc[i] = multiply<Value>(w[i][l], rows[l], acc[i]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            p.multiply_half(f[h]);
+            if (bias) add_bias_grads(f[h].n[0], bias_acc);
+        }
+        const int row = first + row16;
+        store_sixteen_rows(acc, out + static_cast<int64_t>(row) * a.channels + m0, a.channels, t.rows - row, a.channels - m0);
+    }
+    wait_for_loads<0>();  // (nothing is on its way into the LDS when the workgroup ends)
+    store_weight_grads(a, t, piece, 0, 0, p, bias, bias_acc);
 }
 
 constexpr int kSumThreads = 256;
@@ -547,7 +647,9 @@ WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t 
     p.side = channels <= 64 || outputs <= 64 ? 64 : kSize == 2 && channels % 8 == 0 && outputs % 8 == 0 && channels >= 256 && outputs >= 256 && static_cast<double>(rows) * static_cast<double>(channels * outputs) >= 0x1p34 ? 256 : 128;
     const int64_t side = p.side;
     p.tiles = ((channels + side - 1) / side) * ((outputs + side - 1) / side);
-    const int64_t wanted = ((side == 256 ? 512 : side == 128 ? 1024 : 2048) + p.tiles - 1) / p.tiles;  // pieces for four workgroups to a compute unit
+    // pieces for four workgroups to a compute unit; of layers of one tile for the three that have room there at a time (2^20 x 64 by 64 fp32, all of the layer:
+    // 299 us, of twice as many 305, of 4, 8 and 2 to a compute unit 325, 316 and 347)
+    const int64_t wanted = p.tiles == 1 ? 3 * kUnits : ((side == 256 ? 512 : side == 128 ? 1024 : 2048) + p.tiles - 1) / p.tiles;
     int64_t most = experts >= wanted ? 2 * ((rows + experts - 1) / experts) : (rows + wanted - 1) / wanted;
     most = std::max<int64_t>((most + 63) / 64 * 64, 512);
     p.most = std::min<int64_t>(most, (int64_t{1} << 30));
@@ -564,6 +666,12 @@ int launch_weights(WeightArgs a, const WeightPlan& plan, hipStream_t stream) {
     // (pieces take different times: all dies work on the same ones)
     a.spread = Spread(items, a.tiles / 8);
     expert_weights_kernel<P><<<a.spread.grid(), P::kThreads, 0, stream>>>(a);
+    return launched();
+}
+
+int launch_narrow_grads(WeightArgs a, const WeightPlan& plan, const void* weight, void* dx, hipStream_t stream) {
+    a.spread = Spread(plan.pieces, 1);
+    expert_narrow_grads_kernel<<<a.spread.grid() + kTailBlocks, kNarrowThreads, 0, stream>>>(a, weight, dx);
     return launched();
 }
 
@@ -598,15 +706,20 @@ size_t expert_weights_workspace<PENC_TYPE>(int64_t rows, int64_t experts, int64_
 }
 
 template <>
-int expert_weights<PENC_TYPE>(int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t x_stride, const void* grad, int64_t grad_stride,
-                              const int32_t* offsets, void* weight, void* bias, void* workspace, hipStream_t stream) {
+int expert_grads<PENC_TYPE>(int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t x_stride, const void* grad, int64_t grad_stride,
+                            const void* weight, const int32_t* offsets, void* dx, void* dweight, void* dbias, void* workspace, hipStream_t stream) {
     const WeightPlan plan = weight_plan(rows, experts, channels, outputs);
     WeightArgs a{x, grad, x_stride, grad_stride, offsets, experts, static_cast<int>(rows), static_cast<int>(channels), static_cast<int>(outputs),
-                 static_cast<int>(plan.most), {}, 0, 0, weight, bias, static_cast<float*>(workspace), plan.pieces};
+                 static_cast<int>(plan.most), {}, 0, 0, dweight, dbias, static_cast<float*>(workspace), plan.pieces};
     const Chunks chunks = std::max(chunks_of(x, x_stride, channels), chunks_of(grad, grad_stride, outputs));
-    if (const int rc = chunks == Chunks::kDirect ? weights_of_experts<Chunks::kDirect>(a, plan, stream)
-                       : chunks == Chunks::kHeld ? weights_of_experts<Chunks::kHeld>(a, plan, stream)
-                                                 : weights_of_experts<Chunks::kSingle>(a, plan, stream))
+    const bool together = dx != nullptr && channels <= 64 && outputs <= 64 && chunks == Chunks::kDirect && aligned_to(weight, 16) && aligned_to(dx, 16);
+    if (dx != nullptr && !together) {
+        if (const int rc = expert_rows<PENC_TYPE>(true, rows, experts, channels, outputs, grad, grad_stride, weight, nullptr, offsets, dx, stream)) return rc;
+    }
+    if (const int rc = together                     ? launch_narrow_grads(a, plan, weight, dx, stream)
+                       : chunks == Chunks::kDirect ? weights_of_experts<Chunks::kDirect>(a, plan, stream)
+                       : chunks == Chunks::kHeld   ? weights_of_experts<Chunks::kHeld>(a, plan, stream)
+                                                   : weights_of_experts<Chunks::kSingle>(a, plan, stream))
         return rc;
     if (rows <= plan.most) return PENC_OK;
     const int64_t results = outputs * (channels + 1);

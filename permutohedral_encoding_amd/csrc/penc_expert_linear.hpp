@@ -12,8 +12,9 @@ int expert_rows(bool back, int64_t rows, int experts, int64_t wide, int64_t deep
                 const int32_t* offsets, void* out, hipStream_t stream);
 template <int kType>
 size_t expert_weights_workspace(int64_t rows, int64_t experts, int64_t channels, int64_t outputs);
+// dW, db (may be null) and, where it is not null, dx.
 template <int kType>
-int expert_weights(int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t x_stride, const void* grad, int64_t grad_stride,
-                   const int32_t* offsets, void* weight, void* bias, void* workspace, hipStream_t stream);
+int expert_grads(int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t x_stride, const void* grad, int64_t grad_stride, const void* weight,
+                 const int32_t* offsets, void* dx, void* dweight, void* dbias, void* workspace, hipStream_t stream);
 
 }  // namespace penc

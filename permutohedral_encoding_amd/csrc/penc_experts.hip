@@ -786,23 +786,30 @@ size_t penc_expert_weight_grad_workspace_bytes(int type, int64_t rows, int exper
     }
 }
 
-int penc_expert_weight_grad(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t row_stride, const void* grad,
-                            int64_t grad_row_stride, const int32_t* offsets, void* weight_grad, void* bias_grad, void* workspace, size_t workspace_bytes,
-                            void* stream) {
+int penc_expert_linear_grads(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t row_stride, const void* grad,
+                             int64_t grad_row_stride, const void* weight, const int32_t* offsets, void* dx, void* weight_grad, void* bias_grad, void* workspace,
+                             size_t workspace_bytes, void* stream) {
     return with_constant_type(type, [&](auto constant) -> int {
         constexpr int kType = decltype(constant)::value;
         if (bad_layer(rows, experts, channels, outputs) || bad_row_stride(rows, row_stride, channels) || bad_row_stride(rows, grad_row_stride, outputs))
             return PENC_ERR_BAD_LAYER_SIZE;
-        if ((rows > 0 && (!x || !grad)) || !offsets || !weight_grad) return PENC_ERR_NULL_POINTER;
+        if ((rows > 0 && (!x || !grad || (dx && !weight))) || !offsets || !weight_grad) return PENC_ERR_NULL_POINTER;
         const size_t size = kType == PENC_FP32 ? 4 : 2, need = penc_expert_weight_grad_workspace_bytes(type, rows, experts, channels, outputs);
-        if (!aligned_to(x, size) || !aligned_to(grad, size) || !aligned_to(weight_grad, size) || !aligned_to(bias_grad, size) || !aligned_to(offsets, 4) ||
-            !aligned_to(workspace, 16))
+        if (!aligned_to(x, size) || !aligned_to(grad, size) || !aligned_to(weight, size) || !aligned_to(dx, size) || !aligned_to(weight_grad, size) ||
+            !aligned_to(bias_grad, size) || !aligned_to(offsets, 4) || !aligned_to(workspace, 16))
             return PENC_ERR_MISALIGNED;
         if (workspace_bytes < need) return PENC_ERR_WORKSPACE_TOO_SMALL;
         if (need > 0 && !workspace) return PENC_ERR_NULL_POINTER;
-        return expert_weights<kType>(rows, experts, channels, outputs, x, rows > 1 ? row_stride : channels, grad, rows > 1 ? grad_row_stride : outputs, offsets,
-                                     weight_grad, bias_grad, workspace, static_cast<hipStream_t>(stream));
+        return expert_grads<kType>(rows, experts, channels, outputs, x, rows > 1 ? row_stride : channels, grad, rows > 1 ? grad_row_stride : outputs, weight, offsets,
+                                   rows > 0 ? dx : nullptr, weight_grad, bias_grad, workspace, static_cast<hipStream_t>(stream));
     });
+}
+
+int penc_expert_weight_grad(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t row_stride, const void* grad,
+                            int64_t grad_row_stride, const int32_t* offsets, void* weight_grad, void* bias_grad, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+    return penc_expert_linear_grads(type, rows, experts, channels, outputs, x, row_stride, grad, grad_row_stride, nullptr, offsets, nullptr, weight_grad, bias_grad,
+                                    workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

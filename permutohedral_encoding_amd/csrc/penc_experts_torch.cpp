@@ -20,7 +20,7 @@ struct Api {
     PENC_FN(expert_linear);
     PENC_FN(expert_linear_input_grad);
     PENC_FN(expert_weight_grad_workspace_bytes);
-    PENC_FN(expert_weight_grad);
+    PENC_FN(expert_linear_grads);
 #undef PENC_FN
 } api;
 
@@ -324,27 +324,29 @@ struct ExpertLinearNode : public ExpertNode {
         const auto options = grads[0].options().dtype(scalar);
         void* const stream = current_stream(grads[0].device());
         variable_list out(3);
-        if (t[1].defined() && task_should_compute_output(0)) {
+        const bool want_x = t[1].defined() && task_should_compute_output(0), want_bias = has_bias && task_should_compute_output(2);
+        Tensor weight;
+        if (want_x) {
             require_saved(t[1], weight_sizes, scalar);
-            const Tensor weight = t[1].contiguous();
+            weight = t[1].contiguous();
             out[0] = at::empty(sizes, options);
-            check(api.expert_linear_input_grad(type, rows, experts, channels, outputs, g.data(), g.stride, weight.const_data_ptr(), offsets, out[0].data_ptr(),
-                                               stream),
-                  "expert_linear");
         }
-        const bool want_bias = has_bias && task_should_compute_output(2);
-        if (t[0].defined() && (task_should_compute_output(1) || want_bias)) {
-            require_saved(t[0], sizes, scalar);
-            const Rows x = product_rows(rows_of(t[0], "x"));
-            Tensor weight = at::empty(weight_sizes, options);
-            if (want_bias) out[2] = at::empty({weight_sizes[0], outputs}, options);
-            const size_t n = api.expert_weight_grad_workspace_bytes(type, rows, experts, channels, outputs);
-            const Tensor ws = at::empty({static_cast<int64_t>(n)}, options.dtype(at::kByte));
-            check(api.expert_weight_grad(type, rows, experts, channels, outputs, x.data(), x.stride, g.data(), g.stride, offsets, weight.data_ptr(),
-                                         want_bias ? out[2].data_ptr() : nullptr, ws.data_ptr(), n, stream),
-                  "expert_linear");
-            if (task_should_compute_output(1)) out[1] = std::move(weight);
+        if (!t[0].defined() || !(task_should_compute_output(1) || want_bias)) {
+            if (want_x)
+                check(api.expert_linear_input_grad(type, rows, experts, channels, outputs, g.data(), g.stride, weight.const_data_ptr(), offsets, out[0].data_ptr(), stream),
+                      "expert_linear");
+            return out;
         }
+        require_saved(t[0], sizes, scalar);
+        const Rows x = product_rows(rows_of(t[0], "x"));
+        Tensor of_weight = at::empty(weight_sizes, options);
+        if (want_bias) out[2] = at::empty({weight_sizes[0], outputs}, options);
+        const size_t n = api.expert_weight_grad_workspace_bytes(type, rows, experts, channels, outputs);
+        const Tensor ws = at::empty({static_cast<int64_t>(n)}, options.dtype(at::kByte));
+        check(api.expert_linear_grads(type, rows, experts, channels, outputs, x.data(), x.stride, g.data(), g.stride, want_x ? weight.const_data_ptr() : nullptr, offsets,
+                                      want_x ? out[0].data_ptr() : nullptr, of_weight.data_ptr(), want_bias ? out[2].data_ptr() : nullptr, ws.data_ptr(), n, stream),
+              "expert_linear");
+        if (task_should_compute_output(1)) out[1] = std::move(of_weight);
         return out;
     }
 };
@@ -503,7 +505,7 @@ void bind_experts(void* library) {
     PENC_FN(expert_linear);
     PENC_FN(expert_linear_input_grad);
     PENC_FN(expert_weight_grad_workspace_bytes);
-    PENC_FN(expert_weight_grad);
+    PENC_FN(expert_linear_grads);
     PENC_FN(route);
 #undef PENC_FN
 }

@@ -66,6 +66,30 @@ def test_the_products_refuse_before_they_launch():
     assert lib.penc_expert_weight_grad(0, 4, 8, 64, 64, p, 64, p, 64, p, z, p, p, need, z) == 1
 
 
+def test_all_gradients_refuse_before_they_launch():
+    lib = _native.lib()
+    block, p = _memory()
+    z = None
+    assert lib.penc_expert_linear_grads(7, 4, 2, 8, 8, p, 8, p, 8, p, p, p, p, p, p, 0, z) == 10
+    for bad in ((-1, 2, 8, 8), (1 << 31, 2, 8, 8), (4, 0, 8, 8), (4, 1025, 8, 8), (4, 2, 0, 8), (4, 2, 8, 0), (4, 2, (1 << 18) + 1, 8), (4, 2, 8, (1 << 18) + 1)):
+        assert lib.penc_expert_linear_grads(0, *bad, p, 1 << 19, p, 1 << 19, p, p, p, p, p, p, 0, z) == 12
+    for stride in (7, -8, (1 << 20) + 1):
+        assert lib.penc_expert_linear_grads(0, 4, 2, 8, 8, p, 8, p, stride, p, p, p, p, p, p, 0, z) == 12
+        assert lib.penc_expert_linear_grads(0, 4, 2, 8, 8, p, stride, p, 8, p, p, p, p, p, p, 0, z) == 12
+    for k in (0, 1, 2, 3, 5):  # x, the gradient, the weight (where dx is wanted), the offsets and the weight's gradient
+        given = [p] * 6
+        given[k] = z
+        x, grad, weight, offsets, dx, dweight = given
+        assert lib.penc_expert_linear_grads(0, 4, 2, 8, 8, x, 8, grad, 8, weight, offsets, dx, dweight, z, z, 0, z) == 1
+        given = [p] * 6
+        given[k] = p + 2
+        x, grad, weight, offsets, dx, dweight = given
+        assert lib.penc_expert_linear_grads(0, 4, 2, 8, 8, x, 8, grad, 8, weight, offsets, dx, dweight, z, z, 0, z) == 5
+    need = lib.penc_expert_weight_grad_workspace_bytes(0, 1 << 20, 8, 64, 64)
+    assert lib.penc_expert_linear_grads(0, 1 << 20, 8, 64, 64, p, 64, p, 64, p, p, p, p, p, p, need - 1, z) == 8
+    assert lib.penc_expert_linear_grads(0, 1 << 20, 8, 64, 64, p, 64, p, 64, p, p, p, p, p, z, need, z) == 1
+
+
 def test_tensors_in_host_memory_are_refused():
     x, experts = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int64)
     plan = layers.Routing(experts, 3, experts.int(), torch.zeros(4, dtype=torch.int32))
