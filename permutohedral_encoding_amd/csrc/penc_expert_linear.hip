@@ -8,6 +8,7 @@
 //
 // The type of values (PENC_TYPE: those of penc.h) is one compilation each.
 #include <algorithm>
+#include <limits>
 
 #include "penc_expert_linear.hpp"
 #include "penc_product.hpp"
@@ -647,10 +648,17 @@ WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t 
     p.side = channels <= 64 || outputs <= 64 ? 64 : kSize == 2 && channels % 8 == 0 && outputs % 8 == 0 && channels >= 256 && outputs >= 256 && static_cast<double>(rows) * static_cast<double>(channels * outputs) >= 0x1p34 ? 256 : 128;
     const int64_t side = p.side;
     p.tiles = ((channels + side - 1) / side) * ((outputs + side - 1) / side);
-    // pieces for four workgroups to a compute unit; of layers of one tile for the three that have room there at a time (2^20 x 64 by 64 fp32, all of the layer:
-    // 299 us, of twice as many 305, of 4, 8 and 2 to a compute unit 325, 316 and 347)
-    const int64_t wanted = p.tiles == 1 ? 3 * kUnits : ((side == 256 ? 512 : side == 128 ? 1024 : 2048) + p.tiles - 1) / p.tiles;
-    int64_t most = experts >= wanted ? 2 * ((rows + experts - 1) / experts) : (rows + wanted - 1) / wanted;
+    // Workgroups that have room at a time, and for one to four rounds of them the rows of a piece: the least of rounds times a piece and what a workgroup takes beside, as long as two
+    // steps.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and 6 for the sums, now 28 and 5;
+    // 2^20 x 64 by 64 fp32, all of the layer, with 2, 4, 6 and 8 to a compute unit 347, 325, 305 and 316 us, with 3 299.)
+    const int64_t room = (side == 256 ? 1 : side == 128 ? 2 : 3) * kUnits;
+    int64_t most = 2 * ((rows + experts - 1) / experts), least = std::numeric_limits<int64_t>::max();
+    for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+        const int64_t pieces = rounds * room / p.tiles - experts;
+        if (pieces <= 0) continue;
+        const int64_t each = std::max<int64_t>(((rows + pieces - 1) / pieces + 63) / 64 * 64, 512), time = rounds * (each + 128);
+        if (time < least) least = time, most = each;
+    }
     most = std::max<int64_t>((most + 63) / 64 * 64, 512);
     p.most = std::min<int64_t>(most, (int64_t{1} << 30));
     p.pieces = rows / p.most + experts;
