@@ -61,6 +61,15 @@ __device__ __forceinline__ void store_stored(char* row, int column, floats<8> v)
     if constexpr (std::is_same_v<E, split_t>) *reinterpret_cast<halves<8>*>(p + 64) = rest_of<8>(v, hi);
 }
 
+// f v + w, rounded once.
+template <class V>
+__device__ __forceinline__ V weighted(float f, V v, V w) {
+    constexpr int kWide = sizeof(V) / sizeof(float);
+#pragma unroll
+    for (int i = 0; i < kWide; ++i) w[i] = __builtin_fmaf(f, v[i], w[i]);
+    return w;
+}
+
 // ------------------------------------------------------------------------------------------
 // the norm, and X
 
@@ -220,7 +229,7 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
             m += m0, n += n0;
             v *= kPerScale;
             const bool there = n < a.small && m < a.small_padded;
-            if constexpr (kStage == kSquare) v = a.b * (there ? load_stored<E>(s + n * small_stride, m) : floats<8>{}) + a.c * v;
+            if constexpr (kStage == kSquare) v = weighted(a.b, there ? load_stored<E>(s + n * small_stride, m) : floats<8>{}, a.c * v);
             if (there) store_stored<E>(out + n * small_stride, m, v);
             if (m0 == n0) return;
             const halves<8> hi = __builtin_convertvector(v, halves<8>);
@@ -256,7 +265,7 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
         p.each_eight([&](int m, int n, floats<8> v) {
             m += m0, n += n0;
             if (n >= a.rows || m >= a.padded) return;
-            v = a.a * load_stored<E>(x + n * stride, m) + v * kPerScale;
+            v = weighted(a.a, load_stored<E>(x + n * stride, m), v * kPerScale);
             if (a.result == nullptr) store_stored<E>(out + n * stride, m, v);
             else if (m < a.columns) store_values<Result, 8>(result + static_cast<int64_t>(n) * a.columns + m, __builtin_convertvector(v * kPerScale, Eight), a.columns - m);
         });
@@ -302,6 +311,7 @@ __global__ __launch_bounds__(kSumThreads) void gram_sum_kernel(StepArgs a) {
 
 constexpr int kResidentThreads = 512, kResidentWaves = kResidentThreads / 64;
 constexpr int kMostSmall = 128;
+constexpr int kSliceBytes = 8192;  // for sums of S that waves share (matrices of up to 32 rows)
 constexpr int kMostResident = 160 * 1024 - 256;  // bytes of the LDS
 
 // A matrix of Split numbers in the LDS.  Chunks of a row's 128 bytes are permuted by the row, so that neither 8 rows of one chunk nor 4 rows of two chunks meet in a bank.
@@ -338,8 +348,10 @@ struct Resident {
     }
 };
 
-// (the products with a lo have sums of their own: see Product::low)
+// (the products with a lo have sums of their own: see Product::low.  kAll: with lo lo, for fp32 results)
+template <bool kAll>
 __device__ __forceinline__ void multiply_split(chunk16 a, chunk16 a_low, chunk16 b, chunk16 b_low, tile_acc& high, tile_acc& low) {
+    if constexpr (kAll) low = multiply<half_t>(a_low, b_low, low);
     low = multiply<half_t>(a, b_low, low);
     low = multiply<half_t>(a_low, b, low);
     high = multiply<half_t>(a, b, high);
@@ -354,6 +366,7 @@ template <class G, int kTiles, int kBlocks>
 __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, int columns, int steps, Coefficients k, const G* __restrict__ g, G* __restrict__ result) {
     __shared__ __attribute__((aligned(1024))) char lds[kMostResident];
     constexpr int kPadded = 16 * kTiles, kLines = kPadded / 32, kTogether = kBlocks > 1 && kTiles <= 4 ? 2 : 1;
+    constexpr bool kAll = std::is_same_v<G, float>;
     constexpr int kUnroll = kTiles <= 4 ? kLines : 1;  // (more would not fit the registers)
     const bool tall = rows > columns;
     const int small = min(rows, columns), large = max(rows, columns), large_padded = (large + 63) / 64 * 64;
@@ -413,10 +426,41 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
         }
     __syncthreads();
     constexpr int kUnits = kTiles * kTiles / 2, kMostUnits = (kUnits + kResidentWaves - 1) / kResidentWaves;
+    // Of 32 rows there are two units of S: four waves share the k of each, and what three of them have is added by way of the LDS.  Sums of a quarter of the length round less, too.
+    constexpr int kSlices = kUnits < kResidentWaves ? kResidentWaves / kUnits : 1;
+    static_assert(kSlices == 1 || (kSlices == 4 && kSliceBytes == 2 * kUnits * 2 * 64 * 16));
     for (int step = 0; step < steps; ++step) {
         tile_acc of_s[kMostUnits][2];
+        if constexpr (kSlices > 1) {
+            const int unit = wave % kUnits, slice = wave / kUnits, m = unit % kTiles * 16, n = unit / kTiles * 32, pairs = large_padded / 64;
+            tile_acc high[2] = {}, low[2] = {};
+            for (int first = slice * pairs / kSlices * 2; first < (slice + 1) * pairs / kSlices * 2; first += 2) {
 #pragma unroll
-        for (int u = 0; u < kMostUnits; ++u) {
+                for (int line = first; line < first + 2; ++line) {
+                    const chunk16 a = x.across(m, line, 0), a_low = x.across(m, line, 1);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) multiply_split<kAll>(a, a_low, x.across(n + 16 * h, line, 0), x.across(n + 16 * h, line, 1), high[h], low[h]);
+                }
+            }
+            // slices 2 and 3 to 0 and 1, and 1 to 0
+            tile_acc* const left = reinterpret_cast<tile_acc*>(s.first + kPadded * s.pitch) + (slice % 2 * kUnits + unit) * 128 + lane;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) of_s[0][h] = high[h] + low[h];
+#pragma unroll
+            for (int most = kSlices; most > 1; most /= 2) {
+                if (slice >= most / 2 && slice < most) left[0] = of_s[0][0], left[64] = of_s[0][1];
+                __syncthreads();
+                const tile_acc* const right = most == 2 ? left + kUnits * 128 : left;
+                if (slice < most / 2) of_s[0][0] += right[0], of_s[0][1] += right[64];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                of_s[0][h] *= kPerScale;
+                if (slice == 0) s.store<4>(n + 16 * h + l16, m + q4, of_s[0][h]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < (kSlices > 1 ? 0 : kMostUnits); ++u) {
             const int unit = u * kResidentWaves + wave, m = unit % kTiles * 16, n = unit / kTiles * 32;
             if (unit >= kUnits) continue;
             tile_acc high[2] = {}, low[2] = {};
@@ -425,7 +469,7 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
                 for (int line = first; line < first + 2; ++line) {
                     const chunk16 a = x.across(m, line, 0), a_low = x.across(m, line, 1);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) multiply_split(a, a_low, x.across(n + 16 * h, line, 0), x.across(n + 16 * h, line, 1), high[h], low[h]);
+                    for (int h = 0; h < 2; ++h) multiply_split<kAll>(a, a_low, x.across(n + 16 * h, line, 0), x.across(n + 16 * h, line, 1), high[h], low[h]);
                 }
             }
 #pragma unroll
@@ -444,10 +488,10 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
             for (int line = 0; line < kLines; ++line) {
                 const chunk16 a = s.across(m, line, 0), a_low = s.across(m, line, 1);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) multiply_split(a, a_low, s.across(n + 16 * h, line, 0), s.across(n + 16 * h, line, 1), high[h], low[h]);
+                for (int h = 0; h < 2; ++h) multiply_split<kAll>(a, a_low, s.across(n + 16 * h, line, 0), s.across(n + 16 * h, line, 1), high[h], low[h]);
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) of_s[u][h] = k.b * of_s[u][h] + (k.c * kPerScale) * (high[h] + low[h]);
+            for (int h = 0; h < 2; ++h) of_s[u][h] = weighted(k.c * kPerScale, high[h], weighted(k.b, of_s[u][h], (k.c * kPerScale) * low[h]));
         }
         __syncthreads();
 #pragma unroll
@@ -477,7 +521,7 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
                 for (int n = 0; n < kTiles; ++n) {
                     const chunk16 f = s.across(n * 16, line, 0), f_low = s.across(n * 16, line, 1);
 #pragma unroll
-                    for (int t = 0; t < kTogether; ++t) multiply_split(a[t][0], a[t][1], f, f_low, high[t][n], low[t][n]);
+                    for (int t = 0; t < kTogether; ++t) multiply_split<kAll>(a[t][0], a[t][1], f, f_low, high[t][n], low[t][n]);
                 }
             }
 #pragma unroll
@@ -486,7 +530,7 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
                 if (b + t >= kBlocks || m >= large_padded) continue;
 #pragma unroll
                 for (int n = 0; n < kTiles; ++n) {
-                    own[b + t][n] = k.a * own[b + t][n] + (high[t][n] + low[t][n]) * kPerScale;
+                    own[b + t][n] = weighted(k.a, own[b + t][n], (high[t][n] + low[t][n]) * kPerScale);
                     if (!last) x.store<4>(n * 16 + l16, m + q4, own[b + t][n]);
                 }
             }
@@ -546,7 +590,7 @@ bool is_resident(int64_t rows, int64_t columns) {
     const int64_t small = std::min(rows, columns), large = std::max(rows, columns);
     if (small > kMostSmall || large > 1 << 12) return false;
     const int s = round_to_32(static_cast<int>(small)), l = (static_cast<int>(large) + 63) / 64 * 64;
-    return static_cast<int64_t>(s) * (resident_pitch(l) + resident_pitch(s)) <= kMostResident;
+    return static_cast<int64_t>(s) * (resident_pitch(l) + resident_pitch(s)) + (s <= 32 ? kSliceBytes : 0) <= kMostResident;
 }
 
 template <class G>
