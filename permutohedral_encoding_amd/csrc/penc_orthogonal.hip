@@ -3,11 +3,11 @@
 //     X = G / (|G|_F + eps);    `steps` times:  S = X X^T (of a tall X: X^T X),  F = b S + c S S,  X = a X + F X (X F)
 //
 // takes every singular value s in 0 .. 1 through as many times a s + b s^3 + c s^5.  What is small in X is taken up by a factor a in each step, and so is what a rounding has
-// added to it.  In 16 bits with 8 of them behind the point (bfloat16) the result is off by 1e-2 of it, in float16 by 1.4e-3, in float16 twice (22 bits) by 2.7e-7, of
-// which float32 itself has 1.8e-7 (random matrices of 32 to 1024 rows, 5 steps).  So X, S and F are kept
+// added to it.  In 16 bits with 8 of them behind the point (bfloat16) the result would be off by 1e-2 of it, in float16 by 1.4e-3.  So X, S and F are kept
 //
-//     for bfloat16 results     as float16, one product for each: with the result's own rounding (1.66e-3) 2.1e-3
-//     for float16 and float32  as two float16 values, hi + lo, three products for each
+//     for bfloat16 results     as float16, one product for each, and F's diagonal, which is most of F, in float32: with the result's own rounding (1.66e-3) 1.8e-3 to 2.0e-3
+//                              (with the diagonal in float16 2.0e-3 to 2.4e-3)
+//     for float16 and float32  as two float16 values, hi + lo, three products for each: 0.7e-6 to 1.5e-6 of float32 results, which float32 products leave 0.9e-6 to 1.7e-6 off
 //
 // times 2^12: with |X| <= 1.2, S <= 1.5 and F <= 3 they stay under 2^14 (a bound on the coefficients sees to that), and what matters of lo is no subnormal number.
 // The matrix cores run float16 8 times as fast as float32, so that three products take 3/8 of the time.
@@ -120,15 +120,22 @@ __global__ __launch_bounds__(kThreads) void squares_kernel(int64_t values, int p
     if (threadIdx.x == 0) sums[blockIdx.x] = sum[0];
 }
 
-// X 2^12 as it is stored, zeros behind each row's end.
+// X 2^12 as it is stored, zeros behind each row's end.  As one float16 (E = half_t) it is rounded to 11 bits, and each of the five steps takes that up again.  So the first X is the update times a
+// power of two, which of bfloat16 is no rounding, and what the norm has beside, 1 to 2, is left to the first step (`rest`, for each matrix): an error of 1.9e-3 to 2.2e-3 became 1.8e-3 to 2.0e-3.
 template <class E, class G>
 __global__ __launch_bounds__(kThreads) void stage_kernel(int rows, int columns, int padded, int pieces, const G* __restrict__ g, const double* __restrict__ sums,
-                                                         float eps, char* __restrict__ x, uint32_t blocks) {
+                                                         float eps, char* __restrict__ x, float* __restrict__ rest, uint32_t blocks) {
     const int64_t matrix = blockIdx.x / blocks;
     const double* const mine = sums + matrix * pieces;
     double squares = 0.0;
     for (int i = static_cast<int>(threadIdx.x); i < pieces; i += kThreads) squares += mine[i];
-    const double factor = per_norm(workgroup_sum<kThreads>(squares), eps);
+    double factor = per_norm(workgroup_sum<kThreads>(squares), eps);
+    if constexpr (std::is_same_v<E, half_t>) {
+        // (of a norm that is not finite the factor is 0 or NaN: all of it is left then)
+        const double power = factor > 0.0 ? ldexp(1.0, ilogb(factor)) : 1.0;
+        if (blockIdx.x % blocks == 0 && threadIdx.x == 0) rest[matrix] = static_cast<float>(factor / power);
+        factor = power;
+    }
     const G* const from = g + matrix * rows * columns;
     const int64_t stride = static_cast<int64_t>(padded) * ProductType<E>::kBytes;
     char* const to = x + matrix * rows * stride;
@@ -166,8 +173,12 @@ struct StepArgs {
     uint32_t each, tiles_m;  // each: items of a matrix
     int splits;              // kGram: workgroups that share a tile's k, each of which leaves its sums in `partial`
     float* partial;
+    float* diagonal;         // F's: [matrices][small_padded]
+    const float* rest;       // the first step's, else null: what X is to be multiplied by
     float a, b, c;
 };
+
+__device__ __forceinline__ float rest_of_norm(const StepArgs& a, int64_t matrix) { return a.rest != nullptr ? a.rest[matrix] : 1.0f; }
 
 // Pair `t` of tiles on and behind the diagonal: i <= j.
 __device__ __forceinline__ void pair_of(uint32_t t, uint32_t& i, uint32_t& j) {
@@ -222,14 +233,24 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
         constexpr int kWideM = P::kM / P::kWavesM, kWideN = P::kN / P::kWavesN, kParts = ProductType<E>::kParts;
         // The other side of the diagonal: a wave's results as halves in the LDS, rows of n, and read back by columns.
         static_assert(kParts * P::kThreads / 64 * kWideM * kWideN * 2 <= P::kLds);
+        const float r = kStage == kGram ? rest_of_norm(a, matrix) : 1.0f, per_scale = kPerScale * r * r;
         char* const turned = lds + P::wave() * (kParts * kWideM * kWideN * 2);
         if (m0 != n0) __syncthreads();
         p.each_eight([&](int m, int n, floats<8> v) {
             const int lm = m - P::wave_m(), ln = n - P::wave_n();
             m += m0, n += n0;
-            v *= kPerScale;
+            v *= per_scale;
             const bool there = n < a.small && m < a.small_padded;
             if constexpr (kStage == kSquare) v = weighted(a.b, there ? load_stored<E>(s + n * small_stride, m) : floats<8>{}, a.c * v);
+            if (kStage == kSquare && m0 == n0) {
+                float* const diagonal = a.diagonal + matrix * a.small_padded + n;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (m + k != n) continue;
+                    if (n < a.small_padded) *diagonal = n < a.small ? v[k] * kPerScale : 0.0f;  // (zeros behind the end, as in X)
+                    v[k] = 0.0f;
+                }
+            }
             if (there) store_stored<E>(out + n * small_stride, m, v);
             if (m0 == n0) return;
             const halves<8> hi = __builtin_convertvector(v, halves<8>);
@@ -260,12 +281,22 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
                 }
     } else {
         char* const out = a.out + matrix * a.rows * stride;
+        const float r = rest_of_norm(a, matrix), per_scale = kPerScale * r;
+        const float* const diagonal = a.diagonal + matrix * a.small_padded;
         Result* const result = static_cast<Result*>(a.result) + matrix * a.rows * a.columns;
         using Eight = Result __attribute__((ext_vector_type(8)));
         p.each_eight([&](int m, int n, floats<8> v) {
             m += m0, n += n0;
             if (n >= a.rows || m >= a.padded) return;
-            v = weighted(a.a, load_stored<E>(x + n * stride, m), v * kPerScale);
+            const floats<8> from = load_stored<E>(x + n * stride, m);
+            v *= per_scale;
+            if constexpr (kTall) {
+                const floats<8> keep = (*reinterpret_cast<const floats<8>*>(diagonal + m) + a.a) * r;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = __builtin_fmaf(keep[k], from[k], v[k]);
+            } else {
+                v = weighted((diagonal[n] + a.a) * r, from, v);
+            }
             if (a.result == nullptr) store_stored<E>(out + n * stride, m, v);
             else if (m < a.columns) store_values<Result, 8>(result + static_cast<int64_t>(n) * a.columns + m, __builtin_convertvector(v * kPerScale, Eight), a.columns - m);
         });
@@ -285,11 +316,12 @@ __global__ __launch_bounds__(kSumThreads) void gram_sum_kernel(StepArgs a) {
     char* const out = a.out + matrix * a.small * stride;
     const float* const from = a.partial + static_cast<int64_t>(blockIdx.x) * a.splits * (kSumSide * kSumSide);
     const int m0 = static_cast<int>(i) * kSumSide, n0 = static_cast<int>(j) * kSumSide;
+    const float r = rest_of_norm(a, matrix), per_scale = kPerScale * r * r;
     for (int at = static_cast<int>(threadIdx.x) * 8; at < kSumSide * kSumSide; at += kSumThreads * 8) {
         floats<8> v{};
 #pragma unroll 8
         for (int k = 0; k < a.splits; ++k) v += *reinterpret_cast<const floats<8>*>(from + k * (kSumSide * kSumSide) + at);
-        v *= kPerScale;
+        v *= per_scale;
         const int n = at / kSumSide, m = at % kSumSide;
 #pragma unroll
         for (int k = 0; k < 8; ++k) lds[m + k][n] = v[k];
@@ -348,7 +380,8 @@ struct Resident {
     }
 };
 
-// (the products with a lo have sums of their own: see Product::low.  kAll: with lo lo, for fp32 results)
+// (the products with a lo have sums of their own: see Product::low.  kAll: with lo lo: of 18 x 1104 fp32 1.4e-6 of error became 1.15e-6
+// (float32's own 1.0e-6); of 256 x 64, where it is 1.1e-6 (1.2e-6) without, all of it would take 36 us and not 33)
 template <bool kAll>
 __device__ __forceinline__ void multiply_split(chunk16 a, chunk16 a_low, chunk16 b, chunk16 b_low, tile_acc& high, tile_acc& low) {
     if constexpr (kAll) low = multiply<half_t>(a_low, b_low, low);
@@ -366,7 +399,7 @@ template <class G, int kTiles, int kBlocks>
 __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, int columns, int steps, Coefficients k, const G* __restrict__ g, G* __restrict__ result) {
     __shared__ __attribute__((aligned(1024))) char lds[kMostResident];
     constexpr int kPadded = 16 * kTiles, kLines = kPadded / 32, kTogether = kBlocks > 1 && kTiles <= 4 ? 2 : 1;
-    constexpr bool kAll = std::is_same_v<G, float>;
+    constexpr bool kAll = std::is_same_v<G, float> && kTiles <= 2;
     constexpr int kUnroll = kTiles <= 4 ? kLines : 1;  // (more would not fit the registers)
     const bool tall = rows > columns;
     const int small = min(rows, columns), large = max(rows, columns), large_padded = (large + 63) / 64 * 64;
@@ -628,6 +661,7 @@ struct Layout {
     int64_t padded, small, small_padded, x, s;  // x, s: bytes of all matrices'
     int pieces, splits;
     int64_t partial;  // bytes of the sums of workgroups that share tiles
+    int64_t sums;     // of the squares'
     size_t total;
 };
 template <class E>
@@ -644,7 +678,8 @@ Layout layout_of(int64_t matrices, int64_t rows, int64_t columns) {
     const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     l.x = up(l.x), l.s = up(l.s);
     l.partial = l.splits > 1 ? matrices * pairs_of(l.small, kSumSide) * l.splits * (4 * kSumSide * kSumSide) : 0;
-    l.total = static_cast<size_t>(2 * l.x + 2 * l.s + l.partial + up(8 * matrices * l.pieces));
+    l.sums = up(8 * matrices * l.pieces);
+    l.total = static_cast<size_t>(2 * l.x + 2 * l.s + l.partial + l.sums + up(4 * matrices) + up(4 * matrices * l.small_padded));
     return l;
 }
 
@@ -687,16 +722,18 @@ int orthogonalise(int64_t matrices, int64_t rows, int64_t columns, int steps, Co
     char *x = workspace, *next = x + l.x, *const s = next + l.x, *const f = s + l.s;
     float* const partial = reinterpret_cast<float*>(f + l.s);
     double* const sums = reinterpret_cast<double*>(f + l.s + l.partial);
+    float* const rest = reinterpret_cast<float*>(f + l.s + l.partial + l.sums);
+    float* const diagonal = rest + (matrices + 63) / 64 * 64;
     squares_kernel<G><<<static_cast<unsigned>(matrices * l.pieces), kThreads, 0, stream>>>(rows * columns, l.pieces, g, sums);
     if (const int rc = launched()) return rc;
     const int64_t eights = rows * (l.padded / 8);
     const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>((eights + kThreads - 1) / kThreads, std::max<int64_t>(1, 4096 / matrices)));
     stage_kernel<E, G><<<static_cast<unsigned>(matrices * blocks), kThreads, 0, stream>>>(static_cast<int>(rows), static_cast<int>(columns), static_cast<int>(l.padded),
-                                                                                         l.pieces, g, sums, k.eps, x, blocks);
+                                                                                         l.pieces, g, sums, k.eps, x, rest, blocks);
     if (const int rc = launched()) return rc;
     for (int step = 0; step < steps; ++step) {
         StepArgs a{x, s, f, s, nullptr, static_cast<int>(rows), static_cast<int>(columns), static_cast<int>(l.padded), static_cast<int>(l.small),
-                   static_cast<int>(l.small_padded), {}, 0, 0, l.splits, l.splits > 1 ? partial : nullptr, k.a, k.b, k.c};
+                   static_cast<int>(l.small_padded), {}, 0, 0, l.splits, l.splits > 1 ? partial : nullptr, diagonal, step == 0 && std::is_same_v<E, half_t> ? rest : nullptr, k.a, k.b, k.c};
         const auto all = [&](auto tall) -> int {
             constexpr bool kTall = decltype(tall)::value;
             if (const int rc = launch_step<kGram, kTall, E, G>(a, matrices, stream)) return rc;
