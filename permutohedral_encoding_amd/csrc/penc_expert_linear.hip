@@ -8,7 +8,6 @@
 //
 // The type of values (PENC_TYPE: those of penc.h) is one compilation each.
 #include <algorithm>
-#include <limits>
 
 #include "penc_expert_linear.hpp"
 #include "penc_product.hpp"
@@ -642,13 +641,14 @@ template <bool kBack, Chunks kChunks>
 int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
     if constexpr (kChunks == Chunks::kDirect) {
         if (a.wide <= 16 * kNarrowTiles && a.deep * kSize <= 64 * kNarrowLines && a.stride * kSize * 64 < 1 << 30) return launch_narrow<kBack>(a, stream);
-        if (!kBack && a.rows <= kFewRows * static_cast<int64_t>(a.experts)) return launch_few(a, stream);
+        // (rows that are 4 to an expert, 64 experts of 1024 by 4096 bf16: 99 us and 122 without; 16 to an expert 140 and 108)
+        if (!kBack && a.rows <= kFewRows / 2 * static_cast<int64_t>(a.experts)) return launch_few(a, stream);
     }
-    // (129 to 192 results: three tiles of 64, not two of 128)
-    if (a.wide <= 64 || (a.wide > 128 && a.wide <= 192) || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks>>(a, stream);
+    if (a.wide <= 64 || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks>>(a, stream);
     if constexpr (kChunks != Chunks::kSingle) {
         if constexpr (kChunks == Chunks::kDirect && kSize == 2) {
-            if (static_cast<int64_t>(a.rows / 256 + a.experts) * ((a.wide + 255) / 256) >= 512)
+            // (1024 by 4096 bf16, 16 experts, of 2048 rows each: 302 us and 347 without; of 512 89 and 86, of 256 58 and 50: tiles of 256 rows that are not full)
+            if (a.rows >= 1024 * static_cast<int64_t>(a.experts) && static_cast<int64_t>(a.rows / 256) * ((a.wide + 255) / 256) >= 512)
                 return launch_rows<kBack, Product<Value, kBack, false, 256, 256, 4, 2, kChunks>, Product<Value, kBack, false, 128, 128, 4, 2, kChunks>>(a, stream);
         }
         return launch_rows<kBack, Product<Value, kBack, false, 128, 128, 2, 2, kChunks>>(a, stream);
@@ -662,33 +662,45 @@ int rows_of_experts(const RowsArgs& a, Chunks chunks, hipStream_t stream) {
     return rows_of_experts<kBack, Chunks::kSingle>(a, stream);
 }
 
-// How the rows of the weights' gradient are cut.
+// How the rows of the weights' gradient are cut, and the tiles.  A time is in rows that a workgroup multiplies.
 struct WeightPlan {
     int side;      // of a tile
     int64_t tiles; // of an expert
     int64_t most;  // rows of a piece
     int64_t pieces;
+    double time;
 };
-WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
+// Workgroups go in rounds of as many as have room at a time.  Beside its rows a workgroup takes as long as for two steps, and where its sums go through memory, as long again as kCut
+// rows.  Either an expert's rows are one piece (up to twice as many as experts have on average, and a quarter of the time for experts that are not alike), or they are cut for one to four whole
+// rounds.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and 6 for the sums, now 28 and 5;
+// 2^20 x 64 by 64 fp32, all of the layer, with 2, 4, 6 and 8 to a compute unit 347, 325, 305 and 316 us, with 3 299.  16384 x 1024 by 2048 bf16, 4 experts, y and dW: cut for three rounds
+// 216 us, in one piece 165.)
+WeightPlan weight_plan_of(int side, int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
+    constexpr double kBeside = 128.0, kCut = kSize == 2 ? 512.0 : 128.0;
     WeightPlan p;
-    p.side = channels <= 64 || outputs <= 64 ? 64 : kSize == 2 && channels % 8 == 0 && outputs % 8 == 0 && channels >= 256 && outputs >= 256 && static_cast<double>(rows) * static_cast<double>(channels * outputs) >= 0x1p34 ? 256 : 128;
-    const int64_t side = p.side;
+    p.side = side;
     p.tiles = ((channels + side - 1) / side) * ((outputs + side - 1) / side);
-    // Workgroups that have room at a time, and for one to four rounds of them the rows of a piece: the least of rounds times a piece and what a workgroup takes beside, as long as two
-    // steps.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and 6 for the sums, now 28 and 5;
-    // 2^20 x 64 by 64 fp32, all of the layer, with 2, 4, 6 and 8 to a compute unit 347, 325, 305 and 316 us, with 3 299.)
-    const int64_t room = (side == 256 ? 1 : side == 128 ? 2 : 3) * kUnits;
-    int64_t most = 2 * ((rows + experts - 1) / experts), least = std::numeric_limits<int64_t>::max();
+    const int64_t room = (side == 256 ? 1 : side == 128 ? 2 : 3) * kUnits, own = (rows + experts - 1) / experts;
+    p.most = 2 * own;
+    p.time = static_cast<double>((experts * p.tiles + room - 1) / room) * 1.25 * (static_cast<double>(own) + kBeside);
     for (int64_t rounds = 1; rounds <= 4; ++rounds) {
         const int64_t pieces = rounds * room / p.tiles - experts;
         if (pieces <= 0) continue;
-        const int64_t each = std::max<int64_t>(((rows + pieces - 1) / pieces + 63) / 64 * 64, 512), time = rounds * (each + 128);
-        if (time < least) least = time, most = each;
+        const int64_t each = std::max<int64_t>((rows + pieces - 1) / pieces, 512);
+        const double time = static_cast<double>(rounds) * (static_cast<double>(each) + kBeside + kCut);
+        if (time < p.time) p.time = time, p.most = each;
     }
-    most = std::max<int64_t>((most + 63) / 64 * 64, 512);
-    p.most = std::min<int64_t>(most, (int64_t{1} << 30));
+    p.most = std::min<int64_t>(std::max<int64_t>((p.most + 63) / 64 * 64, 512), int64_t{1} << 30);
     p.pieces = rows / p.most + experts;
     return p;
+}
+WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
+    if (channels <= 64 || outputs <= 64) return weight_plan_of(64, rows, experts, channels, outputs);
+    const WeightPlan p = weight_plan_of(128, rows, experts, channels, outputs);
+    if (kSize != 2 || channels % 8 != 0 || outputs % 8 != 0 || channels < 256 || outputs < 256) return p;
+    // Two tiles of 128 have half of the work of one of 256 a row, which they do in 0.6 of its time (32768 x 1024 by 4096 bf16, 16 experts, all of the layer: 256 897 us, 128 940).
+    const WeightPlan large = weight_plan_of(256, rows, experts, channels, outputs);
+    return large.time < 0.6 * p.time ? large : p;
 }
 
 template <class P>
