@@ -426,7 +426,7 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
     if (item >= a.spread.items) return;
     uint32_t piece;
     const RowTile t = row_tile_by_size(a.offsets, a.experts, a.rows, item / a.tiles, a.most, piece);
-    if (t.expert < 0) return;
+    if (t.expert < 0 || piece >= a.pieces) return;  // (the second: offsets that no plan has)
     const int c0 = static_cast<int>(tile % a.channel_tiles) * P::kM, o0 = static_cast<int>(tile / a.channel_tiles) * P::kN;
     const bool bias = a.bias != nullptr && c0 == 0 && P::wave_m() == 0;
     const Operand m{static_cast<const char*>(a.x) + (static_cast<int64_t>(t.first) * a.x_stride + c0) * kSize, a.x_stride * kSize, t.rows, min(a.channels - c0, P::kM) * kSize};
@@ -644,7 +644,8 @@ int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
         // (rows that are 4 to an expert, 64 experts of 1024 by 4096 bf16: 99 us and 122 without; 16 to an expert 140 and 108)
         if (!kBack && a.rows <= kFewRows / 2 * static_cast<int64_t>(a.experts)) return launch_few(a, stream);
     }
-    if (a.wide <= 64 || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks>>(a, stream);
+    // (129 to 192 results of rows that begin anywhere: three tiles of 64 take 32.5 us of 70001 x 203 by 130 fp16, two of 128 35.4; of rows on 16 bytes, 208 by 136, 22.3 and 21.0)
+    if (a.wide <= 64 || (kChunks == Chunks::kHeld && a.wide > 128 && a.wide <= 192) || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks>>(a, stream);
     if constexpr (kChunks != Chunks::kSingle) {
         if constexpr (kChunks == Chunks::kDirect && kSize == 2) {
             // (1024 by 4096 bf16, 16 experts, of 2048 rows each: 302 us and 347 without; of 512 89 and 86, of 256 58 and 50: tiles of 256 rows that are not full)

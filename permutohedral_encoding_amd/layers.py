@@ -1,13 +1,22 @@
-"""What the layers behind the encoding train with: checkpoints of activations in 8 bits, and layers whose backward reads them.
+"""What the layers behind the encoding train with: checkpoints of activations in 8 bits and layers whose backward reads them, and layers of experts.
 
 No counterpart in the reference, whose scripts take these layers from torch.  An encoding of 2^20 points and 24 levels is 200 MB that a linear layer
-behind it keeps for its weight gradient, and each hidden layer keeps as much again, several times over.  The functions here keep what their backward
+behind it keeps for its weight gradient, and each hidden layer keeps as much again, several times over.  The first functions here keep what their backward
 needs in 8 bits a value (a quarter of fp32) and are one pass over memory in either direction:
 
     x = encoding(positions)                                            # (N, 48)
     h = layers.linear(x, w0, b0)
     f = layers.linear(layers.activation(h, "gelu"), w1, b1)
     h, n = layers.residual_norm(h, f, gate=gate, post_weight=wp, pre_weight=wn)     # h + gate * norm(f), and its norm for the next block
+
+A decoder of experts sends each row to a few of many small layers, by a router that is trained with them.  Its rows are sorted by expert, multiplied, and brought back:
+
+    weights, routing = layers.route(layers.linear(x, w_router), 2)                  # 2 of the experts for each row, their shares, and where each choice stands
+    h = layers.expert_linear(layers.dispatch(x, routing), w_up, b_up, routing)      # (rows * 2, O): each expert's rows one after the other
+    y = layers.expert_linear(layers.activation(h), w_down, None, routing)
+    out = layers.combine(y, weights, routing)                                       # back in the rows' order, weighted
+
+What the experts' functions need for the backward they keep as it is, and which rows go where stays on the device: nothing waits for it.
 
 All of them take float32, float16 or bfloat16 tensors ``(..., C)`` in GPU memory, on the current stream of the tensor's device, of any strides (rows whose
 channels are adjacent are read in place, as is the encoding's own result).  Sums and statistics are float32, results are rounded once, and

@@ -531,10 +531,11 @@ def test_an_expert_twice_in_a_row():
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
-def test_expert_linear_of_wide_layers(dtype):
+@pytest.mark.parametrize("channels,outputs", [(384, 520), (512, 512)])
+def test_expert_linear_of_wide_layers(dtype, channels, outputs):
     """Tiles of 256 x 256 in each direction, the last of them in quarters; experts of no row, of one, and of nearly all; rows without an expert; rows that are further apart, on
     16 bytes and not."""
-    rows, number, channels, outputs = 100000, 7, 384, 520
+    rows, number = 100000, 7
     generator = torch.Generator(device="cuda").manual_seed(5)
     experts = torch.randint(0, 4, (rows, 1), generator=generator, device="cuda").clamp_(max=2)  # (half of them to expert 2)
     experts[:300] = -1
