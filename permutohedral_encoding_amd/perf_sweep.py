@@ -59,6 +59,14 @@ def _timed(step, nr_points, iters, warmup):
     return float(np.mean(kept))
 
 
+def _added_at_peak(step):
+    """What a step asks for beside what is there, at its peak.  (Not the allocator's blocks: one that it has from before, and gives whole for something smaller, would count whole.)"""
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_stats()["requested_bytes.all.current"]
+    step()
+    return torch.cuda.memory_stats()["requested_bytes.all.peak"] - before
+
+
 def measure(pos_dim, nr_points, iters, warmup, levels=24, log2_capacity=18, fused_optimizer=False, contiguous_output=False):
     torch.manual_seed(0)
     enc = PermutoEncoding(pos_dim, 1 << log2_capacity, levels, 2, np.geomspace(1.0, 1e-4, num=levels),
@@ -241,10 +249,7 @@ def decoder(nr_points, iters, warmup, width=64, blocks=2, dtype=torch.float32, p
         for _ in range(2):
             step()
         torch.cuda.synchronize()
-        torch.cuda.reset_peak_memory_stats()
-        before = torch.cuda.memory_allocated()
-        step()
-        peak = torch.cuda.max_memory_allocated() - before
+        peak = _added_at_peak(step)
         rows.append({"layers": name, "points": nr_points, "width": width, "blocks": blocks, "dtype": str(dtype).split(".")[-1],
                      "train": _timed(step, nr_points, iters, warmup), "peak_bytes": peak})
         print(f"| {name} | {rows[-1]['train']:.3g} | {peak / 2 ** 20:.0f} |", flush=True)
@@ -329,10 +334,7 @@ def experts(nr_points, iters, warmup, width=64, number=16, dtype=torch.float32, 
         for _ in range(2):
             step()
         torch.cuda.synchronize()
-        torch.cuda.reset_peak_memory_stats()
-        before = torch.cuda.memory_allocated()
-        step()
-        peak = torch.cuda.max_memory_allocated() - before
+        peak = _added_at_peak(step)
         rows.append({"layers": name, "points": nr_points, "width": width, "experts": number, "dtype": str(dtype).split(".")[-1],
                      "train": _timed(step, nr_points, iters, warmup), "peak_bytes": peak})
         print(f"| {name} | {rows[-1]['train']:.3g} | {peak / 2 ** 20:.0f} |", flush=True)
