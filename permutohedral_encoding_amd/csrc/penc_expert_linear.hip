@@ -637,30 +637,46 @@ int launch_few(RowsArgs a, hipStream_t stream) {
     return launched();
 }
 
-template <bool kBack, Chunks kChunks>
+// kChunks: of the weights' rows; kChunksN: of the others.
+template <bool kBack, Chunks kChunks, Chunks kChunksN = kChunks>
 int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
     if constexpr (kChunks == Chunks::kDirect) {
         if (a.wide <= 16 * kNarrowTiles && a.deep * kSize <= 64 * kNarrowLines && a.stride * kSize * 64 < 1 << 30) return launch_narrow<kBack>(a, stream);
-        // (rows that are 4 to an expert, 64 experts of 1024 by 4096 bf16: 99 us and 122 without; 16 to an expert 140 and 108)
-        if (!kBack && a.rows <= kFewRows / 2 * static_cast<int64_t>(a.experts)) return launch_few(a, stream);
+        // A few rows: 64 experts of 1024 by 4096 bf16, 4 rows to an expert, 99 us, and 122 without; 16 to an expert 140 and 108.  More of them where the workgroups would be few otherwise, each with
+        // all of a long row: 1257 rows of 82 experts, 2048 by 24 fp32, 23 us and 135.
+        if (!kBack && (a.rows <= kFewRows / 2 * static_cast<int64_t>(a.experts) ||
+                       (a.rows <= 2 * kFewRows * static_cast<int64_t>(a.experts) && row_tiles(a, 256) * ((a.wide + 63) / 64) < kUnits)))
+            return launch_few(a, stream);
+    }
+    // Where tiles of 128 x 128 would leave half of the compute units without one, tiles of 64 x 64, loaded three steps ahead where they come directly: 500 rows of 4096 by 64 bf16 39 us -> 21, of fp32 264 -> 84,
+    // 1000 rows of 512 by 512 fp32 with 3 experts, y and dx, 76 -> 29; with 180 such tiles (5000 rows, 4 experts, bf16) 20 -> 23.
+    if constexpr (kChunks != Chunks::kSingle && kChunksN != Chunks::kSingle) {
+        if (row_tiles(a, 128) * ((a.wide + 127) / 128) < static_cast<int64_t>(kUnits / 2))
+            return launch_rows<kBack, Product<Value, kBack, false, 64, 64, 2, 2, kChunks, kChunks == Chunks::kDirect ? 4 : 2>>(a, stream);
     }
     // (129 to 192 results of rows that begin anywhere: three tiles of 64 take 32.5 us of 70001 x 203 by 130 fp16, two of 128 35.4; of rows on 16 bytes, 208 by 136, 22.3 and 21.0)
-    if (a.wide <= 64 || (kChunks == Chunks::kHeld && a.wide > 128 && a.wide <= 192) || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks>>(a, stream);
+    if (a.wide <= 64 || (kChunks == Chunks::kHeld && a.wide > 128 && a.wide <= 192) || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks, 2, kChunksN>>(a, stream);
     if constexpr (kChunks != Chunks::kSingle) {
         if constexpr (kChunks == Chunks::kDirect && kSize == 2) {
             // (1024 by 4096 bf16, 16 experts, of 2048 rows each: 302 us and 347 without; of 512 89 and 86, of 256 58 and 50: tiles of 256 rows that are not full)
             if (a.rows >= 1024 * static_cast<int64_t>(a.experts) && static_cast<int64_t>(a.rows / 256) * ((a.wide + 255) / 256) >= 512)
                 return launch_rows<kBack, Product<Value, kBack, false, 256, 256, 4, 2, kChunks>, Product<Value, kBack, false, 128, 128, 4, 2, kChunks>>(a, stream);
         }
-        return launch_rows<kBack, Product<Value, kBack, false, 128, 128, 2, 2, kChunks>>(a, stream);
+        return launch_rows<kBack, Product<Value, kBack, false, 128, 128, 2, 2, kChunks, 2, kChunksN>>(a, stream);
     }
 }
 
+// Both operands come directly, or both through registers; value by value only the one whose rows are that short (363113 x 1032 by 4 bf16, with gradients: 915 us, both so 1430).
 template <bool kBack>
-int rows_of_experts(const RowsArgs& a, Chunks chunks, hipStream_t stream) {
-    if (chunks == Chunks::kDirect) return rows_of_experts<kBack, Chunks::kDirect>(a, stream);
-    if (chunks == Chunks::kHeld) return rows_of_experts<kBack, Chunks::kHeld>(a, stream);
-    return rows_of_experts<kBack, Chunks::kSingle>(a, stream);
+int rows_of_experts(const RowsArgs& a, Chunks weight, Chunks rows, hipStream_t stream) {
+    constexpr Chunks kHeld = Chunks::kHeld, kSingle = Chunks::kSingle;
+    if (weight == Chunks::kDirect && rows == Chunks::kDirect) return rows_of_experts<kBack, Chunks::kDirect>(a, stream);
+    if (weight != kSingle && rows != kSingle) return rows_of_experts<kBack, kHeld>(a, stream);
+    if constexpr (kBack) {
+        if (weight != kSingle) return rows_of_experts<kBack, kHeld, kSingle>(a, stream);
+        if (rows != kSingle) return rows_of_experts<kBack, kSingle, kHeld>(a, stream);
+    }
+    return rows_of_experts<kBack, kSingle>(a, stream);
 }
 
 // How the rows of the weights' gradient are cut, and the tiles.  A time is in rows that a workgroup multiplies.
@@ -722,16 +738,24 @@ int launch_narrow_grads(WeightArgs a, const WeightPlan& plan, const void* weight
     return launched();
 }
 
-template <Chunks kChunks>
+template <Chunks kChunks, Chunks kChunksN = kChunks>
 int weights_of_experts(const WeightArgs& a, const WeightPlan& plan, hipStream_t stream) {
-    if (plan.side == 64) return launch_weights<Product<Value, true, true, 64, 64, 2, 2, kChunks>>(a, plan, stream);
-    if constexpr (kChunks != Chunks::kSingle) {
+    if (plan.side == 64) return launch_weights<Product<Value, true, true, 64, 64, 2, 2, kChunks, 2, kChunksN>>(a, plan, stream);
+    if constexpr (kChunks != Chunks::kSingle && kChunksN != Chunks::kSingle) {
         if constexpr (kChunks == Chunks::kDirect && kSize == 2) {
             if (plan.side == 256) return launch_weights<Product<Value, true, true, 256, 256, 2, 4, kChunks>>(a, plan, stream);
         }
         return launch_weights<Product<Value, true, true, 128, 128, 2, 2, kChunks>>(a, plan, stream);
     }
     return PENC_ERR_BAD_LAYER_SIZE;  // (not reached: rows of less than 16 bytes have less than 64 values)
+}
+int weights_of_experts(const WeightArgs& a, const WeightPlan& plan, Chunks x, Chunks grad, hipStream_t stream) {
+    constexpr Chunks kHeld = Chunks::kHeld, kSingle = Chunks::kSingle;
+    if (x == Chunks::kDirect && grad == Chunks::kDirect) return weights_of_experts<Chunks::kDirect>(a, plan, stream);
+    if (x != kSingle && grad != kSingle) return weights_of_experts<kHeld>(a, plan, stream);
+    if (x != kSingle) return weights_of_experts<kHeld, kSingle>(a, plan, stream);
+    if (grad != kSingle) return weights_of_experts<kSingle, kHeld>(a, plan, stream);
+    return weights_of_experts<kSingle>(a, plan, stream);
 }
 
 }  // namespace
@@ -741,8 +765,8 @@ int expert_rows<PENC_TYPE>(bool back, int64_t rows, int experts, int64_t wide, i
                            const int32_t* offsets, void* out, hipStream_t stream) {
     if (rows == 0) return PENC_OK;
     RowsArgs a{in, weight, bias, out, stride, offsets, experts, static_cast<int>(rows), static_cast<int>(wide), static_cast<int>(deep), {}, 0};
-    const Chunks chunks = std::max(chunks_of(in, stride, deep), chunks_of(weight, back ? wide : deep, back ? wide : deep));
-    return back ? rows_of_experts<true>(a, chunks, stream) : rows_of_experts<false>(a, chunks, stream);
+    const Chunks of_weight = chunks_of(weight, back ? wide : deep, back ? wide : deep), of_rows = chunks_of(in, stride, deep);
+    return back ? rows_of_experts<true>(a, of_weight, of_rows, stream) : rows_of_experts<false>(a, of_weight, of_rows, stream);
 }
 
 template <>
@@ -758,15 +782,12 @@ int expert_grads<PENC_TYPE>(int64_t rows, int experts, int64_t channels, int64_t
     const WeightPlan plan = weight_plan(rows, experts, channels, outputs);
     WeightArgs a{x, grad, x_stride, grad_stride, offsets, experts, static_cast<int>(rows), static_cast<int>(channels), static_cast<int>(outputs),
                  static_cast<int>(plan.most), {}, 0, 0, dweight, dbias, static_cast<float*>(workspace), plan.pieces};
-    const Chunks chunks = std::max(chunks_of(x, x_stride, channels), chunks_of(grad, grad_stride, outputs));
-    const bool together = dx != nullptr && channels <= 64 && outputs <= 64 && chunks == Chunks::kDirect && aligned_to(weight, 16) && aligned_to(dx, 16);
+    const Chunks of_x = chunks_of(x, x_stride, channels), of_grad = chunks_of(grad, grad_stride, outputs);
+    const bool together = dx != nullptr && channels <= 64 && outputs <= 64 && of_x == Chunks::kDirect && of_grad == Chunks::kDirect && aligned_to(weight, 16) && aligned_to(dx, 16);
     if (dx != nullptr && !together) {
         if (const int rc = expert_rows<PENC_TYPE>(true, rows, experts, channels, outputs, grad, grad_stride, weight, nullptr, offsets, dx, stream)) return rc;
     }
-    if (const int rc = together                     ? launch_narrow_grads(a, plan, weight, dx, stream)
-                       : chunks == Chunks::kDirect ? weights_of_experts<Chunks::kDirect>(a, plan, stream)
-                       : chunks == Chunks::kHeld   ? weights_of_experts<Chunks::kHeld>(a, plan, stream)
-                                                   : weights_of_experts<Chunks::kSingle>(a, plan, stream))
+    if (const int rc = together ? launch_narrow_grads(a, plan, weight, dx, stream) : weights_of_experts(a, plan, of_x, of_grad, stream))
         return rc;
     if (rows <= plan.most) return PENC_OK;
     const int64_t results = outputs * (channels + 1);

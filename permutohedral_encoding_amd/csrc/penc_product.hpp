@@ -260,16 +260,17 @@ __device__ __forceinline__ void wait_for_loads() {
 }
 
 // A workgroup of kWavesM x kWavesN waves, each with kM / kWavesM x kN / kWavesN results; kRing steps have room in the LDS.
-template <class E, bool kAlongM, bool kAlongN, int kM_, int kN_, int kWavesM_, int kWavesN_, Chunks kChunksCome, int kRing = 2>
+template <class E, bool kAlongM, bool kAlongN, int kM_, int kN_, int kWavesM_, int kWavesN_, Chunks kChunksM, int kRing = 2, Chunks kChunksN = kChunksM>
 struct Product {
     static constexpr int kWavesM = kWavesM_, kWavesN = kWavesN_;
     static constexpr int kM = kM_, kN = kN_, kThreads = 64 * kWavesM * kWavesN;
     static constexpr int kTilesM = kM / kWavesM / 16, kTilesN = kN / kWavesN / 16;
     using TileM = OperandTile<E, kAlongM, kM>;
     using TileN = OperandTile<E, kAlongN, kN>;
-    static constexpr bool kDirect = kChunksCome == Chunks::kDirect;
-    using LoadM = Loader<E, kAlongM, kM, kThreads, kChunksCome>;
-    using LoadN = Loader<E, kAlongN, kN, kThreads, kChunksCome>;
+    static constexpr bool kDirect = kChunksM == Chunks::kDirect;
+    static_assert(kDirect == (kChunksN == Chunks::kDirect));
+    using LoadM = Loader<E, kAlongM, kM, kThreads, kChunksM>;
+    using LoadN = Loader<E, kAlongN, kN, kThreads, kChunksN>;
     static constexpr int kStage = TileM::kSize + TileN::kSize;
     static constexpr int kLds = kRing * kStage;
     static constexpr int kDepth = ProductType<E>::kDepth, kParts = ProductType<E>::kParts;

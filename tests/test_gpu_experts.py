@@ -286,13 +286,21 @@ def test_expert_linear_of_narrow_layers_and_of_few_rows(dtype, rows, number, cha
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,channels,outputs", [(500, 1, 1024, 64), (130, 7, 1032, 24), (500, 1, 1023, 63), (300, 2, 64, 1030), (65, 1, 136, 136), (900, 2, 3, 300), (900, 2, 300, 2)])
+def test_expert_linear_of_long_rows_that_are_few(dtype, rows, number, channels, outputs):
+    check_products(rows, number, channels, outputs, TYPES[dtype])
+    check_products(rows, number, channels, outputs, TYPES[dtype], bias=False, none=0.4, extra=8, empty=(0,) if number > 1 else ())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_expert_linear_of_rows_that_begin_anywhere(dtype):
     for extra in (1, 2, 3, 5):
         check_products(401, 3, 64, 136, TYPES[dtype], extra=extra)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,number,channels,outputs", [(70001, 2, 64, 64), (50000, 1, 48, 130), (40000, 3, 128, 128), (20000, 300, 32, 64)])
+@pytest.mark.parametrize("rows,number,channels,outputs", [(70001, 2, 64, 64), (50000, 1, 48, 130), (40000, 3, 128, 128), (20000, 300, 32, 64), (40000, 3, 101, 130),
+                                                          (40000, 3, 101, 60), (30000, 2, 3, 200), (30000, 2, 200, 3), (30000, 2, 5, 6), (30000, 3, 200, 264)])
 def test_expert_linear_of_many_rows(dtype, rows, number, channels, outputs):
     """(the rows of an expert are cut for its weights' gradient)"""
     first = check_products(rows, number, channels, outputs, TYPES[dtype])
