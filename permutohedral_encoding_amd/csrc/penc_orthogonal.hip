@@ -13,7 +13,7 @@
 // The matrix cores run float16 8 times as fast as float32, so that three products take 3/8 of the time.
 //
 // S and S S are symmetric: tiles on one side of the diagonal are computed and stored twice.  Matrices of up to 128 rows (or columns) that fit the LDS go through all of their
-// steps there, one to a workgroup.
+// steps there, one to a workgroup; thin ones in 64 bits, by their S alone.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -590,6 +590,216 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
 }
 
 // ------------------------------------------------------------------------------------------
+// thin matrices
+
+constexpr int kThin = 64, kThinThreads = 256, kThinChunk = 64;  // rows; numbers of the long side at a time
+constexpr int kMostThinPieces = 64;
+constexpr double kMostThinGrowth = 1 << 27;  // of 2^-53
+using four_doubles = double __attribute__((ext_vector_type(4)));
+
+// Matrices of up to 64 rows (or columns) that are long, or too long for the LDS.  X stays what it is multiplied by from the left: X = Q G / (|G| + eps) with Q = P P' .., P = a + b S + c S S and S' = P S P, all of them small, so that G is read once for S and once
+// for the result.  S is off by 2^-53 of its largest value, and what is small in it is taken up by a^2 in each step: in 64 bits five steps make 2^-35 of it (in 32 it would be 2^-6).
+
+// 64 numbers of the long side from m0 on, for each of the small side's: x[small][64], zeros behind the end.
+template <class G, int kRows>
+__device__ __forceinline__ void load_thin(float (&x)[kRows][kThinChunk + 1], const G* __restrict__ g, int small, int large, bool tall, int m0) {
+    const int there = min(large - m0, kThinChunk);
+    if (tall) {
+        const G* const from = g + static_cast<int64_t>(m0) * small;
+        for (int i = static_cast<int>(threadIdx.x); i < kThinChunk * small; i += kThinThreads) x[i % small][i / small] = i < there * small ? static_cast<float>(from[i]) : 0.0f;
+    } else {
+        for (int i = static_cast<int>(threadIdx.x); i < kThinChunk * small; i += kThinThreads) {
+            const int j = i / kThinChunk, m = i % kThinChunk;
+            x[j][m] = m < there ? static_cast<float>(g[static_cast<int64_t>(j) * large + m0 + m]) : 0.0f;
+        }
+    }
+}
+template <int kRows>
+__device__ __forceinline__ void clear_rows_behind(float (&x)[kRows][kThinChunk + 1], int small) {
+    for (int i = small * kThinChunk + static_cast<int>(threadIdx.x); i < kRows * kThinChunk; i += kThinThreads) x[i / kThinChunk][i % kThinChunk] = 0.0f;
+}
+
+// Where result r of a lane is in a tile of 16 x 16: v_mfma_f64_16x16x4_f64 takes row (column) lane % 16 of k lane / 16.
+__device__ __forceinline__ int thin_row(int r) { return 4 * r + static_cast<int>(threadIdx.x) % 64 / 16; }
+
+// The tiles of 16 x 16 on and behind the diagonal, of 16 kTiles rows: waves have every fourth.  All that is multiplied here is symmetric: polynomials of one S.
+template <int kTiles>
+struct ThinTiles {
+    static constexpr int kRows = 16 * kTiles, kUnits = kTiles * (kTiles + 1) / 2, kEach = (kUnits + 3) / 4;
+    int i[kEach], j[kEach];
+    bool there[kEach];
+    __device__ __forceinline__ ThinTiles() {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            int unit = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) + 4 * e, row = 0;
+            there[e] = unit < kUnits;
+            if (!there[e]) unit = 0;
+            while (unit >= kTiles - row) unit -= kTiles - row, ++row;
+            i[e] = row * 16, j[e] = (row + unit) * 16;
+        }
+    }
+};
+
+// G G^T of a piece of the long side, each wave's tiles as its registers have them; of one tile each wave has a quarter of the numbers.
+template <class G, int kTiles>
+__global__ __launch_bounds__(kThinThreads) void thin_gram_kernel(int small, int large, bool tall, int pieces, const G* __restrict__ g, four_doubles* __restrict__ sums) {
+    using Tiles = ThinTiles<kTiles>;
+    __shared__ float x[16 * kTiles][kThinChunk + 1];
+    const int64_t matrix = blockIdx.x / pieces;
+    const int l16 = threadIdx.x % 16, q = threadIdx.x % 64 / 16, quarter = kTiles == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * (kThinChunk / 4) : 0;
+    const int chunks = (large + kThinChunk - 1) / kThinChunk, piece = static_cast<int>(blockIdx.x % pieces);
+    const Tiles tiles;
+    g += matrix * small * large;
+    clear_rows_behind(x, small);
+    four_doubles sum[Tiles::kEach] = {};
+    for (int c = piece * chunks / pieces; c < (piece + 1) * chunks / pieces; ++c) {
+        load_thin(x, g, small, large, tall, c * kThinChunk);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < (kTiles == 1 ? kThinChunk / 4 : kThinChunk); k += 4) {
+#pragma unroll
+            for (int e = 0; e < Tiles::kEach; ++e) {
+                const int at = quarter + k + q;
+                sum[e] = __builtin_amdgcn_mfma_f64_16x16x4f64(static_cast<double>(x[tiles.i[e] + l16][at]), static_cast<double>(x[tiles.j[e] + l16][at]), sum[e], 0, 0, 0);
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int e = 0; e < Tiles::kEach; ++e) sums[(static_cast<int64_t>(blockIdx.x) * Tiles::kEach + e) * kThinThreads + threadIdx.x] = sum[e];
+}
+
+// Q / (|G| + eps) of a matrix.
+template <int kTiles>
+__global__ __launch_bounds__(kThinThreads) void thin_steps_kernel(int small, int pieces, int steps, Coefficients k, const four_doubles* __restrict__ sums, double* __restrict__ result) {
+    using Tiles = ThinTiles<kTiles>;
+    constexpr int kRows = Tiles::kRows, kEach = Tiles::kEach;
+    constexpr int kPitch = kRows + 1;  // (16 rows, or 16 numbers of one, meet no bank twice; kRows + 4, so that 16 rows of 4 do not, is 10 to 20% slower)
+    __shared__ double s[kRows][kPitch], p[kRows][kPitch], q[kRows][kPitch], v[kRows][kPitch];
+    const int l16 = threadIdx.x % 16, q4 = threadIdx.x % 64 / 16, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const Tiles tiles;
+    using Matrix = double[kRows][kPitch];
+    const auto product = [&](int e, const Matrix& a, const Matrix& b) {
+        four_doubles sum{};
+#pragma unroll
+        for (int n = 0; n < kRows; n += 4) sum = __builtin_amdgcn_mfma_f64_16x16x4f64(a[tiles.i[e] + l16][n + q4], b[n + q4][tiles.j[e] + l16], sum, 0, 0, 0);
+        return sum;
+    };
+    const auto store = [&](int e, Matrix& to, four_doubles x) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            to[tiles.i[e] + thin_row(r)][tiles.j[e] + l16] = x[r];
+            if (tiles.i[e] != tiles.j[e]) to[tiles.j[e] + l16][tiles.i[e] + thin_row(r)] = x[r];
+        }
+    };
+    const auto own = [&](int e, const Matrix& from) {
+        four_doubles x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = from[tiles.i[e] + thin_row(r)][tiles.j[e] + l16];
+        return x;
+    };
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const four_doubles* const from = sums + (static_cast<int64_t>(blockIdx.x) * pieces * kEach + e) * kThinThreads + threadIdx.x;
+        four_doubles sum{};
+#pragma unroll 8
+        for (int n = 0; n < pieces; ++n) sum += from[n * (kEach * kThinThreads)];
+        if constexpr (kTiles > 1) {
+            if (tiles.there[e]) store(e, s, sum);
+        } else {
+            // (the four waves' quarters, in order)
+            if (wave == 0) store(e, s, sum);
+            if (wave == 1) store(e, p, sum);
+            if (wave == 2) store(e, q, sum);
+            if (wave == 3) store(e, v, sum);
+            __syncthreads();
+            if (wave == 0) store(e, s, (sum + own(e, p)) + (own(e, q) + own(e, v)));
+        }
+    }
+    __syncthreads();
+    double squares = 0.0;
+    for (int i = 0; i < small; ++i) squares += s[i][i];
+    const double factor = 1.0 / (sqrt(squares) + static_cast<double>(k.eps));
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+        if (tiles.there[e]) store(e, s, own(e, s) * (factor * factor));
+    for (int step = 0; step < steps; ++step) {
+        const bool last = step + 1 == steps;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (!tiles.there[e]) continue;
+            four_doubles x = product(e, s, s) * static_cast<double>(k.c) + own(e, s) * static_cast<double>(k.b);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] += tiles.i[e] + thin_row(r) == tiles.j[e] + l16 ? static_cast<double>(k.a) : 0.0;
+            store(e, p, x);
+        }
+        __syncthreads();
+        four_doubles next[kEach];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (!tiles.there[e]) continue;
+            next[e] = step > 0 ? product(e, q, p) : own(e, p);
+            if (!last) store(e, v, product(e, p, s));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (!tiles.there[e]) continue;
+            store(e, q, next[e]);
+            if (!last) store(e, s, product(e, v, p));
+        }
+    }
+    __syncthreads();
+    for (int i = static_cast<int>(threadIdx.x); i < kRows * kRows; i += kThinThreads) result[static_cast<int64_t>(blockIdx.x) * kRows * kRows + i] = q[i / kRows][i % kRows] * factor;
+}
+
+// Q G: a workgroup takes 64 numbers of the long side at a time.
+template <class G, int kTiles>
+__global__ __launch_bounds__(kThinThreads) void thin_apply_kernel(int small, int large, bool tall, int blocks, const double* __restrict__ factors, const G* __restrict__ g,
+                                                                  G* __restrict__ result) {
+    constexpr int kRows = 16 * kTiles;
+    __shared__ float x[kRows][kThinChunk + 1];
+    const int64_t matrix = blockIdx.x / blocks;
+    const int lane = threadIdx.x % 64, l16 = lane % 16, q4 = lane / 16, m = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 16 + l16;
+    g += matrix * small * large, result += matrix * small * large;
+    double q[kTiles][kRows / 4];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int n = 0; n < kRows / 4; ++n) q[t][n] = factors[matrix * kRows * kRows + (t * 16 + l16) * kRows + n * 4 + q4];
+    clear_rows_behind(x, small);
+    for (int m0 = static_cast<int>(blockIdx.x % blocks) * kThinChunk; m0 < large; m0 += blocks * kThinChunk) {
+        load_thin(x, g, small, large, tall, m0);
+        __syncthreads();
+        four_doubles sum[kTiles] = {};
+#pragma unroll
+        for (int n = 0; n < kRows / 4; ++n) {
+            const double b = static_cast<double>(x[n * 4 + q4][m]);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) sum[t] = __builtin_amdgcn_mfma_f64_16x16x4f64(q[t][n], b, sum[t], 0, 0, 0);
+        }
+        // (a wave's columns are its own: it has read them; rows behind the last stay zeros)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (t * 16 + thin_row(r) < small) x[t * 16 + thin_row(r)][m] = static_cast<float>(sum[t][r]);
+        __syncthreads();
+        const int there = min(large - m0, kThinChunk);
+        if (tall) {
+            G* const to = result + static_cast<int64_t>(m0) * small;
+            for (int i = static_cast<int>(threadIdx.x); i < there * small; i += kThinThreads) to[i] = static_cast<G>(x[i % small][i / small]);
+        } else {
+            for (int i = static_cast<int>(threadIdx.x); i < kThinChunk * small; i += kThinThreads)
+                if (i % kThinChunk < there) result[static_cast<int64_t>(i / kThinChunk) * large + m0 + i % kThinChunk] = static_cast<G>(x[i / kThinChunk][i % kThinChunk]);
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------------------
 // the optimiser's own part: a pass over memory before the products and one behind them
 
 // m += (1 - momentum) (g - m), and the update g + momentum (m - g) or m itself
@@ -639,6 +849,43 @@ int resident(int64_t matrices, int64_t rows, int64_t columns, int steps, Coeffic
     if (small <= 64) return launch(std::integral_constant<int, 4>{});
     if (small <= 96) return launch(std::integral_constant<int, 6>{});
     return launch(std::integral_constant<int, 8>{});
+}
+
+// Three launches against a chain of them, or against one workgroup that has a matrix to itself (us, fp32, so and otherwise): 14 x 2048 x 6 15 and 121, 1 x 32 x 4096 25 and 120, 8 x 64 x 4096 81 and 125;
+// 1 x 18 x 1104 23 and 50, 1 x 16 x 128 12 and 16, 1 x 18 x 300 21 and 22, 1 x 48 x 400 45 and 50, 1 x 64 x 400 67 and 53; 64 x 32 x 1100 44 and 53, 256 of them 83 and 56.
+bool is_thin(int64_t matrices, int64_t rows, int64_t columns) {
+    const int64_t small = std::min(rows, columns);
+    return small <= kThin && (!is_resident(rows, columns) || (matrices <= 64 && small <= 48 && std::max(rows, columns) >= (small <= 16 ? 128 : small <= 32 ? 300 : 350)));
+}
+int thin_pieces(int64_t matrices, int64_t large) {
+    return static_cast<int>(std::max<int64_t>(1, std::min({(large + 4 * kThinChunk - 1) / (4 * kThinChunk), int64_t{kMostThinPieces}, (int64_t{1} << 22) / matrices})));
+}
+int thin_tiles(int64_t rows, int64_t columns) { return static_cast<int>((std::min(rows, columns) + 15) / 16); }
+size_t thin_workspace(int64_t matrices, int64_t rows, int64_t columns) {
+    const int tiles = thin_tiles(rows, columns);
+    return static_cast<size_t>(matrices) * (thin_pieces(matrices, std::max(rows, columns)) * static_cast<size_t>((tiles * (tiles + 1) / 2 + 3) / 4) * (kThinThreads * sizeof(four_doubles)) +
+                                            256 * tiles * tiles * sizeof(double));
+}
+template <class G>
+int thin(int64_t matrices, int64_t rows, int64_t columns, int steps, Coefficients k, const G* g, G* result, char* workspace, hipStream_t stream) {
+    const bool tall = rows > columns;
+    const int small = static_cast<int>(std::min(rows, columns)), large = static_cast<int>(std::max(rows, columns)), pieces = thin_pieces(matrices, large), tiles = thin_tiles(rows, columns);
+    double* const factors = reinterpret_cast<double*>(workspace);
+    four_doubles* const sums = reinterpret_cast<four_doubles*>(factors + matrices * 256 * tiles * tiles);
+    const int blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((large + kThinChunk - 1) / kThinChunk, (int64_t{1} << 22) / matrices)));
+    const auto launch = [&](auto tiles) -> int {
+        constexpr int kTiles = decltype(tiles)::value;
+        thin_gram_kernel<G, kTiles><<<static_cast<unsigned>(matrices * pieces), kThinThreads, 0, stream>>>(small, large, tall, pieces, g, sums);
+        if (const int rc = launched()) return rc;
+        thin_steps_kernel<kTiles><<<static_cast<unsigned>(matrices), kThinThreads, 0, stream>>>(small, pieces, steps, k, sums, factors);
+        if (const int rc = launched()) return rc;
+        thin_apply_kernel<G, kTiles><<<static_cast<unsigned>(matrices * blocks), kThinThreads, 0, stream>>>(small, large, tall, blocks, factors, g, result);
+        return launched();
+    };
+    if (tiles == 1) return launch(std::integral_constant<int, 1>{});
+    if (tiles == 2) return launch(std::integral_constant<int, 2>{});
+    if (tiles == 3) return launch(std::integral_constant<int, 3>{});
+    return launch(std::integral_constant<int, 4>{});
 }
 
 // Whether a launch takes tiles of 64 x 64: where there would not be a workgroup of 128 x 128 for each compute unit.
@@ -754,15 +1001,17 @@ int orthogonalise(int64_t matrices, int64_t rows, int64_t columns, int steps, Co
     return PENC_OK;
 }
 
-// What the steps make of 0 .. 1 has to stay where float16 times 2^12 has room: |X| <= 3, and F <= 15.
-bool bounded(double a, double b, double c, int steps) {
+// What the steps make of 0 .. 1 has to stay where float16 times 2^12 has room: |X| <= 3, and F <= 15.  `growth`: the most that they make of a rounding of S.
+bool bounded(double a, double b, double c, int steps, double& growth) {
     double most = 1.0;
+    growth = 1.0;
     for (int step = 0; step < steps; ++step) {
         const double t = most * most;
+        double p = std::max(std::abs(a), std::abs(a + b * t + c * t * t));
         double f = std::max(0.0, std::abs(b * t + c * t * t)), x = std::abs((a + b * t + c * t * t) * most);
         if (c != 0.0) {
             const double at = -b / (2.0 * c);  // of b t + c t^2
-            if (at > 0.0 && at < t) f = std::max(f, std::abs(b * at + c * at * at));
+            if (at > 0.0 && at < t) f = std::max(f, std::abs(b * at + c * at * at)), p = std::max(p, std::abs(a + b * at + c * at * at));
             const double d = 9.0 * b * b - 20.0 * a * c;  // of a s + b s^3 + c s^5, whose slope is a + 3 b t + 5 c t^2
             if (d >= 0.0)
                 for (const double sign : {-1.0, 1.0}) {
@@ -774,6 +1023,7 @@ bool bounded(double a, double b, double c, int steps) {
             if (u > 0.0 && u < t) x = std::max(x, std::abs((a + b * u) * std::sqrt(u)));
         }
         if (!(f <= 15.0) || !(x <= 3.0)) return false;
+        growth *= p * p;
         most = std::max(x, 1e-30);
     }
     return true;
@@ -791,8 +1041,11 @@ using namespace penc;
 extern "C" {
 
 size_t penc_orthogonalise_workspace_bytes(int type, int64_t matrices, int64_t rows, int64_t columns) {
-    if (bad_matrices(matrices, rows, columns) || is_resident(rows, columns)) return 0;
-    return type == PENC_BF16 ? layout_of<half_t>(matrices, rows, columns).total : layout_of<split_t>(matrices, rows, columns).total;
+    if (bad_matrices(matrices, rows, columns) || matrices == 0) return 0;
+    const size_t of_thin = is_thin(matrices, rows, columns) ? thin_workspace(matrices, rows, columns) : 0;
+    if (is_resident(rows, columns)) return of_thin;
+    // (thin matrices too, for steps that are not theirs)
+    return std::max(of_thin, type == PENC_BF16 ? layout_of<half_t>(matrices, rows, columns).total : layout_of<split_t>(matrices, rows, columns).total);
 }
 
 int penc_orthogonalise(int type, int64_t matrices, int64_t rows, int64_t columns, int steps, float a, float b, float c, float eps, const void* update, void* result,
@@ -800,7 +1053,8 @@ int penc_orthogonalise(int type, int64_t matrices, int64_t rows, int64_t columns
     return with_type(type, [&](auto e) -> int {
         using G = decltype(e);
         if (bad_matrices(matrices, rows, columns) || steps < 1 || steps > PENC_MAX_ORTHOGONAL_STEPS) return PENC_ERR_BAD_LAYER_SIZE;
-        if (!(eps >= 1e-30f) || std::isinf(eps) || !bounded(a, b, c, steps)) return PENC_ERR_UNSUPPORTED_KIND;
+        double growth;
+        if (!(eps >= 1e-30f) || std::isinf(eps) || !bounded(a, b, c, steps, growth)) return PENC_ERR_UNSUPPORTED_KIND;
         if (matrices == 0) return PENC_OK;
         if (!update || !result) return PENC_ERR_NULL_POINTER;
         if (!aligned_to(update, sizeof(G)) || !aligned_to(result, 4 * sizeof(G)) || !aligned_to(workspace, 256)) return PENC_ERR_MISALIGNED;
@@ -811,7 +1065,8 @@ int penc_orthogonalise(int type, int64_t matrices, int64_t rows, int64_t columns
         const hipStream_t s = static_cast<hipStream_t>(stream);
         const G* const from = static_cast<const G*>(update);
         G* const to = static_cast<G*>(result);
-        if (need == 0) return resident<G>(matrices, rows, columns, steps, k, from, to, s);
+        if (is_thin(matrices, rows, columns) && growth <= kMostThinGrowth) return thin<G>(matrices, rows, columns, steps, k, from, to, static_cast<char*>(workspace), s);
+        if (is_resident(rows, columns)) return resident<G>(matrices, rows, columns, steps, k, from, to, s);
         using E = std::conditional_t<std::is_same_v<G, bf16_t>, half_t, split_t>;
         return orthogonalise<E, G>(matrices, rows, columns, steps, k, from, to, static_cast<char*>(workspace), s);
     });

@@ -61,6 +61,34 @@ def test_larger_matrices(dtype, matrices, rows, columns):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("matrices,rows,columns", [(1, 1, 128), (3, 16, 129), (2, 300, 7), (64, 5, 200), (65, 5, 200), (1, 17, 300), (2, 1104, 18), (5, 32, 2000), (1, 33, 350), (2, 48, 1000), (1, 1000, 47), (2, 64, 2500),
+                                                   (1, 3001, 50), (1, 20, 65536), (300, 2000, 3)])
+def test_thin_matrices(dtype, matrices, rows, columns):
+    update = updates(matrices, rows, columns, TYPES[dtype])
+    assert_orthogonalised(optim.orthogonalise(update), update)
+
+
+def test_thin_matrices_of_every_kind():
+    """Rows that are alike, or zero: S has eigenvalues of zero, and roundings of S may be below.  Steps that a rounding of S would not survive go another way."""
+    for shape in ((2, 12, 300), (2, 700, 30), (1, 60, 1500)):
+        update = updates(*shape, torch.float32)
+        alike = update.clone()
+        alike[..., 1, :] = alike[..., 0, :]
+        alike[..., 2, :] = 0.0
+        for given in (update, alike):
+            for options in (dict(), dict(steps=1), dict(steps=7), dict(steps=8), dict(steps=20), dict(coefficients=(1.5, -0.5, 0.0), steps=12), dict(eps=1.0)):
+                assert_orthogonalised(optim.orthogonalise(given, **options), given, **options)
+        update[0, 0, 0] = math.nan
+        got = optim.orthogonalise(update)
+        assert bool(got[0].isnan().all()) and bool(torch.isfinite(got[1:]).all())
+        update[0, 0, 0] = -math.inf
+        assert torch.equal(optim.orthogonalise(update)[1:], got[1:]) and bool(optim.orthogonalise(update)[0].isnan().all())
+        for scale in (2.0 ** 116, 2.0 ** -110):
+            given = updates(*shape, torch.float32, scale=scale)
+            assert_orthogonalised(optim.orthogonalise(given, eps=1e-30), given, eps=1e-30)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_steps_coefficients_and_eps(dtype):
     for shape in ((3, 40, 60), (2, 140, 200)):
         update = updates(*shape, TYPES[dtype])
@@ -118,7 +146,7 @@ def test_refusals():
 
 
 def test_on_another_stream_and_in_a_graph():
-    for shape in ((4, 64, 96), (2, 150, 200)):
+    for shape in ((4, 64, 96), (2, 150, 200), (3, 20, 1000)):
         given = updates(*shape, torch.bfloat16)
         want = optim.orthogonalise(given)
         side = torch.cuda.Stream()
