@@ -42,12 +42,11 @@ __device__ __forceinline__ T over_lanes(T v, F&& f) {
     return v;
 }
 
-// A logit as an integer that is larger where the logit is: a NaN is the largest, -0 is 0; 0 for what cannot be chosen.
+// A logit as an integer that is larger where the logit is: a NaN is the largest, -0 is 0.  Up to kNone nothing is chosen: -inf, and 0 for what has been chosen before.
+constexpr uint32_t kNone = 0x007FFFFFu;
 __device__ __forceinline__ uint32_t key_of(float v) {
-    const uint32_t b = __float_as_uint(v + 0.0f);
-    if (v != v) return 0xFFFFFFFFu;
-    const uint32_t key = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
-    return v == -__builtin_inff() ? 0u : key;
+    const uint32_t b = __float_as_uint(v + 0.0f), key = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+    return v != v ? 0xFFFFFFFFu : key;
 }
 __device__ __forceinline__ float logit_of(uint32_t key) {
     return key == 0xFFFFFFFFu ? __builtin_nanf("") : __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xFFFFFFFFu));
@@ -105,17 +104,35 @@ struct LogitRow {
     }
 };
 
-// A row to kLanes lanes, which have it in registers: k times the largest key, and the lowest index that has it.  1048576 x 64 fp32, two choices: see the
-// figures in route_backward_kernel's comment.
+// A logit of 16 bits, which has the last 13 bits of a float free, and its expert in one integer: the largest of them is the largest logit's, and of equal ones the lowest expert's.
+constexpr uint32_t kPackedIndex = 0x1FFFu;
+static_assert(PENC_MAX_EXPERTS <= kPackedIndex);
+__device__ __forceinline__ uint32_t packed_key(float v, int index) { return (key_of(v) & ~kPackedIndex) | (kPackedIndex - static_cast<uint32_t>(index)); }
+__device__ __forceinline__ float packed_logit(uint32_t key) {
+    const uint32_t k = key & ~kPackedIndex;
+    return k == ~kPackedIndex ? __builtin_nanf("") : logit_of(k >> 31 ? k : k | kPackedIndex);
+}
+
+// A row to kLanes lanes, which have it in registers: k times the largest key, and the lowest index that has it.  Of 16 bits both are one integer.  Instructions bound it but for a few
+// choices of a few experts: 435701 x 144 bf16, four choices, 65 us (with both apart, 32 lanes and 64 logits more than there are 120), 2^20 x 64 fp32, two choices, 52 (5.5 TB/s).
 template <class E, int kLanes, int kChunks, int kMost>
 __global__ __launch_bounds__(kThreads) void route_kernel(row_t rows, int experts, int choices, bool normalise, const E* __restrict__ logits, uint32_t stride,
                                                          float* __restrict__ weights, int32_t* __restrict__ chosen) {
     for (row_t row = blockIdx.x * static_cast<row_t>(kThreads / kLanes) + threadIdx.x / kLanes; row < rows; row += gridDim.x * static_cast<row_t>(kThreads / kLanes)) {
         using Row = LogitRow<E, kLanes, kChunks>;
         const Row r(logits + offset_of(row, stride), experts);
+        constexpr bool kPacked = sizeof(E) == 2;
         uint32_t keys[Row::kValues];
 #pragma unroll
-        for (int i = 0; i < Row::kValues; ++i) keys[i] = key_of(r.v[i]);
+        for (int i = 0; i < Row::kValues; ++i) {
+            if constexpr (kPacked) keys[i] = packed_key(r.v[i], Row::index_of(i));
+            else keys[i] = key_of(r.v[i]);
+        }
+        const auto largest = [](uint32_t a, uint32_t b) { return max(a, b); };
+        const auto logit = [](uint32_t key) {
+            if constexpr (kPacked) return packed_logit(key);
+            else return logit_of(key);
+        };
         uint32_t best[kMost];
         int at[kMost];
 #pragma unroll
@@ -123,31 +140,42 @@ __global__ __launch_bounds__(kThreads) void route_kernel(row_t rows, int experts
             best[j] = 0, at[j] = -1;
             if (j >= choices) continue;
             uint32_t key = keys[0];
-            int index = Row::index_of(0);
+            if constexpr (kPacked) {
 #pragma unroll
-            for (int i = 1; i < Row::kValues; ++i)
-                if (keys[i] > key) key = keys[i], index = Row::index_of(i);
-            best[j] = over_lanes<kLanes>(key, [](uint32_t a, uint32_t b) { return max(a, b); });
-            const uint32_t mine = key == best[j] ? static_cast<uint32_t>(index) : 0x7FFFFFFFu;
-            at[j] = static_cast<int>(over_lanes<kLanes>(mine, [](uint32_t a, uint32_t b) { return min(a, b); }));
+                for (int i = 1; i < Row::kValues; ++i) key = max(key, keys[i]);
+                best[j] = over_lanes<kLanes>(key, largest);
+                at[j] = static_cast<int>(kPackedIndex - (best[j] & kPackedIndex));
+                if (j + 1 == kMost) continue;
 #pragma unroll
-            for (int i = 0; i < Row::kValues; ++i) keys[i] = at[j] == Row::index_of(i) ? 0u : keys[i];
+                for (int i = 0; i < Row::kValues; ++i) keys[i] = keys[i] == best[j] ? 0u : keys[i];
+            } else {
+                int index = Row::index_of(0);
+#pragma unroll
+                for (int i = 1; i < Row::kValues; ++i)
+                    if (keys[i] > key) key = keys[i], index = Row::index_of(i);
+                best[j] = over_lanes<kLanes>(key, largest);
+                const uint32_t mine = key == best[j] ? static_cast<uint32_t>(index) : 0x7FFFFFFFu;
+                at[j] = static_cast<int>(over_lanes<kLanes>(mine, [](uint32_t a, uint32_t b) { return min(a, b); }));
+                if (j + 1 == kMost) continue;
+#pragma unroll
+                for (int i = 0; i < Row::kValues; ++i) keys[i] = at[j] == Row::index_of(i) ? 0u : keys[i];
+            }
         }
-        const float top = logit_of(best[0]);
+        const float top = logit(best[0]);
         float w[kMost], sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < kMost; ++j) {
-            w[j] = best[j] != 0 ? expf(logit_of(best[j]) - top) : 0.0f;
+            w[j] = best[j] > kNone ? expf(logit(best[j]) - top) : 0.0f;
             sum += w[j];
         }
-        if (!normalise) sum = best[0] != 0 ? r.total(top) : 1.0f;
-        if (best[0] == 0) sum = 1.0f;
+        if (!normalise) sum = best[0] > kNone ? r.total(top) : 1.0f;
+        if (best[0] <= kNone) sum = 1.0f;
 #pragma unroll
         for (int j = 0; j < kMost; ++j) {
             if (j >= choices || static_cast<int>(threadIdx.x) % kLanes != j % kLanes) continue;
             const uint64_t to = offset_of(row, static_cast<uint32_t>(choices)) + j;
             weights[to] = w[j] / sum;
-            chosen[to] = best[j] != 0 ? at[j] : -1;
+            chosen[to] = best[j] > kNone ? at[j] : -1;
         }
     }
 }
@@ -210,8 +238,12 @@ int with_row_layout(int experts, int choices, F&& f) {
     if (chunks <= 4) return with_most(std::integral_constant<int, 4>{}, one);
     if (chunks <= 8) return with_most(std::integral_constant<int, 8>{}, one);
     if (chunks <= 16) return with_most(std::integral_constant<int, 16>{}, one);
-    if (chunks <= 32) return with_most(std::integral_constant<int, 32>{}, one);
-    if (chunks <= 64) return with_most(std::integral_constant<int, 64>{}, one);
+    if (chunks <= 24) return with_most(std::integral_constant<int, 8>{}, std::integral_constant<int, 3>{});
+    // (more lanes exchange what they have through the LDS: 200000 x 512 bf16, 8 choices, 187 us, with 64 of them 287; of 50000 x 1000, which would not fit the registers, 113 and 187)
+    constexpr std::integral_constant<int, 16> sixteen{};
+    if (chunks <= 32) return with_most(sixteen, std::integral_constant<int, 2>{});
+    if (chunks <= 48) return with_most(sixteen, std::integral_constant<int, 3>{});
+    if (chunks <= 64) return with_most(sixteen, std::integral_constant<int, 4>{});
     return with_most(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
 }
 

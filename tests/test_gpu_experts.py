@@ -36,7 +36,7 @@ def assert_within(got, want, bound, what):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("normalise", [True, False])
-@pytest.mark.parametrize("rows,number,choices", [(1, 1, 1), (5, 2, 2), (1000, 7, 2), (257, 8, 8), (4097, 9, 3), (300, 16, 1), (300, 33, 5), (1000, 64, 2), (70, 100, 4),
+@pytest.mark.parametrize("rows,number,choices", [(1, 1, 1), (5, 2, 2), (1000, 7, 2), (257, 8, 8), (4097, 9, 3), (300, 16, 1), (300, 33, 5), (1000, 64, 2), (70, 100, 4), (129, 150, 3), (50, 200, 8), (61, 300, 4), (45, 390, 2),
                                                  (65, 256, 8), (33, 257, 2), (17, 512, 6), (9, 513, 2), (19, 1000, 8), (3, 1024, 4)])
 def test_route(dtype, normalise, rows, number, choices):
     logits = random((rows, number + 3), 1, TYPES[dtype])[:, :number]
