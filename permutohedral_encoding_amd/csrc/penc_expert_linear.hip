@@ -688,8 +688,8 @@ struct WeightPlan {
     double time;
 };
 // Workgroups go in rounds of as many as have room at a time.  Beside its rows a workgroup takes as long as for two steps, and where its sums go through memory, as long again as kCut
-// rows.  Either an expert's rows are one piece (up to twice as many as experts have on average, and a quarter of the time for experts that are not alike), or they are cut for one to four whole
-// rounds.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and 6 for the sums, now 28 and 5;
+// rows.  Either an expert's rows are one piece (up to twice as many as experts have on average, or 3/4 of all that a workgroup has if that is more: 32768 x 1024 by 4096 bf16, 16 experts in uneven demand,
+// y and dW, 614 us and then 591; and a quarter of the time for experts that are not alike), or they are cut for one to four whole rounds.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and 6 for the sums, now 28 and 5;
 // 2^20 x 64 by 64 fp32, all of the layer, with 2, 4, 6 and 8 to a compute unit 347, 325, 305 and 316 us, with 3 299.  16384 x 1024 by 2048 bf16, 4 experts, y and dW: cut for three rounds
 // 216 us, in one piece 165.)
 WeightPlan weight_plan_of(int side, int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
@@ -698,7 +698,7 @@ WeightPlan weight_plan_of(int side, int64_t rows, int64_t experts, int64_t chann
     p.side = side;
     p.tiles = ((channels + side - 1) / side) * ((outputs + side - 1) / side);
     const int64_t room = (side == 256 ? 1 : side == 128 ? 2 : 3) * kUnits, own = (rows + experts - 1) / experts;
-    p.most = 2 * own;
+    p.most = std::max(2 * own, rows / 4 * 3 * p.tiles / room);
     p.time = static_cast<double>((experts * p.tiles + room - 1) / room) * 1.25 * (static_cast<double>(own) + kBeside);
     for (int64_t rounds = 1; rounds <= 4; ++rounds) {
         const int64_t pieces = rounds * room / p.tiles - experts;
