@@ -7,7 +7,7 @@
 //     dispatch   s[p(i)] = x[i / k], zeros for a choice without an expert;    dx[t] = sum of ds[p] over t's choices
 //     combine    o[t] = sum of w y[p] over t's choices;                      dy[p] = w do[t],  dw = <do[t], y[p]>
 //
-// All of it is bound by memory.  Results, and the logits, go past the caches (nontemporal): a pass over rows of 256 MiB that leaves what it wrote in them has the next pass wait until that
+// All but some of route is bound by memory.  Results, and the logits, go past the caches (nontemporal), but for short rows that go to places of their own (with_past): a pass over rows of 256 MiB that leaves what it wrote in them has the next pass wait until that
 // is in memory.  Route and its gradient of 2^20 x 64 fp32: 160 us without, 115 so; rows of 2^20 x 64 fp32 there and back, two choices, with gradients 729 and 698, of 16381 x 2048 bf16
 // 195 and 181.  With rows that the caches hold (a decoder of 2^11 to 2^17 points, its passes one after the other) the two are within 1%.
 #include <hip/hip_runtime.h>
@@ -425,7 +425,12 @@ struct Piece {
     using Floats = float __attribute__((ext_vector_type(kWide)));
 
     __device__ __forceinline__ static Vector load(const E* p) { return *reinterpret_cast<const Unaligned*>(p); }
-    __device__ __forceinline__ static void store(E* p, Vector v) { __builtin_nontemporal_store(v, reinterpret_cast<Unaligned*>(p)); }
+    // (the two in one function, chosen by a flag, would become one store)
+    template <bool kPast>
+    __device__ __forceinline__ static void store(E* p, Vector v) {
+        if constexpr (kPast) __builtin_nontemporal_store(v, reinterpret_cast<Unaligned*>(p));
+        else *reinterpret_cast<Unaligned*>(p) = v;
+    }
     __device__ __forceinline__ static Floats floats(Vector v) { return __builtin_convertvector(v, Floats); }
     __device__ __forceinline__ static Vector rounded(Floats v) { return __builtin_convertvector(v, Vector); }
 };
@@ -437,6 +442,7 @@ struct Single {
     using Floats = float __attribute__((ext_vector_type(1)));
 
     __device__ __forceinline__ static Vector load(const E* p) { return Vector{*p}; }
+    template <bool kPast>
     __device__ __forceinline__ static void store(E* p, Vector v) { *p = v[0]; }
     __device__ __forceinline__ static Floats floats(Vector v) { return Floats{static_cast<float>(v[0])}; }
     __device__ __forceinline__ static Vector rounded(Floats v) { return Vector{static_cast<E>(v[0])}; }
@@ -453,7 +459,7 @@ struct Group {
 };
 
 // Each row is read once and written to the places of its choices.
-template <class P, class E>
+template <class P, class E, bool kPast>
 __global__ __launch_bounds__(kThreads) void dispatch_kernel(RowPlan plan, int log2_lanes, const E* __restrict__ x, uint32_t stride, E* __restrict__ sorted) {
     const Group g(log2_lanes);
     const uint32_t most = plan.most();
@@ -464,7 +470,7 @@ __global__ __launch_bounds__(kThreads) void dispatch_kernel(RowPlan plan, int lo
             const typename P::Vector v = P::load(from + at);
             for (int j = 0; j < plan.choices; ++j) {
                 const uint32_t to = plan.position(row, j);
-                if (to < plan.items) P::store(sorted + offset_of(to, plan.channels) + at, to < most ? v : typename P::Vector{});
+                if (to < plan.items) P::template store<kPast>(sorted + offset_of(to, plan.channels) + at, to < most ? v : typename P::Vector{});
             }
         }
     }
@@ -503,13 +509,13 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(RowPlan plan, int log2
                 for (int j = 0; j < kMost; ++j)
                     if (from[j] != nullptr) sum += P::floats(v[j]) * w[j];
             }
-            P::store(out + offset_of(row, plan.channels) + at, P::rounded(sum));
+            P::template store<true>(out + offset_of(row, plan.channels) + at, P::rounded(sum));
         }
     }
 }
 
 // dy[p] = w do[t] (zeros behind the last choice that has an expert), dw = <do[t], y[p]>: each row of do is read once for kMost choices.
-template <class P, class E, class W, int kMost>
+template <class P, class E, class W, int kMost, bool kPast>
 __global__ __launch_bounds__(kThreads) void combine_backward_kernel(RowPlan plan, int log2_lanes, const E* __restrict__ grad, uint32_t grad_stride,
                                                                     const E* __restrict__ y, uint32_t stride, const W* __restrict__ weights,
                                                                     E* __restrict__ dy, W* __restrict__ dweights) {
@@ -538,7 +544,7 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(RowPlan plan
     #pragma unroll
                 for (int j = 0; j < kMost; ++j) {
                     if (dy != nullptr && position[j] < plan.items)
-                        P::store(dy + offset_of(position[j], plan.channels) + at, position[j] < most ? P::rounded(d * w[j]) : typename P::Vector{});
+                        P::template store<kPast>(dy + offset_of(position[j], plan.channels) + at, position[j] < most ? P::rounded(d * w[j]) : typename P::Vector{});
                     if (dweights != nullptr && position[j] < most) {
                         const typename P::Floats f = P::floats(v[j]);
     #pragma unroll
@@ -571,6 +577,14 @@ int with_pieces(int64_t channels, int most, F&& f) {
     };
     if (channels >= kWide) return f(Piece<E>{}, log2_lanes((channels + kWide - 1) / kWide));
     return f(Single<E>{}, log2_lanes(channels));
+}
+
+// Rows that go to places of their own go past the caches where they are whole lines, or long; the ends of short ones would be read back from memory (2^20 x 48 bf16 to two places each:
+// 61 us, past them 102; 64 channels 77 and 62; 50000 x 1000 fp16 53 and 50).
+template <class F>
+int with_past(const void* to, size_t row_bytes, F&& f) {
+    if (aligned_to(to, 64) && (row_bytes % 64 == 0 || row_bytes >= 1024)) return f(std::true_type{});
+    return f(std::false_type{});
 }
 
 template <class F>
@@ -684,9 +698,11 @@ int penc_dispatch(int type, int64_t rows, int choices, int64_t channels, const v
         using E = decltype(e);
         if (!aligned_to(x, sizeof(E)) || !aligned_to(sorted, sizeof(E)) || !aligned_to(positions, 4) || !aligned_to(routed, 4)) return PENC_ERR_MISALIGNED;
         return with_pieces<E>(channels, kLog2Threads, [&](auto piece, int log2_lanes) -> int {
-            dispatch_kernel<decltype(piece)><<<grid_of(rows, kThreads >> log2_lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-                row_plan(rows, choices, channels, positions, routed), log2_lanes, static_cast<const E*>(x), static_cast<uint32_t>(row_stride), static_cast<E*>(sorted));
-            return launched();
+            return with_past(sorted, channels * sizeof(E), [&](auto past) -> int {
+                dispatch_kernel<decltype(piece), E, decltype(past)::value><<<grid_of(rows, kThreads >> log2_lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+                    row_plan(rows, choices, channels, positions, routed), log2_lanes, static_cast<const E*>(x), static_cast<uint32_t>(row_stride), static_cast<E*>(sorted));
+                return launched();
+            });
         });
     };
     return type == PENC_FP32 ? copy(uint32_t{}) : copy(uint16_t{});
@@ -734,11 +750,13 @@ int penc_combine_backward(int type, int weight_type, int64_t rows, int choices, 
             return with_most(choices, [&](auto most) -> int {
                 const auto launch = [&](auto w) -> int {
                     using W = decltype(w);
-                    combine_backward_kernel<decltype(piece), E, W, decltype(most)::value>
-                        <<<grid_of(rows, kThreads >> log2_lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-                            row_plan(rows, choices, channels, positions, routed), log2_lanes, static_cast<const E*>(grad), static_cast<uint32_t>(grad_row_stride),
-                            static_cast<const E*>(y), static_cast<uint32_t>(row_stride), static_cast<const W*>(weights), static_cast<E*>(dy), static_cast<W*>(dweights));
-                    return launched();
+                    return with_past(dy, channels * sizeof(E), [&](auto past) -> int {
+                        combine_backward_kernel<decltype(piece), E, W, decltype(most)::value, decltype(past)::value>
+                            <<<grid_of(rows, kThreads >> log2_lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+                                row_plan(rows, choices, channels, positions, routed), log2_lanes, static_cast<const E*>(grad), static_cast<uint32_t>(grad_row_stride),
+                                static_cast<const E*>(y), static_cast<uint32_t>(row_stride), static_cast<const W*>(weights), static_cast<E*>(dy), static_cast<W*>(dweights));
+                        return launched();
+                    });
                 };
                 return weight_type == PENC_FP32 ? launch(float{}) : launch(e);
             });
