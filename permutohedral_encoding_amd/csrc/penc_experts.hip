@@ -415,11 +415,11 @@ struct RowPlan {
     __device__ __forceinline__ uint32_t most() const { return min(static_cast<uint32_t>(max(*routed, 0)), items); }
 };
 
-// A lane's kWide channels of a row: 16 bytes, wherever they are.  The last lane of a row that has no whole number of those takes some that its neighbour has too;
-// rows of fewer channels go one by one.
-template <class E>
+// A lane's kWide channels of a row, 16 bytes or what a shorter row has of 8 and 4, wherever they are.  The last lane of a row that has no whole number of those takes some that its
+// neighbour has too.  (2^20 x 7 bf16 there and back with gradients, two choices: 136 us channel by channel, 67 so.)
+template <class E, int kWide_ = 16 / sizeof(E)>
 struct Piece {
-    static constexpr int kWide = 16 / sizeof(E);
+    static constexpr int kWide = kWide_;
     using Vector = E __attribute__((ext_vector_type(kWide)));
     using Unaligned = E __attribute__((ext_vector_type(kWide), aligned(sizeof(E))));
     using Floats = float __attribute__((ext_vector_type(kWide)));
@@ -576,7 +576,11 @@ int with_pieces(int64_t channels, int most, F&& f) {
         return n;
     };
     if (channels >= kWide) return f(Piece<E>{}, log2_lanes((channels + kWide - 1) / kWide));
-    return f(Single<E>{}, log2_lanes(channels));
+    if constexpr (kWide == 8) {
+        if (channels >= 4) return f(Piece<E, 4>{}, log2_lanes((channels + 3) / 4));
+    }
+    if (channels >= 2) return f(Piece<E, 2>{}, log2_lanes((channels + 1) / 2));
+    return f(Single<E>{}, 0);
 }
 
 // Rows that go to places of their own go past the caches where they are whole lines, or long; the ends of short ones would be read back from memory (2^20 x 48 bf16 to two places each:
