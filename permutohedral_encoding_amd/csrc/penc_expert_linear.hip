@@ -714,6 +714,8 @@ WeightPlan weight_plan_of(int side, int64_t rows, int64_t experts, int64_t chann
 WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
     if (channels <= 64 || outputs <= 64) return weight_plan_of(64, rows, experts, channels, outputs);
     const WeightPlan p = weight_plan_of(128, rows, experts, channels, outputs);
+    // (half of the compute units without a workgroup: 1000 x 512 by 512 fp32, 3 experts, y and dW, 47 us, 30 so; 4000 x 512 by 512 bf16, 4 experts, 28 and 26)
+    if (std::max(experts, rows / p.most) * p.tiles < static_cast<int64_t>(kUnits / 2)) return weight_plan_of(64, rows, experts, channels, outputs);
     if (kSize != 2 || channels % 8 != 0 || outputs % 8 != 0 || channels < 256 || outputs < 256) return p;
     // Two tiles of 128 have half of the work of one of 256 a row, which they do in 0.6 of its time (32768 x 1024 by 4096 bf16, 16 experts, all of the layer: 256 897 us, 128 940).
     const WeightPlan large = weight_plan_of(256, rows, experts, channels, outputs);
