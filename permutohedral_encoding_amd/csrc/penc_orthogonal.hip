@@ -5,9 +5,10 @@
 // takes every singular value s in 0 .. 1 through as many times a s + b s^3 + c s^5.  What is small in X is taken up by a factor a in each step, and so is what a rounding has
 // added to it.  In 16 bits with 8 of them behind the point (bfloat16) the result would be off by 1e-2 of it, in float16 by 1.4e-3.  So X, S and F are kept
 //
-//     for bfloat16 results     as float16, one product for each, and F's diagonal, which is most of F, in float32: with the result's own rounding (1.66e-3) 1.8e-3 to 2.0e-3
-//                              (with the diagonal in float16 2.0e-3 to 2.4e-3)
-//     for float16 and float32  as two float16 values, hi + lo, three products for each: 0.7e-6 to 1.5e-6 of float32 results, which float32 products leave 0.9e-6 to 1.7e-6 off
+//     as two float16 values, hi + lo, three products for each: 0.7e-6 to 1.5e-6 of float32 results, which float32 products leave 0.9e-6 to 3.4e-6 off.  16-bit results are off by their own
+//         rounding and no more, 1.66e-3 in bfloat16
+//     for bfloat16 results, where the caller asks for it (`halves`), as float16, one product for each, and F's diagonal, which is most of F, in float32: 1.8e-3 to 2.0e-3
+//         (with the diagonal in float16 2.0e-3 to 2.4e-3) in a third of the time: 16 x 4096 x 1024 1517 us, as two values 4796
 //
 // times 2^12: with |X| <= 1.2, S <= 1.5 and F <= 3 they stay under 2^14 (a bound on the coefficients sees to that), and what matters of lo is no subnormal number.
 // The matrix cores run float16 8 times as fast as float32, so that three products take 3/8 of the time.
@@ -963,8 +964,9 @@ int launch_step(StepArgs a, int64_t matrices, hipStream_t stream) {
     return launch(std::common_type<Product<E, kAlongM, kAlongN, 128, 128, 2, 2, Chunks::kDirect>>{});
 }
 
+// Matrices of any size.
 template <class E, class G>
-int orthogonalise(int64_t matrices, int64_t rows, int64_t columns, int steps, Coefficients k, const G* g, G* result, char* workspace, hipStream_t stream) {
+int large(int64_t matrices, int64_t rows, int64_t columns, int steps, Coefficients k, const G* g, G* result, char* workspace, hipStream_t stream) {
     const Layout l = layout_of<E>(matrices, rows, columns);
     char *x = workspace, *next = x + l.x, *const s = next + l.x, *const f = s + l.s;
     float* const partial = reinterpret_cast<float*>(f + l.s);
@@ -1033,6 +1035,43 @@ bool bad_matrices(int64_t matrices, int64_t rows, int64_t columns) {
     return matrices < 0 || matrices > PENC_MAX_MATRICES || rows < 1 || rows > PENC_MAX_MATRIX_SIDE || columns < 1 || columns > PENC_MAX_MATRIX_SIDE;
 }
 
+// Whether the products are of float16 once.
+bool in_halves(const penc_orthogonal& o) { return o.type == PENC_BF16 && o.halves != 0; }
+
+size_t workspace_bytes(const penc_orthogonal& o) {
+    if (bad_matrices(o.matrices, o.rows, o.columns) || o.matrices == 0) return 0;
+    const size_t of_thin = is_thin(o.matrices, o.rows, o.columns) ? thin_workspace(o.matrices, o.rows, o.columns) : 0;
+    if (is_resident(o.rows, o.columns)) return of_thin;
+    // (thin matrices too, for steps that are not theirs)
+    return std::max(of_thin, in_halves(o) ? layout_of<half_t>(o.matrices, o.rows, o.columns).total : layout_of<split_t>(o.matrices, o.rows, o.columns).total);
+}
+
+int run(const penc_orthogonal& o, const void* update, void* result, void* workspace, size_t bytes, void* stream) {
+    return with_type(o.type, [&](auto e) -> int {
+        using G = decltype(e);
+        if (bad_matrices(o.matrices, o.rows, o.columns) || o.steps < 1 || o.steps > PENC_MAX_ORTHOGONAL_STEPS) return PENC_ERR_BAD_LAYER_SIZE;
+        double growth;
+        if (!(o.eps >= 1e-30f) || std::isinf(o.eps) || !bounded(o.a, o.b, o.c, o.steps, growth)) return PENC_ERR_UNSUPPORTED_KIND;
+        if (o.matrices == 0) return PENC_OK;
+        if (!update || !result) return PENC_ERR_NULL_POINTER;
+        if (!aligned_to(update, sizeof(G)) || !aligned_to(result, 4 * sizeof(G)) || !aligned_to(workspace, 256)) return PENC_ERR_MISALIGNED;
+        const size_t need = workspace_bytes(o);
+        if (bytes < need) return PENC_ERR_WORKSPACE_TOO_SMALL;
+        if (need > 0 && !workspace) return PENC_ERR_NULL_POINTER;
+        const Coefficients k{o.a, o.b, o.c, o.eps};
+        const hipStream_t s = static_cast<hipStream_t>(stream);
+        const G* const from = static_cast<const G*>(update);
+        G* const to = static_cast<G*>(result);
+        char* const room = static_cast<char*>(workspace);
+        if (is_thin(o.matrices, o.rows, o.columns) && growth <= kMostThinGrowth) return thin<G>(o.matrices, o.rows, o.columns, o.steps, k, from, to, room, s);
+        if (is_resident(o.rows, o.columns)) return resident<G>(o.matrices, o.rows, o.columns, o.steps, k, from, to, s);
+        if constexpr (std::is_same_v<G, bf16_t>) {
+            if (in_halves(o)) return large<half_t, G>(o.matrices, o.rows, o.columns, o.steps, k, from, to, room, s);
+        }
+        return large<split_t, G>(o.matrices, o.rows, o.columns, o.steps, k, from, to, room, s);
+    });
+}
+
 }  // namespace
 }  // namespace penc
 
@@ -1040,36 +1079,20 @@ using namespace penc;
 
 extern "C" {
 
+size_t penc_orthogonal_workspace_bytes(const penc_orthogonal* orthogonal) { return orthogonal ? workspace_bytes(*orthogonal) : 0; }
+
+int penc_orthogonal_matrices(const penc_orthogonal* orthogonal, const void* update, void* result, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!orthogonal) return PENC_ERR_NULL_POINTER;
+    return run(*orthogonal, update, result, workspace, workspace_bytes, stream);
+}
+
 size_t penc_orthogonalise_workspace_bytes(int type, int64_t matrices, int64_t rows, int64_t columns) {
-    if (bad_matrices(matrices, rows, columns) || matrices == 0) return 0;
-    const size_t of_thin = is_thin(matrices, rows, columns) ? thin_workspace(matrices, rows, columns) : 0;
-    if (is_resident(rows, columns)) return of_thin;
-    // (thin matrices too, for steps that are not theirs)
-    return std::max(of_thin, type == PENC_BF16 ? layout_of<half_t>(matrices, rows, columns).total : layout_of<split_t>(matrices, rows, columns).total);
+    return workspace_bytes({type, 1, matrices, rows, columns, 1, 0.0f, 0.0f, 0.0f, 0.0f});
 }
 
 int penc_orthogonalise(int type, int64_t matrices, int64_t rows, int64_t columns, int steps, float a, float b, float c, float eps, const void* update, void* result,
                        void* workspace, size_t workspace_bytes, void* stream) {
-    return with_type(type, [&](auto e) -> int {
-        using G = decltype(e);
-        if (bad_matrices(matrices, rows, columns) || steps < 1 || steps > PENC_MAX_ORTHOGONAL_STEPS) return PENC_ERR_BAD_LAYER_SIZE;
-        double growth;
-        if (!(eps >= 1e-30f) || std::isinf(eps) || !bounded(a, b, c, steps, growth)) return PENC_ERR_UNSUPPORTED_KIND;
-        if (matrices == 0) return PENC_OK;
-        if (!update || !result) return PENC_ERR_NULL_POINTER;
-        if (!aligned_to(update, sizeof(G)) || !aligned_to(result, 4 * sizeof(G)) || !aligned_to(workspace, 256)) return PENC_ERR_MISALIGNED;
-        const size_t need = penc_orthogonalise_workspace_bytes(type, matrices, rows, columns);
-        if (workspace_bytes < need) return PENC_ERR_WORKSPACE_TOO_SMALL;
-        if (need > 0 && !workspace) return PENC_ERR_NULL_POINTER;
-        const Coefficients k{a, b, c, eps};
-        const hipStream_t s = static_cast<hipStream_t>(stream);
-        const G* const from = static_cast<const G*>(update);
-        G* const to = static_cast<G*>(result);
-        if (is_thin(matrices, rows, columns) && growth <= kMostThinGrowth) return thin<G>(matrices, rows, columns, steps, k, from, to, static_cast<char*>(workspace), s);
-        if (is_resident(rows, columns)) return resident<G>(matrices, rows, columns, steps, k, from, to, s);
-        using E = std::conditional_t<std::is_same_v<G, bf16_t>, half_t, split_t>;
-        return orthogonalise<E, G>(matrices, rows, columns, steps, k, from, to, static_cast<char*>(workspace), s);
-    });
+    return run({type, 1, matrices, rows, columns, steps, a, b, c, eps}, update, result, workspace, workspace_bytes, stream);
 }
 
 int penc_muon_momentum(int type, int64_t n, const void* grad, float* average, float momentum, int nesterov, void* update, void* stream) {

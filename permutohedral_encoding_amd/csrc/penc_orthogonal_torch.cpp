@@ -10,8 +10,8 @@ using namespace penc_torch;
 struct Api {
 #define PENC_FN(name) decltype(&penc_##name) name = nullptr
     PENC_FN(status_string);
-    PENC_FN(orthogonalise_workspace_bytes);
-    PENC_FN(orthogonalise);
+    PENC_FN(orthogonal_workspace_bytes);
+    PENC_FN(orthogonal_matrices);
     PENC_FN(muon_momentum);
     PENC_FN(muon_apply);
 #undef PENC_FN
@@ -24,6 +24,7 @@ void check(int status, const char* what) {
 struct Options {
     int64_t steps;
     double a, b, c, eps;
+    int halves;
 };
 
 void require_matrices(const Tensor& t, const char* name) {
@@ -40,13 +41,12 @@ void require_options(const Options& o) {
 
 // The matrices of `update` (dense) into `result` (dense).
 void orthogonalise(const Tensor& update, const Tensor& result, const Options& o) {
-    const int type = type_of(update.scalar_type(), "update");
-    const int64_t rows = update.size(-2), columns = update.size(-1), matrices = update.numel() / (rows * columns);
-    const size_t n = api.orthogonalise_workspace_bytes(type, matrices, rows, columns);
+    const int64_t rows = update.size(-2), columns = update.size(-1);
+    const penc_orthogonal matrices{type_of(update.scalar_type(), "update"), o.halves, update.numel() / (rows * columns), rows, columns, static_cast<int>(o.steps),
+                                   static_cast<float>(o.a), static_cast<float>(o.b), static_cast<float>(o.c), static_cast<float>(o.eps)};
+    const size_t n = api.orthogonal_workspace_bytes(&matrices);
     const Tensor ws = at::empty({static_cast<int64_t>(n)}, update.options().dtype(at::kByte));
-    const int status = api.orthogonalise(type, matrices, rows, columns, static_cast<int>(o.steps), static_cast<float>(o.a), static_cast<float>(o.b),
-                                         static_cast<float>(o.c), static_cast<float>(o.eps), update.const_data_ptr(), result.data_ptr(), ws.data_ptr(), n,
-                                         current_stream(update.device()));
+    const int status = api.orthogonal_matrices(&matrices, update.const_data_ptr(), result.data_ptr(), ws.data_ptr(), n, current_stream(update.device()));
     PENC_REQUIRE(status != PENC_ERR_UNSUPPORTED_KIND, "coefficients should keep singular values under 3 and the factor under 15, however they are ", o.a, ", ", o.b, ", ", o.c);
     check(status, "orthogonalise");
 }
@@ -55,14 +55,15 @@ Options options_of(PyObject* const* args) {
     Options o;
     o.steps = PyLong_AsLongLong(args[0]);
     o.a = PyFloat_AsDouble(args[1]), o.b = PyFloat_AsDouble(args[2]), o.c = PyFloat_AsDouble(args[3]), o.eps = PyFloat_AsDouble(args[4]);
+    o.halves = PyObject_IsTrue(args[5]);
     return o;
 }
 
-// orthogonalise(update, steps, a, b, c, eps)
+// orthogonalise(update, steps, a, b, c, eps, halves)
 PyObject* py_orthogonalise(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
-        TORCH_CHECK(n_args == 6, "orthogonalise takes 6 arguments");
-        TORCH_CHECK(api.orthogonalise != nullptr, "bind() has not been called");
+        TORCH_CHECK(n_args == 7, "orthogonalise takes 7 arguments");
+        TORCH_CHECK(api.orthogonal_matrices != nullptr, "bind() has not been called");
         const Tensor& update = tensor_arg(args[0], "update");
         const Options o = options_of(args + 1);
         if (PyErr_Occurred()) return nullptr;
@@ -122,19 +123,19 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
     }
 }
 
-// muon_step(params, grads, averages, steps, a, b, c, eps, momentum, nesterov, decay, rate): lists of dense tensors of one size, type and device
+// muon_step(params, grads, averages, steps, a, b, c, eps, halves, momentum, nesterov, decay, rate): lists of dense tensors of one size, type and device
 PyObject* py_muon_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
-        TORCH_CHECK(n_args == 12, "muon_step takes 12 arguments");
-        TORCH_CHECK(api.orthogonalise != nullptr, "bind() has not been called");
+        TORCH_CHECK(n_args == 13, "muon_step takes 13 arguments");
+        TORCH_CHECK(api.orthogonal_matrices != nullptr, "bind() has not been called");
         std::vector<Tensor> lists[3];
         for (int k = 0; k < 3; ++k) {
             TORCH_CHECK(PyList_Check(args[k]) && PyList_Size(args[k]) == PyList_Size(args[0]), "muon_step takes three lists of one length");
             for (Py_ssize_t i = 0; i < PyList_Size(args[k]); ++i) lists[k].push_back(tensor_arg(PyList_GetItem(args[k], i), "a parameter, gradient or average"));
         }
         const Options o = options_of(args + 3);
-        const double momentum = PyFloat_AsDouble(args[8]), decay = PyFloat_AsDouble(args[10]), rate = PyFloat_AsDouble(args[11]);
-        const int nesterov = PyObject_IsTrue(args[9]);
+        const double momentum = PyFloat_AsDouble(args[9]), decay = PyFloat_AsDouble(args[11]), rate = PyFloat_AsDouble(args[12]);
+        const int nesterov = PyObject_IsTrue(args[10]);
         if (PyErr_Occurred()) return nullptr;
         const auto& [params, grads, averages] = lists;
         if (params.empty()) Py_RETURN_NONE;
@@ -158,10 +159,10 @@ void bind_orthogonal(void* library) {
     api.fn = reinterpret_cast<decltype(api.fn)>(dlsym(library, "penc_" #fn)); \
     TORCH_CHECK(api.fn != nullptr, "the library does not export penc_" #fn)
     PENC_FN(status_string);
-    PENC_FN(orthogonalise_workspace_bytes);
+    PENC_FN(orthogonal_workspace_bytes);
     PENC_FN(muon_momentum);
     PENC_FN(muon_apply);
-    PENC_FN(orthogonalise);
+    PENC_FN(orthogonal_matrices);
 #undef PENC_FN
 }
 

@@ -1,0 +1,68 @@
+"""Orthogonalised updates on the GPU: what results of few bits are off by, and the way of half as many bits.
+
+A result of 16 bits should be its value rounded once: off by half a step at the value's own magnitude, and by what the steps leave before that.  Those are measured as in
+test_gpu_orthogonal.py, by the same steps in float32: eight times their error, and 144 roundings of float32.  A single value is off by at most 16 times the mean of that."""
+import math
+
+import pytest
+import torch
+
+import expert_reference as ref
+from permutohedral_encoding_amd import optim
+from test_gpu_orthogonal import TYPES, norms, updates
+
+pytestmark = pytest.mark.gpu
+
+
+def step_of(values, dtype):
+    """The distance of neighbouring numbers of a type, at each value's magnitude."""
+    info = torch.finfo(dtype)
+    exponent = torch.frexp(values.abs().clamp(min=info.smallest_normal)).exponent - 1
+    return torch.ldexp(torch.full_like(values, info.eps), exponent)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("matrices,rows,columns", [(1, 130, 130), (1, 203, 1000), (1, 1000, 203), (2, 257, 513), (1, 2100, 161), (3, 300, 700), (8, 512, 512), (33, 531, 390), (2, 2048, 1024), (16, 64, 256),
+                                                   (2, 48, 1000)])
+def test_results_of_16_bits_are_rounded_once(dtype, matrices, rows, columns):
+    dtype = TYPES[dtype]
+    update = updates(matrices, rows, columns, dtype)
+    for given in (dict(), dict(steps=2), dict(coefficients=(1.875, -1.25, 0.375), steps=4)):
+        want = ref.orthogonalise(update, **given)
+        allowed = 8 * norms(ref.orthogonalise(update, dtype=torch.float32, **given).double() - want) + 144 * ref.U * norms(want)
+        behind = ((optim.orthogonalise(update, **given).double() - want).abs() - step_of(want, dtype) / 2).clamp(min=0.0)
+        worst = 16 * allowed / math.sqrt(rows * columns)
+        assert bool((behind.amax((-1, -2)) <= worst).all()), f"{given}: worst error behind half a step/bound {float((behind.amax((-1, -2)) / worst).max()):.3g}"
+
+
+@pytest.mark.parametrize("matrices,rows,columns", [(1, 130, 130), (1, 203, 1000), (1, 1000, 203), (40, 520, 530), (16, 64, 256), (1, 2100, 161), (1, 20, 3000)])
+def test_halves(matrices, rows, columns):
+    """X, S and the factor in float16, as the definition does with them; other types take no notice."""
+    update = updates(matrices, rows, columns, torch.bfloat16)
+    want = ref.orthogonalise(update)
+    got = optim.orthogonalise(update, halves=True)
+    allowed = 4 * norms(ref.orthogonalise(update, stored=ref.in_float16) - want) + norms(ref.half_step(want, torch.bfloat16))
+    assert got.dtype == torch.bfloat16 and bool((norms(got.double() - want) <= allowed).all())
+    assert torch.equal(optim.orthogonalise(update, halves=True), got)
+    for dtype in (torch.float32, torch.float16):
+        assert torch.equal(optim.orthogonalise(update.to(dtype), halves=True), optim.orthogonalise(update.to(dtype)))
+
+
+def test_muon_in_halves():
+    start = updates(2, 160, 200, torch.bfloat16, seed=1, scale=0.1)
+    grad = updates(2, 160, 200, torch.bfloat16, seed=2)
+    for halves in (False, True):
+        p = torch.nn.Parameter(start.clone())
+        opt = optim.Muon([p], lr=0.02, momentum=0.0, nesterov=False, weight_decay=0.0, halves=halves)
+        p.grad = grad.clone()
+        opt.step()
+        # (the average of one step without momentum is the gradient itself)
+        assert torch.equal(p.detach(), (start.float() - torch.tensor(0.02 * math.sqrt(1.0)).cuda() * optim.orthogonalise(grad, halves=halves).float()).bfloat16())
+    # state that was saved without it
+    saved = opt.state_dict()
+    for group in saved["param_groups"]:
+        del group["halves"]
+    again = optim.Muon([p], lr=0.02)
+    again.load_state_dict(saved)
+    again.step()
+    assert again.param_groups[0]["halves"] is False
