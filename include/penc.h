@@ -556,7 +556,7 @@ typedef struct penc_orthogonal {
     int steps;
     float a, b, c, eps;
 } penc_orthogonal;
-size_t penc_orthogonal_workspace_bytes(const penc_orthogonal* orthogonal);
+size_t penc_orthogonal_workspace_bytes(const penc_orthogonal* orthogonal); /* 0 for what is refused */
 int penc_orthogonal_matrices(const penc_orthogonal* orthogonal, const void* update, void* result, void* workspace, size_t workspace_bytes, void* stream);
 /* The same with `halves`; the workspace is enough for any steps and coefficients. */
 size_t penc_orthogonalise_workspace_bytes(int type, int64_t matrices, int64_t rows, int64_t columns);

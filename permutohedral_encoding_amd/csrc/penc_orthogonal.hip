@@ -1038,12 +1038,30 @@ bool bad_matrices(int64_t matrices, int64_t rows, int64_t columns) {
 // Whether the products are of float16 once.
 bool in_halves(const penc_orthogonal& o) { return o.type == PENC_BF16 && o.halves != 0; }
 
+bool bad_options(const penc_orthogonal& o) { return o.steps < 1 || o.steps > PENC_MAX_ORTHOGONAL_STEPS || !(o.eps >= 1e-30f) || std::isinf(o.eps); }
+
+// Which way matrices go.
+enum Way { kThinWay, kResidentWay, kLargeWay };
+Way way_of(const penc_orthogonal& o, double growth) {
+    if (growth <= kMostThinGrowth && is_thin(o.matrices, o.rows, o.columns)) return kThinWay;
+    return is_resident(o.rows, o.columns) ? kResidentWay : kLargeWay;
+}
+
+// What it takes.  (Thin matrices that are not to go their own way take far more than they have: columns are padded to 32.)
+size_t workspace_bytes(const penc_orthogonal& o, Way way) {
+    if (way == kThinWay) return thin_workspace(o.matrices, o.rows, o.columns);
+    if (way == kResidentWay) return 0;
+    return in_halves(o) ? layout_of<half_t>(o.matrices, o.rows, o.columns).total : layout_of<split_t>(o.matrices, o.rows, o.columns).total;
+}
 size_t workspace_bytes(const penc_orthogonal& o) {
+    double growth;
+    if (bad_matrices(o.matrices, o.rows, o.columns) || o.matrices == 0 || bad_options(o) || !bounded(o.a, o.b, o.c, o.steps, growth)) return 0;
+    return workspace_bytes(o, way_of(o, growth));
+}
+// What matrices take with any steps and coefficients.
+size_t most_workspace_bytes(const penc_orthogonal& o) {
     if (bad_matrices(o.matrices, o.rows, o.columns) || o.matrices == 0) return 0;
-    const size_t of_thin = is_thin(o.matrices, o.rows, o.columns) ? thin_workspace(o.matrices, o.rows, o.columns) : 0;
-    if (is_resident(o.rows, o.columns)) return of_thin;
-    // (thin matrices too, for steps that are not theirs)
-    return std::max(of_thin, in_halves(o) ? layout_of<half_t>(o.matrices, o.rows, o.columns).total : layout_of<split_t>(o.matrices, o.rows, o.columns).total);
+    return std::max(workspace_bytes(o, way_of(o, 1.0)), workspace_bytes(o, way_of(o, INFINITY)));
 }
 
 int run(const penc_orthogonal& o, const void* update, void* result, void* workspace, size_t bytes, void* stream) {
@@ -1051,11 +1069,12 @@ int run(const penc_orthogonal& o, const void* update, void* result, void* worksp
         using G = decltype(e);
         if (bad_matrices(o.matrices, o.rows, o.columns) || o.steps < 1 || o.steps > PENC_MAX_ORTHOGONAL_STEPS) return PENC_ERR_BAD_LAYER_SIZE;
         double growth;
-        if (!(o.eps >= 1e-30f) || std::isinf(o.eps) || !bounded(o.a, o.b, o.c, o.steps, growth)) return PENC_ERR_UNSUPPORTED_KIND;
+        if (bad_options(o) || !bounded(o.a, o.b, o.c, o.steps, growth)) return PENC_ERR_UNSUPPORTED_KIND;
         if (o.matrices == 0) return PENC_OK;
         if (!update || !result) return PENC_ERR_NULL_POINTER;
         if (!aligned_to(update, sizeof(G)) || !aligned_to(result, 4 * sizeof(G)) || !aligned_to(workspace, 256)) return PENC_ERR_MISALIGNED;
-        const size_t need = workspace_bytes(o);
+        const Way way = way_of(o, growth);
+        const size_t need = workspace_bytes(o, way);
         if (bytes < need) return PENC_ERR_WORKSPACE_TOO_SMALL;
         if (need > 0 && !workspace) return PENC_ERR_NULL_POINTER;
         const Coefficients k{o.a, o.b, o.c, o.eps};
@@ -1063,8 +1082,8 @@ int run(const penc_orthogonal& o, const void* update, void* result, void* worksp
         const G* const from = static_cast<const G*>(update);
         G* const to = static_cast<G*>(result);
         char* const room = static_cast<char*>(workspace);
-        if (is_thin(o.matrices, o.rows, o.columns) && growth <= kMostThinGrowth) return thin<G>(o.matrices, o.rows, o.columns, o.steps, k, from, to, room, s);
-        if (is_resident(o.rows, o.columns)) return resident<G>(o.matrices, o.rows, o.columns, o.steps, k, from, to, s);
+        if (way == kThinWay) return thin<G>(o.matrices, o.rows, o.columns, o.steps, k, from, to, room, s);
+        if (way == kResidentWay) return resident<G>(o.matrices, o.rows, o.columns, o.steps, k, from, to, s);
         if constexpr (std::is_same_v<G, bf16_t>) {
             if (in_halves(o)) return large<half_t, G>(o.matrices, o.rows, o.columns, o.steps, k, from, to, room, s);
         }
@@ -1087,7 +1106,7 @@ int penc_orthogonal_matrices(const penc_orthogonal* orthogonal, const void* upda
 }
 
 size_t penc_orthogonalise_workspace_bytes(int type, int64_t matrices, int64_t rows, int64_t columns) {
-    return workspace_bytes({type, 1, matrices, rows, columns, 1, 0.0f, 0.0f, 0.0f, 0.0f});
+    return most_workspace_bytes({type, 1, matrices, rows, columns, 0, 0.0f, 0.0f, 0.0f, 0.0f});
 }
 
 int penc_orthogonalise(int type, int64_t matrices, int64_t rows, int64_t columns, int steps, float a, float b, float c, float eps, const void* update, void* result,

@@ -25,6 +25,7 @@ struct Options {
     int64_t steps;
     double a, b, c, eps;
     int halves;
+    int64_t most_bytes;  // of a workspace, and of the updates of several parameters
 };
 
 void require_matrices(const Tensor& t, const char* name) {
@@ -36,17 +37,34 @@ void require_matrices(const Tensor& t, const char* name) {
 
 void require_options(const Options& o) {
     PENC_REQUIRE(o.steps >= 1 && o.steps <= PENC_MAX_ORTHOGONAL_STEPS, "steps should be 1 to ", PENC_MAX_ORTHOGONAL_STEPS, ", however they are ", o.steps);
+    PENC_REQUIRE(o.most_bytes >= 0, "a workspace should have no negative number of bytes, however it has ", o.most_bytes);
     PENC_REQUIRE(o.eps >= 1e-30 && o.eps < 1e30, "eps should be a positive number, however it is ", o.eps);
 }
 
-// The matrices of `update` (dense) into `result` (dense).
+// The matrices of `update` (dense) into `result` (dense): as many at a time as the workspace has room for, and one, or two or four of them that together are whole fours of values, at least.
 void orthogonalise(const Tensor& update, const Tensor& result, const Options& o) {
-    const int64_t rows = update.size(-2), columns = update.size(-1);
-    const penc_orthogonal matrices{type_of(update.scalar_type(), "update"), o.halves, update.numel() / (rows * columns), rows, columns, static_cast<int>(o.steps),
-                                   static_cast<float>(o.a), static_cast<float>(o.b), static_cast<float>(o.c), static_cast<float>(o.eps)};
-    const size_t n = api.orthogonal_workspace_bytes(&matrices);
-    const Tensor ws = at::empty({static_cast<int64_t>(n)}, update.options().dtype(at::kByte));
-    const int status = api.orthogonal_matrices(&matrices, update.const_data_ptr(), result.data_ptr(), ws.data_ptr(), n, current_stream(update.device()));
+    const int64_t rows = update.size(-2), columns = update.size(-1), values = rows * columns, all = update.numel() / values;
+    const int64_t fours = values % 4 == 0 ? 1 : values % 2 == 0 ? 2 : 4;
+    penc_orthogonal matrices{type_of(update.scalar_type(), "update"), o.halves, all, rows, columns, static_cast<int>(o.steps),
+                             static_cast<float>(o.a), static_cast<float>(o.b), static_cast<float>(o.c), static_cast<float>(o.eps)};
+    while (matrices.matrices > fours && api.orthogonal_workspace_bytes(&matrices) > static_cast<size_t>(o.most_bytes))
+        matrices.matrices = (matrices.matrices / 2 + fours - 1) / fours * fours;
+    const int64_t most = std::max<int64_t>(matrices.matrices, 1), bytes = values * static_cast<int64_t>(update.element_size());
+    for (int64_t first = 0; first < all; first += most) {
+        matrices.matrices = std::min(most, all - first);
+        const size_t n = api.orthogonal_workspace_bytes(&matrices);
+        const Tensor ws = at::empty({static_cast<int64_t>(n)}, update.options().dtype(at::kByte));
+        check(api.orthogonal_matrices(&matrices, static_cast<const char*>(update.const_data_ptr()) + first * bytes, static_cast<char*>(result.data_ptr()) + first * bytes, ws.data_ptr(), n,
+                                      current_stream(update.device())),
+              "orthogonalise");
+    }
+}
+
+// Refuses coefficients and eps before anything is changed.
+void require_accepted(const Options& o) {
+    require_options(o);
+    const penc_orthogonal none{PENC_FP32, 0, 0, 1, 1, static_cast<int>(o.steps), static_cast<float>(o.a), static_cast<float>(o.b), static_cast<float>(o.c), static_cast<float>(o.eps)};
+    const int status = api.orthogonal_matrices(&none, nullptr, nullptr, nullptr, 0, nullptr);
     PENC_REQUIRE(status != PENC_ERR_UNSUPPORTED_KIND, "coefficients should keep singular values under 3 and the factor under 15, however they are ", o.a, ", ", o.b, ", ", o.c);
     check(status, "orthogonalise");
 }
@@ -56,13 +74,14 @@ Options options_of(PyObject* const* args) {
     o.steps = PyLong_AsLongLong(args[0]);
     o.a = PyFloat_AsDouble(args[1]), o.b = PyFloat_AsDouble(args[2]), o.c = PyFloat_AsDouble(args[3]), o.eps = PyFloat_AsDouble(args[4]);
     o.halves = PyObject_IsTrue(args[5]);
+    o.most_bytes = PyLong_AsLongLong(args[6]);
     return o;
 }
 
-// orthogonalise(update, steps, a, b, c, eps, halves)
+// orthogonalise(update, steps, a, b, c, eps, halves, most_bytes)
 PyObject* py_orthogonalise(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
-        TORCH_CHECK(n_args == 7, "orthogonalise takes 7 arguments");
+        TORCH_CHECK(n_args == 8, "orthogonalise takes 8 arguments");
         TORCH_CHECK(api.orthogonal_matrices != nullptr, "bind() has not been called");
         const Tensor& update = tensor_arg(args[0], "update");
         const Options o = options_of(args + 1);
@@ -72,7 +91,7 @@ PyObject* py_orthogonalise(PyObject*, PyObject* const* args, Py_ssize_t n_args) 
             NoGil no_gil;
             require_plain({&update});
             require_matrices(update, "update");
-            require_options(o);
+            require_accepted(o);
             at::NoGradGuard no_grad;
             const c10::DeviceGuard device(update.device());
             const Tensor dense = update.detach().contiguous();
@@ -83,13 +102,11 @@ PyObject* py_orthogonalise(PyObject*, PyObject* const* args, Py_ssize_t n_args) 
     });
 }
 
-constexpr int64_t kValuesAtOnce = int64_t{1} << 28;  // so that updates and workspaces stay within a few GB
-
 void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& averages, const Options& o, double momentum,
                int nesterov, double decay, double rate) {
     const Tensor& first = params[0];
     require_matrices(first, "a parameter");
-    require_options(o);
+    require_accepted(o);
     for (size_t i = 0; i < params.size(); ++i) {
         require_plain({&params[i], &grads[i], &averages[i]});
         TORCH_CHECK(params[i].sizes() == first.sizes() && params[i].scalar_type() == first.scalar_type() && params[i].device() == first.device() &&
@@ -104,8 +121,8 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
     const int type = type_of(first.scalar_type(), "a parameter");
     const int64_t values = first.numel(), stack = values / (first.size(-1) * first.size(-2));
     if (values == 0) return;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kValuesAtOnce / values, PENC_MAX_MATRICES / stack));
-    const size_t size = first.element_size();
+    const int64_t size = static_cast<int64_t>(first.element_size());
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(o.most_bytes / (2 * size * values), PENC_MAX_MATRICES / stack));
     for (int64_t begin = 0; begin < static_cast<int64_t>(params.size()); begin += most) {
         const int64_t count = std::min<int64_t>(most, static_cast<int64_t>(params.size()) - begin);
         const Tensor update = at::empty({count * stack, first.size(-2), first.size(-1)}, first.options()), result = at::empty_like(update);
@@ -123,10 +140,10 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
     }
 }
 
-// muon_step(params, grads, averages, steps, a, b, c, eps, halves, momentum, nesterov, decay, rate): lists of dense tensors of one size, type and device
+// muon_step(params, grads, averages, steps, a, b, c, eps, halves, most_bytes, momentum, nesterov, decay, rate): lists of dense tensors of one size, type and device
 PyObject* py_muon_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
-        TORCH_CHECK(n_args == 13, "muon_step takes 13 arguments");
+        TORCH_CHECK(n_args == 14, "muon_step takes 14 arguments");
         TORCH_CHECK(api.orthogonal_matrices != nullptr, "bind() has not been called");
         std::vector<Tensor> lists[3];
         for (int k = 0; k < 3; ++k) {
@@ -134,8 +151,8 @@ PyObject* py_muon_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
             for (Py_ssize_t i = 0; i < PyList_Size(args[k]); ++i) lists[k].push_back(tensor_arg(PyList_GetItem(args[k], i), "a parameter, gradient or average"));
         }
         const Options o = options_of(args + 3);
-        const double momentum = PyFloat_AsDouble(args[9]), decay = PyFloat_AsDouble(args[11]), rate = PyFloat_AsDouble(args[12]);
-        const int nesterov = PyObject_IsTrue(args[10]);
+        const double momentum = PyFloat_AsDouble(args[10]), decay = PyFloat_AsDouble(args[12]), rate = PyFloat_AsDouble(args[13]);
+        const int nesterov = PyObject_IsTrue(args[11]);
         if (PyErr_Occurred()) return nullptr;
         const auto& [params, grads, averages] = lists;
         if (params.empty()) Py_RETURN_NONE;

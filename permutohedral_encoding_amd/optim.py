@@ -13,6 +13,7 @@ import torch
 
 from . import _native
 
+WORKSPACE_BYTES = 4 << 30  # the most that orthogonalise and Muon take beside their updates (but for matrices that need more on their own), and that Muon takes for updates
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # a s + b s^3 + c s^5 takes small singular values up fastest (K. Jordan et al., "Muon", 2024)
 
 
@@ -24,7 +25,7 @@ def orthogonalise(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, halves=F
     2.0e-3 of the result's norm, where its rounding alone makes 1.66e-3; for others it changes nothing.  Zeros stay zeros, a matrix with an infinity or a NaN becomes NaN.
     Coefficients that make more than 3 of a singular value, or more than 15 of the factor, are refused.  No gradient is recorded."""
     a, b, c = coefficients
-    return _native.bridge().orthogonalise(update, steps, a, b, c, eps, halves)
+    return _native.bridge().orthogonalise(update, steps, a, b, c, eps, halves, WORKSPACE_BYTES)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -188,6 +189,6 @@ class Muon(torch.optim.Optimizer):
                 rows, columns = shape[-2:]
                 scale = 0.2 * math.sqrt(max(rows, columns)) if group["match_rms_adamw"] else math.sqrt(max(1.0, rows / columns))
                 params, grads, averages = map(list, zip(*members))
-                _native.bridge().muon_step(params, grads, averages, group["steps"], *group["coefficients"], group["eps"], group["halves"], group["momentum"],
-                                           group["nesterov"], 1.0 - group["lr"] * group["weight_decay"], group["lr"] * scale)
+                _native.bridge().muon_step(params, grads, averages, group["steps"], *group["coefficients"], group["eps"], group["halves"],
+                                           WORKSPACE_BYTES, group["momentum"], group["nesterov"], 1.0 - group["lr"] * group["weight_decay"], group["lr"] * scale)
         return loss

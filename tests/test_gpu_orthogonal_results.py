@@ -9,7 +9,7 @@ import torch
 
 import expert_reference as ref
 from permutohedral_encoding_amd import optim
-from test_gpu_orthogonal import TYPES, norms, updates
+from test_gpu_orthogonal import TYPES, assert_orthogonalised, norms, updates
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,44 @@ def test_muon_in_halves():
     again.load_state_dict(saved)
     again.step()
     assert again.param_groups[0]["halves"] is False
+
+
+@pytest.mark.parametrize("matrices,rows,columns", [(7, 300, 140), (9, 203, 131), (6, 129, 130), (70, 200, 5), (5, 64, 48)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_as_many_matrices_as_the_workspace_has_room_for(monkeypatch, dtype, matrices, rows, columns):
+    """(131 * 203 values are odd: four matrices at a time at the least)"""
+    update = updates(matrices, rows, columns, TYPES[dtype])
+    for most in (0, 1 << 20, 3 << 20):
+        monkeypatch.setattr(optim, "WORKSPACE_BYTES", most)
+        assert_orthogonalised(optim.orthogonalise(update), update)
+        assert_orthogonalised(optim.orthogonalise(update, steps=8), update, steps=8)
+    monkeypatch.setattr(optim, "WORKSPACE_BYTES", -1)
+    with pytest.raises(ValueError, match="negative"):
+        optim.orthogonalise(update)
+
+
+def test_muon_takes_the_parameters_of_a_size_in_several_parts(monkeypatch):
+    start = [updates(2, 40, 30, torch.float32, seed=i, scale=0.1) for i in range(5)]
+    grads = [updates(2, 40, 30, torch.float32, seed=10 + i) for i in range(5)]
+    results = []
+    for most in (4 << 30, 0, 2 * 2 * 2 * 40 * 30 * 4):  # all at once, each alone, two at a time
+        monkeypatch.setattr(optim, "WORKSPACE_BYTES", most)
+        params = [torch.nn.Parameter(s.clone()) for s in start]
+        opt = optim.Muon(params, lr=0.02)
+        for _ in range(2):
+            for p, g in zip(params, grads):
+                p.grad = g.clone()
+            opt.step()
+        results.append([t for p in params for t in (p.detach(), opt.state[p]["momentum_buffer"])])
+    assert all(torch.equal(a, b) for other in results[1:] for a, b in zip(results[0], other))
+
+
+def test_thin_matrices_take_no_more_than_their_sums():
+    """2^24 values in matrices of one column: 16 GB if they went as large ones do."""
+    update = updates(4096, 4096, 1, torch.float32)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = optim.orthogonalise(update)
+    assert torch.cuda.max_memory_allocated() - before <= 10 * 4 * update.numel()
+    assert_orthogonalised(got, update)

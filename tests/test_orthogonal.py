@@ -53,3 +53,35 @@ def test_workspace_of_halves():
         assert workspace(type=type, **large) == workspace(type=type, halves=1, **large) == workspace(type=2, **large) >= 2 * 4 * values
     assert 2 * 2 * values <= workspace(type=2, halves=1, **large) < 2 * 4 * values
     assert _native.lib().penc_orthogonalise_workspace_bytes(2, 16, 4096, 1024) == workspace(type=2, halves=1, **large)
+
+
+def test_workspace_is_what_the_way_takes():
+    """Thin matrices go by sums of their S alone; columns padded to 32 and two copies of X are for steps that they do not survive in 64 bits."""
+    gib, lib = 1 << 30, _native.lib()
+    for type in (0, 1, 2):
+        for (matrices, rows, columns), most in (((16384, 4096, 1), 2.2 * gib), ((1024, 4096, 3), 0.15 * gib), ((4096, 65536, 1), 2.2 * gib)):
+            given = dict(type=type, matrices=matrices, rows=rows, columns=columns)
+            assert 0 < workspace(**given) <= most
+            assert workspace(steps=7, **given) == workspace(steps=1, **given) == workspace(**given)
+            assert workspace(steps=8, **given) > 4 * rows * columns * matrices
+            assert lib.penc_orthogonalise_workspace_bytes(type, matrices, rows, columns) >= max(workspace(halves=1, **given), workspace(halves=1, steps=8, **given))
+    # matrices that stay in the LDS take none, long ones of 48 rows and fewer a little, as long as there are few
+    assert workspace(matrices=1000, rows=64, columns=256) == 0 == workspace(matrices=3, rows=64, columns=300, steps=20) == workspace(matrices=65, rows=5, columns=200)
+    assert 0 < workspace(matrices=64, rows=5, columns=200) < 1 << 20 and workspace(matrices=64, rows=5, columns=200, steps=8) == 0
+    # nothing for what is refused
+    for given in (dict(steps=0), dict(steps=65), dict(eps=0.0), dict(coefficients=(4.0, 0.0, 0.0)), dict(matrices=-1), dict(rows=0)):
+        assert workspace(**{"rows": 1000, "columns": 203, **given}) == 0
+
+
+def test_less_workspace_than_the_way_takes_is_refused():
+    block, p = _memory()
+    given = dict(matrices=3, rows=3000, columns=50)
+    need = workspace(**given)
+    large = workspace(steps=20, **given)
+    assert 0 < need < large
+
+    def call(n, g=p, **more):
+        return _native.lib().penc_orthogonal_matrices(ctypes.byref(orthogonal(**given, **more)), g, p + 1024, p, n, None)
+
+    assert call(need - 1) == 8 and call(large - 1, steps=20) == 8 and call(need, steps=20) == 8
+    assert _native.lib().penc_orthogonalise(0, 3, 3000, 50, 5, *MUON, 1e-7, p, p + 1024, p, need - 1, None) == 8
