@@ -102,6 +102,29 @@ PyObject* py_orthogonalise(PyObject*, PyObject* const* args, Py_ssize_t n_args) 
     });
 }
 
+// orthogonal_options(steps, a, b, c, eps, halves, most_bytes): raises what the functions here would
+PyObject* py_orthogonal_options(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        TORCH_CHECK(n_args == 7, "orthogonal_options takes 7 arguments");
+        TORCH_CHECK(api.orthogonal_matrices != nullptr, "bind() has not been called");
+        const Options o = options_of(args);
+        if (PyErr_Occurred()) return nullptr;
+        require_accepted(o);
+        Py_RETURN_NONE;
+    });
+}
+
+// orthogonal_sizes(param, grad), likewise
+PyObject* py_orthogonal_sizes(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        TORCH_CHECK(n_args == 2, "orthogonal_sizes takes 2 arguments");
+        const Tensor &param = tensor_arg(args[0], "a parameter"), &grad = tensor_arg(args[1], "a gradient");
+        require_plain({&param, &grad});
+        require_matrices(param, "a parameter");
+        Py_RETURN_NONE;
+    });
+}
+
 void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& averages, const Options& o, double momentum,
                int nesterov, double decay, double rate) {
     const Tensor& first = params[0];
@@ -164,6 +187,8 @@ PyObject* py_muon_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     });
 }
 PyMethodDef methods[] = {fast<py_orthogonalise>("orthogonalise", "nearly orthogonal matrices from updates"),
+                         fast<py_orthogonal_options>("orthogonal_options", "what steps, coefficients and eps are refused for"),
+                         fast<py_orthogonal_sizes>("orthogonal_sizes", "what a parameter and its gradient are refused for"),
                          fast<py_muon_step>("muon_step", "a step with orthogonalised updates"),
                          {nullptr, nullptr, 0, nullptr}};
 

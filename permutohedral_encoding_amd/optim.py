@@ -170,8 +170,10 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # (what may be refused is looked at before anything is changed)
+        bridge = _native.bridge()
         for group in self.param_groups:
-            together = {}
+            bridge.orthogonal_options(group["steps"], *group["coefficients"], group["eps"], group["halves"], WORKSPACE_BYTES)
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -179,16 +181,22 @@ class Muon(torch.optim.Optimizer):
                     raise RuntimeError("Muon: parameters must be contiguous tensors in GPU memory")
                 if p.grad.layout != torch.strided or p.grad.dtype != p.dtype:
                     raise RuntimeError("Muon: gradients must be dense and of the parameter's type")
+                bridge.orthogonal_sizes(p, p.grad)
+                if not self.state.get(p) and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("Muon: a step has to be taken before one is captured (a graph would begin the averages anew each time)")
+        for group in self.param_groups:
+            together = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
                 state = self.state[p]
                 if not state:
-                    if torch.cuda.is_current_stream_capturing():
-                        raise RuntimeError("Muon: a step has to be taken before one is captured (a graph would begin the averages anew each time)")
                     state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 together.setdefault((tuple(p.shape), p.dtype, p.device), []).append((p, p.grad.contiguous(), state["momentum_buffer"]))
             for (shape, _, _), members in together.items():
                 rows, columns = shape[-2:]
                 scale = 0.2 * math.sqrt(max(rows, columns)) if group["match_rms_adamw"] else math.sqrt(max(1.0, rows / columns))
                 params, grads, averages = map(list, zip(*members))
-                _native.bridge().muon_step(params, grads, averages, group["steps"], *group["coefficients"], group["eps"], group["halves"],
-                                           WORKSPACE_BYTES, group["momentum"], group["nesterov"], 1.0 - group["lr"] * group["weight_decay"], group["lr"] * scale)
+                bridge.muon_step(params, grads, averages, group["steps"], *group["coefficients"], group["eps"], group["halves"], WORKSPACE_BYTES,
+                                 group["momentum"], group["nesterov"], 1.0 - group["lr"] * group["weight_decay"], group["lr"] * scale)
         return loss

@@ -107,3 +107,54 @@ def test_thin_matrices_take_no_more_than_their_sums():
     got = optim.orthogonalise(update)
     assert torch.cuda.max_memory_allocated() - before <= 10 * 4 * update.numel()
     assert_orthogonalised(got, update)
+
+
+def test_a_refused_step_changes_nothing():
+    """Whatever is refused, in whichever group: parameters, averages and their versions stay as they are, and the next step is the one that it would have been."""
+    def refused_options(p, opt):
+        opt.param_groups[1]["coefficients"] = (4.0, 0.0, 0.0)
+        return ValueError, "coefficients"
+
+    def refused_eps(p, opt):
+        opt.param_groups[1]["eps"] = 0.0
+        return ValueError, "eps"
+
+    def refused_type(p, opt):
+        p[2].data = p[2].data.double()
+        p[2].grad = torch.ones_like(p[2])
+        return ValueError, "type"
+
+    def refused_gradient(p, opt):
+        p[2].grad = p[2].grad.to_sparse()
+        return RuntimeError, "dense"
+
+    def refused_layout(p, opt):
+        p[2].data = p[2].data.t().contiguous().t()
+        return RuntimeError, "contiguous"
+
+    for refusal in (refused_options, refused_eps, refused_type, refused_gradient, refused_layout):
+        for steps_before in (0, 1):
+            params = [torch.nn.Parameter(updates(1, 40, 30, torch.float32, seed=i, scale=0.1)[0]) for i in range(3)]
+            opt = optim.Muon([dict(params=params[:2]), dict(params=params[2:])], lr=0.02)
+            for p in params:
+                p.grad = updates(1, 40, 30, torch.float32, seed=7)[0]
+            for _ in range(steps_before):
+                opt.step()
+            kept = [p.detach().clone() for p in params[:2]]
+            averages = [opt.state[p]["momentum_buffer"].clone() if steps_before else None for p in params]
+            versions = [p._version for p in params[:2]]
+            error, message = refusal(params, opt)
+            with pytest.raises(error, match=message):
+                opt.step()
+            assert all(torch.equal(p, k) for p, k in zip(params, kept)) and versions == [p._version for p in params[:2]]
+            assert all(torch.equal(opt.state[p]["momentum_buffer"], a) if steps_before else not opt.state.get(p) for p, a in zip(params, averages))
+    # a single group, and one matrix
+    p = torch.nn.Parameter(updates(1, 40, 30, torch.float32, scale=0.1)[0])
+    opt = optim.Muon([p], lr=0.02)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    average = opt.state[p]["momentum_buffer"].clone()
+    opt.param_groups[0]["coefficients"] = (4.0, 0.0, 0.0)
+    with pytest.raises(ValueError, match="coefficients"):
+        opt.step()
+    assert torch.equal(opt.state[p]["momentum_buffer"], average)
