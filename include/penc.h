@@ -58,7 +58,7 @@ extern "C" {
 #define PENC_ERR_WORKSPACE_TOO_SMALL 8  /* penc_backward_rowmajor with positions_grad, penc_forward_rowmajor: no room for the level-major array */
 #define PENC_ERR_UNSUPPORTED_TABLE_FORMAT 9 /* the *_half entry points: table_format is neither PENC_TABLE_FP16 nor PENC_TABLE_BF16 */
 #define PENC_ERR_UNSUPPORTED_TYPE 10        /* the layers: a type is none of PENC_FP32, PENC_FP16, PENC_BF16 */
-#define PENC_ERR_UNSUPPORTED_KIND 11        /* the layers: no such activation or norm */
+#define PENC_ERR_UNSUPPORTED_KIND 11        /* the layers: no such activation or norm; refused coefficients or eps */
 #define PENC_ERR_BAD_LAYER_SIZE 12          /* the layers: a negative number of rows, channels not in 1..the entry point's most, or strides it does not take */
 
 const char* penc_status_string(int status);

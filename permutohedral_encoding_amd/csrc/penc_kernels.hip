@@ -1695,7 +1695,7 @@ const char* penc_status_string(int status) {
         case PENC_ERR_UNSUPPORTED_TABLE_FORMAT: return "table_format must be PENC_TABLE_FP16 or PENC_TABLE_BF16, with PENC_TABLE_CELLS for capacities that are powers of two and fill a line";
         case PENC_ERR_SCRATCH_TOO_SMALL: return "the problem is too large for the library's static scratch (penc_static_scratch_bytes): use penc_backward with a workspace";
         case PENC_ERR_UNSUPPORTED_TYPE: return "a type must be PENC_FP32, PENC_FP16 or PENC_BF16, that of parameters and gates the rows' or PENC_FP32";
-        case PENC_ERR_UNSUPPORTED_KIND: return "no such activation or norm";
+        case PENC_ERR_UNSUPPORTED_KIND: return "no such activation or norm, or coefficients or an eps that are refused (penc_orthogonal_matrices)";
         case PENC_ERR_BAD_LAYER_SIZE: return "rows must not be negative and a multiple of those of a gate, channels, experts and choices at least 1 and at most what the layer takes";
         default: return "unknown status";
     }

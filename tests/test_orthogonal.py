@@ -85,3 +85,13 @@ def test_less_workspace_than_the_way_takes_is_refused():
 
     assert call(need - 1) == 8 and call(large - 1, steps=20) == 8 and call(need, steps=20) == 8
     assert _native.lib().penc_orthogonalise(0, 3, 3000, 50, 5, *MUON, 1e-7, p, p + 1024, p, need - 1, None) == 8
+
+
+def test_the_status_names_what_was_refused():
+    block, p = _memory()
+    lib = _native.lib()
+    lib.penc_status_string.restype = ctypes.c_char_p
+    for given in (dict(eps=0.0), dict(coefficients=(4.0, 0.0, 0.0))):
+        status = lib.penc_orthogonal_matrices(ctypes.byref(orthogonal(**given)), p, p + 1024, p, 1 << 40, None)
+        text = lib.penc_status_string(status).decode()
+        assert "coefficients" in text and "eps" in text and "activation" in text
