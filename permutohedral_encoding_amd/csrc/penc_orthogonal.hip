@@ -10,7 +10,8 @@
 //     for bfloat16 results, where the caller asks for it (`halves`), as float16, one product for each, and F's diagonal, which is most of F, in float32: 1.8e-3 to 2.0e-3
 //         (with the diagonal in float16 2.0e-3 to 2.4e-3) in a third of the time: 16 x 4096 x 1024 1517 us, as two values 4796
 //
-// times 2^12: with |X| <= 1.2, S <= 1.5 and F <= 3 they stay under 2^14 (a bound on the coefficients sees to that), and what matters of lo is no subnormal number.
+// times 2^12, so that what matters of lo is no subnormal number.  Of the steps above |X| <= 1.2, S <= 1.5 and F <= 3, which is under 2^14.  Coefficients are accepted up to |X| <= 3 and F <= 15:
+// S 2^12 <= 36864 and F 2^12 <= 61440, where float16 ends at 65504 and roundings of X (2^-22, in halves 2^-11) add less than 2% to F.
 // The matrix cores run float16 8 times as fast as float32, so that three products take 3/8 of the time.
 //
 // S and S S are symmetric: tiles on one side of the diagonal are computed and stored twice.  Matrices of up to 128 rows (or columns) that fit the LDS go through all of their

@@ -158,3 +158,23 @@ def test_a_refused_step_changes_nothing():
     with pytest.raises(ValueError, match="coefficients"):
         opt.step()
     assert torch.equal(opt.state[p]["momentum_buffer"], average)
+
+
+@pytest.mark.parametrize("shape", [(3, 40, 60), (2, 140, 150), (2, 300, 140), (2, 500, 3)])
+def test_coefficients_at_the_limits(shape):
+    """2.4 times the Chebyshev polynomial of degree 5 has a factor of 15 below (at singular values of sqrt(5/8)), and 3 s is the most that is made of a singular value.  A few directions have all of the
+    norm, so that there are such singular values."""
+    rank = min(3, *shape[1:])
+    for seed in range(3):
+        kw = dict(generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+        sizes = torch.tensor([0.79, 0.5, 0.35], device="cuda")[:rank]
+        left, right = (torch.linalg.qr(torch.randn((shape[0], n, rank), **kw)).Q for n in shape[1:])
+        update = (left * sizes) @ right.transpose(-1, -2).contiguous() + 1e-4 * torch.randn(shape, **kw) / math.sqrt(shape[1])
+        for coefficients in ((11.99, -47.96, 38.368), (-11.99, 47.96, -38.368), (3.0, 0.0, 0.0), (2.0, 1.0, 0.0)):
+            for dtype in TYPES.values():
+                given = update.to(dtype)
+                assert_orthogonalised(optim.orthogonalise(given, coefficients=coefficients, steps=1), given, coefficients=coefficients, steps=1)
+                if dtype == torch.bfloat16:
+                    assert_orthogonalised(optim.orthogonalise(given, coefficients=coefficients, steps=1, halves=True), given, coefficients=coefficients, steps=1)
+    with pytest.raises(ValueError, match="coefficients"):
+        optim.orthogonalise(update, coefficients=(12.02, -48.08, 38.464), steps=1)
