@@ -1,0 +1,125 @@
+"""Sums of the layers of experts whose every partial sum is a whole number that float32 holds, so that any order gives the same: results have to be the sum of 64 bits, rounded once.
+
+A row that is lost, doubled or read from next to where it is changes them, which a tolerance that grows with the rows does not see."""
+import math
+
+import pytest
+import torch
+
+from permutohedral_encoding_amd import layers
+from test_gpu_experts import TYPES, chosen_experts
+
+pytestmark = pytest.mark.gpu
+
+
+def whole(shape, seed, dtype, most=2):
+    generator = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-most, most + 1, shape, generator=generator, device="cuda").to(dtype)
+
+
+def uneven_experts(rows, number, seed=0, none=300):
+    """Half of the rows to the last expert, one row to expert 1, none to expert 0 (from three experts on), and some without an expert."""
+    generator = torch.Generator(device="cuda").manual_seed(seed)
+    e = torch.randint(0, number, (rows, 1), generator=generator, device="cuda")
+    e = torch.where(torch.rand((rows, 1), generator=generator, device="cuda") < 0.5, number - 1, e)
+    if number > 2:
+        e[e < 2] = 2
+        e[rows // 2] = 1
+    e[torch.randperm(rows, generator=generator, device="cuda")[:min(none, rows // 10)]] = -1
+    return e
+
+
+def check_whole(rows, number, channels, outputs, dtype, extra=(0, 0), bias=True, seed=0):
+    routing = layers.routing(uneven_experts(rows, number, seed), number)
+    offsets = routing.offsets.tolist()
+    x, grad = whole((rows, channels + extra[0]), seed + 1, dtype)[:, :channels], whole((rows, outputs + extra[1]), seed + 2, dtype)[:, :outputs]
+    weight, b = whole((number, outputs, channels), seed + 3, dtype), whole((number, outputs), seed + 4, dtype)
+    assert 4 * max(rows, channels, outputs) + 2 < 1 << 24
+    xd, gd, wd, bd = (t.double() for t in (x, grad, weight, b))
+    want = {"y": torch.zeros((rows, outputs), dtype=torch.float64, device="cuda"), "dx": torch.zeros((rows, channels), dtype=torch.float64, device="cuda"),
+            "dweight": torch.zeros_like(wd), "dbias": torch.zeros_like(bd)}
+    for e in range(number):
+        at = slice(offsets[e], offsets[e + 1])
+        want["y"][at] = xd[at] @ wd[e].t() + (bd[e] if bias else 0.0)
+        want["dx"][at] = gd[at] @ wd[e]
+        want["dweight"][e] = gd[at].t() @ xd[at]
+        want["dbias"][e] = gd[at].sum(0)
+    x[offsets[-1]:] = math.nan  # (what stands in rows without an expert is not read)
+    grad[offsets[-1]:] = math.nan
+    given = [t.requires_grad_(True) for t in ((x, weight, b) if bias else (x, weight))]
+    y = layers.expert_linear(x, weight, b if bias else None, routing)
+    got = {"y": y.detach(), **dict(zip(("dx", "dweight", "dbias"), torch.autograd.grad(y, given, grad)))}
+    for name, g in got.items():
+        wrong = g != want[name].to(dtype)
+        assert not bool(wrong.any()), f"{name}: {int(wrong.sum())} of {wrong.numel()} values, the first at {wrong.nonzero()[0].tolist()}"
+    # each gradient alone goes its own way
+    for k, name in enumerate(("dx", "dweight", "dbias")[:len(given)]):
+        alone = [t.detach().requires_grad_(i == k) for i, t in enumerate(given)]
+        y = layers.expert_linear(alone[0], alone[1], alone[2] if bias else None, routing)
+        assert torch.equal(torch.autograd.grad(y, alone[k], grad)[0], want[name].to(dtype)), name
+
+
+# Rows of an expert are cut for the weights' gradient, in tiles of 64, 128 and (16-bit types) 256.  `extra`: how much further apart rows of x and of the gradient are than they are long: with 3 they
+# begin anywhere.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,channels,outputs", [(70001, 2, 64, 64), (40001, 5, 24, 56), (50000, 1, 48, 130), (40000, 3, 128, 128), (100000, 40, 136, 136), (30000, 3, 200, 264), (100003, 7, 512, 512),
+                                                          (65537, 1, 1024, 1024)])
+@pytest.mark.parametrize("extra", [(0, 0), (3, 5), (8, 3)])
+def test_experts_of_many_rows(dtype, rows, number, channels, outputs, extra):
+    check_whole(rows, number, channels, outputs, TYPES[dtype], extra)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,channels,outputs", [(30000, 2, 3, 200), (30000, 2, 200, 3), (30000, 3, 5, 6), (30000, 2, 1, 64), (20000, 2, 130, 1), (40000, 3, 101, 130), (30011, 4, 264, 1032)])
+def test_experts_of_odd_sizes(dtype, rows, number, channels, outputs):
+    check_whole(rows, number, channels, outputs, TYPES[dtype])
+    check_whole(rows, number, channels, outputs, TYPES[dtype], extra=(1, 2), bias=False, seed=5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,channels,outputs", [(1000, 3, 512, 512), (4000, 4, 512, 512), (500, 1, 4096, 64), (1257, 82, 2048, 24), (20, 6, 1024, 264), (300, 100, 64, 64), (1, 1, 65, 63), (129, 2, 129, 129),
+                                                          (63, 1, 512, 200), (64, 1, 200, 512), (65, 1, 512, 512), (513, 1, 136, 200)])
+def test_experts_of_few_rows(dtype, rows, number, channels, outputs):
+    check_whole(rows, number, channels, outputs, TYPES[dtype])
+    check_whole(rows, number, channels, outputs, TYPES[dtype], extra=(3, 1), seed=7)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("rows,number,channels,outputs", [(140000, 2, 1024, 72), (140000, 2, 1032, 128), (140000, 1, 264, 1024), (70000, 3, 1024, 1040)])
+def test_wide_tiles_of_results(dtype, rows, number, channels, outputs):
+    check_whole(rows, number, channels, outputs, TYPES[dtype])
+
+
+# Rows of a few bytes go in pieces of 2, 4 and 8 values; rows that are whole lines of 64 bytes, or long, go past the caches.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("channels", [1, 2, 3, 4, 5, 6, 7, 8, 9, 15, 16, 17, 24, 31, 32, 33, 48, 64, 200, 256, 500, 511, 512, 1000, 1024, 2049])
+@pytest.mark.parametrize("choices", [1, 2, 3, 8])
+def test_rows_there_and_back(dtype, channels, choices):
+    rows, number, dtype = 1003, 6, TYPES[dtype]
+    experts = chosen_experts(rows, choices, number, seed=channels)
+    routing = layers.routing(experts, number)
+    there, flat = experts >= 0, routing.positions.view(-1).long()
+    items = rows * choices
+    assert torch.equal(torch.sort(flat).values, torch.arange(items, device="cuda"))
+
+    def sort(t):
+        out = torch.empty((items, channels), dtype=t.dtype, device="cuda")
+        out[flat] = torch.where(there[:, :, None], t, 0).reshape(items, channels)
+        return out
+
+    def back(t):
+        return torch.where(there[:, :, None], t[flat].view(rows, choices, channels), 0)
+
+    x, y, weights = whole((rows, channels), 1, dtype), whole((items, channels), 2, dtype), whole((rows, choices), 3, torch.float32, most=3)
+    grad_sorted, grad_out = whole((items, channels), 4, dtype), whole((rows, channels), 5, dtype)
+    total = int(routing.offsets[-1])
+    y[total:] = math.nan
+    grad_sorted[total:] = math.nan
+    for t in (x, y, weights):
+        t.requires_grad_(True)
+    ordered, out = layers.dispatch(x, routing), layers.combine(y, weights, routing)
+    got = dict(zip(("dx", "dy", "dweights"), torch.autograd.grad((ordered, out), (x, y, weights), (grad_sorted, grad_out))))
+    yd, wd, gd = back(y.detach().double()), weights.detach().double()[:, :, None], grad_out.double()[:, None]
+    want = {"sorted": sort(x.detach().double()[:, None].expand(-1, choices, -1)), "out": (yd * wd).sum(1), "dx": back(grad_sorted.double()).sum(1), "dy": sort(gd * wd), "dweights": (gd * yd).sum(2)}
+    for name, g in dict(got, sorted=ordered.detach(), out=out.detach()).items():
+        assert torch.equal(g, want[name].to(g.dtype)), name
