@@ -8,6 +8,7 @@
 //
 // The type of values (PENC_TYPE: those of penc.h) is one compilation each.
 #include <algorithm>
+#include <cmath>
 
 #include "penc_expert_linear.hpp"
 #include "penc_product.hpp"
@@ -374,34 +375,38 @@ struct WeightArgs {
     int64_t pieces;
 };
 
-// Adds what a step has of dy to a wave's sums of dy itself: of 16-bit types its products with ones, of fp32, whose products take eight times as long, each lane's own k.
+// A wave's sums of dy itself: of 16-bit types its products with ones, of fp32, whose products take eight times as long, each lane's own k, in 64 bits.
 template <int kTilesN>
-__device__ __forceinline__ void add_bias_grads(const chunk16 (&grad)[kTilesN], tile_acc (&bias_acc)[kTilesN]) {
-    const uint32_t one = PENC_TYPE == PENC_FP16 ? 0x3C003C00u : 0x3F803F80u;
-    const chunk16 ones = {one, one, one, one};
+struct BiasGrads {
+    static constexpr bool kWide = PENC_TYPE == PENC_FP32;
+    tile_acc acc[kWide ? 1 : kTilesN] = {};
+    double wide[kWide ? kTilesN : 1] = {};
+
+    __device__ __forceinline__ void add(const chunk16 (&grad)[kTilesN]) {
+        const uint32_t one = PENC_TYPE == PENC_FP16 ? 0x3C003C00u : 0x3F803F80u;
+        const chunk16 ones = {one, one, one, one};
 #pragma unroll
-    for (int j = 0; j < kTilesN; ++j) {
-        if constexpr (PENC_TYPE == PENC_FP32) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) bias_acc[j][k] += __uint_as_float(grad[j][k]);
-        } else {
-            bias_acc[j] = multiply<Value>(ones, grad[j], bias_acc[j]);
+        for (int j = 0; j < kTilesN; ++j) {
+            if constexpr (kWide) wide[j] += static_cast<double>((__uint_as_float(grad[j][0]) + __uint_as_float(grad[j][1])) + (__uint_as_float(grad[j][2]) + __uint_as_float(grad[j][3])));
+            else acc[j] = multiply<Value>(ones, grad[j], acc[j]);
         }
     }
-}
+    // The sum of tile j, where lanes 16 apart have a part each (fp32; of 16-bit types all have all).
+    __device__ __forceinline__ float sum(int j) const {
+        if constexpr (kWide) {
+            double v = wide[j];
+            v += __shfl_xor(v, 16);
+            v += __shfl_xor(v, 32);
+            return static_cast<float>(v);
+        } else {
+            return acc[j][0];
+        }
+    }
+};
 
 // Stores what a workgroup has of dW, and the waves with `bias` of db: the results where the expert's rows are one piece, else the piece's sums.
 template <class P>
-__device__ __forceinline__ void store_weight_grads(const WeightArgs& a, const RowTile& t, uint32_t piece, int c0, int o0, const P& p, bool bias, tile_acc (&bias_acc)[P::kTilesN]) {
-    if constexpr (PENC_TYPE == PENC_FP32) {
-#pragma unroll
-        for (int j = 0; j < P::kTilesN; ++j) {
-            float sum = (bias_acc[j][0] + bias_acc[j][1]) + (bias_acc[j][2] + bias_acc[j][3]);
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            bias_acc[j][0] = sum;
-        }
-    }
+__device__ __forceinline__ void store_weight_grads(const WeightArgs& a, const RowTile& t, uint32_t piece, int c0, int o0, const P& p, bool bias, const BiasGrads<P::kTilesN>& of_bias) {
     const int64_t n_weights = static_cast<int64_t>(a.outputs) * a.channels;
     const bool whole = t.tiles == 1;
     const int64_t at = static_cast<int64_t>(o0) * a.channels + c0;
@@ -411,10 +416,11 @@ __device__ __forceinline__ void store_weight_grads(const WeightArgs& a, const Ro
     const int lane = threadIdx.x % 64;
 #pragma unroll
     for (int j = 0; j < P::kTilesN; ++j) {
+        const float sum = of_bias.sum(j);
         const int o = o0 + P::wave_n() + 16 * j + lane;
         if (lane >= 16 || o >= a.outputs) continue;
-        if (whole) static_cast<Value*>(a.bias)[static_cast<int64_t>(t.expert) * a.outputs + o] = static_cast<Value>(bias_acc[j][0]);
-        else a.sums[a.pieces * n_weights + static_cast<int64_t>(piece) * a.outputs + o] = bias_acc[j][0];
+        if (whole) static_cast<Value*>(a.bias)[static_cast<int64_t>(t.expert) * a.outputs + o] = static_cast<Value>(sum);
+        else a.sums[a.pieces * n_weights + static_cast<int64_t>(piece) * a.outputs + o] = sum;
     }
 }
 
@@ -433,11 +439,11 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
     const Operand n{static_cast<const char*>(a.grad) + (static_cast<int64_t>(t.first) * a.grad_stride + o0) * kSize, a.grad_stride * kSize, t.rows,
                     min(a.outputs - o0, P::kN) * kSize};
     P p;
-    tile_acc bias_acc[P::kTilesN] = {};
+    BiasGrads<P::kTilesN> of_bias;
     p.run(lds, m, n, t.rows, P::kZero, [&](const chunk16 (&grad)[P::kTilesN]) {
-        if (bias) add_bias_grads(grad, bias_acc);
+        if (bias) of_bias.add(grad);
     });
-    store_weight_grads(a, t, piece, c0, o0, p, bias, bias_acc);
+    store_weight_grads(a, t, piece, c0, o0, p, bias, of_bias);
 }
 
 constexpr int kNarrowRing = 3, kTailBlocks = 256;
@@ -492,7 +498,7 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_grads_kernel(Wei
     P p;
     p.start(P::kZero);
     const bool bias = a.bias != nullptr && P::wave_m() == 0;
-    tile_acc bias_acc[P::kTilesN] = {};
+    BiasGrads<P::kTilesN> of_bias;
     wait_for_loads<P::kLoads * (kNarrowRing - 1)>();
     meet();
     chunk16 w[kTiles][kLines];
@@ -521,22 +527,22 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_grads_kernel(Wei
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             p.multiply_half(f[h]);
-            if (bias) add_bias_grads(f[h].n[0], bias_acc);
+            if (bias) of_bias.add(f[h].n[0]);
         }
         const int row = first + row16;
         store_sixteen_rows(acc, out + static_cast<int64_t>(row) * a.channels + m0, a.channels, t.rows - row, a.channels - m0);
     }
     wait_for_loads<0>();  // (nothing is on its way into the LDS when the workgroup ends)
-    store_weight_grads(a, t, piece, 0, 0, p, bias, bias_acc);
+    store_weight_grads(a, t, piece, 0, 0, p, bias, of_bias);
 }
 
 constexpr int kSumThreads = 256;
 
-// The sums of experts whose rows are several pieces: kSlices lanes share a result's pieces, each taking every kSlices-th in order, and their sums are added in order.
+// The sums of experts whose rows are several pieces, in 64 bits: kSlices lanes share a result's pieces, each taking every kSlices-th in order, and their sums are added in order.
 template <int kSlices>
 __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, uint32_t blocks) {
     constexpr int kResults = kSumThreads / kSlices;
-    __shared__ float lds[kSlices][kResults];
+    __shared__ double lds[kSlices][kResults];
     const int e = static_cast<int>(blockIdx.x / blocks);
     // the first of the expert's pieces, and how many there are
     uint32_t first = 0, mine = 0;
@@ -556,23 +562,25 @@ __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, 
     const bool fours = kWide == 4 && weights % 4 == 0;
     if (fours) {
         using Four = float __attribute__((ext_vector_type(4)));
+        using Doubles = double __attribute__((ext_vector_type(4)));
         for (int64_t i = (static_cast<int64_t>(blockIdx.x % blocks) * kResults + result) * 4; i < weights; i += static_cast<int64_t>(blocks) * kResults * 4) {
             const float* const from = a.sums + first * weights + i;
-            Four sum{};
+            Doubles sum{};
 #pragma unroll 4
-            for (uint32_t k = 0; k < mine; ++k) sum += *reinterpret_cast<const Four*>(from + k * weights);
-            store_values<Value, 4>(static_cast<Value*>(a.weight) + e * weights + i, __builtin_convertvector(sum, Value __attribute__((ext_vector_type(4)))), 4);
+            for (uint32_t k = 0; k < mine; ++k) sum += __builtin_convertvector(*reinterpret_cast<const Four*>(from + k * weights), Doubles);
+            store_values<Value, 4>(static_cast<Value*>(a.weight) + e * weights + i,
+                                   __builtin_convertvector(__builtin_convertvector(sum, Four), Value __attribute__((ext_vector_type(4)))), 4);
         }
     }
     for (int64_t begin = static_cast<int64_t>(blockIdx.x % blocks) * kResults + (fours ? weights : 0); begin < n; begin += static_cast<int64_t>(blocks) * kResults) {
         const int64_t i = begin + result;
         const bool there = i < n, weight = i < weights;
         const int64_t each = weight ? weights : a.outputs, at = weight ? i : i - weights;
-        float sum = 0.0f;
+        double sum = 0.0;
         if (there) {
             const float* const from = a.sums + (weight ? 0 : a.pieces * weights) + first * each + at;
 #pragma unroll 4
-            for (uint32_t k = slice; k < mine; k += kSlices) sum += from[k * each];
+            for (uint32_t k = slice; k < mine; k += kSlices) sum += static_cast<double>(from[k * each]);
         }
         if constexpr (kSlices > 1) {
             lds[slice][result] = sum;
@@ -582,7 +590,7 @@ __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, 
             for (int k = 1; k < kSlices; ++k) sum += lds[k][result];
             __syncthreads();
         }
-        if (there && slice == 0) static_cast<Value*>(weight ? a.weight : a.bias)[e * each + at] = static_cast<Value>(sum);
+        if (there && slice == 0) static_cast<Value*>(weight ? a.weight : a.bias)[e * each + at] = static_cast<Value>(static_cast<float>(sum));
     }
 }
 
@@ -689,9 +697,12 @@ struct WeightPlan {
 };
 // Workgroups go in rounds of as many as have room at a time.  Beside its rows a workgroup takes as long as for two steps, and where its sums go through memory, as long again as kCut
 // rows.  Either an expert's rows are one piece (up to twice as many as experts have on average, or 3/4 of all that a workgroup has if that is more: 32768 x 1024 by 4096 bf16, 16 experts in uneven demand,
-// y and dW, 614 us and then 591; and a quarter of the time for experts that are not alike), or they are cut for one to four whole rounds.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and 6 for the sums, now 28 and 5;
+// y and dW, 614 us and then 591; and a quarter of the time for experts that are not alike), or they are cut for whole rounds, as few as there can be or up to three more.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and 6 for the sums, now 28 and 5;
 // 2^20 x 64 by 64 fp32, all of the layer, with 2, 4, 6 and 8 to a compute unit 347, 325, 305 and 316 us, with 3 299.  16384 x 1024 by 2048 bf16, 4 experts, y and dW: cut for three rounds
 // 216 us, in one piece 165.)
+// No piece is longer than kLongest.  A chain of n additions of one sign is off by n / 2 times 2^-24 of it at the most: fp32, whose products are added one by one, by 2^-12 (in one chain of
+// 98304 rows 1.2e-3 was seen), 16-bit types, which add 32 products at a time, by 2^-14.  Pieces are added in 64 bits.  (2^20 x 256 by 256 fp32, 4 experts: 3400 us in two rounds of shorter pieces, 3350 without a limit, 3860 with the limit alone.)
+constexpr int64_t kLongest = kSize == 2 ? 1 << 16 : 1 << 13;
 WeightPlan weight_plan_of(int side, int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
     constexpr double kBeside = 128.0, kCut = kSize == 2 ? 512.0 : 128.0;
     WeightPlan p;
@@ -700,14 +711,16 @@ WeightPlan weight_plan_of(int side, int64_t rows, int64_t experts, int64_t chann
     const int64_t room = (side == 256 ? 1 : side == 128 ? 2 : 3) * kUnits, own = (rows + experts - 1) / experts;
     p.most = std::max(2 * own, rows / 4 * 3 * p.tiles / room);
     p.time = static_cast<double>((experts * p.tiles + room - 1) / room) * 1.25 * (static_cast<double>(own) + kBeside);
-    for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+    if (own > kLongest) p.time = INFINITY;
+    const int64_t least = (((rows + kLongest - 1) / kLongest + experts) * p.tiles + room - 1) / room;  // with pieces of kLongest rows
+    for (int64_t rounds = std::max<int64_t>(least, 1); rounds < std::max<int64_t>(least, 1) + 4; ++rounds) {
         const int64_t pieces = rounds * room / p.tiles - experts;
         if (pieces <= 0) continue;
         const int64_t each = std::max<int64_t>((rows + pieces - 1) / pieces, 512);
         const double time = static_cast<double>(rounds) * (static_cast<double>(each) + kBeside + kCut);
         if (time < p.time) p.time = time, p.most = each;
     }
-    p.most = std::min<int64_t>(std::max<int64_t>((p.most + 63) / 64 * 64, 512), int64_t{1} << 30);
+    p.most = std::min<int64_t>(std::max<int64_t>((p.most + 63) / 64 * 64, 512), kLongest);
     p.pieces = rows / p.most + experts;
     return p;
 }

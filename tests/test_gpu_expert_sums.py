@@ -123,3 +123,24 @@ def test_rows_there_and_back(dtype, channels, choices):
     want = {"sorted": sort(x.detach().double()[:, None].expand(-1, choices, -1)), "out": (yd * wd).sum(1), "dx": back(grad_sorted.double()).sum(1), "dy": sort(gd * wd), "dweights": (gd * yd).sum(2)}
     for name, g in dict(got, sorted=ordered.detach(), out=out.detach()).items():
         assert torch.equal(g, want[name].to(g.dtype)), name
+
+
+# Sums of one sign, of values that are all alike: what is rounded away is of one sign, too.  A chain of n additions is off by n / 2 half steps, 2^-24 of the sum each, as its partial sums are half of
+# it on average; 8192 products of fp32 are one chain, 65536 rows of 16-bit values 2048 additions of 32 products (which may be rounded twice).  Pieces are added in 64 bits; products of fp32 and the
+# result are rounded once each.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,channels,outputs", [(1 << 18, 8, 2048, 2048), (1 << 21, 1, 64, 64), (300000, 16, 1024, 1024)])
+def test_long_sums_of_one_sign(dtype, rows, number, channels, outputs):
+    dtype = TYPES[dtype]
+    routing = layers.routing(torch.zeros((rows, 1), dtype=torch.int32, device="cuda"), number)
+    bound = (4096 + 2) * 2.0 ** -24 if dtype == torch.float32 else 2 * 1024 * 2.0 ** -24
+    for a, b in ((1 / 3, 0.1), (1.0, 0.2504880859375), (0.7, 0.9)):
+        a, b = (a, b) if dtype != torch.float16 else (a / 64, b / 64)
+        x, grad = torch.full((1, channels), a, dtype=dtype, device="cuda").expand(rows, channels).contiguous(), torch.full((1, outputs), b, dtype=dtype, device="cuda").expand(rows, outputs).contiguous()
+        weight, bias = (torch.zeros(s, dtype=dtype, device="cuda", requires_grad=True) for s in ((number, outputs, channels), (number, outputs)))
+        y = layers.expert_linear(x.requires_grad_(True), weight, bias, routing)
+        dx, dweight, dbias = torch.autograd.grad(y, (x, weight, bias), grad)
+        for name, got, want in (("dweight", dweight[0], rows * float(x[0, 0].detach()) * float(grad[0, 0])), ("dbias", dbias[0], rows * float(grad[0, 0]))):
+            half = torch.finfo(dtype).eps / 2
+            worst = float((got.double() - want).abs().max()) / want
+            assert worst <= bound + half, f"{name}: {worst:.3g} of the sum, bound {bound + half:.3g}"
