@@ -41,14 +41,15 @@ __device__ __forceinline__ uint32_t sum_to_lane(uint32_t v) {
 
 // Tile `t` of rows: those of an expert (`experts`: the rows behind the last one's), cut every `most` rows.
 struct RowTile {
-    int expert, first, rows, of_expert, tiles;  // of_expert: which of the expert's tiles it is; tiles: the expert's; expert < 0: there is no such tile
+    int expert, first, rows, tiles;  // tiles: the expert's; expert < 0: there is no such tile
+    int64_t slot;                    // pieces: which it is of those of experts with several, whose sums go through memory
 };
 
 // All lanes of a wave call it.  kWhole: tiles of the rows behind the last expert's too; else each expert has a tile at least, be it one of no rows.
 template <bool kWhole>
 __device__ __forceinline__ RowTile row_tile(const int32_t* __restrict__ offsets, int experts, int rows, uint32_t t, int most) {
     const int lane = threadIdx.x % 64;
-    uint32_t before = 0;
+    uint32_t before = 0, cut_before = 0;
     for (int base = 0; base < experts + (kWhole ? 1 : 0); base += 64) {
         const int e = base + lane;
         int from = 0, to = 0;
@@ -59,7 +60,8 @@ __device__ __forceinline__ RowTile row_tile(const int32_t* __restrict__ offsets,
         uint32_t tiles = (static_cast<uint32_t>(n) + most - 1) / most;
         if (!kWhole && e < experts) tiles = max(tiles, 1u);
         if (e > experts || (!kWhole && e == experts)) tiles = 0;
-        const uint32_t sum = sum_to_lane(tiles);
+        const uint32_t cut = !kWhole && tiles > 1 ? tiles : 0u;
+        const uint32_t sum = sum_to_lane(tiles), sum_of_cut = kWhole ? 0u : sum_to_lane(cut);
         const uint64_t behind = __ballot(t < before + sum);
         if (behind != 0) {
             const int found = __builtin_ctzll(behind);
@@ -68,21 +70,20 @@ __device__ __forceinline__ RowTile row_tile(const int32_t* __restrict__ offsets,
             const uint32_t its = its_own(tiles), at = t - before - (its_own(sum) - its);
             // (tiles of rows are full but for the last one; pieces for the weights' gradient are alike)
             const int each = kWhole ? most : (count / static_cast<int>(its) / 64 + 1) * 64, skip = min(static_cast<int>(at) * each, count);
-            return {base + found, first + skip, min(count - skip, each), static_cast<int>(at), static_cast<int>(its)};
+            return {base + found, first + skip, min(count - skip, each), static_cast<int>(its), int64_t{cut_before} + static_cast<uint32_t>(its_own(sum_of_cut)) - static_cast<uint32_t>(its_own(cut)) + at};
         }
-        before += __builtin_amdgcn_readlane(sum, 63);
+        before += __builtin_amdgcn_readlane(sum, 63), cut_before += __builtin_amdgcn_readlane(sum_of_cut, 63);
     }
     return {-1, 0, 0, 0, 0};
 }
 
-// Piece `t` of all experts' (row_tile<false>), the largest pieces first, in classes of an eighth of `most`: workgroups that begin last are short then.  `piece`: which it is in the experts'
-// order.  (32768 rows of 16 experts in uneven demand, 1024 by 4096 bf16, all of the layer: 896 us in the experts' order, 887 so.)  For the experts of a wave's lanes; more of them have more pieces than matter.
-__device__ __forceinline__ RowTile row_tile_by_size(const int32_t* __restrict__ offsets, int experts, int rows, uint32_t t, int most, uint32_t& piece) {
-    piece = t;
+// Piece `t` of all experts' (row_tile<false>), the largest pieces first, in classes of an eighth of `most`: workgroups that begin last are short then.
+// (32768 rows of 16 experts in uneven demand, 1024 by 4096 bf16, all of the layer: 896 us in the experts' order, 887 so.)  For the experts of a wave's lanes; more of them have more pieces than matter.
+__device__ __forceinline__ RowTile row_tile_by_size(const int32_t* __restrict__ offsets, int experts, int rows, uint32_t t, int most) {
     if (experts > 64) return row_tile<false>(offsets, experts, rows, t, most);
     const int lane = threadIdx.x % 64, from = lane < experts ? min(max(offsets[lane], 0), rows) : 0, to = lane < experts ? min(max(offsets[lane + 1], 0), rows) : 0;
     const int n = max(to - from, 0);
-    const uint32_t tiles = lane < experts ? max((static_cast<uint32_t>(n) + most - 1) / most, 1u) : 0u, before = sum_to_lane(tiles) - tiles;
+    const uint32_t tiles = lane < experts ? max((static_cast<uint32_t>(n) + most - 1) / most, 1u) : 0u, cut = tiles > 1 ? tiles : 0u, cut_before = sum_to_lane(cut) - cut;
     const int each = tiles > 0 ? (n / static_cast<int>(tiles) / 64 + 1) * 64 : 0, size = static_cast<int>(static_cast<int64_t>(each) * 8 / most);  // 0 to 9
     uint32_t done = 0;
     for (int s = 9; s >= 0; --s) {
@@ -92,8 +93,7 @@ __device__ __forceinline__ RowTile row_tile_by_size(const int32_t* __restrict__ 
             const int found = __builtin_ctzll(here);
             const auto its_own = [&](uint32_t v) { return static_cast<int>(__builtin_amdgcn_readlane(static_cast<int>(v), found)); };
             const int its = its_own(tiles), at = static_cast<int>(t - done) - (its_own(sum) - its), rows_each = its_own(each), count = its_own(n), skip = min(at * rows_each, count);
-            piece = its_own(before) + at;
-            return {found, its_own(from) + skip, min(count - skip, rows_each), at, its};
+            return {found, its_own(from) + skip, min(count - skip, rows_each), its, int64_t{static_cast<uint32_t>(its_own(cut_before))} + at};
         }
         done += __builtin_amdgcn_readlane(static_cast<int>(sum), 63);
     }
@@ -371,8 +371,8 @@ struct WeightArgs {
     Spread spread;
     uint32_t channel_tiles, tiles;
     void *weight, *bias;  // results, written where an expert's rows are one piece
-    float* sums;          // [pieces][outputs][channels], and behind them [pieces][outputs]
-    int64_t pieces;
+    float* sums;          // [slots][outputs][channels], and behind them [slots][outputs]: of pieces of experts with several
+    int64_t slots;
 };
 
 // A wave's sums of dy itself: of 16-bit types its products with ones, of fp32, whose products take eight times as long, each lane's own k, in 64 bits.
@@ -406,12 +406,12 @@ struct BiasGrads {
 
 // Stores what a workgroup has of dW, and the waves with `bias` of db: the results where the expert's rows are one piece, else the piece's sums.
 template <class P>
-__device__ __forceinline__ void store_weight_grads(const WeightArgs& a, const RowTile& t, uint32_t piece, int c0, int o0, const P& p, bool bias, const BiasGrads<P::kTilesN>& of_bias) {
+__device__ __forceinline__ void store_weight_grads(const WeightArgs& a, const RowTile& t, int c0, int o0, const P& p, bool bias, const BiasGrads<P::kTilesN>& of_bias) {
     const int64_t n_weights = static_cast<int64_t>(a.outputs) * a.channels;
     const bool whole = t.tiles == 1;
     const int64_t at = static_cast<int64_t>(o0) * a.channels + c0;
     if (whole) store_rows(p, static_cast<Value*>(a.weight) + t.expert * n_weights + at, a.channels, a.outputs - o0, a.channels - c0);
-    else store_rows(p, a.sums + piece * n_weights + at, a.channels, a.outputs - o0, a.channels - c0);
+    else store_rows(p, a.sums + t.slot * n_weights + at, a.channels, a.outputs - o0, a.channels - c0);
     if (!bias) return;
     const int lane = threadIdx.x % 64;
 #pragma unroll
@@ -420,7 +420,7 @@ __device__ __forceinline__ void store_weight_grads(const WeightArgs& a, const Ro
         const int o = o0 + P::wave_n() + 16 * j + lane;
         if (lane >= 16 || o >= a.outputs) continue;
         if (whole) static_cast<Value*>(a.bias)[static_cast<int64_t>(t.expert) * a.outputs + o] = static_cast<Value>(sum);
-        else a.sums[a.pieces * n_weights + static_cast<int64_t>(piece) * a.outputs + o] = sum;
+        else a.sums[a.slots * n_weights + t.slot * a.outputs + o] = sum;
     }
 }
 
@@ -430,9 +430,8 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
     __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
     const uint32_t item = a.spread.item(), tile = item % a.tiles;
     if (item >= a.spread.items) return;
-    uint32_t piece;
-    const RowTile t = row_tile_by_size(a.offsets, a.experts, a.rows, item / a.tiles, a.most, piece);
-    if (t.expert < 0 || piece >= a.pieces) return;  // (the second: offsets that no plan has)
+    const RowTile t = row_tile_by_size(a.offsets, a.experts, a.rows, item / a.tiles, a.most);
+    if (t.expert < 0 || (t.tiles > 1 && t.slot >= a.slots)) return;  // (the second: offsets that no plan has)
     const int c0 = static_cast<int>(tile % a.channel_tiles) * P::kM, o0 = static_cast<int>(tile / a.channel_tiles) * P::kN;
     const bool bias = a.bias != nullptr && c0 == 0 && P::wave_m() == 0;
     const Operand m{static_cast<const char*>(a.x) + (static_cast<int64_t>(t.first) * a.x_stride + c0) * kSize, a.x_stride * kSize, t.rows, min(a.channels - c0, P::kM) * kSize};
@@ -443,7 +442,7 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
     p.run(lds, m, n, t.rows, P::kZero, [&](const chunk16 (&grad)[P::kTilesN]) {
         if (bias) of_bias.add(grad);
     });
-    store_weight_grads(a, t, piece, c0, o0, p, bias, of_bias);
+    store_weight_grads(a, t, c0, o0, p, bias, of_bias);
 }
 
 constexpr int kNarrowRing = 3, kTailBlocks = 256;
@@ -472,7 +471,7 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_grads_kernel(Wei
     const uint32_t piece = a.spread.item();
     if (piece >= a.spread.items) return;
     const RowTile t = row_tile<false>(a.offsets, a.experts, a.rows, piece, a.most);
-    if (t.expert < 0) return;
+    if (t.expert < 0 || (t.tiles > 1 && t.slot >= a.slots)) return;  // (the second: offsets that no plan has)
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
     const int64_t row_bytes = static_cast<int64_t>(a.channels) * kSize;
     Load load_w(Operand{static_cast<const char*>(weight) + t.expert * a.outputs * row_bytes, row_bytes, a.outputs, static_cast<int>(row_bytes)});
@@ -533,7 +532,7 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_grads_kernel(Wei
         store_sixteen_rows(acc, out + static_cast<int64_t>(row) * a.channels + m0, a.channels, t.rows - row, a.channels - m0);
     }
     wait_for_loads<0>();  // (nothing is on its way into the LDS when the workgroup ends)
-    store_weight_grads(a, t, piece, 0, 0, p, bias, of_bias);
+    store_weight_grads(a, t, 0, 0, p, bias, of_bias);
 }
 
 constexpr int kSumThreads = 256;
@@ -544,17 +543,17 @@ __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, 
     constexpr int kResults = kSumThreads / kSlices;
     __shared__ double lds[kSlices][kResults];
     const int e = static_cast<int>(blockIdx.x / blocks);
-    // the first of the expert's pieces, and how many there are
+    // the slot of the expert's first piece, and how many pieces there are
     uint32_t first = 0, mine = 0;
     for (int i = static_cast<int>(threadIdx.x) % 64; i <= e; i += 64) {
         const int from = min(max(a.offsets[i], 0), a.rows), to = min(max(a.offsets[i + 1], 0), a.rows);
         const uint32_t n = max((static_cast<uint32_t>(max(to - from, 0)) + a.most - 1) / a.most, 1u);
-        if (i < e) first += n;
+        if (i < e) first += n > 1 ? n : 0u;
         else mine = n;
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) first += __shfl_xor(first, d), mine = max(mine, static_cast<uint32_t>(__shfl_xor(mine, d)));
-    if (mine <= 1 || first + mine > a.pieces) return;  // (the second: offsets that no plan has)
+    if (mine <= 1 || int64_t{first} + mine > a.slots) return;  // (the second: offsets that no plan has)
     const int64_t weights = static_cast<int64_t>(a.outputs) * a.channels, n = weights + (a.bias != nullptr ? a.outputs : 0);
     const int slice = static_cast<int>(threadIdx.x) / kResults, result = static_cast<int>(threadIdx.x) % kResults;
     // (a lane has kWide results: with one slice four, where those of every piece and expert begin on four)
@@ -578,7 +577,7 @@ __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, 
         const int64_t each = weight ? weights : a.outputs, at = weight ? i : i - weights;
         double sum = 0.0;
         if (there) {
-            const float* const from = a.sums + (weight ? 0 : a.pieces * weights) + first * each + at;
+            const float* const from = a.sums + (weight ? 0 : a.slots * weights) + first * each + at;
 #pragma unroll 4
             for (uint32_t k = slice; k < mine; k += kSlices) sum += static_cast<double>(from[k * each]);
         }
@@ -693,6 +692,7 @@ struct WeightPlan {
     int64_t tiles; // of an expert
     int64_t most;  // rows of a piece
     int64_t pieces;
+    int64_t slots; // the most pieces of experts of more than `most` rows
     double time;
 };
 // Workgroups go in rounds of as many as have room at a time.  Beside its rows a workgroup takes as long as for two steps, and where its sums go through memory, as long again as kCut
@@ -722,6 +722,7 @@ WeightPlan weight_plan_of(int side, int64_t rows, int64_t experts, int64_t chann
     }
     p.most = std::min<int64_t>(std::max<int64_t>((p.most + 63) / 64 * 64, 512), kLongest);
     p.pieces = rows / p.most + experts;
+    p.slots = rows / p.most + std::min(experts, rows / (p.most + 1));
     return p;
 }
 WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
@@ -788,7 +789,7 @@ template <>
 size_t expert_weights_workspace<PENC_TYPE>(int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
     const WeightPlan p = weight_plan(rows, experts, channels, outputs);
     if (rows <= p.most) return 0;  // no expert's rows are cut
-    return 4 * static_cast<size_t>(p.pieces) * static_cast<size_t>(outputs) * (static_cast<size_t>(channels) + 1);
+    return 4 * static_cast<size_t>(p.slots) * static_cast<size_t>(outputs) * (static_cast<size_t>(channels) + 1);
 }
 
 template <>
@@ -796,7 +797,7 @@ int expert_grads<PENC_TYPE>(int64_t rows, int experts, int64_t channels, int64_t
                             const void* weight, const int32_t* offsets, void* dx, void* dweight, void* dbias, void* workspace, hipStream_t stream) {
     const WeightPlan plan = weight_plan(rows, experts, channels, outputs);
     WeightArgs a{x, grad, x_stride, grad_stride, offsets, experts, static_cast<int>(rows), static_cast<int>(channels), static_cast<int>(outputs),
-                 static_cast<int>(plan.most), {}, 0, 0, dweight, dbias, static_cast<float*>(workspace), plan.pieces};
+                 static_cast<int>(plan.most), {}, 0, 0, dweight, dbias, static_cast<float*>(workspace), plan.slots};
     const Chunks of_x = chunks_of(x, x_stride, channels), of_grad = chunks_of(grad, grad_stride, outputs);
     const bool together = dx != nullptr && channels <= 64 && outputs <= 64 && of_x == Chunks::kDirect && of_grad == Chunks::kDirect && aligned_to(weight, 16) && aligned_to(dx, 16);
     if (dx != nullptr && !together) {
