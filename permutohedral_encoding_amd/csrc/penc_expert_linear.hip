@@ -665,8 +665,9 @@ int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
     if (a.wide <= 64 || (kChunks == Chunks::kHeld && a.wide > 128 && a.wide <= 192) || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks, 2, kChunksN>>(a, stream);
     if constexpr (kChunks != Chunks::kSingle) {
         if constexpr (kChunks == Chunks::kDirect && kSize == 2) {
-            // (1024 by 4096 bf16, 16 experts, of 2048 rows each: 302 us and 347 without; of 512 89 and 86, of 256 58 and 50: tiles of 256 rows that are not full)
-            if (a.rows >= 1024 * static_cast<int64_t>(a.experts) && static_cast<int64_t>(a.rows / 256) * ((a.wide + 255) / 256) >= 512)
+            // (1024 by 4096 bf16, 16 experts, of 2048 rows each: 302 us and 347 without; of 512 89 and 86, of 256 58 and 50: tiles of 256 rows that are not full.
+            // 2^18 rows of 1024, 4 experts, y and dx: of 72 results 144 and 152 us, without 129 and 130; of 128 152 and 153, 139 and 140; of 264 232 and 239, 232 and 248; 2^17 of 640 189 and 192, 211 and 216)
+            if (a.wide > 128 && a.rows >= 1024 * static_cast<int64_t>(a.experts) && static_cast<int64_t>(a.rows / 256) * ((a.wide + 255) / 256) >= 512)
                 return launch_rows<kBack, Product<Value, kBack, false, 256, 256, 4, 2, kChunks>, Product<Value, kBack, false, 128, 128, 4, 2, kChunks>>(a, stream);
         }
         return launch_rows<kBack, Product<Value, kBack, false, 128, 128, 2, 2, kChunks, 2, kChunksN>>(a, stream);
