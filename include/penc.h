@@ -535,6 +535,10 @@ size_t penc_expert_weight_grad_workspace_bytes(int type, int64_t rows, int exper
 int penc_expert_weight_grad(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t row_stride, const void* grad,
                             int64_t grad_row_stride, const int32_t* offsets, void* weight_grad, void* bias_grad, void* workspace, size_t workspace_bytes,
                             void* stream);
+/* The gradient of the biases alone. */
+size_t penc_expert_bias_grad_workspace_bytes(int type, int64_t rows, int experts, int64_t outputs);
+int penc_expert_bias_grad(int type, int64_t rows, int experts, int64_t outputs, const void* grad, int64_t grad_row_stride, const int32_t* offsets, void* bias_grad,
+                          void* workspace, size_t workspace_bytes, void* stream);
 /* All gradients, with the workspace of the weights' alone: dx as penc_expert_linear_input_grad makes it.  One pass over x and grad for at most 64 channels and outputs. */
 int penc_expert_linear_grads(int type, int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t row_stride, const void* grad,
                              int64_t grad_row_stride, const void* weight, const int32_t* offsets, void* dx, void* weight_grad, void* bias_grad, void* workspace,

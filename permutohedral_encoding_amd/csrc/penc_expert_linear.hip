@@ -535,9 +535,35 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_grads_kernel(Wei
     store_weight_grads(a, t, 0, 0, p, bias, of_bias);
 }
 
+constexpr int kBiasThreads = 256;
+
+// db alone, of pieces of experts' rows: kLanes neighbouring outputs to as many lanes, whose others take the next rows; sums in 64 bits.  Memory bounds it: 32768 x 4096 bf16 of 16 experts 50 us
+// with the sums, 5.4 TB/s (dW with it, and thrown away, 290), 2^20 x 64 fp32 47.
+template <int kLanes>
+__global__ __launch_bounds__(kBiasThreads) void expert_bias_kernel(WeightArgs a) {
+    constexpr int kRows = kBiasThreads / kLanes;
+    __shared__ double lds[kRows][kLanes];
+    const uint32_t item = a.spread.item();
+    if (item >= a.spread.items) return;
+    const RowTile t = row_tile<false>(a.offsets, a.experts, a.rows, item / a.tiles, a.most);
+    if (t.expert < 0 || (t.tiles > 1 && t.slot >= a.slots)) return;  // (the second: offsets that no plan has)
+    const int row = static_cast<int>(threadIdx.x) / kLanes, lane = static_cast<int>(threadIdx.x) % kLanes, o = static_cast<int>(item % a.tiles) * kLanes + lane;
+    // (lanes behind the last output read it too)
+    const Value* const from = static_cast<const Value*>(a.grad) + static_cast<int64_t>(t.first) * a.grad_stride + min(o, a.outputs - 1);
+    double sum = 0.0;
+#pragma unroll 8
+    for (int r = row; r < t.rows; r += kRows) sum += static_cast<double>(static_cast<float>(from[r * a.grad_stride]));
+    lds[row][lane] = sum;
+    __syncthreads();
+    if (row > 0 || o >= a.outputs) return;
+    for (int k = 1; k < kRows; ++k) sum += lds[k][lane];
+    if (t.tiles == 1) static_cast<Value*>(a.bias)[static_cast<int64_t>(t.expert) * a.outputs + o] = static_cast<Value>(static_cast<float>(sum));
+    else a.sums[t.slot * a.outputs + o] = static_cast<float>(sum);
+}
+
 constexpr int kSumThreads = 256;
 
-// The sums of experts whose rows are several pieces, in 64 bits: kSlices lanes share a result's pieces, each taking every kSlices-th in order, and their sums are added in order.
+// The sums of experts whose rows are several pieces (of db alone: with no channels), in 64 bits: kSlices lanes share a result's pieces, each taking every kSlices-th in order, and their sums are added in order.
 template <int kSlices>
 __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, uint32_t blocks) {
     constexpr int kResults = kSumThreads / kSlices;
@@ -687,6 +713,18 @@ int rows_of_experts(const RowsArgs& a, Chunks weight, Chunks rows, hipStream_t s
     return rows_of_experts<kBack, kSingle>(a, stream);
 }
 
+// The same of db alone: pieces for four workgroups to a compute unit, were the outputs of one workgroup.
+struct BiasPlan {
+    int64_t most, pieces, slots;
+};
+BiasPlan bias_plan(int64_t rows, int64_t experts) {
+    BiasPlan p;
+    p.most = std::max<int64_t>((rows / (4 * kUnits) + 63) / 64 * 64, 512);
+    p.pieces = rows / p.most + experts;
+    p.slots = rows / p.most + std::min(experts, rows / (p.most + 1));
+    return p;
+}
+
 // How the rows of the weights' gradient are cut, and the tiles.  A time is in rows that a workgroup multiplies.
 struct WeightPlan {
     int side;      // of a tile
@@ -755,6 +793,18 @@ int launch_narrow_grads(WeightArgs a, const WeightPlan& plan, const void* weight
     return launched();
 }
 
+int launch_sums(const WeightArgs& a, int64_t pieces, hipStream_t stream) {
+    const int64_t results = int64_t{a.outputs} * (a.channels + 1);
+    // (many pieces: a few results, and lanes that share them)
+    const auto sum = [&](auto slices) -> int {
+        constexpr int kSlices = decltype(slices)::value, kResults = kSumThreads / kSlices;
+        const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>((results + kResults - 1) / kResults, std::max<int64_t>(16, 8192 / a.experts)));
+        expert_sums_kernel<kSlices><<<static_cast<uint32_t>(a.experts) * blocks, kSumThreads, 0, stream>>>(a, blocks);
+        return launched();
+    };
+    return pieces >= 32 * int64_t{a.experts} ? sum(std::integral_constant<int, 16>{}) : sum(std::integral_constant<int, 1>{});
+}
+
 template <Chunks kChunks, Chunks kChunksN = kChunks>
 int weights_of_experts(const WeightArgs& a, const WeightPlan& plan, hipStream_t stream) {
     if (plan.side == 64) return launch_weights<Product<Value, true, true, 64, 64, 2, 2, kChunks, 2, kChunksN>>(a, plan, stream);
@@ -806,16 +856,32 @@ int expert_grads<PENC_TYPE>(int64_t rows, int experts, int64_t channels, int64_t
     }
     if (const int rc = together ? launch_narrow_grads(a, plan, weight, dx, stream) : weights_of_experts(a, plan, of_x, of_grad, stream))
         return rc;
-    if (rows <= plan.most) return PENC_OK;
-    const int64_t results = outputs * (channels + 1);
-    // (many pieces: a few results, and lanes that share them)
-    const auto sum = [&](auto slices) -> int {
-        constexpr int kSlices = decltype(slices)::value, kResults = kSumThreads / kSlices;
-        const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>((results + kResults - 1) / kResults, std::max<int64_t>(16, 8192 / experts)));
-        expert_sums_kernel<kSlices><<<static_cast<uint32_t>(experts) * blocks, kSumThreads, 0, stream>>>(a, blocks);
+    return rows <= plan.most ? PENC_OK : launch_sums(a, plan.pieces, stream);
+}
+
+template <>
+size_t expert_bias_workspace<PENC_TYPE>(int64_t rows, int64_t experts, int64_t outputs) {
+    const BiasPlan p = bias_plan(rows, experts);
+    return rows <= p.most ? 0 : 4 * static_cast<size_t>(p.slots) * static_cast<size_t>(outputs);
+}
+
+template <>
+int expert_bias<PENC_TYPE>(int64_t rows, int experts, int64_t outputs, const void* grad, int64_t grad_stride, const int32_t* offsets, void* dbias, void* workspace,
+                           hipStream_t stream) {
+    const BiasPlan plan = bias_plan(rows, experts);
+    WeightArgs a{nullptr, grad, 0, grad_stride, offsets, experts, static_cast<int>(rows), 0, static_cast<int>(outputs), static_cast<int>(plan.most), {}, 0, 0, nullptr, dbias,
+                 static_cast<float*>(workspace), plan.slots};
+    const auto launch = [&](auto lanes) -> int {
+        constexpr int kLanes = decltype(lanes)::value;
+        a.tiles = static_cast<uint32_t>((outputs + kLanes - 1) / kLanes);
+        const int64_t items = plan.pieces * a.tiles;
+        if (items * kBiasThreads >= kMostThreads) return PENC_ERR_BAD_LAYER_SIZE;
+        a.spread = Spread(items, 1);
+        expert_bias_kernel<kLanes><<<a.spread.grid(), kBiasThreads, 0, stream>>>(a);
         return launched();
     };
-    return plan.pieces >= 32 * static_cast<int64_t>(experts) ? sum(std::integral_constant<int, 16>{}) : sum(std::integral_constant<int, 1>{});
+    if (const int rc = outputs <= 16 ? launch(std::integral_constant<int, 16>{}) : launch(std::integral_constant<int, 64>{})) return rc;
+    return rows <= plan.most ? PENC_OK : launch_sums(a, plan.pieces, stream);
 }
 
 }  // namespace penc

@@ -16,5 +16,10 @@ size_t expert_weights_workspace(int64_t rows, int64_t experts, int64_t channels,
 template <int kType>
 int expert_grads(int64_t rows, int experts, int64_t channels, int64_t outputs, const void* x, int64_t x_stride, const void* grad, int64_t grad_stride, const void* weight,
                  const int32_t* offsets, void* dx, void* dweight, void* dbias, void* workspace, hipStream_t stream);
+// db alone.
+template <int kType>
+size_t expert_bias_workspace(int64_t rows, int64_t experts, int64_t outputs);
+template <int kType>
+int expert_bias(int64_t rows, int experts, int64_t outputs, const void* grad, int64_t grad_stride, const int32_t* offsets, void* dbias, void* workspace, hipStream_t stream);
 
 }  // namespace penc

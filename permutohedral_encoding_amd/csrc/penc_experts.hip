@@ -862,4 +862,28 @@ int penc_expert_weight_grad(int type, int64_t rows, int experts, int64_t channel
                                     workspace, workspace_bytes, stream);
 }
 
+size_t penc_expert_bias_grad_workspace_bytes(int type, int64_t rows, int experts, int64_t outputs) {
+    if (bad_layer(rows, experts, 1, outputs)) return 0;
+    switch (type) {
+        case PENC_FP32: return expert_bias_workspace<PENC_FP32>(rows, experts, outputs);
+        case PENC_FP16: return expert_bias_workspace<PENC_FP16>(rows, experts, outputs);
+        case PENC_BF16: return expert_bias_workspace<PENC_BF16>(rows, experts, outputs);
+        default: return 0;
+    }
+}
+
+int penc_expert_bias_grad(int type, int64_t rows, int experts, int64_t outputs, const void* grad, int64_t grad_row_stride, const int32_t* offsets, void* bias_grad,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+    return with_constant_type(type, [&](auto constant) -> int {
+        constexpr int kType = decltype(constant)::value;
+        if (bad_layer(rows, experts, 1, outputs) || bad_row_stride(rows, grad_row_stride, outputs)) return PENC_ERR_BAD_LAYER_SIZE;
+        if ((rows > 0 && !grad) || !offsets || !bias_grad) return PENC_ERR_NULL_POINTER;
+        const size_t size = kType == PENC_FP32 ? 4 : 2, need = penc_expert_bias_grad_workspace_bytes(type, rows, experts, outputs);
+        if (!aligned_to(grad, size) || !aligned_to(bias_grad, size) || !aligned_to(offsets, 4) || !aligned_to(workspace, 16)) return PENC_ERR_MISALIGNED;
+        if (workspace_bytes < need) return PENC_ERR_WORKSPACE_TOO_SMALL;
+        if (need > 0 && !workspace) return PENC_ERR_NULL_POINTER;
+        return expert_bias<kType>(rows, experts, outputs, grad, rows > 1 ? grad_row_stride : outputs, offsets, bias_grad, workspace, static_cast<hipStream_t>(stream));
+    });
+}
+
 }  // extern "C"

@@ -21,6 +21,8 @@ struct Api {
     PENC_FN(expert_linear_input_grad);
     PENC_FN(expert_weight_grad_workspace_bytes);
     PENC_FN(expert_linear_grads);
+    PENC_FN(expert_bias_grad_workspace_bytes);
+    PENC_FN(expert_bias_grad);
 #undef PENC_FN
 } api;
 
@@ -313,7 +315,7 @@ struct ExpertLinearNode : public ExpertNode {
 
     std::string name() const override { return "LayersExpertLinearBackward"; }
     variable_list gradients(const variable_list& grads) override {
-        const std::vector<Tensor> t = unpacked();  // x (where a parameter wants a gradient), weight (where x does), offsets
+        const std::vector<Tensor> t = unpacked();  // x (where the weight wants a gradient), weight (where x does), offsets
         const auto scalar = scalar_type_of(type);
         const c10::DeviceGuard device(grads[0].device());
         TORCH_CHECK(t[2].defined() && t[2].is_cuda() && t[2].scalar_type() == at::kInt && t[2].is_contiguous() && t[2].numel() == experts + 1,
@@ -331,22 +333,26 @@ struct ExpertLinearNode : public ExpertNode {
             weight = t[1].contiguous();
             out[0] = at::empty(sizes, options);
         }
-        if (!t[0].defined() || !(task_should_compute_output(1) || want_bias)) {
+        if (want_bias) out[2] = at::empty({weight_sizes[0], outputs}, options);
+        if (!t[0].defined() || !task_should_compute_output(1)) {
             if (want_x)
                 check(api.expert_linear_input_grad(type, rows, experts, channels, outputs, g.data(), g.stride, weight.const_data_ptr(), offsets, out[0].data_ptr(), stream),
                       "expert_linear");
+            if (want_bias) {
+                const size_t n = api.expert_bias_grad_workspace_bytes(type, rows, experts, outputs);
+                const Tensor ws = at::empty({static_cast<int64_t>(n)}, options.dtype(at::kByte));
+                check(api.expert_bias_grad(type, rows, experts, outputs, g.data(), g.stride, offsets, out[2].data_ptr(), ws.data_ptr(), n, stream), "expert_linear");
+            }
             return out;
         }
         require_saved(t[0], sizes, scalar);
         const Rows x = product_rows(rows_of(t[0], "x"));
-        Tensor of_weight = at::empty(weight_sizes, options);
-        if (want_bias) out[2] = at::empty({weight_sizes[0], outputs}, options);
+        out[1] = at::empty(weight_sizes, options);
         const size_t n = api.expert_weight_grad_workspace_bytes(type, rows, experts, channels, outputs);
         const Tensor ws = at::empty({static_cast<int64_t>(n)}, options.dtype(at::kByte));
         check(api.expert_linear_grads(type, rows, experts, channels, outputs, x.data(), x.stride, g.data(), g.stride, want_x ? weight.const_data_ptr() : nullptr, offsets,
-                                      want_x ? out[0].data_ptr() : nullptr, of_weight.data_ptr(), want_bias ? out[2].data_ptr() : nullptr, ws.data_ptr(), n, stream),
+                                      want_x ? out[0].data_ptr() : nullptr, out[1].data_ptr(), want_bias ? out[2].data_ptr() : nullptr, ws.data_ptr(), n, stream),
               "expert_linear");
-        if (task_should_compute_output(1)) out[1] = std::move(of_weight);
         return out;
     }
 };
@@ -384,7 +390,7 @@ Tensor expert_linear(const Tensor& x, const Tensor& weight, const Tensor& bias, 
     node->sizes = x.sizes().vec(), node->weight_sizes = weight.sizes().vec();
     node->has_bias = bias.defined();
     const Tensor none;
-    node->save({weight.requires_grad() || (bias.defined() && bias.requires_grad()) ? &x : &none, x.requires_grad() ? &weight : &none, &offsets});
+    node->save({weight.requires_grad() ? &x : &none, x.requires_grad() ? &weight : &none, &offsets});
     torch::autograd::set_history(y, node);
     return y;
 }
@@ -506,6 +512,8 @@ void bind_experts(void* library) {
     PENC_FN(expert_linear_input_grad);
     PENC_FN(expert_weight_grad_workspace_bytes);
     PENC_FN(expert_linear_grads);
+    PENC_FN(expert_bias_grad_workspace_bytes);
+    PENC_FN(expert_bias_grad);
     PENC_FN(route);
 #undef PENC_FN
 }

@@ -144,3 +144,41 @@ def test_long_sums_of_one_sign(dtype, rows, number, channels, outputs):
             half = torch.finfo(dtype).eps / 2
             worst = float((got.double() - want).abs().max()) / want
             assert worst <= bound + half, f"{name}: {worst:.3g} of the sum, bound {bound + half:.3g}"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,outputs", [(0, 3, 5), (1, 1, 1), (700, 5, 3), (513, 1, 16), (4000, 1000, 17), (100001, 4, 1), (70001, 13, 130), (1 << 20, 2, 65), (600000, 1, 7)])
+def test_the_gradient_of_the_biases_alone(dtype, rows, number, outputs):
+    """Neither x nor the weights are needed for it, and x is not kept."""
+    dtype = TYPES[dtype]
+    routing = layers.routing(uneven_experts(rows, number) if rows > 3 else torch.zeros((rows, 1), dtype=torch.int32, device="cuda"), number)
+    offsets = routing.offsets.tolist()
+    grad = whole((rows, outputs + 3), 2, dtype)[:, :outputs]
+    want = torch.stack([grad[first:last].double().sum(0) for first, last in zip(offsets, offsets[1:])]).to(dtype)
+    grad[offsets[-1]:] = math.nan
+    x, weight, bias = whole((rows, 40), 1, dtype), whole((number, outputs, 40), 3, dtype), whole((number, outputs), 4, dtype).requires_grad_(True)
+    y = layers.expert_linear(x, weight, bias, routing)
+    with torch.no_grad():
+        x += 1.0
+    assert torch.equal(torch.autograd.grad(y, bias, grad, retain_graph=True)[0], want)
+    # with the gradient of x, and by itself of a layer whose weights are trained too
+    x.requires_grad_(True)
+    y = layers.expert_linear(x, weight, bias, routing)
+    both = torch.autograd.grad(y, (x, bias), grad)
+    assert torch.equal(both[1], want)
+    y = layers.expert_linear(x, weight.requires_grad_(True), bias, routing)
+    all_of_them = torch.autograd.grad(y, (x, weight, bias), grad, retain_graph=True)
+    assert torch.equal(all_of_them[0], both[0]) and torch.equal(all_of_them[2], want) and torch.equal(torch.autograd.grad(y, bias, grad)[0], want)
+
+
+def test_the_gradient_of_the_biases_alone_takes_no_room_for_the_weights():
+    routing = layers.routing(torch.zeros((4096, 1), dtype=torch.int32, device="cuda"), 4)
+    x, weight, bias = torch.ones((4096, 1024), device="cuda"), torch.ones((4, 1024, 1024), device="cuda"), torch.zeros((4, 1024), device="cuda", requires_grad=True)
+    y = layers.expert_linear(x, weight, bias, routing)
+    grad = torch.ones_like(y)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    db, = torch.autograd.grad(y, bias, grad)
+    assert torch.cuda.max_memory_allocated() - before <= 4 * weight.numel() // 8
+    assert bool((db[0] == 4096.0).all()) and not bool(db[1:].any())
