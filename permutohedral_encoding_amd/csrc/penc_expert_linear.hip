@@ -78,7 +78,8 @@ __device__ __forceinline__ RowTile row_tile(const int32_t* __restrict__ offsets,
 }
 
 // Piece `t` of all experts' (row_tile<false>), the largest pieces first, in classes of an eighth of `most`: workgroups that begin last are short then.
-// (32768 rows of 16 experts in uneven demand, 1024 by 4096 bf16, all of the layer: 896 us in the experts' order, 887 so.)  For the experts of a wave's lanes; more of them have more pieces than matter.
+// (dW in the experts' order and so, experts in uneven demand: 32768 x 1024 by 4096 bf16 of 16 experts 363 and 306 us, 65536 x 512 by 2048 bf16 of 32 198 and 175,
+// 32768 x 1024 by 1024 fp32 of 16 723 and 570; 131072 x 1024 by 1024 bf16 of 8, which are cut for whole rounds, 347 and 340, 50000 x 512 by 512 fp32 of 20 247 and 242.)  For the experts of a wave's lanes; more of them have more pieces than matter.
 __device__ __forceinline__ RowTile row_tile_by_size(const int32_t* __restrict__ offsets, int experts, int rows, uint32_t t, int most) {
     if (experts > 64) return row_tile<false>(offsets, experts, rows, t, most);
     const int lane = threadIdx.x % 64, from = lane < experts ? min(max(offsets[lane], 0), rows) : 0, to = lane < experts ? min(max(offsets[lane + 1], 0), rows) : 0;
@@ -687,8 +688,10 @@ int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
         if (row_tiles(a, 128) * ((a.wide + 127) / 128) < static_cast<int64_t>(kUnits / 2))
             return launch_rows<kBack, Product<Value, kBack, false, 64, 64, 2, 2, kChunks, kChunks == Chunks::kDirect ? 4 : 2>>(a, stream);
     }
-    // (129 to 192 results of rows that begin anywhere: three tiles of 64 take 32.5 us of 70001 x 203 by 130 fp16, two of 128 35.4; of rows on 16 bytes, 208 by 136, 22.3 and 21.0)
-    if (a.wide <= 64 || (kChunks == Chunks::kHeld && a.wide > 128 && a.wide <= 192) || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks, 2, kChunksN>>(a, stream);
+    // (129 to 192 results of rows that begin anywhere: three tiles of 64, where they are two rounds of compute units at least, 33.6 us of 70001 x 203 by 130 fp16, two of 128 35.7; 34.6 and 37.7 of 203 by 190;
+    // of 200000 x 513 by 132 bf16 113 and 120; but of 30000 x 1001 by 160 fp16, which has 366 such tiles, 37.0 and 31.8.  Of rows on 16 bytes, 208 by 136, 22.3 and 21.0.)
+    const bool threes = kChunks == Chunks::kHeld && a.wide > 128 && a.wide <= 192 && 3 * row_tiles(a, 256) >= 2 * kUnits;
+    if (a.wide <= 64 || threes || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks, 2, kChunksN>>(a, stream);
     if constexpr (kChunks != Chunks::kSingle) {
         if constexpr (kChunks == Chunks::kDirect && kSize == 2) {
             // (1024 by 4096 bf16, 16 experts, of 2048 rows each: 302 us and 347 without; of 512 89 and 86, of 256 58 and 50: tiles of 256 rows that are not full.
@@ -735,8 +738,8 @@ struct WeightPlan {
     double time;
 };
 // Workgroups go in rounds of as many as have room at a time.  Beside its rows a workgroup takes as long as for two steps, and where its sums go through memory, as long again as kCut
-// rows.  Either an expert's rows are one piece (up to twice as many as experts have on average, or 3/4 of all that a workgroup has if that is more: 32768 x 1024 by 4096 bf16, 16 experts in uneven demand,
-// y and dW, 614 us and then 591; and a quarter of the time for experts that are not alike), or they are cut for whole rounds, as few as there can be or up to three more.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and 6 for the sums, now 28 and 5;
+// rows.  Either an expert's rows are one piece (up to twice as many as experts have on average, or 3/4 of all that a workgroup has if that is more: dW of 32768 x 1024 by 4096 bf16, 16 experts in uneven demand,
+// 324 us and then 304, of 16384 x 2048 by 2048 bf16, 16 experts, 205 and 185, of 16384 x 1024 by 2048 fp32 568 and 556; and a quarter of the time for experts that are not alike), or they are cut for whole rounds, as few as there can be or up to three more.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and 6 for the sums, now 28 and 5;
 // 2^20 x 64 by 64 fp32, all of the layer, with 2, 4, 6 and 8 to a compute unit 347, 325, 305 and 316 us, with 3 299.  16384 x 1024 by 2048 bf16, 4 experts, y and dW: cut for three rounds
 // 216 us, in one piece 165.)
 // No piece is longer than kLongest.  A chain of n additions of one sign is off by n / 2 times 2^-24 of it at the most: fp32, whose products are added one by one, by 2^-12 (in one chain of
