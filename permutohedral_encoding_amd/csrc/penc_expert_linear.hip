@@ -3,8 +3,8 @@
 //     y[r][o] = sum over c of W[e][o][c] x[r][c] + b[e][o],      dx[r][c] = sum over o of W[e][o][c] dy[r][o],
 //     dW[e][o][c] = sum over these r of dy[r][o] x[r][c],        db[e][o] = sum of dy[r][o].
 //
-// Which rows a workgroup has it finds from the offsets, which are on the device: tiles of rows do not cross from one expert to the next, and the grid has room for one
-// tile of each expert that is not full.  Rows behind the last expert's are zero in y and dx and not read otherwise.
+// Which rows a workgroup has it finds from the offsets, which are on the device: tiles of rows do not cross from one expert to the next, and the grid has
+// room for one tile of each expert that is not full.  Rows behind the last expert's are zero in y and dx and not read otherwise.
 //
 // The type of values (PENC_TYPE: those of penc.h) is one compilation each.
 #include <algorithm>
@@ -70,7 +70,8 @@ __device__ __forceinline__ RowTile row_tile(const int32_t* __restrict__ offsets,
             const uint32_t its = its_own(tiles), at = t - before - (its_own(sum) - its);
             // (tiles of rows are full but for the last one; pieces for the weights' gradient are alike)
             const int each = kWhole ? most : (count / static_cast<int>(its) / 64 + 1) * 64, skip = min(static_cast<int>(at) * each, count);
-            return {base + found, first + skip, min(count - skip, each), static_cast<int>(its), int64_t{cut_before} + static_cast<uint32_t>(its_own(sum_of_cut)) - static_cast<uint32_t>(its_own(cut)) + at};
+            return {base + found, first + skip, min(count - skip, each), static_cast<int>(its),
+                int64_t{cut_before} + static_cast<uint32_t>(its_own(sum_of_cut)) - static_cast<uint32_t>(its_own(cut)) + at};
         }
         before += __builtin_amdgcn_readlane(sum, 63), cut_before += __builtin_amdgcn_readlane(sum_of_cut, 63);
     }
@@ -78,8 +79,9 @@ __device__ __forceinline__ RowTile row_tile(const int32_t* __restrict__ offsets,
 }
 
 // Piece `t` of all experts' (row_tile<false>), the largest pieces first, in classes of an eighth of `most`: workgroups that begin last are short then.
-// (dW in the experts' order and so, experts in uneven demand: 32768 x 1024 by 4096 bf16 of 16 experts 363 and 306 us, 65536 x 512 by 2048 bf16 of 32 198 and 175,
-// 32768 x 1024 by 1024 fp32 of 16 723 and 570; 131072 x 1024 by 1024 bf16 of 8, which are cut for whole rounds, 347 and 340, 50000 x 512 by 512 fp32 of 20 247 and 242.)  For the experts of a wave's lanes; more of them have more pieces than matter.
+// (dW in the experts' order and so, experts in uneven demand: 32768 x 1024 by 4096 bf16 of 16 experts 363 and 306 us, 65536 x 512 by 2048 bf16 of 32 198 and
+// 175, 32768 x 1024 by 1024 fp32 of 16 723 and 570; 131072 x 1024 by 1024 bf16 of 8, which are cut for whole rounds, 347 and 340, 50000 x 512 by 512 fp32 of
+// 20 247 and 242.)  For the experts of a wave's lanes; more of them have more pieces than matter.
 __device__ __forceinline__ RowTile row_tile_by_size(const int32_t* __restrict__ offsets, int experts, int rows, uint32_t t, int most) {
     if (experts > 64) return row_tile<false>(offsets, experts, rows, t, most);
     const int lane = threadIdx.x % 64, from = lane < experts ? min(max(offsets[lane], 0), rows) : 0, to = lane < experts ? min(max(offsets[lane + 1], 0), rows) : 0;
@@ -93,7 +95,8 @@ __device__ __forceinline__ RowTile row_tile_by_size(const int32_t* __restrict__ 
         if (here != 0) {
             const int found = __builtin_ctzll(here);
             const auto its_own = [&](uint32_t v) { return static_cast<int>(__builtin_amdgcn_readlane(static_cast<int>(v), found)); };
-            const int its = its_own(tiles), at = static_cast<int>(t - done) - (its_own(sum) - its), rows_each = its_own(each), count = its_own(n), skip = min(at * rows_each, count);
+            const int its = its_own(tiles), at = static_cast<int>(t - done) - (its_own(sum) - its), rows_each = its_own(each), count = its_own(n),
+                skip = min(at * rows_each, count);
             return {found, its_own(from) + skip, min(count - skip, rows_each), its, int64_t{static_cast<uint32_t>(its_own(cut_before))} + at};
         }
         done += __builtin_amdgcn_readlane(static_cast<int>(sum), 63);
@@ -153,8 +156,9 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, char* lds, const Ro
     store_rows(p, static_cast<Value*>(a.rows_out) + static_cast<int64_t>(first_row) * a.wide + m0, a.wide, rows, columns);
 }
 
-// kSplit: with as many tiles as compute units, or twice or three times as many, and a few more, those few take as long as all before them; where the last round has at most half of the compute
-// units, its tiles go in quarters, which then are one round or two of a third of the time (32768 x 4096 by 1024 bf16, 544 tiles: 310 -> 250 us).
+// kSplit: with as many tiles as compute units, or twice or three times as many, and a few more, those few take as long as all before them; where the last
+// round has at most half of the compute units, its tiles go in quarters, which then are one round or two of a third of the time (32768 x 4096 by 1024 bf16,
+// 544 tiles: 310 -> 250 us).
 template <bool kBack, class P, class Quarter>
 __global__ __launch_bounds__(P::kThreads) void expert_rows_kernel(RowsArgs a) {
     constexpr bool kSplit = !std::is_same_v<P, Quarter>;
@@ -223,8 +227,8 @@ __device__ __forceinline__ void store_sixteen_rows(const tile_acc (&v)[kTiles], 
 constexpr int kNarrowThreads = 256, kNarrowLines = 4, kNarrowTiles = 4;  // 64 results of 256 bytes
 constexpr int kNarrowGroups = kSize == 2 ? 2 : 1;                       // of 16 rows that a wave has at a time
 
-// Layers whose weights fit a wave's registers: at most 64 results of rows of at most 256 bytes.  The weights come through the LDS once; then waves walk over rows, 16 (or twice 16) at a
-// time, straight from memory into the fragments' registers, the next ones on their way.
+// Layers whose weights fit a wave's registers: at most 64 results of rows of at most 256 bytes.  The weights come through the LDS once; then waves walk over
+// rows, 16 (or twice 16) at a time, straight from memory into the fragments' registers, the next ones on their way.
 template <bool kBack, int kLines, int kTiles>
 __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_kernel(RowsArgs a, int most) {
     using Load = Loader<Value, kBack, 64, kNarrowThreads, Chunks::kDirect>;
@@ -240,11 +244,13 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_kernel(RowsArgs 
     constexpr int kStep = 16 * kNarrowGroups * kNarrowThreads / 64;
     if (t.expert == a.experts) {
         const tile_acc zero[kTiles] = {};
-        for (int row = wave * 16; row < t.rows; row += 16 * kNarrowThreads / 64) store_sixteen_rows(zero, out + static_cast<int64_t>(row) * a.wide, a.wide, t.rows - row, a.wide);
+        for (int row = wave * 16; row < t.rows; row += 16 * kNarrowThreads / 64)
+            store_sixteen_rows(zero, out + static_cast<int64_t>(row) * a.wide, a.wide, t.rows - row, a.wide);
         return;
     }
     const char* const weight = static_cast<const char*>(a.weight) + static_cast<int64_t>(t.expert) * a.wide * a.deep * kSize;
-    Load load(kBack ? Operand{weight, static_cast<int64_t>(a.wide) * kSize, a.deep, a.wide * kSize} : Operand{weight, static_cast<int64_t>(a.deep) * kSize, a.wide, a.deep * kSize});
+    Load load(kBack ? Operand{weight, static_cast<int64_t>(a.wide) * kSize, a.deep, a.wide * kSize}
+                    : Operand{weight, static_cast<int64_t>(a.deep) * kSize, a.wide, a.deep * kSize});
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
 #pragma unroll
     for (int l = 0; l < kLines / 2; ++l) load.begin(lds_at + l * Tile::kSize);
@@ -311,8 +317,8 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_kernel(RowsArgs 
 
 constexpr int kFewRows = 16, kFewOutputs = 64, kFewThreads = 256, kFewWaves = kFewThreads / 64;
 
-// A few rows of an expert, whose weights are what there is to read: 64 outputs of 16 rows to a workgroup, whose waves take each fourth line of 64 bytes of all of them straight into the
-// fragments' registers, four lines on their way, and add their sums in order.
+// A few rows of an expert, whose weights are what there is to read: 64 outputs of 16 rows to a workgroup, whose waves take each fourth line of 64 bytes of
+// all of them straight into the fragments' registers, four lines on their way, and add their sums in order.
 __global__ __launch_bounds__(kFewThreads) void expert_few_kernel(RowsArgs a) {
     constexpr int kTiles = kFewOutputs / 16, kAhead = 4;
     __shared__ tile_acc lds[kFewWaves - 1][kTiles][64];
@@ -320,11 +326,13 @@ __global__ __launch_bounds__(kFewThreads) void expert_few_kernel(RowsArgs a) {
     if (item >= a.spread.items) return;
     const RowTile t = row_tile<true>(a.offsets, a.experts, a.rows, item / a.tiles, kFewRows);
     if (t.expert < 0) return;
-    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), m0 = static_cast<int>(item % a.tiles) * kFewOutputs, columns = a.wide - m0;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), m0 = static_cast<int>(item % a.tiles) * kFewOutputs,
+        columns = a.wide - m0;
     tile_acc acc[kTiles] = {};
     if (t.expert < a.experts) {
         const int deep_bytes = a.deep * kSize, stride = static_cast<int>(a.stride) * kSize;
-        const auto weights = buffer_of(static_cast<const char*>(a.weight) + (static_cast<int64_t>(t.expert) * a.wide + m0) * deep_bytes, static_cast<int64_t>(min(columns, kFewOutputs)) * deep_bytes);
+        const auto weights = buffer_of(static_cast<const char*>(a.weight) + (static_cast<int64_t>(t.expert) * a.wide + m0) * deep_bytes,
+            static_cast<int64_t>(min(columns, kFewOutputs)) * deep_bytes);
         const auto rows = buffer_of(static_cast<const char*>(a.rows_in) + static_cast<int64_t>(t.first) * stride, static_cast<int64_t>(t.rows - 1) * stride + deep_bytes);
         const int w_at = lane % 16 * deep_bytes + lane / 16 * 16, x_at = lane % 16 * stride + lane / 16 * 16;
         for (int first = wave * 64; first < deep_bytes; first += kAhead * kFewWaves * 64) {
@@ -388,7 +396,8 @@ struct BiasGrads {
         const chunk16 ones = {one, one, one, one};
 #pragma unroll
         for (int j = 0; j < kTilesN; ++j) {
-            if constexpr (kWide) wide[j] += static_cast<double>((__uint_as_float(grad[j][0]) + __uint_as_float(grad[j][1])) + (__uint_as_float(grad[j][2]) + __uint_as_float(grad[j][3])));
+            const auto value = [&](int k) { return __uint_as_float(grad[j][k]); };
+            if constexpr (kWide) wide[j] += static_cast<double>((value(0) + value(1)) + (value(2) + value(3)));
             else acc[j] = multiply<Value>(ones, grad[j], acc[j]);
         }
     }
@@ -435,7 +444,8 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
     if (t.expert < 0 || (t.tiles > 1 && t.slot >= a.slots)) return;  // (the second: offsets that no plan has)
     const int c0 = static_cast<int>(tile % a.channel_tiles) * P::kM, o0 = static_cast<int>(tile / a.channel_tiles) * P::kN;
     const bool bias = a.bias != nullptr && c0 == 0 && P::wave_m() == 0;
-    const Operand m{static_cast<const char*>(a.x) + (static_cast<int64_t>(t.first) * a.x_stride + c0) * kSize, a.x_stride * kSize, t.rows, min(a.channels - c0, P::kM) * kSize};
+    const Operand m{static_cast<const char*>(a.x) + (static_cast<int64_t>(t.first) * a.x_stride + c0) * kSize, a.x_stride * kSize, t.rows,
+        min(a.channels - c0, P::kM) * kSize};
     const Operand n{static_cast<const char*>(a.grad) + (static_cast<int64_t>(t.first) * a.grad_stride + o0) * kSize, a.grad_stride * kSize, t.rows,
                     min(a.outputs - o0, P::kN) * kSize};
     P p;
@@ -448,9 +458,10 @@ __global__ __launch_bounds__(P::kThreads) void expert_weights_kernel(WeightArgs 
 
 constexpr int kNarrowRing = 3, kTailBlocks = 256;
 
-// All gradients of a narrow layer, of at most 64 channels and outputs: x and dy are read once, where dx and dW on their own read dy twice.  A wave has the weights for some of dx's
-// columns in registers and reads, of each step that the workgroup brings into the LDS, the fragments for both products.  Workgroups behind those of the pieces clear dx behind the
-// last expert's rows.  2^20 x 64 by 64 fp32 (8 experts): 175 us, 4.7 TB/s, and 8 for the sums; dx and dW on their own 119 and 136, and 13.
+// All gradients of a narrow layer, of at most 64 channels and outputs: x and dy are read once, where dx and dW on their own read dy twice.  A wave has the
+// weights for some of dx's columns in registers and reads, of each step that the workgroup brings into the LDS, the fragments for both products.  Workgroups
+// behind those of the pieces clear dx behind the last expert's rows.  2^20 x 64 by 64 fp32 (8 experts): 175 us, 4.7 TB/s, and 8 for the sums; dx and dW on
+// their own 119 and 136, and 13.
 __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_grads_kernel(WeightArgs a, const void* weight, void* dx) {
     using P = Product<Value, true, true, 64, 64, 2, 2, Chunks::kDirect, kNarrowRing>;
     using Load = Loader<Value, true, 64, kNarrowThreads, Chunks::kDirect>;
@@ -466,7 +477,8 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_grads_kernel(Wei
         const int routed = min(max(a.offsets[a.experts], 0), a.rows);
         const int64_t chunks = static_cast<int64_t>(a.rows - routed) * a.channels * kSize / 16;
         chunk16* const to = reinterpret_cast<chunk16*>(static_cast<Value*>(dx) + static_cast<int64_t>(routed) * a.channels);
-        for (int64_t i = static_cast<int64_t>(blockIdx.x - (gridDim.x - kTailBlocks)) * kNarrowThreads + threadIdx.x; i < chunks; i += kTailBlocks * kNarrowThreads) to[i] = chunk16{};
+        const uint32_t block = blockIdx.x - (gridDim.x - kTailBlocks);
+        for (int64_t i = static_cast<int64_t>(block) * kNarrowThreads + threadIdx.x; i < chunks; i += kTailBlocks * kNarrowThreads) to[i] = chunk16{};
         return;
     }
     const uint32_t piece = a.spread.item();
@@ -516,8 +528,10 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_grads_kernel(Wei
         f[0].read(lds + here, 0);
         f[1].read(lds + here, 1);
         chunk16 rows[kLines];
+        const int mine = row16 + lane % 16;
+        const char* const its = lds + here + Tile::kSize + mine * Tile::kRowBytes;
 #pragma unroll
-        for (int l = 0; l < kLines; ++l) rows[l] = *reinterpret_cast<const chunk16*>(lds + here + Tile::kSize + (row16 + lane % 16) * Tile::kRowBytes + Tile::place(row16 + lane % 16, l * 4 + lane / 16) * 16);
+        for (int l = 0; l < kLines; ++l) rows[l] = *reinterpret_cast<const chunk16*>(its + Tile::place(mine, l * 4 + lane / 16) * 16);
         here = behind(here);
         tile_acc acc[kTiles] = {};
 #pragma unroll
@@ -538,8 +552,8 @@ __global__ __launch_bounds__(kNarrowThreads) void expert_narrow_grads_kernel(Wei
 
 constexpr int kBiasThreads = 256;
 
-// db alone, of pieces of experts' rows: kLanes neighbouring outputs to as many lanes, whose others take the next rows; sums in 64 bits.  Memory bounds it: 32768 x 4096 bf16 of 16 experts 50 us
-// with the sums, 5.4 TB/s (dW with it, and thrown away, 290), 2^20 x 64 fp32 47.
+// db alone, of pieces of experts' rows: kLanes neighbouring outputs to as many lanes, whose others take the next rows; sums in 64 bits.  Memory bounds it:
+// 32768 x 4096 bf16 of 16 experts 50 us with the sums, 5.4 TB/s (dW with it, and thrown away, 290), 2^20 x 64 fp32 47.
 template <int kLanes>
 __global__ __launch_bounds__(kBiasThreads) void expert_bias_kernel(WeightArgs a) {
     constexpr int kRows = kBiasThreads / kLanes;
@@ -564,7 +578,8 @@ __global__ __launch_bounds__(kBiasThreads) void expert_bias_kernel(WeightArgs a)
 
 constexpr int kSumThreads = 256;
 
-// The sums of experts whose rows are several pieces (of db alone: with no channels), in 64 bits: kSlices lanes share a result's pieces, each taking every kSlices-th in order, and their sums are added in order.
+// The sums of experts whose rows are several pieces (of db alone: with no channels), in 64 bits: kSlices lanes share a result's pieces, each taking every
+// kSlices-th in order, and their sums are added in order.
 template <int kSlices>
 __global__ __launch_bounds__(kSumThreads) void expert_sums_kernel(WeightArgs a, uint32_t blocks) {
     constexpr int kResults = kSumThreads / kSlices;
@@ -676,26 +691,29 @@ template <bool kBack, Chunks kChunks, Chunks kChunksN = kChunks>
 int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
     if constexpr (kChunks == Chunks::kDirect) {
         if (a.wide <= 16 * kNarrowTiles && a.deep * kSize <= 64 * kNarrowLines && a.stride * kSize * 64 < 1 << 30) return launch_narrow<kBack>(a, stream);
-        // A few rows: 64 experts of 1024 by 4096 bf16, 4 rows to an expert, 99 us, and 122 without; 16 to an expert 140 and 108.  More of them where the workgroups would be few otherwise, each with
-        // all of a long row: 1257 rows of 82 experts, 2048 by 24 fp32, 23 us and 135.
+        // A few rows: 64 experts of 1024 by 4096 bf16, 4 rows to an expert, 99 us, and 122 without; 16 to an expert 140 and 108.  More of them where the
+        // workgroups would be few otherwise, each with all of a long row: 1257 rows of 82 experts, 2048 by 24 fp32, 23 us and 135.
         if (!kBack && (a.rows <= kFewRows / 2 * static_cast<int64_t>(a.experts) ||
                        (a.rows <= 2 * kFewRows * static_cast<int64_t>(a.experts) && row_tiles(a, 256) * ((a.wide + 63) / 64) < kUnits)))
             return launch_few(a, stream);
     }
-    // Where tiles of 128 x 128 would leave half of the compute units without one, tiles of 64 x 64, loaded three steps ahead where they come directly: 500 rows of 4096 by 64 bf16 39 us -> 21, of fp32 264 -> 84,
-    // 1000 rows of 512 by 512 fp32 with 3 experts, y and dx, 76 -> 29; with 180 such tiles (5000 rows, 4 experts, bf16) 20 -> 23.
+    // Where tiles of 128 x 128 would leave half of the compute units without one, tiles of 64 x 64, loaded three steps ahead where they come directly: 500
+    // rows of 4096 by 64 bf16 39 us -> 21, of fp32 264 -> 84, 1000 rows of 512 by 512 fp32 with 3 experts, y and dx, 76 -> 29; with 180 such tiles (5000
+    // rows, 4 experts, bf16) 20 -> 23.
     if constexpr (kChunks != Chunks::kSingle && kChunksN != Chunks::kSingle) {
         if (row_tiles(a, 128) * ((a.wide + 127) / 128) < static_cast<int64_t>(kUnits / 2))
             return launch_rows<kBack, Product<Value, kBack, false, 64, 64, 2, 2, kChunks, kChunks == Chunks::kDirect ? 4 : 2>>(a, stream);
     }
-    // (129 to 192 results of rows that begin anywhere: three tiles of 64, where they are two rounds of compute units at least, 33.6 us of 70001 x 203 by 130 fp16, two of 128 35.7; 34.6 and 37.7 of 203 by 190;
-    // of 200000 x 513 by 132 bf16 113 and 120; but of 30000 x 1001 by 160 fp16, which has 366 such tiles, 37.0 and 31.8.  Of rows on 16 bytes, 208 by 136, 22.3 and 21.0.)
+    // (129 to 192 results of rows that begin anywhere: three tiles of 64, where they are two rounds of compute units at least, 33.6 us of 70001 x 203 by 130
+    // fp16, two of 128 35.7; 34.6 and 37.7 of 203 by 190; of 200000 x 513 by 132 bf16 113 and 120; but of 30000 x 1001 by 160 fp16, which has 366 such tiles,
+    // 37.0 and 31.8.  Of rows on 16 bytes, 208 by 136, 22.3 and 21.0.)
     const bool threes = kChunks == Chunks::kHeld && a.wide > 128 && a.wide <= 192 && 3 * row_tiles(a, 256) >= 2 * kUnits;
     if (a.wide <= 64 || threes || kChunks == Chunks::kSingle) return launch_rows<kBack, Product<Value, kBack, false, 64, 256, 1, 4, kChunks, 2, kChunksN>>(a, stream);
     if constexpr (kChunks != Chunks::kSingle) {
         if constexpr (kChunks == Chunks::kDirect && kSize == 2) {
-            // (1024 by 4096 bf16, 16 experts, of 2048 rows each: 302 us and 347 without; of 512 89 and 86, of 256 58 and 50: tiles of 256 rows that are not full.
-            // 2^18 rows of 1024, 4 experts, y and dx: of 72 results 144 and 152 us, without 129 and 130; of 128 152 and 153, 139 and 140; of 264 232 and 239, 232 and 248; 2^17 of 640 189 and 192, 211 and 216)
+            // (1024 by 4096 bf16, 16 experts, of 2048 rows each: 302 us and 347 without; of 512 89 and 86, of 256 58 and 50: tiles of 256 rows that are not
+            // full. 2^18 rows of 1024, 4 experts, y and dx: of 72 results 144 and 152 us, without 129 and 130; of 128 152 and 153, 139 and 140; of 264 232
+            // and 239, 232 and 248; 2^17 of 640 189 and 192, 211 and 216)
             if (a.wide > 128 && a.rows >= 1024 * static_cast<int64_t>(a.experts) && static_cast<int64_t>(a.rows / 256) * ((a.wide + 255) / 256) >= 512)
                 return launch_rows<kBack, Product<Value, kBack, false, 256, 256, 4, 2, kChunks>, Product<Value, kBack, false, 128, 128, 4, 2, kChunks>>(a, stream);
         }
@@ -703,7 +721,8 @@ int rows_of_experts(const RowsArgs& a, hipStream_t stream) {
     }
 }
 
-// Both operands come directly, or both through registers; value by value only the one whose rows are that short (363113 x 1032 by 4 bf16, with gradients: 915 us, both so 1430).
+// Both operands come directly, or both through registers; value by value only the one whose rows are that short (363113 x 1032 by 4 bf16, with gradients: 915
+// us, both so 1430).
 template <bool kBack>
 int rows_of_experts(const RowsArgs& a, Chunks weight, Chunks rows, hipStream_t stream) {
     constexpr Chunks kHeld = Chunks::kHeld, kSingle = Chunks::kSingle;
@@ -737,13 +756,16 @@ struct WeightPlan {
     int64_t slots; // the most pieces of experts of more than `most` rows
     double time;
 };
-// Workgroups go in rounds of as many as have room at a time.  Beside its rows a workgroup takes as long as for two steps, and where its sums go through memory, as long again as kCut
-// rows.  Either an expert's rows are one piece (up to twice as many as experts have on average, or 3/4 of all that a workgroup has if that is more: dW of 32768 x 1024 by 4096 bf16, 16 experts in uneven demand,
-// 324 us and then 304, of 16384 x 2048 by 2048 bf16, 16 experts, 205 and 185, of 16384 x 1024 by 2048 fp32 568 and 556; and a quarter of the time for experts that are not alike), or they are cut for whole rounds, as few as there can be or up to three more.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and 6 for the sums, now 28 and 5;
-// 2^20 x 64 by 64 fp32, all of the layer, with 2, 4, 6 and 8 to a compute unit 347, 325, 305 and 316 us, with 3 299.  16384 x 1024 by 2048 bf16, 4 experts, y and dW: cut for three rounds
-// 216 us, in one piece 165.)
-// No piece is longer than kLongest.  A chain of n additions of one sign is off by n / 2 times 2^-24 of it at the most: fp32, whose products are added one by one, by 2^-12 (in one chain of
-// 98304 rows 1.2e-3 was seen), 16-bit types, which add 32 products at a time, by 2^-14.  Pieces are added in 64 bits.  (2^20 x 256 by 256 fp32, 4 experts: 3400 us in two rounds of shorter pieces, 3350 without a limit, 3860 with the limit alone.)
+// Workgroups go in rounds of as many as have room at a time.  Beside its rows a workgroup takes as long as for two steps, and where its sums go through
+// memory, as long again as kCut rows.  Either an expert's rows are one piece (up to twice as many as experts have on average, or 3/4 of all that a workgroup
+// has if that is more: dW of 32768 x 1024 by 4096 bf16, 16 experts in uneven demand, 324 us and then 304, of 16384 x 2048 by 2048 bf16, 16 experts, 205 and
+// 185, of 16384 x 1024 by 2048 fp32 568 and 556; and a quarter of the time for experts that are not alike), or they are cut for whole rounds, as few as there
+// can be or up to three more.  (Four workgroups to a compute unit whatever their tiles: 70001 x 203 by 130 fp16, where 600 of them are two rounds, 38 us and
+// 6 for the sums, now 28 and 5; 2^20 x 64 by 64 fp32, all of the layer, with 2, 4, 6 and 8 to a compute unit 347, 325, 305 and 316 us, with 3 299.  16384 x
+// 1024 by 2048 bf16, 4 experts, y and dW: cut for three rounds 216 us, in one piece 165.) No piece is longer than kLongest.  A chain of n additions of one
+// sign is off by n / 2 times 2^-24 of it at the most: fp32, whose products are added one by one, by 2^-12 (in one chain of 98304 rows 1.2e-3 was seen),
+// 16-bit types, which add 32 products at a time, by 2^-14.  Pieces are added in 64 bits.  (2^20 x 256 by 256 fp32, 4 experts: 3400 us in two rounds of
+// shorter pieces, 3350 without a limit, 3860 with the limit alone.)
 constexpr int64_t kLongest = kSize == 2 ? 1 << 16 : 1 << 13;
 WeightPlan weight_plan_of(int side, int64_t rows, int64_t experts, int64_t channels, int64_t outputs) {
     constexpr double kBeside = 128.0, kCut = kSize == 2 ? 512.0 : 128.0;
@@ -773,7 +795,8 @@ WeightPlan weight_plan(int64_t rows, int64_t experts, int64_t channels, int64_t 
     // (half of the compute units without a workgroup: 1000 x 512 by 512 fp32, 3 experts, y and dW, 47 us, 30 so; 4000 x 512 by 512 bf16, 4 experts, 28 and 26)
     if (std::max(experts, rows / p.most) * p.tiles < static_cast<int64_t>(kUnits / 2)) return weight_plan_of(64, rows, experts, channels, outputs);
     if (kSize != 2 || channels % 8 != 0 || outputs % 8 != 0 || channels < 256 || outputs < 256) return p;
-    // Two tiles of 128 have half of the work of one of 256 a row, which they do in 0.6 of its time (32768 x 1024 by 4096 bf16, 16 experts, all of the layer: 256 897 us, 128 940).
+    // Two tiles of 128 have half of the work of one of 256 a row, which they do in 0.6 of its time (32768 x 1024 by 4096 bf16, 16 experts, all of the layer:
+    // 256 897 us, 128 940).
     const WeightPlan large = weight_plan_of(256, rows, experts, channels, outputs);
     return large.time < 0.6 * p.time ? large : p;
 }
@@ -853,7 +876,8 @@ int expert_grads<PENC_TYPE>(int64_t rows, int experts, int64_t channels, int64_t
     WeightArgs a{x, grad, x_stride, grad_stride, offsets, experts, static_cast<int>(rows), static_cast<int>(channels), static_cast<int>(outputs),
                  static_cast<int>(plan.most), {}, 0, 0, dweight, dbias, static_cast<float*>(workspace), plan.slots};
     const Chunks of_x = chunks_of(x, x_stride, channels), of_grad = chunks_of(grad, grad_stride, outputs);
-    const bool together = dx != nullptr && channels <= 64 && outputs <= 64 && of_x == Chunks::kDirect && of_grad == Chunks::kDirect && aligned_to(weight, 16) && aligned_to(dx, 16);
+    const bool together = dx != nullptr && channels <= 64 && outputs <= 64 && of_x == Chunks::kDirect && of_grad == Chunks::kDirect &&
+        aligned_to(weight, 16) && aligned_to(dx, 16);
     if (dx != nullptr && !together) {
         if (const int rc = expert_rows<PENC_TYPE>(true, rows, experts, channels, outputs, grad, grad_stride, weight, nullptr, offsets, dx, stream)) return rc;
     }
@@ -872,7 +896,8 @@ template <>
 int expert_bias<PENC_TYPE>(int64_t rows, int experts, int64_t outputs, const void* grad, int64_t grad_stride, const int32_t* offsets, void* dbias, void* workspace,
                            hipStream_t stream) {
     const BiasPlan plan = bias_plan(rows, experts);
-    WeightArgs a{nullptr, grad, 0, grad_stride, offsets, experts, static_cast<int>(rows), 0, static_cast<int>(outputs), static_cast<int>(plan.most), {}, 0, 0, nullptr, dbias,
+    WeightArgs a{nullptr, grad, 0, grad_stride, offsets, experts, static_cast<int>(rows), 0, static_cast<int>(outputs), static_cast<int>(plan.most),
+        {}, 0, 0, nullptr, dbias,
                  static_cast<float*>(workspace), plan.slots};
     const auto launch = [&](auto lanes) -> int {
         constexpr int kLanes = decltype(lanes)::value;

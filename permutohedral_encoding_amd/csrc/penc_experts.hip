@@ -7,9 +7,10 @@
 //     dispatch   s[p(i)] = x[i / k], zeros for a choice without an expert;    dx[t] = sum of ds[p] over t's choices
 //     combine    o[t] = sum of w y[p] over t's choices;                      dy[p] = w do[t],  dw = <do[t], y[p]>
 //
-// All but some of route is bound by memory.  Results, and the logits, go past the caches (nontemporal), but for short rows that go to places of their own (with_past): a pass over rows of 256 MiB that leaves what it wrote in them has the next pass wait until that
-// is in memory.  Route and its gradient of 2^20 x 64 fp32: 160 us without, 115 so; rows of 2^20 x 64 fp32 there and back, two choices, with gradients 729 and 698, of 16381 x 2048 bf16
-// 195 and 181.  With rows that the caches hold (a decoder of 2^11 to 2^17 points, its passes one after the other) the two are within 1%.
+// All but some of route is bound by memory.  Results, and the logits, go past the caches (nontemporal), but for short rows that go to places of their own
+// (with_past): a pass over rows of 256 MiB that leaves what it wrote in them has the next pass wait until that is in memory.  Route and its gradient of 2^20
+// x 64 fp32: 160 us without, 115 so; rows of 2^20 x 64 fp32 there and back, two choices, with gradients 729 and 698, of 16381 x 2048 bf16 195 and 181.  With
+// rows that the caches hold (a decoder of 2^11 to 2^17 points, its passes one after the other) the two are within 1%.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -42,7 +43,8 @@ __device__ __forceinline__ T over_lanes(T v, F&& f) {
     return v;
 }
 
-// A logit as an integer that is larger where the logit is: a NaN is the largest, -0 is 0.  Up to kNone nothing is chosen: -inf, and 0 for what has been chosen before.
+// A logit as an integer that is larger where the logit is: a NaN is the largest, -0 is 0.  Up to kNone nothing is chosen: -inf, and 0 for what has been
+// chosen before.
 constexpr uint32_t kNone = 0x007FFFFFu;
 __device__ __forceinline__ uint32_t key_of(float v) {
     const uint32_t b = __float_as_uint(v + 0.0f), key = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
@@ -104,7 +106,8 @@ struct LogitRow {
     }
 };
 
-// A logit of 16 bits, which has the last 13 bits of a float free, and its expert in one integer: the largest of them is the largest logit's, and of equal ones the lowest expert's.
+// A logit of 16 bits, which has the last 13 bits of a float free, and its expert in one integer: the largest of them is the largest logit's, and of equal
+// ones the lowest expert's.
 constexpr uint32_t kPackedIndex = 0x1FFFu;
 static_assert(PENC_MAX_EXPERTS <= kPackedIndex);
 __device__ __forceinline__ uint32_t packed_key(float v, int index) { return (key_of(v) & ~kPackedIndex) | (kPackedIndex - static_cast<uint32_t>(index)); }
@@ -113,8 +116,9 @@ __device__ __forceinline__ float packed_logit(uint32_t key) {
     return k == ~kPackedIndex ? __builtin_nanf("") : logit_of(k >> 31 ? k : k | kPackedIndex);
 }
 
-// A row to kLanes lanes, which have it in registers: k times the largest key, and the lowest index that has it.  Of 16 bits both are one integer.  Instructions bound it but for a few
-// choices of a few experts: 435701 x 144 bf16, four choices, 65 us (with both apart, 32 lanes and 64 logits more than there are 120), 2^20 x 64 fp32, two choices, 52 (5.5 TB/s).
+// A row to kLanes lanes, which have it in registers: k times the largest key, and the lowest index that has it.  Of 16 bits both are one integer.
+// Instructions bound it but for a few choices of a few experts: 435701 x 144 bf16, four choices, 65 us (with both apart, 32 lanes and 64 logits more than
+// there are 120), 2^20 x 64 fp32, two choices, 52 (5.5 TB/s).
 template <class E, int kLanes, int kChunks, int kMost>
 __global__ __launch_bounds__(kThreads) void route_kernel(row_t rows, int experts, int choices, bool normalise, const E* __restrict__ logits, uint32_t stride,
                                                          float* __restrict__ weights, int32_t* __restrict__ chosen) {
@@ -239,7 +243,8 @@ int with_row_layout(int experts, int choices, F&& f) {
     if (chunks <= 8) return with_most(std::integral_constant<int, 8>{}, one);
     if (chunks <= 16) return with_most(std::integral_constant<int, 16>{}, one);
     if (chunks <= 24) return with_most(std::integral_constant<int, 8>{}, std::integral_constant<int, 3>{});
-    // (more lanes exchange what they have through the LDS: 200000 x 512 bf16, 8 choices, 187 us, with 64 of them 287; of 50000 x 1000, which would not fit the registers, 113 and 187)
+    // (more lanes exchange what they have through the LDS: 200000 x 512 bf16, 8 choices, 187 us, with 64 of them 287; of 50000 x 1000, which would not fit
+    // the registers, 113 and 187)
     constexpr std::integral_constant<int, 16> sixteen{};
     if (chunks <= 32) return with_most(sixteen, std::integral_constant<int, 2>{});
     if (chunks <= 48) return with_most(sixteen, std::integral_constant<int, 3>{});
@@ -325,8 +330,8 @@ __global__ __launch_bounds__(kThreads) void plan_scan_kernel(int64_t chunks, uin
     if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
-// Where each choice of a chunk stands.  A wave takes 64 consecutive choices after the other; lanes of one expert find each other by a ballot for each bit of its
-// number, and each stands behind those of the wave's choices before.  Without `counts` there is one chunk, which counts for itself.
+// Where each choice of a chunk stands.  A wave takes 64 consecutive choices after the other; lanes of one expert find each other by a ballot for each bit of
+// its number, and each stands behind those of the wave's choices before.  Without `counts` there is one chunk, which counts for itself.
 template <class I, int kLanes, int kItems>
 __global__ __launch_bounds__(kLanes) void plan_place_kernel(int64_t items, int experts, int bits, const I* __restrict__ chosen,
                                                               const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
@@ -415,8 +420,8 @@ struct RowPlan {
     __device__ __forceinline__ uint32_t most() const { return min(static_cast<uint32_t>(max(*routed, 0)), items); }
 };
 
-// A lane's kWide channels of a row, 16 bytes or what a shorter row has of 8 and 4, wherever they are.  The last lane of a row that has no whole number of those takes some that its
-// neighbour has too.  (2^20 x 7 bf16 there and back with gradients, two choices: 136 us channel by channel, 67 so.)
+// A lane's kWide channels of a row, 16 bytes or what a shorter row has of 8 and 4, wherever they are.  The last lane of a row that has no whole number of
+// those takes some that its neighbour has too.  (2^20 x 7 bf16 there and back with gradients, two choices: 136 us channel by channel, 67 so.)
 template <class E, int kWide_ = 16 / sizeof(E)>
 struct Piece {
     static constexpr int kWide = kWide_;
@@ -583,8 +588,8 @@ int with_pieces(int64_t channels, int most, F&& f) {
     return f(Single<E>{}, 0);
 }
 
-// Rows that go to places of their own go past the caches where they are whole lines, or long; the ends of short ones would be read back from memory (2^20 x 48 bf16 to two places each:
-// 61 us, past them 102; 64 channels 77 and 62; 50000 x 1000 fp16 53 and 50).
+// Rows that go to places of their own go past the caches where they are whole lines, or long; the ends of short ones would be read back from memory (2^20 x
+// 48 bf16 to two places each: 61 us, past them 102; 64 channels 77 and 62; 50000 x 1000 fp16 53 and 50).
 template <class F>
 int with_past(const void* to, size_t row_bytes, F&& f) {
     if (aligned_to(to, 64) && (row_bytes % 64 == 0 || row_bytes >= 1024)) return f(std::true_type{});
@@ -704,7 +709,8 @@ int penc_dispatch(int type, int64_t rows, int choices, int64_t channels, const v
         return with_pieces<E>(channels, kLog2Threads, [&](auto piece, int log2_lanes) -> int {
             return with_past(sorted, channels * sizeof(E), [&](auto past) -> int {
                 dispatch_kernel<decltype(piece), E, decltype(past)::value><<<grid_of(rows, kThreads >> log2_lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-                    row_plan(rows, choices, channels, positions, routed), log2_lanes, static_cast<const E*>(x), static_cast<uint32_t>(row_stride), static_cast<E*>(sorted));
+                    row_plan(rows, choices, channels, positions, routed), log2_lanes, static_cast<const E*>(x), static_cast<uint32_t>(row_stride),
+                        static_cast<E*>(sorted));
                 return launched();
             });
         });
@@ -758,7 +764,8 @@ int penc_combine_backward(int type, int weight_type, int64_t rows, int choices, 
                         combine_backward_kernel<decltype(piece), E, W, decltype(most)::value, decltype(past)::value>
                             <<<grid_of(rows, kThreads >> log2_lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
                                 row_plan(rows, choices, channels, positions, routed), log2_lanes, static_cast<const E*>(grad), static_cast<uint32_t>(grad_row_stride),
-                                static_cast<const E*>(y), static_cast<uint32_t>(row_stride), static_cast<const W*>(weights), static_cast<E*>(dy), static_cast<W*>(dweights));
+                                static_cast<const E*>(y), static_cast<uint32_t>(row_stride), static_cast<const W*>(weights), static_cast<E*>(dy),
+                                    static_cast<W*>(dweights));
                         return launched();
                     });
                 };

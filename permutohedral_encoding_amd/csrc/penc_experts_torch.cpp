@@ -336,7 +336,8 @@ struct ExpertLinearNode : public ExpertNode {
         if (want_bias) out[2] = at::empty({weight_sizes[0], outputs}, options);
         if (!t[0].defined() || !task_should_compute_output(1)) {
             if (want_x)
-                check(api.expert_linear_input_grad(type, rows, experts, channels, outputs, g.data(), g.stride, weight.const_data_ptr(), offsets, out[0].data_ptr(), stream),
+                check(api.expert_linear_input_grad(type, rows, experts, channels, outputs, g.data(), g.stride, weight.const_data_ptr(), offsets,
+                    out[0].data_ptr(), stream),
                       "expert_linear");
             if (want_bias) {
                 const size_t n = api.expert_bias_grad_workspace_bytes(type, rows, experts, outputs);

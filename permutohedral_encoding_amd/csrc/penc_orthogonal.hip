@@ -2,20 +2,21 @@
 //
 //     X = G / (|G|_F + eps);    `steps` times:  S = X X^T (of a tall X: X^T X),  F = b S + c S S,  X = a X + F X (X F)
 //
-// takes every singular value s in 0 .. 1 through as many times a s + b s^3 + c s^5.  What is small in X is taken up by a factor a in each step, and so is what a rounding has
-// added to it.  In 16 bits with 8 of them behind the point (bfloat16) the result would be off by 1e-2 of it, in float16 by 1.4e-3.  So X, S and F are kept
+// takes every singular value s in 0 .. 1 through as many times a s + b s^3 + c s^5.  What is small in X is taken up by a factor a in each step, and so is
+// what a rounding has added to it.  In 16 bits with 8 of them behind the point (bfloat16) the result would be off by 1e-2 of it, in float16 by 1.4e-3.  So X,
+// S and F are kept
 //
-//     as two float16 values, hi + lo, three products for each: 0.7e-6 to 1.5e-6 of float32 results, which float32 products leave 0.9e-6 to 3.4e-6 off.  16-bit results are off by their own
-//         rounding and no more, 1.66e-3 in bfloat16
-//     for bfloat16 results, where the caller asks for it (`halves`), as float16, one product for each, and F's diagonal, which is most of F, in float32: 1.8e-3 to 2.0e-3
-//         (with the diagonal in float16 2.0e-3 to 2.4e-3) in a third of the time: 16 x 4096 x 1024 1517 us, as two values 4796
+//     as two float16 values, hi + lo, three products for each: 0.7e-6 to 1.5e-6 of float32 results, which float32 products leave 0.9e-6 to 3.4e-6 off.
+//         16-bit results are off by their own rounding and no more, 1.66e-3 in bfloat16
+//     for bfloat16 results, where the caller asks for it (`halves`), as float16, one product for each, and F's diagonal, which is most of F, in float32:
+//         1.8e-3 to 2.0e-3 (with the diagonal in float16 2.0e-3 to 2.4e-3) in a third of the time: 16 x 4096 x 1024 1517 us, as two values 4796
 //
-// times 2^12, so that what matters of lo is no subnormal number.  Of the steps above |X| <= 1.2, S <= 1.5 and F <= 3, which is under 2^14.  Coefficients are accepted up to |X| <= 3 and F <= 15:
-// S 2^12 <= 36864 and F 2^12 <= 61440, where float16 ends at 65504 and roundings of X (2^-22, in halves 2^-11) add less than 2% to F.
-// The matrix cores run float16 8 times as fast as float32, so that three products take 3/8 of the time.
+// times 2^12, so that what matters of lo is no subnormal number.  Of the steps above |X| <= 1.2, S <= 1.5 and F <= 3, which is under 2^14.  Coefficients are
+// accepted up to |X| <= 3 and F <= 15: S 2^12 <= 36864 and F 2^12 <= 61440, where float16 ends at 65504 and roundings of X (2^-22, in halves 2^-11) add less
+// than 2% to F. The matrix cores run float16 8 times as fast as float32, so that three products take 3/8 of the time.
 //
-// S and S S are symmetric: tiles on one side of the diagonal are computed and stored twice.  Matrices of up to 128 rows (or columns) that fit the LDS go through all of their
-// steps there, one to a workgroup; thin ones in 64 bits, by their S alone.
+// S and S S are symmetric: tiles on one side of the diagonal are computed and stored twice.  Matrices of up to 128 rows (or columns) that fit the LDS go
+// through all of their steps there, one to a workgroup; thin ones in 64 bits, by their S alone.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -122,8 +123,9 @@ __global__ __launch_bounds__(kThreads) void squares_kernel(int64_t values, int p
     if (threadIdx.x == 0) sums[blockIdx.x] = sum[0];
 }
 
-// X 2^12 as it is stored, zeros behind each row's end.  As one float16 (E = half_t) it is rounded to 11 bits, and each of the five steps takes that up again.  So the first X is the update times a
-// power of two, which of bfloat16 is no rounding, and what the norm has beside, 1 to 2, is left to the first step (`rest`, for each matrix): an error of 1.9e-3 to 2.2e-3 became 1.8e-3 to 2.0e-3.
+// X 2^12 as it is stored, zeros behind each row's end.  As one float16 (E = half_t) it is rounded to 11 bits, and each of the five steps takes that up again.
+// So the first X is the update times a power of two, which of bfloat16 is no rounding, and what the norm has beside, 1 to 2, is left to the first step
+// (`rest`, for each matrix): an error of 1.9e-3 to 2.2e-3 became 1.8e-3 to 2.0e-3.
 template <class E, class G>
 __global__ __launch_bounds__(kThreads) void stage_kernel(int rows, int columns, int padded, int pieces, const G* __restrict__ g, const double* __restrict__ sums,
                                                          float eps, char* __restrict__ x, float* __restrict__ rest, uint32_t blocks) {
@@ -210,13 +212,16 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
     uint32_t i = t % a.tiles_m, j = t / a.tiles_m;
     if constexpr (kStage != kUpdate) pair_of(t, i, j);
     const int m0 = uniform(static_cast<int>(i)) * P::kM, n0 = uniform(static_cast<int>(j)) * P::kN;
-    const auto rows_from = [&](const char* p, int64_t row_bytes, int rows, int first, int most) { return Operand{p + first * row_bytes, row_bytes, min(rows - first, most), static_cast<int>(row_bytes)}; };
+    const auto rows_from = [&](const char* p, int64_t row_bytes, int rows, int first, int most) {
+        return Operand{p + first * row_bytes, row_bytes, min(rows - first, most), static_cast<int>(row_bytes)};
+    };
     const auto columns_from = [&](int first, int most) { return Operand{x + first * kBytes, stride, a.rows, min(a.padded - first, most) * kBytes}; };
     P p;
     if constexpr (kStage == kGram) {
         const int all = kTall ? a.rows : a.padded, each = ((all + P::kDepth - 1) / P::kDepth + a.splits - 1) / a.splits * P::kDepth;
         const int k0 = min(static_cast<int>(split) * each, all), depth = min(all - k0, each);
-        Operand m = kTall ? columns_from(m0, P::kM) : rows_from(x, stride, a.rows, m0, P::kM), n = kTall ? columns_from(n0, P::kN) : rows_from(x, stride, a.rows, n0, P::kN);
+        Operand m = kTall ? columns_from(m0, P::kM) : rows_from(x, stride, a.rows, m0, P::kM);
+        Operand n = kTall ? columns_from(n0, P::kN) : rows_from(x, stride, a.rows, n0, P::kN);
         m.first += k0 * (kTall ? stride : kBytes), n.first += k0 * (kTall ? stride : kBytes);
         if constexpr (kTall) m.rows = n.rows = depth;
         else m.bytes = n.bytes = depth * kBytes;
@@ -227,9 +232,11 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
             return;
         }
     }
-    if constexpr (kStage == kSquare) p.run(lds, rows_from(s, small_stride, a.small, m0, P::kM), rows_from(s, small_stride, a.small, n0, P::kN), a.small_padded, P::kZero, P::kNothing);
+    if constexpr (kStage == kSquare)
+        p.run(lds, rows_from(s, small_stride, a.small, m0, P::kM), rows_from(s, small_stride, a.small, n0, P::kN), a.small_padded, P::kZero, P::kNothing);
     if constexpr (kStage == kUpdate && !kTall) p.run(lds, columns_from(m0, P::kM), rows_from(f, small_stride, a.small, n0, P::kN), a.small, P::kZero, P::kNothing);
-    if constexpr (kStage == kUpdate && kTall) p.run(lds, rows_from(f, small_stride, a.small, m0, P::kM), rows_from(x, stride, a.rows, n0, P::kN), a.padded, P::kZero, P::kNothing);
+    if constexpr (kStage == kUpdate && kTall)
+        p.run(lds, rows_from(f, small_stride, a.small, m0, P::kM), rows_from(x, stride, a.rows, n0, P::kN), a.padded, P::kZero, P::kNothing);
     if constexpr (kStage != kUpdate) {
         char* const out = a.out + matrix * a.small * small_stride;
         constexpr int kWideM = P::kM / P::kWavesM, kWideN = P::kN / P::kWavesN, kParts = ProductType<E>::kParts;
@@ -300,7 +307,8 @@ __global__ __launch_bounds__(P::kThreads) void step_kernel(StepArgs a) {
                 v = weighted((diagonal[n] + a.a) * r, from, v);
             }
             if (a.result == nullptr) store_stored<E>(out + n * stride, m, v);
-            else if (m < a.columns) store_values<Result, 8>(result + static_cast<int64_t>(n) * a.columns + m, __builtin_convertvector(v * kPerScale, Eight), a.columns - m);
+            else if (m < a.columns)
+                store_values<Result, 8>(result + static_cast<int64_t>(n) * a.columns + m, __builtin_convertvector(v * kPerScale, Eight), a.columns - m);
         });
     }
 }
@@ -348,12 +356,15 @@ constexpr int kMostSmall = 128;
 constexpr int kSliceBytes = 8192;  // for sums of S that waves share (matrices of up to 32 rows)
 constexpr int kMostResident = 160 * 1024 - 256;  // bytes of the LDS
 
-// A matrix of Split numbers in the LDS.  Chunks of a row's 128 bytes are permuted by the row, so that neither 8 rows of one chunk nor 4 rows of two chunks meet in a bank.
+// A matrix of Split numbers in the LDS.  Chunks of a row's 128 bytes are permuted by the row, so that neither 8 rows of one chunk nor 4 rows of two chunks
+// meet in a bank.
 struct Resident {
     char* first;
     int pitch;
 
-    __device__ __forceinline__ char* chunk(int row, int byte) const { return first + row * pitch + (byte & ~127) + ((byte >> 4 & 7) ^ ((row & 3) << 1 | (row >> 2 & 1))) * 16 + (byte & 15); }
+    __device__ __forceinline__ char* chunk(int row, int byte) const {
+        return first + row * pitch + (byte & ~127) + ((byte >> 4 & 7) ^ ((row & 3) << 1 | (row >> 2 & 1))) * 16 + (byte & 15);
+    }
     // 16 rows from `row` on, 32 k from 32 `line` on
     __device__ __forceinline__ chunk16 across(int row, int line, int q) const {
         const int lane = threadIdx.x % 64;
@@ -395,8 +406,9 @@ __device__ __forceinline__ void multiply_split(chunk16 a, chunk16 a_low, chunk16
 __host__ __device__ constexpr int resident_pitch(int padded) { return padded * 4; }
 __host__ __device__ constexpr int round_to_32(int n) { return (n + 31) / 32 * 32; }
 
-// One matrix to a workgroup, X as `small` rows (at most 16 kTiles) of `large` numbers whichever way it lies in memory.  A wave has 16 x 32 results of S and of F, and up to kBlocks times 16
-// columns of X, which are its own: in fp32 in its registers, for a X, and as operands in the LDS, which it overwrites when it has read them.
+// One matrix to a workgroup, X as `small` rows (at most 16 kTiles) of `large` numbers whichever way it lies in memory.  A wave has 16 x 32 results of S and
+// of F, and up to kBlocks times 16 columns of X, which are its own: in fp32 in its registers, for a X, and as operands in the LDS, which it overwrites when
+// it has read them.
 template <class G, int kTiles, int kBlocks>
 __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, int columns, int steps, Coefficients k, const G* __restrict__ g, G* __restrict__ result) {
     __shared__ __attribute__((aligned(1024))) char lds[kMostResident];
@@ -411,7 +423,8 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
     // (where number `column` of row `row` is in memory)
     const int row_step = tall ? 1 : columns, column_step = tall ? columns : 1;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), q4 = lane / 16 * 4, l16 = lane % 16;
-    // The matrix once from memory: eight numbers of a row to a lane, neighbouring lanes neighbours in memory.
+    // The matrix from memory: eight numbers of a row to a lane, neighbouring lanes neighbours in memory.  (What a wave has as results is read a second time,
+    // below, from the cache.)
     constexpr int kEights = (kMostResident / 4 / 8 + kResidentThreads - 1) / kResidentThreads;
     const int eights = large_padded / 8, all = kPadded * eights;
     floats<8> read[kEights];
@@ -461,7 +474,8 @@ __global__ __launch_bounds__(kResidentThreads) void resident_kernel(int rows, in
         }
     __syncthreads();
     constexpr int kUnits = kTiles * kTiles / 2, kMostUnits = (kUnits + kResidentWaves - 1) / kResidentWaves;
-    // Of 32 rows there are two units of S: four waves share the k of each, and what three of them have is added by way of the LDS.  Sums of a quarter of the length round less, too.
+    // Of 32 rows there are two units of S: four waves share the k of each, and what three of them have is added by way of the LDS.  Sums of a quarter of the
+    // length round less, too.
     constexpr int kSlices = kUnits < kResidentWaves ? kResidentWaves / kUnits : 1;
     static_assert(kSlices == 1 || (kSlices == 4 && kSliceBytes == 2 * kUnits * 2 * 64 * 16));
     for (int step = 0; step < steps; ++step) {
@@ -599,8 +613,9 @@ constexpr int kMostThinPieces = 64;
 constexpr double kMostThinGrowth = 1 << 27;  // of 2^-53
 using four_doubles = double __attribute__((ext_vector_type(4)));
 
-// Matrices of up to 64 rows (or columns) that are long, or too long for the LDS.  X stays what it is multiplied by from the left: X = Q G / (|G| + eps) with Q = P P' .., P = a + b S + c S S and S' = P S P, all of them small, so that G is read once for S and once
-// for the result.  S is off by 2^-53 of its largest value, and what is small in it is taken up by a^2 in each step: in 64 bits five steps make 2^-35 of it (in 32 it would be 2^-6).
+// Matrices of up to 64 rows (or columns) that are long, or too long for the LDS.  X stays what it is multiplied by from the left: X = Q G / (|G| + eps) with
+// Q = P P' .., P = a + b S + c S S and S' = P S P, all of them small, so that G is read once for S and once for the result.  S is off by 2^-53 of its largest
+// value, and what is small in it is taken up by a^2 in each step: in 64 bits five steps make 2^-35 of it (in 32 it would be 2^-6).
 
 // 64 numbers of the long side from m0 on, for each of the small side's: x[small][64], zeros behind the end.
 template <class G, int kRows>
@@ -608,7 +623,8 @@ __device__ __forceinline__ void load_thin(float (&x)[kRows][kThinChunk + 1], con
     const int there = min(large - m0, kThinChunk);
     if (tall) {
         const G* const from = g + static_cast<int64_t>(m0) * small;
-        for (int i = static_cast<int>(threadIdx.x); i < kThinChunk * small; i += kThinThreads) x[i % small][i / small] = i < there * small ? static_cast<float>(from[i]) : 0.0f;
+        for (int i = static_cast<int>(threadIdx.x); i < kThinChunk * small; i += kThinThreads)
+            x[i % small][i / small] = i < there * small ? static_cast<float>(from[i]) : 0.0f;
     } else {
         for (int i = static_cast<int>(threadIdx.x); i < kThinChunk * small; i += kThinThreads) {
             const int j = i / kThinChunk, m = i % kThinChunk;
@@ -662,7 +678,8 @@ __global__ __launch_bounds__(kThinThreads) void thin_gram_kernel(int small, int 
 #pragma unroll
             for (int e = 0; e < Tiles::kEach; ++e) {
                 const int at = quarter + k + q;
-                sum[e] = __builtin_amdgcn_mfma_f64_16x16x4f64(static_cast<double>(x[tiles.i[e] + l16][at]), static_cast<double>(x[tiles.j[e] + l16][at]), sum[e], 0, 0, 0);
+                sum[e] = __builtin_amdgcn_mfma_f64_16x16x4f64(static_cast<double>(x[tiles.i[e] + l16][at]),
+                    static_cast<double>(x[tiles.j[e] + l16][at]), sum[e], 0, 0, 0);
             }
         }
         __syncthreads();
@@ -673,7 +690,8 @@ __global__ __launch_bounds__(kThinThreads) void thin_gram_kernel(int small, int 
 
 // Q / (|G| + eps) of a matrix.
 template <int kTiles>
-__global__ __launch_bounds__(kThinThreads) void thin_steps_kernel(int small, int pieces, int steps, Coefficients k, const four_doubles* __restrict__ sums, double* __restrict__ result) {
+__global__ __launch_bounds__(kThinThreads) void thin_steps_kernel(int small, int pieces, int steps, Coefficients k,
+    const four_doubles* __restrict__ sums, double* __restrict__ result) {
     using Tiles = ThinTiles<kTiles>;
     constexpr int kRows = Tiles::kRows, kEach = Tiles::kEach;
     constexpr int kPitch = kRows + 1;  // (16 rows, or 16 numbers of one, meet no bank twice; kRows + 4, so that 16 rows of 4 do not, is 10 to 20% slower)
@@ -754,12 +772,14 @@ __global__ __launch_bounds__(kThinThreads) void thin_steps_kernel(int small, int
         }
     }
     __syncthreads();
-    for (int i = static_cast<int>(threadIdx.x); i < kRows * kRows; i += kThinThreads) result[static_cast<int64_t>(blockIdx.x) * kRows * kRows + i] = q[i / kRows][i % kRows] * factor;
+    for (int i = static_cast<int>(threadIdx.x); i < kRows * kRows; i += kThinThreads)
+        result[static_cast<int64_t>(blockIdx.x) * kRows * kRows + i] = q[i / kRows][i % kRows] * factor;
 }
 
 // Q G: a workgroup takes 64 numbers of the long side at a time.
 template <class G, int kTiles>
-__global__ __launch_bounds__(kThinThreads) void thin_apply_kernel(int small, int large, bool tall, int blocks, const double* __restrict__ factors, const G* __restrict__ g,
+__global__ __launch_bounds__(kThinThreads) void thin_apply_kernel(int small, int large, bool tall, int blocks, const double* __restrict__ factors,
+    const G* __restrict__ g,
                                                                   G* __restrict__ result) {
     constexpr int kRows = 16 * kTiles;
     __shared__ float x[kRows][kThinChunk + 1];
@@ -795,7 +815,8 @@ __global__ __launch_bounds__(kThinThreads) void thin_apply_kernel(int small, int
             for (int i = static_cast<int>(threadIdx.x); i < there * small; i += kThinThreads) to[i] = static_cast<G>(x[i % small][i / small]);
         } else {
             for (int i = static_cast<int>(threadIdx.x); i < kThinChunk * small; i += kThinThreads)
-                if (i % kThinChunk < there) result[static_cast<int64_t>(i / kThinChunk) * large + m0 + i % kThinChunk] = static_cast<G>(x[i / kThinChunk][i % kThinChunk]);
+                if (i % kThinChunk < there)
+                    result[static_cast<int64_t>(i / kThinChunk) * large + m0 + i % kThinChunk] = static_cast<G>(x[i / kThinChunk][i % kThinChunk]);
         }
         __syncthreads();
     }
@@ -842,7 +863,8 @@ template <class G>
 int resident(int64_t matrices, int64_t rows, int64_t columns, int steps, Coefficients k, const G* g, G* result, hipStream_t stream) {
     const auto launch = [&](auto tiles) -> int {
         constexpr int kTiles = decltype(tiles)::value;
-        resident_kernel<G, kTiles, kMostBlocks<kTiles>><<<static_cast<unsigned>(matrices), kResidentThreads, 0, stream>>>(static_cast<int>(rows), static_cast<int>(columns), steps,
+        resident_kernel<G, kTiles, kMostBlocks<kTiles>><<<static_cast<unsigned>(matrices), kResidentThreads, 0, stream>>>(
+            static_cast<int>(rows), static_cast<int>(columns), steps,
                                                                                                                           k, g, result);
         return launched();
     };
@@ -853,8 +875,9 @@ int resident(int64_t matrices, int64_t rows, int64_t columns, int steps, Coeffic
     return launch(std::integral_constant<int, 8>{});
 }
 
-// Three launches against a chain of them, or against one workgroup that has a matrix to itself (us, fp32, so and otherwise): 14 x 2048 x 6 15 and 121, 1 x 32 x 4096 25 and 120, 8 x 64 x 4096 81 and 125;
-// 1 x 18 x 1104 23 and 50, 1 x 16 x 128 12 and 16, 1 x 18 x 300 21 and 22, 1 x 48 x 400 45 and 50, 1 x 64 x 400 67 and 53; 64 x 32 x 1100 44 and 53, 256 of them 83 and 56.
+// Three launches against a chain of them, or against one workgroup that has a matrix to itself (us, fp32, so and otherwise): 14 x 2048 x 6 15 and 121, 1 x 32
+// x 4096 25 and 120, 8 x 64 x 4096 81 and 125; 1 x 18 x 1104 23 and 50, 1 x 16 x 128 12 and 16, 1 x 18 x 300 21 and 22, 1 x 48 x 400 45 and 50, 1 x 64 x 400
+// 67 and 53; 64 x 32 x 1100 44 and 53, 256 of them 83 and 56.
 bool is_thin(int64_t matrices, int64_t rows, int64_t columns) {
     const int64_t small = std::min(rows, columns);
     return small <= kThin && (!is_resident(rows, columns) || (matrices <= 64 && small <= 48 && std::max(rows, columns) >= (small <= 16 ? 128 : small <= 32 ? 300 : 350)));
@@ -865,13 +888,15 @@ int thin_pieces(int64_t matrices, int64_t large) {
 int thin_tiles(int64_t rows, int64_t columns) { return static_cast<int>((std::min(rows, columns) + 15) / 16); }
 size_t thin_workspace(int64_t matrices, int64_t rows, int64_t columns) {
     const int tiles = thin_tiles(rows, columns);
-    return static_cast<size_t>(matrices) * (thin_pieces(matrices, std::max(rows, columns)) * static_cast<size_t>((tiles * (tiles + 1) / 2 + 3) / 4) * (kThinThreads * sizeof(four_doubles)) +
+    const size_t of_piece = static_cast<size_t>((tiles * (tiles + 1) / 2 + 3) / 4) * (kThinThreads * sizeof(four_doubles));
+    return static_cast<size_t>(matrices) * (thin_pieces(matrices, std::max(rows, columns)) * of_piece +
                                             256 * tiles * tiles * sizeof(double));
 }
 template <class G>
 int thin(int64_t matrices, int64_t rows, int64_t columns, int steps, Coefficients k, const G* g, G* result, char* workspace, hipStream_t stream) {
     const bool tall = rows > columns;
-    const int small = static_cast<int>(std::min(rows, columns)), large = static_cast<int>(std::max(rows, columns)), pieces = thin_pieces(matrices, large), tiles = thin_tiles(rows, columns);
+    const int small = static_cast<int>(std::min(rows, columns)), large = static_cast<int>(std::max(rows, columns)),
+        pieces = thin_pieces(matrices, large), tiles = thin_tiles(rows, columns);
     double* const factors = reinterpret_cast<double*>(workspace);
     four_doubles* const sums = reinterpret_cast<four_doubles*>(factors + matrices * 256 * tiles * tiles);
     const int blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((large + kThinChunk - 1) / kThinChunk, (int64_t{1} << 22) / matrices)));
@@ -898,7 +923,8 @@ int64_t pairs_of(int64_t small, int side) {
     const int64_t tiles = (small + side - 1) / side;
     return tiles * (tiles + 1) / 2;
 }
-// How many workgroups share the k of a tile of S: up to one for each compute unit, each with two steps at least (1000 x 203 fp16: 14 us without, 4 and 3 for the sums).
+// How many workgroups share the k of a tile of S: up to one for each compute unit, each with two steps at least (1000 x 203 fp16: 14 us without, 4 and 3 for
+// the sums).
 int gram_splits(int64_t matrices, int64_t small, int64_t depth, int step) {
     const int64_t items = matrices * pairs_of(small, kSumSide);
     if (!small_tiles(matrices, small, small, true) || items > 64) return 1;
@@ -983,7 +1009,8 @@ int large(int64_t matrices, int64_t rows, int64_t columns, int steps, Coefficien
     if (const int rc = launched()) return rc;
     for (int step = 0; step < steps; ++step) {
         StepArgs a{x, s, f, s, nullptr, static_cast<int>(rows), static_cast<int>(columns), static_cast<int>(l.padded), static_cast<int>(l.small),
-                   static_cast<int>(l.small_padded), {}, 0, 0, l.splits, l.splits > 1 ? partial : nullptr, diagonal, step == 0 && std::is_same_v<E, half_t> ? rest : nullptr, k.a, k.b, k.c};
+                   static_cast<int>(l.small_padded), {}, 0, 0, l.splits, l.splits > 1 ? partial : nullptr, diagonal,
+                   step == 0 && std::is_same_v<E, half_t> ? rest : nullptr, k.a, k.b, k.c};
         const auto all = [&](auto tall) -> int {
             constexpr bool kTall = decltype(tall)::value;
             if (const int rc = launch_step<kGram, kTall, E, G>(a, matrices, stream)) return rc;

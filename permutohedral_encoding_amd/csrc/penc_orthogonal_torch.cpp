@@ -41,7 +41,8 @@ void require_options(const Options& o) {
     PENC_REQUIRE(o.eps >= 1e-30 && o.eps < 1e30, "eps should be a positive number, however it is ", o.eps);
 }
 
-// The matrices of `update` (dense) into `result` (dense): as many at a time as the workspace has room for, and one, or two or four of them that together are whole fours of values, at least.
+// The matrices of `update` (dense) into `result` (dense): as many at a time as the workspace has room for, and one, or two or four of them that together are
+// whole fours of values, at least.
 void orthogonalise(const Tensor& update, const Tensor& result, const Options& o) {
     const int64_t rows = update.size(-2), columns = update.size(-1), values = rows * columns, all = update.numel() / values;
     const int64_t fours = values % 4 == 0 ? 1 : values % 2 == 0 ? 2 : 4;
@@ -54,7 +55,8 @@ void orthogonalise(const Tensor& update, const Tensor& result, const Options& o)
         matrices.matrices = std::min(most, all - first);
         const size_t n = api.orthogonal_workspace_bytes(&matrices);
         const Tensor ws = at::empty({static_cast<int64_t>(n)}, update.options().dtype(at::kByte));
-        check(api.orthogonal_matrices(&matrices, static_cast<const char*>(update.const_data_ptr()) + first * bytes, static_cast<char*>(result.data_ptr()) + first * bytes, ws.data_ptr(), n,
+        check(api.orthogonal_matrices(&matrices, static_cast<const char*>(update.const_data_ptr()) + first * bytes,
+            static_cast<char*>(result.data_ptr()) + first * bytes, ws.data_ptr(), n,
                                       current_stream(update.device())),
               "orthogonalise");
     }
@@ -63,9 +65,11 @@ void orthogonalise(const Tensor& update, const Tensor& result, const Options& o)
 // Refuses coefficients and eps before anything is changed.
 void require_accepted(const Options& o) {
     require_options(o);
-    const penc_orthogonal none{PENC_FP32, 0, 0, 1, 1, static_cast<int>(o.steps), static_cast<float>(o.a), static_cast<float>(o.b), static_cast<float>(o.c), static_cast<float>(o.eps)};
+    const penc_orthogonal none{PENC_FP32, 0, 0, 1, 1, static_cast<int>(o.steps), static_cast<float>(o.a), static_cast<float>(o.b),
+        static_cast<float>(o.c), static_cast<float>(o.eps)};
     const int status = api.orthogonal_matrices(&none, nullptr, nullptr, nullptr, 0, nullptr);
-    PENC_REQUIRE(status != PENC_ERR_UNSUPPORTED_KIND, "coefficients should keep singular values under 3 and the factor under 15, however they are ", o.a, ", ", o.b, ", ", o.c);
+    PENC_REQUIRE(status != PENC_ERR_UNSUPPORTED_KIND, "coefficients should keep singular values under 3 and the factor under 15, however they are ",
+        o.a, ", ", o.b, ", ", o.c);
     check(status, "orthogonalise");
 }
 
@@ -163,7 +167,8 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
     }
 }
 
-// muon_step(params, grads, averages, steps, a, b, c, eps, halves, most_bytes, momentum, nesterov, decay, rate): lists of dense tensors of one size, type and device
+// muon_step(params, grads, averages, steps, a, b, c, eps, halves, most_bytes, momentum, nesterov, decay, rate): lists of dense tensors of one size, type and
+// device
 PyObject* py_muon_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
         TORCH_CHECK(n_args == 14, "muon_step takes 14 arguments");

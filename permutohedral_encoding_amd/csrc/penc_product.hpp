@@ -1,22 +1,23 @@
 // Matrix products of a workgroup: D[m][n] = sum over k of A[m][k] B[n][k], for a tile of kM x kN results that stay in the registers of its waves.
 //
-// Operands come in steps of k through the LDS; one or more steps are on their way while one is multiplied, and the fragments of each half of a step are read from the LDS while the half
-// before is.  An operand is
+// Operands come in steps of k through the LDS; one or more steps are on their way while one is multiplied, and the fragments of each half of a step are read
+// from the LDS while the half before is.  An operand is
 //
 //     Across   rows of adjacent k: 128 bytes of each row in a step, 64 k of a 16-bit type and 32 of fp32
 //     Along    rows of one k, adjacent in m (or n): as many k in a step, transposed on the way from the LDS into registers
 //
-// 16-bit types are multiplied by v_mfma_f32_16x16x32, fp32 by v_mfma_f32_16x16x4_f32.  A Split number is two halves, hi = the nearest to x and lo = the nearest to x - hi
-// (22 bits of x together, where x - hi is no less than 2^-14): of every 32 numbers the hi and behind them the lo, twice 128 bytes in a step; a product is
-// hi hi + hi lo + lo hi, and what is left out is 2^-22 of it.
+// 16-bit types are multiplied by v_mfma_f32_16x16x32, fp32 by v_mfma_f32_16x16x4_f32.  A Split number is two halves, hi = the nearest to x and lo = the
+// nearest to x - hi (22 bits of x together, where x - hi is no less than 2^-14): of every 32 numbers the hi and behind them the lo, twice 128 bytes in a
+// step; a product is hi hi + hi lo + lo hi, and what is left out is 2^-22 of it.
 //
-// Chunks of 16 bytes go from memory into the LDS directly, where rows and their ends are on 16 bytes.  Where a chunk stands in the LDS is fixed by the lane that brings it, so
-// a lane brings the chunk that belongs there.  Addresses behind an operand's end (rows, k, or columns) read zeros, which the buffer's bounds see to.  Of rows that begin anywhere,
-// lanes load chunks into registers and write them into the LDS a step later; where a row ends, its last 16 bytes, of which what the chunk does not have is moved out then.
+// Chunks of 16 bytes go from memory into the LDS directly, where rows and their ends are on 16 bytes.  Where a chunk stands in the LDS is fixed by the lane
+// that brings it, so a lane brings the chunk that belongs there.  Addresses behind an operand's end (rows, k, or columns) read zeros, which the buffer's
+// bounds see to.  Of rows that begin anywhere, lanes load chunks into registers and write them into the LDS a step later; where a row ends, its last 16
+// bytes, of which what the chunk does not have is moved out then.
 //
-// Where a chunk stands: a read of 16 bytes takes 8 lanes at a time, one of 8 bytes 16 and one of 4 bytes 32, which should meet the 32 banks of 4 bytes once.  Across: lanes read one chunk c
-// of 8 rows; c stands at c ^ (row mod 8).  Along: 16 lanes read 32 bytes (fp32: 64) of each of 4 neighbouring k (fp32: 32 lanes of two k, 4 apart);
-// pieces of 32 (64) bytes are permuted by these bits of k.
+// Where a chunk stands: a read of 16 bytes takes 8 lanes at a time, one of 8 bytes 16 and one of 4 bytes 32, which should meet the 32 banks of 4 bytes once.
+// Across: lanes read one chunk c of 8 rows; c stands at c ^ (row mod 8).  Along: 16 lanes read 32 bytes (fp32: 64) of each of 4 neighbouring k (fp32: 32
+// lanes of two k, 4 apart); pieces of 32 (64) bytes are permuted by these bits of k.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -130,9 +131,9 @@ struct OperandTile {
     }
 };
 
-// 16 bytes to each lane from buffer + at + more, to the LDS from `to` on, lane after lane.  (Not the builtin: of that the compiler knows that it writes to the LDS, but not where, and has every
-// read of the LDS wait for it.  It has no result: what it brings is waited for by wait_for_loads.  The wait states are those that a scalar register written by a vector
-// instruction needs before it is an address, and M0 before it is used.)
+// 16 bytes to each lane from buffer + at + more, to the LDS from `to` on, lane after lane.  (Not the builtin: of that the compiler knows that it writes to
+// the LDS, but not where, and has every read of the LDS wait for it.  It has no result: what it brings is waited for by wait_for_loads.  The wait states are
+// those that a scalar register written by a vector instruction needs before it is an address, and M0 before it is used.)
 __device__ __forceinline__ void load_to_lds(__attribute__((ext_vector_type(4))) uint32_t buffer, int at, int more, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(to), "v"(at), "s"(buffer), "s"(more) : "memory");
 }
@@ -197,7 +198,8 @@ struct Loader {
         if constexpr (kDirect) {
             const int there = left <= 0 ? 0 : kAlong ? min(left, T::kDepth) * stride + rest : rest + left;
             const uint64_t p = reinterpret_cast<uint64_t>(first);
-            const __attribute__((ext_vector_type(4))) uint32_t buffer = {static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xFFFFu, static_cast<uint32_t>(there), 0x00020000u};
+            const __attribute__((ext_vector_type(4))) uint32_t buffer = {static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xFFFFu,
+                static_cast<uint32_t>(there), 0x00020000u};
             const uint32_t to = lds + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * 1024;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
@@ -299,7 +301,8 @@ struct Product {
     // A wave issues in order: reads of the LDS, which all waves begin at the same time, are spread over the products, which go on meanwhile.
     template <size_t... kRead>
     __device__ __forceinline__ static void alternate(std::index_sequence<kRead...>) {
-        ((__builtin_amdgcn_sched_group_barrier(0x008, (kRead + 1) * kProducts / kReads - kRead * kProducts / kReads, 0), __builtin_amdgcn_sched_group_barrier(0x100, 1, 0)), ...);
+        ((__builtin_amdgcn_sched_group_barrier(0x008, (kRead + 1) * kProducts / kReads - kRead * kProducts / kReads, 0),
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0)), ...);
     }
 
     tile_acc acc[kTilesM][kTilesN];
@@ -402,7 +405,8 @@ struct Product {
         };
         for (int step = 1; step < steps; ++step) {
             turn(even, odd, lds + here, 1);
-            // What is brought for the next step is there for all waves, and all have read the second half of this one, whose room the step kRing behind it takes.
+            // What is brought for the next step is there for all waves, and all have read the second half of this one, whose room the step kRing behind it
+            // takes.
             if constexpr (kDirect) wait_for_loads<kLoads * (kRing - 2)>();
             else end();
             meet();
@@ -474,7 +478,8 @@ __device__ __forceinline__ void store_rows(const P& p, E* out, int64_t stride, i
             const int n = P::wave_n() + 16 * j + lane % 16;
 #pragma unroll
             for (int i = 0; i < P::kTilesM; i += 2) {
-                const uint2 a = __builtin_bit_cast(uint2, __builtin_convertvector(p.acc[i][j], Four)), b = __builtin_bit_cast(uint2, __builtin_convertvector(p.acc[i + 1][j], Four));
+                const uint2 a = __builtin_bit_cast(uint2, __builtin_convertvector(p.acc[i][j], Four)),
+                    b = __builtin_bit_cast(uint2, __builtin_convertvector(p.acc[i + 1][j], Four));
                 const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
                 const int m = P::wave_m() + 16 * (i + g % 2) + g / 2 * 8;
                 if (n < rows && m < columns) store_values<E, 8>(out + n * stride + m, __builtin_bit_cast(Eight, make_uint4(x[0], y[0], x[1], y[1])), columns - m);
@@ -487,8 +492,8 @@ __device__ __forceinline__ void store_rows(const P& p, E* out, int64_t stride, i
     }
 }
 
-// How items are spread over a launch.  Consecutive workgroups go to the 8 dies in turn; each die gets `run` neighbouring items at a time, whose operands its cache then holds,
-// and all of them go through the items alike: items take different times, and of some there is nothing to do.
+// How items are spread over a launch.  Consecutive workgroups go to the 8 dies in turn; each die gets `run` neighbouring items at a time, whose operands its
+// cache then holds, and all of them go through the items alike: items take different times, and of some there is nothing to do.
 struct Spread {
     uint32_t items, run;
     static constexpr uint32_t kDies = 8;

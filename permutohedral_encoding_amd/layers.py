@@ -143,6 +143,7 @@ class Routing:
 def route(logits, choices=1, normalise=True):
     """The experts of rows: the ``choices`` (at most 8) largest of each row's logits ``(..., experts)``, at most 1024.  Returns ``(weights, routing)``, weights (..., choices) in
     float32: the softmax over the chosen experts or, with ``normalise=False``, their share of the softmax over all.
+    (The softmax over a single choice is 1 and has no gradient: a router of one choice trains with ``normalise=False``.)
 
     Of equal logits the lowest expert's is first, a NaN is the largest, and -inf is never chosen: a row with nothing else has no expert (-1) and weights of zero."""
     weights, experts, positions, offsets = _bridge().layers_route(logits, choices, normalise)
