@@ -7,9 +7,17 @@ import pytest
 import torch
 
 from permutohedral_encoding_amd import layers
+from settled_memory import settle
 from test_gpu_experts import TYPES, chosen_experts
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def memory_is_settled():
+    settle()
+    yield
+    settle()
 
 
 def whole(shape, seed, dtype, most=2):

@@ -9,9 +9,17 @@ import torch
 
 import expert_reference as ref
 from permutohedral_encoding_amd import optim
+from settled_memory import settle
 from test_gpu_orthogonal import TYPES, assert_orthogonalised, norms, updates
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def memory_is_settled():
+    settle()
+    yield
+    settle()
 
 
 def step_of(values, dtype):
