@@ -155,7 +155,7 @@ def test_long_sums_of_one_sign(dtype, rows, number, channels, outputs):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,number,outputs", [(0, 3, 5), (1, 1, 1), (700, 5, 3), (513, 1, 16), (4000, 1000, 17), (100001, 4, 1), (70001, 13, 130), (1 << 20, 2, 65), (600000, 1, 7)])
+@pytest.mark.parametrize("rows,number,outputs", [(0, 3, 5), (1, 1, 1), (700, 5, 3), (513, 1, 16), (4000, 1000, 17), (100001, 4, 1), (70001, 13, 130), (1 << 20, 2, 65), (600000, 1, 7), (200000, 200, 33), (150001, 1024, 20)])
 def test_the_gradient_of_the_biases_alone(dtype, rows, number, outputs):
     """Neither x nor the weights are needed for it, and x is not kept."""
     dtype = TYPES[dtype]
@@ -190,3 +190,44 @@ def test_the_gradient_of_the_biases_alone_takes_no_room_for_the_weights():
     db, = torch.autograd.grad(y, bias, grad)
     assert torch.cuda.max_memory_allocated() - before <= 4 * weight.numel() // 8
     assert bool((db[0] == 4096.0).all()) and not bool(db[1:].any())
+
+
+# Experts that a wave does not find in one step (more than 64 of them), of which some are cut and most are not.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,channels,outputs", [(150001, 130, 64, 64), (150001, 130, 136, 72), (100000, 1024, 40, 48), (70000, 65, 203, 130), (150001, 200, 200, 264)])
+def test_more_experts_than_a_wave_has_lanes(dtype, rows, number, channels, outputs):
+    check_whole(rows, number, channels, outputs, TYPES[dtype])
+    check_whole(rows, number, channels, outputs, TYPES[dtype], extra=(5, 3), seed=3)
+
+
+# Layers whose experts' rows are one piece unless an expert has most of all, and tiles of results by how many there are.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,number,channels,outputs", [(16384, 16, 2048, 2048), (32768, 16, 1024, 1024), (30000, 5, 1001, 160), (70001, 13, 203, 190), (70001, 13, 190, 203)])
+def test_layers_of_many_tiles(dtype, rows, number, channels, outputs):
+    check_whole(rows, number, channels, outputs, TYPES[dtype])
+
+
+def test_the_gradient_of_the_biases_alone_in_two_graphs():
+    """Of rows that are cut: each graph has sums of its own."""
+    rows, number, outputs = 20000, 3, 40
+    routing = layers.routing(uneven_experts(rows, number), number)
+    offsets = routing.offsets.tolist()
+    x, weight = torch.zeros((rows, 8), device="cuda"), torch.zeros((number, outputs, 8), device="cuda")
+    given, graphs, results = [], [], []
+    for k in range(2):
+        bias, grad = torch.zeros((number, outputs), device="cuda", requires_grad=True), whole((rows, outputs), k, torch.float32)
+        stream = torch.cuda.Stream()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            results.append(torch.autograd.grad(layers.expert_linear(x, weight, bias, routing), bias, grad)[0])
+        given.append((grad, stream))
+    for seed in range(3):
+        for k, (grad, _) in enumerate(given):
+            grad.copy_(whole((rows, outputs), 10 * seed + k, torch.float32))
+        torch.cuda.synchronize()
+        for graph, (_, stream) in zip(graphs, given):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        wanted = [torch.stack([grad[a:b].double().sum(0) for a, b in zip(offsets, offsets[1:])]).float() for grad, _ in given]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(results, wanted))

@@ -186,3 +186,28 @@ def test_coefficients_at_the_limits(shape):
                     assert_orthogonalised(optim.orthogonalise(given, coefficients=coefficients, steps=1, halves=True), given, coefficients=coefficients, steps=1)
     with pytest.raises(ValueError, match="coefficients"):
         optim.orthogonalise(update, coefficients=(12.02, -48.08, 38.464), steps=1)
+
+
+def test_parts_and_halves_in_graphs(monkeypatch):
+    """Stacks that go in parts, one after the other in the same workspace, captured and replayed, with the way of 11 bits beside."""
+    monkeypatch.setattr(optim, "WORKSPACE_BYTES", 1 << 20)
+    for shape in ((7, 200, 150), (9, 201, 131), (200, 900, 3)):
+        given = updates(*shape, torch.bfloat16)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, halves = optim.orthogonalise(given), optim.orthogonalise(given, halves=True)
+        for seed in range(3):
+            given.copy_(updates(*shape, torch.bfloat16, seed=seed + 1))
+            graph.replay()
+            want, want_halves = optim.orthogonalise(given), optim.orthogonalise(given, halves=True)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(halves, want_halves)
+            assert_orthogonalised(want, given)
+
+
+def test_in_inference_mode_and_without_gradients():
+    update = updates(2, 140, 150, torch.bfloat16)
+    want = optim.orthogonalise(update)
+    for context in (torch.no_grad(), torch.inference_mode(), torch.autocast("cuda", dtype=torch.float16)):
+        with context:
+            assert torch.equal(optim.orthogonalise(update), want)
