@@ -71,7 +71,7 @@ __device__ __forceinline__ RowTile row_tile(const int32_t* __restrict__ offsets,
             // (tiles of rows are full but for the last one; pieces for the weights' gradient are alike)
             const int each = kWhole ? most : (count / static_cast<int>(its) / 64 + 1) * 64, skip = min(static_cast<int>(at) * each, count);
             return {base + found, first + skip, min(count - skip, each), static_cast<int>(its),
-                int64_t{cut_before} + static_cast<uint32_t>(its_own(sum_of_cut)) - static_cast<uint32_t>(its_own(cut)) + at};
+                    int64_t{cut_before} + static_cast<uint32_t>(its_own(sum_of_cut)) - static_cast<uint32_t>(its_own(cut)) + at};
         }
         before += __builtin_amdgcn_readlane(sum, 63), cut_before += __builtin_amdgcn_readlane(sum_of_cut, 63);
     }
@@ -735,7 +735,7 @@ int rows_of_experts(const RowsArgs& a, Chunks weight, Chunks rows, hipStream_t s
     return rows_of_experts<kBack, kSingle>(a, stream);
 }
 
-// The same of db alone: pieces for four workgroups to a compute unit, were the outputs of one workgroup.
+// How rows are cut for db alone: for four workgroups to a compute unit, where one has all outputs.
 struct BiasPlan {
     int64_t most, pieces, slots;
 };
@@ -896,9 +896,8 @@ template <>
 int expert_bias<PENC_TYPE>(int64_t rows, int experts, int64_t outputs, const void* grad, int64_t grad_stride, const int32_t* offsets, void* dbias, void* workspace,
                            hipStream_t stream) {
     const BiasPlan plan = bias_plan(rows, experts);
-    WeightArgs a{nullptr, grad, 0, grad_stride, offsets, experts, static_cast<int>(rows), 0, static_cast<int>(outputs), static_cast<int>(plan.most),
-        {}, 0, 0, nullptr, dbias,
-                 static_cast<float*>(workspace), plan.slots};
+    WeightArgs a{nullptr, grad, 0, grad_stride, offsets, experts, static_cast<int>(rows), 0, static_cast<int>(outputs), static_cast<int>(plan.most), {}, 0, 0,
+                 nullptr, dbias, static_cast<float*>(workspace), plan.slots};
     const auto launch = [&](auto lanes) -> int {
         constexpr int kLanes = decltype(lanes)::value;
         a.tiles = static_cast<uint32_t>((outputs + kLanes - 1) / kLanes);
