@@ -1066,6 +1066,7 @@ bool bad_matrices(int64_t matrices, int64_t rows, int64_t columns) {
 // Whether the products are of float16 once.
 bool in_halves(const penc_orthogonal& o) { return o.type == PENC_BF16 && o.halves != 0; }
 
+bool bad_type(int type) { return type != PENC_FP32 && type != PENC_FP16 && type != PENC_BF16; }
 bool bad_options(const penc_orthogonal& o) { return o.steps < 1 || o.steps > PENC_MAX_ORTHOGONAL_STEPS || !(o.eps >= 1e-30f) || std::isinf(o.eps); }
 
 // Which way matrices go.
@@ -1083,12 +1084,12 @@ size_t workspace_bytes(const penc_orthogonal& o, Way way) {
 }
 size_t workspace_bytes(const penc_orthogonal& o) {
     double growth;
-    if (bad_matrices(o.matrices, o.rows, o.columns) || o.matrices == 0 || bad_options(o) || !bounded(o.a, o.b, o.c, o.steps, growth)) return 0;
+    if (bad_type(o.type) || bad_matrices(o.matrices, o.rows, o.columns) || o.matrices == 0 || bad_options(o) || !bounded(o.a, o.b, o.c, o.steps, growth)) return 0;
     return workspace_bytes(o, way_of(o, growth));
 }
 // What matrices take with any steps and coefficients.
 size_t most_workspace_bytes(const penc_orthogonal& o) {
-    if (bad_matrices(o.matrices, o.rows, o.columns) || o.matrices == 0) return 0;
+    if (bad_type(o.type) || bad_matrices(o.matrices, o.rows, o.columns) || o.matrices == 0) return 0;
     return std::max(workspace_bytes(o, way_of(o, 1.0)), workspace_bytes(o, way_of(o, INFINITY)));
 }
 

@@ -69,7 +69,7 @@ def test_workspace_is_what_the_way_takes():
     assert workspace(matrices=1000, rows=64, columns=256) == 0 == workspace(matrices=3, rows=64, columns=300, steps=20) == workspace(matrices=65, rows=5, columns=200)
     assert 0 < workspace(matrices=64, rows=5, columns=200) < 1 << 20 and workspace(matrices=64, rows=5, columns=200, steps=8) == 0
     # nothing for what is refused
-    for given in (dict(steps=0), dict(steps=65), dict(eps=0.0), dict(coefficients=(4.0, 0.0, 0.0)), dict(matrices=-1), dict(rows=0)):
+    for given in (dict(type=3), dict(type=-1), dict(steps=0), dict(steps=65), dict(eps=0.0), dict(coefficients=(4.0, 0.0, 0.0)), dict(matrices=-1), dict(rows=0)):
         assert workspace(**{"rows": 1000, "columns": 203, **given}) == 0
 
 
